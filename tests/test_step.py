@@ -1,0 +1,727 @@
+"""The decoder steps (include/urb_step.h) against their definitions in 64 bits.
+
+Tolerances are derived per value, before any run: u = 2^-24 for an f32 rounding, a chain of n f32
+additions of terms t_i is off by at most n * 2u * sum |t_i| (MFMA sums may truncate, hence 2u), and
+the output's own rounding is half a step (BF16 2^-8, f32 2^-24, relative)."""
+
+import ctypes
+import math
+from fractions import Fraction
+
+import numpy as np
+import pytest
+
+from urbilateria_amd import configs as C
+from urbilateria_amd import native as N
+from urbilateria_amd import synth
+
+from .test_gpu_parity import _small_layer, moe_mod
+
+pytestmark = pytest.mark.gpu
+
+torch = pytest.importorskip("torch")
+
+U = 2.0 ** -24
+BF16, F32 = torch.bfloat16, torch.float32
+HALF_STEP = {BF16: 2.0 ** -8, F32: U}
+FMTS = {"bf16": C.FMT_BF16, "mxfp4": C.FMT_MXFP4, "mxfp8": C.FMT_MXFP8}
+
+
+@pytest.fixture(scope="module", autouse=True)
+def _gpu(require_gpu):
+    torch.cuda.set_device(0)
+    yield
+    torch.cuda.synchronize()
+
+
+def step():
+    from urbilateria_amd import step as s
+    return s
+
+
+def _gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+def _status(call):
+    try:
+        call()
+    except N.UrbError as e:
+        return e.status
+    return N.OK
+
+
+# ---- projections --------------------------------------------------------------------------------
+
+E2M1 = torch.tensor([0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0], dtype=torch.float64)
+
+
+def _weight(fmt, rows, cols, g):
+    """(data, scales, the matrix in f64) in the checkpoint layout, on the host."""
+    if fmt == "bf16":
+        w = (torch.randn(rows, cols, generator=g) * 0.05).to(BF16)
+        return w, None, w.double()
+    scales = torch.randint(117, 123, (rows, cols // 32), generator=g, dtype=torch.uint8)
+    by = torch.exp2(scales.double() - 127).repeat_interleave(32, 1)
+    if fmt == "mxfp4":
+        data = torch.randint(0, 256, (rows, cols // 2), generator=g, dtype=torch.uint8)
+        codes = torch.stack((data & 15, data >> 4), 2).view(rows, cols).long()
+        v = E2M1[codes & 7] * torch.where(codes > 7, -1.0, 1.0)
+    else:
+        data = torch.randint(0, 256, (rows, cols), generator=g, dtype=torch.uint8)
+        data = torch.where((data & 0x7F) == 0x7F, data - 1, data)   # no NaN codes
+        v = data.view(torch.float8_e4m3fn).double()
+    return data, scales, v * by
+
+
+class Proj:
+    """A projection with adapters of the given ranks, and its definition in 64 bits."""
+
+    def __init__(self, fmt, rows, cols, max_tokens, dtype, out_dtype=None, ranks=(), seed=1,
+                 max_rank=None, host=False):
+        g = _gen(seed)
+        self.g, self.cols, self.out_dtype = g, cols, out_dtype or dtype
+        data, scales, self.w = _weight(fmt, rows, cols, g)
+        up = lambda t: t if t is None or host else t.cuda()
+        self.dtype = dtype
+        self.p = step().AdaptedProjection(up(data), up(scales), FMTS[fmt], rows, cols, max_tokens,
+                                          dtype, out_dtype, slots=len(ranks),
+                                          max_rank=max_rank or max(ranks, default=0))
+        self.adapters = {}
+        for i, r in enumerate(ranks):
+            if r:
+                self.fill(i, r)
+
+    def fill(self, slot, rank, scale=None, host=False):
+        a = (torch.randn(rank, self.cols, generator=self.g) * self.cols ** -0.5).to(BF16)
+        b = torch.randn(self.w.shape[0], rank, generator=self.g).to(BF16)
+        scale = 0.5 + 0.25 * slot if scale is None else scale
+        self.p.set_adapter(slot, a if host else a.cuda(), b if host else b.cuda(), scale)
+        self.adapters[slot] = (a.double(), b.double(), float(np.float32(scale)))
+
+    def rows_of(self, T, values="normal"):
+        x = torch.randn(T, self.cols, generator=self.g)
+        if values == "bf16":
+            x = x.to(BF16).float()
+        elif values == "wide":     # magnitudes 2^-30 .. 2^30
+            x = x * torch.exp2(torch.randint(-30, 31, x.shape, generator=self.g).float())
+        return x.to(self.dtype)
+
+    def check(self, got, x, ids=None):
+        x = x.cpu().double()
+        want, size = x @ self.w.T, x.abs() @ self.w.abs().T
+        # chains of cols / 32 MFMAs, their 32 terms and the split parts' sums
+        chain = 2 * U * (self.cols / 32 + 64)
+        off = chain * size
+        for slot, (a, b, s) in self.adapters.items():
+            at = torch.zeros(len(x), dtype=torch.bool) if ids is None else ids.cpu() == slot
+            u, usize = x[at] @ a.T, x[at].abs() @ a.abs().T
+            want[at] += s * (u @ b.T)
+            # u's own chain; its planes (16 bits for BF16 outputs); the second product's chain
+            planes = 2.0 ** -16 if self.out_dtype == BF16 else 0.0
+            off[at] += abs(s) * ((chain + planes + 40 * U) * usize) @ b.abs().T
+        tol = off + HALF_STEP[self.out_dtype] * (want.abs() + off)
+        got = got.cpu().double()
+        assert got.shape == want.shape and bool(torch.isfinite(got).all())
+        bad = (got - want).abs() > tol
+        assert not bool(bad.any()), (int(bad.sum()), float(((got - want).abs() / tol).max()),
+                                     bad.nonzero()[:4].tolist())
+
+
+def _mixed(T, slots, g, idle=0.3):
+    ids = torch.randint(0, slots, (T,), generator=g, dtype=torch.int32)
+    return torch.where(torch.rand(T, generator=g) < idle, torch.full_like(ids, -1), ids).cuda()
+
+
+@pytest.mark.parametrize("fmt", sorted(FMTS))
+@pytest.mark.parametrize("dtype,out", [(BF16, BF16), (F32, F32), (BF16, F32), (F32, BF16)])
+@pytest.mark.parametrize("T", [1, 2, 15, 16, 17, 33, 64, 65, 130])
+def test_projection_with_adapters(fmt, dtype, out, T):
+    p = Proj(fmt, 208, 640, T, dtype, out, ranks=(16, 1, 7, 8, 33))
+    x, ids = p.rows_of(T).cuda(), _mixed(T, 5, p.g)
+    p.check(p.p.forward(x, ids), x, ids)
+
+
+@pytest.mark.parametrize("rows,cols", [(16, 128), (32, 8192), (48, 32768), (1040, 256)])
+@pytest.mark.parametrize("T", [1, 20, 200])
+def test_projection_shapes(rows, cols, T):
+    p = Proj("mxfp8", rows, cols, T, BF16, F32, ranks=(4, 64))
+    x, ids = p.rows_of(T).cuda(), _mixed(T, 2, p.g)
+    p.check(p.p.forward(x, ids), x, ids)
+
+
+@pytest.mark.parametrize("rank", [1, 8, 9, 31, 32, 100, 256])
+@pytest.mark.parametrize("out", [BF16, F32])
+def test_adapter_ranks(rank, out):
+    p = Proj("bf16", 96, 256, 40, BF16, out, ranks=(rank, 2), max_rank=256)
+    x, ids = p.rows_of(40).cuda(), _mixed(40, 2, p.g, idle=0.0)
+    p.check(p.p.forward(x, ids), x, ids)
+
+
+@pytest.mark.parametrize("values", ["bf16", "wide"])
+@pytest.mark.parametrize("T", [3, 150])
+def test_f32_rows_keep_all_their_bits(values, T):
+    p = Proj("mxfp4", 64, 512, T, F32, ranks=(12,))
+    x, ids = p.rows_of(T, values).cuda(), _mixed(T, 1, p.g)
+    p.check(p.p.forward(x, ids), x, ids)
+
+
+@pytest.mark.parametrize("T,slots", [(1, 1), (40, 64), (700, 3), (1300, 40), (1300, 600)])
+def test_many_rows_and_many_adapters(T, slots):
+    # more rows than a scan takes at once; more slots than rows and fewer
+    p = Proj("mxfp4", 320, 256, T, BF16, F32, ranks=tuple(1 + i % 5 for i in range(slots)))
+    x = p.rows_of(T).cuda()
+    for ids in (_mixed(T, slots, p.g), _mixed(T, slots, p.g).sort().values,
+                torch.full((T,), slots - 1, dtype=torch.int32, device="cuda"),
+                torch.full((T,), -1, dtype=torch.int32, device="cuda"), None):
+        p.check(p.p.forward(x, ids), x, ids)
+
+
+def test_calls_longer_than_one_pass():
+    T = 8192 + 77
+    p = Proj("bf16", 16, 128, T, BF16, F32, ranks=(3, 2))
+    x, ids = p.rows_of(T).cuda(), _mixed(T, 2, p.g)
+    p.check(p.p.forward(x, ids), x, ids)
+
+
+@pytest.mark.parametrize("T", [5, 140])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_strided_rows_and_outputs_leave_the_rest(T, dtype):
+    p = Proj("bf16", 48, 256, T, dtype, ranks=(8, 8))
+    wide = torch.randn(T, 256 + 8 + 16, generator=p.g).to(dtype).cuda()
+    x, ids = wide[:, 8:264], _mixed(T, 2, p.g)
+    for start in (0, 1, 8):    # outputs at any value
+        y = torch.full((T + 1, 61), 7.0, dtype=dtype, device="cuda")
+        p.p.forward_into(x, y[:T, start:start + 48], ids)
+        p.p.sync()
+        p.check(y[:T, start:start + 48], x, ids)
+        rest = torch.ones_like(y, dtype=torch.bool)
+        rest[:T, start:start + 48] = False
+        assert bool((y[rest] == 7.0).all())
+
+
+def test_a_row_of_infinities_touches_no_other():
+    for dtype in (BF16, F32):
+        p = Proj("bf16", 64, 256, 20, dtype, F32, ranks=(4, 4))
+        x, ids = p.rows_of(20), _mixed(20, 2, p.g, idle=0.0)
+        clean = p.p.forward(x.cuda(), ids)
+        x[3, 7], x[9, 100], x[9, 101] = math.inf, math.nan, -math.inf
+        got = p.p.forward(x.cuda(), ids)
+        rows = [i for i in range(20) if i not in (3, 9)]
+        assert torch.equal(got[rows], clean[rows])
+        assert not bool(torch.isfinite(got[[3, 9]]).any())
+
+
+def test_results_do_not_depend_on_the_other_rows():
+    p = Proj("mxfp8", 64, 512, 16, BF16, F32, ranks=(8, 8, 8))
+    x, ids = p.rows_of(16).cuda(), _mixed(16, 3, p.g)
+    first = p.p.forward(x, ids)
+    for _ in range(3):
+        assert torch.equal(p.p.forward(x, ids), first)
+    order = torch.randperm(16, generator=p.g).cuda()
+    assert torch.equal(p.p.forward(x[order].contiguous(), ids[order].contiguous()), first[order])
+
+
+def test_slots_change_in_stream_order():
+    p = Proj("bf16", 64, 256, 8, F32, ranks=(4, 6), max_rank=16)
+    x = p.rows_of(8).cuda()
+    ids = torch.tensor([0, 1, -1, 0, 1, 0, 1, -1], dtype=torch.int32, device="cuda")
+    p.check(p.p.forward(x, ids), x, ids)
+    y0, old = torch.empty(8, 64, device="cuda"), dict(p.adapters)
+    p.p.forward_into(x, y0, ids)          # before the change, not waited for
+    p.fill(1, 16, scale=-2.0)
+    y1 = p.p.forward(x, ids)
+    p.check(y1, x, ids)
+    p.fill(0, 5, host=True)
+    p.check(p.p.forward(x, ids), x, ids)
+    p.adapters = old
+    p.check(y0, x, ids)
+
+
+def test_ids_without_an_adapter_are_reported_and_projected_alone():
+    p = Proj("bf16", 64, 256, 6, F32, ranks=(4, 0), max_rank=8)
+    x = p.rows_of(6).cuda()
+    for bad in (1, 2, 2**31 - 1):
+        ids = torch.tensor([0, bad, -1, -2**31, 0, -7], dtype=torch.int32, device="cuda")
+        y = torch.empty(6, 64, device="cuda")
+        p.p.forward_into(x, y, ids)
+        assert _status(p.p.sync) == N.ERR_ARGUMENT
+        assert _status(p.p.sync) == N.OK
+        p.check(y, x, torch.where(ids == bad, -1, ids))
+    p.p.clear_adapter(0)
+    p.adapters = {}
+    assert _status(lambda: p.p.forward(x, torch.zeros(6, dtype=torch.int32, device="cuda"))) \
+        == N.ERR_ARGUMENT
+    without = Proj("bf16", 64, 256, 6, F32)
+    y = torch.empty(6, 64, device="cuda")
+    without.p.forward_into(x, y, torch.zeros(6, dtype=torch.int32, device="cuda"))
+    assert _status(without.p.sync) == N.ERR_ARGUMENT
+    without.check(y, x)
+
+
+def test_projection_payloads_are_validated():
+    w = torch.zeros(16, 128, dtype=BF16)
+    w[3, 5] = math.inf
+    make = lambda d, s, f: step().AdaptedProjection(d, s, f, 16, 128, 4, F32)
+    assert _status(lambda: make(w.cuda(), None, C.FMT_BF16)) == N.ERR_NONFINITE
+    assert _status(lambda: make(w, None, C.FMT_BF16)) == N.ERR_NONFINITE
+    s = torch.full((16, 4), 127, dtype=torch.uint8)
+    s[2, 1] = 255
+    assert _status(lambda: make(torch.zeros(16, 64, dtype=torch.uint8).cuda(), s.cuda(),
+                                C.FMT_MXFP4)) == N.ERR_INVALID_SCALE
+    p = Proj("bf16", 16, 128, 4, F32, ranks=(2,))
+    for where in "ab":
+        a, b = torch.zeros(2, 128, dtype=BF16), torch.zeros(16, 2, dtype=BF16)
+        (a if where == "a" else b)[1, 1] = math.nan
+        p.p.set_adapter(0, a.cuda(), b.cuda())
+        assert _status(p.p.sync) == N.ERR_NONFINITE
+        x = p.rows_of(4).cuda()
+        y = torch.empty(4, 16, device="cuda")
+        p.p.forward_into(x, y, torch.zeros(4, dtype=torch.int32, device="cuda"))
+        assert _status(p.p.sync) == N.ERR_ARGUMENT   # the slot is empty
+        p.adapters = {}
+        p.check(y, x)
+    p.fill(0, 2)
+    p.check(p.p.forward(x, torch.zeros(4, dtype=torch.int32, device="cuda")), x,
+            torch.zeros(4, dtype=torch.int32))
+
+
+def test_projection_refuses_calls():
+    p = Proj("bf16", 64, 256, 4, F32, ranks=(4,))
+    lib, ctx = N.moe_lib(), p.p._ctx
+    x, y = torch.zeros(8, 256, device="cuda"), torch.zeros(8, 64, device="cuda")
+    call = lambda T=4, xp=x.data_ptr(), xs=256, ys=64, yp=y.data_ptr(): lib.urb_proj_forward(
+        ctx, xp, xs, None, T, yp, ys, None)
+    assert call() == N.OK
+    assert call(T=0) == call(T=5) == call(xs=252) == call(ys=63) == N.ERR_SHAPE
+    assert call(xp=x.data_ptr() + 4) == call(xs=258) == call(yp=y.data_ptr() + 2) == N.ERR_ARGUMENT
+    assert call(xp=None) == call(yp=None) == N.ERR_ARGUMENT
+    a, b = torch.zeros(4, 256, dtype=BF16, device="cuda"), torch.zeros(64, 4, dtype=BF16, device="cuda")
+    assert _status(lambda: p.p.set_adapter(1, a, b)) == N.ERR_SHAPE
+    assert _status(lambda: p.p.set_adapter(0, a, b, math.inf)) == N.ERR_NONFINITE
+    wide = Proj("bf16", 64, 256, 4, F32, ranks=(4,)).p
+    big = torch.zeros(5, 256, dtype=BF16, device="cuda"), torch.zeros(64, 5, dtype=BF16, device="cuda")
+    assert _status(lambda: wide.set_adapter(0, *big)) == N.ERR_SHAPE
+    ad = N.Adapter(a.data_ptr(), b.data_ptr(), 4, 1.0)
+    assert lib.urb_proj_set_adapter(ctx, 0, ctypes.byref(ad), N.SOURCE_DEVICE_BORROW, None) \
+        == N.ERR_ARGUMENT
+    for bad in (dict(x=x.half()), dict(x=x[:, ::2]), dict(y=y[:4]), dict(ids=[1, 2]),
+                dict(ids=torch.zeros(8, dtype=torch.int64, device="cuda"))):
+        with pytest.raises((ValueError, AttributeError)):
+            p.p.forward_into(bad.get("x", x), bad.get("y", y), bad.get("ids"))
+    with pytest.raises(ValueError):
+        step().AdaptedProjection(torch.zeros(64, 255, dtype=BF16), None, 0, 64, 256, 4)
+    torch.cuda.synchronize()
+
+
+def test_borrowed_panels_and_host_matrices_give_the_same():
+    g = _gen(5)
+    data, scales, _ = _weight("mxfp4", 64, 256, g)
+    x = torch.randn(9, 256, generator=g).cuda()
+    make = lambda d, s, src=None: step().AdaptedProjection(d, s, C.FMT_MXFP4, 64, 256, 9, F32,
+                                                           source=src)
+    want = make(data.cuda(), scales.cuda()).forward(x)
+    pd, ps = moe_mod().pack_matrix(C.FMT_MXFP4, data.cuda(), scales.cuda(), 64, 256)
+    torch.cuda.synchronize()
+    borrowed = make(pd, ps, N.SOURCE_DEVICE_BORROW)
+    assert torch.equal(borrowed.forward(x), want)
+    assert torch.equal(make(data, scales).forward(x), want)
+    assert borrowed.memory()[0] == 0 and make(data, scales).memory()[0] >= 64 * 256 // 2
+
+
+# ---- norms and rotation ------------------------------------------------------------------------
+
+def _turned(h, w, positions, freq, eps, zero_centered, interleaved):
+    """(the definition in f64, the size its rounding errors are relative to)."""
+    x = h.cpu().double()
+    n = x / (x.pow(2).mean(-1, keepdim=True) + eps).sqrt() * (w.cpu().double() + zero_centered)
+    out, size = n.clone(), n.abs()
+    r = 2 * freq.numel()
+    if r:
+        a, b = (slice(0, r, 2), slice(1, r, 2)) if interleaved else (slice(0, r // 2),
+                                                                     slice(r // 2, r))
+        angle = torch.outer(positions.cpu().double(), freq.cpu().double()).unsqueeze(1)
+        c, s = angle.cos(), angle.sin()
+        out[..., a], out[..., b] = (n[..., a] * c - n[..., b] * s, n[..., b] * c + n[..., a] * s)
+        both = n[..., a].abs() + n[..., b].abs()
+        size[..., a], size[..., b] = both, both
+    return out, size
+
+
+def _check_turned(got, h, w, positions, freq, eps=1e-6, zero_centered=True, interleaved=False):
+    want, size = _turned(h, w, positions, freq, eps, zero_centered, interleaved)
+    # the row's sum (16 terms per lane and six steps of the tree; half of it after the root), the
+    # mean, root, reciprocal, weight and products, cosine and sine and two FMAs: under 32 roundings
+    tol = 32 * U * size + HALF_STEP[h.dtype] * want.abs() * (1 + 2.0 ** -10)
+    bad = (got.cpu().double() - want).abs() > tol
+    assert not bool(bad.any()), (int(bad.sum()), bad.nonzero()[:4].tolist())
+
+
+def _freq(r):
+    half = r // 2
+    return (1e4 ** (-torch.arange(half, dtype=torch.float64) / max(half, 1))).float().cuda()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("D,R", [(64, 64), (128, 128), (256, 64), (80, 80), (80, 32), (96, 24),
+                                 (2, 2), (34, 34), (34, 6), (192, 0), (1024, 1024), (16, 16),
+                                 (576, 96), (112, 112)])
+def test_heads_normed_and_turned(dtype, interleaved, D, R):
+    g = _gen(D + R)
+    for T, hq, hk in ((1, 1, 0), (1, 16, 2), (7, 5, 3), (130, 4, 1)):
+        q, k = (torch.randn(T, h, D, generator=g).mul(3.0).to(dtype).cuda() for h in (hq, hk))
+        wq, wk = (torch.randn(D, generator=g).mul(0.2).cuda() for _ in range(2))
+        pos = torch.randint(0, 1 << 20, (T,), generator=g).cuda()
+        qo, ko = step().qk_norm_rope(q, k if hk else None, wq, wk, pos, _freq(R), 1e-6,
+                                     zero_centered=True, interleaved=interleaved)
+        _check_turned(qo, q, wq, pos, _freq(R), interleaved=interleaved)
+        if hk:
+            _check_turned(ko, k, wk, pos, _freq(R), interleaved=interleaved)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("shift", [0, 1, 8])
+def test_strided_heads_in_place_and_beside(dtype, shift):
+    # heads of a fused q/k/v row, at any value of it; out of place, then in place
+    g = _gen(3)
+    T, hq, hk, D = 33, 6, 2, 64
+    row = torch.randn(T, shift + (hq + 2 * hk) * D + 8, generator=g).to(dtype).cuda()
+    q = row[:, shift:shift + hq * D].unflatten(1, (hq, D))
+    k = row[:, shift + hq * D:shift + (hq + hk) * D].unflatten(1, (hk, D))
+    w, pos = torch.rand(D, generator=g).cuda(), torch.arange(T).cuda() + 5000
+    before, q0, k0 = row.clone(), q.clone(), k.clone()
+    # head-major outputs
+    qo, ko = (torch.empty(h, T, D, dtype=dtype, device="cuda").transpose(0, 1) for h in (hq, hk))
+    call = lambda out: step().qk_norm_rope(q, k, w, w, pos, _freq(32), 1e-5, out=out)
+    call((qo, ko))
+    _check_turned(qo, q0, w, pos, _freq(32), 1e-5, False)
+    _check_turned(ko, k0, w, pos, _freq(32), 1e-5, False)
+    assert torch.equal(row, before)
+    call((q, k))
+    assert torch.equal(q, qo) and torch.equal(k, ko)
+    rest = torch.ones_like(row, dtype=torch.bool)
+    rest[:, shift:shift + (hq + hk) * D] = False
+    assert torch.equal(row[rest], before[rest])
+
+
+def test_angles_of_far_positions():
+    D = 64
+    h = torch.randn(5, 1, D, generator=_gen(1)).cuda()
+    w = torch.ones(D, device="cuda")
+    # exact products up to 2^29; the sign of a position turns the other way
+    pos = torch.tensor([0, -1, (1 << 24) + 1, (1 << 29) - 1, -(1 << 28) - 3]).cuda()
+    got, _ = step().qk_norm_rope(h, None, w, None, pos, _freq(D), 1e-6)
+    _check_turned(got, h, w, pos, _freq(D), zero_centered=False)
+
+
+def test_rotation_of_rows_with_zeros_and_nan():
+    h = torch.randn(3, 2, 64, generator=_gen(2)).cuda()
+    h[0] = 0.0
+    h[1, 0, 5] = math.nan
+    w, pos = torch.ones(64, device="cuda"), torch.arange(3).cuda()
+    got, _ = step().qk_norm_rope(h, None, w, None, pos, _freq(64), 1e-6)
+    assert bool((got[0] == 0).all()) and bool(got[1, 0].isnan().all())
+    rest = torch.stack((h[1, 1], h[2, 0], h[2, 1])).unsqueeze(1)
+    _check_turned(torch.stack((got[1, 1], got[2, 0], got[2, 1])).unsqueeze(1), rest, w,
+                  torch.tensor([1, 2, 2]), _freq(64), zero_centered=False)
+
+
+def test_rotation_wrapper_refuses():
+    q, w = torch.zeros(2, 3, 64, device="cuda"), torch.ones(64, device="cuda")
+    pos = torch.arange(2).cuda()
+    call = lambda **c: step().qk_norm_rope(c.get("q", q), c.get("k"), c.get("w", w), w,
+                                           c.get("pos", pos), _freq(64), 1e-6, out=c.get("out"))
+    for c in (dict(q=q[0]), dict(k=q[:1]), dict(w=w[:32]), dict(w=w.double()), dict(pos=pos.int()),
+              dict(out=(q[:, :2], None)), dict(q=q.transpose(1, 2)), dict(k=q.bfloat16())):
+        with pytest.raises(ValueError):
+            call(**c)
+    assert _status(lambda: call(q=q.half())) == N.ERR_ARGUMENT
+
+
+# ---- sampling ------------------------------------------------------------------------------------
+
+def _drawn(row, tau=1.0, k=0, p=1.0, min_p=0.0, u=0.5):
+    """(id, probability) by the definition: e in f64, its sums in whole multiples of 2^-shift.  (In
+    f64 a sum of many ones loses the small masses that decide a border between equal tokens.)"""
+    shift = 62 - max(1, math.ceil(math.log2(row.numel())))
+    row = row.cpu().double().numpy()
+    at = np.flatnonzero(row > -np.inf)
+    if not at.size:
+        return -1, 0.0
+    order = at[np.lexsort((at, -row[at]))]
+    if tau == 0:
+        return int(order[0]), 1.0
+    top = row[order[0]]
+    with np.errstate(invalid="ignore", over="ignore"):
+        e = np.exp(np.where(row[order] == top, 0.0, (row[order] - top) / tau))
+    q = np.floor(e * 2.0 ** shift + 0.5).astype(np.int64)
+    n = min(k, e.size) if k > 0 else e.size
+    if p < 1:
+        mass = np.cumsum(q[:n])
+        want = math.ceil(Fraction(p) * int(mass[-1]))
+        n = 1 + int(np.searchsorted(mass[:-1], want, side="left"))
+    n = max(1, min(n, int(np.count_nonzero(e >= min_p))))
+    kept = np.argsort(order[:n])
+    mass = np.cumsum(q[kept])
+    target = math.floor(Fraction(u) * int(mass[-1]))
+    i = int(np.searchsorted(mass, target, side="right"))
+    return int(order[kept[i]]), float(e[kept[i]] / (int(mass[-1]) / 2.0 ** shift))
+
+
+def _check_drawn(logits, uniform, sampler=None, **params):
+    T, V = logits.shape
+    sampler = sampler or step().Sampler(V, T, logits.dtype)
+    names = {"tau": "temperature", "k": "top_k", "p": "top_p", "min_p": "min_p"}
+    dev = {names[n]: torch.tensor(v, dtype=torch.int32 if n == "k" else F32).cuda()
+           for n, v in params.items()}
+    u = torch.tensor(uniform, dtype=F32).cuda()
+    ids, probs = sampler.sample(logits, u, **dev)
+    ids, probs, u = ids.tolist(), probs.tolist(), u.tolist()
+    host = {n: dev[names[n]].tolist() for n in params}
+    for t in range(T):
+        id_, prob = _drawn(logits[t], u=u[t], **{n: host[n][t] for n in params})
+        assert ids[t] == id_, (t, ids[t], id_, {n: host[n][t] for n in params}, u[t])
+        # one rounding to f32, and sums that are exact to 2^-20 of it
+        assert abs(probs[t] - prob) <= (U + 2.0 ** -40) * prob, (t, probs[t], prob)
+
+
+def _logits(T, V, g, dtype=F32, spread=3.0):
+    x = torch.randn(T, V, generator=g) * spread
+    x[torch.rand(T, V, generator=g) < 0.05] = -math.inf
+    return x.to(dtype).cuda()
+
+
+GRID = [dict(), dict(tau=0.7), dict(tau=0.0), dict(k=1), dict(k=7), dict(k=300), dict(p=0.9),
+        dict(p=0.2), dict(p=1e-9), dict(p=0.9999), dict(min_p=0.1), dict(min_p=1.0),
+        dict(tau=1.7, k=40, p=0.8), dict(tau=0.5, k=500, p=0.95, min_p=0.02),
+        dict(p=0.99, min_p=0.001), dict(tau=100.0, p=0.9), dict(tau=0.01), dict(k=20000, p=0.5)]
+
+
+@pytest.mark.parametrize("V", [1, 2, 63, 64, 1000, 4097, 32000])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_draws_under_every_filter(V, dtype):
+    g = _gen(V)
+    T = 3 * len(GRID)
+    x = _logits(T, V, g, dtype)
+    full = [dict(dict(tau=1.0, k=0, p=1.0, min_p=0.0), **d) for d in GRID for _ in range(3)]
+    params = {n: [d[n] for d in full] for n in ("tau", "k", "p", "min_p")}
+    _check_drawn(x, torch.rand(T, generator=g).tolist(), **params)
+
+
+@pytest.mark.parametrize("V", [129280, 262144 + 3, 1 << 20])
+def test_draws_from_large_vocabularies(V):
+    g = _gen(V)
+    x = _logits(6, V, g)
+    _check_drawn(x, torch.rand(6, generator=g).tolist(), tau=[1.0, 0.8, 1.0, 2.0, 0.0, 1.0],
+                 k=[0, 50, 0, 100000, 0, 3000], p=[1.0, 0.9, 0.95, 0.9, 1.0, 0.97],
+                 min_p=[0.0, 0.0, 0.01, 0.0, 0.0, 0.0])
+
+
+@pytest.mark.parametrize("V", [5, 900, 40000])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_ties_go_to_the_lowest_index(V, dtype):
+    g = _gen(V)
+    same = torch.full((V,), 1.5)
+    few = torch.randint(0, 3, (V,), generator=g).float()          # three values
+    signed = torch.zeros(V)
+    signed[::2] = -0.0                                            # equal to +0
+    two = torch.where(torch.arange(V) % 2 == 0, 4.0, -30.0)
+    rows = [same, few, signed, two]
+    cases = [(r, k, p, u) for r in rows for k, p in ((0, 1.0), (3, 1.0), (0, 0.5), (V // 2 + 1, 0.7))
+             for u in (0.0, 0.3, 1.0 - 2.0 ** -24)]
+    x = torch.stack([c[0] for c in cases]).to(dtype).cuda()
+    _check_drawn(x, [c[3] for c in cases], k=[c[1] for c in cases], p=[c[2] for c in cases])
+    _check_drawn(x, [c[3] for c in cases], tau=[0.0] * len(cases))
+
+
+@pytest.mark.parametrize("V", [3, 700, 33000])
+def test_masked_rows(V):
+    inf, nan, low = math.inf, math.nan, torch.finfo(F32).min
+    base = torch.randn(V, generator=_gen(V))
+    rows = []
+    for change in ({0: -inf}, {0: nan}, {1: inf}, {1: inf, 2: inf}, {0: low, 1: low}, {0: nan, 1: -inf}):
+        r = base.clone()
+        for i, v in change.items():
+            r[i] = v
+        rows.append(r)
+    rows += [torch.full((V,), v) for v in (-inf, nan, low, inf)]
+    only = torch.full((V,), -inf)
+    only[V - 1] = -5.0
+    rows.append(only)
+    x = torch.stack(rows).cuda()
+    T = len(rows)
+    for params in (dict(), dict(tau=[0.0] * T), dict(p=[0.9] * T), dict(k=[2] * T),
+                   dict(k=[V - 1] * T, p=[0.5] * T, min_p=[0.3] * T)):
+        for u in (0.0, 0.6, 1.0 - 2.0 ** -24):
+            _check_drawn(x, [u] * T, **params)
+
+
+def test_strided_and_unaligned_logits_and_extra_rows():
+    g = _gen(8)
+    for dtype in (BF16, F32):
+        wide = _logits(9, 1003 + 5, g, dtype)
+        sampler = step().Sampler(1003, 12, dtype)
+        _check_drawn(wide[:, 3:1006], torch.rand(9, generator=g).tolist(), sampler, p=[0.9] * 9)
+        _check_drawn(wide[:1, 1:1004], [0.4], sampler)
+        _check_drawn(wide[::2, :1003], [0.1, 0.2, 0.3, 0.4, 0.5], sampler, k=[0, 1, 2, 30, 4000])
+
+
+def test_extreme_temperatures():
+    x = _logits(6, 500, _gen(4))
+    _check_drawn(x, [0.9] * 6, tau=[1e-45, 1e-30, 1e30, 3e38, 1e-3, 1e3])
+
+
+def test_parameters_out_of_range_are_reported():
+    g = _gen(6)
+    x = _logits(4, 300, g)
+    s = step().Sampler(300, 4)
+    good = dict(temperature=[1.0] * 4, top_p=[0.9] * 4, min_p=[0.0] * 4, uniform=[0.5] * 4)
+    bad = dict(temperature=[-1.0, math.nan, math.inf], top_p=[0.0, -0.5, math.nan],
+               min_p=[-0.1, 1.5, math.nan], uniform=[-0.1, 1.0, math.nan])
+    for name, values in bad.items():
+        for v in values:
+            p = {n: torch.tensor([v if (n == name and t == 2) else q for t, q in enumerate(c)]).cuda()
+                 for n, c in good.items()}
+            u = p.pop("uniform")
+            ids = torch.empty(4, dtype=torch.int32, device="cuda")
+            probs = torch.empty(4, device="cuda")
+            s.sample_into(x, u, ids, probs, **p)
+            assert _status(s.sync) == N.ERR_ARGUMENT and _status(s.sync) == N.OK
+            assert ids[2] == -1 and probs[2] == 0
+            for t in (0, 1, 3):
+                assert int(ids[t]) == _drawn(x[t], p=float(np.float32(0.9)))[0]
+
+
+def test_sampler_refuses_calls():
+    s = step().Sampler(300, 4)
+    lib = N.moe_lib()
+    x, v = torch.zeros(8, 300, device="cuda"), torch.zeros(8, dtype=torch.int32, device="cuda")
+    u = torch.zeros(8, device="cuda")
+    call = lambda rows=4, stride=300, at=0, uni=u.data_ptr(), ids=v.data_ptr(): lib.urb_sample(
+        s._ctx, x.data_ptr() + at, stride, rows, None, uni, ids, None, None)
+    assert call() == N.OK
+    assert call(rows=0) == call(rows=5) == call(stride=299) == N.ERR_SHAPE
+    assert call(at=2) == call(uni=None) == call(ids=None) == N.ERR_ARGUMENT
+    with pytest.raises(ValueError):
+        s.sample(x[:4].half(), u[:4])
+    with pytest.raises(ValueError):
+        s.sample(x[:4], u[:4], top_k=u[:4])
+    torch.cuda.synchronize()
+
+
+# ---- together, and under capture ----------------------------------------------------------------
+
+class TokenStep:
+    """A decoder's token step around one MoE block: fused q/k/v projection of the residual stream with
+    adapters, norm and rotation of its heads, the block call, the vocabulary projection and the draw."""
+
+    HQ, HK, D, V = 4, 2, 64, 1008
+
+    def __init__(self, T):
+        self.T, self.host = T, _small_layer("c1_bf16_decode")
+        H = self.H = self.host.spec.hidden
+        self.layer = moe_mod().MoeLayer(self.host, max_tokens=T)
+        self.qkv = Proj("bf16", (self.HQ + 2 * self.HK) * self.D, H, T, F32, BF16, ranks=(8, 4), seed=2)
+        self.head = Proj("mxfp8", self.V, H, T, F32, ranks=(8,), seed=3)
+        self.sampler = step().Sampler(self.V, T)
+        g = _gen(9)
+        self.h = torch.empty(T, H, device="cuda")
+        self.norm = torch.from_numpy(synth.activations("norm", 1, H)[0] * np.float32(0.1)).cuda()
+        self.ids = torch.tensor([(t % 3) - 1 for t in range(T)], dtype=torch.int32, device="cuda")
+        self.head_ids = torch.clamp(self.ids, max=0)
+        self.w = torch.randn(self.D, generator=g).mul(0.1).cuda()
+        self.pos = torch.randint(0, 100000, (T,), generator=g).cuda()
+        self.u = torch.rand(T, generator=g).cuda()
+        self.p = torch.full((T,), 0.9, device="cuda")
+        self.freq = _freq(self.D)
+        rows = (self.HQ + 2 * self.HK) * self.D
+        self.out = dict(qkv=torch.empty(T, rows, dtype=BF16, device="cuda"),
+                        block=torch.empty(T, H, device="cuda"),
+                        logits=torch.empty(T, self.V, device="cuda"),
+                        tokens=torch.empty(T, dtype=torch.int32, device="cuda"),
+                        probs=torch.empty(T, device="cuda"))
+
+    def heads(self):
+        row, a, b = self.out["qkv"], self.HQ * self.D, (self.HQ + self.HK) * self.D
+        return (row[:, :a].unflatten(1, (self.HQ, self.D)),
+                row[:, a:b].unflatten(1, (self.HK, self.D)))
+
+    def run(self):
+        o = self.out
+        s = torch.cuda.current_stream()
+        self.qkv.p.forward_into(self.h, o["qkv"], self.ids)
+        q, k = self.heads()
+        step().qk_norm_rope(q, k, self.w, self.w, self.pos, self.freq, 1e-6,
+                            zero_centered=True, out=(q, k))
+        N.check(N.moe_lib().urb_moe_forward_block(
+            self.layer._ctx, self.h.data_ptr(), self.norm.data_ptr(), 1e-6, self.T,
+            o["block"].data_ptr(), None, None, s.cuda_stream or None), "block")
+        self.head.p.forward_into(o["block"], o["logits"], self.head_ids)
+        self.sampler.sample_into(o["logits"], self.u, o["tokens"], o["probs"], top_p=self.p)
+
+    def results(self):
+        torch.cuda.synchronize()
+        for c in (self.qkv.p, self.head.p, self.sampler, self.layer):
+            c.sync()
+        return {n: t.clone() for n, t in self.out.items()}
+
+    def check(self, got):
+        # each step against its definition on the step before's output
+        raw = self.qkv.p.forward(self.h, self.ids)
+        self.qkv.check(raw, self.h, self.ids)
+        a, b = self.HQ * self.D, (self.HQ + self.HK) * self.D
+        for lo, hi, n in ((0, a, self.HQ), (a, b, self.HK)):
+            _check_turned(got["qkv"][:, lo:hi].unflatten(1, (n, self.D)),
+                          raw[:, lo:hi].unflatten(1, (n, self.D)), self.w, self.pos, _freq(self.D))
+        assert torch.equal(got["qkv"][:, b:], raw[:, b:])
+        block, _, _ = self.layer.forward_block(self.h, self.norm, 1e-6)
+        assert torch.equal(got["block"], block)
+        self.head.check(got["logits"], block, self.head_ids)
+        for t in range(self.T):
+            id_, prob = _drawn(got["logits"][t], p=float(self.p[t]), u=float(self.u[t]))
+            assert int(got["tokens"][t]) == id_ and abs(float(got["probs"][t]) - prob) < 1e-6
+
+
+@pytest.mark.parametrize("T", [1, 5, 40])
+def test_a_token_step_around_the_block(T):
+    run = TokenStep(T)
+    run.h.copy_(torch.from_numpy(synth.activations("h", T, run.H)))
+    run.run()
+    run.check(run.results())
+
+
+@pytest.mark.parametrize("T", [1, 21])
+def test_a_captured_token_step_replays_on_new_inputs(T):
+    run, other = TokenStep(T), TokenStep(T)
+    inputs = [torch.from_numpy(synth.activations(f"h.{i}", T, run.H)).cuda() for i in range(4)]
+    run.h.copy_(inputs[0])
+    run.run()
+    run.results()
+    stream, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.graph(graph, stream=stream):
+        run.run()
+    for x in inputs[1:]:
+        for t in run.out.values():
+            t.zero_()
+        run.h.copy_(x)
+        graph.replay()
+        got = run.results()
+        other.h.copy_(x)      # eager work of the same program between the replays
+        other.run()
+        want = other.results()
+        for n in got:
+            assert torch.equal(got[n], want[n]), n
+    run.check(got)
+
+
+def test_steps_on_a_stream_of_their_own():
+    run, side = TokenStep(9), torch.cuda.Stream()
+    x = torch.from_numpy(synth.activations("h.side", 9, run.H)).cuda()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        run.h.copy_(x)
+        run.run()
+    side.synchronize()
+    run.check(run.results())

@@ -22,7 +22,8 @@ HIPCC_FLAGS = [
 MOE_SOURCES = ["urb_route.hip", "urb_panel.hip", "urb_combine.hip", "urb_gemm.hip",
                "urb_tall.hip", "urb_hy4.hip", "urb_decode.hip", "urb_scratch.hip",
                "urb_dense.hip", "urb_block.hip",
-               "urb_moe_host.cpp", "urb_residency.cpp"]
+               "urb_rotate.hip", "urb_sample.hip", "urb_project.hip",
+               "urb_moe_host.cpp", "urb_step_host.cpp", "urb_residency.cpp"]
 SYNTH_SOURCES = ["urb_synth.hip"]
 
 

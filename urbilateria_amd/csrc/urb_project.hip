@@ -1,0 +1,451 @@
+// urb_project.hip -- projections of token rows by one packed matrix with a low-rank adapter per row.
+//
+//   y[t] = W x[t] + scale_a B_a (A_a x[t])
+//
+// Two launches: the adapters' first products u = A x into the workspace, then W x with the
+// second products added to the accumulators before they are rounded (without adapters only the latter).
+//
+// Operands.  W streams in the panel layout (urb_kernels.hpp) straight into MFMA operands, MX codes
+// decoded to BF16 in registers (exact).  f32 rows are carried as three BF16 planes: truncating v to
+// 8 significant bits, then the rest, then the rest of that, loses none of its 24 bits; planes that are
+// zero for a whole operand (rows whose values are BF16 already) are skipped.  u is split the
+// same way, into two planes (16 bits) where the outputs are BF16, three where they are f32.
+//
+// A tile may hold rows of any adapters: each distinct adapter of the tile multiplies the tile's u with
+// the other adapters' rows set to zero, so order and mix of the rows cost time but no sorting pass.
+#include "urb_panel.hpp"
+#include "urb_step.hpp"
+
+namespace urb {
+
+namespace {
+
+constexpr int kThreads = 256;
+
+// v as BF16 planes by truncation, v = hi + mid + lo exactly (v finite and not subnormal in the
+// lower planes); an infinity keeps its first plane alone.
+__device__ __forceinline__ float plane_rest(float v, float hi) { return v == hi ? 0.0f : v - hi; }
+__device__ __forceinline__ float trunc_bf16(float v) { return u2f(f2u(v) & 0xffff0000u); }
+// the upper halves of two words: a's in the low half
+__device__ __forceinline__ uint32_t high_halves(float a, float b) {
+  return __builtin_amdgcn_perm(f2u(b), f2u(a), 0x07060302u);
+}
+
+// Eight values in BF16 planes.
+template <int P>
+struct Planes {
+  uint32_t w[P][4];
+  __device__ __forceinline__ bf16x8 operand(int p) const {
+    return __builtin_bit_cast(bf16x8, make_uint4(w[p][0], w[p][1], w[p][2], w[p][3]));
+  }
+};
+template <int P>
+__device__ __forceinline__ Planes<P> split_planes(const float (&v)[8]) {
+  Planes<P> r;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    float a = v[2 * i], b = v[2 * i + 1];
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+      if (P == 2 && p == 1) {  // the last of two planes: rounded
+        r.w[p][i] = pk_bf16(a, b);
+      } else {
+        r.w[p][i] = high_halves(a, b);
+        const float ha = trunc_bf16(a), hb = trunc_bf16(b);
+        a = plane_rest(a, ha);
+        b = plane_rest(b, hb);
+      }
+    }
+  }
+  return r;
+}
+
+__device__ __forceinline__ f32x4 mfma(bf16x8 a, bf16x8 b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+
+// The eight values at `k` of a token row as MFMA planes: one for BF16 rows, three for f32 ones.
+template <bool XB>
+constexpr int x_planes() { return XB ? 1 : 3; }
+template <bool XB>
+__device__ __forceinline__ Planes<x_planes<XB>()> load_x(const uint8_t* row, int k) {
+  if constexpr (XB) {
+    const uint4 q = ldg16(row + 2 * (size_t)k);
+    return {{{q.x, q.y, q.z, q.w}}};
+  } else {
+    const float4 a = u2f4(ldg16(row + 4 * (size_t)k)), b = u2f4(ldg16(row + 4 * (size_t)k + 16));
+    const float v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+    return split_planes<3>(v);
+  }
+}
+// acc += w * x over the planes of x that hold anything for some lane.
+template <int P>
+__device__ __forceinline__ f32x4 mma_planes(bf16x8 w, const Planes<P>& x, f32x4 acc) {
+  acc = mfma(w, x.operand(0), acc);
+  if constexpr (P == 3) {
+    if (__ballot((x.w[1][0] | x.w[1][1] | x.w[1][2] | x.w[1][3]) != 0)) {
+      acc = mfma(w, x.operand(1), acc);
+      acc = mfma(w, x.operand(2), acc);
+    }
+  }
+  return acc;
+}
+
+// ---- u[slice][t] = A x[t] over the slice's part of K, for every row with an adapter ----
+
+constexpr int kScan = 512;  // tokens per workgroup of the first product
+
+// grid: (adapter or token, K slice, segment of kScan tokens).  BY_TOKEN: blockIdx.x is a token, whose
+// workgroup computes for all rows of the same adapter if it is the first of them.
+// Four waves split the slice's K; each takes 16 tokens x 64 ranks at a time.
+template <bool XB, bool BY_TOKEN>
+__global__ __launch_bounds__(kThreads) void shrink_kernel(ProjArgs p, int u_ld, int slices) {
+  __shared__ int s_tokens[kScan];
+  __shared__ int s_count[kThreads / 64 + 1];
+  __shared__ f32x4 s_red[3][4][64];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int first = blockIdx.z * kScan, last = min(first + kScan, p.tokens);
+  int slot;
+  if constexpr (BY_TOKEN) {
+    slot = p.ids[blockIdx.x];
+  } else {
+    slot = blockIdx.x;
+  }
+  // ids that name no adapter: reported once, by the first workgroup of each segment
+  if (blockIdx.x == 0 && blockIdx.y == 0) {
+    for (int t = first + tid; t < last; t += kThreads) {
+      const int id = p.ids[t];
+      if (id >= p.slots || (id >= 0 && p.table[id].rank == 0)) flag(p.status, kStepArgument);
+    }
+  }
+  if (slot < 0 || slot >= p.slots) return;
+  const int rank = p.table[slot].rank;
+  if (rank == 0) return;
+  // this segment's rows of the adapter, in order
+  int n = 0;
+  for (int t0 = first; t0 < last; t0 += kThreads) {
+    const int t = t0 + tid;
+    const bool mine = t < last && p.ids[t] == slot;
+    const uint64_t vote = __ballot(mine);
+    if (lane == 0) s_count[wave] = __popcll(vote);
+    __syncthreads();
+    int at = n;
+    for (int w = 0; w < wave; ++w) at += s_count[w];
+    if (mine) s_tokens[at + __popcll(vote & ((1ull << lane) - 1))] = t;
+    for (int w = 0; w < kThreads / 64; ++w) n += s_count[w];
+    __syncthreads();
+  }
+  if (n == 0) return;
+  if (BY_TOKEN && s_tokens[0] != (int)blockIdx.x) return;
+
+  const int ln = lane & 15, lq = lane >> 4;
+  const int steps = p.cols / 32;
+  // the slice's steps of 32 columns, and the wave's among them
+  const int s0 = (int)((long long)steps * blockIdx.y / slices);
+  const int s1 = (int)((long long)steps * (blockIdx.y + 1) / slices);
+  const int w0 = s0 + (s1 - s0) * wave / 4, w1 = s0 + (s1 - s0) * (wave + 1) / 4;
+  const uint8_t* x = reinterpret_cast<const uint8_t*>(p.x);
+  const size_t xs = p.x_stride * (XB ? 2 : 4);
+  const uint16_t* a = p.a + (size_t)slot * p.a_slot;
+  const int panels = (rank + 15) / 16;
+  float* u = p.u + (size_t)blockIdx.y * p.tokens * u_ld;
+  for (int m = 0; m < n; m += 16) {
+    const bool there = m + ln < n;
+    const int t = s_tokens[there ? m + ln : m];
+    const uint8_t* row = x + (size_t)t * xs;
+    for (int q0 = 0; q0 < panels; q0 += 4) {
+      f32x4 acc[4];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) acc[q] = f32x4{0.f, 0.f, 0.f, 0.f};
+      for (int s = w0; s < w1; ++s) {
+        const auto xv = load_x<XB>(row, 32 * s + 8 * lq);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          if (q0 + q >= panels) break;
+          uint4 w = make_uint4(0, 0, 0, 0);
+          if (16 * (q0 + q) + ln < rank)
+            w = ldg16(a + ((size_t)(q0 + q) * steps + s) * 512 + 8 * lane);
+          acc[q] = mma_planes(__builtin_bit_cast(bf16x8, w), xv, acc[q]);
+        }
+      }
+      // the waves' parts, in order; lane (ln, lq) holds ranks 4 lq + [0, 4) of token ln
+      __syncthreads();
+      if (wave > 0)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) s_red[wave - 1][q][lane] = acc[q];
+      __syncthreads();
+      if (wave == 0 && there) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          if (q0 + q >= panels) break;
+          f32x4 v = acc[q];
+          for (int w = 0; w < 3; ++w) v += s_red[w][q][lane];
+          *reinterpret_cast<f32x4*>(u + (size_t)t * u_ld + 16 * (q0 + q) + 4 * lq) = v;
+        }
+      }
+    }
+  }
+}
+
+// ---- the second products, added to the accumulators of a tile ----
+
+// The distinct filled slots among `count` rows from `t0` (at most kMax), in LDS.
+template <int MAX>
+struct TileSlots {
+  int ids[MAX];
+  int list[MAX];
+  int n;
+};
+template <int MAX>
+__device__ __forceinline__ void find_slots(const ProjArgs& p, int t0, int count, TileSlots<MAX>& s) {
+  const int tid = threadIdx.x;
+  if (tid == 0) s.n = 0;
+  for (int i = tid; i < MAX; i += blockDim.x) {
+    int id = i < count ? p.ids[t0 + i] : -1;
+    if (id >= p.slots || (id >= 0 && p.table[id].rank == 0)) id = -1;
+    s.ids[i] = id;
+  }
+  __syncthreads();
+  for (int i = tid; i < count; i += blockDim.x) {
+    const int id = s.ids[i];
+    if (id < 0) continue;
+    bool first = true;
+    for (int j = 0; j < i && first; ++j) first = s.ids[j] != id;
+    // (in any order: every row is in one adapter's product, so the order changes no sum)
+    if (first) s.list[atomicAdd(&s.n, 1)] = id;
+  }
+  __syncthreads();
+}
+
+// acc (lane (ln, lq): rows 16 panel + 4 lq + [0, 4) of token `local`, at `t`) += the adapters' parts.
+template <int P, int MAX>
+__device__ __forceinline__ void add_adapters(const ProjArgs& p, const TileSlots<MAX>& s, int u_ld,
+                                             int slices, int panel, int local, int t, f32x4& acc) {
+  const int lane = threadIdx.x & 63, lq = lane >> 4;
+  const int mine = s.ids[local];
+  for (int i = 0; i < s.n; ++i) {
+    const int slot = s.list[i];
+    if (!__ballot(mine == slot)) continue;
+    const AdapterEntry e = p.table[slot];
+    const int units = (e.rank + 7) / 8;
+    const uint16_t* b = p.b + (size_t)slot * p.b_slot + (size_t)panel * units * 128;
+    for (int r = 0; r < units; r += 4) {
+      uint4 w = make_uint4(0, 0, 0, 0);
+      float v[8] = {};
+      if (r + lq < units) {
+        w = ldg16(b + (size_t)r * 128 + 8 * lane);
+        if (mine == slot) {
+          const float* u = p.u + (size_t)t * u_ld + 8 * (r + lq);
+          for (int z = 0; z < slices; ++z) {
+            const float4 c = *reinterpret_cast<const float4*>(u);
+            const float4 d = *reinterpret_cast<const float4*>(u + 4);
+            v[0] += c.x; v[1] += c.y; v[2] += c.z; v[3] += c.w;
+            v[4] += d.x; v[5] += d.y; v[6] += d.z; v[7] += d.w;
+            u += (size_t)p.tokens * u_ld;
+          }
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] *= e.scale;
+      const Planes<P> uv = split_planes<P>(v);
+#pragma unroll
+      for (int q = 0; q < P; ++q) acc = mfma(__builtin_bit_cast(bf16x8, w), uv.operand(q), acc);
+    }
+  }
+}
+
+// Four consecutive outputs of a token.
+template <bool YB>
+__device__ __forceinline__ void store_y(const ProjArgs& p, int t, int row, f32x4 v) {
+  const size_t at = (size_t)t * p.y_stride + row;
+  if constexpr (YB) {
+    uint16_t* y = reinterpret_cast<uint16_t*>(p.y) + at;
+    const uint32_t a = pk_bf16(v[0], v[1]), b = pk_bf16(v[2], v[3]);
+    if (reinterpret_cast<uintptr_t>(y) % 8 == 0) {
+      *reinterpret_cast<uint2*>(y) = make_uint2(a, b);
+    } else {
+      y[0] = (uint16_t)a; y[1] = (uint16_t)(a >> 16);
+      y[2] = (uint16_t)b; y[3] = (uint16_t)(b >> 16);
+    }
+  } else {
+    float* y = reinterpret_cast<float*>(p.y) + at;
+    if (reinterpret_cast<uintptr_t>(y) % 16 == 0) {
+      *reinterpret_cast<float4*>(y) = make_float4(v[0], v[1], v[2], v[3]);
+    } else {
+      y[0] = v[0]; y[1] = v[1]; y[2] = v[2]; y[3] = v[3];
+    }
+  }
+}
+
+// ---- W x for a few tokens: eight waves split K of NP panels, 16 MB tokens per tile ----
+constexpr int kSplitWaves = 8;
+
+template <int FMT, bool XB, bool YB, int MB, int NP>
+__global__ __launch_bounds__(64 * kSplitWaves) void split_kernel(ProjArgs p, int u_ld, int slices) {
+  constexpr int TILE = 16 * MB;
+  __shared__ f32x4 red[kSplitWaves][NP * MB][64];
+  __shared__ TileSlots<TILE> slots;
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int ln = lane & 15, lq = lane >> 4;
+  const int t0 = blockIdx.y * TILE, count = min(TILE, p.tokens - t0);
+  const int panels = p.rows / kPanelRows;
+  const int panel0 = blockIdx.x * NP;
+  const int steps = p.cols / kGemmKStep;
+  const int s0 = steps * wave / kSplitWaves, s1 = steps * (wave + 1) / kSplitWaves;
+  const size_t pbytes = kPanelRows * panel_row_bytes<FMT>(p.cols);
+  const size_t pscales = (size_t)kPanelRows * (p.cols / 32);
+  const uint8_t* pd[NP];
+  const uint8_t* ps[NP];
+#pragma unroll
+  for (int q = 0; q < NP; ++q) {  // a panel past the last reads the last again and stores nothing
+    const int panel = min(panel0 + q, panels - 1);
+    pd[q] = p.data + panel * pbytes;
+    ps[q] = FMT == kFmtBF16 ? nullptr : p.scales + panel * pscales;
+  }
+  const uint8_t* row[MB];
+#pragma unroll
+  for (int m = 0; m < MB; ++m)
+    row[m] = reinterpret_cast<const uint8_t*>(p.x) +
+             (size_t)(t0 + min(16 * m + ln, count - 1)) * p.x_stride * (XB ? 2 : 4);
+  f32x4 acc[NP][MB];
+#pragma unroll
+  for (int q = 0; q < NP; ++q)
+#pragma unroll
+    for (int m = 0; m < MB; ++m) acc[q][m] = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int s = s0; s < s1; ++s) {
+    BRaw<FMT> r[NP];
+#pragma unroll
+    for (int q = 0; q < NP; ++q) load_b<FMT>(r[q], pd[q], 16u * lane, ps[q], lane, s);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      bf16x8 w[NP];
+#pragma unroll
+      for (int q = 0; q < NP; ++q) w[q] = decode_b<FMT>(r[q], j);
+#pragma unroll
+      for (int m = 0; m < MB; ++m) {
+        const auto xv = load_x<XB>(row[m], kGemmKStep * s + frag_k<FMT>(j, lq));
+#pragma unroll
+        for (int q = 0; q < NP; ++q) acc[q][m] = mma_planes(w[q], xv, acc[q][m]);
+      }
+    }
+  }
+#pragma unroll
+  for (int q = 0; q < NP; ++q)
+#pragma unroll
+    for (int m = 0; m < MB; ++m) red[wave][q * MB + m][lane] = acc[q][m];
+  if (p.ids) find_slots(p, t0, count, slots);
+  __syncthreads();
+  for (int i = wave; i < NP * MB; i += kSplitWaves) {
+    const int q = i / MB, m = i % MB, panel = panel0 + q;
+    if (panel >= panels) break;
+    f32x4 v = red[0][i][lane];
+#pragma unroll
+    for (int z = 1; z < kSplitWaves; ++z) v += red[z][i][lane];  // K parts in order
+    const int local = 16 * m + ln, t = t0 + local;
+    if (p.ids) add_adapters<YB ? 2 : 3>(p, slots, u_ld, slices, panel, local, t, v);
+    if (local < count) store_y<YB>(p, t, panel * kPanelRows + 4 * lq, v);
+  }
+}
+
+// ---- laying an adapter out ----
+// A: 16-rank panels of the BF16 panel layout; B: units of 8 ranks, [panel of 16 rows][unit][row].
+__global__ void pack_adapter_kernel(const uint16_t* __restrict__ a, const uint16_t* __restrict__ b,
+                                    int rank, int rows, int cols, uint16_t* __restrict__ pa,
+                                    uint16_t* __restrict__ pb, int* flag_word) {
+  const size_t stride = (size_t)gridDim.x * blockDim.x;
+  const size_t at = blockIdx.x * (size_t)blockDim.x + threadIdx.x;
+  bool bad = false;
+  auto take = [&](uint16_t v) {
+    bad |= (v & 0x7f80u) == 0x7f80u;
+    return v;
+  };
+  const int panels = (rank + 15) / 16, slabs = cols / 32;
+  for (size_t i = at; i < (size_t)panels * 16 * cols; i += stride) {
+    const size_t unit = i / 8;
+    const int l = (int)(unit % 64), slab = (int)(unit / 64 % slabs), panel = (int)(unit / 64 / slabs);
+    const int r = 16 * panel + (l & 15), c = 32 * slab + 8 * (l >> 4) + (int)(i % 8);
+    pa[i] = r < rank ? take(a[(size_t)r * cols + c]) : 0;
+  }
+  const int units = (rank + 7) / 8;
+  for (size_t i = at; i < (size_t)rows * units * 8; i += stride) {
+    const size_t unit = i / 8;
+    const int ln = (int)(unit % 16), ru = (int)(unit / 16 % units);
+    const size_t row = unit / 16 / units * 16 + ln;
+    const int r = 8 * ru + (int)(i % 8);
+    pb[i] = r < rank ? take(b[row * rank + r]) : 0;
+  }
+  if (bad) atomicOr(flag_word, 1);
+}
+__global__ void enter_adapter_kernel(int rank, float scale, AdapterEntry* entry, int* flag_word,
+                                     int* status) {
+  if (*flag_word) {
+    flag(status, kStepNonFinite);
+    rank = 0;
+  }
+  *flag_word = 0;
+  *entry = AdapterEntry{rank, scale};
+}
+
+template <int FMT, bool XB, bool YB>
+void launch_rows(const ProjArgs& p, int u_ld, int slices, hipStream_t s) {
+  const int panels = p.rows / kPanelRows;
+  auto go = [&](auto mb, auto np) {
+    constexpr int MB = decltype(mb)::value, NP = decltype(np)::value;
+    const dim3 grid((panels + NP - 1) / NP, (p.tokens + 16 * MB - 1) / (16 * MB));
+    split_kernel<FMT, XB, YB, MB, NP><<<grid, 64 * kSplitWaves, 0, s>>>(p, u_ld, slices);
+  };
+  if (p.tokens <= 16) go(Int<1>{}, Int<1>{});
+  else if (p.tokens <= 32) go(Int<2>{}, Int<2>{});
+  else go(Int<4>{}, Int<2>{});
+}
+
+template <bool XB>
+void launch_shrink(const ProjArgs& p, int u_ld, int slices, hipStream_t s) {
+  const bool by_token = p.tokens <= kScan && p.tokens <= p.slots;
+  // (without slots one workgroup per segment, which reports the ids)
+  const dim3 grid(by_token ? p.tokens : std::max(1, p.slots), slices,
+                  (p.tokens + kScan - 1) / kScan);
+  if (by_token) shrink_kernel<XB, true><<<grid, kThreads, 0, s>>>(p, u_ld, slices);
+  else shrink_kernel<XB, false><<<grid, kThreads, 0, s>>>(p, u_ld, slices);
+}
+
+template <int FMT>
+void launch_types(const ProjArgs& p, int u_ld, int slices, hipStream_t s) {
+  if (p.x_bf16) {
+    if (p.y_bf16) launch_rows<FMT, true, true>(p, u_ld, slices, s);
+    else launch_rows<FMT, true, false>(p, u_ld, slices, s);
+  } else {
+    if (p.y_bf16) launch_rows<FMT, false, true>(p, u_ld, slices, s);
+    else launch_rows<FMT, false, false>(p, u_ld, slices, s);
+  }
+}
+
+}  // namespace
+
+void launch_project(const ProjArgs& p, hipStream_t s) {
+  const int u_ld = 16 * rank_panels(p.max_rank);
+  int slices = 1;
+  if (p.ids) {
+    slices = std::min(kMaxSlices, std::max(1, p.cols / 512));
+    if (p.x_bf16) launch_shrink<true>(p, u_ld, slices, s);
+    else launch_shrink<false>(p, u_ld, slices, s);
+  }
+  if (p.format == kFmtBF16) launch_types<kFmtBF16>(p, u_ld, slices, s);
+  else if (p.format == kFmtMXFP4) launch_types<kFmtMXFP4>(p, u_ld, slices, s);
+  else launch_types<kFmtMXFP8>(p, u_ld, slices, s);
+}
+
+void launch_set_adapter(const uint16_t* a, const uint16_t* b, int rank, float scale, int rows,
+                        int cols, uint16_t* slot_a, uint16_t* slot_b, AdapterEntry* entry,
+                        int* flag_word, int* status, hipStream_t s) {
+  if (rank > 0) {
+    const size_t n = (size_t)rank_panels(rank) * 16 * cols + (size_t)rows * rank_units(rank) * 8;
+    const int blocks = (int)std::min<size_t>((n + 255) / 256, 2048);
+    pack_adapter_kernel<<<blocks, 256, 0, s>>>(a, b, rank, rows, cols, slot_a, slot_b, flag_word);
+  }
+  enter_adapter_kernel<<<1, 1, 0, s>>>(rank, scale, entry, flag_word, status);
+}
+
+}  // namespace urb

@@ -1,5 +1,5 @@
-"""ctypes binding of the C ABI in ``include/urb_moe.h`` (``liburb_moe.so``) and of the device
-workload generator (``liburb_synth.so``).
+"""ctypes binding of the C ABI in ``include/urb_moe.h`` and ``include/urb_step.h``
+(``liburb_moe.so``) and of the device workload generator (``liburb_synth.so``).
 
 The shared libraries are built in-tree by ``__graft_entry__.build()``.  Loading fails loudly
 when they are missing: there is no CPU fallback for any entry point.
@@ -27,6 +27,10 @@ EXPORTS = ("urb_moe_create", "urb_moe_destroy", "urb_moe_forward", "urb_moe_rout
            "urb_moe_set_expert", "urb_moe_forward_tokens", "urb_moe_route_tokens",
            "urb_quantize_e4m3_blocks", "urb_gemm_placement", "urb_moe_forward_noalloc",
            "urb_inspect_matrix", "urb_gemm_tile_rows")
+# Every symbol include/urb_step.h declares.
+STEP_EXPORTS = ("urb_proj_create", "urb_proj_destroy", "urb_proj_set_adapter",
+                "urb_proj_forward", "urb_proj_sync", "urb_proj_memory", "urb_qk_norm_rope",
+                "urb_sampler_create", "urb_sampler_destroy", "urb_sample", "urb_sampler_sync")
 STAGES = ("router", "route", "permute", "gate_up", "down", "shared_gate_up", "shared_down",
           "combine")
 SYNTH_EXPORTS = ("urb_synth_bf16", "urb_synth_activations", "urb_synth_fp4", "urb_synth_fp8",
@@ -73,6 +77,39 @@ class Weights(ctypes.Structure):
                 ("experts", ctypes.c_void_p), ("shared", ctypes.c_void_p),
                 ("shared_expert_gate", ctypes.c_void_p),
                 ("hash_experts", ctypes.c_void_p), ("hash_vocab", ctypes.c_uint32)]
+
+
+class ProjDesc(ctypes.Structure):
+    _fields_ = [("rows", ctypes.c_uint32), ("cols", ctypes.c_uint32), ("format", ctypes.c_int),
+                ("x_dtype", ctypes.c_int), ("y_dtype", ctypes.c_int),
+                ("max_tokens", ctypes.c_uint32), ("adapter_slots", ctypes.c_uint32),
+                ("max_rank", ctypes.c_uint32)]
+
+
+class Adapter(ctypes.Structure):
+    _fields_ = [("a", ctypes.c_void_p), ("b", ctypes.c_void_p), ("rank", ctypes.c_uint32),
+                ("scale", ctypes.c_float)]
+
+
+class QkDesc(ctypes.Structure):
+    _fields_ = [("dtype", ctypes.c_int), ("q_heads", ctypes.c_uint32),
+                ("k_heads", ctypes.c_uint32), ("head_dim", ctypes.c_uint32),
+                ("rotary_dim", ctypes.c_uint32), ("interleaved", ctypes.c_int32),
+                ("zero_centered", ctypes.c_int32), ("eps", ctypes.c_float)] + [
+        (name, ctypes.c_uint64) for name in (
+            "q_token_stride", "q_head_stride", "k_token_stride", "k_head_stride",
+            "q_out_token_stride", "q_out_head_stride", "k_out_token_stride",
+            "k_out_head_stride")]
+
+
+class SamplerDesc(ctypes.Structure):
+    _fields_ = [("vocab", ctypes.c_uint32), ("max_rows", ctypes.c_uint32),
+                ("dtype", ctypes.c_int)]
+
+
+class SampleParams(ctypes.Structure):
+    _fields_ = [("temperature", ctypes.c_void_p), ("top_k", ctypes.c_void_p),
+                ("top_p", ctypes.c_void_p), ("min_p", ctypes.c_void_p)]
 
 
 _moe = None
@@ -145,7 +182,23 @@ def moe_lib() -> ctypes.CDLL:
         lib.urb_gemm_tile_rows.restype = u32
         lib.urb_status_string.argtypes = [ctypes.c_int]
         lib.urb_status_string.restype = ctypes.c_char_p
-        for f in EXPORTS:
+        u64, status = ctypes.c_uint64, ctypes.c_int
+        lib.urb_proj_create.argtypes = [ctypes.POINTER(ProjDesc), ctypes.POINTER(Matrix),
+                                        ctypes.c_int, ctypes.POINTER(ctypes.c_void_p)]
+        lib.urb_proj_destroy.argtypes = [P]
+        lib.urb_proj_set_adapter.argtypes = [P, u32, ctypes.POINTER(Adapter), ctypes.c_int, P]
+        lib.urb_proj_forward.argtypes = [P, P, u64, P, u32, P, u64, P]
+        lib.urb_proj_sync.argtypes = [P, P]
+        lib.urb_proj_memory.argtypes = [P] + [ctypes.POINTER(ctypes.c_size_t)] * 3
+        lib.urb_qk_norm_rope.argtypes = [ctypes.POINTER(QkDesc), P, P, P, P, P, P, u32, P, P, P]
+        lib.urb_sampler_create.argtypes = [ctypes.POINTER(SamplerDesc),
+                                           ctypes.POINTER(ctypes.c_void_p)]
+        lib.urb_sampler_destroy.argtypes = [P]
+        lib.urb_sample.argtypes = [P, P, u64, u32, ctypes.POINTER(SampleParams), P, P, P, P]
+        lib.urb_sampler_sync.argtypes = [P, P]
+        for f in STEP_EXPORTS:
+            getattr(lib, f).restype = None if f.endswith("_destroy") else status
+        for f in EXPORTS + STEP_EXPORTS:
             if getattr(lib, f).argtypes is None:
                 raise RuntimeError(f"{f}: no ctypes signature")
         _moe = lib
