@@ -37,19 +37,38 @@ def _on_host(t) -> bool:
     return isinstance(t, np.ndarray) or t.device.type == "cpu"
 
 
-def _vector(t, name: str, n: int, dtype, device) -> Optional[int]:
-    """The address of a contiguous device vector of n values, or None."""
+class _Current:
+    """torch.cuda.device(index), entered only where another device is current."""
+    __slots__ = ("index", "guard")
+
+    def __init__(self, index: int):
+        self.index = index
+
+    def __enter__(self):
+        self.guard = None
+        if torch.cuda.current_device() != self.index:
+            self.guard = torch.cuda.device(self.index)
+            self.guard.__enter__()
+
+    def __exit__(self, *error):
+        if self.guard is not None:
+            self.guard.__exit__(*error)
+
+
+def _vector(t, name: str, n: int, dtype, device: int) -> Optional[int]:
+    """The address of a contiguous vector of n values on the device, or None."""
     if t is None:
         return None
-    if t.device != device or t.dtype != dtype or t.numel() != n or not t.is_contiguous():
-        raise ValueError(f"{name} must be a contiguous {dtype} tensor of {n} values on {device}")
+    if t.get_device() != device or t.dtype != dtype or t.numel() != n or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous {dtype} tensor of {n} values on "
+                         f"cuda:{device}")
     return t.data_ptr()
 
 
-def _rows(t, name: str, cols: int, dtype, device) -> int:
-    """The row stride of a [rows, cols] device tensor whose rows are contiguous."""
-    if t.device != device or t.dtype != dtype or t.dim() != 2 or t.shape[1] != cols:
-        raise ValueError(f"{name} must be a {dtype} [rows, {cols}] tensor on {device}")
+def _rows(t, name: str, cols: int, dtype, device: int) -> int:
+    """The row stride of a [rows, cols] tensor on the device whose rows are contiguous."""
+    if t.get_device() != device or t.dtype != dtype or t.dim() != 2 or t.shape[1] != cols:
+        raise ValueError(f"{name} must be a {dtype} [rows, {cols}] tensor on cuda:{device}")
     if cols > 1 and t.stride(1) != 1:
         raise ValueError(f"{name}: the values of a row must be contiguous")
     return t.stride(0) if t.shape[0] > 1 else cols
@@ -60,14 +79,14 @@ class _Context:
     _destroy = _sync = None
 
     def _make(self, create, *args) -> None:
-        self.device = torch.device("cuda", torch.cuda.current_device())
+        self.device = torch.cuda.current_device()
         ctx = ctypes.c_void_p()
         N.check(create(*args, ctypes.byref(ctx)), create.__name__)
         self._ctx = ctx
 
     def sync(self, stream=None) -> None:
         """Waits for the stream and raises UrbError for a failure of the calls before."""
-        with torch.cuda.device(self.device):
+        with _Current(self.device):
             N.check(getattr(N.moe_lib(), self._sync)(self._ctx, _stream_handle(stream)),
                     self._sync)
 
@@ -128,13 +147,13 @@ class AdaptedProjection(_Context):
             raise ValueError("a and b must be in the same memory")
         ad = N.Adapter(_ptr(a), _ptr(b), rank, float(scale))
         source = N.SOURCE_HOST if _on_host(a) else N.SOURCE_DEVICE_COPY
-        with torch.cuda.device(self.device):
+        with _Current(self.device):
             N.check(N.moe_lib().urb_proj_set_adapter(self._ctx, slot, ctypes.byref(ad), source,
                                                      _stream_handle(stream)),
                     "urb_proj_set_adapter")
 
     def clear_adapter(self, slot: int, stream=None) -> None:
-        with torch.cuda.device(self.device):
+        with _Current(self.device):
             N.check(N.moe_lib().urb_proj_set_adapter(self._ctx, slot, None, N.SOURCE_DEVICE_COPY,
                                                      _stream_handle(stream)),
                     "urb_proj_set_adapter")
@@ -148,7 +167,7 @@ class AdaptedProjection(_Context):
         if y.shape[0] != T:
             raise ValueError("x and y must have the same number of rows")
         ids = _vector(adapter_ids, "adapter_ids", T, torch.int32, self.device)
-        with torch.cuda.device(self.device):
+        with _Current(self.device):
             N.check(N.moe_lib().urb_proj_forward(self._ctx, x.data_ptr(), xs, ids, T, y.data_ptr(),
                                                  ys, _stream_handle(stream)), "urb_proj_forward")
 
@@ -176,6 +195,9 @@ def qk_norm_rope(q, k, q_weight, k_weight, positions, inv_freq, eps: float,
                                            or k.shape[2] != q.shape[2])):
         raise ValueError("q must be [T, heads, D] and k [T, k_heads, D]")
     T, hq, D = q.shape
+    device = q.get_device()
+    if device < 0:
+        raise ValueError("q must be on a GPU")
     hk = 0 if k is None else k.shape[1]
     if out is None:
         out = (torch.empty((T, hq, D), dtype=q.dtype, device=q.device),
@@ -185,17 +207,17 @@ def qk_norm_rope(q, k, q_weight, k_weight, positions, inv_freq, eps: float,
         raise ValueError("out must have the shapes of q and k")
     used = [("q", q), ("q_out", qo)] + ([] if k is None else [("k", k), ("k_out", ko)])
     for name, t in used:
-        if t.dtype != q.dtype or t.device != q.device or (D > 1 and t.stride(2) != 1):
+        if t.dtype != q.dtype or t.get_device() != device or (D > 1 and t.stride(2) != 1):
             raise ValueError(f"{name}: heads must be contiguous, of q's type and device")
     half = 0 if inv_freq is None else inv_freq.numel()
     strides = [s for t in (q, k, qo, ko) for s in ((0, 0) if t is None else t.stride()[:2])]
     desc = N.QkDesc(_type(q.dtype), hq, hk, D, 2 * half, int(interleaved), int(zero_centered),
                     float(eps), *strides)
-    args = [_vector(q_weight, "q_weight", D, torch.float32, q.device),
-            _vector(k_weight if hk else None, "k_weight", D, torch.float32, q.device),
-            _vector(positions, "positions", T, torch.int64, q.device),
-            _vector(inv_freq, "inv_freq", half, torch.float32, q.device)]
-    with torch.cuda.device(q.device):
+    args = (_vector(q_weight, "q_weight", D, torch.float32, device),
+            _vector(k_weight, "k_weight", D, torch.float32, device) if hk else None,
+            _vector(positions, "positions", T, torch.int64, device),
+            _vector(inv_freq, "inv_freq", half, torch.float32, device))
+    with _Current(device):
         N.check(N.moe_lib().urb_qk_norm_rope(ctypes.byref(desc), q.data_ptr(),
                                              k.data_ptr() if hk else None, *args, T,
                                              qo.data_ptr(), ko.data_ptr() if hk else None,
@@ -226,7 +248,7 @@ class Sampler(_Context):
                                 _vector(top_k, "top_k", T, torch.int32, dev),
                                 _vector(top_p, "top_p", T, f32, dev),
                                 _vector(min_p, "min_p", T, f32, dev))
-        with torch.cuda.device(dev):
+        with _Current(dev):
             N.check(N.moe_lib().urb_sample(
                 self._ctx, logits.data_ptr(), stride, T, ctypes.byref(params),
                 _vector(uniform, "uniform", T, f32, dev), _vector(ids, "ids", T, torch.int32, dev),
