@@ -44,7 +44,11 @@ struct SampleArgs {
   int32_t* ids;
   float* probs;
   int* status;
+  void* work;  // sample_work_bytes(vocab, the most rows of a call)
 };
+// Rows per pass of a call (longer calls run in passes of this many).
+constexpr int kSamplePass = 512;
+size_t sample_work_bytes(int vocab, int rows);
 void launch_sample(const SampleArgs& a, bool bf16, hipStream_t s);
 
 // ---- projections with adapters (urb_project.hip) ----

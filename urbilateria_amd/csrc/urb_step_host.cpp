@@ -352,7 +352,7 @@ urb_status urb_sampler_create(const urb_sampler_desc* d, urb_sampler** out) {
   c->desc = *d;
   const urb_status st = [&]() -> urb_status {
     URB_HIP(hipGetDevice(&c->device));
-    URB_HIP(hipMalloc(&c->work, kAlign));
+    URB_HIP(hipMalloc(&c->work, kAlign + urb::sample_work_bytes((int)d->vocab, (int)d->max_rows)));
     c->status = static_cast<int*>(c->work);
     urb::launch_fill_i32(c->status, 0, kAlign / 4, nullptr);
     URB_HIP(hipGetLastError());
@@ -402,6 +402,7 @@ urb_status urb_sample(urb_sampler* c, const void* logits, uint64_t row_stride, u
   a.ids = ids;
   a.probs = probs;
   a.status = c->status;
+  a.work = static_cast<char*>(c->work) + kAlign;
   urb::launch_sample(a, d.dtype == URB_DTYPE_BF16, static_cast<hipStream_t>(stream));
   URB_HIP(hipGetLastError());
   return URB_OK;

@@ -19,14 +19,22 @@ import numpy as np
 
 from . import configs as C
 from . import native as N
-from .moe import _ptr, _stream_handle, torch
+from .moe import _ptr, torch
 
-_TYPES = {"bfloat16": N.DTYPES["BF16"], "float32": N.DTYPES["F32"]}
+# the urb_dtype of rows; other types are the library's to refuse
+_TYPES = {} if torch is None else {torch.bfloat16: N.DTYPES["BF16"], torch.float32: N.DTYPES["F32"]}
 
 
 def _type(dtype) -> int:
-    """The urb_dtype of rows; other types are the library's to refuse."""
-    return _TYPES.get(str(dtype).replace("torch.", ""), 7)
+    return _TYPES.get(dtype, 7)
+
+
+def _stream(stream, device: int) -> int:
+    """The handle of a stream, or of the device's current one (the call that torch's own generated
+    code makes: torch.cuda.current_stream() builds an object, 2.9 us of a 10 us call)."""
+    if stream is not None:
+        return stream.cuda_stream
+    return torch._C._cuda_getCurrentRawStream(device)
 
 
 def _bytes(t) -> int:
@@ -87,7 +95,7 @@ class _Context:
     def sync(self, stream=None) -> None:
         """Waits for the stream and raises UrbError for a failure of the calls before."""
         with _Current(self.device):
-            N.check(getattr(N.moe_lib(), self._sync)(self._ctx, _stream_handle(stream)),
+            N.check(getattr(N.moe_lib(), self._sync)(self._ctx, _stream(stream, self.device)),
                     self._sync)
 
     def close(self) -> None:
@@ -149,13 +157,13 @@ class AdaptedProjection(_Context):
         source = N.SOURCE_HOST if _on_host(a) else N.SOURCE_DEVICE_COPY
         with _Current(self.device):
             N.check(N.moe_lib().urb_proj_set_adapter(self._ctx, slot, ctypes.byref(ad), source,
-                                                     _stream_handle(stream)),
+                                                     _stream(stream, self.device)),
                     "urb_proj_set_adapter")
 
     def clear_adapter(self, slot: int, stream=None) -> None:
         with _Current(self.device):
             N.check(N.moe_lib().urb_proj_set_adapter(self._ctx, slot, None, N.SOURCE_DEVICE_COPY,
-                                                     _stream_handle(stream)),
+                                                     _stream(stream, self.device)),
                     "urb_proj_set_adapter")
 
     def forward_into(self, x, y, adapter_ids=None, stream=None) -> None:
@@ -169,7 +177,7 @@ class AdaptedProjection(_Context):
         ids = _vector(adapter_ids, "adapter_ids", T, torch.int32, self.device)
         with _Current(self.device):
             N.check(N.moe_lib().urb_proj_forward(self._ctx, x.data_ptr(), xs, ids, T, y.data_ptr(),
-                                                 ys, _stream_handle(stream)), "urb_proj_forward")
+                                                 ys, _stream(stream, self.device)), "urb_proj_forward")
 
     def forward(self, x, adapter_ids=None):
         """x [T, cols] -> y [T, rows]; raises UrbError for ids that name no filled slot."""
@@ -185,44 +193,58 @@ class AdaptedProjection(_Context):
         return tuple(v.value for v in n)
 
 
+def _heads(t, name: str, shape, dtype, device: int):
+    if t.shape != shape or t.dtype is not dtype or t.get_device() != device:
+        raise ValueError(f"{name} must be a {dtype} {list(shape)} tensor on cuda:{device}")
+    token, head, value = t.stride()
+    if value != 1 and shape[2] > 1:
+        raise ValueError(f"{name}: the values of a head must be contiguous")
+    return token, head
+
+
 def qk_norm_rope(q, k, q_weight, k_weight, positions, inv_freq, eps: float,
                  zero_centered: bool = False, interleaved: bool = False, out=None, stream=None):
     """``urb_qk_norm_rope``: q [T, heads, D] and k [T, k_heads, D] (or None) normed per head by
     ``q_weight`` / ``k_weight`` [D] f32 and turned by ``positions`` [T] int64 times ``inv_freq``
     [rotary_dim / 2] f32.  Tokens and heads may be strided, as in a fused q/k/v row.  ``out``: the
     (q, k) tensors to write, which may be q and k themselves.  Stream-ordered."""
-    if q.dim() != 3 or (k is not None and (k.dim() != 3 or k.shape[0] != q.shape[0]
-                                           or k.shape[2] != q.shape[2])):
-        raise ValueError("q must be [T, heads, D] and k [T, k_heads, D]")
-    T, hq, D = q.shape
-    device = q.get_device()
-    if device < 0:
-        raise ValueError("q must be on a GPU")
-    hk = 0 if k is None else k.shape[1]
+    dtype, device, shape = q.dtype, q.get_device(), q.shape
+    if q.dim() != 3 or device < 0:
+        raise ValueError("q must be a [T, heads, D] tensor on a GPU")
+    T, hq, D = shape
+    hk = 0
+    if k is not None:
+        if k.dim() != 3:
+            raise ValueError("k must be [T, k_heads, D]")
+        hk = k.shape[1]
+    k_shape = (T, hk, D)
     if out is None:
-        out = (torch.empty((T, hq, D), dtype=q.dtype, device=q.device),
-               None if k is None else torch.empty((T, hk, D), dtype=q.dtype, device=q.device))
+        out = (torch.empty(shape, dtype=dtype, device=q.device),
+               None if k is None else torch.empty(k_shape, dtype=dtype, device=q.device))
     qo, ko = out
-    if qo.shape != q.shape or (k is not None and (ko is None or ko.shape != k.shape)):
-        raise ValueError("out must have the shapes of q and k")
-    used = [("q", q), ("q_out", qo)] + ([] if k is None else [("k", k), ("k_out", ko)])
-    for name, t in used:
-        if t.dtype != q.dtype or t.get_device() != device or (D > 1 and t.stride(2) != 1):
-            raise ValueError(f"{name}: heads must be contiguous, of q's type and device")
+    q_in, q_out = _heads(q, "q", shape, dtype, device), _heads(qo, "q_out", shape, dtype, device)
+    k_in = k_out = (0, 0)
+    k_at = ko_at = kw_at = None
+    if hk:
+        if ko is None:
+            raise ValueError("out must hold a tensor for k")
+        k_in = _heads(k, "k", k_shape, dtype, device)
+        k_out = _heads(ko, "k_out", k_shape, dtype, device)
+        k_at, ko_at = k.data_ptr(), ko.data_ptr()
+        kw_at = _vector(k_weight, "k_weight", D, torch.float32, device)
     half = 0 if inv_freq is None else inv_freq.numel()
-    strides = [s for t in (q, k, qo, ko) for s in ((0, 0) if t is None else t.stride()[:2])]
-    desc = N.QkDesc(_type(q.dtype), hq, hk, D, 2 * half, int(interleaved), int(zero_centered),
-                    float(eps), *strides)
-    args = (_vector(q_weight, "q_weight", D, torch.float32, device),
-            _vector(k_weight, "k_weight", D, torch.float32, device) if hk else None,
-            _vector(positions, "positions", T, torch.int64, device),
-            _vector(inv_freq, "inv_freq", half, torch.float32, device))
+    desc = N.QkDesc(_TYPES.get(dtype, 7), hq, hk, D, 2 * half, interleaved, zero_centered, eps,
+                    *q_in, *k_in, *q_out, *k_out)
     with _Current(device):
-        N.check(N.moe_lib().urb_qk_norm_rope(ctypes.byref(desc), q.data_ptr(),
-                                             k.data_ptr() if hk else None, *args, T,
-                                             qo.data_ptr(), ko.data_ptr() if hk else None,
-                                             _stream_handle(stream)), "urb_qk_norm_rope")
-    return qo, ko
+        st = N.moe_lib().urb_qk_norm_rope(
+            ctypes.byref(desc), q.data_ptr(), k_at,
+            _vector(q_weight, "q_weight", D, torch.float32, device), kw_at,
+            _vector(positions, "positions", T, torch.int64, device),
+            _vector(inv_freq, "inv_freq", half, torch.float32, device), T, qo.data_ptr(), ko_at,
+            _stream(stream, device))
+    if st:
+        raise N.UrbError(st, "urb_qk_norm_rope")
+    return out
 
 
 class Sampler(_Context):
@@ -252,7 +274,7 @@ class Sampler(_Context):
             N.check(N.moe_lib().urb_sample(
                 self._ctx, logits.data_ptr(), stride, T, ctypes.byref(params),
                 _vector(uniform, "uniform", T, f32, dev), _vector(ids, "ids", T, torch.int32, dev),
-                _vector(probs, "probs", T, f32, dev), _stream_handle(stream)), "urb_sample")
+                _vector(probs, "probs", T, f32, dev), _stream(stream, self.device)), "urb_sample")
 
     def sample(self, logits, uniform, **params):
         """-> (ids [T] int32, probs [T] f32); raises UrbError for parameters out of range."""
