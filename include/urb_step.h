@@ -143,7 +143,7 @@ urb_status urb_qk_norm_rope(const urb_qk_desc *desc, const void *q, const void *
  *      over the kept tokens of index <= i exceeds uniform times the sum over all kept ones.
  * tau = 0 takes the lowest index of the largest logit.  NaN logits count as -inf and are never
  * drawn; a row with nothing above -inf gives id -1 and probability 0.  With logits of +inf the draw is among those.
- * e is computed in f64 and enters the sums as the nearest multiple of 2^(L - 62), L = max(1,
+ * e is computed in f64 and enters the sums as the nearest multiple of 2^-min(51, 62 -
  * ceil(log2(vocab))): 2^-42 of the largest for 2^20 tokens, 2^-45 for 131072.  Sums of integers do
  * not depend on their order, so a result depends on nothing but the row and its parameters; tokens
  * below half of that unit are never drawn.

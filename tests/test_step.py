@@ -444,7 +444,7 @@ def test_rotation_wrapper_refuses():
 def _drawn(row, tau=1.0, k=0, p=1.0, min_p=0.0, u=0.5):
     """(id, probability) by the definition: e in f64, its sums in whole multiples of 2^-shift.  (In
     f64 a sum of many ones loses the small masses that decide a border between equal tokens.)"""
-    shift = 62 - max(1, math.ceil(math.log2(row.numel())))
+    shift = min(51, 62 - math.ceil(math.log2(row.numel())))
     row = row.cpu().double().numpy()
     at = np.flatnonzero(row > -np.inf)
     if not at.size:

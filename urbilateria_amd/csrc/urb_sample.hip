@@ -3,7 +3,7 @@
 // All three filters keep a beginning of one order (logit descending, index ascending), so a row's
 // kept tokens are those above a threshold logit plus the first few of those equal to it, and no row
 // is ever sorted.  Logits are compared as 32-bit keys in their order; masses e = exp((l - m) / tau) are
-// computed in f64 and summed as integers of 2^-shift (shift 42 to 61, by the vocabulary), so sums do not depend
+// computed in f64 and summed as integers of 2^-shift (shift 42 to 51, by the vocabulary), so sums do not depend
 // on their order and a row's result is the same whatever workgroups share it.
 #include "urb_device.hpp"
 #include "urb_step.hpp"
@@ -34,50 +34,59 @@ __device__ __forceinline__ float load_logit(const void* p, size_t i) {
   else return reinterpret_cast<const float*>(p)[i];
 }
 
-// exp(x) for x <= 0 in f64, 0 below 2^-63 (half of the finest unit that masses are summed in).
-// x = n ln 2 + r with |r| <= ln(2) / 2; the Taylor series to r^13 leaves out less than 5e-18.
-__device__ __forceinline__ double exp_down(double x) {
-  if (!(x > -43.7)) return 0.0;
-  const double n = rint(x * 1.4426950408889634074);
-  double r = fma(-n, 0x1.62e42fefa39efp-1, x);  // ln 2, high and low part
-  r = fma(-n, 0x1.abc9e3b39803fp-56, r);
-  double s = 1.0 / 6227020800.0;
-  s = fma(s, r, 1.0 / 479001600.0);
-  s = fma(s, r, 1.0 / 39916800.0);
-  s = fma(s, r, 1.0 / 3628800.0);
-  s = fma(s, r, 1.0 / 362880.0);
-  s = fma(s, r, 1.0 / 40320.0);
-  s = fma(s, r, 1.0 / 5040.0);
-  s = fma(s, r, 1.0 / 720.0);
+// exp(x) for x <= 0 in f64, 0 below 2^-52.  x = n ln 2 / 16 + r with |r| <= ln(2) / 32, 2^(n / 16) by a table
+// of sixteenth powers of two; the Taylor series to r^6 leaves out less than 5e-16.
+constexpr int kPowers = 16;
+__device__ const double kPower[kPowers] = {
+    1.0,                    1.0442737824274138403, 1.0905077326652576592, 1.1387886347566916537,
+    1.1892071150027210667,  1.2418578120734840486, 1.2968395546510096659, 1.3542555469368927283,
+    1.4142135623730950488,  1.4768261459394993114, 1.5422108254079408236, 1.6104903319492543082,
+    1.6817928305074290861,  1.7562521603732994831, 1.8340080864093424635, 1.9152065613971472939};
+// The table in LDS (a barrier follows before its first use).
+__device__ __forceinline__ void fill_powers(double* powers) {
+  if (threadIdx.x < kPowers) powers[threadIdx.x] = kPower[threadIdx.x];
+}
+__device__ __forceinline__ double exp_down(double x, const double* powers) {
+  if (!(x > -36.1)) return 0.0;
+  const double magic = 0x1.8p52;  // adding it leaves an integer in the low bits
+  const double t = fma(x, 23.083120654223414518, magic);  // 16 / ln 2
+  const int n = (int)__double_as_longlong(t);
+  const double d = t - magic;
+  double r = fma(-d, 0x1.62e42fefa39efp-5, x);  // ln 2 / 16, high and low part
+  r = fma(-d, 0x1.abc9e3b39803fp-60, r);
+  double s = 1.0 / 720.0;
   s = fma(s, r, 1.0 / 120.0);
   s = fma(s, r, 1.0 / 24.0);
   s = fma(s, r, 1.0 / 6.0);
   s = fma(s, r, 0.5);
   s = fma(s, r, 1.0);
-  s = fma(s, r, 1.0);
-  return ldexp(s, (int)n);
+  const double p = powers[n & (kPowers - 1)];
+  return ldexp(fma(s * r, p, p), n >> 4);
 }
 
-// e of a logit key, and e as an integer.
+// e of a logit, e as an integer, and the bin it falls into.
 struct Mass {
   double top, inv, scale;  // largest logit, 1 / temperature, 2^shift
-  uint32_t top_key;
-  float topf, bins;  // kBins / kBinRange / temperature
-  __device__ __forceinline__ Mass(uint32_t key, float tau, double scale_)
-      : top((double)key_value(key)), inv(1.0 / (double)tau), scale(scale_), top_key(key),
-        topf(key_value(key)), bins((kBins / kBinRange) / tau) {}
-  __device__ __forceinline__ double e(uint32_t key) const {
-    if (key == top_key) return 1.0;  // also where both are +inf
-    return exp_down(((double)key_value(key) - top) * inv);
+  float topf, bins;        // kBins / kBinRange / temperature
+  const double* powers;
+  __device__ __forceinline__ Mass(uint32_t key, float tau, double scale_, const double* powers_)
+      : top((double)key_value(key)), inv(1.0 / (double)tau), scale(scale_), topf(key_value(key)),
+        bins((kBins / kBinRange) / tau), powers(powers_) {}
+  __device__ __forceinline__ double e(float l) const {
+    if (l == topf) return 1.0;  // also where both are +inf
+    return exp_down(((double)l - top) * inv, powers);
   }
-  __device__ __forceinline__ u64 fixed(double e) const { return (u64)(e * scale + 0.5); }
-  // Bins of (m - l) / tau over [0, kBinRange), the last one open; the f32 steps keep the logits' order.
-  static constexpr int kBins = 2048;
-  static constexpr float kBinRange = 44.5f;  // beyond it masses are zero
-  __device__ __forceinline__ int bin(uint32_t key) const {
-    if (key == top_key) return 0;
-    const float z = (topf - key_value(key)) * bins;
-    return z < (float)(kBins - 1) ? (int)z : kBins - 1;
+  __device__ __forceinline__ double e(uint32_t key) const { return e(key_value(key)); }
+  // (scale <= 2^51: the sum's low bits are the integer)
+  __device__ __forceinline__ u64 fixed(double e) const {
+    return (u64)__double_as_longlong(fma(e, scale, 0x1p52)) & 0xfffffffffffffull;
+  }
+  // (m - l) / tau in bins of 36.25 / 4096; from the last one on masses are zero.  The f32 steps keep the
+  // logits' order; a NaN logit gives NaN.
+  static constexpr int kBins = 4096;
+  static constexpr float kBinRange = 36.25f;
+  __device__ __forceinline__ float place(float l) const {
+    return l == topf ? 0.0f : (topf - l) * bins;
   }
 };
 constexpr int kBins = Mass::kBins;
@@ -92,50 +101,72 @@ __device__ __forceinline__ u64 mass_wanted(float top_p, u64 total) {
 constexpr int kRowThreads = 1024;
 constexpr int kRowWaves = kRowThreads / 64;
 
-template <class T>
-__device__ __forceinline__ T wave_sum(T v) {
-  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+// Running sums and maxima over a wave's lanes by DPP moves (a shuffle goes through the LDS, some ten times
+// the latency).  All 64 lanes take part.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int moved(int v) {
+  return __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xf, false);
+}
+template <int CTRL, int ROWS>
+__device__ __forceinline__ u64 moved(u64 v) {
+  return (u64)(uint32_t)moved<CTRL, ROWS>((int)(uint32_t)v) |
+         (u64)(uint32_t)moved<CTRL, ROWS>((int)(v >> 32)) << 32;
+}
+template <class T, class F>
+__device__ __forceinline__ T wave_running(T v, F op) {
+  v = op(v, moved<0x111, 0xf>(v));  // row_shr 1, 2, 4, 8: rows of 16
+  v = op(v, moved<0x112, 0xf>(v));
+  v = op(v, moved<0x114, 0xf>(v));
+  v = op(v, moved<0x118, 0xf>(v));
+  v = op(v, moved<0x142, 0xa>(v));  // row 0's last into row 1, row 2's into row 3
+  v = op(v, moved<0x143, 0xc>(v));  // row 1's last into rows 2 and 3
   return v;
 }
-template <int WAVES = kRowWaves, class T>
-__device__ __forceinline__ T block_sum(T v, T* slots) {
-  v = wave_sum(v);
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) slots[threadIdx.x >> 6] = v;
-  __syncthreads();
-  T s = 0;
-  for (int w = 0; w < WAVES; ++w) s += slots[w];
-  return s;
+template <class T>
+__device__ __forceinline__ T wave_upto(T v) {
+  return wave_running(v, [](T a, T b) { return a + b; });
+}
+__device__ __forceinline__ int lane_of(int v, int lane) { return __builtin_amdgcn_readlane(v, lane); }
+__device__ __forceinline__ u64 lane_of(u64 v, int lane) {
+  return (u64)(uint32_t)lane_of((int)(uint32_t)v, lane) | (u64)(uint32_t)lane_of((int)(v >> 32), lane) << 32;
+}
+template <class T>
+__device__ __forceinline__ T wave_sum(T v) {
+  return lane_of(wave_upto(v), 63);
+}
+__device__ __forceinline__ u64 wave_max(u64 v) {
+  return lane_of(wave_running(v, [](u64 a, u64 b) { return a > b ? a : b; }), 63);
 }
 // Sum over the threads before this one; *total over all.
-template <int WAVES = kRowWaves, class T>
+template <class T>
 __device__ __forceinline__ T block_before(T v, T* slots, T* total) {
-  T inc = v;
   const int lane = threadIdx.x & 63;
-  for (int o = 1; o < 64; o <<= 1) {
-    const T up = __shfl_up(inc, o, 64);
-    if (lane >= o) inc += up;
-  }
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const T upto = wave_upto(v);
   __syncthreads();
-  if (lane == 63) slots[threadIdx.x >> 6] = inc;
+  if (lane == 63) slots[wave] = upto;
   __syncthreads();
-  T before = 0, all = 0;
-  for (int w = 0; w < WAVES; ++w) {
-    if (w < (int)(threadIdx.x >> 6)) before += slots[w];
-    all += slots[w];
-  }
-  *total = all;
-  return before + inc - v;
+  const T all = wave_upto(lane < kRowWaves ? slots[lane] : T(0));
+  *total = lane_of(all, kRowWaves - 1);
+  return (wave ? lane_of(all, wave - 1) : T(0)) + upto - v;
+}
+template <class T>
+__device__ __forceinline__ T block_sum(T v, T* slots) {
+  T total;
+  block_before(v, slots, &total);
+  return total;
 }
 
-// The bin where the running sum of `hist` from the highest bin down reaches `want` (1 <= want <= the
+constexpr int kDigits = 2048;  // of a radix pass
+
+// The digit where the running sum of `hist` from the highest bin down reaches `want` (1 <= want <= the
 // sum of all), and the sum above it.  All threads get both.
 __device__ void find_bin(const u64* hist, u64 want, u64* slots, int* bin, u64* above) {
   __shared__ int s_bin;
   __shared__ u64 s_above;
-  constexpr int PER = kBins / kRowThreads;
+  constexpr int PER = kDigits / kRowThreads;
   u64 mine[PER], sum = 0;
-  const int first = kBins - 1 - (int)threadIdx.x * PER;  // highest bins first
+  const int first = kDigits - 1 - (int)threadIdx.x * PER;  // highest bins first
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
     mine[i] = hist[first - i];
@@ -177,7 +208,7 @@ __device__ __forceinline__ RowParams row_params(const SampleArgs& a, int row) {
 // ---- a row in one workgroup, whatever it holds: the thresholds by radix selection over the keys ----
 
 struct RowLds {
-  u64 hist[kBins];
+  u64 hist[kDigits];
   u64 slots[kRowWaves];
   int islots[kRowWaves];
   int found;
@@ -201,7 +232,7 @@ __device__ __noinline__ int draw_by_radix(const uint8_t* base, int V, const RowP
     for (int level = 0; level < 3; ++level) {
       const int low = level == 0 ? 21 : level == 1 ? 10 : 0;   // digits of 11, 11 and 10 bits
       const int bits = level == 2 ? 10 : 11;
-      for (int b = tid; b < kBins; b += kRowThreads) hist[b] = 0;
+      for (int b = tid; b < kDigits; b += kRowThreads) hist[b] = 0;
       __syncthreads();
       for (int i = tid; i < V; i += kRowThreads) {
         const uint32_t k = key(i);
@@ -313,18 +344,18 @@ __device__ __noinline__ int draw_by_radix(const uint8_t* base, int V, const RowP
 
 // ---- rows shared by many workgroups ----
 //
-// Four launches: the largest logit of every chunk; a histogram of the row in bins of (m - l) / tau,
-// whose last workgroup finds the bin in which the kept tokens end; the sums of the chunks' tokens
-// before that bin, and a list of the tokens in it; and one workgroup per row that orders the list,
-// finds the last kept token, the chunk of the draw and the token in it.  A list too long for LDS
-// (many equal logits) sends its row to draw_by_radix.
+// Four launches: the largest logit of every part; a histogram of the row in bins of (m - l) / tau; the
+// sums of the chunks' tokens before the bin in which the kept tokens end, and a list of the tokens in
+// it; and one workgroup per row that orders the list, finds the last kept token, the chunk of the draw
+// and the token in it.  A list too long for LDS (many equal logits) sends its row to draw_by_radix.
+// (With the bin found by the histogram's last workgroup, behind a device-scope fence in each, that launch
+// took 66 us for 256 rows, 53 of them without any sums: the fences write back and drop the L2s.)
 //
-// Where the kept tokens are few, the list holds all of them and no sums are needed.  The row is read up
-// to three times, after the first time from the Infinity Cache where a batch's logits fit it.
+// The row is read up to three times, after the first time from the Infinity Cache where a batch's logits fit it.
 
-constexpr int kList = 2048;       // tokens that the last launch orders in LDS
-constexpr int kChunkUnit = 2048;  // values per chunk and 256 threads: eight per thread
-constexpr int kThreads = 256;
+constexpr int kList = 1024;                 // tokens that the last launch orders, one per thread
+constexpr int kChunk = 8 * kRowThreads;     // values per chunk: eight per thread
+constexpr int kMaxChunks = (1 << 20) / kChunk + 1;
 
 enum RowMode {
   kNoCut = 1,     // no top_k, no top_p: everything (that min_p leaves)
@@ -335,21 +366,23 @@ enum RowMode {
 
 struct RowRecord {
   int mode, bin;
-  int listed;     // tokens in the list
-  int arrived;    // workgroups of the histogram that are through
+  int few;        // kBinListed: the tokens up to the cut's bin fit a list too
   int above_n;    // tokens before the cut's bin
-  int pad;
   u64 above, want;  // their mass; the mass that top_p asks for
 };
 
+constexpr int kGroup = 64, kAllBins = kBins + kBins / kGroup;
+
 struct Work {
-  int chunks, chunk;  // of every row; values per chunk
-  u64* best;          // [rows][chunks] largest key << 32 | ~lowest index
+  int chunks;            // of a row
+  int parts, bin_parts;  // workgroups that share a row's chunks; those of the histogram
+  u64* best;          // [rows][parts] largest key << 32 | ~lowest index
   u64* sums;          // [rows][chunks]
-  u64* mass;          // [rows][kBins]
-  int* count;         // [rows][kBins]
+  u64* mass;          // [rows][kAllBins]: the bins, then groups of kGroup of them
+  int* count;         // [rows][kAllBins]
   u64* list;          // [rows][kList] key << 32 | ~index
   RowRecord* record;  // [rows]
+  int* listed;        // [rows] tokens in the list
 };
 
 template <bool BF16>
@@ -360,9 +393,9 @@ struct Row {
       : base(reinterpret_cast<const uint8_t*>(a.logits) +
              (size_t)row * a.row_stride * (BF16 ? 2 : 4)),
         V(a.vocab), lead((int)(reinterpret_cast<uintptr_t>(base) % 16) / (BF16 ? 2 : 4)) {}
-  // Keys of the eight values at place v (from the boundary; v % 8 == 0), 0 outside the row; returns
-  // the index of the first.
-  __device__ __forceinline__ int keys(int v, uint32_t (&k)[8]) const {
+  // The eight values at place v (from the boundary; v % 8 == 0), -inf outside the row; returns the
+  // index of the first.
+  __device__ __forceinline__ int values(int v, float (&l)[8]) const {
     const int i = v - lead;
     if (i >= 0 && i + 8 <= V) {
       if constexpr (BF16) {
@@ -370,75 +403,81 @@ struct Row {
         const uint32_t w[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
-          k[2 * u] = key_of(bf16_lo(w[u]));
-          k[2 * u + 1] = key_of(bf16_hi(w[u]));
+          l[2 * u] = bf16_lo(w[u]);
+          l[2 * u + 1] = bf16_hi(w[u]);
         }
       } else {
         const float4 q = u2f4(ldg16(base + 4 * (size_t)i)), r = u2f4(ldg16(base + 4 * (size_t)i + 16));
-        k[0] = key_of(q.x); k[1] = key_of(q.y); k[2] = key_of(q.z); k[3] = key_of(q.w);
-        k[4] = key_of(r.x); k[5] = key_of(r.y); k[6] = key_of(r.z); k[7] = key_of(r.w);
+        l[0] = q.x; l[1] = q.y; l[2] = q.z; l[3] = q.w;
+        l[4] = r.x; l[5] = r.y; l[6] = r.z; l[7] = r.w;
       }
     } else {
 #pragma unroll
       for (int u = 0; u < 8; ++u)
-        k[u] = i + u >= 0 && i + u < V ? key_of(load_logit<BF16>(base, i + u)) : 0;
+        l[u] = i + u >= 0 && i + u < V ? load_logit<BF16>(base, i + u) : -__builtin_inff();
     }
     return i;
   }
 };
 
-__device__ __forceinline__ u64 wave_max(u64 v) {
-  for (int o = 32; o > 0; o >>= 1) {
-    const u64 c = __shfl_xor(v, o, 64);
-    v = c > v ? c : v;
-  }
-  return v;
+// A logit and its index as one number: larger logits first, then lower indexes.
+__device__ __forceinline__ u64 order_of(float l, int i) {
+  return ((u64)key_of(l) << 32) | (0xffffffffu - (uint32_t)i);
 }
-template <int WAVES>
+__device__ __forceinline__ int index_of(u64 order) { return (int)(0xffffffffu - (uint32_t)order); }
+__device__ __forceinline__ uint32_t key_in(u64 order) { return (uint32_t)(order >> 32); }
+
 __device__ __forceinline__ u64 block_max(u64 v, u64* slots) {
   v = wave_max(v);
   __syncthreads();
   if ((threadIdx.x & 63) == 0) slots[threadIdx.x >> 6] = v;
   __syncthreads();
 #pragma unroll
-  for (int w = 0; w < WAVES; ++w) v = slots[w] > v ? slots[w] : v;
+  for (int w = 0; w < kRowWaves; ++w) v = slots[w] > v ? slots[w] : v;
   return v;
 }
 
-// Largest key of each chunk; clears what the next launches add to.
+// The chunks of a part: [first, last).
+struct Part {
+  int first, last;
+  __device__ __forceinline__ Part(const Work& w, int part, int parts)
+      : first(w.chunks * part / parts), last(w.chunks * (part + 1) / parts) {}
+};
+
+// Largest key of each part; clears what the next launches add to.
 template <bool BF16>
-__global__ __launch_bounds__(kThreads) void sample_best_kernel(SampleArgs a, Work w) {
-  __shared__ u64 slots[kThreads / 64];
-  const int row = blockIdx.y, c = blockIdx.x;
+__global__ __launch_bounds__(kRowThreads, 8) void sample_best_kernel(SampleArgs a, Work w) {
+  __shared__ u64 slots[kRowWaves];
+  const int row = blockIdx.y, tid = threadIdx.x;
   const Row<BF16> r(a, row);
+  const Part part(w, blockIdx.x, w.parts);
   u64 best = 0;
-  for (int j = 0; j < w.chunk; j += kChunkUnit) {
-    uint32_t k[8];
-    const int i = r.keys(c * w.chunk + j + 8 * threadIdx.x, k);
+  for (int c = part.first; c < part.last; ++c) {
+    float l[8];
+    const int i = r.values(c * kChunk + 8 * tid, l);
 #pragma unroll
     for (int u = 0; u < 8; ++u) {
-      const u64 v = ((u64)k[u] << 32) | (0xffffffffu - (uint32_t)(i + u));
+      const u64 v = order_of(l[u], i + u);
       best = v > best ? v : best;
     }
   }
-  best = block_max<kThreads / 64>(best, slots);
-  if (threadIdx.x == 0) w.best[(size_t)row * w.chunks + c] = best;
-  for (int b = c * kThreads + threadIdx.x; b < kBins; b += w.chunks * kThreads) {
-    w.mass[(size_t)row * kBins + b] = 0;
-    w.count[(size_t)row * kBins + b] = 0;
+  best = block_max(best, slots);
+  if (tid == 0) w.best[(size_t)row * w.parts + blockIdx.x] = best;
+  for (int b = blockIdx.x * kRowThreads + tid; b < kAllBins; b += w.parts * kRowThreads) {
+    w.mass[(size_t)row * kAllBins + b] = 0;
+    w.count[(size_t)row * kAllBins + b] = 0;
   }
-  if (c == 0 && threadIdx.x == 0) w.record[row] = RowRecord{};
+  if (blockIdx.x == 0 && tid == 0) w.listed[row] = 0;
 }
 
 // The row's largest key and its lowest index.
-template <int WAVES>
-__device__ __forceinline__ u64 row_best(const Work& w, int row, u64* slots) {
+__device__ __forceinline__ u64 row_best(const Work& w, int row) {
   u64 best = 0;
-  for (int c = threadIdx.x; c < w.chunks; c += 64 * WAVES) {
-    const u64 v = w.best[(size_t)row * w.chunks + c];
+  for (int c = threadIdx.x & 63; c < w.parts; c += 64) {
+    const u64 v = w.best[(size_t)row * w.parts + c];
     best = v > best ? v : best;
   }
-  return block_max<WAVES>(best, slots);
+  return wave_max(best);
 }
 
 // A row that needs no sums at all: parameters out of range, nothing to draw, or the largest asked for.
@@ -446,161 +485,205 @@ __device__ __forceinline__ bool trivial(const RowParams& p, u64 best) {
   return !p.ok || (uint32_t)(best >> 32) <= kMinusInf || p.tau == 0.0f;
 }
 
-// The row's histogram, and by its last workgroup the bin where the kept tokens end.
+// The row's histogram, of counts and, for top_p alone, of masses.
 template <bool BF16>
-__global__ __launch_bounds__(kThreads) void sample_bins_kernel(SampleArgs a, Work w, double scale) {
+__global__ __launch_bounds__(kRowThreads, 8) void sample_bins_kernel(SampleArgs a, Work w,
+                                                                     double scale) {
   __shared__ u64 mass_lds[kBins];
   __shared__ int count_lds[kBins];
-  __shared__ u64 slots[kThreads / 64];
-  __shared__ int last;
+  __shared__ double powers[kPowers];
   const int row = blockIdx.y, tid = threadIdx.x;
   const RowParams p = row_params(a, row);
-  const u64 best = row_best<kThreads / 64>(w, row, slots);
-  const bool by_count = p.top_k > 0 && p.top_k < a.vocab, by_mass = p.top_p < 1.0f;
-  if (trivial(p, best)) return;
-  RowRecord& rec = w.record[row];
-  if (!by_count && !by_mass) {
-    if (blockIdx.x == 0 && tid == 0) rec.mode = kNoCut;
-    return;
-  }
+  const u64 best = row_best(w, row);
+  const bool by_count = p.top_k > 0 && p.top_k < a.vocab;
+  if (trivial(p, best) || !(by_count || p.top_p < 1.0f)) return;
   const Row<BF16> r(a, row);
-  const Mass m((uint32_t)(best >> 32), p.tau, scale);
-  for (int b = tid; b < kBins; b += kThreads) {
+  const Mass m(key_in(best), p.tau, scale, powers);
+  const Part part(w, blockIdx.x, w.bin_parts);
+  float next[8];
+  r.values(part.first * kChunk + 8 * tid, next);
+  fill_powers(powers);
+  for (int b = tid; b < kBins; b += kRowThreads) {
     mass_lds[b] = 0;
     count_lds[b] = 0;
   }
   __syncthreads();
-  for (int j = 0; j < w.chunk; j += kChunkUnit) {
-    uint32_t k[8];
-    r.keys(blockIdx.x * w.chunk + j + 8 * tid, k);
+  for (int c = part.first; c < part.last; ++c) {
+    float l[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) l[u] = next[u];
+    if (c + 1 < part.last) r.values((c + 1) * kChunk + 8 * tid, next);
 #pragma unroll
     for (int u = 0; u < 8; ++u) {
-      if (k[u] <= kMinusInf) continue;
-      const int b = m.bin(k[u]);
-      atomicAdd(&count_lds[b], 1);
-      if (!by_count) {
-        const u64 f = m.fixed(m.e(k[u]));
-        if (f) atomicAdd(&mass_lds[b], f);
-      }
+      // (logits without mass count for nothing: top_k ends before them or does not matter)
+      const float z = m.place(l[u]);
+      if (!(z < (float)(kBins - 1))) continue;
+      atomicAdd(&count_lds[(int)z], 1);
+      if (!by_count) atomicAdd(&mass_lds[(int)z], m.fixed(m.e(l[u])));
     }
   }
   __syncthreads();
-  u64* const mass = w.mass + (size_t)row * kBins;
-  int* const count = w.count + (size_t)row * kBins;
-  for (int b = tid; b < kBins; b += kThreads) {
-    if (count_lds[b]) atomicAdd(&count[b], count_lds[b]);
-    if (mass_lds[b]) atomicAdd(&mass[b], mass_lds[b]);
-  }
-  __syncthreads();
-  if (tid == 0)
-    last = __hip_atomic_fetch_add(&rec.arrived, 1, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) ==
-           w.chunks - 1;
-  __syncthreads();
-  if (!last) return;
-
-  // 8 bins per thread, in order
-  constexpr int PER = kBins / kThreads;
-  int n[PER], n_sum = 0;
-  u64 f[PER], f_sum = 0;
-#pragma unroll
-  for (int i = 0; i < PER; ++i) {
-    n[i] = __hip_atomic_load(&count[tid * PER + i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    f[i] = by_count ? 0
-                    : __hip_atomic_load(&mass[tid * PER + i], __ATOMIC_RELAXED,
-                                        __HIP_MEMORY_SCOPE_AGENT);
-    n_sum += n[i];
-    f_sum += f[i];
-  }
-  __shared__ int n_slots[kThreads / 64];
-  int n_all;
-  u64 f_all;
-  int n_run = block_before<kThreads / 64>(n_sum, n_slots, &n_all);
-  u64 f_run = block_before<kThreads / 64>(f_sum, slots, &f_all);
-  const u64 want = by_count ? 0 : mass_wanted(p.top_p, f_all);
-  const int k = min(p.top_k, n_all);
-#pragma unroll
-  for (int i = 0; i < PER; ++i) {
-    const bool here = by_count ? n_run < k && n_run + n[i] >= k : f_run < want && f_run + f[i] >= want;
-    if (here) {
-      rec.bin = tid * PER + i;
-      rec.above_n = n_run;
-      rec.above = f_run;
-      rec.want = want;
-      rec.mode = n_run + n[i] <= kList                        ? kAllListed
-                 : n[i] <= kList && !(by_count && by_mass) ? kBinListed
-                                                              : kByRadix;
+  u64* const mass = w.mass + (size_t)row * kAllBins;
+  int* const count = w.count + (size_t)row * kAllBins;
+  for (int b = tid; b < kBins; b += kRowThreads) {
+    int n = count_lds[b];
+    u64 f = mass_lds[b];
+    if (n) atomicAdd(&count[b], n);
+    if (f) atomicAdd(&mass[b], f);
+    // a wave holds a group
+    n = wave_sum(n);
+    f = wave_sum(f);
+    if (b % kGroup == 0) {
+      if (n) atomicAdd(&count[kBins + b / kGroup], n);
+      if (f) atomicAdd(&mass[kBins + b / kGroup], f);
     }
-    n_run += n[i];
-    f_run += f[i];
   }
 }
 
-// The chunks' sums over the tokens before the cut's bin, and the list.
+// Where the row's kept tokens end, by the histogram: every wave for itself.
+__device__ __forceinline__ RowRecord find_cut(const Work& w, int row, const RowParams& p, int V) {
+  static_assert(kBins == kGroup * 64 && kGroup == 64, "a lane per group, then one per bin");
+  RowRecord rec{};
+  const bool by_count = p.top_k > 0 && p.top_k < V, by_mass = p.top_p < 1.0f;
+  if (!by_count && !by_mass) {
+    rec.mode = kNoCut;
+    return rec;
+  }
+  const int lane = threadIdx.x & 63;
+  const u64* const mass = w.mass + (size_t)row * kAllBins;
+  const int* const count = w.count + (size_t)row * kAllBins;
+  int n = count[kBins + lane];
+  u64 f = mass[kBins + lane];
+  int n_upto = wave_upto(n);
+  u64 f_upto = wave_upto(f);
+  const int k = min(p.top_k, lane_of(n_upto, 63));
+  rec.want = by_count ? 0 : mass_wanted(p.top_p, lane_of(f_upto, 63));
+  // the first lane whose sums reach what is asked for, and the sums before it
+  auto cross = [&] {
+    const bool reached = by_count ? rec.above_n + n_upto >= k : rec.above + f_upto >= rec.want;
+    const int at = __ffsll(__ballot(reached)) - 1;
+    rec.above_n += lane_of(n_upto - n, at);
+    rec.above += lane_of(f_upto - f, at);
+    return at;
+  };
+  const int group = cross();
+  n = count[group * kGroup + lane];
+  f = mass[group * kGroup + lane];
+  n_upto = wave_upto(n);
+  f_upto = wave_upto(f);
+  const int at = cross();
+  rec.bin = group * kGroup + at;
+  const int here = lane_of(n, at);
+  rec.few = rec.above_n + here <= kList;
+  // (top_p of top_k's tokens needs all of them in order)
+  if (by_count && by_mass) rec.mode = rec.few ? kAllListed : kByRadix;
+  else rec.mode = here <= kList ? kBinListed : kByRadix;
+  return rec;
+}
+
+// The chunks' sums over the tokens before the cut's bin, and the list.  Each workgroup gathers both in
+// LDS and adds its part of the list with one atomic, so its chunks follow one another without barriers.
+// Where the tokens up to the cut are few, they are gathered first and their masses computed from there:
+// inside the loop any one of them costs its whole wave an exponential.
 template <bool BF16>
-__global__ __launch_bounds__(kThreads) void sample_list_kernel(SampleArgs a, Work w, double scale) {
-  __shared__ u64 slots[kThreads / 64];
+__global__ __launch_bounds__(kRowThreads, 8) void sample_list_kernel(SampleArgs a, Work w,
+                                                                     double scale) {
+  __shared__ u64 list[kList];
+  __shared__ u64 sums[kMaxChunks];
+  __shared__ int s_n, s_at;
+  __shared__ double powers[kPowers];
   const int row = blockIdx.y, tid = threadIdx.x, lane = tid & 63;
-  RowRecord& rec = w.record[row];
-  const int mode = rec.mode, cut = rec.bin;
-  if (mode == 0 || mode == kByRadix) return;
   const RowParams p = row_params(a, row);
-  const Mass m((uint32_t)(row_best<kThreads / 64>(w, row, slots) >> 32), p.tau, scale);
+  const u64 best = row_best(w, row);
+  if (trivial(p, best)) return;
   const Row<BF16> r(a, row);
+  const Part part(w, blockIdx.x, w.parts);
+  float next[8];
+  int at_next = r.values(part.first * kChunk + 8 * tid, next);
+  const RowRecord rec = find_cut(w, row, p, a.vocab);
+  if (blockIdx.x == 0 && tid == 0) w.record[row] = rec;
+  if (rec.mode == kByRadix) return;
+  const Mass m(key_in(best), p.tau, scale, powers);
   const double min_e = (double)p.min_p;
-  u64 sum = 0;
-  for (int j = 0; j < w.chunk; j += kChunkUnit) {
-    uint32_t k[8];
-    const int i = r.keys(blockIdx.x * w.chunk + j + 8 * tid, k);
+  fill_powers(powers);
+  if (tid < part.last - part.first) sums[tid] = 0;
+  if (tid == 0) s_n = 0;
+  __syncthreads();
+  // places below `sum_to` are summed in the loop, those from there to below `list_to` listed
+  const bool dense = rec.mode == kAllListed || rec.few;
+  const float sum_to = rec.mode == kNoCut ? (float)(kBins - 1) : dense ? 0.0f : (float)rec.bin;
+  const float list_to = rec.mode == kNoCut ? 0.0f : (float)(rec.bin + 1);
+  for (int c = part.first; c < part.last; ++c) {
+    float l[8];
+    const int i = at_next;
+#pragma unroll
+    for (int u = 0; u < 8; ++u) l[u] = next[u];
+    if (c + 1 < part.last) at_next = r.values((c + 1) * kChunk + 8 * tid, next);
+    u64 sum = 0;
 #pragma unroll
     for (int u = 0; u < 8; ++u) {
-      const bool valid = k[u] > kMinusInf;
-      const int b = m.bin(k[u]);
-      if (valid && (mode == kNoCut || (mode == kBinListed && b < cut))) {
-        const double e = m.e(k[u]);
+      const float z = m.place(l[u]);
+      if (z < sum_to) {
+        const double e = m.e(l[u]);
         if (e >= min_e) sum += m.fixed(e);
-      }
-      const bool listed = valid && (mode == kBinListed ? b == cut : mode == kAllListed && b <= cut);
-      const u64 vote = __ballot(listed);
-      if (vote) {
-        int at = 0;
-        if (lane == 0) at = atomicAdd(&rec.listed, __popcll(vote));
-        at = __shfl(at, 0, 64) + __popcll(vote & ((1ull << lane) - 1));
-        if (listed && at < kList)  // (at most kList: the histogram counted them)
-          w.list[(size_t)row * kList + at] = ((u64)k[u] << 32) | (0xffffffffu - (uint32_t)(i + u));
+      } else if (z < list_to) {
+        const int at = atomicAdd(&s_n, 1);
+        if (at < kList) list[at] = order_of(l[u], i + u);  // (it is: the histogram counted them)
       }
     }
-  }
-  if (mode != kAllListed) {
-    sum = wave_sum(sum);
-    __syncthreads();
-    if (lane == 0) slots[tid >> 6] = sum;
-    __syncthreads();
-    if (tid == 0) {
-      for (int v = 1; v < kThreads / 64; ++v) sum += slots[v];
-      w.sums[(size_t)row * w.chunks + blockIdx.x] = sum;
+    if (!dense) {
+      sum = wave_sum(sum);
+      if (lane == 0 && sum) atomicAdd(&sums[c - part.first], sum);
     }
   }
+  __syncthreads();
+  const int n = min(s_n, kList);
+  const u64 mine = tid < n ? list[tid] : 0;
+  bool listed = tid < n;
+  if (rec.mode == kBinListed && rec.few) {
+    if (listed && m.place(key_value(key_in(mine))) < (float)rec.bin) {
+      listed = false;
+      const double e = m.e(key_in(mine));
+      if (e >= min_e) atomicAdd(&sums[(index_of(mine) + r.lead) / kChunk - part.first], m.fixed(e));
+    }
+    __syncthreads();
+    if (tid == 0) s_n = 0;
+    __syncthreads();
+    int at = 0;
+    if (listed) at = atomicAdd(&s_n, 1);
+    __syncthreads();
+    if (listed) list[at] = mine;
+    __syncthreads();
+  }
+  const int out = min(s_n, kList);
+  if (tid == 0 && out) s_at = atomicAdd(&w.listed[row], out);
+  __syncthreads();
+  if (tid < out && s_at + tid < kList) w.list[(size_t)row * kList + s_at + tid] = list[tid];
+  if (rec.mode != kAllListed && tid < part.last - part.first)
+    w.sums[(size_t)row * w.chunks + part.first + tid] = sums[tid];
 }
 
-// Sorts the first n values of v (padded with zeros to a power of two of at least 64 within kList):
-// descending.
-__device__ void sort_descending(u64* v, int n) {
+// Sorts the block's values, one per thread, the first n of them not zero: descending by thread.
+// A bitonic network whose exchanges within a wave are shuffles.
+__device__ __forceinline__ u64 sort_descending(u64 v, int n, u64* lds) {
+  const int tid = threadIdx.x;
   int size = 64;
   while (size < n) size *= 2;
-  for (int i = n + threadIdx.x; i < size; i += kRowThreads) v[i] = 0;
   for (int width = 2; width <= size; width *= 2)
     for (int gap = width / 2; gap > 0; gap /= 2) {
-      __syncthreads();
-      for (int t = threadIdx.x; t < size / 2; t += kRowThreads) {
-        const int i = 2 * t - (t & (gap - 1)), j = i + gap;
-        const u64 x = v[i], y = v[j];
-        if ((x < y) == ((i & width) == 0)) {
-          v[i] = y;
-          v[j] = x;
-        }
+      u64 o;
+      if (gap >= 64) {
+        __syncthreads();
+        lds[tid] = v;
+        __syncthreads();
+        o = lds[tid ^ gap];
+      } else {
+        o = __shfl_xor(v, gap, 64);
       }
+      const bool larger = ((tid & gap) == 0) == ((tid & width) == 0);
+      v = (o > v) == larger ? o : v;
     }
-  __syncthreads();
+  return v;
 }
 
 // One workgroup per row: the last kept token of the list, then the draw.  SMALL: a vocabulary that fits
@@ -618,6 +701,9 @@ __global__ __launch_bounds__(kRowThreads) void sample_draw_kernel(SampleArgs a, 
   } lds;
   __shared__ int s_n, s_found;
   __shared__ u64 s_cut, s_before;
+  __shared__ double powers[kPowers];
+  fill_powers(powers);
+  __syncthreads();
   const int row = blockIdx.x, tid = threadIdx.x;
   const RowParams p = row_params(a, row);
   const Row<BF16> r(a, row);
@@ -626,19 +712,15 @@ __global__ __launch_bounds__(kRowThreads) void sample_draw_kernel(SampleArgs a, 
   if constexpr (SMALL) {
     if (tid == 0) s_n = 0;
     __syncthreads();
-    uint32_t k[8];
-    const int i = r.keys(8 * tid, k);   // (a row of kList values starts at most 7 past a boundary)
-#pragma unroll
-    for (int u = 0; u < 8; ++u)
-      if (k[u] > kMinusInf) {
-        const u64 v = ((u64)k[u] << 32) | (0xffffffffu - (uint32_t)(i + u));
-        best = v > best ? v : best;
-        lds.s.list[atomicAdd(&s_n, 1)] = v;
-      }
-    best = block_max<kRowWaves>(best, lds.s.slots);
+    const u64 v = tid < r.V ? order_of(load_logit<BF16>(r.base, tid), tid) : 0;
+    if (key_in(v) > kMinusInf) {
+      best = v;
+      lds.s.list[atomicAdd(&s_n, 1)] = best;
+    }
+    best = block_max(best, lds.s.slots);
     n = s_n;
   } else {
-    best = row_best<kRowWaves>(w, row, lds.s.slots);
+    best = row_best(w, row);
   }
   auto done = [&](int id, float prob) {
     if (tid == 0) {
@@ -649,10 +731,10 @@ __global__ __launch_bounds__(kRowThreads) void sample_draw_kernel(SampleArgs a, 
   if (trivial(p, best)) {
     if (!p.ok && tid == 0) flag(a.status, kStepArgument);
     const bool greedy = p.ok && (uint32_t)(best >> 32) > kMinusInf;
-    done(greedy ? (int)(0xffffffffu - (uint32_t)best) : -1, greedy ? 1.0f : 0.0f);
+    done(greedy ? index_of(best) : -1, greedy ? 1.0f : 0.0f);
     return;
   }
-  const Mass m((uint32_t)(best >> 32), p.tau, scale);
+  const Mass m(key_in(best), p.tau, scale, powers);
   const double min_e = (double)p.min_p, uniform = (double)p.uniform;
   auto prob_of = [&](uint32_t key, u64 total) {
     return (float)(m.e(key) / ((double)total / scale));
@@ -661,7 +743,7 @@ __global__ __launch_bounds__(kRowThreads) void sample_draw_kernel(SampleArgs a, 
   if constexpr (!SMALL) {
     rec = w.record[row];
     mode = rec.mode;
-    n = min(rec.listed, kList);
+    n = min(w.listed[row], kList);
     if (mode == kByRadix) {
       u64 total;
       __syncthreads();
@@ -669,149 +751,107 @@ __global__ __launch_bounds__(kRowThreads) void sample_draw_kernel(SampleArgs a, 
       done(id, prob_of(key_of(load_logit<BF16>(r.base, id)), total));
       return;
     }
-    for (int i = tid; i < n; i += kRowThreads) lds.s.list[i] = w.list[(size_t)row * kList + i];
+    if (tid < n) lds.s.list[tid] = w.list[(size_t)row * kList + tid];
   }
+  u64 mine = tid < n ? lds.s.list[tid] : 0;  // (its own store, or SMALL's before the barriers)
   // the list's kept tokens are its first `kept` in order
   int kept = 0;
   u64 kept_mass = 0;
   if (mode != kNoCut) {
-    sort_descending(lds.s.list, n);
+    mine = sort_descending(mine, n, lds.s.list);
     const bool by_count = p.top_k > 0 && p.top_k < r.V;
     // (with every kept token in the list nothing comes before it)
-    const int above_n = mode == kBinListed ? rec.above_n : 0;
-    const int most = by_count ? min(n, p.top_k - above_n) : n;
-    u64 f[2], mine = 0;
-    double e[2];
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      const int i = 2 * tid + u;
-      e[u] = i < most ? m.e((uint32_t)(lds.s.list[i] >> 32)) : 0.0;
-      f[u] = i < most ? m.fixed(e[u]) : 0;
-      mine += f[u];
-    }
+    const bool part = mode == kBinListed;
+    const int most = by_count ? min(n, p.top_k - (part ? rec.above_n : 0)) : n;
+    const double e = tid < most ? m.e(key_in(mine)) : 0.0;
+    const u64 f = tid < most ? m.fixed(e) : 0;
     u64 all;
-    u64 run = (mode == kBinListed ? rec.above : 0) + block_before<kRowWaves>(mine, lds.s.slots, &all);
+    const u64 run = (part ? rec.above : 0) + block_before(f, lds.s.slots, &all);
     u64 want = ~0ull;
-    if (p.top_p < 1.0f) want = by_count || SMALL ? mass_wanted(p.top_p, all) : rec.want;
-    int mine_n = 0;
-    u64 mine_f = 0;
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      // (with equal logits e >= min_p holds for all or none, so the kept ones stay a beginning)
-      if (2 * tid + u < most && run < want && e[u] >= min_e) {
-        ++mine_n;
-        mine_f += f[u];
-      }
-      run += f[u];
-    }
-    kept = block_sum<kRowWaves>(mine_n, lds.s.islots);
-    kept_mass = block_sum<kRowWaves>(mine_f, lds.s.slots);
+    if (p.top_p < 1.0f) want = SMALL || by_count ? mass_wanted(p.top_p, all) : rec.want;
+    // (with equal logits e >= min_p holds for all or none, so the kept ones stay a beginning)
+    const bool keep = tid < most && run < want && e >= min_e;
+    kept = __syncthreads_count(keep);
+    kept_mass = block_sum(keep ? f : 0, lds.s.slots);
   }
   if (mode == kAllListed) {
     // the draw among the kept tokens by index: sorted by it, the key in the low half
     const double target = uniform * (double)kept_mass;
-    for (int i = tid; i < kept; i += kRowThreads) {
-      const u64 v = lds.s.list[i];
-      lds.s.list[i] = (v << 32) | (v >> 32);   // ~index descending
-    }
-    sort_descending(lds.s.list, kept);
-    u64 f[2];
-    uint32_t key[2];
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      const int i = 2 * tid + u;
-      key[u] = i < kept ? (uint32_t)lds.s.list[i] : 0;
-      f[u] = i < kept ? m.fixed(m.e(key[u])) : 0;
-    }
+    mine = sort_descending(tid < kept ? (mine << 32) | (mine >> 32) : 0, kept, lds.s.list);
+    const uint32_t key = (uint32_t)mine;
+    const u64 f = tid < kept ? m.fixed(m.e(key)) : 0;
     u64 all;
-    u64 run = block_before<kRowWaves>(f[0] + f[1], lds.s.slots, &all);
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      if (!((double)run > target) && (double)(run + f[u]) > target) {
-        a.ids[row] = (int)(0xffffffffu - (uint32_t)(lds.s.list[2 * tid + u] >> 32));
-        if (a.probs) a.probs[row] = prob_of(key[u], kept_mass);
-      }
-      run += f[u];
+    const u64 run = block_before(f, lds.s.slots, &all);
+    if (!((double)run > target) && (double)(run + f) > target) {
+      a.ids[row] = (int)(0xffffffffu - (uint32_t)(mine >> 32));
+      if (a.probs) a.probs[row] = prob_of(key, kept_mass);
     }
     return;
   }
-  // the draw among the chunks' sums and the kept tokens of the list, which are added to theirs
+  // the draw among the chunks' sums, with the list's kept tokens added to theirs
+  // Kept are the valid tokens not after the list's last kept one in order, of e >= min_p.  (None of
+  // the list, because of min_p: then those of the bins before it, as far as min_p keeps them.)
   if (tid == 0) {
-    s_cut = mode == kNoCut ? 0 : kept ? lds.s.list[kept - 1] : ~0ull;
+    s_cut = mode == kNoCut ? 0 : ~0ull;
     s_found = 0;
     s_before = 0;
   }
+  u64* const sums = lds.s.list;  // (at most kList chunks)
+  __syncthreads();
+  if (kept && tid == kept - 1) s_cut = mine;
+  if (tid < w.chunks) sums[tid] = w.sums[(size_t)row * w.chunks + tid];
   __syncthreads();
   const u64 cut = s_cut;
-  // tokens kept: valid, not after the cut in order, e >= min_p.  (Nothing kept of the list, because
-  // of min_p: then nothing below its bin is kept and e decides.)
-  u64 list_mine[2];
-#pragma unroll
-  for (int u = 0; u < 2; ++u) list_mine[u] = 2 * tid + u < kept ? lds.s.list[2 * tid + u] : 0;
-  __syncthreads();
-  u64* const sums = lds.s.list;  // at most kList chunks
-  for (int c = tid; c < w.chunks; c += kRowThreads) sums[c] = w.sums[(size_t)row * w.chunks + c];
-  __syncthreads();
-#pragma unroll
-  for (int u = 0; u < 2; ++u)
-    if (list_mine[u]) {
-      const int i = (int)(0xffffffffu - (uint32_t)list_mine[u]);
-      atomicAdd(&sums[(i + r.lead) / w.chunk], m.fixed(m.e((uint32_t)(list_mine[u] >> 32))));
-    }
-  __syncthreads();
-  const u64 s0 = 2 * tid < w.chunks ? sums[2 * tid] : 0;
-  const u64 s1 = 2 * tid + 1 < w.chunks ? sums[2 * tid + 1] : 0;
-  u64 total;
-  const u64 before = block_before<kRowWaves>(s0 + s1, lds.s.slots, &total);
-  const double target = uniform * (double)total;
-  if (!((double)before > target)) {
-    if ((double)(before + s0) > target) {
-      s_found = 2 * tid;
-      s_before = before;
-    } else if ((double)(before + s0 + s1) > target) {
-      s_found = 2 * tid + 1;
-      s_before = before + s0;
-    }
+  if (tid < kept) {
+    const int i = index_of(mine);
+    atomicAdd(&sums[(i + r.lead) / kChunk], m.fixed(m.e(key_in(mine))));
   }
   __syncthreads();
-  const int c = s_found;
-  u64 run = s_before;
-  for (int j = 0; j < w.chunk; j += 8 * kRowThreads) {
-    uint32_t k[8];
-    const int v = j + 8 * tid;
-    const bool inside = v < w.chunk;
-    const int i = r.keys(c * w.chunk + (inside ? v : 0), k);
-    u64 f[8], mine = 0;
+  const u64 own = tid < w.chunks ? sums[tid] : 0;
+  u64 total;
+  const u64 before = block_before(own, lds.s.slots, &total);
+  const double target = uniform * (double)total;
+  if (!((double)before > target) && (double)(before + own) > target) {
+    s_found = tid;
+    s_before = before;
+  }
+  __syncthreads();
+  float l[8];
+  const int i = r.values(s_found * kChunk + 8 * tid, l);
+  u64 f[8], sum = 0;
 #pragma unroll
-    for (int u = 0; u < 8; ++u) {
-      const u64 at = ((u64)k[u] << 32) | (0xffffffffu - (uint32_t)(i + u));
-      f[u] = 0;
-      const bool in_order = cut == ~0ull ? m.bin(k[u]) < rec.bin : at >= cut;
-      if (inside && k[u] > kMinusInf && in_order) {
-        const double e = m.e(k[u]);
-        if (e >= min_e) f[u] = m.fixed(e);
-      }
-      mine += f[u];
+  for (int u = 0; u < 8; ++u) {
+    const float z = m.place(l[u]);
+    f[u] = 0;
+    if (z < (float)(kBins - 1) &&
+        (cut == ~0ull ? z < (float)rec.bin : order_of(l[u], i + u) >= cut)) {
+      const double e = m.e(l[u]);
+      if (e >= min_e) f[u] = m.fixed(e);
     }
-    u64 all;
-    u64 at = run + block_before<kRowWaves>(mine, lds.s.slots, &all);
+    sum += f[u];
+  }
+  u64 all;
+  u64 run = s_before + block_before(sum, lds.s.slots, &all);
 #pragma unroll
-    for (int u = 0; u < 8; ++u) {
-      if (!((double)at > target) && (double)(at + f[u]) > target) {
-        a.ids[row] = i + u;
-        if (a.probs) a.probs[row] = prob_of(k[u], total);
-      }
-      at += f[u];
+  for (int u = 0; u < 8; ++u) {
+    if (!((double)run > target) && (double)(run + f[u]) > target) {
+      a.ids[row] = i + u;
+      if (a.probs) a.probs[row] = prob_of(key_of(l[u]), total);
     }
-    run += all;
-    if ((double)run > target) break;  // the same in all threads
+    run += f[u];
   }
 }
 
+#ifndef KP1
+#define KP1 2048
+#define KP2 1024
+#endif
+constexpr int kP1 = KP1, kP2 = KP2;
 size_t row_bytes(int chunks) {
-  return (size_t)chunks * 16 + kBins * 12 + kList * 8 + sizeof(RowRecord);
+  return (size_t)chunks * 16 + kAllBins * 12 + kList * 8 + sizeof(RowRecord) + 4;
 }
-int most_chunks(int vocab) { return (vocab + 7 + kChunkUnit - 1) / kChunkUnit; }
+// (a row may start up to 7 values past a 16-byte boundary)
+int row_chunks(int vocab) { return (vocab + 7 + kChunk - 1) / kChunk; }
 
 template <bool BF16>
 void launch_rows(const SampleArgs& a, const Work& w, double scale, hipStream_t s) {
@@ -819,23 +859,23 @@ void launch_rows(const SampleArgs& a, const Work& w, double scale, hipStream_t s
     sample_draw_kernel<BF16, true><<<a.rows, kRowThreads, 0, s>>>(a, w, scale);
     return;
   }
-  const dim3 grid(w.chunks, a.rows);
-  sample_best_kernel<BF16><<<grid, kThreads, 0, s>>>(a, w);
-  sample_bins_kernel<BF16><<<grid, kThreads, 0, s>>>(a, w, scale);
-  sample_list_kernel<BF16><<<grid, kThreads, 0, s>>>(a, w, scale);
+  const dim3 grid(w.parts, a.rows);
+  sample_best_kernel<BF16><<<grid, kRowThreads, 0, s>>>(a, w);
+  sample_bins_kernel<BF16><<<dim3(w.bin_parts, a.rows), kRowThreads, 0, s>>>(a, w, scale);
+  sample_list_kernel<BF16><<<grid, kRowThreads, 0, s>>>(a, w, scale);
   sample_draw_kernel<BF16, false><<<a.rows, kRowThreads, 0, s>>>(a, w, scale);
 }
 
 }  // namespace
 
 size_t sample_work_bytes(int vocab, int rows) {
-  return vocab <= kList ? 0 : (size_t)std::min(rows, kSamplePass) * row_bytes(most_chunks(vocab));
+  return vocab <= kList ? 0 : (size_t)std::min(rows, kSamplePass) * row_bytes(row_chunks(vocab));
 }
 
 void launch_sample(const SampleArgs& a, bool bf16, hipStream_t s) {
   int log = 0;
   while ((1 << log) < a.vocab) ++log;
-  const double scale = (double)(1ull << (62 - (log < 1 ? 1 : log)));
+  const double scale = (double)(1ull << std::min(51, 62 - log));
   for (int row = 0; row < a.rows; row += kSamplePass) {
     SampleArgs p = a;
     p.rows = std::min(kSamplePass, a.rows - row);
@@ -849,12 +889,12 @@ void launch_sample(const SampleArgs& a, bool bf16, hipStream_t s) {
     if (a.probs) p.probs += row;
     Work w{};
     if (a.vocab > kList) {
-      // chunks of 2048 values for few rows, up to 8192 where that still leaves 16 workgroups per CU
-      int units = 1;
-      while (units < 4 && (long long)p.rows * ((a.vocab + 7) / (kChunkUnit * units)) > 4096) units *= 2;
-      w.chunk = kChunkUnit * units;
-      w.chunks = (a.vocab + 7 + w.chunk - 1) / w.chunk;
-      const size_t rows = p.rows, most = most_chunks(a.vocab);
+      // Enough workgroups that rows which cost more than others are spread over the chip; fewer for the
+      // histogram, where each adds up to 4096 bins to the row's.
+      w.chunks = row_chunks(a.vocab);
+      w.parts = std::min(w.chunks, std::max(1, kP1 / p.rows));
+      w.bin_parts = std::min(w.chunks, std::max(1, kP2 / p.rows));
+      const size_t rows = p.rows, most = w.chunks;
       char* at = static_cast<char*>(a.work);
       auto take = [&](auto** q, size_t n) {
         *q = reinterpret_cast<std::remove_reference_t<decltype(*q)>>(at);
@@ -862,10 +902,11 @@ void launch_sample(const SampleArgs& a, bool bf16, hipStream_t s) {
       };
       take(&w.best, rows * most);
       take(&w.sums, rows * most);
-      take(&w.mass, rows * kBins);
+      take(&w.mass, rows * kAllBins);
       take(&w.list, rows * kList);
       take(&w.record, rows);
-      take(&w.count, rows * kBins);
+      take(&w.count, rows * kAllBins);
+      take(&w.listed, rows);
     }
     if (bf16) launch_rows<true>(p, w, scale, s);
     else launch_rows<false>(p, w, scale, s);
