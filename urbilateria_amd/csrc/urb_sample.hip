@@ -355,7 +355,8 @@ __device__ __noinline__ int draw_by_radix(const uint8_t* base, int V, const RowP
 
 constexpr int kList = 1024;                 // tokens that the last launch orders, one per thread
 constexpr int kChunk = 8 * kRowThreads;     // values per chunk: eight per thread
-constexpr int kMaxChunks = (1 << 20) / kChunk + 1;
+constexpr int kSpan = kChunk / kRowWaves;   // values per sum: a wave's of a chunk
+constexpr int kMaxSpans = ((1 << 20) / kChunk + 1) * kRowWaves;
 
 enum RowMode {
   kNoCut = 1,     // no top_k, no top_p: everything (that min_p leaves)
@@ -369,6 +370,7 @@ struct RowRecord {
   int few;        // kBinListed: the tokens up to the cut's bin fit a list too
   int above_n;    // tokens before the cut's bin
   u64 above, want;  // their mass; the mass that top_p asks for
+  u64 best;         // the row's largest logit (order_of)
 };
 
 constexpr int kGroup = 64, kAllBins = kBins + kBins / kGroup;
@@ -377,7 +379,7 @@ struct Work {
   int chunks;            // of a row
   int parts, bin_parts;  // workgroups that share a row's chunks; those of the histogram
   u64* best;          // [rows][parts] largest key << 32 | ~lowest index
-  u64* sums;          // [rows][chunks]
+  u64* sums;          // [rows][chunks * kRowWaves]: one per span
   u64* mass;          // [rows][kAllBins]: the bins, then groups of kGroup of them
   int* count;         // [rows][kAllBins]
   u64* list;          // [rows][kList] key << 32 | ~index
@@ -589,24 +591,29 @@ template <bool BF16>
 __global__ __launch_bounds__(kRowThreads, 8) void sample_list_kernel(SampleArgs a, Work w,
                                                                      double scale) {
   __shared__ u64 list[kList];
-  __shared__ u64 sums[kMaxChunks];
+  __shared__ u64 sums[kMaxSpans];
   __shared__ int s_n, s_at;
   __shared__ double powers[kPowers];
   const int row = blockIdx.y, tid = threadIdx.x, lane = tid & 63;
   const RowParams p = row_params(a, row);
   const u64 best = row_best(w, row);
-  if (trivial(p, best)) return;
+  if (trivial(p, best)) {
+    if (blockIdx.x == 0 && tid == 0) w.record[row].best = best;
+    return;
+  }
   const Row<BF16> r(a, row);
   const Part part(w, blockIdx.x, w.parts);
   float next[8];
   int at_next = r.values(part.first * kChunk + 8 * tid, next);
-  const RowRecord rec = find_cut(w, row, p, a.vocab);
+  RowRecord rec = find_cut(w, row, p, a.vocab);
+  rec.best = best;
   if (blockIdx.x == 0 && tid == 0) w.record[row] = rec;
   if (rec.mode == kByRadix) return;
   const Mass m(key_in(best), p.tau, scale, powers);
   const double min_e = (double)p.min_p;
   fill_powers(powers);
-  if (tid < part.last - part.first) sums[tid] = 0;
+  const int spans = (part.last - part.first) * kRowWaves;
+  for (int i = tid; i < spans; i += kRowThreads) sums[i] = 0;
   if (tid == 0) s_n = 0;
   __syncthreads();
   // places below `sum_to` are summed in the loop, those from there to below `list_to` listed
@@ -633,7 +640,7 @@ __global__ __launch_bounds__(kRowThreads, 8) void sample_list_kernel(SampleArgs 
     }
     if (!dense) {
       sum = wave_sum(sum);
-      if (lane == 0 && sum) atomicAdd(&sums[c - part.first], sum);
+      if (lane == 0) sums[(c - part.first) * kRowWaves + tid / 64] = sum;
     }
   }
   __syncthreads();
@@ -644,7 +651,7 @@ __global__ __launch_bounds__(kRowThreads, 8) void sample_list_kernel(SampleArgs 
     if (listed && m.place(key_value(key_in(mine))) < (float)rec.bin) {
       listed = false;
       const double e = m.e(key_in(mine));
-      if (e >= min_e) atomicAdd(&sums[(index_of(mine) + r.lead) / kChunk - part.first], m.fixed(e));
+      if (e >= min_e) atomicAdd(&sums[(index_of(mine) + r.lead) / kSpan - part.first * kRowWaves], m.fixed(e));
     }
     __syncthreads();
     if (tid == 0) s_n = 0;
@@ -659,35 +666,89 @@ __global__ __launch_bounds__(kRowThreads, 8) void sample_list_kernel(SampleArgs 
   if (tid == 0 && out) s_at = atomicAdd(&w.listed[row], out);
   __syncthreads();
   if (tid < out && s_at + tid < kList) w.list[(size_t)row * kList + s_at + tid] = list[tid];
-  if (rec.mode != kAllListed && tid < part.last - part.first)
-    w.sums[(size_t)row * w.chunks + part.first + tid] = sums[tid];
+  if (rec.mode != kAllListed)
+    for (int i = tid; i < spans; i += kRowThreads)
+      w.sums[((size_t)row * w.chunks + part.first) * kRowWaves + i] = sums[i];
 }
 
-// Sorts the block's values, one per thread, the first n of them not zero: descending by thread.
-// A bitonic network whose exchanges within a wave are shuffles.
-__device__ __forceinline__ u64 sort_descending(u64 v, int n, u64* lds) {
+// The value of lane (this ^ GAP), by moves between lanes where the hardware has one: within four
+// lanes, rotation by half a row of 16, swaps of rows and of half waves.
+template <int GAP>
+__device__ __forceinline__ uint32_t lane_xor(uint32_t v) {
+  if constexpr (GAP == 1) return __builtin_amdgcn_update_dpp(0, v, 0xb1, 0xf, 0xf, false);
+  if constexpr (GAP == 2) return __builtin_amdgcn_update_dpp(0, v, 0x4e, 0xf, 0xf, false);
+  if constexpr (GAP == 4) {  // mirrored in eight lanes, then in four
+    const uint32_t m = __builtin_amdgcn_update_dpp(0, v, 0x141, 0xf, 0xf, false);
+    return __builtin_amdgcn_update_dpp(0, m, 0x1b, 0xf, 0xf, false);
+  }
+  if constexpr (GAP == 8) return __builtin_amdgcn_update_dpp(0, v, 0x128, 0xf, 0xf, false);
+  if constexpr (GAP == 16) {
+    const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    return threadIdx.x & 16 ? r[0] : r[1];
+  }
+  if constexpr (GAP == 32) {
+    const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    return threadIdx.x & 32 ? r[0] : r[1];
+  }
+}
+template <int GAP>
+__device__ __forceinline__ u64 lane_xor(u64 v) {
+  return (u64)lane_xor<GAP>((uint32_t)v) | (u64)lane_xor<GAP>((uint32_t)(v >> 32)) << 32;
+}
+
+// Waves that hold the first n of a block's values, one per thread, as a power of two.
+__device__ __forceinline__ int waves_for(int n) {
+  int waves = 1;
+  while (64 * waves < n) waves *= 2;
+  return waves;
+}
+
+// Sorts the values of the block's first `waves` waves, one per thread: descending by thread.  A bitonic
+// network; the waves beyond keep to the barriers.
+__device__ __forceinline__ u64 sort_descending(u64 v, int waves, u64* lds) {
   const int tid = threadIdx.x;
-  int size = 64;
-  while (size < n) size *= 2;
-  for (int width = 2; width <= size; width *= 2)
-    for (int gap = width / 2; gap > 0; gap /= 2) {
-      u64 o;
-      if (gap >= 64) {
-        __syncthreads();
-        lds[tid] = v;
-        __syncthreads();
-        o = lds[tid ^ gap];
-      } else {
-        o = __shfl_xor(v, gap, 64);
-      }
-      const bool larger = ((tid & gap) == 0) == ((tid & width) == 0);
-      v = (o > v) == larger ? o : v;
+  const bool part = __builtin_amdgcn_readfirstlane(tid >> 6) < waves;
+  int width;
+  auto take = [&](u64 o, int gap) {
+    const bool larger = ((tid & gap) == 0) == ((tid & width) == 0);
+    v = (o > v) == larger ? o : v;
+  };
+  for (width = 2; width <= 64 * waves; width *= 2) {
+    for (int gap = width / 2; gap >= 64; gap /= 2) {
+      __syncthreads();
+      if (part) lds[tid] = v;
+      __syncthreads();
+      if (part) take(lds[tid ^ gap], gap);
     }
+    if (!part) continue;
+    if (width >= 64) take(lane_xor<32>(v), 32);
+    if (width >= 32) take(lane_xor<16>(v), 16);
+    if (width >= 16) take(lane_xor<8>(v), 8);
+    if (width >= 8) take(lane_xor<4>(v), 4);
+    if (width >= 4) take(lane_xor<2>(v), 2);
+    take(lane_xor<1>(v), 1);
+  }
   return v;
 }
 
+// block_before for values of the first `waves` waves; the others get nothing but the total.
+__device__ __forceinline__ u64 first_before(u64 v, int waves, u64* slots, u64* total) {
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  u64 upto = 0;
+  if (wave < waves) {
+    upto = wave_upto(v);
+    if (lane == 63) slots[wave] = upto;
+  }
+  __syncthreads();
+  const u64 all = wave_upto(lane < waves ? slots[lane] : 0);
+  *total = lane_of(all, 63);
+  return (wave && wave < waves ? lane_of(all, wave - 1) : 0) + upto - v;
+}
+
 // One workgroup per row: the last kept token of the list, then the draw.  SMALL: a vocabulary that fits
-// the list, in this launch alone.
+// the list, in this launch alone.  Bound by latency, 10 us or so of one step after another, so waves without a
+// value skip what only the others need.
 template <bool BF16, bool SMALL>
 __global__ __launch_bounds__(kRowThreads) void sample_draw_kernel(SampleArgs a, Work w,
                                                                   double scale) {
@@ -695,32 +756,38 @@ __global__ __launch_bounds__(kRowThreads) void sample_draw_kernel(SampleArgs a, 
     RowLds radix;
     struct {
       u64 list[kList];
-      u64 slots[kRowWaves];
-      int islots[kRowWaves];
+      u64 sums[kMaxSpans];
+      u64 slots[3][kRowWaves];
     } s;
   } lds;
   __shared__ int s_n, s_found;
   __shared__ u64 s_cut, s_before;
   __shared__ double powers[kPowers];
-  fill_powers(powers);
-  __syncthreads();
   const int row = blockIdx.x, tid = threadIdx.x;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const RowParams p = row_params(a, row);
   const Row<BF16> r(a, row);
-  u64 best = 0;
-  int mode = kAllListed, n = 0;
+  RowRecord rec{};
+  int n = 0;
+  u64 mine = 0;
+  if constexpr (!SMALL) {
+    rec = w.record[row];
+    n = min(w.listed[row], kList);
+    mine = w.list[(size_t)row * kList + tid];
+  }
+  fill_powers(powers);
+  if (tid == 0) s_n = 0;
+  __syncthreads();
   if constexpr (SMALL) {
-    if (tid == 0) s_n = 0;
-    __syncthreads();
     const u64 v = tid < r.V ? order_of(load_logit<BF16>(r.base, tid), tid) : 0;
     if (key_in(v) > kMinusInf) {
-      best = v;
-      lds.s.list[atomicAdd(&s_n, 1)] = best;
+      rec.best = v;
+      lds.s.list[atomicAdd(&s_n, 1)] = v;
     }
-    best = block_max(best, lds.s.slots);
+    rec.best = block_max(rec.best, lds.s.slots[0]);
+    rec.mode = kAllListed;
     n = s_n;
-  } else {
-    best = row_best(w, row);
+    mine = lds.s.list[tid];
   }
   auto done = [&](int id, float prob) {
     if (tid == 0) {
@@ -728,117 +795,101 @@ __global__ __launch_bounds__(kRowThreads) void sample_draw_kernel(SampleArgs a, 
       if (a.probs) a.probs[row] = prob;
     }
   };
-  if (trivial(p, best)) {
+  if (trivial(p, rec.best)) {
     if (!p.ok && tid == 0) flag(a.status, kStepArgument);
-    const bool greedy = p.ok && (uint32_t)(best >> 32) > kMinusInf;
-    done(greedy ? index_of(best) : -1, greedy ? 1.0f : 0.0f);
+    const bool greedy = p.ok && key_in(rec.best) > kMinusInf;
+    done(greedy ? index_of(rec.best) : -1, greedy ? 1.0f : 0.0f);
     return;
   }
-  const Mass m(key_in(best), p.tau, scale, powers);
+  const Mass m(key_in(rec.best), p.tau, scale, powers);
   const double min_e = (double)p.min_p, uniform = (double)p.uniform;
-  auto prob_of = [&](uint32_t key, u64 total) {
-    return (float)(m.e(key) / ((double)total / scale));
-  };
-  RowRecord rec{};
   if constexpr (!SMALL) {
-    rec = w.record[row];
-    mode = rec.mode;
-    n = min(w.listed[row], kList);
-    if (mode == kByRadix) {
+    if (rec.mode == kByRadix) {
       u64 total;
-      __syncthreads();
       const int id = draw_by_radix<BF16>(r.base, r.V, p, m, lds.radix, &total);
-      done(id, prob_of(key_of(load_logit<BF16>(r.base, id)), total));
+      done(id, (float)(m.e(load_logit<BF16>(r.base, id)) / ((double)total / scale)));
       return;
     }
-    if (tid < n) lds.s.list[tid] = w.list[(size_t)row * kList + tid];
   }
-  u64 mine = tid < n ? lds.s.list[tid] : 0;  // (its own store, or SMALL's before the barriers)
-  // the list's kept tokens are its first `kept` in order
-  int kept = 0;
-  u64 kept_mass = 0;
-  if (mode != kNoCut) {
-    mine = sort_descending(mine, n, lds.s.list);
+  if (tid >= n) mine = 0;
+  const int spans = SMALL ? (kList + 7 + kSpan - 1) / kSpan : w.chunks * kRowWaves;
+  for (int i = tid; i < spans; i += kRowThreads)
+    lds.s.sums[i] =
+        rec.mode == kAllListed ? 0 : w.sums[(size_t)row * w.chunks * kRowWaves + i];
+  // Kept are the valid tokens not after the cut in order, of e >= min_p: the cut is the list's last
+  // kept one.  (None of the list, because of min_p: then those of the bins before it, as far as min_p
+  // keeps them.)  The list's kept tokens are added to their spans' sums.
+  u64 cut = 0;
+  if (rec.mode != kNoCut) {
+    const int waves = waves_for(n);
+    mine = sort_descending(mine, waves, lds.s.list);
     const bool by_count = p.top_k > 0 && p.top_k < r.V;
     // (with every kept token in the list nothing comes before it)
-    const bool part = mode == kBinListed;
+    const bool part = rec.mode == kBinListed;
     const int most = by_count ? min(n, p.top_k - (part ? rec.above_n : 0)) : n;
-    const double e = tid < most ? m.e(key_in(mine)) : 0.0;
-    const u64 f = tid < most ? m.fixed(e) : 0;
+    double e = 0.0;
+    u64 f = 0;
+    if (tid < most) {
+      e = m.e(key_in(mine));
+      f = m.fixed(e);
+    }
     u64 all;
-    const u64 run = (part ? rec.above : 0) + block_before(f, lds.s.slots, &all);
+    const u64 run = (part ? rec.above : 0) + first_before(f, waves, lds.s.slots[0], &all);
     u64 want = ~0ull;
     if (p.top_p < 1.0f) want = SMALL || by_count ? mass_wanted(p.top_p, all) : rec.want;
     // (with equal logits e >= min_p holds for all or none, so the kept ones stay a beginning)
     const bool keep = tid < most && run < want && e >= min_e;
-    kept = __syncthreads_count(keep);
-    kept_mass = block_sum(keep ? f : 0, lds.s.slots);
-  }
-  if (mode == kAllListed) {
-    // the draw among the kept tokens by index: sorted by it, the key in the low half
-    const double target = uniform * (double)kept_mass;
-    mine = sort_descending(tid < kept ? (mine << 32) | (mine >> 32) : 0, kept, lds.s.list);
-    const uint32_t key = (uint32_t)mine;
-    const u64 f = tid < kept ? m.fixed(m.e(key)) : 0;
-    u64 all;
-    const u64 run = block_before(f, lds.s.slots, &all);
-    if (!((double)run > target) && (double)(run + f) > target) {
-      a.ids[row] = (int)(0xffffffffu - (uint32_t)(mine >> 32));
-      if (a.probs) a.probs[row] = prob_of(key, kept_mass);
-    }
-    return;
-  }
-  // the draw among the chunks' sums, with the list's kept tokens added to theirs
-  // Kept are the valid tokens not after the list's last kept one in order, of e >= min_p.  (None of
-  // the list, because of min_p: then those of the bins before it, as far as min_p keeps them.)
-  if (tid == 0) {
-    s_cut = mode == kNoCut ? 0 : ~0ull;
-    s_found = 0;
-    s_before = 0;
-  }
-  u64* const sums = lds.s.list;  // (at most kList chunks)
-  __syncthreads();
-  if (kept && tid == kept - 1) s_cut = mine;
-  if (tid < w.chunks) sums[tid] = w.sums[(size_t)row * w.chunks + tid];
-  __syncthreads();
-  const u64 cut = s_cut;
-  if (tid < kept) {
-    const int i = index_of(mine);
-    atomicAdd(&sums[(i + r.lead) / kChunk], m.fixed(m.e(key_in(mine))));
+    const int kept = __syncthreads_count(keep);
+    if (keep) atomicAdd(&lds.s.sums[(index_of(mine) + r.lead) / kSpan], f);
+    if (kept == 0 && tid == 0) s_cut = ~0ull;
+    if (keep && tid == kept - 1) s_cut = mine;
   }
   __syncthreads();
-  const u64 own = tid < w.chunks ? sums[tid] : 0;
+  if (rec.mode != kNoCut) cut = s_cut;
+  // the span of the draw: up to three per thread, in order
+  const int per = (spans + kRowThreads - 1) / kRowThreads;
+  const int span_waves = (spans + 64 * per - 1) / (64 * per);
+  u64 own[3] = {}, sum = 0;
+#pragma unroll
+  for (int j = 0; j < 3; ++j) {
+    const int i = tid * per + j;
+    if (j < per && i < spans) own[j] = lds.s.sums[i];
+    sum += own[j];
+  }
   u64 total;
-  const u64 before = block_before(own, lds.s.slots, &total);
+  u64 before = first_before(sum, span_waves, lds.s.slots[1], &total);
   const double target = uniform * (double)total;
-  if (!((double)before > target) && (double)(before + own) > target) {
-    s_found = tid;
+  if (!((double)before > target) && (double)(before + sum) > target) {
+    int j = 0;
+    if (!((double)(before + own[0]) > target)) {
+      before += own[0];
+      j = 1;
+      if (!((double)(before + own[1]) > target)) {
+        before += own[1];
+        j = 2;
+      }
+    }
+    s_found = tid * per + j;
     s_before = before;
   }
   __syncthreads();
-  float l[8];
-  const int i = r.values(s_found * kChunk + 8 * tid, l);
-  u64 f[8], sum = 0;
-#pragma unroll
-  for (int u = 0; u < 8; ++u) {
-    const float z = m.place(l[u]);
-    f[u] = 0;
-    if (z < (float)(kBins - 1) &&
-        (cut == ~0ull ? z < (float)rec.bin : order_of(l[u], i + u) >= cut)) {
-      const double e = m.e(l[u]);
-      if (e >= min_e) f[u] = m.fixed(e);
+  // the draw in it, a value per thread
+  u64 f = 0;
+  double e = 0.0;
+  const int i = s_found * kSpan + tid - r.lead;
+  if (tid < kSpan && i >= 0 && i < r.V) {
+    const float l = load_logit<BF16>(r.base, i);
+    const float z = m.place(l);
+    if (z < (float)(kBins - 1) && (cut == ~0ull ? z < (float)rec.bin : order_of(l, i) >= cut)) {
+      e = m.e(l);
+      if (e >= min_e) f = m.fixed(e);
     }
-    sum += f[u];
   }
   u64 all;
-  u64 run = s_before + block_before(sum, lds.s.slots, &all);
-#pragma unroll
-  for (int u = 0; u < 8; ++u) {
-    if (!((double)run > target) && (double)(run + f[u]) > target) {
-      a.ids[row] = i + u;
-      if (a.probs) a.probs[row] = prob_of(key_of(l[u]), total);
-    }
-    run += f[u];
+  const u64 run = s_before + first_before(f, kSpan / 64, lds.s.slots[2], &all);
+  if (wave < kSpan / 64 && !((double)run > target) && (double)(run + f) > target) {
+    a.ids[row] = i;
+    if (a.probs) a.probs[row] = (float)(e / ((double)total / scale));
   }
 }
 
@@ -848,7 +899,7 @@ __global__ __launch_bounds__(kRowThreads) void sample_draw_kernel(SampleArgs a, 
 #endif
 constexpr int kP1 = KP1, kP2 = KP2;
 size_t row_bytes(int chunks) {
-  return (size_t)chunks * 16 + kAllBins * 12 + kList * 8 + sizeof(RowRecord) + 4;
+  return (size_t)chunks * 8 * (1 + kRowWaves) + kAllBins * 12 + kList * 8 + sizeof(RowRecord) + 4;
 }
 // (a row may start up to 7 values past a 16-byte boundary)
 int row_chunks(int vocab) { return (vocab + 7 + kChunk - 1) / kChunk; }
@@ -901,7 +952,7 @@ void launch_sample(const SampleArgs& a, bool bf16, hipStream_t s) {
         at += n * sizeof(**q);
       };
       take(&w.best, rows * most);
-      take(&w.sums, rows * most);
+      take(&w.sums, rows * most * kRowWaves);
       take(&w.mass, rows * kAllBins);
       take(&w.list, rows * kList);
       take(&w.record, rows);
