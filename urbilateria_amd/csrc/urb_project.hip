@@ -349,6 +349,220 @@ __global__ __launch_bounds__(64 * kSplitWaves) void split_kernel(ProjArgs p, int
   }
 }
 
+// ---- W x for many tokens: tiles of WM x MB 16-token blocks by WN x NP panels ----
+//
+// Each of WM x WN waves multiplies NP panels by MB blocks.  Weights go from L2 straight into registers
+// (a panel's slab is an MFMA operand as it lies), two slabs ahead; rows go through registers into LDS,
+// one step of 128 values ahead, in two halves between the step's MFMAs.  Row m's chunk c (16 bytes) of a
+// step lies at position c ^ x_swizzle(m) of the row's 256 bytes: a wave stores 1 KiB in a run, and the 16
+// lanes that an LDS read serves at a time hit 16 distinct bank groups.  Scheduling fences hold the loads
+// where they are written; left alone, the compiler sinks them to just before their use.
+constexpr int kTileStep = kGemmKStep;
+
+template <int FMT>
+__device__ __forceinline__ int x_swizzle(int m) {
+  // chunks read together: c and c ^ 1 (BF16), c and c ^ 4 (MX: frag_k)
+  return FMT == kFmtBF16 ? m & 15 : (m & 3) | ((m & 8) ? 12 : 0);
+}
+
+// __builtin_amdgcn_sched_barrier: VALU, SALU and LDS reads may cross; loads, LDS stores, MFMAs stay.
+constexpr int kHoldLoads = 0x106;
+
+// Slabs of a panel per step, and the operands in each.
+template <int FMT>
+constexpr int tile_slabs() { return FMT == kFmtMXFP4 ? 1 : FMT == kFmtMXFP8 ? 2 : 4; }
+template <int FMT>
+__device__ __forceinline__ bf16x8 tile_operand(const uint4& q, float sc, int part) {
+  if constexpr (FMT == kFmtBF16) {
+    return __builtin_bit_cast(bf16x8, q);
+  } else if constexpr (FMT == kFmtMXFP4) {
+    const uint32_t w = part == 0 ? q.x : part == 1 ? q.y : part == 2 ? q.z : q.w;
+    return pack8(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, sc, 0),
+                 __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, sc, 1),
+                 __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, sc, 2),
+                 __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, sc, 3));
+  } else {
+    const uint32_t w0 = part ? q.z : q.x, w1 = part ? q.w : q.y;
+    return pack8(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w0, sc, false),
+                 __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w0, sc, true),
+                 __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w1, sc, false),
+                 __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w1, sc, true));
+  }
+}
+
+// Rows in BF16 planes: plane i of row t at x + i * plane + t * x_stride; `planes`: how many of them each
+// row needs (NULL: one).
+struct TileRows {
+  size_t plane;
+  const int* planes;
+};
+
+template <int FMT, bool YB, int WM, int WN, int MB, int NP>
+__global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(
+    ProjArgs p, TileRows rows, int u_ld, int slices, int col_tiles) {
+  constexpr int WAVES = WM * WN, TM = 16 * WM * MB, TN = WN * NP;  // tokens, panels
+  constexpr int COPIES = TM * 16 / (64 * WAVES), HALF = COPIES / 2;  // per thread and step
+  constexpr int SL = tile_slabs<FMT>(), PARTS = 4 / SL;
+  constexpr bool MX = FMT != kFmtBF16;
+  __shared__ __attribute__((aligned(16))) u16 x0[TM * kTileStep];
+  __shared__ __attribute__((aligned(16))) u16 x1[TM * kTileStep];
+  __shared__ TileSlots<TM> slots;
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int ln = lane & 15, lq = lane >> 4;
+  const int wm = wave % WM, wn = wave / WM;
+  const int t0 = (blockIdx.x / col_tiles) * TM, count = min(TM, p.tokens - t0);
+  const int panels = p.rows / kPanelRows;
+  const int panel0 = (blockIdx.x % col_tiles) * TN + wn * NP;
+  const int steps = p.cols / kTileStep;
+  const size_t pbytes = kPanelRows * panel_row_bytes<FMT>(p.cols);
+  const size_t pscales = (size_t)kPanelRows * (p.cols / 32);
+  const uint8_t* pd[NP];
+  const uint8_t* ps[NP];
+#pragma unroll
+  for (int q = 0; q < NP; ++q) {  // a panel past the last reads the last again and stores nothing
+    const int panel = min(panel0 + q, panels - 1);
+    pd[q] = p.data + panel * pbytes;
+    ps[q] = MX ? p.scales + panel * pscales : nullptr;
+  }
+  int planes = 1;
+  if (rows.planes) {
+    for (int i = lane; i < count; i += 64) planes = max(planes, rows.planes[t0 + i]);
+    for (int o = 32; o > 0; o >>= 1) planes = max(planes, __shfl_xor(planes, o, 64));
+    planes = __builtin_amdgcn_readfirstlane(planes);
+  }
+  // this lane's copies: rows 4 (wave + WAVES i) + lane / 16, the same chunk of each
+  const int copy_row = 4 * wave + lane / 16;
+  const int copy_chunk = (lane & 15) ^ x_swizzle<FMT>(copy_row);
+  const uint8_t* const xt = reinterpret_cast<const uint8_t*>(p.x) + (size_t)t0 * p.x_stride * 2;
+  uint32_t copy_off[COPIES];
+#pragma unroll
+  for (int i = 0; i < COPIES; ++i)
+    copy_off[i] = (uint32_t)min(copy_row + 4 * WAVES * i, count - 1) * (uint32_t)(p.x_stride * 2) +
+                  16u * copy_chunk;
+  // the rows of step s, plane pl: copies `first` .. first + HALF
+  auto load_rows = [&](uint4* st, int first, int s, int pl) {
+    const uint8_t* from = xt + pl * rows.plane + (size_t)s * (2 * kTileStep);
+#pragma unroll
+    for (int i = 0; i < HALF; ++i) st[i] = ldg16(from + copy_off[first + i]);
+  };
+  auto store_rows = [&](const uint4* st, int first, u16* to) {
+#pragma unroll
+    for (int i = 0; i < HALF; ++i)
+      *reinterpret_cast<uint4*>(to + (wave + WAVES * (first + i)) * 512 + 8 * lane) = st[i];
+  };
+  // fragment reads: byte offsets of MFMA j's operand in block 0 of the wave's rows
+  uint32_t fo[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    fo[j] = (uint32_t)(wm * MB * 16 + ln) * 256u +
+            16u * ((frag_k<FMT>(j, lq) >> 3) ^ x_swizzle<FMT>(ln));
+
+  f32x4 acc[NP][MB];
+#pragma unroll
+  for (int q = 0; q < NP; ++q)
+#pragma unroll
+    for (int m = 0; m < MB; ++m) acc[q][m] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+  uint4 slab[2][NP];
+  uint32_t sc[2][NP];
+  const uint32_t doff = 16u * lane;
+  auto fetch = [&](uint4* to, int u) {
+#pragma unroll
+    for (int q = 0; q < NP; ++q) to[q] = ldg16(pd[q] + (doff + (uint32_t)u * 1024u));
+  };
+  auto fetch_scales = [&](uint32_t* to, int s) {
+    if constexpr (MX) {
+#pragma unroll
+      for (int q = 0; q < NP; ++q) to[q] = ldg_u8(ps[q] + ((uint32_t)lane + (uint32_t)s * 64u));
+    }
+  };
+  // One step: rows in `from`, the next step's (s1, pl1) into `to`.  PAR: parity of the step.
+  auto step = [&](auto par, const u16* from, u16* to, int s, int s1, int pl1) {
+    constexpr int PAR = decltype(par)::value;
+    const uint8_t* base = reinterpret_cast<const uint8_t*>(from);
+    uint4 st[HALF];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int part = j % PARTS, slot = FMT == kFmtMXFP4 ? PAR : (j / PARTS) & 1;
+      if (j == 0) {
+        load_rows(st, 0, s1, pl1);
+        if constexpr (FMT == kFmtMXFP4) fetch(slab[PAR ^ 1], s1);
+        fetch_scales(sc[PAR ^ 1], s1);
+      }
+      if (j == 2) {
+        store_rows(st, 0, to);
+        load_rows(st, HALF, s1, pl1);
+      }
+      __builtin_amdgcn_sched_barrier(kHoldLoads);
+      bf16x8 a[MB];
+#pragma unroll
+      for (int m = 0; m < MB; ++m)
+        a[m] = __builtin_bit_cast(bf16x8, *reinterpret_cast<const uint4*>(base + fo[j] + m * 4096));
+#pragma unroll
+      for (int q = 0; q < NP; ++q) {
+        const bf16x8 w =
+            tile_operand<FMT>(slab[slot][q], MX ? e8m0_to_f32(sc[PAR][q]) : 1.0f, part);
+#pragma unroll
+        for (int m = 0; m < MB; ++m) acc[q][m] = mfma(w, a[m], acc[q][m]);
+      }
+      __builtin_amdgcn_sched_barrier(kHoldLoads);
+      if constexpr (FMT != kFmtMXFP4) {
+        // the slab two on takes this one's place: of this step or the next
+        if (part == PARTS - 1) {
+          const int k = j / PARTS + 2;
+          fetch(slab[slot], k < SL ? s * SL + k : s1 * SL + k - SL);
+        }
+      }
+    }
+    store_rows(st, HALF, to);
+    __syncthreads();
+  };
+
+  fetch(slab[0], 0);
+  if constexpr (FMT != kFmtMXFP4) fetch(slab[1], 1);
+  fetch_scales(sc[0], 0);
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    uint4 st[HALF];
+    load_rows(st, h * HALF, 0, 0);
+    store_rows(st, h * HALF, x0);
+  }
+  __syncthreads();
+  // steps in order, each over its planes; the one after the last reads the last again
+  int s = 0, pl = 0;
+  auto advance = [&](auto par, const u16* from, u16* to) {
+    int s1 = s, pl1 = pl + 1;
+    if (pl1 == planes) {
+      pl1 = 0;
+      s1 = s + 1;
+    }
+    step(par, from, to, s, min(s1, steps - 1), pl1);
+    s = s1;
+    pl = pl1;
+  };
+  while (true) {
+    advance(Int<0>{}, x0, x1);
+    if (s == steps) break;
+    advance(Int<1>{}, x1, x0);
+    if (s == steps) break;
+  }
+  if (p.ids) find_slots(p, t0, count, slots);
+#pragma unroll
+  for (int m = 0; m < MB; ++m) {
+    const int local = (wm * MB + m) * 16 + ln, t = t0 + local;
+    if ((wm * MB + m) * 16 >= count) break;
+#pragma unroll
+    for (int q = 0; q < NP; ++q) {
+      const int panel = panel0 + q;
+      if (panel >= panels) break;
+      f32x4 v = acc[q][m];
+      if (p.ids) add_adapters<YB ? 2 : 3>(p, slots, u_ld, slices, panel, local, t, v);
+      if (local < count) store_y<YB>(p, t, panel * kPanelRows + 4 * lq, v);
+    }
+  }
+}
+
 // ---- laying an adapter out ----
 // A: 16-rank panels of the BF16 panel layout; B: units of 8 ranks, [panel of 16 rows][unit][row].
 __global__ void pack_adapter_kernel(const uint16_t* __restrict__ a, const uint16_t* __restrict__ b,
@@ -401,6 +615,26 @@ void launch_rows(const ProjArgs& p, int u_ld, int slices, hipStream_t s) {
   else go(Int<4>{}, Int<2>{});
 }
 
+template <int FMT, bool YB>
+void launch_tiles(const ProjArgs& p, const TileRows& rows, int u_ld, int slices, hipStream_t s) {
+  const int panels = p.rows / kPanelRows;
+  auto go = [&](auto wm, auto wn, auto mb, auto np) {
+    constexpr int WM = decltype(wm)::value, WN = decltype(wn)::value, MB = decltype(mb)::value,
+                  NP = decltype(np)::value;
+    const int col_tiles = (panels + WN * NP - 1) / (WN * NP);
+    const int row_tiles = (p.tokens + 16 * WM * MB - 1) / (16 * WM * MB);
+    tile_kernel<FMT, YB, WM, WN, MB, NP><<<col_tiles * row_tiles, 64 * WM * WN, 0, s>>>(
+        p, rows, u_ld, slices, col_tiles);
+  };
+#ifdef TILEB
+  go(Int<2>{}, Int<2>{}, Int<4>{}, Int<4>{});
+#elif defined TILEC
+  go(Int<1>{}, Int<4>{}, Int<8>{}, Int<4>{});
+#else
+  go(Int<2>{}, Int<4>{}, Int<8>{}, Int<4>{});
+#endif
+}
+
 template <bool XB>
 void launch_shrink(const ProjArgs& p, int u_ld, int slices, hipStream_t s) {
   const bool by_token = p.tokens <= kScan && p.tokens <= p.slots;
@@ -413,6 +647,12 @@ void launch_shrink(const ProjArgs& p, int u_ld, int slices, hipStream_t s) {
 
 template <int FMT>
 void launch_types(const ProjArgs& p, int u_ld, int slices, hipStream_t s) {
+  if (p.x_bf16 && p.tokens >= 256 && p.x_stride < (1u << 22)) {
+    const TileRows rows{0, nullptr};
+    if (p.y_bf16) launch_tiles<FMT, true>(p, rows, u_ld, slices, s);
+    else launch_tiles<FMT, false>(p, rows, u_ld, slices, s);
+    return;
+  }
   if (p.x_bf16) {
     if (p.y_bf16) launch_rows<FMT, true, true>(p, u_ld, slices, s);
     else launch_rows<FMT, true, false>(p, u_ld, slices, s);
