@@ -397,9 +397,29 @@ struct TileRows {
   const int* planes;
 };
 
+// Tiles by workgroup.  Workgroup b runs on XCD b % 8, which has an L2 of its own: the tiles are cut into
+// 8 rectangles of by_rows x by_cols XCDs, so that an XCD reads a part of the rows and a part of the weights
+// (all of both otherwise).  Within it, bands of `band` row tiles are walked column by column.
+struct TileGrid {
+  int rows, cols;        // tiles
+  int by_rows, by_cols;  // XCDs
+  int band;
+  __host__ __device__ int tall() const { return (rows + by_rows - 1) / by_rows; }
+  __host__ __device__ int wide() const { return (cols + by_cols - 1) / by_cols; }
+  __device__ bool place(int block, int* row, int* col) const {
+    const int xcd = block % 8, i = block / 8, h = tall(), w = wide();
+    const int b = i / (band * w), in = i - b * band * w;
+    const int here = min(band, h - b * band);  // rows of this band
+    const int r = b * band + in % here, c = in / here;
+    *row = xcd % by_rows * h + r;
+    *col = xcd / by_rows * w + c;
+    return r < h && c < w && *row < rows && *col < cols;
+  }
+};
+
 template <int FMT, bool YB, int WM, int WN, int MB, int NP>
 __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(
-    ProjArgs p, TileRows rows, int u_ld, int slices, int col_tiles) {
+    ProjArgs p, TileRows rows, int u_ld, int slices, TileGrid grid) {
   constexpr int WAVES = WM * WN, TM = 16 * WM * MB, TN = WN * NP;  // tokens, panels
   constexpr int COPIES = TM * 16 / (64 * WAVES), HALF = COPIES / 2;  // per thread and step
   constexpr int SL = tile_slabs<FMT>(), PARTS = 4 / SL;
@@ -411,9 +431,11 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int ln = lane & 15, lq = lane >> 4;
   const int wm = wave % WM, wn = wave / WM;
-  const int t0 = (blockIdx.x / col_tiles) * TM, count = min(TM, p.tokens - t0);
+  int row_tile, col_tile;
+  if (!grid.place(blockIdx.x, &row_tile, &col_tile)) return;
+  const int t0 = row_tile * TM, count = min(TM, p.tokens - t0);
   const int panels = p.rows / kPanelRows;
-  const int panel0 = (blockIdx.x % col_tiles) * TN + wn * NP;
+  const int panel0 = col_tile * TN + wn * NP;
   const int steps = p.cols / kTileStep;
   const size_t pbytes = kPanelRows * panel_row_bytes<FMT>(p.cols);
   const size_t pscales = (size_t)kPanelRows * (p.cols / 32);
@@ -615,16 +637,40 @@ void launch_rows(const ProjArgs& p, int u_ld, int slices, hipStream_t s) {
   else go(Int<4>{}, Int<2>{});
 }
 
+template <int FMT>
+constexpr double kWeightBits = FMT == kFmtBF16 ? 16 : FMT == kFmtMXFP8 ? 8.25 : 4.25;
+
 template <int FMT, bool YB>
 void launch_tiles(const ProjArgs& p, const TileRows& rows, int u_ld, int slices, hipStream_t s) {
   const int panels = p.rows / kPanelRows;
   auto go = [&](auto wm, auto wn, auto mb, auto np) {
     constexpr int WM = decltype(wm)::value, WN = decltype(wn)::value, MB = decltype(mb)::value,
                   NP = decltype(np)::value;
-    const int col_tiles = (panels + WN * NP - 1) / (WN * NP);
-    const int row_tiles = (p.tokens + 16 * WM * MB - 1) / (16 * WM * MB);
-    tile_kernel<FMT, YB, WM, WN, MB, NP><<<col_tiles * row_tiles, 64 * WM * WN, 0, s>>>(
-        p, rows, u_ld, slices, col_tiles);
+    TileGrid grid{};
+    grid.cols = (panels + WN * NP - 1) / (WN * NP);
+    grid.rows = (p.tokens + 16 * WM * MB - 1) / (16 * WM * MB);
+    // the cut that leaves an XCD the fewest tiles, then the fewest bytes to read
+    const double row_bytes = 16.0 * WM * MB * 2, col_bytes = 16.0 * WN * NP * kWeightBits<FMT> / 8;
+    long best = -1;
+    double bytes = 0;
+    for (int r = 1; r <= 8; r *= 2) {
+      TileGrid g = grid;
+      g.by_rows = r;
+      g.by_cols = 8 / r;
+      const long tiles = (long)g.tall() * g.wide();
+      const double read = g.tall() * row_bytes + g.wide() * col_bytes;
+      if (best < 0 || tiles < best || (tiles == best && read < bytes)) {
+        best = tiles;
+        bytes = read;
+        grid = g;
+      }
+    }
+#ifndef BAND
+#define BAND 8
+#endif
+    grid.band = std::min(BAND, grid.tall());
+    const int blocks = 8 * grid.tall() * grid.wide();
+    tile_kernel<FMT, YB, WM, WN, MB, NP><<<blocks, 64 * WM * WN, 0, s>>>(p, rows, u_ld, slices, grid);
   };
 #ifdef TILEB
   go(Int<2>{}, Int<2>{}, Int<4>{}, Int<4>{});
