@@ -2,8 +2,8 @@
 //
 //   y[t] = W x[t] + scale_a B_a (A_a x[t])
 //
-// Two launches: the adapters' first products u = A x into the workspace, then W x with the
-// second products added to the accumulators before they are rounded (without adapters only the latter).
+// The adapters' first products u = A x come first, into the workspace; then W x, with the second products
+// added to the accumulators before they are rounded (without adapters only the latter).
 //
 // Operands.  W streams in the panel layout (urb_kernels.hpp) straight into MFMA operands, MX codes
 // decoded to BF16 in registers (exact).  f32 rows are carried as three BF16 planes: truncating v to
@@ -12,7 +12,8 @@
 // same way, into two planes (16 bits) where the outputs are BF16, three where they are f32.
 //
 // A tile may hold rows of any adapters: each distinct adapter of the tile multiplies the tile's u with
-// the other adapters' rows set to zero, so order and mix of the rows cost time but no sorting pass.
+// the other adapters' rows set to zero.  A row has one adapter, so the order in which a tile takes its
+// adapters changes no sum, and a row's result does not depend on the rows beside it.
 #include "urb_panel.hpp"
 #include "urb_step.hpp"
 
@@ -21,6 +22,8 @@ namespace urb {
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int kTileTokens = 256;  // rows of a call that takes tiles
+constexpr int kMaxSlices = 16;    // most K slices of the first product for few tokens
 
 // v as BF16 planes by truncation, v = hi + mid + lo exactly (v finite and not subnormal in the
 // lower planes); an infinity keeps its first plane alone.
@@ -188,55 +191,233 @@ __global__ __launch_bounds__(kThreads) void shrink_kernel(ProjArgs p, int u_ld, 
   }
 }
 
-// ---- the second products, added to the accumulators of a tile ----
+// ---- u for many tokens: blocks of 16 rows of one adapter ----
 
-// The distinct filled slots among `count` rows from `t0` (at most kMax), in LDS.
+constexpr int kOrderThreads = 1024;
+
+// The rows in order of their adapters, and the blocks of up to 16 rows of one adapter: slot, first place
+// in the order, rows.  One workgroup; `order` holds `tokens` entries, `blocks` (3 ints each) at most
+// order_blocks().  Which row of an adapter comes first is left to chance: no sum goes over rows.
+__global__ __launch_bounds__(kOrderThreads) void order_kernel(ProjArgs p, int* order, int* blocks,
+                                                              int* n_blocks) {
+  __shared__ int count[4096];   // rows per slot, then the place of its next one
+  __shared__ int waves[2][kOrderThreads / 64];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  for (int i = tid; i < p.slots; i += kOrderThreads) count[i] = 0;
+  __syncthreads();
+  for (int t = tid; t < p.tokens; t += kOrderThreads) {
+    const int id = p.ids[t];
+    if (id < 0) continue;
+    if (id < p.slots && p.table[id].rank > 0) atomicAdd(&count[id], 1);
+    else flag(p.status, kStepArgument);
+  }
+  __syncthreads();
+  // four slots per thread, in order: running sums of rows and of blocks
+  int n[4], rows = 0, tiles = 0;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    n[j] = 4 * tid + j < p.slots ? count[4 * tid + j] : 0;
+    rows += n[j];
+    tiles += (n[j] + 15) / 16;
+  }
+  int row = rows, tile = tiles;
+  for (int o = 1; o < 64; o <<= 1) {
+    const int r = __shfl_up(row, o, 64), b = __shfl_up(tile, o, 64);
+    if (lane >= o) {
+      row += r;
+      tile += b;
+    }
+  }
+  if (lane == 63) {
+    waves[0][wave] = row;
+    waves[1][wave] = tile;
+  }
+  __syncthreads();
+  row -= rows;
+  tile -= tiles;
+  for (int w = 0; w < wave; ++w) {
+    row += waves[0][w];
+    tile += waves[1][w];
+  }
+  if (tid == kOrderThreads - 1) *n_blocks = tile + tiles;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    if (4 * tid + j < p.slots) count[4 * tid + j] = row;
+    for (int i = 0; i < n[j]; i += 16) {
+      blocks[3 * tile] = 4 * tid + j;
+      blocks[3 * tile + 1] = row + i;
+      blocks[3 * tile + 2] = min(16, n[j] - i);
+      ++tile;
+    }
+    row += n[j];
+  }
+  __syncthreads();
+  for (int t = tid; t < p.tokens; t += kOrderThreads) {
+    const int id = p.ids[t];
+    if (id >= 0 && id < p.slots && p.table[id].rank > 0) order[atomicAdd(&count[id], 1)] = t;
+  }
+}
+
+constexpr int kBlockWaves = 8;
+
+// u of one block, whole: eight waves split K, four 16-rank panels at a time.  Written scaled, in the
+// planes that the second product multiplies: u_planes[(t * P + plane) * u_ld + rank].
+template <bool XB, int P>
+__global__ __launch_bounds__(64 * kBlockWaves) void shrink_block_kernel(ProjArgs p, const int* order,
+                                                                        const int* blocks,
+                                                                        const int* n_blocks,
+                                                                        uint16_t* u_planes, int u_ld) {
+  __shared__ f32x4 red[kBlockWaves][4][64];
+  if ((int)blockIdx.x >= *n_blocks) return;
+  const int slot = blocks[3 * blockIdx.x], first = blocks[3 * blockIdx.x + 1];
+  const int n = blocks[3 * blockIdx.x + 2];
+  const int lane = threadIdx.x & 63, ln = lane & 15, lq = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const AdapterEntry e = p.table[slot];
+  const int steps = p.cols / 32, panels = (e.rank + 15) / 16;
+  const int s0 = steps * wave / kBlockWaves, s1 = steps * (wave + 1) / kBlockWaves;
+  const int t = order[first + min(ln, n - 1)];
+  const uint8_t* row = reinterpret_cast<const uint8_t*>(p.x) + (size_t)t * p.x_stride * (XB ? 2 : 4);
+  const uint16_t* a = p.a + (size_t)slot * p.a_slot + 8 * lane;
+  for (int q0 = 0; q0 < panels; q0 += 4) {
+    f32x4 acc[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) acc[q] = f32x4{0.f, 0.f, 0.f, 0.f};
+    auto sweep = [&](auto count) {
+      constexpr int NQ = decltype(count)::value;
+#pragma unroll 4
+      for (int s = s0; s < s1; ++s) {
+        const auto xv = load_x<XB>(row, 32 * s + 8 * lq);
+#pragma unroll
+        for (int q = 0; q < NQ; ++q)
+          acc[q] = mma_planes(__builtin_bit_cast(bf16x8, ldg16(a + ((size_t)(q0 + q) * steps + s) * 512)),
+                              xv, acc[q]);
+      }
+    };
+    const int nq = min(4, panels - q0);
+    if (nq == 1) sweep(Int<1>{});
+    else if (nq == 2) sweep(Int<2>{});
+    else if (nq == 3) sweep(Int<3>{});
+    else sweep(Int<4>{});
+    __syncthreads();
+#pragma unroll
+    for (int q = 0; q < 4; ++q) red[wave][q][lane] = acc[q];
+    __syncthreads();
+    if (wave < nq && ln < n) {
+      // lane (ln, lq) holds ranks 4 lq + [0, 4) of token ln; the parts of K in order
+      f32x4 v = red[0][wave][lane];
+#pragma unroll
+      for (int z = 1; z < kBlockWaves; ++z) v += red[z][wave][lane];
+      float w[8] = {v[0] * e.scale, v[1] * e.scale, v[2] * e.scale, v[3] * e.scale};
+      const Planes<P> planes = split_planes<P>(w);
+#pragma unroll
+      for (int pl = 0; pl < P; ++pl)
+        *reinterpret_cast<uint2*>(u_planes + ((size_t)t * P + pl) * u_ld + 16 * (q0 + wave) + 4 * lq) =
+            make_uint2(planes.w[pl][0], planes.w[pl][1]);
+    }
+  }
+}
+
+// ---- the second products, added to a tile's accumulators ----
+
+// The slots of a tile's rows (-1: none) and its distinct filled ones, in LDS.
 template <int MAX>
 struct TileSlots {
   int ids[MAX];
   int list[MAX];
   int n;
+  uint32_t seen[4096 / 32];
 };
 template <int MAX>
 __device__ __forceinline__ void find_slots(const ProjArgs& p, int t0, int count, TileSlots<MAX>& s) {
   const int tid = threadIdx.x;
   if (tid == 0) s.n = 0;
+  for (int i = tid; i < 4096 / 32; i += blockDim.x) s.seen[i] = 0;
+  __syncthreads();
   for (int i = tid; i < MAX; i += blockDim.x) {
     int id = i < count ? p.ids[t0 + i] : -1;
     if (id >= p.slots || (id >= 0 && p.table[id].rank == 0)) id = -1;
     s.ids[i] = id;
-  }
-  __syncthreads();
-  for (int i = tid; i < count; i += blockDim.x) {
-    const int id = s.ids[i];
     if (id < 0) continue;
-    bool first = true;
-    for (int j = 0; j < i && first; ++j) first = s.ids[j] != id;
-    // (in any order: every row is in one adapter's product, so the order changes no sum)
-    if (first) s.list[atomicAdd(&s.n, 1)] = id;
+    const uint32_t bit = 1u << (id & 31);
+    if (!(atomicOr(&s.seen[id >> 5], bit) & bit)) s.list[atomicAdd(&s.n, 1)] = id;
   }
   __syncthreads();
 }
 
-// acc (lane (ln, lq): rows 16 panel + 4 lq + [0, 4) of token `local`, at `t`) += the adapters' parts.
-template <int P, int MAX>
-__device__ __forceinline__ void add_adapters(const ProjArgs& p, const TileSlots<MAX>& s, int u_ld,
-                                             int slices, int panel, int local, int t, f32x4& acc) {
+// The B operands of `units` rank units from r on, of a panel (zero past the last).
+__device__ __forceinline__ bf16x8 load_up(const uint16_t* b, int r, int units) {
   const int lane = threadIdx.x & 63, lq = lane >> 4;
-  const int mine = s.ids[local];
+  uint4 w = make_uint4(0, 0, 0, 0);
+  if (r + lq < units) w = ldg16(b + (size_t)r * 128 + 8 * lane);
+  return __builtin_bit_cast(bf16x8, w);
+}
+
+// acc[q][m] (lane (ln, lq): rows 16 (panel0 + q) + 4 lq + [0, 4) of the tile's row first + 16 m + ln) +=
+// the adapters' parts, from the planes of shrink_block_kernel.
+template <int P, int MAX, int NP, int MB>
+__device__ __forceinline__ void add_adapters(const ProjArgs& p, const TileSlots<MAX>& s,
+                                             const uint16_t* u_planes, int u_ld, int panel0, int panels,
+                                             int t0, int first, f32x4 (&acc)[NP][MB]) {
+  const int lane = threadIdx.x & 63, ln = lane & 15, lq = lane >> 4;
   for (int i = 0; i < s.n; ++i) {
     const int slot = s.list[i];
-    if (!__ballot(mine == slot)) continue;
+    const int units = (p.table[slot].rank + 7) / 8;
+    const uint16_t* b = p.b + (size_t)slot * p.b_slot;
+    for (int r = 0; r < units; r += 4) {
+      bf16x8 w[NP];
+#pragma unroll
+      for (int q = 0; q < NP; ++q)
+        w[q] = load_up(b + (size_t)min(panel0 + q, panels - 1) * units * 128, r, units);
+#pragma unroll
+      for (int m = 0; m < MB; ++m) {
+        const int local = first + 16 * m + ln;
+        const bool mine = s.ids[local] == slot;
+        if (!__ballot(mine)) continue;
+        bf16x8 v[P];
+#pragma unroll
+        for (int pl = 0; pl < P; ++pl) {
+          uint4 x = make_uint4(0, 0, 0, 0);
+          if (mine && r + lq < units)
+            x = ldg16(u_planes + ((size_t)(t0 + local) * P + pl) * u_ld + 8 * (r + lq));
+          v[pl] = __builtin_bit_cast(bf16x8, x);
+        }
+#pragma unroll
+        for (int q = 0; q < NP; ++q)
+#pragma unroll
+          for (int pl = 0; pl < P; ++pl) acc[q][m] = mfma(w[q], v[pl], acc[q][m]);
+      }
+    }
+  }
+}
+
+// The same from the partial sums of shrink_kernel, the slots shared out over a workgroup's waves (which
+// add their accumulators up afterwards): slot % waves, so that a row's sum has the same order in any batch.
+template <int P, int MAX, int NP, int MB>
+__device__ __forceinline__ void add_adapter_parts(const ProjArgs& p, const TileSlots<MAX>& s, int u_ld,
+                                                  int slices, int panel0, int panels, int t0, int wave,
+                                                  int waves, f32x4 (&acc)[NP][MB]) {
+  const int lane = threadIdx.x & 63, ln = lane & 15, lq = lane >> 4;
+  for (int i = 0; i < s.n; ++i) {
+    const int slot = __builtin_amdgcn_readfirstlane(s.list[i]);
+    if (slot % waves != wave) continue;
     const AdapterEntry e = p.table[slot];
     const int units = (e.rank + 7) / 8;
-    const uint16_t* b = p.b + (size_t)slot * p.b_slot + (size_t)panel * units * 128;
+    const uint16_t* b = p.b + (size_t)slot * p.b_slot;
     for (int r = 0; r < units; r += 4) {
-      uint4 w = make_uint4(0, 0, 0, 0);
-      float v[8] = {};
-      if (r + lq < units) {
-        w = ldg16(b + (size_t)r * 128 + 8 * lane);
-        if (mine == slot) {
-          const float* u = p.u + (size_t)t * u_ld + 8 * (r + lq);
+      bf16x8 w[NP];
+#pragma unroll
+      for (int q = 0; q < NP; ++q)
+        w[q] = load_up(b + (size_t)min(panel0 + q, panels - 1) * units * 128, r, units);
+#pragma unroll
+      for (int m = 0; m < MB; ++m) {
+        const int local = 16 * m + ln;
+        const bool mine = s.ids[local] == slot;
+        if (!__ballot(mine)) continue;
+        float v[8] = {};
+        if (mine && r + lq < units) {
+          const float* u = p.u + (size_t)(t0 + local) * u_ld + 8 * (r + lq);
+#pragma unroll 4
           for (int z = 0; z < slices; ++z) {
             const float4 c = *reinterpret_cast<const float4*>(u);
             const float4 d = *reinterpret_cast<const float4*>(u + 4);
@@ -245,12 +426,14 @@ __device__ __forceinline__ void add_adapters(const ProjArgs& p, const TileSlots<
             u += (size_t)p.tokens * u_ld;
           }
         }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] *= e.scale;
+        const Planes<P> uv = split_planes<P>(v);
+#pragma unroll
+        for (int q = 0; q < NP; ++q)
+#pragma unroll
+          for (int pl = 0; pl < P; ++pl) acc[q][m] = mfma(w[q], uv.operand(pl), acc[q][m]);
       }
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] *= e.scale;
-      const Planes<P> uv = split_planes<P>(v);
-#pragma unroll
-      for (int q = 0; q < P; ++q) acc = mfma(__builtin_bit_cast(bf16x8, w), uv.operand(q), acc);
     }
   }
 }
@@ -314,20 +497,37 @@ __global__ __launch_bounds__(64 * kSplitWaves) void split_kernel(ProjArgs p, int
   for (int q = 0; q < NP; ++q)
 #pragma unroll
     for (int m = 0; m < MB; ++m) acc[q][m] = f32x4{0.f, 0.f, 0.f, 0.f};
-  for (int s = s0; s < s1; ++s) {
-    BRaw<FMT> r[NP];
+  // weights DW steps ahead, in a ring
+  constexpr int DW = 2, R = DW + 1;
+  BRaw<FMT> ring[R][NP];
+  auto fetch = [&](int slot, int s) {
 #pragma unroll
-    for (int q = 0; q < NP; ++q) load_b<FMT>(r[q], pd[q], 16u * lane, ps[q], lane, s);
+    for (int q = 0; q < NP; ++q) load_b<FMT>(ring[slot][q], pd[q], 16u * lane, ps[q], lane, s);
+  };
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      bf16x8 w[NP];
+  for (int d = 0; d < DW; ++d)
+    if (s0 + d < s1) fetch(d, s0 + d);
+  if (p.ids) {
+    find_slots(p, t0, count, slots);
+    add_adapter_parts<YB ? 2 : 3>(p, slots, u_ld, slices, panel0, panels, t0, wave, kSplitWaves, acc);
+  }
+  for (int i0 = s0; i0 < s1; i0 += R) {
 #pragma unroll
-      for (int q = 0; q < NP; ++q) w[q] = decode_b<FMT>(r[q], j);
+    for (int d = 0; d < R; ++d) {
+      const int s = i0 + d;
+      if (s >= s1) break;
+      if (s + DW < s1) fetch((d + DW) % R, s + DW);
 #pragma unroll
-      for (int m = 0; m < MB; ++m) {
-        const auto xv = load_x<XB>(row[m], kGemmKStep * s + frag_k<FMT>(j, lq));
+      for (int j = 0; j < 4; ++j) {
+        bf16x8 w[NP];
 #pragma unroll
-        for (int q = 0; q < NP; ++q) acc[q][m] = mma_planes(w[q], xv, acc[q][m]);
+        for (int q = 0; q < NP; ++q) w[q] = decode_b<FMT>(ring[d][q], j);
+#pragma unroll
+        for (int m = 0; m < MB; ++m) {
+          const auto xv = load_x<XB>(row[m], kGemmKStep * s + frag_k<FMT>(j, lq));
+#pragma unroll
+          for (int q = 0; q < NP; ++q) acc[q][m] = mma_planes(w[q], xv, acc[q][m]);
+        }
       }
     }
   }
@@ -335,7 +535,6 @@ __global__ __launch_bounds__(64 * kSplitWaves) void split_kernel(ProjArgs p, int
   for (int q = 0; q < NP; ++q)
 #pragma unroll
     for (int m = 0; m < MB; ++m) red[wave][q * MB + m][lane] = acc[q][m];
-  if (p.ids) find_slots(p, t0, count, slots);
   __syncthreads();
   for (int i = wave; i < NP * MB; i += kSplitWaves) {
     const int q = i / MB, m = i % MB, panel = panel0 + q;
@@ -344,7 +543,6 @@ __global__ __launch_bounds__(64 * kSplitWaves) void split_kernel(ProjArgs p, int
 #pragma unroll
     for (int z = 1; z < kSplitWaves; ++z) v += red[z][i][lane];  // K parts in order
     const int local = 16 * m + ln, t = t0 + local;
-    if (p.ids) add_adapters<YB ? 2 : 3>(p, slots, u_ld, slices, panel, local, t, v);
     if (local < count) store_y<YB>(p, t, panel * kPanelRows + 4 * lq, v);
   }
 }
@@ -390,8 +588,8 @@ __device__ __forceinline__ bf16x8 tile_operand(const uint4& q, float sc, int par
   }
 }
 
-// Rows in BF16 planes: plane i of row t at x + i * plane + t * x_stride; `planes`: how many of them each
-// row needs (NULL: one).
+// Rows in BF16 planes: plane i of row t is `plane` bytes after plane i - 1 of it; `planes`: how many of them
+// each row needs (NULL: one).
 struct TileRows {
   size_t plane;
   const int* planes;
@@ -419,7 +617,7 @@ struct TileGrid {
 
 template <int FMT, bool YB, int WM, int WN, int MB, int NP>
 __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(
-    ProjArgs p, TileRows rows, int u_ld, int slices, TileGrid grid) {
+    ProjArgs p, TileRows rows, const uint16_t* u_planes, int u_ld, TileGrid grid) {
   constexpr int WAVES = WM * WN, TM = 16 * WM * MB, TN = WN * NP;  // tokens, panels
   constexpr int COPIES = TM * 16 / (64 * WAVES), HALF = COPIES / 2;  // per thread and step
   constexpr int SL = tile_slabs<FMT>(), PARTS = 4 / SL;
@@ -569,7 +767,10 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(
     advance(Int<1>{}, x1, x0);
     if (s == steps) break;
   }
-  if (p.ids) find_slots(p, t0, count, slots);
+  if (p.ids) {
+    find_slots(p, t0, count, slots);
+    add_adapters<YB ? 2 : 3>(p, slots, u_planes, u_ld, panel0, panels, t0, wm * MB * 16, acc);
+  }
 #pragma unroll
   for (int m = 0; m < MB; ++m) {
     const int local = (wm * MB + m) * 16 + ln, t = t0 + local;
@@ -578,9 +779,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(
     for (int q = 0; q < NP; ++q) {
       const int panel = panel0 + q;
       if (panel >= panels) break;
-      f32x4 v = acc[q][m];
-      if (p.ids) add_adapters<YB ? 2 : 3>(p, slots, u_ld, slices, panel, local, t, v);
-      if (local < count) store_y<YB>(p, t, panel * kPanelRows + 4 * lq, v);
+      if (local < count) store_y<YB>(p, t, panel * kPanelRows + 4 * lq, acc[q][m]);
     }
   }
 }
@@ -641,7 +840,8 @@ template <int FMT>
 constexpr double kWeightBits = FMT == kFmtBF16 ? 16 : FMT == kFmtMXFP8 ? 8.25 : 4.25;
 
 template <int FMT, bool YB>
-void launch_tiles(const ProjArgs& p, const TileRows& rows, int u_ld, int slices, hipStream_t s) {
+void launch_tiles(const ProjArgs& p, const TileRows& rows, const uint16_t* u_planes, int u_ld,
+                  hipStream_t s) {
   const int panels = p.rows / kPanelRows;
   auto go = [&](auto wm, auto wn, auto mb, auto np) {
     constexpr int WM = decltype(wm)::value, WN = decltype(wn)::value, MB = decltype(mb)::value,
@@ -670,7 +870,7 @@ void launch_tiles(const ProjArgs& p, const TileRows& rows, int u_ld, int slices,
 #endif
     grid.band = std::min(BAND, grid.tall());
     const int blocks = 8 * grid.tall() * grid.wide();
-    tile_kernel<FMT, YB, WM, WN, MB, NP><<<blocks, 64 * WM * WN, 0, s>>>(p, rows, u_ld, slices, grid);
+    tile_kernel<FMT, YB, WM, WN, MB, NP><<<blocks, 64 * WM * WN, 0, s>>>(p, rows, u_planes, u_ld, grid);
   };
 #ifdef TILEB
   go(Int<2>{}, Int<2>{}, Int<4>{}, Int<4>{});
@@ -691,36 +891,141 @@ void launch_shrink(const ProjArgs& p, int u_ld, int slices, hipStream_t s) {
   else shrink_kernel<XB, false><<<grid, kThreads, 0, s>>>(p, u_ld, slices);
 }
 
-template <int FMT>
-void launch_types(const ProjArgs& p, int u_ld, int slices, hipStream_t s) {
-  if (p.x_bf16 && p.tokens >= 256 && p.x_stride < (1u << 22)) {
-    const TileRows rows{0, nullptr};
-    if (p.y_bf16) launch_tiles<FMT, true>(p, rows, u_ld, slices, s);
-    else launch_tiles<FMT, false>(p, rows, u_ld, slices, s);
-    return;
+// f32 rows as planes [3][tokens][cols], and how many of them each row needs (1: its values are BF16).
+__global__ __launch_bounds__(256) void planes_kernel(const float* __restrict__ x, size_t x_stride,
+                                                     int tokens, int cols, uint16_t* __restrict__ planes,
+                                                     int* __restrict__ needed) {
+  const int t = blockIdx.x;
+  const uint8_t* row = reinterpret_cast<const uint8_t*>(x + (size_t)t * x_stride);
+  bool more = false;
+  for (int c = 8 * threadIdx.x; c < cols; c += 8 * 256) {
+    const Planes<3> v = load_x<false>(row, c);
+#pragma unroll
+    for (int pl = 0; pl < 3; ++pl)
+      *reinterpret_cast<uint4*>(planes + ((size_t)pl * tokens + t) * cols + c) =
+          make_uint4(v.w[pl][0], v.w[pl][1], v.w[pl][2], v.w[pl][3]);
+    more |= (v.w[1][0] | v.w[1][1] | v.w[1][2] | v.w[1][3]) != 0;
   }
-  if (p.x_bf16) {
-    if (p.y_bf16) launch_rows<FMT, true, true>(p, u_ld, slices, s);
-    else launch_rows<FMT, true, false>(p, u_ld, slices, s);
+  more = __syncthreads_or(more);
+  if (threadIdx.x == 0) needed[t] = more ? 3 : 1;
+}
+
+// What a call's launches share: the rows in planes where x is f32, the first products, their leading
+// dimension and slices.
+struct Pass {
+  bool tiles;
+  TileRows rows;
+  const uint16_t* u_planes;
+  int u_ld, slices;
+};
+
+template <int FMT>
+void launch_types(const ProjArgs& p, const Pass& a, hipStream_t s) {
+  if (a.tiles) {
+    if (p.y_bf16) launch_tiles<FMT, true>(p, a.rows, a.u_planes, a.u_ld, s);
+    else launch_tiles<FMT, false>(p, a.rows, a.u_planes, a.u_ld, s);
+  } else if (p.x_bf16) {
+    if (p.y_bf16) launch_rows<FMT, true, true>(p, a.u_ld, a.slices, s);
+    else launch_rows<FMT, true, false>(p, a.u_ld, a.slices, s);
   } else {
-    if (p.y_bf16) launch_rows<FMT, false, true>(p, u_ld, slices, s);
-    else launch_rows<FMT, false, false>(p, u_ld, slices, s);
+    if (p.y_bf16) launch_rows<FMT, false, true>(p, a.u_ld, a.slices, s);
+    else launch_rows<FMT, false, false>(p, a.u_ld, a.slices, s);
   }
 }
 
+// Most blocks of 16 rows of one adapter.
+int order_blocks(int tokens, int slots) { return tokens / 16 + std::min(tokens, slots); }
+
+// The workspace of a pass: the adapters' first products (a call of few tokens: partial sums in f32; of
+// many: planes, the order and its blocks), then f32 rows' planes and their counts.
+struct WorkLayout {
+  size_t u, order, n_blocks, blocks, planes, needed, total;
+  WorkLayout(int tokens, int slots, int max_rank, int cols, bool x_bf16) {
+    const size_t u_ld = 16 * rank_panels(max_rank);
+    size_t at = 0;
+    auto take = [&](size_t bytes) {
+      const size_t here = at;
+      at += (bytes + 255) / 256 * 256;
+      return here;
+    };
+    u = take(slots ? std::max((size_t)kMaxSlices * std::min(tokens, kTileTokens - 1) * u_ld * 4,
+                              tokens * u_ld * 6)
+                   : 0);
+    order = take(slots ? (size_t)tokens * 4 : 0);
+    n_blocks = take(16);
+    blocks = take(slots ? (size_t)order_blocks(tokens, slots) * 12 : 0);
+    const bool split = !x_bf16 && tokens >= kTileTokens;
+    planes = take(split ? (size_t)tokens * cols * 6 : 0);
+    needed = take(split ? (size_t)tokens * 4 : 0);
+    total = at;
+  }
+};
+
 }  // namespace
 
+int proj_pass_tokens(bool x_bf16) { return x_bf16 ? 8192 : 2048; }
+
+size_t proj_work_bytes(int max_tokens, int slots, int max_rank, int cols, bool x_bf16) {
+  const int tokens = std::min(max_tokens, proj_pass_tokens(x_bf16));
+  return WorkLayout(tokens, slots, max_rank, cols, x_bf16).total;
+}
+
 void launch_project(const ProjArgs& p, hipStream_t s) {
-  const int u_ld = 16 * rank_panels(p.max_rank);
-  int slices = 1;
-  if (p.ids) {
-    slices = std::min(kMaxSlices, std::max(1, p.cols / 512));
-    if (p.x_bf16) launch_shrink<true>(p, u_ld, slices, s);
-    else launch_shrink<false>(p, u_ld, slices, s);
+  // (tiles address their rows by 32-bit offsets: a wider stride takes passes of few rows)
+  const bool tiles = p.tokens >= kTileTokens && p.x_stride < (1u << 22);
+  const int most = tiles ? proj_pass_tokens(p.x_bf16) : kTileTokens - 1;
+  if (p.tokens > most) {
+    for (int t = 0; t < p.tokens; t += most) {
+      ProjArgs q = p;
+      q.tokens = std::min(most, p.tokens - t);
+      q.x = static_cast<const char*>(p.x) + (size_t)t * p.x_stride * (p.x_bf16 ? 2 : 4);
+      q.y = static_cast<char*>(p.y) + (size_t)t * p.y_stride * (p.y_bf16 ? 2 : 4);
+      if (p.ids) q.ids = p.ids + t;
+      launch_project(q, s);
+    }
+    return;
   }
-  if (p.format == kFmtBF16) launch_types<kFmtBF16>(p, u_ld, slices, s);
-  else if (p.format == kFmtMXFP4) launch_types<kFmtMXFP4>(p, u_ld, slices, s);
-  else launch_types<kFmtMXFP8>(p, u_ld, slices, s);
+  const WorkLayout w(p.tokens, p.slots, p.max_rank, p.cols, p.x_bf16);
+  char* const work = static_cast<char*>(p.work);
+  ProjArgs q = p;
+  q.u = reinterpret_cast<float*>(work + w.u);
+  Pass a{tiles, {0, nullptr}, nullptr, 16 * rank_panels(p.max_rank), 1};
+  if (p.ids && tiles) {
+    uint16_t* const u_planes = reinterpret_cast<uint16_t*>(work + w.u);
+    int* const order = reinterpret_cast<int*>(work + w.order);
+    int* const blocks = reinterpret_cast<int*>(work + w.blocks);
+    int* const n_blocks = reinterpret_cast<int*>(work + w.n_blocks);
+    a.u_planes = u_planes;
+    order_kernel<<<1, kOrderThreads, 0, s>>>(p, order, blocks, n_blocks);
+    const int grid = std::max(1, order_blocks(p.tokens, p.slots));
+    auto go = [&](auto xb, auto planes) {
+      shrink_block_kernel<decltype(xb)::value, decltype(planes)::value>
+          <<<grid, 64 * kBlockWaves, 0, s>>>(p, order, blocks, n_blocks, u_planes, a.u_ld);
+    };
+    if (p.x_bf16) {
+      if (p.y_bf16) go(std::true_type{}, Int<2>{});
+      else go(std::true_type{}, Int<3>{});
+    } else {
+      if (p.y_bf16) go(std::false_type{}, Int<2>{});
+      else go(std::false_type{}, Int<3>{});
+    }
+  } else if (p.ids) {
+    a.slices = std::min(kMaxSlices, std::max(1, p.cols / 512));
+    if (p.x_bf16) launch_shrink<true>(q, a.u_ld, a.slices, s);
+    else launch_shrink<false>(q, a.u_ld, a.slices, s);
+  }
+  if (tiles && !p.x_bf16) {
+    uint16_t* const planes = reinterpret_cast<uint16_t*>(work + w.planes);
+    int* const needed = reinterpret_cast<int*>(work + w.needed);
+    planes_kernel<<<p.tokens, 256, 0, s>>>(static_cast<const float*>(p.x), p.x_stride, p.tokens, p.cols,
+                                           planes, needed);
+    q.x = planes;
+    q.x_stride = p.cols;
+    a.rows = TileRows{(size_t)p.tokens * p.cols * 2, needed};
+  }
+  if (p.format == kFmtBF16) launch_types<kFmtBF16>(q, a, s);
+  else if (p.format == kFmtMXFP4) launch_types<kFmtMXFP4>(q, a, s);
+  else launch_types<kFmtMXFP8>(q, a, s);
 }
 
 void launch_set_adapter(const uint16_t* a, const uint16_t* b, int rank, float scale, int rows,

@@ -80,13 +80,13 @@ struct ProjArgs {
   const uint16_t* a;      // slot i at a + i * a_slot
   const uint16_t* b;
   size_t a_slot, b_slot;  // values
-  float* u;               // [slices][tokens][16 * rank_panels(max_rank)]
+  void* work;             // proj_work_bytes
+  float* u;               // (set by launch_project: partial first products [slices][tokens][..])
   int* status;
 };
-// Most K slices of the adapters' first product (the rows of ProjArgs::u a workspace must hold).
-constexpr int kMaxSlices = 16;
 // Tokens per pass of a call (longer calls run in passes of this many).
-constexpr int kProjChunk = 8192;
+int proj_pass_tokens(bool x_bf16);
+size_t proj_work_bytes(int max_tokens, int slots, int max_rank, int cols, bool x_bf16);
 void launch_project(const ProjArgs& a, hipStream_t s);
 // Lays an adapter out in its slot and enters it in the table.
 void launch_set_adapter(const uint16_t* a, const uint16_t* b, int rank, float scale, int rows,

@@ -49,7 +49,7 @@ struct urb_proj_ctx {
   int device = 0;
   void* weights = nullptr;   // own copy, panel layout
   void* adapters = nullptr;  // A and B of every slot
-  void* work = nullptr;      // table, status words, first products
+  void* work = nullptr;      // status words, table, a pass's workspace
   size_t weight_bytes = 0, adapter_bytes = 0, work_bytes = 0;
   const uint8_t* data = nullptr;
   const uint8_t* scales = nullptr;
@@ -58,7 +58,7 @@ struct urb_proj_ctx {
   size_t a_slot = 0, b_slot = 0;
   int* status = nullptr;  // [0] latched failures, [1] an adapter being entered, [2] validation
   urb::AdapterEntry* table = nullptr;
-  float* u = nullptr;
+  void* pass = nullptr;
 };
 
 struct urb_sampler {
@@ -94,20 +94,18 @@ urb_status create_proj(const urb_proj_desc* d, const urb_matrix* w, urb_weight_s
   const size_t scale_bytes = mx ? rows * (cols / 32) : 0;
   URB_HIP(hipGetDevice(&c->device));
   c->desc = *d;
-  // ---- table, status words and the adapters' first products
+  // ---- table, status words and what a pass holds between its launches
   const size_t slots = d->adapter_slots;
-  const size_t chunk = std::min<size_t>(d->max_tokens, urb::kProjChunk);
-  const size_t u_floats =
-      slots ? (size_t)urb::kMaxSlices * chunk * 16 * urb::rank_panels((int)d->max_rank) : 0;
   const size_t table_at = align_up(4 * sizeof(int));
-  const size_t u_at = table_at + align_up(slots * sizeof(urb::AdapterEntry));
-  c->work_bytes = u_at + align_up(u_floats * sizeof(float));
+  const size_t pass_at = table_at + align_up(slots * sizeof(urb::AdapterEntry));
+  c->work_bytes = pass_at + urb::proj_work_bytes((int)d->max_tokens, (int)slots, (int)d->max_rank,
+                                                 (int)cols, d->x_dtype == URB_DTYPE_BF16);
   URB_HIP(hipMalloc(&c->work, c->work_bytes));
   char* work = static_cast<char*>(c->work);
   c->status = reinterpret_cast<int*>(work);
   c->table = reinterpret_cast<urb::AdapterEntry*>(work + table_at);
-  c->u = reinterpret_cast<float*>(work + u_at);
-  urb::launch_fill_i32(c->status, 0, u_at / 4, nullptr);
+  c->pass = work + pass_at;
+  urb::launch_fill_i32(c->status, 0, pass_at / 4, nullptr);
   if (slots) {
     c->a_slot = (size_t)urb::rank_panels((int)d->max_rank) * 16 * cols;
     c->b_slot = rows * urb::rank_units((int)d->max_rank) * urb::kRankUnit;
@@ -251,8 +249,6 @@ urb_status urb_proj_forward(urb_proj_ctx* c, const void* x, uint64_t x_stride,
   if (reinterpret_cast<uintptr_t>(x) % 16 || x_stride * xb % 16 ||
       reinterpret_cast<uintptr_t>(y) % yb)
     return URB_ERR_ARGUMENT;
-  // adapters in use need slots: without any, every id is out of range
-  const bool adapters = adapter_ids != nullptr;
   urb::ProjArgs p{};
   p.format = (int)d.format;
   p.rows = (int)d.rows;
@@ -270,15 +266,13 @@ urb_status urb_proj_forward(urb_proj_ctx* c, const void* x, uint64_t x_stride,
   p.b = c->b;
   p.a_slot = c->a_slot;
   p.b_slot = c->b_slot;
-  p.u = c->u;
+  p.work = c->pass;
   p.status = c->status;
-  for (uint32_t t0 = 0; t0 < tokens; t0 += urb::kProjChunk) {
-    p.tokens = (int)std::min<uint32_t>(urb::kProjChunk, tokens - t0);
-    p.x = static_cast<const char*>(x) + (size_t)t0 * x_stride * xb;
-    p.y = static_cast<char*>(y) + (size_t)t0 * y_stride * yb;
-    p.ids = adapters ? adapter_ids + t0 : nullptr;
-    urb::launch_project(p, static_cast<hipStream_t>(stream));
-  }
+  p.tokens = (int)tokens;
+  p.x = x;
+  p.y = y;
+  p.ids = adapter_ids;
+  urb::launch_project(p, static_cast<hipStream_t>(stream));
   URB_HIP(hipGetLastError());
   return URB_OK;
 }
