@@ -22,7 +22,10 @@ namespace urb {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kTileTokens = 256;  // rows of a call that takes tiles
+#ifndef TT
+#define TT 33
+#endif
+constexpr int kTileTokens = TT;   // rows of a call that takes tiles
 constexpr int kMaxSlices = 16;    // most K slices of the first product for few tokens
 
 // v as BF16 planes by truncation, v = hi + mid + lo exactly (v finite and not subnormal in the
@@ -195,31 +198,65 @@ __global__ __launch_bounds__(kThreads) void shrink_kernel(ProjArgs p, int u_ld, 
 
 constexpr int kOrderThreads = 1024;
 
+// Adds one to count[id] for every lane with id >= 0; returns what was there before the lane's own (lanes of
+// one id get consecutive values).  Ids that many lanes share, as in a batch sorted by request, are
+// counted by one atomic: 64 on one address take turns.
+__device__ __forceinline__ int count_up(int* count, int id) {
+  const int lane = threadIdx.x & 63;
+  int at = 0;
+  for (int round = 0; round < 4; ++round) {
+    const uint64_t open = __ballot(id >= 0);
+    if (!open) return at;
+    const int some = __shfl(id, __ffsll((unsigned long long)open) - 1, 64);
+    const uint64_t same = __ballot(id == some);
+    if (__popcll(same) < 8) break;
+    int first = 0;
+    if (lane == __ffsll((unsigned long long)same) - 1) first = atomicAdd(&count[some], __popcll(same));
+    first = __shfl(first, __ffsll((unsigned long long)same) - 1, 64);
+    if (id == some) {
+      at = first + __popcll(same & ((1ull << lane) - 1));
+      id = -1;
+    }
+  }
+  return id >= 0 ? atomicAdd(&count[id], 1) : at;
+}
+
 // The rows in order of their adapters, and the blocks of up to 16 rows of one adapter: slot, first place
 // in the order, rows.  One workgroup; `order` holds `tokens` entries, `blocks` (3 ints each) at most
 // order_blocks().  Which row of an adapter comes first is left to chance: no sum goes over rows.
 __global__ __launch_bounds__(kOrderThreads) void order_kernel(ProjArgs p, int* order, int* blocks,
                                                               int* n_blocks) {
-  __shared__ int count[4096];   // rows per slot, then the place of its next one
+  __shared__ int count[4096];   // rows per slot, then the place of its next one (-1: an empty slot)
   __shared__ int waves[2][kOrderThreads / 64];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   for (int i = tid; i < p.slots; i += kOrderThreads) count[i] = 0;
   __syncthreads();
-  for (int t = tid; t < p.tokens; t += kOrderThreads) {
-    const int id = p.ids[t];
-    if (id < 0) continue;
-    if (id < p.slots && p.table[id].rank > 0) atomicAdd(&count[id], 1);
-    else flag(p.status, kStepArgument);
+  bool bad = false;
+  for (int t0 = 0; t0 < p.tokens; t0 += kOrderThreads) {
+    int id = t0 + tid < p.tokens ? p.ids[t0 + tid] : -1;
+    if (id >= p.slots) {
+      bad = true;
+      id = -1;
+    }
+    count_up(count, id);
   }
   __syncthreads();
   // four slots per thread, in order: running sums of rows and of blocks
   int n[4], rows = 0, tiles = 0;
+  bool filled[4];
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    n[j] = 4 * tid + j < p.slots ? count[4 * tid + j] : 0;
+    const int slot = 4 * tid + j;
+    n[j] = slot < p.slots ? count[slot] : 0;
+    filled[j] = n[j] && p.table[slot].rank > 0;
+    if (n[j] && !filled[j]) {
+      bad = true;
+      n[j] = 0;
+    }
     rows += n[j];
     tiles += (n[j] + 15) / 16;
   }
+  if (bad) flag(p.status, kStepArgument);
   int row = rows, tile = tiles;
   for (int o = 1; o < 64; o <<= 1) {
     const int r = __shfl_up(row, o, 64), b = __shfl_up(tile, o, 64);
@@ -242,7 +279,7 @@ __global__ __launch_bounds__(kOrderThreads) void order_kernel(ProjArgs p, int* o
   if (tid == kOrderThreads - 1) *n_blocks = tile + tiles;
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    if (4 * tid + j < p.slots) count[4 * tid + j] = row;
+    if (4 * tid + j < p.slots) count[4 * tid + j] = filled[j] ? row : -1;
     for (int i = 0; i < n[j]; i += 16) {
       blocks[3 * tile] = 4 * tid + j;
       blocks[3 * tile + 1] = row + i;
@@ -252,9 +289,12 @@ __global__ __launch_bounds__(kOrderThreads) void order_kernel(ProjArgs p, int* o
     row += n[j];
   }
   __syncthreads();
-  for (int t = tid; t < p.tokens; t += kOrderThreads) {
-    const int id = p.ids[t];
-    if (id >= 0 && id < p.slots && p.table[id].rank > 0) order[atomicAdd(&count[id], 1)] = t;
+  for (int t0 = 0; t0 < p.tokens; t0 += kOrderThreads) {
+    const int t = t0 + tid;
+    int id = t < p.tokens ? p.ids[t] : -1;
+    if (id >= p.slots || (id >= 0 && count[id] < 0)) id = -1;
+    const int at = count_up(count, id);
+    if (id >= 0) order[at] = t;
   }
 }
 
@@ -588,6 +628,12 @@ __device__ __forceinline__ bf16x8 tile_operand(const uint4& q, float sc, int par
   }
 }
 
+// The adapters' first products: planes (tiles), or the partial sums of shrink_kernel in ProjArgs::u.
+struct FirstProduct {
+  uint16_t* planes;
+  int ld, slices;
+};
+
 // Rows in BF16 planes: plane i of row t is `plane` bytes after plane i - 1 of it; `planes`: how many of them
 // each row needs (NULL: one).
 struct TileRows {
@@ -617,7 +663,7 @@ struct TileGrid {
 
 template <int FMT, bool YB, int WM, int WN, int MB, int NP>
 __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(
-    ProjArgs p, TileRows rows, const uint16_t* u_planes, int u_ld, TileGrid grid) {
+    ProjArgs p, TileRows rows, FirstProduct u, TileGrid grid, float* parts) {
   constexpr int WAVES = WM * WN, TM = 16 * WM * MB, TN = WN * NP;  // tokens, panels
   constexpr int COPIES = TM * 16 / (64 * WAVES), HALF = COPIES / 2;  // per thread and step
   constexpr int SL = tile_slabs<FMT>(), PARTS = 4 / SL;
@@ -634,7 +680,10 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(
   const int t0 = row_tile * TM, count = min(TM, p.tokens - t0);
   const int panels = p.rows / kPanelRows;
   const int panel0 = col_tile * TN + wn * NP;
-  const int steps = p.cols / kTileStep;
+  // this slice's steps
+  const int all_steps = p.cols / kTileStep;
+  const int begin = all_steps * (int)blockIdx.y / (int)gridDim.y;
+  const int steps = all_steps * ((int)blockIdx.y + 1) / (int)gridDim.y - begin;
   const size_t pbytes = kPanelRows * panel_row_bytes<FMT>(p.cols);
   const size_t pscales = (size_t)kPanelRows * (p.cols / 32);
   const uint8_t* pd[NP];
@@ -642,8 +691,8 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(
 #pragma unroll
   for (int q = 0; q < NP; ++q) {  // a panel past the last reads the last again and stores nothing
     const int panel = min(panel0 + q, panels - 1);
-    pd[q] = p.data + panel * pbytes;
-    ps[q] = MX ? p.scales + panel * pscales : nullptr;
+    pd[q] = p.data + panel * pbytes + (size_t)begin * (SL * 1024);
+    ps[q] = MX ? p.scales + panel * pscales + (size_t)begin * 64 : nullptr;
   }
   int planes = 1;
   if (rows.planes) {
@@ -654,7 +703,8 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(
   // this lane's copies: rows 4 (wave + WAVES i) + lane / 16, the same chunk of each
   const int copy_row = 4 * wave + lane / 16;
   const int copy_chunk = (lane & 15) ^ x_swizzle<FMT>(copy_row);
-  const uint8_t* const xt = reinterpret_cast<const uint8_t*>(p.x) + (size_t)t0 * p.x_stride * 2;
+  const uint8_t* const xt = reinterpret_cast<const uint8_t*>(p.x) + (size_t)t0 * p.x_stride * 2 +
+                            (size_t)begin * (2 * kTileStep);
   uint32_t copy_off[COPIES];
 #pragma unroll
   for (int i = 0; i < COPIES; ++i)
@@ -740,7 +790,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(
   };
 
   fetch(slab[0], 0);
-  if constexpr (FMT != kFmtMXFP4) fetch(slab[1], 1);
+  if constexpr (FMT != kFmtMXFP4) fetch(slab[1], 1);  // (a step has two slabs at least)
   fetch_scales(sc[0], 0);
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
@@ -767,9 +817,10 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(
     advance(Int<1>{}, x1, x0);
     if (s == steps) break;
   }
-  if (p.ids) {
+  // the first slice adds the adapters
+  if (p.ids && blockIdx.y == 0) {
     find_slots(p, t0, count, slots);
-    add_adapters<YB ? 2 : 3>(p, slots, u_planes, u_ld, panel0, panels, t0, wm * MB * 16, acc);
+    add_adapters<YB ? 2 : 3>(p, slots, u.planes, u.ld, panel0, panels, t0, wm * MB * 16, acc);
   }
 #pragma unroll
   for (int m = 0; m < MB; ++m) {
@@ -779,9 +830,27 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(
     for (int q = 0; q < NP; ++q) {
       const int panel = panel0 + q;
       if (panel >= panels) break;
-      if (local < count) store_y<YB>(p, t, panel * kPanelRows + 4 * lq, acc[q][m]);
+      if (local >= count) continue;
+      const int row = panel * kPanelRows + 4 * lq;
+      if (parts)
+        *reinterpret_cast<f32x4*>(parts + ((size_t)blockIdx.y * p.tokens + t) * p.rows + row) = acc[q][m];
+      else
+        store_y<YB>(p, t, row, acc[q][m]);
     }
   }
+}
+
+// y from the slices' sums, in order; four outputs per thread.
+template <bool YB>
+__global__ __launch_bounds__(256) void join_kernel(ProjArgs p, const float* parts, int slices) {
+  const size_t quads = (size_t)p.tokens * p.rows / 4;
+  const size_t i = blockIdx.x * (size_t)blockDim.x + threadIdx.x;
+  if (i >= quads) return;
+  f32x4 v = reinterpret_cast<const f32x4*>(parts)[i];
+#pragma unroll 4
+  for (int z = 1; z < slices; ++z) v += reinterpret_cast<const f32x4*>(parts)[z * quads + i];
+  const int t = (int)(i / (p.rows / 4));
+  store_y<YB>(p, t, (int)(i - (size_t)t * (p.rows / 4)) * 4, v);
 }
 
 // ---- laying an adapter out ----
@@ -839,46 +908,64 @@ void launch_rows(const ProjArgs& p, int u_ld, int slices, hipStream_t s) {
 template <int FMT>
 constexpr double kWeightBits = FMT == kFmtBF16 ? 16 : FMT == kFmtMXFP8 ? 8.25 : 4.25;
 
+// How a call of many rows is cut: 16-row blocks per tile (of 256 outputs), tiles, and slices of K.
+struct TileShape {
+  int blocks, row_tiles, col_tiles, slices;
+};
+constexpr int kTilePanels = 16;
+TileShape tile_shape(int tokens, int rows, int cols, int planes) {
+  // tiles of equal height, at most 128 rows, an even number of blocks
+  TileShape t{};
+  t.row_tiles = (tokens + 127) / 128;
+  const int blocks = ((tokens + t.row_tiles - 1) / t.row_tiles + 15) / 16;
+  t.blocks = blocks <= 2 ? 2 : (blocks + 1) / 2 * 2;
+  t.row_tiles = (tokens + 16 * t.blocks - 1) / (16 * t.blocks);
+  t.col_tiles = (rows / kPanelRows + kTilePanels - 1) / kTilePanels;
+  // K in slices until the chip has kFill workgroups, of four steps at least
+  const int tiles = t.row_tiles * t.col_tiles, steps = cols / kTileStep;
+#ifndef KFILL
+#define KFILL 384
+#endif
+  t.slices = std::max(1, std::min({KFILL / tiles, steps * planes / 4, steps, kMaxSlices}));
+  return t;
+}
+
 template <int FMT, bool YB>
-void launch_tiles(const ProjArgs& p, const TileRows& rows, const uint16_t* u_planes, int u_ld,
-                  hipStream_t s) {
-  const int panels = p.rows / kPanelRows;
-  auto go = [&](auto wm, auto wn, auto mb, auto np) {
-    constexpr int WM = decltype(wm)::value, WN = decltype(wn)::value, MB = decltype(mb)::value,
-                  NP = decltype(np)::value;
-    TileGrid grid{};
-    grid.cols = (panels + WN * NP - 1) / (WN * NP);
-    grid.rows = (p.tokens + 16 * WM * MB - 1) / (16 * WM * MB);
-    // the cut that leaves an XCD the fewest tiles, then the fewest bytes to read
-    const double row_bytes = 16.0 * WM * MB * 2, col_bytes = 16.0 * WN * NP * kWeightBits<FMT> / 8;
-    long best = -1;
-    double bytes = 0;
-    for (int r = 1; r <= 8; r *= 2) {
-      TileGrid g = grid;
-      g.by_rows = r;
-      g.by_cols = 8 / r;
-      const long tiles = (long)g.tall() * g.wide();
-      const double read = g.tall() * row_bytes + g.wide() * col_bytes;
-      if (best < 0 || tiles < best || (tiles == best && read < bytes)) {
-        best = tiles;
-        bytes = read;
-        grid = g;
-      }
+void launch_tiles(const ProjArgs& p, const TileRows& rows, const FirstProduct& u, const TileShape& t,
+                  float* parts, hipStream_t s) {
+  TileGrid grid{};
+  grid.cols = t.col_tiles;
+  grid.rows = t.row_tiles;
+  // the cut that leaves an XCD the fewest tiles, then the fewest bytes to read
+  const double row_bytes = 16.0 * t.blocks * 2, col_bytes = 16.0 * kTilePanels * kWeightBits<FMT> / 8;
+  long best = -1;
+  double bytes = 0;
+  for (int r = 1; r <= 8; r *= 2) {
+    TileGrid g = grid;
+    g.by_rows = r;
+    g.by_cols = 8 / r;
+    const long tiles = (long)g.tall() * g.wide();
+    const double read = g.tall() * row_bytes + g.wide() * col_bytes;
+    if (best < 0 || tiles < best || (tiles == best && read < bytes)) {
+      best = tiles;
+      bytes = read;
+      grid = g;
     }
-#ifndef BAND
-#define BAND 8
-#endif
-    grid.band = std::min(BAND, grid.tall());
-    const int blocks = 8 * grid.tall() * grid.wide();
-    tile_kernel<FMT, YB, WM, WN, MB, NP><<<blocks, 64 * WM * WN, 0, s>>>(p, rows, u_planes, u_ld, grid);
+  }
+  grid.band = std::min(8, grid.tall());
+  const dim3 blocks(8 * grid.tall() * grid.wide(), t.slices);
+  float* const out = t.slices > 1 ? parts : nullptr;
+  auto go = [&](auto mb) {
+    tile_kernel<FMT, YB, 1, 4, decltype(mb)::value, 4><<<blocks, 256, 0, s>>>(p, rows, u, grid, out);
   };
-#ifdef TILEB
-  go(Int<2>{}, Int<2>{}, Int<4>{}, Int<4>{});
-#elif defined TILEC
-  go(Int<1>{}, Int<4>{}, Int<8>{}, Int<4>{});
-#else
-  go(Int<2>{}, Int<4>{}, Int<8>{}, Int<4>{});
-#endif
+  if (t.blocks == 2) go(Int<2>{});
+  else if (t.blocks == 4) go(Int<4>{});
+  else if (t.blocks == 6) go(Int<6>{});
+  else go(Int<8>{});
+  if (out) {
+    const size_t quads = (size_t)p.tokens * p.rows / 4;
+    join_kernel<YB><<<(unsigned)((quads + 255) / 256), 256, 0, s>>>(p, parts, t.slices);
+  }
 }
 
 template <bool XB>
@@ -891,89 +978,121 @@ void launch_shrink(const ProjArgs& p, int u_ld, int slices, hipStream_t s) {
   else shrink_kernel<XB, false><<<grid, kThreads, 0, s>>>(p, u_ld, slices);
 }
 
-// f32 rows as planes [3][tokens][cols], and how many of them each row needs (1: its values are BF16).
-__global__ __launch_bounds__(256) void planes_kernel(const float* __restrict__ x, size_t x_stride,
-                                                     int tokens, int cols, uint16_t* __restrict__ planes,
-                                                     int* __restrict__ needed) {
+// What tiles need of a row beforehand.  f32 rows (planes not NULL) as planes [3][tokens][cols], and how
+// many of them each row needs (1: its values are BF16).  First products of shrink_kernel (slices > 0):
+// summed over its slices in order, scaled, as the planes that the second product multiplies.
+template <int P>
+__global__ __launch_bounds__(256) void rows_kernel(ProjArgs p, FirstProduct u, uint16_t* planes,
+                                                   int* needed) {
   const int t = blockIdx.x;
-  const uint8_t* row = reinterpret_cast<const uint8_t*>(x + (size_t)t * x_stride);
-  bool more = false;
-  for (int c = 8 * threadIdx.x; c < cols; c += 8 * 256) {
-    const Planes<3> v = load_x<false>(row, c);
+  if (planes) {
+    const uint8_t* row = reinterpret_cast<const uint8_t*>(p.x) + (size_t)t * p.x_stride * 4;
+    bool more = false;
+    for (int c = 8 * threadIdx.x; c < p.cols; c += 8 * 256) {
+      const Planes<3> v = load_x<false>(row, c);
 #pragma unroll
-    for (int pl = 0; pl < 3; ++pl)
-      *reinterpret_cast<uint4*>(planes + ((size_t)pl * tokens + t) * cols + c) =
-          make_uint4(v.w[pl][0], v.w[pl][1], v.w[pl][2], v.w[pl][3]);
-    more |= (v.w[1][0] | v.w[1][1] | v.w[1][2] | v.w[1][3]) != 0;
+      for (int pl = 0; pl < 3; ++pl)
+        *reinterpret_cast<uint4*>(planes + ((size_t)pl * p.tokens + t) * p.cols + c) =
+            make_uint4(v.w[pl][0], v.w[pl][1], v.w[pl][2], v.w[pl][3]);
+      more |= (v.w[1][0] | v.w[1][1] | v.w[1][2] | v.w[1][3]) != 0;
+    }
+    more = __syncthreads_or(more);
+    if (threadIdx.x == 0) needed[t] = more ? 3 : 1;
   }
-  more = __syncthreads_or(more);
-  if (threadIdx.x == 0) needed[t] = more ? 3 : 1;
+  if (u.slices == 0) return;
+  const int id = p.ids[t];
+  if (id < 0 || id >= p.slots) return;
+  const AdapterEntry e = p.table[id];
+  const int r = 8 * threadIdx.x;
+  if (r >= 16 * ((e.rank + 15) / 16)) return;
+  float v[8] = {};
+  const float* from = p.u + (size_t)t * u.ld + r;
+#pragma unroll 4
+  for (int z = 0; z < u.slices; ++z) {
+    const float4 c = *reinterpret_cast<const float4*>(from);
+    const float4 d = *reinterpret_cast<const float4*>(from + 4);
+    v[0] += c.x; v[1] += c.y; v[2] += c.z; v[3] += c.w;
+    v[4] += d.x; v[5] += d.y; v[6] += d.z; v[7] += d.w;
+    from += (size_t)p.tokens * u.ld;
+  }
+#pragma unroll
+  for (int j = 0; j < 8; ++j) v[j] *= e.scale;
+  const Planes<P> out = split_planes<P>(v);
+#pragma unroll
+  for (int pl = 0; pl < P; ++pl)
+    *reinterpret_cast<uint4*>(u.planes + ((size_t)t * P + pl) * u.ld + r) =
+        make_uint4(out.w[pl][0], out.w[pl][1], out.w[pl][2], out.w[pl][3]);
 }
 
-// What a call's launches share: the rows in planes where x is f32, the first products, their leading
-// dimension and slices.
+// What a call's launches share.
 struct Pass {
   bool tiles;
+  TileShape shape;
   TileRows rows;
-  const uint16_t* u_planes;
-  int u_ld, slices;
+  FirstProduct u;
+  float* parts;
 };
 
 template <int FMT>
 void launch_types(const ProjArgs& p, const Pass& a, hipStream_t s) {
   if (a.tiles) {
-    if (p.y_bf16) launch_tiles<FMT, true>(p, a.rows, a.u_planes, a.u_ld, s);
-    else launch_tiles<FMT, false>(p, a.rows, a.u_planes, a.u_ld, s);
+    if (p.y_bf16) launch_tiles<FMT, true>(p, a.rows, a.u, a.shape, a.parts, s);
+    else launch_tiles<FMT, false>(p, a.rows, a.u, a.shape, a.parts, s);
   } else if (p.x_bf16) {
-    if (p.y_bf16) launch_rows<FMT, true, true>(p, a.u_ld, a.slices, s);
-    else launch_rows<FMT, true, false>(p, a.u_ld, a.slices, s);
+    if (p.y_bf16) launch_rows<FMT, true, true>(p, a.u.ld, a.u.slices, s);
+    else launch_rows<FMT, true, false>(p, a.u.ld, a.u.slices, s);
   } else {
-    if (p.y_bf16) launch_rows<FMT, false, true>(p, a.u_ld, a.slices, s);
-    else launch_rows<FMT, false, false>(p, a.u_ld, a.slices, s);
+    if (p.y_bf16) launch_rows<FMT, false, true>(p, a.u.ld, a.u.slices, s);
+    else launch_rows<FMT, false, false>(p, a.u.ld, a.u.slices, s);
   }
 }
 
 // Most blocks of 16 rows of one adapter.
 int order_blocks(int tokens, int slots) { return tokens / 16 + std::min(tokens, slots); }
 
-// The workspace of a pass: the adapters' first products (a call of few tokens: partial sums in f32; of
-// many: planes, the order and its blocks), then f32 rows' planes and their counts.
+// The workspace of a pass: the adapters' first products (up to kScan rows: partial sums in f32; more:
+// planes, the order and its blocks), f32 rows' planes and their counts, the slices' sums.
 struct WorkLayout {
-  size_t u, order, n_blocks, blocks, planes, needed, total;
-  WorkLayout(int tokens, int slots, int max_rank, int cols, bool x_bf16) {
-    const size_t u_ld = 16 * rank_panels(max_rank);
+  size_t u, u_planes, order, n_blocks, blocks, planes, needed, parts, total;
+  WorkLayout(int tokens, const ProjArgs& p) {
+    const size_t u_ld = 16 * rank_panels(p.max_rank);
     size_t at = 0;
     auto take = [&](size_t bytes) {
       const size_t here = at;
       at += (bytes + 255) / 256 * 256;
       return here;
     };
-    u = take(slots ? std::max((size_t)kMaxSlices * std::min(tokens, kTileTokens - 1) * u_ld * 4,
-                              tokens * u_ld * 6)
-                   : 0);
-    order = take(slots ? (size_t)tokens * 4 : 0);
+    const bool few = tokens <= kScan, tiles = tokens >= kTileTokens;
+    u = take(p.slots && few ? tokens * u_ld * 4 * kMaxSlices : 0);
+    u_planes = take(p.slots && tiles ? tokens * u_ld * 6 : 0);
+    order = take(p.slots && !few ? (size_t)tokens * 4 : 0);
     n_blocks = take(16);
-    blocks = take(slots ? (size_t)order_blocks(tokens, slots) * 12 : 0);
-    const bool split = !x_bf16 && tokens >= kTileTokens;
-    planes = take(split ? (size_t)tokens * cols * 6 : 0);
-    needed = take(split ? (size_t)tokens * 4 : 0);
+    blocks = take(p.slots && !few ? (size_t)order_blocks(tokens, p.slots) * 12 : 0);
+    planes = take(!p.x_bf16 && tiles ? (size_t)tokens * p.cols * 6 : 0);
+    needed = take(!p.x_bf16 && tiles ? (size_t)tokens * 4 : 0);
+    const int slices = tiles ? tile_shape(tokens, p.rows, p.cols, p.x_bf16 ? 1 : 3).slices : 1;
+    parts = take(slices > 1 ? (size_t)slices * tokens * p.rows * 4 : 0);
     total = at;
   }
 };
 
+// Tokens per pass of a call (longer calls run in passes of this many): f32 rows are held in planes.
+int pass_tokens(const ProjArgs& p) { return p.x_bf16 ? 8192 : 2048; }
+
 }  // namespace
 
-int proj_pass_tokens(bool x_bf16) { return x_bf16 ? 8192 : 2048; }
-
-size_t proj_work_bytes(int max_tokens, int slots, int max_rank, int cols, bool x_bf16) {
-  const int tokens = std::min(max_tokens, proj_pass_tokens(x_bf16));
-  return WorkLayout(tokens, slots, max_rank, cols, x_bf16).total;
+size_t proj_work_bytes(const ProjArgs& p, int max_tokens) {
+  // (not monotonic in the rows: fewer may take more slices)
+  size_t most = 0;
+  for (int t = 1; t <= std::min(max_tokens, pass_tokens(p)); ++t)
+    most = std::max(most, WorkLayout(t, p).total);
+  return most;
 }
 
 void launch_project(const ProjArgs& p, hipStream_t s) {
   // (tiles address their rows by 32-bit offsets: a wider stride takes passes of few rows)
   const bool tiles = p.tokens >= kTileTokens && p.x_stride < (1u << 22);
-  const int most = tiles ? proj_pass_tokens(p.x_bf16) : kTileTokens - 1;
+  const int most = tiles ? pass_tokens(p) : kTileTokens - 1;
   if (p.tokens > most) {
     for (int t = 0; t < p.tokens; t += most) {
       ProjArgs q = p;
@@ -985,22 +1104,23 @@ void launch_project(const ProjArgs& p, hipStream_t s) {
     }
     return;
   }
-  const WorkLayout w(p.tokens, p.slots, p.max_rank, p.cols, p.x_bf16);
+  const WorkLayout w(p.tokens, p);
   char* const work = static_cast<char*>(p.work);
   ProjArgs q = p;
   q.u = reinterpret_cast<float*>(work + w.u);
-  Pass a{tiles, {0, nullptr}, nullptr, 16 * rank_panels(p.max_rank), 1};
-  if (p.ids && tiles) {
-    uint16_t* const u_planes = reinterpret_cast<uint16_t*>(work + w.u);
+  Pass a{tiles, {}, {0, nullptr},
+         {reinterpret_cast<uint16_t*>(work + w.u_planes), 16 * rank_panels(p.max_rank), 0},
+         reinterpret_cast<float*>(work + w.parts)};
+  if (tiles) a.shape = tile_shape(p.tokens, p.rows, p.cols, p.x_bf16 ? 1 : 3);
+  if (p.ids && p.tokens > kScan) {
     int* const order = reinterpret_cast<int*>(work + w.order);
     int* const blocks = reinterpret_cast<int*>(work + w.blocks);
     int* const n_blocks = reinterpret_cast<int*>(work + w.n_blocks);
-    a.u_planes = u_planes;
     order_kernel<<<1, kOrderThreads, 0, s>>>(p, order, blocks, n_blocks);
     const int grid = std::max(1, order_blocks(p.tokens, p.slots));
     auto go = [&](auto xb, auto planes) {
       shrink_block_kernel<decltype(xb)::value, decltype(planes)::value>
-          <<<grid, 64 * kBlockWaves, 0, s>>>(p, order, blocks, n_blocks, u_planes, a.u_ld);
+          <<<grid, 64 * kBlockWaves, 0, s>>>(p, order, blocks, n_blocks, a.u.planes, a.u.ld);
     };
     if (p.x_bf16) {
       if (p.y_bf16) go(std::true_type{}, Int<2>{});
@@ -1010,18 +1130,20 @@ void launch_project(const ProjArgs& p, hipStream_t s) {
       else go(std::false_type{}, Int<3>{});
     }
   } else if (p.ids) {
-    a.slices = std::min(kMaxSlices, std::max(1, p.cols / 512));
-    if (p.x_bf16) launch_shrink<true>(q, a.u_ld, a.slices, s);
-    else launch_shrink<false>(q, a.u_ld, a.slices, s);
+    a.u.slices = std::min(kMaxSlices, std::max(1, p.cols / 512));
+    if (p.x_bf16) launch_shrink<true>(q, a.u.ld, a.u.slices, s);
+    else launch_shrink<false>(q, a.u.ld, a.u.slices, s);
   }
-  if (tiles && !p.x_bf16) {
-    uint16_t* const planes = reinterpret_cast<uint16_t*>(work + w.planes);
+  if (tiles && (!p.x_bf16 || a.u.slices)) {
+    uint16_t* const planes = p.x_bf16 ? nullptr : reinterpret_cast<uint16_t*>(work + w.planes);
     int* const needed = reinterpret_cast<int*>(work + w.needed);
-    planes_kernel<<<p.tokens, 256, 0, s>>>(static_cast<const float*>(p.x), p.x_stride, p.tokens, p.cols,
-                                           planes, needed);
-    q.x = planes;
-    q.x_stride = p.cols;
-    a.rows = TileRows{(size_t)p.tokens * p.cols * 2, needed};
+    if (p.y_bf16) rows_kernel<2><<<p.tokens, 256, 0, s>>>(q, a.u, planes, needed);
+    else rows_kernel<3><<<p.tokens, 256, 0, s>>>(q, a.u, planes, needed);
+    if (planes) {
+      q.x = planes;
+      q.x_stride = p.cols;
+      a.rows = TileRows{(size_t)p.tokens * p.cols * 2, needed};
+    }
   }
   if (p.format == kFmtBF16) launch_types<kFmtBF16>(q, a, s);
   else if (p.format == kFmtMXFP4) launch_types<kFmtMXFP4>(q, a, s);

@@ -84,9 +84,8 @@ struct ProjArgs {
   float* u;               // (set by launch_project: partial first products [slices][tokens][..])
   int* status;
 };
-// Tokens per pass of a call (longer calls run in passes of this many).
-int proj_pass_tokens(bool x_bf16);
-size_t proj_work_bytes(int max_tokens, int slots, int max_rank, int cols, bool x_bf16);
+// The workspace of calls of up to max_tokens rows (of the geometry, types, slots and ranks in p).
+size_t proj_work_bytes(const ProjArgs& p, int max_tokens);
 void launch_project(const ProjArgs& a, hipStream_t s);
 // Lays an adapter out in its slot and enters it in the table.
 void launch_set_adapter(const uint16_t* a, const uint16_t* b, int rank, float scale, int rows,

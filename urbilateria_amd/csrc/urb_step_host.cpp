@@ -84,6 +84,19 @@ struct DeviceBuffer {
   }
 };
 
+// The part of a call's arguments that the context fixes.
+urb::ProjArgs proj_args(const urb_proj_desc& d) {
+  urb::ProjArgs p{};
+  p.format = (int)d.format;
+  p.rows = (int)d.rows;
+  p.cols = (int)d.cols;
+  p.x_bf16 = d.x_dtype == URB_DTYPE_BF16;
+  p.y_bf16 = d.y_dtype == URB_DTYPE_BF16;
+  p.slots = (int)d.adapter_slots;
+  p.max_rank = (int)d.max_rank;
+  return p;
+}
+
 urb_status create_proj(const urb_proj_desc* d, const urb_matrix* w, urb_weight_source source,
                        urb_proj_ctx* c) {
   const size_t rows = d->rows, cols = d->cols;
@@ -98,8 +111,7 @@ urb_status create_proj(const urb_proj_desc* d, const urb_matrix* w, urb_weight_s
   const size_t slots = d->adapter_slots;
   const size_t table_at = align_up(4 * sizeof(int));
   const size_t pass_at = table_at + align_up(slots * sizeof(urb::AdapterEntry));
-  c->work_bytes = pass_at + urb::proj_work_bytes((int)d->max_tokens, (int)slots, (int)d->max_rank,
-                                                 (int)cols, d->x_dtype == URB_DTYPE_BF16);
+  c->work_bytes = pass_at + urb::proj_work_bytes(proj_args(*d), (int)d->max_tokens);
   URB_HIP(hipMalloc(&c->work, c->work_bytes));
   char* work = static_cast<char*>(c->work);
   c->status = reinterpret_cast<int*>(work);
@@ -249,18 +261,11 @@ urb_status urb_proj_forward(urb_proj_ctx* c, const void* x, uint64_t x_stride,
   if (reinterpret_cast<uintptr_t>(x) % 16 || x_stride * xb % 16 ||
       reinterpret_cast<uintptr_t>(y) % yb)
     return URB_ERR_ARGUMENT;
-  urb::ProjArgs p{};
-  p.format = (int)d.format;
-  p.rows = (int)d.rows;
-  p.cols = (int)d.cols;
+  urb::ProjArgs p = proj_args(d);
   p.data = c->data;
   p.scales = c->scales;
-  p.x_bf16 = d.x_dtype == URB_DTYPE_BF16;
-  p.y_bf16 = d.y_dtype == URB_DTYPE_BF16;
   p.x_stride = x_stride;
   p.y_stride = y_stride;
-  p.slots = (int)d.adapter_slots;
-  p.max_rank = (int)d.max_rank;
   p.table = c->table;
   p.a = c->a;
   p.b = c->b;
