@@ -23,7 +23,7 @@ namespace {
 
 constexpr int kThreads = 256;
 #ifndef TT
-#define TT 33
+#define TT 17
 #endif
 constexpr int kTileTokens = TT;   // rows of a call that takes tiles
 constexpr int kMaxSlices = 16;    // most K slices of the first product for few tokens
@@ -197,6 +197,7 @@ __global__ __launch_bounds__(kThreads) void shrink_kernel(ProjArgs p, int u_ld, 
 // ---- u for many tokens: blocks of 16 rows of one adapter ----
 
 constexpr int kOrderThreads = 1024;
+constexpr int kMaxPass = 8192;  // most rows of a pass
 
 // Adds one to count[id] for every lane with id >= 0; returns what was there before the lane's own (lanes of
 // one id get consecutive values).  Ids that many lanes share, as in a batch sorted by request, are
@@ -231,14 +232,22 @@ __global__ __launch_bounds__(kOrderThreads) void order_kernel(ProjArgs p, int* o
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   for (int i = tid; i < p.slots; i += kOrderThreads) count[i] = 0;
   __syncthreads();
+  // (all ids at once: the loads of a loop would wait for the atomics before them)
+  constexpr int PER = kMaxPass / kOrderThreads;
+  int ids[PER];
+#pragma unroll
+  for (int j = 0; j < PER; ++j) {
+    const int t = j * kOrderThreads + tid;
+    ids[j] = t < p.tokens ? p.ids[t] : -1;
+  }
   bool bad = false;
-  for (int t0 = 0; t0 < p.tokens; t0 += kOrderThreads) {
-    int id = t0 + tid < p.tokens ? p.ids[t0 + tid] : -1;
-    if (id >= p.slots) {
+#pragma unroll
+  for (int j = 0; j < PER; ++j) {
+    if (ids[j] >= p.slots) {
       bad = true;
-      id = -1;
+      ids[j] = -1;
     }
-    count_up(count, id);
+    if (j * kOrderThreads < p.tokens) count_up(count, ids[j]);
   }
   __syncthreads();
   // four slots per thread, in order: running sums of rows and of blocks
@@ -289,18 +298,21 @@ __global__ __launch_bounds__(kOrderThreads) void order_kernel(ProjArgs p, int* o
     row += n[j];
   }
   __syncthreads();
-  for (int t0 = 0; t0 < p.tokens; t0 += kOrderThreads) {
-    const int t = t0 + tid;
-    int id = t < p.tokens ? p.ids[t] : -1;
-    if (id >= p.slots || (id >= 0 && count[id] < 0)) id = -1;
+#pragma unroll
+  for (int j = 0; j < PER; ++j) {
+    if (j * kOrderThreads >= p.tokens) break;
+    const int id = ids[j] >= 0 && count[ids[j]] >= 0 ? ids[j] : -1;
     const int at = count_up(count, id);
-    if (id >= 0) order[at] = t;
+    if (id >= 0) order[at] = j * kOrderThreads + tid;
   }
 }
 
-constexpr int kBlockWaves = 8;
+#ifndef KBW
+#define KBW 16
+#endif
+constexpr int kBlockWaves = KBW;
 
-// u of one block, whole: eight waves split K, four 16-rank panels at a time.  Written scaled, in the
+// u of one block, whole: its waves split K, four 16-rank panels at a time.  Written scaled, in the
 // planes that the second product multiplies: u_planes[(t * P + plane) * u_ld + rank].
 template <bool XB, int P>
 __global__ __launch_bounds__(64 * kBlockWaves) void shrink_block_kernel(ProjArgs p, const int* order,
@@ -790,6 +802,8 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(
   };
 
   fetch(slab[0], 0);
+  const bool adapters = p.ids && blockIdx.y == 0;  // the first slice adds them
+  if (adapters) find_slots(p, t0, count, slots);
   if constexpr (FMT != kFmtMXFP4) fetch(slab[1], 1);  // (a step has two slabs at least)
   fetch_scales(sc[0], 0);
 #pragma unroll
@@ -817,11 +831,8 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(
     advance(Int<1>{}, x1, x0);
     if (s == steps) break;
   }
-  // the first slice adds the adapters
-  if (p.ids && blockIdx.y == 0) {
-    find_slots(p, t0, count, slots);
+  if (adapters)
     add_adapters<YB ? 2 : 3>(p, slots, u.planes, u.ld, panel0, panels, t0, wm * MB * 16, acc);
-  }
 #pragma unroll
   for (int m = 0; m < MB; ++m) {
     const int local = (wm * MB + m) * 16 + ln, t = t0 + local;
@@ -910,9 +921,11 @@ constexpr double kWeightBits = FMT == kFmtBF16 ? 16 : FMT == kFmtMXFP8 ? 8.25 : 
 
 // How a call of many rows is cut: 16-row blocks per tile (of 256 outputs), tiles, and slices of K.
 struct TileShape {
-  int blocks, row_tiles, col_tiles, slices;
+  int blocks, panels, row_tiles, col_tiles, slices;
 };
-constexpr int kTilePanels = 16;
+#ifndef TNP
+#define TNP 4
+#endif
 TileShape tile_shape(int tokens, int rows, int cols, int planes) {
   // tiles of equal height, at most 128 rows, an even number of blocks
   TileShape t{};
@@ -920,7 +933,8 @@ TileShape tile_shape(int tokens, int rows, int cols, int planes) {
   const int blocks = ((tokens + t.row_tiles - 1) / t.row_tiles + 15) / 16;
   t.blocks = blocks <= 2 ? 2 : (blocks + 1) / 2 * 2;
   t.row_tiles = (tokens + 16 * t.blocks - 1) / (16 * t.blocks);
-  t.col_tiles = (rows / kPanelRows + kTilePanels - 1) / kTilePanels;
+  t.panels = 4 * TNP;
+  t.col_tiles = (rows / kPanelRows + t.panels - 1) / t.panels;
   // K in slices until the chip has kFill workgroups, of four steps at least
   const int tiles = t.row_tiles * t.col_tiles, steps = cols / kTileStep;
 #ifndef KFILL
@@ -937,7 +951,7 @@ void launch_tiles(const ProjArgs& p, const TileRows& rows, const FirstProduct& u
   grid.cols = t.col_tiles;
   grid.rows = t.row_tiles;
   // the cut that leaves an XCD the fewest tiles, then the fewest bytes to read
-  const double row_bytes = 16.0 * t.blocks * 2, col_bytes = 16.0 * kTilePanels * kWeightBits<FMT> / 8;
+  const double row_bytes = 16.0 * t.blocks * 2, col_bytes = 16.0 * t.panels * kWeightBits<FMT> / 8;
   long best = -1;
   double bytes = 0;
   for (int r = 1; r <= 8; r *= 2) {
@@ -956,7 +970,7 @@ void launch_tiles(const ProjArgs& p, const TileRows& rows, const FirstProduct& u
   const dim3 blocks(8 * grid.tall() * grid.wide(), t.slices);
   float* const out = t.slices > 1 ? parts : nullptr;
   auto go = [&](auto mb) {
-    tile_kernel<FMT, YB, 1, 4, decltype(mb)::value, 4><<<blocks, 256, 0, s>>>(p, rows, u, grid, out);
+    tile_kernel<FMT, YB, 1, 4, decltype(mb)::value, TNP><<<blocks, 256, 0, s>>>(p, rows, u, grid, out);
   };
   if (t.blocks == 2) go(Int<2>{});
   else if (t.blocks == 4) go(Int<4>{});
@@ -1077,7 +1091,7 @@ struct WorkLayout {
 };
 
 // Tokens per pass of a call (longer calls run in passes of this many): f32 rows are held in planes.
-int pass_tokens(const ProjArgs& p) { return p.x_bf16 ? 8192 : 2048; }
+int pass_tokens(const ProjArgs& p) { return p.x_bf16 ? kMaxPass : 2048; }
 
 }  // namespace
 
