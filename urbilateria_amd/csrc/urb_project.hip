@@ -21,12 +21,14 @@ namespace urb {
 
 namespace {
 
-constexpr int kThreads = 256;
 #ifndef TT
 #define TT 17
 #endif
 constexpr int kTileTokens = TT;   // rows of a call that takes tiles
-constexpr int kMaxSlices = 16;    // most K slices of the first product for few tokens
+constexpr int kMaxSlices = 16;    // most slices of K
+
+// __builtin_amdgcn_sched_barrier: VALU, SALU and LDS reads may cross; loads, LDS stores, MFMAs stay.
+constexpr int kHoldLoads = 0x106;
 
 // v as BF16 planes by truncation, v = hi + mid + lo exactly (v finite and not subnormal in the
 // lower planes); an infinity keeps its first plane alone.
@@ -84,6 +86,24 @@ __device__ __forceinline__ Planes<x_planes<XB>()> load_x(const uint8_t* row, int
     return split_planes<3>(v);
   }
 }
+// The same as loaded, for loads ahead of their use.
+template <bool XB>
+struct XRaw {
+  uint4 q[XB ? 1 : 2];
+  __device__ __forceinline__ void load(const uint8_t* row, int k) {
+    q[0] = ldg16(row + (XB ? 2 : 4) * (size_t)k);
+    if constexpr (!XB) q[1] = ldg16(row + 4 * (size_t)k + 16);
+  }
+  __device__ __forceinline__ Planes<x_planes<XB>()> planes() const {
+    if constexpr (XB) {
+      return {{{q[0].x, q[0].y, q[0].z, q[0].w}}};
+    } else {
+      const float4 a = u2f4(q[0]), b = u2f4(q[1]);
+      const float v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+      return split_planes<3>(v);
+    }
+  }
+};
 // acc += w * x over the planes of x that hold anything for some lane.
 template <int P>
 __device__ __forceinline__ f32x4 mma_planes(bf16x8 w, const Planes<P>& x, f32x4 acc) {
@@ -97,107 +117,14 @@ __device__ __forceinline__ f32x4 mma_planes(bf16x8 w, const Planes<P>& x, f32x4 
   return acc;
 }
 
-// ---- u[slice][t] = A x[t] over the slice's part of K, for every row with an adapter ----
+// ---- u = A x for every row with an adapter ----
 
-constexpr int kScan = 512;  // tokens per workgroup of the first product
-
-// grid: (adapter or token, K slice, segment of kScan tokens).  BY_TOKEN: blockIdx.x is a token, whose
-// workgroup computes for all rows of the same adapter if it is the first of them.
-// Four waves split the slice's K; each takes 16 tokens x 64 ranks at a time.
-template <bool XB, bool BY_TOKEN>
-__global__ __launch_bounds__(kThreads) void shrink_kernel(ProjArgs p, int u_ld, int slices) {
-  __shared__ int s_tokens[kScan];
-  __shared__ int s_count[kThreads / 64 + 1];
-  __shared__ f32x4 s_red[3][4][64];
-  const int tid = threadIdx.x, lane = tid & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int first = blockIdx.z * kScan, last = min(first + kScan, p.tokens);
-  int slot;
-  if constexpr (BY_TOKEN) {
-    slot = p.ids[blockIdx.x];
-  } else {
-    slot = blockIdx.x;
-  }
-  // ids that name no adapter: reported once, by the first workgroup of each segment
-  if (blockIdx.x == 0 && blockIdx.y == 0) {
-    for (int t = first + tid; t < last; t += kThreads) {
-      const int id = p.ids[t];
-      if (id >= p.slots || (id >= 0 && p.table[id].rank == 0)) flag(p.status, kStepArgument);
-    }
-  }
-  if (slot < 0 || slot >= p.slots) return;
-  const int rank = p.table[slot].rank;
-  if (rank == 0) return;
-  // this segment's rows of the adapter, in order
-  int n = 0;
-  for (int t0 = first; t0 < last; t0 += kThreads) {
-    const int t = t0 + tid;
-    const bool mine = t < last && p.ids[t] == slot;
-    const uint64_t vote = __ballot(mine);
-    if (lane == 0) s_count[wave] = __popcll(vote);
-    __syncthreads();
-    int at = n;
-    for (int w = 0; w < wave; ++w) at += s_count[w];
-    if (mine) s_tokens[at + __popcll(vote & ((1ull << lane) - 1))] = t;
-    for (int w = 0; w < kThreads / 64; ++w) n += s_count[w];
-    __syncthreads();
-  }
-  if (n == 0) return;
-  if (BY_TOKEN && s_tokens[0] != (int)blockIdx.x) return;
-
-  const int ln = lane & 15, lq = lane >> 4;
-  const int steps = p.cols / 32;
-  // the slice's steps of 32 columns, and the wave's among them
-  const int s0 = (int)((long long)steps * blockIdx.y / slices);
-  const int s1 = (int)((long long)steps * (blockIdx.y + 1) / slices);
-  const int w0 = s0 + (s1 - s0) * wave / 4, w1 = s0 + (s1 - s0) * (wave + 1) / 4;
-  const uint8_t* x = reinterpret_cast<const uint8_t*>(p.x);
-  const size_t xs = p.x_stride * (XB ? 2 : 4);
-  const uint16_t* a = p.a + (size_t)slot * p.a_slot;
-  const int panels = (rank + 15) / 16;
-  float* u = p.u + (size_t)blockIdx.y * p.tokens * u_ld;
-  for (int m = 0; m < n; m += 16) {
-    const bool there = m + ln < n;
-    const int t = s_tokens[there ? m + ln : m];
-    const uint8_t* row = x + (size_t)t * xs;
-    for (int q0 = 0; q0 < panels; q0 += 4) {
-      f32x4 acc[4];
-#pragma unroll
-      for (int q = 0; q < 4; ++q) acc[q] = f32x4{0.f, 0.f, 0.f, 0.f};
-      for (int s = w0; s < w1; ++s) {
-        const auto xv = load_x<XB>(row, 32 * s + 8 * lq);
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          if (q0 + q >= panels) break;
-          uint4 w = make_uint4(0, 0, 0, 0);
-          if (16 * (q0 + q) + ln < rank)
-            w = ldg16(a + ((size_t)(q0 + q) * steps + s) * 512 + 8 * lane);
-          acc[q] = mma_planes(__builtin_bit_cast(bf16x8, w), xv, acc[q]);
-        }
-      }
-      // the waves' parts, in order; lane (ln, lq) holds ranks 4 lq + [0, 4) of token ln
-      __syncthreads();
-      if (wave > 0)
-#pragma unroll
-        for (int q = 0; q < 4; ++q) s_red[wave - 1][q][lane] = acc[q];
-      __syncthreads();
-      if (wave == 0 && there) {
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          if (q0 + q >= panels) break;
-          f32x4 v = acc[q];
-          for (int w = 0; w < 3; ++w) v += s_red[w][q][lane];
-          *reinterpret_cast<f32x4*>(u + (size_t)t * u_ld + 16 * (q0 + q) + 4 * lq) = v;
-        }
-      }
-    }
-  }
-}
-
-// ---- u for many tokens: blocks of 16 rows of one adapter ----
+constexpr int kFew = 64;  // rows whose adapters a wave sorts out by itself
 
 constexpr int kOrderThreads = 1024;
-constexpr int kMaxPass = 8192;  // most rows of a pass
+constexpr int kMaxPass = 8192;   // most rows of a pass
+constexpr int kMaxSlots = 4096;
+static_assert(kMaxSlots == 4 * kOrderThreads, "four slots per thread");
 
 // Adds one to count[id] for every lane with id >= 0; returns what was there before the lane's own (lanes of
 // one id get consecutive values).  Ids that many lanes share, as in a batch sorted by request, are
@@ -227,7 +154,9 @@ __device__ __forceinline__ int count_up(int* count, int id) {
 // order_blocks().  Which row of an adapter comes first is left to chance: no sum goes over rows.
 __global__ __launch_bounds__(kOrderThreads) void order_kernel(ProjArgs p, int* order, int* blocks,
                                                               int* n_blocks) {
-  __shared__ int count[4096];   // rows per slot, then the place of its next one (-1: an empty slot)
+  __shared__ int count[kMaxSlots];  // rows per slot, then the place of its next one (-1: an empty slot)
+  __shared__ int row_at[kMaxSlots + 1], tile_at[kMaxSlots];  // first row and block of each slot
+  __shared__ int s_blocks;
   __shared__ int waves[2][kOrderThreads / 64];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   for (int i = tid; i < p.slots; i += kOrderThreads) count[i] = 0;
@@ -285,19 +214,32 @@ __global__ __launch_bounds__(kOrderThreads) void order_kernel(ProjArgs p, int* o
     row += waves[0][w];
     tile += waves[1][w];
   }
-  if (tid == kOrderThreads - 1) *n_blocks = tile + tiles;
+  if (tid == kOrderThreads - 1) {
+    *n_blocks = tile + tiles;
+    s_blocks = tile + tiles;
+  }
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    if (4 * tid + j < p.slots) count[4 * tid + j] = filled[j] ? row : -1;
-    for (int i = 0; i < n[j]; i += 16) {
-      blocks[3 * tile] = 4 * tid + j;
-      blocks[3 * tile + 1] = row + i;
-      blocks[3 * tile + 2] = min(16, n[j] - i);
-      ++tile;
-    }
+    const int slot = 4 * tid + j;
+    if (slot < p.slots) count[slot] = filled[j] ? row : -1;
+    row_at[slot] = row;
+    tile_at[slot] = tile;
     row += n[j];
+    tile += (n[j] + 15) / 16;
   }
+  if (tid == kOrderThreads - 1) row_at[kMaxSlots] = row;
   __syncthreads();
+  // the slot of each block: the last whose blocks begin at or before it
+  for (int b = tid; b < s_blocks; b += kOrderThreads) {
+    int lo = 0;
+#pragma unroll
+    for (int step = kMaxSlots / 2; step > 0; step /= 2)
+      if (tile_at[lo + step] <= b) lo += step;
+    const int from = row_at[lo] + 16 * (b - tile_at[lo]);
+    blocks[3 * b] = lo;
+    blocks[3 * b + 1] = from;
+    blocks[3 * b + 2] = min(16, row_at[lo + 1] - from);
+  }
 #pragma unroll
   for (int j = 0; j < PER; ++j) {
     if (j * kOrderThreads >= p.tokens) break;
@@ -307,66 +249,115 @@ __global__ __launch_bounds__(kOrderThreads) void order_kernel(ProjArgs p, int* o
   }
 }
 
-#ifndef KBW
-#define KBW 16
-#endif
-constexpr int kBlockWaves = KBW;
+// The adapters' first products, as the planes that the second ones multiply: planes[(t * P + plane) * ld +
+// rank], scaled.
+struct FirstProduct {
+  uint16_t* planes;
+  int ld;
+};
+// What order_kernel found (order NULL: few rows).
+struct Order {
+  const int* order;
+  const int* blocks;
+  const int* n_blocks;
+};
 
-// u of one block, whole: its waves split K, four 16-rank panels at a time.  Written scaled, in the
-// planes that the second product multiplies: u_planes[(t * P + plane) * u_ld + rank].
+constexpr int kPrepareWaves = 16;
+
+// What the products of a call need beforehand, in one launch.  Workgroups below `firsts`: the first product
+// of up to 16 rows of one adapter with up to `per` of its 16-rank panels (per 1 or 4), the waves' parts of K
+// summed in order.  With an order, a workgroup takes a block of it; without, workgroup (who, panels, z)
+// takes the z-th 16 rows of slot `who`, or (by_token) of the slot of row `who` if no row before has it.
+// The others: a row of f32 values each as planes [3][tokens][cols] (x_planes), and how many of them it
+// needs (1: its values are BF16).
 template <bool XB, int P>
-__global__ __launch_bounds__(64 * kBlockWaves) void shrink_block_kernel(ProjArgs p, const int* order,
-                                                                        const int* blocks,
-                                                                        const int* n_blocks,
-                                                                        uint16_t* u_planes, int u_ld) {
-  __shared__ f32x4 red[kBlockWaves][4][64];
-  if ((int)blockIdx.x >= *n_blocks) return;
-  const int slot = blocks[3 * blockIdx.x], first = blocks[3 * blockIdx.x + 1];
-  const int n = blocks[3 * blockIdx.x + 2];
-  const int lane = threadIdx.x & 63, ln = lane & 15, lq = lane >> 4;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+__global__ __launch_bounds__(64 * kPrepareWaves) void prepare_kernel(
+    ProjArgs p, FirstProduct u, Order order, int firsts, int groups, int per, bool by_token,
+    uint16_t* x_planes, int* needed) {
+  __shared__ f32x4 red[kPrepareWaves][4][64];
+  __shared__ int s_rows[kFew];
+  const int tid = threadIdx.x, lane = tid & 63, ln = lane & 15, lq = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  if ((int)blockIdx.x >= firsts) {
+    if constexpr (!XB) {
+      const int t = blockIdx.x - firsts;
+      const uint8_t* row = reinterpret_cast<const uint8_t*>(p.x) + (size_t)t * p.x_stride * 4;
+      bool more = false;
+      for (int c = 8 * tid; c < p.cols; c += 8 * 64 * kPrepareWaves) {
+        const Planes<3> v = load_x<false>(row, c);
+#pragma unroll
+        for (int pl = 0; pl < 3; ++pl)
+          *reinterpret_cast<uint4*>(x_planes + ((size_t)pl * p.tokens + t) * p.cols + c) =
+              make_uint4(v.w[pl][0], v.w[pl][1], v.w[pl][2], v.w[pl][3]);
+        more |= (v.w[1][0] | v.w[1][1] | v.w[1][2] | v.w[1][3]) != 0;
+      }
+      more = __syncthreads_or(more);
+      if (tid == 0) needed[t] = more ? 3 : 1;
+    }
+    return;
+  }
+  const int group = blockIdx.x % groups, unit = blockIdx.x / groups;
+  int slot, n, t;
+  if (order.order) {
+    if (unit >= *order.n_blocks) return;
+    slot = order.blocks[3 * unit];
+    n = order.blocks[3 * unit + 2];
+    t = order.order[order.blocks[3 * unit + 1] + min(ln, n - 1)];
+  } else {
+    const int tiles = (p.tokens + 15) / 16, who = unit / tiles, z = unit % tiles;
+    const int id = lane < p.tokens ? p.ids[lane] : -1;
+    if (blockIdx.x == 0 && wave == 0 && id >= 0 && (id >= p.slots || p.table[id].rank == 0))
+      flag(p.status, kStepArgument);
+    slot = by_token ? __builtin_amdgcn_readlane(id, who) : who;
+    if (slot < 0 || slot >= p.slots) return;
+    const uint64_t same = __ballot(id == slot);
+    if (by_token && __ffsll((unsigned long long)same) - 1 != who) return;
+    n = min(16, (int)__popcll(same) - 16 * z);  // (unsigned, it would never be negative)
+    if (n <= 0) return;
+    if (id == slot) s_rows[__popcll(same & ((1ull << lane) - 1))] = lane;  // (the same from every wave)
+    __syncthreads();
+    t = s_rows[16 * z + min(ln, n - 1)];
+  }
   const AdapterEntry e = p.table[slot];
   const int steps = p.cols / 32, panels = (e.rank + 15) / 16;
-  const int s0 = steps * wave / kBlockWaves, s1 = steps * (wave + 1) / kBlockWaves;
-  const int t = order[first + min(ln, n - 1)];
+  const int q0 = group * per, nq = min(per, panels - q0);
+  if (nq <= 0) return;
+  const int s0 = steps * wave / kPrepareWaves, s1 = steps * (wave + 1) / kPrepareWaves;
   const uint8_t* row = reinterpret_cast<const uint8_t*>(p.x) + (size_t)t * p.x_stride * (XB ? 2 : 4);
   const uint16_t* a = p.a + (size_t)slot * p.a_slot + 8 * lane;
-  for (int q0 = 0; q0 < panels; q0 += 4) {
-    f32x4 acc[4];
+  f32x4 acc[4];
 #pragma unroll
-    for (int q = 0; q < 4; ++q) acc[q] = f32x4{0.f, 0.f, 0.f, 0.f};
-    auto sweep = [&](auto count) {
-      constexpr int NQ = decltype(count)::value;
+  for (int q = 0; q < 4; ++q) acc[q] = f32x4{0.f, 0.f, 0.f, 0.f};
+  auto sweep = [&](auto count) {
+    constexpr int NQ = decltype(count)::value;
 #pragma unroll 4
-      for (int s = s0; s < s1; ++s) {
-        const auto xv = load_x<XB>(row, 32 * s + 8 * lq);
+    for (int s = s0; s < s1; ++s) {
+      const auto xv = load_x<XB>(row, 32 * s + 8 * lq);
 #pragma unroll
-        for (int q = 0; q < NQ; ++q)
-          acc[q] = mma_planes(__builtin_bit_cast(bf16x8, ldg16(a + ((size_t)(q0 + q) * steps + s) * 512)),
-                              xv, acc[q]);
-      }
-    };
-    const int nq = min(4, panels - q0);
-    if (nq == 1) sweep(Int<1>{});
-    else if (nq == 2) sweep(Int<2>{});
-    else if (nq == 3) sweep(Int<3>{});
-    else sweep(Int<4>{});
-    __syncthreads();
-#pragma unroll
-    for (int q = 0; q < 4; ++q) red[wave][q][lane] = acc[q];
-    __syncthreads();
-    if (wave < nq && ln < n) {
-      // lane (ln, lq) holds ranks 4 lq + [0, 4) of token ln; the parts of K in order
-      f32x4 v = red[0][wave][lane];
-#pragma unroll
-      for (int z = 1; z < kBlockWaves; ++z) v += red[z][wave][lane];
-      float w[8] = {v[0] * e.scale, v[1] * e.scale, v[2] * e.scale, v[3] * e.scale};
-      const Planes<P> planes = split_planes<P>(w);
-#pragma unroll
-      for (int pl = 0; pl < P; ++pl)
-        *reinterpret_cast<uint2*>(u_planes + ((size_t)t * P + pl) * u_ld + 16 * (q0 + wave) + 4 * lq) =
-            make_uint2(planes.w[pl][0], planes.w[pl][1]);
+      for (int q = 0; q < NQ; ++q)
+        acc[q] = mma_planes(__builtin_bit_cast(bf16x8, ldg16(a + ((size_t)(q0 + q) * steps + s) * 512)),
+                            xv, acc[q]);
     }
+  };
+  if (nq == 1) sweep(Int<1>{});
+  else if (nq == 2) sweep(Int<2>{});
+  else if (nq == 3) sweep(Int<3>{});
+  else sweep(Int<4>{});
+#pragma unroll
+  for (int q = 0; q < 4; ++q)
+    if (q < nq) red[wave][q][lane] = acc[q];
+  __syncthreads();
+  if (wave < nq && ln < n) {
+    // lane (ln, lq) holds ranks 4 lq + [0, 4) of row ln
+    f32x4 v = red[0][wave][lane];
+#pragma unroll
+    for (int z = 1; z < kPrepareWaves; ++z) v += red[z][wave][lane];
+    const float w[8] = {v[0] * e.scale, v[1] * e.scale, v[2] * e.scale, v[3] * e.scale};
+    const Planes<P> planes = split_planes<P>(w);
+#pragma unroll
+    for (int pl = 0; pl < P; ++pl)
+      *reinterpret_cast<uint2*>(u.planes + ((size_t)t * P + pl) * u.ld + 16 * (q0 + wave) + 4 * lq) =
+          make_uint2(planes.w[pl][0], planes.w[pl][1]);
   }
 }
 
@@ -376,23 +367,25 @@ __global__ __launch_bounds__(64 * kBlockWaves) void shrink_block_kernel(ProjArgs
 template <int MAX>
 struct TileSlots {
   int ids[MAX];
-  int list[MAX];
+  int2 list[MAX];  // slot, rank units
   int n;
-  uint32_t seen[4096 / 32];
+  uint32_t seen[kMaxSlots / 32];
 };
 template <int MAX>
 __device__ __forceinline__ void find_slots(const ProjArgs& p, int t0, int count, TileSlots<MAX>& s) {
   const int tid = threadIdx.x;
   if (tid == 0) s.n = 0;
-  for (int i = tid; i < 4096 / 32; i += blockDim.x) s.seen[i] = 0;
+  for (int i = tid; i < kMaxSlots / 32; i += blockDim.x) s.seen[i] = 0;
   __syncthreads();
   for (int i = tid; i < MAX; i += blockDim.x) {
     int id = i < count ? p.ids[t0 + i] : -1;
-    if (id >= p.slots || (id >= 0 && p.table[id].rank == 0)) id = -1;
+    int rank = 0;
+    if (id >= p.slots || (id >= 0 && (rank = p.table[id].rank) == 0)) id = -1;
     s.ids[i] = id;
     if (id < 0) continue;
     const uint32_t bit = 1u << (id & 31);
-    if (!(atomicOr(&s.seen[id >> 5], bit) & bit)) s.list[atomicAdd(&s.n, 1)] = id;
+    if (!(atomicOr(&s.seen[id >> 5], bit) & bit))
+      s.list[atomicAdd(&s.n, 1)] = make_int2(id, (rank + 7) / 8);
   }
   __syncthreads();
 }
@@ -406,86 +399,60 @@ __device__ __forceinline__ bf16x8 load_up(const uint16_t* b, int r, int units) {
 }
 
 // acc[q][m] (lane (ln, lq): rows 16 (panel0 + q) + 4 lq + [0, 4) of the tile's row first + 16 m + ln) +=
-// the adapters' parts, from the planes of shrink_block_kernel.
+// the adapters' parts.  Of `parts` accumulators that are added up afterwards, each takes the slots with
+// slot % parts == part: a row's sum then has the same order in any batch.  B comes from HBM the first
+// time, so the next operands are loaded before the present ones are used.
 template <int P, int MAX, int NP, int MB>
 __device__ __forceinline__ void add_adapters(const ProjArgs& p, const TileSlots<MAX>& s,
-                                             const uint16_t* u_planes, int u_ld, int panel0, int panels,
-                                             int t0, int first, f32x4 (&acc)[NP][MB]) {
+                                             const FirstProduct& u, int panel0, int panels, int t0,
+                                             int first, int part, int parts, f32x4 (&acc)[NP][MB]) {
   const int lane = threadIdx.x & 63, ln = lane & 15, lq = lane >> 4;
-  for (int i = 0; i < s.n; ++i) {
-    const int slot = s.list[i];
-    const int units = (p.table[slot].rank + 7) / 8;
-    const uint16_t* b = p.b + (size_t)slot * p.b_slot;
-    for (int r = 0; r < units; r += 4) {
-      bf16x8 w[NP];
-#pragma unroll
-      for (int q = 0; q < NP; ++q)
-        w[q] = load_up(b + (size_t)min(panel0 + q, panels - 1) * units * 128, r, units);
-#pragma unroll
-      for (int m = 0; m < MB; ++m) {
-        const int local = first + 16 * m + ln;
-        const bool mine = s.ids[local] == slot;
-        if (!__ballot(mine)) continue;
-        bf16x8 v[P];
-#pragma unroll
-        for (int pl = 0; pl < P; ++pl) {
-          uint4 x = make_uint4(0, 0, 0, 0);
-          if (mine && r + lq < units)
-            x = ldg16(u_planes + ((size_t)(t0 + local) * P + pl) * u_ld + 8 * (r + lq));
-          v[pl] = __builtin_bit_cast(bf16x8, x);
-        }
-#pragma unroll
-        for (int q = 0; q < NP; ++q)
-#pragma unroll
-          for (int pl = 0; pl < P; ++pl) acc[q][m] = mfma(w[q], v[pl], acc[q][m]);
-      }
+  int i = -1, r = 0, slot = 0, units = 0;
+  // the next 32 ranks: of this slot or the next of this part; false past the last
+  auto advance = [&] {
+    r += 4;
+    if (r < units) return true;
+    r = 0;
+    while (++i < s.n) {
+      slot = __builtin_amdgcn_readfirstlane(s.list[i].x);
+      units = __builtin_amdgcn_readfirstlane(s.list[i].y);
+      if (slot % parts == part) return true;
     }
-  }
-}
-
-// The same from the partial sums of shrink_kernel, the slots shared out over a workgroup's waves (which
-// add their accumulators up afterwards): slot % waves, so that a row's sum has the same order in any batch.
-template <int P, int MAX, int NP, int MB>
-__device__ __forceinline__ void add_adapter_parts(const ProjArgs& p, const TileSlots<MAX>& s, int u_ld,
-                                                  int slices, int panel0, int panels, int t0, int wave,
-                                                  int waves, f32x4 (&acc)[NP][MB]) {
-  const int lane = threadIdx.x & 63, ln = lane & 15, lq = lane >> 4;
-  for (int i = 0; i < s.n; ++i) {
-    const int slot = __builtin_amdgcn_readfirstlane(s.list[i]);
-    if (slot % waves != wave) continue;
-    const AdapterEntry e = p.table[slot];
-    const int units = (e.rank + 7) / 8;
+    return false;
+  };
+  auto load = [&](bf16x8* w) {
     const uint16_t* b = p.b + (size_t)slot * p.b_slot;
-    for (int r = 0; r < units; r += 4) {
-      bf16x8 w[NP];
+#pragma unroll
+    for (int q = 0; q < NP; ++q)
+      w[q] = load_up(b + (size_t)min(panel0 + q, panels - 1) * units * 128, r, units);
+  };
+  bf16x8 next[NP];
+  bool more = advance();
+  if (more) load(next);
+  while (more) {
+    bf16x8 w[NP];
+#pragma unroll
+    for (int q = 0; q < NP; ++q) w[q] = next[q];
+    const int now = slot, from = r, to = units;
+    more = advance();
+    if (more) load(next);
+#pragma unroll
+    for (int m = 0; m < MB; ++m) {
+      const int local = first + 16 * m + ln;
+      const bool mine = s.ids[local] == now;
+      if (!__ballot(mine)) continue;
+      bf16x8 v[P];
+#pragma unroll
+      for (int pl = 0; pl < P; ++pl) {
+        uint4 x = make_uint4(0, 0, 0, 0);
+        if (mine && from + lq < to)
+          x = ldg16(u.planes + ((size_t)(t0 + local) * P + pl) * u.ld + 8 * (from + lq));
+        v[pl] = __builtin_bit_cast(bf16x8, x);
+      }
 #pragma unroll
       for (int q = 0; q < NP; ++q)
-        w[q] = load_up(b + (size_t)min(panel0 + q, panels - 1) * units * 128, r, units);
 #pragma unroll
-      for (int m = 0; m < MB; ++m) {
-        const int local = 16 * m + ln;
-        const bool mine = s.ids[local] == slot;
-        if (!__ballot(mine)) continue;
-        float v[8] = {};
-        if (mine && r + lq < units) {
-          const float* u = p.u + (size_t)(t0 + local) * u_ld + 8 * (r + lq);
-#pragma unroll 4
-          for (int z = 0; z < slices; ++z) {
-            const float4 c = *reinterpret_cast<const float4*>(u);
-            const float4 d = *reinterpret_cast<const float4*>(u + 4);
-            v[0] += c.x; v[1] += c.y; v[2] += c.z; v[3] += c.w;
-            v[4] += d.x; v[5] += d.y; v[6] += d.z; v[7] += d.w;
-            u += (size_t)p.tokens * u_ld;
-          }
-        }
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] *= e.scale;
-        const Planes<P> uv = split_planes<P>(v);
-#pragma unroll
-        for (int q = 0; q < NP; ++q)
-#pragma unroll
-          for (int pl = 0; pl < P; ++pl) acc[q][m] = mfma(w[q], uv.operand(pl), acc[q][m]);
-      }
+        for (int pl = 0; pl < P; ++pl) acc[q][m] = mfma(w[q], v[pl], acc[q][m]);
     }
   }
 }
@@ -517,7 +484,7 @@ __device__ __forceinline__ void store_y(const ProjArgs& p, int t, int row, f32x4
 constexpr int kSplitWaves = 8;
 
 template <int FMT, bool XB, bool YB, int MB, int NP>
-__global__ __launch_bounds__(64 * kSplitWaves) void split_kernel(ProjArgs p, int u_ld, int slices) {
+__global__ __launch_bounds__(64 * kSplitWaves) void split_kernel(ProjArgs p, FirstProduct u) {
   constexpr int TILE = 16 * MB;
   __shared__ f32x4 red[kSplitWaves][NP * MB][64];
   __shared__ TileSlots<TILE> slots;
@@ -549,19 +516,29 @@ __global__ __launch_bounds__(64 * kSplitWaves) void split_kernel(ProjArgs p, int
   for (int q = 0; q < NP; ++q)
 #pragma unroll
     for (int m = 0; m < MB; ++m) acc[q][m] = f32x4{0.f, 0.f, 0.f, 0.f};
-  // weights DW steps ahead, in a ring
-  constexpr int DW = 2, R = DW + 1;
+  // Weights DW steps ahead in a ring of R slots, rows one step ahead.  (Rows loaded where they are used
+  // left every step waiting for the L2: 24 rows, MXFP8, 6144 -> 9232 at 27 us.)
+  constexpr int R = FMT == kFmtBF16 ? 2 : 4, DW = R - 1;
   BRaw<FMT> ring[R][NP];
+  XRaw<XB> xr[2][4][MB];
   auto fetch = [&](int slot, int s) {
 #pragma unroll
     for (int q = 0; q < NP; ++q) load_b<FMT>(ring[slot][q], pd[q], 16u * lane, ps[q], lane, s);
   };
+  auto fetch_rows = [&](int half, int s) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int m = 0; m < MB; ++m)
+        xr[half][j][m].load(row[m], kGemmKStep * s + frag_k<FMT>(j, lq));
+  };
 #pragma unroll
   for (int d = 0; d < DW; ++d)
     if (s0 + d < s1) fetch(d, s0 + d);
+  if (s0 < s1) fetch_rows(0, s0);
   if (p.ids) {
     find_slots(p, t0, count, slots);
-    add_adapter_parts<YB ? 2 : 3>(p, slots, u_ld, slices, panel0, panels, t0, wave, kSplitWaves, acc);
+    add_adapters<YB ? 2 : 3>(p, slots, u, panel0, panels, t0, 0, wave, kSplitWaves, acc);
   }
   for (int i0 = s0; i0 < s1; i0 += R) {
 #pragma unroll
@@ -569,6 +546,8 @@ __global__ __launch_bounds__(64 * kSplitWaves) void split_kernel(ProjArgs p, int
       const int s = i0 + d;
       if (s >= s1) break;
       if (s + DW < s1) fetch((d + DW) % R, s + DW);
+      if (s + 1 < s1) fetch_rows((d + 1) & 1, s + 1);
+      __builtin_amdgcn_sched_barrier(kHoldLoads);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         bf16x8 w[NP];
@@ -576,7 +555,7 @@ __global__ __launch_bounds__(64 * kSplitWaves) void split_kernel(ProjArgs p, int
         for (int q = 0; q < NP; ++q) w[q] = decode_b<FMT>(ring[d][q], j);
 #pragma unroll
         for (int m = 0; m < MB; ++m) {
-          const auto xv = load_x<XB>(row[m], kGemmKStep * s + frag_k<FMT>(j, lq));
+          const auto xv = xr[d & 1][j][m].planes();
 #pragma unroll
           for (int q = 0; q < NP; ++q) acc[q][m] = mma_planes(w[q], xv, acc[q][m]);
         }
@@ -615,9 +594,6 @@ __device__ __forceinline__ int x_swizzle(int m) {
   return FMT == kFmtBF16 ? m & 15 : (m & 3) | ((m & 8) ? 12 : 0);
 }
 
-// __builtin_amdgcn_sched_barrier: VALU, SALU and LDS reads may cross; loads, LDS stores, MFMAs stay.
-constexpr int kHoldLoads = 0x106;
-
 // Slabs of a panel per step, and the operands in each.
 template <int FMT>
 constexpr int tile_slabs() { return FMT == kFmtMXFP4 ? 1 : FMT == kFmtMXFP8 ? 2 : 4; }
@@ -639,12 +615,6 @@ __device__ __forceinline__ bf16x8 tile_operand(const uint4& q, float sc, int par
                  __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w1, sc, true));
   }
 }
-
-// The adapters' first products: planes (tiles), or the partial sums of shrink_kernel in ProjArgs::u.
-struct FirstProduct {
-  uint16_t* planes;
-  int ld, slices;
-};
 
 // Rows in BF16 planes: plane i of row t is `plane` bytes after plane i - 1 of it; `planes`: how many of them
 // each row needs (NULL: one).
@@ -802,8 +772,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(
   };
 
   fetch(slab[0], 0);
-  const bool adapters = p.ids && blockIdx.y == 0;  // the first slice adds them
-  if (adapters) find_slots(p, t0, count, slots);
+  if (p.ids) find_slots(p, t0, count, slots);
   if constexpr (FMT != kFmtMXFP4) fetch(slab[1], 1);  // (a step has two slabs at least)
   fetch_scales(sc[0], 0);
 #pragma unroll
@@ -831,8 +800,9 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(
     advance(Int<1>{}, x1, x0);
     if (s == steps) break;
   }
-  if (adapters)
-    add_adapters<YB ? 2 : 3>(p, slots, u.planes, u.ld, panel0, panels, t0, wm * MB * 16, acc);
+  if (p.ids)
+    add_adapters<YB ? 2 : 3>(p, slots, u, panel0, panels, t0, wm * MB * 16, (int)blockIdx.y,
+                             (int)gridDim.y, acc);
 #pragma unroll
   for (int m = 0; m < MB; ++m) {
     const int local = (wm * MB + m) * 16 + ln, t = t0 + local;
@@ -904,16 +874,11 @@ __global__ void enter_adapter_kernel(int rank, float scale, AdapterEntry* entry,
 }
 
 template <int FMT, bool XB, bool YB>
-void launch_rows(const ProjArgs& p, int u_ld, int slices, hipStream_t s) {
+void launch_rows(const ProjArgs& p, const FirstProduct& u, hipStream_t s) {
+  // (the tile of two blocks is for rows whose stride the tiles cannot address)
   const int panels = p.rows / kPanelRows;
-  auto go = [&](auto mb, auto np) {
-    constexpr int MB = decltype(mb)::value, NP = decltype(np)::value;
-    const dim3 grid((panels + NP - 1) / NP, (p.tokens + 16 * MB - 1) / (16 * MB));
-    split_kernel<FMT, XB, YB, MB, NP><<<grid, 64 * kSplitWaves, 0, s>>>(p, u_ld, slices);
-  };
-  if (p.tokens <= 16) go(Int<1>{}, Int<1>{});
-  else if (p.tokens <= 32) go(Int<2>{}, Int<2>{});
-  else go(Int<4>{}, Int<2>{});
+  const dim3 one(panels, (p.tokens + 15) / 16);
+  split_kernel<FMT, XB, YB, 1, 1><<<one, 64 * kSplitWaves, 0, s>>>(p, u);
 }
 
 template <int FMT>
@@ -923,9 +888,7 @@ constexpr double kWeightBits = FMT == kFmtBF16 ? 16 : FMT == kFmtMXFP8 ? 8.25 : 
 struct TileShape {
   int blocks, panels, row_tiles, col_tiles, slices;
 };
-#ifndef TNP
-#define TNP 4
-#endif
+constexpr long kMostSliced = 512;  // workgroups beyond which K is not cut (bounds the slices' sums)
 TileShape tile_shape(int tokens, int rows, int cols, int planes) {
   // tiles of equal height, at most 128 rows, an even number of blocks
   TileShape t{};
@@ -933,14 +896,31 @@ TileShape tile_shape(int tokens, int rows, int cols, int planes) {
   const int blocks = ((tokens + t.row_tiles - 1) / t.row_tiles + 15) / 16;
   t.blocks = blocks <= 2 ? 2 : (blocks + 1) / 2 * 2;
   t.row_tiles = (tokens + 16 * t.blocks - 1) / (16 * t.blocks);
-  t.panels = 4 * TNP;
-  t.col_tiles = (rows / kPanelRows + t.panels - 1) / t.panels;
-  // K in slices until the chip has kFill workgroups, of four steps at least
-  const int tiles = t.row_tiles * t.col_tiles, steps = cols / kTileStep;
-#ifndef KFILL
-#define KFILL 384
-#endif
-  t.slices = std::max(1, std::min({KFILL / tiles, steps * planes / 4, steps, kMaxSlices}));
+  // Panels per wave and slices of K by the time of the CU with the most workgroups.  Measured: a step of
+  // 128 x 256 x 128 takes a workgroup 2.0 us alone on its CU and two 1.72 each, smaller ones 0.9 at least
+  // (loads' latency); 2 us to fill and drain a workgroup; joining slices 4 us and their traffic.  (1000
+  // rows of 4096 -> 6144: 192 tiles of 256 outputs 66 us, 256 of 192 outputs 56; 4096 rows of 7168 -> 7168:
+  // 349 and 371.)
+  const int steps = cols / kTileStep;
+  double best = 0;
+  for (int np = 4; np >= 3; --np) {
+    const int col_tiles = (rows / kPanelRows + 4 * np - 1) / (4 * np);
+    const long tiles = (long)t.row_tiles * col_tiles;
+    const double step = std::max(0.9, 2.0 * np * t.blocks / 32);
+    for (int slices = 1; slices <= std::min(steps, kMaxSlices); ++slices) {
+      if (slices > 1 && tiles * slices > kMostSliced) break;
+      const long per_cu = (tiles * slices + 255) / 256;
+      const int each = (steps + slices - 1) / slices * planes;
+      double us = per_cu * (each * step * (per_cu > 1 ? 0.86 : 1.0) + 2.0);
+      if (slices > 1) us += 4.0 + (double)slices * tokens * rows * 8 / 3.5e6;
+      if (t.slices == 0 || us < best) {
+        best = us;
+        t.panels = 4 * np;
+        t.col_tiles = col_tiles;
+        t.slices = slices;
+      }
+    }
+  }
   return t;
 }
 
@@ -969,73 +949,22 @@ void launch_tiles(const ProjArgs& p, const TileRows& rows, const FirstProduct& u
   grid.band = std::min(8, grid.tall());
   const dim3 blocks(8 * grid.tall() * grid.wide(), t.slices);
   float* const out = t.slices > 1 ? parts : nullptr;
-  auto go = [&](auto mb) {
-    tile_kernel<FMT, YB, 1, 4, decltype(mb)::value, TNP><<<blocks, 256, 0, s>>>(p, rows, u, grid, out);
+  auto go = [&](auto mb, auto np) {
+    tile_kernel<FMT, YB, 1, 4, decltype(mb)::value, decltype(np)::value>
+        <<<blocks, 256, 0, s>>>(p, rows, u, grid, out);
   };
-  if (t.blocks == 2) go(Int<2>{});
-  else if (t.blocks == 4) go(Int<4>{});
-  else if (t.blocks == 6) go(Int<6>{});
-  else go(Int<8>{});
+  auto tall = [&](auto np) {
+    if (t.blocks == 2) go(Int<2>{}, np);
+    else if (t.blocks == 4) go(Int<4>{}, np);
+    else if (t.blocks == 6) go(Int<6>{}, np);
+    else go(Int<8>{}, np);
+  };
+  if (t.panels == 12) tall(Int<3>{});
+  else tall(Int<4>{});
   if (out) {
     const size_t quads = (size_t)p.tokens * p.rows / 4;
     join_kernel<YB><<<(unsigned)((quads + 255) / 256), 256, 0, s>>>(p, parts, t.slices);
   }
-}
-
-template <bool XB>
-void launch_shrink(const ProjArgs& p, int u_ld, int slices, hipStream_t s) {
-  const bool by_token = p.tokens <= kScan && p.tokens <= p.slots;
-  // (without slots one workgroup per segment, which reports the ids)
-  const dim3 grid(by_token ? p.tokens : std::max(1, p.slots), slices,
-                  (p.tokens + kScan - 1) / kScan);
-  if (by_token) shrink_kernel<XB, true><<<grid, kThreads, 0, s>>>(p, u_ld, slices);
-  else shrink_kernel<XB, false><<<grid, kThreads, 0, s>>>(p, u_ld, slices);
-}
-
-// What tiles need of a row beforehand.  f32 rows (planes not NULL) as planes [3][tokens][cols], and how
-// many of them each row needs (1: its values are BF16).  First products of shrink_kernel (slices > 0):
-// summed over its slices in order, scaled, as the planes that the second product multiplies.
-template <int P>
-__global__ __launch_bounds__(256) void rows_kernel(ProjArgs p, FirstProduct u, uint16_t* planes,
-                                                   int* needed) {
-  const int t = blockIdx.x;
-  if (planes) {
-    const uint8_t* row = reinterpret_cast<const uint8_t*>(p.x) + (size_t)t * p.x_stride * 4;
-    bool more = false;
-    for (int c = 8 * threadIdx.x; c < p.cols; c += 8 * 256) {
-      const Planes<3> v = load_x<false>(row, c);
-#pragma unroll
-      for (int pl = 0; pl < 3; ++pl)
-        *reinterpret_cast<uint4*>(planes + ((size_t)pl * p.tokens + t) * p.cols + c) =
-            make_uint4(v.w[pl][0], v.w[pl][1], v.w[pl][2], v.w[pl][3]);
-      more |= (v.w[1][0] | v.w[1][1] | v.w[1][2] | v.w[1][3]) != 0;
-    }
-    more = __syncthreads_or(more);
-    if (threadIdx.x == 0) needed[t] = more ? 3 : 1;
-  }
-  if (u.slices == 0) return;
-  const int id = p.ids[t];
-  if (id < 0 || id >= p.slots) return;
-  const AdapterEntry e = p.table[id];
-  const int r = 8 * threadIdx.x;
-  if (r >= 16 * ((e.rank + 15) / 16)) return;
-  float v[8] = {};
-  const float* from = p.u + (size_t)t * u.ld + r;
-#pragma unroll 4
-  for (int z = 0; z < u.slices; ++z) {
-    const float4 c = *reinterpret_cast<const float4*>(from);
-    const float4 d = *reinterpret_cast<const float4*>(from + 4);
-    v[0] += c.x; v[1] += c.y; v[2] += c.z; v[3] += c.w;
-    v[4] += d.x; v[5] += d.y; v[6] += d.z; v[7] += d.w;
-    from += (size_t)p.tokens * u.ld;
-  }
-#pragma unroll
-  for (int j = 0; j < 8; ++j) v[j] *= e.scale;
-  const Planes<P> out = split_planes<P>(v);
-#pragma unroll
-  for (int pl = 0; pl < P; ++pl)
-    *reinterpret_cast<uint4*>(u.planes + ((size_t)t * P + pl) * u.ld + r) =
-        make_uint4(out.w[pl][0], out.w[pl][1], out.w[pl][2], out.w[pl][3]);
 }
 
 // What a call's launches share.
@@ -1053,35 +982,33 @@ void launch_types(const ProjArgs& p, const Pass& a, hipStream_t s) {
     if (p.y_bf16) launch_tiles<FMT, true>(p, a.rows, a.u, a.shape, a.parts, s);
     else launch_tiles<FMT, false>(p, a.rows, a.u, a.shape, a.parts, s);
   } else if (p.x_bf16) {
-    if (p.y_bf16) launch_rows<FMT, true, true>(p, a.u.ld, a.u.slices, s);
-    else launch_rows<FMT, true, false>(p, a.u.ld, a.u.slices, s);
+    if (p.y_bf16) launch_rows<FMT, true, true>(p, a.u, s);
+    else launch_rows<FMT, true, false>(p, a.u, s);
   } else {
-    if (p.y_bf16) launch_rows<FMT, false, true>(p, a.u.ld, a.u.slices, s);
-    else launch_rows<FMT, false, false>(p, a.u.ld, a.u.slices, s);
+    if (p.y_bf16) launch_rows<FMT, false, true>(p, a.u, s);
+    else launch_rows<FMT, false, false>(p, a.u, s);
   }
 }
 
 // Most blocks of 16 rows of one adapter.
 int order_blocks(int tokens, int slots) { return tokens / 16 + std::min(tokens, slots); }
 
-// The workspace of a pass: the adapters' first products (up to kScan rows: partial sums in f32; more:
-// planes, the order and its blocks), f32 rows' planes and their counts, the slices' sums.
+// The workspace of a pass: the adapters' first products, the order and its blocks, f32 rows' planes and
+// their counts, the slices' sums.
 struct WorkLayout {
-  size_t u, u_planes, order, n_blocks, blocks, planes, needed, parts, total;
+  size_t u, order, n_blocks, blocks, planes, needed, parts, total;
   WorkLayout(int tokens, const ProjArgs& p) {
-    const size_t u_ld = 16 * rank_panels(p.max_rank);
     size_t at = 0;
     auto take = [&](size_t bytes) {
       const size_t here = at;
       at += (bytes + 255) / 256 * 256;
       return here;
     };
-    const bool few = tokens <= kScan, tiles = tokens >= kTileTokens;
-    u = take(p.slots && few ? tokens * u_ld * 4 * kMaxSlices : 0);
-    u_planes = take(p.slots && tiles ? tokens * u_ld * 6 : 0);
-    order = take(p.slots && !few ? (size_t)tokens * 4 : 0);
+    const bool tiles = tokens >= kTileTokens, sorted = p.slots && tokens > kFew;
+    u = take(p.slots ? (size_t)tokens * 16 * rank_panels(p.max_rank) * (p.y_bf16 ? 4 : 6) : 0);
+    order = take(sorted ? (size_t)tokens * 4 : 0);
     n_blocks = take(16);
-    blocks = take(p.slots && !few ? (size_t)order_blocks(tokens, p.slots) * 12 : 0);
+    blocks = take(sorted ? (size_t)order_blocks(tokens, p.slots) * 12 : 0);
     planes = take(!p.x_bf16 && tiles ? (size_t)tokens * p.cols * 6 : 0);
     needed = take(!p.x_bf16 && tiles ? (size_t)tokens * 4 : 0);
     const int slices = tiles ? tile_shape(tokens, p.rows, p.cols, p.x_bf16 ? 1 : 3).slices : 1;
@@ -1120,21 +1047,35 @@ void launch_project(const ProjArgs& p, hipStream_t s) {
   }
   const WorkLayout w(p.tokens, p);
   char* const work = static_cast<char*>(p.work);
-  ProjArgs q = p;
-  q.u = reinterpret_cast<float*>(work + w.u);
-  Pass a{tiles, {}, {0, nullptr},
-         {reinterpret_cast<uint16_t*>(work + w.u_planes), 16 * rank_panels(p.max_rank), 0},
-         reinterpret_cast<float*>(work + w.parts)};
+  auto ints = [&](size_t at) { return reinterpret_cast<int*>(work + at); };
+  const int max_panels = rank_panels(p.max_rank);
+  const FirstProduct u{reinterpret_cast<uint16_t*>(work + w.u), 16 * max_panels};
+  Pass a{tiles, {}, {0, nullptr}, u, reinterpret_cast<float*>(work + w.parts)};
   if (tiles) a.shape = tile_shape(p.tokens, p.rows, p.cols, p.x_bf16 ? 1 : 3);
-  if (p.ids && p.tokens > kScan) {
-    int* const order = reinterpret_cast<int*>(work + w.order);
-    int* const blocks = reinterpret_cast<int*>(work + w.blocks);
-    int* const n_blocks = reinterpret_cast<int*>(work + w.n_blocks);
-    order_kernel<<<1, kOrderThreads, 0, s>>>(p, order, blocks, n_blocks);
-    const int grid = std::max(1, order_blocks(p.tokens, p.slots));
-    auto go = [&](auto xb, auto planes) {
-      shrink_block_kernel<decltype(xb)::value, decltype(planes)::value>
-          <<<grid, 64 * kBlockWaves, 0, s>>>(p, order, blocks, n_blocks, a.u.planes, a.u.ld);
+  // the first products (of ids without any slot: one workgroup or the order, which report them)
+  Order order{};
+  int firsts = 0, groups = 1, per = 1;
+  bool by_token = false;
+  if (p.ids && p.tokens > kFew) {
+    order = Order{ints(w.order), ints(w.blocks), ints(w.n_blocks)};
+    order_kernel<<<1, kOrderThreads, 0, s>>>(p, ints(w.order), ints(w.blocks), ints(w.n_blocks));
+    // (four panels per workgroup share the rows' loads)
+    per = 4;
+    groups = std::max(1, (max_panels + 3) / 4);
+    firsts = order_blocks(p.tokens, p.slots) * groups;
+  } else if (p.ids) {
+    by_token = p.tokens < p.slots;
+    groups = std::max(1, max_panels);
+    firsts = std::max(1, std::min(p.tokens, p.slots)) * groups * ((p.tokens + 15) / 16);
+  }
+  uint16_t* const planes =
+      tiles && !p.x_bf16 ? reinterpret_cast<uint16_t*>(work + w.planes) : nullptr;
+  const int grid = firsts + (planes ? p.tokens : 0);
+  if (grid) {
+    auto go = [&](auto xb, auto count) {
+      prepare_kernel<decltype(xb)::value, decltype(count)::value>
+          <<<grid, 64 * kPrepareWaves, 0, s>>>(p, u, order, firsts, groups, per, by_token, planes,
+                                               ints(w.needed));
     };
     if (p.x_bf16) {
       if (p.y_bf16) go(std::true_type{}, Int<2>{});
@@ -1143,21 +1084,12 @@ void launch_project(const ProjArgs& p, hipStream_t s) {
       if (p.y_bf16) go(std::false_type{}, Int<2>{});
       else go(std::false_type{}, Int<3>{});
     }
-  } else if (p.ids) {
-    a.u.slices = std::min(kMaxSlices, std::max(1, p.cols / 512));
-    if (p.x_bf16) launch_shrink<true>(q, a.u.ld, a.u.slices, s);
-    else launch_shrink<false>(q, a.u.ld, a.u.slices, s);
   }
-  if (tiles && (!p.x_bf16 || a.u.slices)) {
-    uint16_t* const planes = p.x_bf16 ? nullptr : reinterpret_cast<uint16_t*>(work + w.planes);
-    int* const needed = reinterpret_cast<int*>(work + w.needed);
-    if (p.y_bf16) rows_kernel<2><<<p.tokens, 256, 0, s>>>(q, a.u, planes, needed);
-    else rows_kernel<3><<<p.tokens, 256, 0, s>>>(q, a.u, planes, needed);
-    if (planes) {
-      q.x = planes;
-      q.x_stride = p.cols;
-      a.rows = TileRows{(size_t)p.tokens * p.cols * 2, needed};
-    }
+  ProjArgs q = p;
+  if (planes) {
+    q.x = planes;
+    q.x_stride = p.cols;
+    a.rows = TileRows{(size_t)p.tokens * p.cols * 2, ints(w.needed)};
   }
   if (p.format == kFmtBF16) launch_types<kFmtBF16>(q, a, s);
   else if (p.format == kFmtMXFP4) launch_types<kFmtMXFP4>(q, a, s);

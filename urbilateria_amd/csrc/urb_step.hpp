@@ -81,7 +81,6 @@ struct ProjArgs {
   const uint16_t* b;
   size_t a_slot, b_slot;  // values
   void* work;             // proj_work_bytes
-  float* u;               // (set by launch_project: partial first products [slices][tokens][..])
   int* status;
 };
 // The workspace of calls of up to max_tokens rows (of the geometry, types, slots and ranks in p).
