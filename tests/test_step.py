@@ -177,6 +177,25 @@ def test_many_rows_and_many_adapters(T, slots):
         p.check(p.p.forward(x, ids), x, ids)
 
 
+@pytest.mark.parametrize("fmt", sorted(FMTS))
+@pytest.mark.parametrize("dtype,out", [(BF16, BF16), (F32, F32)])
+@pytest.mark.parametrize("T,rank", [(1, 1), (1, 9), (1, 16), (1, 17), (1, 32), (1, 33), (2, 16), (2, 5),
+                                    (2, 17), (3, 16)])
+def test_single_tokens_of_low_rank(fmt, dtype, out, T, rank):
+    # the sizes around which a tile computes its first products itself
+    p = Proj(fmt, 80, 1152, T, dtype, out, ranks=(rank, max(1, rank // 2), rank, 0), max_rank=rank)
+    x = p.rows_of(T).cuda()
+    for ids in ([0, 1, 0], [2, 2, 1], [-1, 0, -1], [-1, -1, -1]):
+        ids = torch.tensor(ids[:T], dtype=torch.int32, device="cuda")
+        p.check(p.p.forward(x, ids), x, ids)
+    y = torch.empty(T, 80, dtype=p.out_dtype, device="cuda")
+    for bad in (3, 4):     # an empty slot, none
+        ids = torch.tensor([bad, 0, 0][:T], dtype=torch.int32, device="cuda")
+        p.p.forward_into(x, y, ids)
+        assert _status(p.p.sync) == N.ERR_ARGUMENT
+        p.check(y, x, torch.where(ids == bad, -1, ids))
+
+
 def test_calls_longer_than_one_pass():
     T = 8192 + 77
     p = Proj("bf16", 16, 128, T, BF16, F32, ranks=(3, 2))

@@ -328,15 +328,28 @@ __global__ __launch_bounds__(64 * kPrepareWaves) void prepare_kernel(
   f32x4 acc[4];
 #pragma unroll
   for (int q = 0; q < 4; ++q) acc[q] = f32x4{0.f, 0.f, 0.f, 0.f};
+  // (loads in batches: the check for empty planes is a branch, across which none would be moved)
   auto sweep = [&](auto count) {
-    constexpr int NQ = decltype(count)::value;
-#pragma unroll 4
-    for (int s = s0; s < s1; ++s) {
-      const auto xv = load_x<XB>(row, 32 * s + 8 * lq);
+    constexpr int NQ = decltype(count)::value, BATCH = XB || NQ <= 2 ? 4 : 2;
+    for (int s = s0; s < s1; s += BATCH) {
+      XRaw<XB> xv[BATCH];
+      uint4 w[BATCH][NQ];
 #pragma unroll
-      for (int q = 0; q < NQ; ++q)
-        acc[q] = mma_planes(__builtin_bit_cast(bf16x8, ldg16(a + ((size_t)(q0 + q) * steps + s) * 512)),
-                            xv, acc[q]);
+      for (int i = 0; i < BATCH; ++i) {
+        const int si = min(s + i, s1 - 1);
+        xv[i].load(row, 32 * si + 8 * lq);
+#pragma unroll
+        for (int q = 0; q < NQ; ++q) w[i][q] = ldg16(a + ((size_t)(q0 + q) * steps + si) * 512);
+      }
+      __builtin_amdgcn_sched_barrier(kHoldLoads);
+#pragma unroll
+      for (int i = 0; i < BATCH; ++i) {
+        if (s + i >= s1) break;
+        const auto x = xv[i].planes();
+#pragma unroll
+        for (int q = 0; q < NQ; ++q)
+          acc[q] = mma_planes(__builtin_bit_cast(bf16x8, w[i][q]), x, acc[q]);
+      }
     }
   };
   if (nq == 1) sweep(Int<1>{});
@@ -483,8 +496,19 @@ __device__ __forceinline__ void store_y(const ProjArgs& p, int t, int row, f32x4
 // ---- W x for a few tokens: eight waves split K of NP panels, 16 MB tokens per tile ----
 constexpr int kSplitWaves = 8;
 
-template <int FMT, bool XB, bool YB, int MB, int NP>
+// ALONE: the tile computes its rows' first products itself, every workgroup all of them (kAloneRanks of at
+// most: rows times ranks), its waves over the K they have anyway.
+constexpr int kAloneRanks = 32;
+#ifndef AB
+#define AB 32e6
+#endif
+constexpr double kAloneBytes = AB;
+
+template <int FMT, bool XB, bool YB, int MB, int NP, bool ALONE>
 __global__ __launch_bounds__(64 * kSplitWaves) void split_kernel(ProjArgs p, FirstProduct u) {
+  static_assert(!ALONE || (MB == 1 && NP == 1), "one block, one panel");
+  constexpr int UP = kAloneRanks / 16;
+  __shared__ f32x4 red_u[ALONE ? kSplitWaves : 1][UP][64];
   constexpr int TILE = 16 * MB;
   __shared__ f32x4 red[kSplitWaves][NP * MB][64];
   __shared__ TileSlots<TILE> slots;
@@ -538,7 +562,36 @@ __global__ __launch_bounds__(64 * kSplitWaves) void split_kernel(ProjArgs p, Fir
   if (s0 < s1) fetch_rows(0, s0);
   if (p.ids) {
     find_slots(p, t0, count, slots);
-    add_adapters<YB ? 2 : 3>(p, slots, u, panel0, panels, t0, 0, wave, kSplitWaves, acc);
+    if constexpr (ALONE) {
+      if (blockIdx.x == 0 && (int)threadIdx.x < count) {
+        const int id = p.ids[t0 + threadIdx.x];
+        if (id >= 0 && slots.ids[threadIdx.x] < 0) flag(p.status, kStepArgument);
+      }
+      int at = 0;
+      for (int i = 0; i < slots.n; ++i) {
+        const int slot = slots.list[i].x;
+        const uint16_t* a = p.a + (size_t)slot * p.a_slot + 8 * lane;
+        for (int q = 0; 2 * q < slots.list[i].y; ++q, ++at) {
+          f32x4 v = f32x4{0.f, 0.f, 0.f, 0.f};
+          for (int s = s0; s < s1; ++s) {
+            XRaw<XB> xv[4];
+            uint4 w[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              xv[j].load(row[0], kGemmKStep * s + 32 * j + 8 * lq);
+              w[j] = ldg16(a + ((size_t)q * (4 * steps) + 4 * s + j) * 512);
+            }
+            __builtin_amdgcn_sched_barrier(kHoldLoads);
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              v = mma_planes(__builtin_bit_cast(bf16x8, w[j]), xv[j].planes(), v);
+          }
+          red_u[wave][at][lane] = v;
+        }
+      }
+    } else {
+      add_adapters<YB ? 2 : 3>(p, slots, u, panel0, panels, t0, 0, wave, kSplitWaves, acc);
+    }
   }
   for (int i0 = s0; i0 < s1; i0 += R) {
 #pragma unroll
@@ -574,6 +627,35 @@ __global__ __launch_bounds__(64 * kSplitWaves) void split_kernel(ProjArgs p, Fir
 #pragma unroll
     for (int z = 1; z < kSplitWaves; ++z) v += red[z][i][lane];  // K parts in order
     const int local = 16 * m + ln, t = t0 + local;
+    if constexpr (ALONE) {
+      constexpr int P = YB ? 2 : 3;
+      int at = 0;
+      for (int j = 0; p.ids && j < slots.n; ++j) {
+        // the lane's eight ranks: of panel lq / 2, held four each by two lanes of its row
+        const int slot = slots.list[j].x, units = slots.list[j].y;
+        const bf16x8 w = load_up(p.b + (size_t)slot * p.b_slot + (size_t)panel * units * 128, 0, units);
+        float uv[8] = {};
+        if (slots.ids[local] == slot && lq < units) {
+          const int from = 32 * (lq & 1) + ln;
+          f32x4 lo = red_u[0][at + lq / 2][from], hi = red_u[0][at + lq / 2][from + 16];
+#pragma unroll
+          for (int z = 1; z < kSplitWaves; ++z) {
+            lo += red_u[z][at + lq / 2][from];
+            hi += red_u[z][at + lq / 2][from + 16];
+          }
+          const float scale = p.table[slot].scale;
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            uv[r] = lo[r] * scale;
+            uv[4 + r] = hi[r] * scale;
+          }
+        }
+        const Planes<P> planes = split_planes<P>(uv);
+#pragma unroll
+        for (int pl = 0; pl < P; ++pl) v = mfma(w, planes.operand(pl), v);
+        at += (units + 1) / 2;
+      }
+    }
     if (local < count) store_y<YB>(p, t, panel * kPanelRows + 4 * lq, v);
   }
 }
@@ -874,11 +956,10 @@ __global__ void enter_adapter_kernel(int rank, float scale, AdapterEntry* entry,
 }
 
 template <int FMT, bool XB, bool YB>
-void launch_rows(const ProjArgs& p, const FirstProduct& u, hipStream_t s) {
-  // (the tile of two blocks is for rows whose stride the tiles cannot address)
-  const int panels = p.rows / kPanelRows;
-  const dim3 one(panels, (p.tokens + 15) / 16);
-  split_kernel<FMT, XB, YB, 1, 1><<<one, 64 * kSplitWaves, 0, s>>>(p, u);
+void launch_rows(const ProjArgs& p, const FirstProduct& u, bool alone, hipStream_t s) {
+  const dim3 grid(p.rows / kPanelRows, (p.tokens + 15) / 16);
+  if (alone) split_kernel<FMT, XB, YB, 1, 1, true><<<grid, 64 * kSplitWaves, 0, s>>>(p, u);
+  else split_kernel<FMT, XB, YB, 1, 1, false><<<grid, 64 * kSplitWaves, 0, s>>>(p, u);
 }
 
 template <int FMT>
@@ -897,8 +978,8 @@ TileShape tile_shape(int tokens, int rows, int cols, int planes) {
   t.blocks = blocks <= 2 ? 2 : (blocks + 1) / 2 * 2;
   t.row_tiles = (tokens + 16 * t.blocks - 1) / (16 * t.blocks);
   // Panels per wave and slices of K by the time of the CU with the most workgroups.  Measured: a step of
-  // 128 x 256 x 128 takes a workgroup 2.0 us alone on its CU and two 1.72 each, smaller ones 0.9 at least
-  // (loads' latency); 2 us to fill and drain a workgroup; joining slices 4 us and their traffic.  (1000
+  // 128 x 256 x 128 takes a workgroup 2.0 us alone on its CU (192 outputs 1.62) and two 1.72 each, smaller
+  // ones 0.9 at least (loads' latency); 2 us to fill and drain a workgroup; joining slices 4 us and their traffic.  (1000
   // rows of 4096 -> 6144: 192 tiles of 256 outputs 66 us, 256 of 192 outputs 56; 4096 rows of 7168 -> 7168:
   // 349 and 371.)
   const int steps = cols / kTileStep;
@@ -906,7 +987,7 @@ TileShape tile_shape(int tokens, int rows, int cols, int planes) {
   for (int np = 4; np >= 3; --np) {
     const int col_tiles = (rows / kPanelRows + 4 * np - 1) / (4 * np);
     const long tiles = (long)t.row_tiles * col_tiles;
-    const double step = std::max(0.9, 2.0 * np * t.blocks / 32);
+    const double step = std::max(0.9, (np == 4 ? 2.0 : 1.62) * t.blocks / 8);
     for (int slices = 1; slices <= std::min(steps, kMaxSlices); ++slices) {
       if (slices > 1 && tiles * slices > kMostSliced) break;
       const long per_cu = (tiles * slices + 255) / 256;
@@ -969,7 +1050,7 @@ void launch_tiles(const ProjArgs& p, const TileRows& rows, const FirstProduct& u
 
 // What a call's launches share.
 struct Pass {
-  bool tiles;
+  bool tiles, alone;
   TileShape shape;
   TileRows rows;
   FirstProduct u;
@@ -982,11 +1063,11 @@ void launch_types(const ProjArgs& p, const Pass& a, hipStream_t s) {
     if (p.y_bf16) launch_tiles<FMT, true>(p, a.rows, a.u, a.shape, a.parts, s);
     else launch_tiles<FMT, false>(p, a.rows, a.u, a.shape, a.parts, s);
   } else if (p.x_bf16) {
-    if (p.y_bf16) launch_rows<FMT, true, true>(p, a.u, s);
-    else launch_rows<FMT, true, false>(p, a.u, s);
+    if (p.y_bf16) launch_rows<FMT, true, true>(p, a.u, a.alone, s);
+    else launch_rows<FMT, true, false>(p, a.u, a.alone, s);
   } else {
-    if (p.y_bf16) launch_rows<FMT, false, true>(p, a.u, s);
-    else launch_rows<FMT, false, false>(p, a.u, s);
+    if (p.y_bf16) launch_rows<FMT, false, true>(p, a.u, a.alone, s);
+    else launch_rows<FMT, false, false>(p, a.u, a.alone, s);
   }
 }
 
@@ -1050,7 +1131,11 @@ void launch_project(const ProjArgs& p, hipStream_t s) {
   auto ints = [&](size_t at) { return reinterpret_cast<int*>(work + at); };
   const int max_panels = rank_panels(p.max_rank);
   const FirstProduct u{reinterpret_cast<uint16_t*>(work + w.u), 16 * max_panels};
-  Pass a{tiles, {}, {0, nullptr}, u, reinterpret_cast<float*>(work + w.parts)};
+  // A token or two of low rank: every workgroup reads all of its adapters' A from L2, which must stay
+  // under what a launch and its wait cost (5 us: 4096 -> 2048, BF16, rank 16, 11.9 -> 8 us).
+  const bool alone = p.ids && p.slots && p.tokens * 16 * max_panels <= kAloneRanks &&
+                     (double)p.rows / 16 * p.tokens * 32 * max_panels * p.cols <= kAloneBytes;
+  Pass a{tiles, alone, {}, {0, nullptr}, u, reinterpret_cast<float*>(work + w.parts)};
   if (tiles) a.shape = tile_shape(p.tokens, p.rows, p.cols, p.x_bf16 ? 1 : 3);
   // the first products (of ids without any slot: one workgroup or the order, which report them)
   Order order{};
@@ -1063,7 +1148,7 @@ void launch_project(const ProjArgs& p, hipStream_t s) {
     per = 4;
     groups = std::max(1, (max_panels + 3) / 4);
     firsts = order_blocks(p.tokens, p.slots) * groups;
-  } else if (p.ids) {
+  } else if (p.ids && !alone) {
     by_token = p.tokens < p.slots;
     groups = std::max(1, max_panels);
     firsts = std::max(1, std::min(p.tokens, p.slots)) * groups * ((p.tokens + 15) / 16);
