@@ -21,10 +21,7 @@ namespace urb {
 
 namespace {
 
-#ifndef TT
-#define TT 17
-#endif
-constexpr int kTileTokens = TT;   // rows of a call that takes tiles
+constexpr int kTileTokens = 17;   // rows of a call that takes tiles
 constexpr int kMaxSlices = 16;    // most slices of K
 
 // __builtin_amdgcn_sched_barrier: VALU, SALU and LDS reads may cross; loads, LDS stores, MFMAs stay.
@@ -264,36 +261,39 @@ struct Order {
 
 constexpr int kPrepareWaves = 16;
 
+// One row of f32 values as planes [3][tokens][cols], and how many of them it needs (1: its values are
+// BF16).  All threads of a workgroup.
+__device__ __forceinline__ void row_planes(const ProjArgs& p, int t, uint16_t* x_planes, int* needed) {
+  const uint8_t* row = reinterpret_cast<const uint8_t*>(p.x) + (size_t)t * p.x_stride * 4;
+  bool more = false;
+  for (int c = 8 * threadIdx.x; c < p.cols; c += 8 * blockDim.x) {
+    const Planes<3> v = load_x<false>(row, c);
+#pragma unroll
+    for (int pl = 0; pl < 3; ++pl)
+      *reinterpret_cast<uint4*>(x_planes + ((size_t)pl * p.tokens + t) * p.cols + c) =
+          make_uint4(v.w[pl][0], v.w[pl][1], v.w[pl][2], v.w[pl][3]);
+    more |= (v.w[1][0] | v.w[1][1] | v.w[1][2] | v.w[1][3]) != 0;
+  }
+  more = __syncthreads_or(more);
+  if (threadIdx.x == 0) needed[t] = more ? 3 : 1;
+}
+
 // What the products of a call need beforehand, in one launch.  Workgroups below `firsts`: the first product
 // of up to 16 rows of one adapter with up to `per` of its 16-rank panels (per 1 or 4), the waves' parts of K
 // summed in order.  With an order, a workgroup takes a block of it; without, workgroup (who, panels, z)
 // takes the z-th 16 rows of slot `who`, or (by_token) of the slot of row `who` if no row before has it.
-// The others: a row of f32 values each as planes [3][tokens][cols] (x_planes), and how many of them it
-// needs (1: its values are BF16).
+// In a grid of several rows each takes a slice of K and writes its sum to u_parts [slice][tokens][ld]
+// for finish_kernel.  The other workgroups: a row of f32 values each (row_planes).
 template <bool XB, int P>
 __global__ __launch_bounds__(64 * kPrepareWaves) void prepare_kernel(
-    ProjArgs p, FirstProduct u, Order order, int firsts, int groups, int per, bool by_token,
-    uint16_t* x_planes, int* needed) {
+    ProjArgs p, FirstProduct u, float* u_parts, Order order, int firsts, int groups, int per,
+    bool by_token, uint16_t* x_planes, int* needed) {
   __shared__ f32x4 red[kPrepareWaves][4][64];
   __shared__ int s_rows[kFew];
   const int tid = threadIdx.x, lane = tid & 63, ln = lane & 15, lq = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   if ((int)blockIdx.x >= firsts) {
-    if constexpr (!XB) {
-      const int t = blockIdx.x - firsts;
-      const uint8_t* row = reinterpret_cast<const uint8_t*>(p.x) + (size_t)t * p.x_stride * 4;
-      bool more = false;
-      for (int c = 8 * tid; c < p.cols; c += 8 * 64 * kPrepareWaves) {
-        const Planes<3> v = load_x<false>(row, c);
-#pragma unroll
-        for (int pl = 0; pl < 3; ++pl)
-          *reinterpret_cast<uint4*>(x_planes + ((size_t)pl * p.tokens + t) * p.cols + c) =
-              make_uint4(v.w[pl][0], v.w[pl][1], v.w[pl][2], v.w[pl][3]);
-        more |= (v.w[1][0] | v.w[1][1] | v.w[1][2] | v.w[1][3]) != 0;
-      }
-      more = __syncthreads_or(more);
-      if (tid == 0) needed[t] = more ? 3 : 1;
-    }
+    if constexpr (!XB) row_planes(p, blockIdx.x - firsts, x_planes, needed);
     return;
   }
   const int group = blockIdx.x % groups, unit = blockIdx.x / groups;
@@ -306,7 +306,7 @@ __global__ __launch_bounds__(64 * kPrepareWaves) void prepare_kernel(
   } else {
     const int tiles = (p.tokens + 15) / 16, who = unit / tiles, z = unit % tiles;
     const int id = lane < p.tokens ? p.ids[lane] : -1;
-    if (blockIdx.x == 0 && wave == 0 && id >= 0 && (id >= p.slots || p.table[id].rank == 0))
+    if (blockIdx.x == 0 && blockIdx.y == 0 && wave == 0 && id >= 0 && (id >= p.slots || p.table[id].rank == 0))
       flag(p.status, kStepArgument);
     slot = by_token ? __builtin_amdgcn_readlane(id, who) : who;
     if (slot < 0 || slot >= p.slots) return;
@@ -322,7 +322,8 @@ __global__ __launch_bounds__(64 * kPrepareWaves) void prepare_kernel(
   const int steps = p.cols / 32, panels = (e.rank + 15) / 16;
   const int q0 = group * per, nq = min(per, panels - q0);
   if (nq <= 0) return;
-  const int s0 = steps * wave / kPrepareWaves, s1 = steps * (wave + 1) / kPrepareWaves;
+  const int waves = kPrepareWaves * gridDim.y, part = kPrepareWaves * blockIdx.y + wave;
+  const int s0 = steps * part / waves, s1 = steps * (part + 1) / waves;
   const uint8_t* row = reinterpret_cast<const uint8_t*>(p.x) + (size_t)t * p.x_stride * (XB ? 2 : 4);
   const uint16_t* a = p.a + (size_t)slot * p.a_slot + 8 * lane;
   f32x4 acc[4];
@@ -365,6 +366,11 @@ __global__ __launch_bounds__(64 * kPrepareWaves) void prepare_kernel(
     f32x4 v = red[0][wave][lane];
 #pragma unroll
     for (int z = 1; z < kPrepareWaves; ++z) v += red[z][wave][lane];
+    if (gridDim.y > 1) {
+      *reinterpret_cast<f32x4*>(u_parts + ((size_t)blockIdx.y * p.tokens + t) * u.ld +
+                                16 * (q0 + wave) + 4 * lq) = v;
+      return;
+    }
     const float w[8] = {v[0] * e.scale, v[1] * e.scale, v[2] * e.scale, v[3] * e.scale};
     const Planes<P> planes = split_planes<P>(w);
 #pragma unroll
@@ -372,6 +378,36 @@ __global__ __launch_bounds__(64 * kPrepareWaves) void prepare_kernel(
       *reinterpret_cast<uint2*>(u.planes + ((size_t)t * P + pl) * u.ld + 16 * (q0 + wave) + 4 * lq) =
           make_uint2(planes.w[pl][0], planes.w[pl][1]);
   }
+}
+
+// The slices' sums of a row's first product, in order, as planes; and the row's own planes (x_planes).
+template <int P>
+__global__ __launch_bounds__(256) void finish_kernel(ProjArgs p, FirstProduct u, const float* u_parts,
+                                                     int slices, uint16_t* x_planes, int* needed) {
+  const int t = blockIdx.x;
+  const int id = p.ids[t], r = 8 * threadIdx.x;
+  AdapterEntry e{0, 0.0f};
+  if (id >= 0 && id < p.slots) e = p.table[id];
+  if (r < 16 * ((e.rank + 15) / 16)) {  // (as many as the panels wrote)
+    float v[8] = {};
+    const float* from = u_parts + (size_t)t * u.ld + r;
+#pragma unroll 8
+    for (int z = 0; z < slices; ++z) {
+      const float4 c = *reinterpret_cast<const float4*>(from);
+      const float4 d = *reinterpret_cast<const float4*>(from + 4);
+      v[0] += c.x; v[1] += c.y; v[2] += c.z; v[3] += c.w;
+      v[4] += d.x; v[5] += d.y; v[6] += d.z; v[7] += d.w;
+      from += (size_t)p.tokens * u.ld;
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] *= e.scale;
+    const Planes<P> out = split_planes<P>(v);
+#pragma unroll
+    for (int pl = 0; pl < P; ++pl)
+      *reinterpret_cast<uint4*>(u.planes + ((size_t)t * P + pl) * u.ld + r) =
+          make_uint4(out.w[pl][0], out.w[pl][1], out.w[pl][2], out.w[pl][3]);
+  }
+  if (x_planes) row_planes(p, t, x_planes, needed);
 }
 
 // ---- the second products, added to a tile's accumulators ----
@@ -499,10 +535,7 @@ constexpr int kSplitWaves = 8;
 // ALONE: the tile computes its rows' first products itself, every workgroup all of them (kAloneRanks of at
 // most: rows times ranks), its waves over the K they have anyway.
 constexpr int kAloneRanks = 32;
-#ifndef AB
-#define AB 32e6
-#endif
-constexpr double kAloneBytes = AB;
+constexpr double kAloneBytes = 50e6;
 
 template <int FMT, bool XB, bool YB, int MB, int NP, bool ALONE>
 __global__ __launch_bounds__(64 * kSplitWaves) void split_kernel(ProjArgs p, FirstProduct u) {
@@ -1074,10 +1107,19 @@ void launch_types(const ProjArgs& p, const Pass& a, hipStream_t s) {
 // Most blocks of 16 rows of one adapter.
 int order_blocks(int tokens, int slots) { return tokens / 16 + std::min(tokens, slots); }
 
-// The workspace of a pass: the adapters' first products, the order and its blocks, f32 rows' planes and
-// their counts, the slices' sums.
+// Slices of K of the first products (1: whole).  One workgroup pulls its rows and A at what a CU can, so
+// long rows of f32 are cut, where the launch that adds the slices also makes the rows' planes (a call of 64,
+// 131, 400 rows, 7168 -> 4096, MXFP4: 48.1 -> 43.2, 74.3 -> 68.8, 123.7 -> 119.4 us; of 131 rows of 2048
+// values 35.7 -> 39.5, so not there; BF16 rows lose as much by the launch as they gain).
+int first_slices(int tokens, const ProjArgs& p) {
+  if (p.x_bf16 || tokens < kTileTokens || tokens > 512) return 1;
+  return p.cols >= 5120 ? std::min(8, p.cols / 1024) : 1;
+}
+
+// The workspace of a pass: the adapters' first products and their slices' sums, the order and its
+// blocks, f32 rows' planes and their counts, the slices' sums.
 struct WorkLayout {
-  size_t u, order, n_blocks, blocks, planes, needed, parts, total;
+  size_t u, u_parts, order, n_blocks, blocks, planes, needed, parts, total;
   WorkLayout(int tokens, const ProjArgs& p) {
     size_t at = 0;
     auto take = [&](size_t bytes) {
@@ -1087,6 +1129,7 @@ struct WorkLayout {
     };
     const bool tiles = tokens >= kTileTokens, sorted = p.slots && tokens > kFew;
     u = take(p.slots ? (size_t)tokens * 16 * rank_panels(p.max_rank) * (p.y_bf16 ? 4 : 6) : 0);
+    u_parts = take(p.slots ? (size_t)first_slices(tokens, p) * tokens * 16 * rank_panels(p.max_rank) * 4 : 0);
     order = take(sorted ? (size_t)tokens * 4 : 0);
     n_blocks = take(16);
     blocks = take(sorted ? (size_t)order_blocks(tokens, p.slots) * 12 : 0);
@@ -1132,7 +1175,7 @@ void launch_project(const ProjArgs& p, hipStream_t s) {
   const int max_panels = rank_panels(p.max_rank);
   const FirstProduct u{reinterpret_cast<uint16_t*>(work + w.u), 16 * max_panels};
   // A token or two of low rank: every workgroup reads all of its adapters' A from L2, which must stay
-  // under what a launch and its wait cost (5 us: 4096 -> 2048, BF16, rank 16, 11.9 -> 8 us).
+  // under what a launch and its wait cost (5 us: 4096 -> 2048, BF16, rank 16, 11.9 -> 9.3 us).
   const bool alone = p.ids && p.slots && p.tokens * 16 * max_panels <= kAloneRanks &&
                      (double)p.rows / 16 * p.tokens * 32 * max_panels * p.cols <= kAloneBytes;
   Pass a{tiles, alone, {}, {0, nullptr}, u, reinterpret_cast<float*>(work + w.parts)};
@@ -1155,12 +1198,16 @@ void launch_project(const ProjArgs& p, hipStream_t s) {
   }
   uint16_t* const planes =
       tiles && !p.x_bf16 ? reinterpret_cast<uint16_t*>(work + w.planes) : nullptr;
-  const int grid = firsts + (planes ? p.tokens : 0);
-  if (grid) {
+  const int slices = firsts ? first_slices(p.tokens, p) : 1;
+  float* const u_parts = reinterpret_cast<float*>(work + w.u_parts);
+  const dim3 grid(firsts + (planes && slices == 1 ? p.tokens : 0), slices);
+  if (grid.x) {
     auto go = [&](auto xb, auto count) {
-      prepare_kernel<decltype(xb)::value, decltype(count)::value>
-          <<<grid, 64 * kPrepareWaves, 0, s>>>(p, u, order, firsts, groups, per, by_token, planes,
-                                               ints(w.needed));
+      constexpr int P = decltype(count)::value;
+      prepare_kernel<decltype(xb)::value, P><<<grid, 64 * kPrepareWaves, 0, s>>>(
+          p, u, u_parts, order, firsts, groups, per, by_token, planes, ints(w.needed));
+      if (slices > 1)
+        finish_kernel<P><<<p.tokens, 256, 0, s>>>(p, u, u_parts, slices, planes, ints(w.needed));
     };
     if (p.x_bf16) {
       if (p.y_bf16) go(std::true_type{}, Int<2>{});

@@ -893,11 +893,9 @@ __global__ __launch_bounds__(kRowThreads) void sample_draw_kernel(SampleArgs a, 
   }
 }
 
-#ifndef KP1
-#define KP1 2048
-#define KP2 1024
-#endif
-constexpr int kP1 = KP1, kP2 = KP2;
+// Workgroups of a launch that shares rows, about: enough that rows which cost more than others are spread
+// over the chip; fewer for the histogram, where each adds up to 4096 bins to the row's.
+constexpr int kRowParts = 2048, kBinParts = 1024;
 size_t row_bytes(int chunks) {
   return (size_t)chunks * 8 * (1 + kRowWaves) + kAllBins * 12 + kList * 8 + sizeof(RowRecord) + 4;
 }
@@ -940,11 +938,9 @@ void launch_sample(const SampleArgs& a, bool bf16, hipStream_t s) {
     if (a.probs) p.probs += row;
     Work w{};
     if (a.vocab > kList) {
-      // Enough workgroups that rows which cost more than others are spread over the chip; fewer for the
-      // histogram, where each adds up to 4096 bins to the row's.
       w.chunks = row_chunks(a.vocab);
-      w.parts = std::min(w.chunks, std::max(1, kP1 / p.rows));
-      w.bin_parts = std::min(w.chunks, std::max(1, kP2 / p.rows));
+      w.parts = std::min(w.chunks, std::max(1, kRowParts / p.rows));
+      w.bin_parts = std::min(w.chunks, std::max(1, kBinParts / p.rows));
       const size_t rows = p.rows, most = w.chunks;
       char* at = static_cast<char*>(a.work);
       auto take = [&](auto** q, size_t n) {
