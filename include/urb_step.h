@@ -125,8 +125,9 @@ typedef struct {
 /* q, k, q_out, k_out as the descriptor (host memory, read by the call) says; q_weight, k_weight
  * [head_dim] f32; positions [tokens] i64; inv_freq [rotary_dim / 2] f32 (may be NULL with
  * rotary_dim 0, as positions).  k, k_weight and k_out are not read with k_heads 0.  tokens 0 ->
- * URB_ERR_SHAPE.  Heads that start at multiples of 16 bytes, with head_dim and rotary_dim multiples of
- * 16, take the wide kernel; others give the same values, slower. */
+ * URB_ERR_SHAPE.  Heads that start at multiples of 16 bytes, with head_dim (and, unless
+ * interleaved, rotary_dim) a multiple of 16, take a kernel of wide loads; others one of single
+ * values. */
 urb_status urb_qk_norm_rope(const urb_qk_desc *desc, const void *q, const void *k,
                             const float *q_weight, const float *k_weight,
                             const int64_t *positions, const float *inv_freq, uint32_t tokens,
@@ -142,8 +143,8 @@ urb_status urb_qk_norm_rope(const urb_qk_desc *desc, const void *q, const void *
  *   5. the first token is always kept; the draw takes the smallest index i at which the sum of e
  *      over the kept tokens of index <= i exceeds uniform times the sum over all kept ones.
  * tau = 0 takes the lowest index of the largest logit.  NaN logits count as -inf and are never
- * drawn; a row with nothing above -inf gives id -1 and probability 0.  With logits of +inf the draw is among those.
- * e is computed in f64 and enters the sums as the nearest multiple of 2^-min(51, 62 -
+ * drawn; a row with nothing above -inf gives id -1 and probability 0.  With logits of +inf the draw
+ * is among those.  e is computed in f64 and enters the sums as the nearest multiple of 2^-min(51, 62 -
  * ceil(log2(vocab))): 2^-42 of the largest for 2^20 tokens, 2^-45 for 131072.  Sums of integers do
  * not depend on their order, so a result depends on nothing but the row and its parameters; tokens
  * below half of that unit are never drawn.

@@ -203,6 +203,129 @@ def test_calls_longer_than_one_pass():
     p.check(p.p.forward(x, ids), x, ids)
 
 
+@pytest.mark.parametrize("fmt", sorted(FMTS))
+@pytest.mark.parametrize("dtype,out", [(BF16, BF16), (F32, F32)])
+@pytest.mark.parametrize("T,rows,cols", [(100, 784, 384), (90, 2064, 1152), (65, 272, 5120), (400, 528, 640),
+                                         (512, 48, 5248), (513, 48, 5248)])
+def test_tiles_of_every_height_and_slices_of_the_long_axis(fmt, dtype, out, T, rows, cols):
+    # rows and columns that end inside a tile, few tiles and long sums, rows that share first products
+    p = Proj(fmt, rows, cols, T, dtype, out, ranks=(24, 3, 40, 0), max_rank=48)
+    x, ids = p.rows_of(T).cuda(), _mixed(T, 3, p.g)
+    p.check(p.p.forward(x, ids), x, ids)
+    p.check(p.p.forward(x[:T // 3], ids[:T // 3]), x[:T // 3], ids[:T // 3])
+    p.check(p.p.forward(x), x)
+
+
+def test_f32_rows_of_more_than_one_pass():
+    T = 2048 + 40
+    p = Proj("mxfp8", 144, 384, T, F32, ranks=(5, 17))
+    x, ids = p.rows_of(T).cuda(), _mixed(T, 2, p.g)
+    p.check(p.p.forward(x, ids), x, ids)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("stride", [(1 << 22) - 8, 1 << 22])
+def test_rows_far_apart(dtype, stride):
+    T, cols = 37, 256
+    p = Proj("bf16", 80, cols, T, dtype, F32, ranks=(8, 9))
+    x, ids = p.rows_of(T).cuda(), _mixed(T, 2, p.g)
+    far = torch.empty((T - 1) * stride + cols, dtype=dtype, device="cuda").as_strided((T, cols), (stride, 1))
+    far.copy_(x)
+    p.check(p.p.forward(far, ids), x, ids)
+    y = torch.empty((T - 1) * stride + 80, device="cuda").as_strided((T, 80), (stride, 1))
+    p.p.forward_into(x, y, ids)
+    p.p.sync()
+    p.check(y, x, ids)
+
+
+def test_a_matrix_of_more_than_4_gib():
+    rows, cols = 65536 + 64, 32768
+    w = torch.randn(rows, cols, device="cuda", dtype=BF16,
+                    generator=torch.Generator("cuda").manual_seed(1))
+    some = list(range(16)) + list(range(rows - 64, rows))
+    for T in (1, 18):
+        proj = step().AdaptedProjection(w, None, C.FMT_BF16, rows, cols, T, BF16, F32, slots=2, max_rank=8)
+        g = _gen(T)
+        a = (torch.randn(8, cols, generator=g) * cols ** -0.5).to(BF16)
+        b = torch.randn(rows, 8, generator=g).to(BF16)
+        proj.set_adapter(1, a.cuda(), b.cuda(), 0.5)
+        x = torch.randn(T, cols, generator=g).to(BF16)
+        got = proj.forward(x.cuda(), torch.ones(T, dtype=torch.int32, device="cuda"))[:, some].cpu().double()
+        xd, wd, bd = x.double(), w[some].cpu().double(), b[some].double()
+        want = xd @ wd.T + 0.5 * (xd @ a.double().T) @ bd.T
+        chain = 2 * U * (cols / 32 + 64)
+        size = xd.abs() @ wd.abs().T + 0.5 * ((xd.abs() @ a.double().abs().T) @ bd.abs().T)
+        # the chains of both products (u and the matrix), the second product's, the output's rounding
+        assert bool(((got - want).abs() <= 2 * (chain + 40 * U) * size).all())
+        del proj
+
+
+def test_every_slot_there_is():
+    p = Proj("bf16", 32, 128, 300, F32, ranks=(0,) * 4096, max_rank=4)
+    for slot in (0, 1, 2047, 4094, 4095):
+        p.fill(slot, 1 + slot % 4, scale=1.5)
+    x = p.rows_of(300).cuda()
+    ids = torch.tensor([0, 1, 2047, 4094, 4095, -1], dtype=torch.int32)
+    ids = ids[torch.randint(0, 6, (300,), generator=p.g)].cuda()
+    for T in (1, 3, 40, 300):
+        p.check(p.p.forward(x[:T], ids[:T].contiguous()), x[:T], ids[:T])
+
+
+@pytest.mark.parametrize("T,rows,cols,dtype", [(1, 64, 256, BF16), (12, 64, 1024, F32), (40, 272, 5120, F32),
+                                               (200, 528, 1024, BF16), (200, 528, 5120, F32)])
+def test_captured_projections_replay_on_new_inputs(T, rows, cols, dtype):
+    # rows, ids and a slot's content change between the replays; eager calls of the context stand between
+    p = Proj("mxfp4", rows, cols, T, dtype, F32, ranks=(16, 3, 20), max_rank=32)
+    x, ids = p.rows_of(T).cuda(), _mixed(T, 3, p.g)
+    y = torch.empty(T, rows, device="cuda")
+    p.p.forward_into(x, y, ids)
+    stream, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=stream):
+        p.p.forward_into(x, y, ids)
+    for i in range(4):
+        x.copy_(p.rows_of(T))
+        ids.copy_(_mixed(T, 3, p.g))
+        p.fill(i % 3, 1 + 7 * i)
+        y.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        p.check(y, x, ids)
+        assert torch.equal(p.p.forward(x, ids), y)
+    p.p.sync()
+
+
+def test_projections_on_two_streams():
+    both = [Proj("mxfp8", 784, 1152, 150, dtype, F32, ranks=(9, 30), seed=i)
+            for i, dtype in enumerate((BF16, F32))]
+    ins = [(p.rows_of(150).cuda(), _mixed(150, 2, p.g)) for p in both]
+    outs = [torch.empty(150, 784, device="cuda") for _ in both]
+    streams = [torch.cuda.Stream() for _ in both]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for p, (x, ids), y, s in zip(both, ins, outs, streams):
+            with torch.cuda.stream(s):
+                p.p.forward_into(x, y, ids)
+    torch.cuda.synchronize()
+    for p, (x, ids), y in zip(both, ins, outs):
+        p.check(y, x, ids)
+        p.p.sync()
+
+
+def test_outputs_of_padded_rows_are_left():
+    # a call over the first rows of a buffer writes nothing behind them
+    p = Proj("bf16", 272, 640, 80, BF16, ranks=(8,))
+    x = p.rows_of(80).cuda()
+    for T in (1, 16, 17, 33, 64, 70):
+        y = torch.full((80, 272), 5.0, dtype=BF16, device="cuda")
+        ids = torch.zeros(80, dtype=torch.int32, device="cuda")
+        ids[T:] = 99     # not read
+        p.p.forward_into(x[:T], y[:T], ids[:T])
+        p.p.sync()
+        p.check(y[:T], x[:T], ids[:T])
+        assert bool((y[T:] == 5.0).all())
+
+
 @pytest.mark.parametrize("T", [5, 140])
 @pytest.mark.parametrize("dtype", [BF16, F32])
 def test_strided_rows_and_outputs_leave_the_rest(T, dtype):
@@ -446,6 +569,54 @@ def test_rotation_of_rows_with_zeros_and_nan():
                   torch.tensor([1, 2, 2]), _freq(64), zero_centered=False)
 
 
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_the_same_heads_in_wide_and_in_single_steps(dtype):
+    # aligned heads and the same ones off every boundary: two kernels, one definition
+    g = _gen(13)
+    T, H, D = 70, 3, 128
+    h = torch.randn(T, H, D, generator=g).to(dtype).cuda()
+    w, pos = torch.rand(D, generator=g).cuda(), torch.arange(T).cuda() * 1000
+    odd = torch.empty(T, H * D + 3, dtype=dtype, device="cuda")[:, 1:1 + H * D].unflatten(1, (H, D))
+    odd.copy_(h)
+    for inter in (False, True):
+        a, _ = step().qk_norm_rope(h, None, w, None, pos, _freq(64), 1e-6, interleaved=inter)
+        b, _ = step().qk_norm_rope(odd, None, w, None, pos, _freq(64), 1e-6, interleaved=inter)
+        for got in (a, b):
+            _check_turned(got, h, w, pos, _freq(64), zero_centered=False, interleaved=inter)
+
+
+def test_captured_rotation_replays_on_new_positions():
+    g = _gen(14)
+    q = torch.randn(1, 8, 128, generator=g).to(BF16).cuda()
+    w, pos, freq = torch.rand(128, generator=g).cuda(), torch.tensor([5]).cuda(), _freq(64)
+    out = torch.empty_like(q)
+    call = lambda: step().qk_norm_rope(q, None, w, None, pos, freq, 1e-6, out=(out, None))
+    call()
+    stream, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=stream):
+        call()
+    for at in (6, 1000, 123456):
+        q.copy_(torch.randn(1, 8, 128, generator=g))
+        pos.fill_(at)
+        graph.replay()
+        torch.cuda.synchronize()
+        _check_turned(out, q, w, pos, freq, zero_centered=False)
+
+
+def test_heads_of_more_than_4_gib():
+    # the last token's heads lie past 32-bit byte offsets, in a fused buffer
+    T, H, D, row = 66000, 2, 64, 33000
+    wide = torch.zeros(T, row, dtype=BF16, device="cuda")
+    q = wide[:, :H * D].unflatten(1, (H, D))
+    q.copy_(torch.randn(T, H, D, generator=_gen(15)))
+    before, w, pos = q.clone(), torch.ones(D, device="cuda"), torch.arange(T).cuda()
+    step().qk_norm_rope(q, None, w, None, pos, _freq(D), 1e-6, out=(q, None))
+    some = [0, 1, 40000, 65999]
+    _check_turned(q[some], before[some], w, pos[some], _freq(D), zero_centered=False)
+    assert bool((wide[-1, H * D:] == 0).all())
+
+
 def test_rotation_wrapper_refuses():
     q, w = torch.zeros(2, 3, 64, device="cuda"), torch.ones(64, device="cuda")
     pos = torch.arange(2).cuda()
@@ -584,6 +755,104 @@ def test_strided_and_unaligned_logits_and_extra_rows():
         _check_drawn(wide[:, 3:1006], torch.rand(9, generator=g).tolist(), sampler, p=[0.9] * 9)
         _check_drawn(wide[:1, 1:1004], [0.4], sampler)
         _check_drawn(wide[::2, :1003], [0.1, 0.2, 0.3, 0.4, 0.5], sampler, k=[0, 1, 2, 30, 4000])
+
+
+def test_more_rows_than_one_pass():
+    g = _gen(21)
+    T, V = 2 * 512 + 3, 1500
+    x = _logits(T, V, g)
+    pick = lambda values: [values[i % len(values)] for i in range(T)]
+    _check_drawn(x, torch.rand(T, generator=g).tolist(), tau=pick([1.0, 0.0, 0.6]), k=pick([0, 5, 0, 70]),
+                 p=pick([0.9, 1.0, 0.5, 0.99, 1.0]), min_p=pick([0.0, 0.05]))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("V", [1025, 8192 * 3 + 5, 70001])
+def test_crowded_bins_and_rows_off_the_boundary(V, dtype):
+    # flat rows, whose cut lies among more tokens than a list holds, beside rows whose cut's bin alone
+    # does, rows without a cut, and rows of one value; each from every start within 16 bytes
+    g = _gen(V)
+    near = lambda at, n: torch.cat((torch.full((n,), at), torch.full((V - n,), at - 8.0)))[
+        torch.randperm(V, generator=g)]
+    rows = [torch.randn(V, generator=g) * spread for spread in (1e-4, 0.02, 0.5, 6.0)]
+    rows += [near(3.0, 5), near(3.0, 1024), near(3.0, min(V, 1030)), torch.full((V,), -2.0)]
+    wide = torch.zeros(len(rows), V + 17, dtype=dtype, device="cuda")
+    lists = [dict(p=0.5), dict(k=1000), dict(k=1024, p=0.7), dict(p=0.9, min_p=0.3), dict()]
+    for start in range(0, 8, 3):
+        view = wide[:, start:start + V]
+        view.copy_(torch.stack(rows))
+        for params in lists:
+            _check_drawn(view, torch.rand(len(rows), generator=g).tolist(),
+                         **{n: [v] * len(rows) for n, v in params.items()})
+
+
+@pytest.mark.parametrize("T,V", [(1, 700), (3, 9000), (40, 33000)])
+def test_captured_draws_replay_on_new_inputs(T, V):
+    g = _gen(T)
+    sampler = step().Sampler(V, T)
+    x, u = _logits(T, V, g), torch.rand(T, generator=g).cuda()
+    p = torch.full((T,), 0.9, device="cuda")
+    ids, probs = torch.empty(T, dtype=torch.int32, device="cuda"), torch.empty(T, device="cuda")
+    call = lambda: sampler.sample_into(x, u, ids, probs, top_p=p)
+    call()
+    stream, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=stream):
+        call()
+    for i in range(4):
+        x.copy_(_logits(T, V, g))
+        u.copy_(torch.rand(T, generator=g))
+        p.fill_(0.3 + 0.2 * i)
+        ids.fill_(-7)
+        graph.replay()
+        torch.cuda.synchronize()
+        got = ids.clone(), probs.clone()
+        for t in range(T):
+            id_, prob = _drawn(x[t], p=float(p[t]), u=float(u[t]))
+            assert int(got[0][t]) == id_ and abs(float(got[1][t]) - prob) <= (U + 2.0 ** -40) * prob
+        call()
+        assert torch.equal(got[0], ids) and torch.equal(got[1], probs)
+    sampler.sync()
+
+
+def test_samplers_on_two_streams():
+    g = _gen(31)
+    both = [step().Sampler(40000, 20) for _ in range(2)]
+    ins = [(_logits(20, 40000, g), torch.rand(20, generator=g).cuda()) for _ in both]
+    p, tau = torch.full((20,), 0.8, device="cuda"), torch.full((20,), 0.7, device="cuda")
+    outs = [(torch.empty(20, dtype=torch.int32, device="cuda"), torch.empty(20, device="cuda")) for _ in both]
+    streams = [torch.cuda.Stream() for _ in both]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for sampler, (x, u), (ids, probs), s in zip(both, ins, outs, streams):
+            with torch.cuda.stream(s):
+                sampler.sample_into(x, u, ids, probs, top_p=p, temperature=tau)
+    torch.cuda.synchronize()
+    for (x, u), (ids, probs) in zip(ins, outs):
+        for t in range(20):
+            id_, prob = _drawn(x[t], tau=float(tau[t]), p=float(p[t]), u=float(u[t]))
+            assert int(ids[t]) == id_ and abs(float(probs[t]) - prob) <= (U + 2.0 ** -40) * prob
+
+
+def test_rows_behind_the_last_are_left():
+    s = step().Sampler(2000, 8)
+    x, u = _logits(8, 2000, _gen(5)), torch.full((8,), 0.5, device="cuda")
+    ids, probs = torch.full((8,), 77, dtype=torch.int32, device="cuda"), torch.full((8,), 7.0, device="cuda")
+    s.sample_into(x[:3], u[:3], ids[:3], probs[:3])
+    s.sync()
+    assert bool((ids[3:] == 77).all()) and bool((probs[3:] == 7.0).all()) and bool((ids[:3] < 2000).all())
+
+
+def test_logits_of_more_than_4_gib():
+    V, T = 1 << 20, 1100
+    x = torch.zeros(T, V, device="cuda")
+    x[T - 1, V - 1] = x[T - 2, 12345] = x[0, 7] = 60.0
+    ids, probs = step().Sampler(V, T).sample(x, torch.full((T,), 0.5, device="cuda"),
+                                             temperature=torch.full((T,), 0.5, device="cuda"))
+    assert [int(ids[i]) for i in (T - 1, T - 2, 0)] == [V - 1, 12345, 7]
+    # the middle of a flat row: the smallest index i at which i + 1 > V / 2
+    assert int(ids[1]) == V // 2 and bool((ids[1:T - 2] == V // 2).all())
+    assert bool((probs[1:T - 2] == 1.0 / V).all()) and bool((probs[[0, T - 1]] == 1.0).all())
 
 
 def test_extreme_temperatures():
