@@ -260,6 +260,76 @@ struct Order {
 };
 
 constexpr int kPrepareWaves = 16;
+constexpr int kOwnBlocks = 64 * kPrepareWaves;  // most rows whose blocks each workgroup finds for itself
+
+// The unit-th block of up to 16 rows of one adapter (slots ascending, rows ascending) of at most
+// kOwnBlocks rows: what order_kernel finds for all, by each workgroup for itself, which costs less than that
+// launch (calls of 131 and of 1000 rows: 68.6 -> 66.0 and 77.1 -> 74.2 us).  Returns the rows in it (0: no such
+// block), their numbers in rows[].
+__device__ __forceinline__ int find_block(const ProjArgs& p, int unit, int* count, int* rows, int* slot) {
+  __shared__ int waves[kPrepareWaves], s_slot, s_z;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  int id = tid < p.tokens ? p.ids[tid] : -1;
+  constexpr int PER = kMaxSlots / (64 * kPrepareWaves);
+  bool filled[PER];
+#pragma unroll
+  for (int j = 0; j < PER; ++j) {
+    const int i = PER * tid + j;
+    filled[j] = i < p.slots && p.table[i].rank > 0;
+    if (i < p.slots) count[i] = 0;
+  }
+  if (tid == 0) s_slot = -1;
+  bool bad = id >= p.slots;
+  if (bad) id = -1;
+  __syncthreads();
+  count_up(count, id);
+  __syncthreads();
+  int n[PER], tiles = 0;
+#pragma unroll
+  for (int j = 0; j < PER; ++j) {
+    const int i = PER * tid + j;
+    n[j] = i < p.slots ? count[i] : 0;
+    bad |= n[j] && !filled[j];
+    if (!filled[j]) n[j] = 0;
+    tiles += (n[j] + 15) / 16;
+  }
+  if (bad && blockIdx.x == 0 && blockIdx.y == 0) flag(p.status, kStepArgument);
+  int tile = tiles;
+  for (int o = 1; o < 64; o <<= 1) {
+    const int b = __shfl_up(tile, o, 64);
+    if (lane >= o) tile += b;
+  }
+  if (lane == 63) waves[wave] = tile;
+  __syncthreads();
+  tile -= tiles;
+  for (int w = 0; w < wave; ++w) tile += waves[w];
+#pragma unroll
+  for (int j = 0; j < PER; ++j) {
+    const int here = (n[j] + 15) / 16;
+    if (unit >= tile && unit < tile + here) {
+      s_slot = PER * tid + j;
+      s_z = unit - tile;
+    }
+    tile += here;
+  }
+  __syncthreads();
+  *slot = s_slot;
+  if (*slot < 0) return 0;
+  const uint64_t same = __ballot(id == *slot);
+  if (lane == 0) waves[wave] = __popcll(same);
+  __syncthreads();
+  int at = 0, all = 0;
+#pragma unroll
+  for (int w = 0; w < kPrepareWaves; ++w) {
+    all += waves[w];
+    if (w < wave) at += waves[w];
+  }
+  at += (int)__popcll(same & ((1ull << lane) - 1)) - 16 * s_z;
+  if (id == *slot && at >= 0 && at < 16) rows[at] = tid;
+  __syncthreads();
+  return min(16, all - 16 * s_z);
+}
 
 // One row of f32 values as planes [3][tokens][cols], and how many of them it needs (1: its values are
 // BF16).  All threads of a workgroup.
@@ -280,8 +350,9 @@ __device__ __forceinline__ void row_planes(const ProjArgs& p, int t, uint16_t* x
 
 // What the products of a call need beforehand, in one launch.  Workgroups below `firsts`: the first product
 // of up to 16 rows of one adapter with up to `per` of its 16-rank panels (per 1 or 4), the waves' parts of K
-// summed in order.  With an order, a workgroup takes a block of it; without, workgroup (who, panels, z)
-// takes the z-th 16 rows of slot `who`, or (by_token) of the slot of row `who` if no row before has it.
+// summed in order.  With an order, a workgroup takes a block of it, or of up to 1024 rows finds its own
+// (find_block); of up to 64 rows workgroup (who, panels, z) takes the z-th 16 rows of slot `who`, or (by_token) of the
+// slot of row `who` if no row before has it.
 // In a grid of several rows each takes a slice of K and writes its sum to u_parts [slice][tokens][ld]
 // for finish_kernel.  The other workgroups: a row of f32 values each (row_planes).
 template <bool XB, int P>
@@ -290,6 +361,7 @@ __global__ __launch_bounds__(64 * kPrepareWaves) void prepare_kernel(
     bool by_token, uint16_t* x_planes, int* needed) {
   __shared__ f32x4 red[kPrepareWaves][4][64];
   __shared__ int s_rows[kFew];
+  static_assert(sizeof(red) >= kMaxSlots * 4, "counts before, sums after");
   const int tid = threadIdx.x, lane = tid & 63, ln = lane & 15, lq = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   if ((int)blockIdx.x >= firsts) {
@@ -303,6 +375,10 @@ __global__ __launch_bounds__(64 * kPrepareWaves) void prepare_kernel(
     slot = order.blocks[3 * unit];
     n = order.blocks[3 * unit + 2];
     t = order.order[order.blocks[3 * unit + 1] + min(ln, n - 1)];
+  } else if (p.tokens > kFew) {
+    n = find_block(p, unit, reinterpret_cast<int*>(red), s_rows, &slot);
+    if (n == 0) return;
+    t = s_rows[min(ln, n - 1)];
   } else {
     const int tiles = (p.tokens + 15) / 16, who = unit / tiles, z = unit % tiles;
     const int id = lane < p.tokens ? p.ids[lane] : -1;
@@ -1185,8 +1261,10 @@ void launch_project(const ProjArgs& p, hipStream_t s) {
   int firsts = 0, groups = 1, per = 1;
   bool by_token = false;
   if (p.ids && p.tokens > kFew) {
-    order = Order{ints(w.order), ints(w.blocks), ints(w.n_blocks)};
-    order_kernel<<<1, kOrderThreads, 0, s>>>(p, ints(w.order), ints(w.blocks), ints(w.n_blocks));
+    if (p.tokens > kOwnBlocks) {
+      order = Order{ints(w.order), ints(w.blocks), ints(w.n_blocks)};
+      order_kernel<<<1, kOrderThreads, 0, s>>>(p, ints(w.order), ints(w.blocks), ints(w.n_blocks));
+    }
     // (four panels per workgroup share the rows' loads)
     per = 4;
     groups = std::max(1, (max_panels + 3) / 4);
