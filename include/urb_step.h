@@ -36,7 +36,7 @@ extern "C" {
  * of the context, in HBM from urb_proj_set_adapter on.  A x is carried in f32.
  *
  * rows % 16 == 0 and cols % 128 == 0 (the panel layout), rows <= 2^20, cols <= 32768, max_tokens
- * >= 1, adapter_slots <= 4096 and max_rank <= 256 (both 0, or neither), else URB_ERR_SHAPE. */
+ * 1 .. 2^30, adapter_slots <= 4096 and max_rank <= 256 (both 0, or neither), else URB_ERR_SHAPE. */
 typedef struct {
   uint32_t rows;          /* outputs per token */
   uint32_t cols;          /* inputs per token */
@@ -102,13 +102,15 @@ urb_status urb_proj_memory(const urb_proj_ctx *ctx, size_t *weight_bytes, size_t
  *   (n_a, n_b) -> (n_a cos - n_b sin, n_b cos + n_a sin)
  * where pair i is values (i, i + rotary_dim / 2), or (2i, 2i + 1) if interleaved; the other values
  * are n_i.  The angle is an f64 product, so far positions keep their fraction; the norm is not
- * rounded before the rotation.
+ * rounded before the rotation.  The squares are summed in f32 (values of 2^60 and more overflow it), and
+ * |position * inv_freq| must stay below 2^40, where the product still has 2^-13 of a radian.
  *
  * head_dim 2 .. 1024 and even, rotary_dim even and <= head_dim (0 = no rotation), q_heads >= 1,
- * q_heads + k_heads <= 65535, else URB_ERR_SHAPE; eps not finite or <= 0 ->
+ * q_heads + k_heads <= 65535, tokens * (q_heads + k_heads) < 2^31, else URB_ERR_SHAPE; eps not finite or <= 0 ->
  * URB_ERR_INVALID_GEOMETRY.  Strides are in values, from token to token and head to head; a head's
  * values are contiguous.  Heads may be parts of a wider buffer (a fused q/k/v row); an output may
- * be its own input (same address and strides) and must not overlap an input otherwise. */
+ * be its own input (same address and strides) and must not overlap an input otherwise; strides by
+ * which the heads of an output overlap each other -> URB_ERR_SHAPE. */
 typedef struct {
   urb_dtype dtype; /* of q, k and the outputs: BF16, F32 */
   uint32_t q_heads, k_heads;
@@ -149,7 +151,7 @@ urb_status urb_qk_norm_rope(const urb_qk_desc *desc, const void *q, const void *
  * not depend on their order, so a result depends on nothing but the row and its parameters; tokens
  * below half of that unit are never drawn.
  *
- * vocab 1 .. 2^20, max_rows >= 1, else URB_ERR_SHAPE. */
+ * vocab 1 .. 2^20, max_rows 1 .. 2^24, else URB_ERR_SHAPE. */
 typedef struct {
   uint32_t vocab;
   uint32_t max_rows;

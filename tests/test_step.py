@@ -354,6 +354,27 @@ def test_a_row_of_infinities_touches_no_other():
         assert not bool(torch.isfinite(got[[3, 9]]).any())
 
 
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("T", [2, 12, 60, 140])
+def test_infinities_among_rows_with_and_without_an_adapter(dtype, T):
+    # few rows and tiles; adapters of the bad row, of others and none
+    p = Proj("mxfp4", 272, 5120, T, dtype, ranks=(20, 4))
+    x, ids = p.rows_of(T), _mixed(T, 2, p.g)
+    clean = p.p.forward(x.cuda(), ids)
+    for bad, value in ((0, math.inf), (T - 1, -math.inf), (T // 2, math.nan)):
+        for id_ in (-1, 0, 1):
+            ids[bad] = id_
+            here = x.clone()
+            here[bad, 4000] = 1.0
+            want = p.p.forward(here.cuda(), ids)
+            here[bad, 4000] = value
+            got = p.p.forward(here.cuda(), ids)
+            rows = [i for i in range(T) if i != bad]
+            assert torch.equal(got[rows], want[rows])
+            assert not bool(torch.isfinite(got[bad]).any())
+    assert bool(torch.isfinite(clean).all())
+
+
 def test_results_do_not_depend_on_the_other_rows():
     p = Proj("mxfp8", 64, 512, 16, BF16, F32, ranks=(8, 8, 8))
     x, ids = p.rows_of(16).cuda(), _mixed(16, 3, p.g)
@@ -617,6 +638,19 @@ def test_heads_of_more_than_4_gib():
     assert bool((wide[-1, H * D:] == 0).all())
 
 
+def test_outputs_that_overlap_themselves_are_refused():
+    q, w = torch.zeros(4, 3, 64, device="cuda"), torch.ones(64, device="cuda")
+    pos, buf = torch.arange(4).cuda(), torch.zeros(4 * 3 * 64, device="cuda")
+    call = lambda strides, q=q: _status(lambda: step().qk_norm_rope(
+        q, None, w, None, pos[:len(q)], _freq(64), 1e-6, out=(buf.as_strided(q.shape, strides), None)))
+    for strides in ((192, 64, 1), (64, 256, 1)):
+        assert call(strides) == N.OK
+    for strides in ((0, 64, 1), (192, 0, 1), (191, 64, 1), (192, 63, 1), (64, 255, 1), (64, 64, 1), (63, 256, 1)):
+        assert call(strides) == N.ERR_SHAPE
+    assert call((0, 64, 1), q[:1]) == N.OK and call((64, 0, 1), q[:, :1]) == N.OK
+    torch.cuda.synchronize()
+
+
 def test_rotation_wrapper_refuses():
     q, w = torch.zeros(2, 3, 64, device="cuda"), torch.ones(64, device="cuda")
     pos = torch.arange(2).cuda()
@@ -858,6 +892,22 @@ def test_logits_of_more_than_4_gib():
 def test_extreme_temperatures():
     x = _logits(6, 500, _gen(4))
     _check_drawn(x, [0.9] * 6, tau=[1e-45, 1e-30, 1e30, 3e38, 1e-3, 1e3])
+
+
+@pytest.mark.parametrize("V", [64, 3000])
+def test_extreme_temperatures_of_extreme_logits(V):
+    # differences that f32 cannot hold, and multiples of them that it cannot, of tokens with mass
+    tiny, low, high = 2.0 ** -149, torch.finfo(F32).min, torch.finfo(F32).max
+    g = _gen(V)
+    small = tiny * torch.randint(-6, 7, (V,), generator=g)
+    large = torch.where(torch.rand(V, generator=g) < 0.5, low, high)
+    x = torch.stack((small, large, large.clone().fill_(low), small)).cuda()
+    x[2, 5] = high
+    for tau in ([tiny, 3e38, 3e38, 4 * tiny], [2e-38, 1.5e38, 2e30, 1e-30]):
+        for u in (0.0, 0.4, 1.0 - 2.0 ** -24):
+            _check_drawn(x, [u] * 4, tau=tau)
+            _check_drawn(x, [u] * 4, tau=tau, p=[0.8, 0.9, 0.95, 0.5])
+            _check_drawn(x, [u] * 4, tau=tau, k=[V - 1] * 4, min_p=[0.2, 0.1, 0.0, 0.5])
 
 
 def test_parameters_out_of_range_are_reported():

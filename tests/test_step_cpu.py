@@ -113,3 +113,13 @@ def _rotate(tokens=2, q=PTR, k=PTR, weight=PTR, positions=PTR, freq=PTR, **chang
 ])
 def test_rotation_refuses(change, status):
     assert _rotate(**change) == status
+
+
+@pytest.mark.parametrize("change", [
+    dict(), dict(q_out_token_stride=255), dict(q_out_token_stride=256, q_out_head_stride=63),
+    dict(q_out_token_stride=256, k_out_token_stride=0), dict(q_out_token_stride=64, q_out_head_stride=127),
+    dict(q_out_token_stride=0, q_out_head_stride=1 << 40),
+    dict(q_out_token_stride=1 << 63, q_out_head_stride=1 << 63),
+])
+def test_rotation_refuses_outputs_that_overlap_themselves(change):
+    assert _rotate(**change) == N.ERR_SHAPE

@@ -82,7 +82,9 @@ struct Mass {
     return (u64)__double_as_longlong(fma(e, scale, 0x1p52)) & 0xfffffffffffffull;
   }
   // (m - l) / tau in bins of 36.25 / 4096; from the last one on masses are zero.  The f32 steps keep the
-  // logits' order; a NaN logit gives NaN.
+  // logits' order; a NaN logit gives NaN.  For temperatures in `usual`: beyond, the difference of two
+  // logits or its multiple may overflow f32 though the token has mass, and rows go by radix.
+  static __device__ __forceinline__ bool usual(float tau) { return tau > 1e-30f && tau < 1e30f; }
   static constexpr int kBins = 4096;
   static constexpr float kBinRange = 36.25f;
   __device__ __forceinline__ float place(float l) const {
@@ -547,6 +549,10 @@ __device__ __forceinline__ RowRecord find_cut(const Work& w, int row, const RowP
   static_assert(kBins == kGroup * 64 && kGroup == 64, "a lane per group, then one per bin");
   RowRecord rec{};
   const bool by_count = p.top_k > 0 && p.top_k < V, by_mass = p.top_p < 1.0f;
+  if (!Mass::usual(p.tau)) {
+    rec.mode = kByRadix;
+    return rec;
+  }
   if (!by_count && !by_mass) {
     rec.mode = kNoCut;
     return rec;
@@ -879,7 +885,8 @@ __global__ __launch_bounds__(kRowThreads) void sample_draw_kernel(SampleArgs a, 
   const int i = s_found * kSpan + tid - r.lead;
   if (tid < kSpan && i >= 0 && i < r.V) {
     const float l = load_logit<BF16>(r.base, i);
-    const float z = m.place(l);
+    // (a whole list has a cut: its first token is kept)
+    const float z = SMALL ? 0.0f : m.place(l);
     if (z < (float)(kBins - 1) && (cut == ~0ull ? z < (float)rec.bin : order_of(l, i) >= cut)) {
       e = m.e(l);
       if (e >= min_e) f = m.fixed(e);

@@ -6,6 +6,7 @@
 
 #include <algorithm>
 #include <new>
+#include <utility>
 
 #include "urb_kernels.hpp"
 #include "urb_step.hpp"
@@ -29,6 +30,18 @@ bool finite_host(float v) { return v == v && v <= 3.4028235e38f && v >= -3.40282
 bool on_device(int device) {
   int now = -1;
   return hipGetDevice(&now) == hipSuccess && now == device;
+}
+
+// Whether the heads of an output lie apart: [tokens][heads] rows of dim values, either stride the larger.
+bool heads_apart(uint64_t tokens, uint64_t token_stride, uint64_t heads, uint64_t head_stride, uint64_t dim) {
+  if (token_stride < head_stride) {
+    std::swap(tokens, heads);
+    std::swap(token_stride, head_stride);
+  }
+  if (heads > 1 && head_stride < dim) return false;
+  if (tokens == 1) return true;
+  // (the larger stride against what the others span, without the product)
+  return token_stride >= dim && (heads == 1 || (token_stride - dim) / (heads - 1) >= head_stride);
 }
 
 // Waits for the stream, then reads and clears a status word (written by kernels of that stream).
@@ -319,6 +332,10 @@ urb_status urb_qk_norm_rope(const urb_qk_desc* d, const void* q, const void* k,
   auto aligned = [&](const void* p) { return reinterpret_cast<uintptr_t>(p) % vb == 0; };
   if (!aligned(q) || !aligned(q_out) || (d->k_heads && (!aligned(k) || !aligned(k_out))))
     return URB_ERR_ARGUMENT;
+  if (!heads_apart(tokens, d->q_out_token_stride, d->q_heads, d->q_out_head_stride, d->head_dim) ||
+      (d->k_heads &&
+       !heads_apart(tokens, d->k_out_token_stride, d->k_heads, d->k_out_head_stride, d->head_dim)))
+    return URB_ERR_SHAPE;
   urb::RotateArgs a{};
   a.q = urb::HeadRows{q, q_out, q_weight, d->q_token_stride, d->q_head_stride,
                       d->q_out_token_stride, d->q_out_head_stride};
