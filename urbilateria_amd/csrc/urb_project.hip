@@ -146,14 +146,15 @@ __device__ __forceinline__ int count_up(int* count, int id) {
   return id >= 0 ? atomicAdd(&count[id], 1) : at;
 }
 
-// The rows in order of their adapters, and the blocks of up to 16 rows of one adapter: slot, first place
-// in the order, rows.  One workgroup; `order` holds `tokens` entries, `blocks` (3 ints each) at most
-// order_blocks().  Which row of an adapter comes first is left to chance: no sum goes over rows.
+// The rows in order of their adapters, those without one last, and the blocks of up to 16 rows of one
+// adapter: slot, first place in the order, rows.  One workgroup; `order` holds `tokens` entries, `blocks`
+// (3 ints each) at most order_blocks().  Which row of an adapter comes first is left to chance: no sum goes
+// over rows.
 __global__ __launch_bounds__(kOrderThreads) void order_kernel(ProjArgs p, int* order, int* blocks,
                                                               int* n_blocks) {
   __shared__ int count[kMaxSlots];  // rows per slot, then the place of its next one (-1: an empty slot)
   __shared__ int row_at[kMaxSlots + 1], tile_at[kMaxSlots];  // first row and block of each slot
-  __shared__ int s_blocks;
+  __shared__ int s_blocks, s_idle;
   __shared__ int waves[2][kOrderThreads / 64];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   for (int i = tid; i < p.slots; i += kOrderThreads) count[i] = 0;
@@ -214,6 +215,7 @@ __global__ __launch_bounds__(kOrderThreads) void order_kernel(ProjArgs p, int* o
   if (tid == kOrderThreads - 1) {
     *n_blocks = tile + tiles;
     s_blocks = tile + tiles;
+    s_idle = row + rows;
   }
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
@@ -240,9 +242,15 @@ __global__ __launch_bounds__(kOrderThreads) void order_kernel(ProjArgs p, int* o
 #pragma unroll
   for (int j = 0; j < PER; ++j) {
     if (j * kOrderThreads >= p.tokens) break;
+    const int t = j * kOrderThreads + tid;
     const int id = ids[j] >= 0 && count[ids[j]] >= 0 ? ids[j] : -1;
-    const int at = count_up(count, id);
-    if (id >= 0) order[at] = j * kOrderThreads + tid;
+    int at = count_up(count, id);
+    const uint64_t idle = __ballot(id < 0 && t < p.tokens);
+    int first = 0;
+    if (lane == 0 && idle) first = atomicAdd(&s_idle, (int)__popcll(idle));
+    first = __shfl(first, 0, 64);
+    if (id < 0) at = first + (int)__popcll(idle & ((1ull << lane) - 1));
+    if (t < p.tokens) order[at] = t;
   }
 }
 
@@ -252,9 +260,10 @@ struct FirstProduct {
   uint16_t* planes;
   int ld;
 };
-// What order_kernel found (order NULL: few rows).
+// The rows in order of their adapters (NULL: few rows), and order_kernel's blocks (NULL: each workgroup finds
+// its own and writes its part of the order).
 struct Order {
-  const int* order;
+  int* order;
   const int* blocks;
   const int* n_blocks;
 };
@@ -262,12 +271,14 @@ struct Order {
 constexpr int kPrepareWaves = 16;
 constexpr int kOwnBlocks = 64 * kPrepareWaves;  // most rows whose blocks each workgroup finds for itself
 
-// The unit-th block of up to 16 rows of one adapter (slots ascending, rows ascending) of at most
-// kOwnBlocks rows: what order_kernel finds for all, by each workgroup for itself, which costs less than that
-// launch (calls of 131 and of 1000 rows: 68.6 -> 66.0 and 77.1 -> 74.2 us).  Returns the rows in it (0: no such
-// block), their numbers in rows[].
-__device__ __forceinline__ int find_block(const ProjArgs& p, int unit, int* count, int* rows, int* slot) {
-  __shared__ int waves[kPrepareWaves], s_slot, s_z;
+// The unit-th block of up to 16 rows of one adapter (slots ascending, rows ascending, at last the blocks
+// of rows without an adapter) of at most kOwnBlocks rows: what order_kernel finds for all, by each workgroup
+// for itself, which costs less than that launch (calls of 131 and of 1000 rows: 68.6 -> 66.0 and 77.1 -> 74.2
+// us).  Returns the rows in it (0: no such block), their numbers in rows[], its slot (-1: none) and
+// its first place in the order.
+__device__ __forceinline__ int find_block(const ProjArgs& p, int unit, int* count, int* rows, int* slot,
+                                          int* place) {
+  __shared__ int waves[kPrepareWaves], s_slot, s_z, s_place;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   int id = tid < p.tokens ? p.ids[tid] : -1;
@@ -281,54 +292,67 @@ __device__ __forceinline__ int find_block(const ProjArgs& p, int unit, int* coun
   }
   if (tid == 0) s_slot = -1;
   bool bad = id >= p.slots;
-  if (bad) id = -1;
+  if (bad || id < 0) id = -1;
   __syncthreads();
   count_up(count, id);
   __syncthreads();
-  int n[PER], tiles = 0;
+  // running sums of rows (high half) and of blocks (low half)
+  int n[PER], sums = 0;
 #pragma unroll
   for (int j = 0; j < PER; ++j) {
     const int i = PER * tid + j;
     n[j] = i < p.slots ? count[i] : 0;
-    bad |= n[j] && !filled[j];
-    if (!filled[j]) n[j] = 0;
-    tiles += (n[j] + 15) / 16;
+    if (!filled[j]) {
+      bad |= n[j] != 0;
+      n[j] = 0;
+      if (i < p.slots) count[i] = -1;
+    }
+    sums += (n[j] << 16) + (n[j] + 15) / 16;
   }
   if (bad && blockIdx.x == 0 && blockIdx.y == 0) flag(p.status, kStepArgument);
-  int tile = tiles;
+  int upto = sums;
   for (int o = 1; o < 64; o <<= 1) {
-    const int b = __shfl_up(tile, o, 64);
-    if (lane >= o) tile += b;
+    const int b = __shfl_up(upto, o, 64);
+    if (lane >= o) upto += b;
   }
-  if (lane == 63) waves[wave] = tile;
+  if (lane == 63) waves[wave] = upto;
   __syncthreads();
-  tile -= tiles;
-  for (int w = 0; w < wave; ++w) tile += waves[w];
-#pragma unroll
-  for (int j = 0; j < PER; ++j) {
-    const int here = (n[j] + 15) / 16;
-    if (unit >= tile && unit < tile + here) {
-      s_slot = PER * tid + j;
-      s_z = unit - tile;
-    }
-    tile += here;
-  }
-  __syncthreads();
-  *slot = s_slot;
-  if (*slot < 0) return 0;
-  const uint64_t same = __ballot(id == *slot);
-  if (lane == 0) waves[wave] = __popcll(same);
-  __syncthreads();
-  int at = 0, all = 0;
+  int at = upto - sums, all = 0;
 #pragma unroll
   for (int w = 0; w < kPrepareWaves; ++w) {
-    all += waves[w];
     if (w < wave) at += waves[w];
+    all += waves[w];
   }
-  at += (int)__popcll(same & ((1ull << lane) - 1)) - 16 * s_z;
-  if (id == *slot && at >= 0 && at < 16) rows[at] = tid;
+#pragma unroll
+  for (int j = 0; j < PER; ++j) {
+    const int next = at + (n[j] << 16) + (n[j] + 15) / 16;
+    if (unit >= (at & 0xffff) && unit < (next & 0xffff)) {
+      s_slot = PER * tid + j;
+      s_z = unit - (at & 0xffff);
+      s_place = at >> 16;
+    }
+    at = next;
+  }
+  if (id >= 0 && count[id] < 0) id = -1;
   __syncthreads();
-  return min(16, all - 16 * s_z);
+  *slot = s_slot;
+  const bool idle = *slot < 0;
+  const int z = idle ? unit - (all & 0xffff) : s_z;
+  *place = (idle ? all >> 16 : s_place) + 16 * z;
+  const bool mine = tid < p.tokens && id == *slot;
+  const uint64_t same = __ballot(mine);
+  if (lane == 0) waves[wave] = (int)__popcll(same);
+  __syncthreads();
+  int first = 0, total = 0;
+#pragma unroll
+  for (int w = 0; w < kPrepareWaves; ++w) {
+    total += waves[w];
+    if (w < wave) first += waves[w];
+  }
+  first += (int)__popcll(same & ((1ull << lane) - 1)) - 16 * z;
+  if (mine && first >= 0 && first < 16) rows[first] = tid;
+  __syncthreads();
+  return max(0, min(16, total - 16 * z));
 }
 
 // One row of f32 values as planes [3][tokens][cols], and how many of them it needs (1: its values are
@@ -370,14 +394,16 @@ __global__ __launch_bounds__(64 * kPrepareWaves) void prepare_kernel(
   }
   const int group = blockIdx.x % groups, unit = blockIdx.x / groups;
   int slot, n, t;
-  if (order.order) {
+  if (order.blocks) {
     if (unit >= *order.n_blocks) return;
     slot = order.blocks[3 * unit];
     n = order.blocks[3 * unit + 2];
     t = order.order[order.blocks[3 * unit + 1] + min(ln, n - 1)];
   } else if (p.tokens > kFew) {
-    n = find_block(p, unit, reinterpret_cast<int*>(red), s_rows, &slot);
-    if (n == 0) return;
+    int place;
+    n = find_block(p, unit, reinterpret_cast<int*>(red), s_rows, &slot, &place);
+    if (group == 0 && blockIdx.y == 0 && tid < n) order.order[place + tid] = s_rows[tid];
+    if (n == 0 || slot < 0) return;
     t = s_rows[min(ln, n - 1)];
   } else {
     const int tiles = (p.tokens + 15) / 16, who = unit / tiles, z = unit % tiles;
@@ -491,19 +517,22 @@ __global__ __launch_bounds__(256) void finish_kernel(ProjArgs p, FirstProduct u,
 // The slots of a tile's rows (-1: none) and its distinct filled ones, in LDS.
 template <int MAX>
 struct TileSlots {
-  int ids[MAX];
+  int ids[MAX], rows[MAX];
   int2 list[MAX];  // slot, rank units
   int n;
   uint32_t seen[kMaxSlots / 32];
 };
 template <int MAX>
-__device__ __forceinline__ void find_slots(const ProjArgs& p, int t0, int count, TileSlots<MAX>& s) {
+__device__ __forceinline__ void find_slots(const ProjArgs& p, const int* order, int t0, int count,
+                                           TileSlots<MAX>& s) {
   const int tid = threadIdx.x;
   if (tid == 0) s.n = 0;
   for (int i = tid; i < kMaxSlots / 32; i += blockDim.x) s.seen[i] = 0;
   __syncthreads();
   for (int i = tid; i < MAX; i += blockDim.x) {
-    int id = i < count ? p.ids[t0 + i] : -1;
+    const int t = t0 + min(i, count - 1), row = order ? order[t] : t;
+    s.rows[i] = row;
+    int id = i < count ? p.ids[row] : -1;
     int rank = 0;
     if (id >= p.slots || (id >= 0 && (rank = p.table[id].rank) == 0)) id = -1;
     s.ids[i] = id;
@@ -529,8 +558,7 @@ __device__ __forceinline__ bf16x8 load_up(const uint16_t* b, int r, int units) {
 // time, so the next operands are loaded before the present ones are used.
 template <int P, int MAX, int NP, int MB>
 __device__ __forceinline__ void add_adapters(const ProjArgs& p, const TileSlots<MAX>& s,
-                                             const FirstProduct& u, int panel0, int panels, int t0,
-                                             int first, int part, int parts, f32x4 (&acc)[NP][MB]) {
+                                             const FirstProduct& u, int panel0, int panels, int first, int part, int parts, f32x4 (&acc)[NP][MB]) {
   const int lane = threadIdx.x & 63, ln = lane & 15, lq = lane >> 4;
   int i = -1, r = 0, slot = 0, units = 0;
   // the next 32 ranks: of this slot or the next of this part; false past the last
@@ -571,7 +599,7 @@ __device__ __forceinline__ void add_adapters(const ProjArgs& p, const TileSlots<
       for (int pl = 0; pl < P; ++pl) {
         uint4 x = make_uint4(0, 0, 0, 0);
         if (mine && from + lq < to)
-          x = ldg16(u.planes + ((size_t)(t0 + local) * P + pl) * u.ld + 8 * (from + lq));
+          x = ldg16(u.planes + ((size_t)s.rows[local] * P + pl) * u.ld + 8 * (from + lq));
         v[pl] = __builtin_bit_cast(bf16x8, x);
       }
 #pragma unroll
@@ -670,7 +698,7 @@ __global__ __launch_bounds__(64 * kSplitWaves) void split_kernel(ProjArgs p, Fir
     if (s0 + d < s1) fetch(d, s0 + d);
   if (s0 < s1) fetch_rows(0, s0);
   if (p.ids) {
-    find_slots(p, t0, count, slots);
+    find_slots(p, nullptr, t0, count, slots);
     if constexpr (ALONE) {
       if (blockIdx.x == 0 && (int)threadIdx.x < count) {
         const int id = p.ids[t0 + threadIdx.x];
@@ -699,7 +727,7 @@ __global__ __launch_bounds__(64 * kSplitWaves) void split_kernel(ProjArgs p, Fir
         }
       }
     } else {
-      add_adapters<YB ? 2 : 3>(p, slots, u, panel0, panels, t0, 0, wave, kSplitWaves, acc);
+      add_adapters<YB ? 2 : 3>(p, slots, u, panel0, panels, 0, wave, kSplitWaves, acc);
     }
   }
   for (int i0 = s0; i0 < s1; i0 += R) {
@@ -808,10 +836,14 @@ __device__ __forceinline__ bf16x8 tile_operand(const uint4& q, float sc, int par
 }
 
 // Rows in BF16 planes: plane i of row t is `plane` bytes after plane i - 1 of it; `planes`: how many of them
-// each row needs (NULL: one).
+// each row needs (NULL: one).  `order`: the rows by adapter (NULL: as they lie), so that a block of 16 holds
+// rows of one or two adapters instead of as many as the batch has: each adapter of a block multiplies all of it
+// (16 adapters of rank 64 mixed over 1000 rows, BF16, 4096 -> 4096: 96.7 -> 71.7 us; 32 over 3000 178 -> 132;
+// already in order 71.0 and 71.2).
 struct TileRows {
   size_t plane;
   const int* planes;
+  const int* order;
 };
 
 // Tiles by workgroup.  Workgroup b runs on XCD b % 8, which has an L2 of its own: the tiles are cut into
@@ -869,20 +901,23 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(
   }
   int planes = 1;
   if (rows.planes) {
-    for (int i = lane; i < count; i += 64) planes = max(planes, rows.planes[t0 + i]);
+    for (int i = lane; i < count; i += 64) planes = max(planes, rows.planes[rows.order ? rows.order[t0 + i] : t0 + i]);
     for (int o = 32; o > 0; o >>= 1) planes = max(planes, __shfl_xor(planes, o, 64));
     planes = __builtin_amdgcn_readfirstlane(planes);
   }
   // this lane's copies: rows 4 (wave + WAVES i) + lane / 16, the same chunk of each
   const int copy_row = 4 * wave + lane / 16;
   const int copy_chunk = (lane & 15) ^ x_swizzle<FMT>(copy_row);
-  const uint8_t* const xt = reinterpret_cast<const uint8_t*>(p.x) + (size_t)t0 * p.x_stride * 2 +
+  const uint8_t* const xt = reinterpret_cast<const uint8_t*>(p.x) +
+                            (rows.order ? 0 : (size_t)t0 * p.x_stride * 2) +
                             (size_t)begin * (2 * kTileStep);
   uint32_t copy_off[COPIES];
 #pragma unroll
-  for (int i = 0; i < COPIES; ++i)
-    copy_off[i] = (uint32_t)min(copy_row + 4 * WAVES * i, count - 1) * (uint32_t)(p.x_stride * 2) +
+  for (int i = 0; i < COPIES; ++i) {
+    const int at = min(copy_row + 4 * WAVES * i, count - 1);
+    copy_off[i] = (uint32_t)(rows.order ? rows.order[t0 + at] : at) * (uint32_t)(p.x_stride * 2) +
                   16u * copy_chunk;
+  }
   // the rows of step s, plane pl: copies `first` .. first + HALF
   auto load_rows = [&](uint4* st, int first, int s, int pl) {
     const uint8_t* from = xt + pl * rows.plane + (size_t)s * (2 * kTileStep);
@@ -963,7 +998,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(
   };
 
   fetch(slab[0], 0);
-  if (p.ids) find_slots(p, t0, count, slots);
+  if (p.ids) find_slots(p, rows.order, t0, count, slots);
   if constexpr (FMT != kFmtMXFP4) fetch(slab[1], 1);  // (a step has two slabs at least)
   fetch_scales(sc[0], 0);
 #pragma unroll
@@ -992,12 +1027,13 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(
     if (s == steps) break;
   }
   if (p.ids)
-    add_adapters<YB ? 2 : 3>(p, slots, u, panel0, panels, t0, wm * MB * 16, (int)blockIdx.y,
+    add_adapters<YB ? 2 : 3>(p, slots, u, panel0, panels, wm * MB * 16, (int)blockIdx.y,
                              (int)gridDim.y, acc);
 #pragma unroll
   for (int m = 0; m < MB; ++m) {
-    const int local = (wm * MB + m) * 16 + ln, t = t0 + local;
+    const int local = (wm * MB + m) * 16 + ln;
     if ((wm * MB + m) * 16 >= count) break;
+    const int t = p.ids ? slots.rows[local] : t0 + local;
 #pragma unroll
     for (int q = 0; q < NP; ++q) {
       const int panel = panel0 + q;
@@ -1180,8 +1216,8 @@ void launch_types(const ProjArgs& p, const Pass& a, hipStream_t s) {
   }
 }
 
-// Most blocks of 16 rows of one adapter.
-int order_blocks(int tokens, int slots) { return tokens / 16 + std::min(tokens, slots); }
+// Most blocks of 16 rows of one adapter or of none.
+int order_blocks(int tokens, int slots) { return tokens / 16 + std::min(tokens, slots + 1); }
 
 // Slices of K of the first products (1: whole).  One workgroup pulls its rows and A at what a CU can, so
 // long rows of f32 are cut, where the launch that adds the slices also makes the rows' planes (a call of 64,
@@ -1203,7 +1239,7 @@ struct WorkLayout {
       at += (bytes + 255) / 256 * 256;
       return here;
     };
-    const bool tiles = tokens >= kTileTokens, sorted = p.slots && tokens > kFew;
+    const bool tiles = tokens >= kTileTokens, sorted = tokens > kFew;
     u = take(p.slots ? (size_t)tokens * 16 * rank_panels(p.max_rank) * (p.y_bf16 ? 4 : 6) : 0);
     u_parts = take(p.slots ? (size_t)first_slices(tokens, p) * tokens * 16 * rank_panels(p.max_rank) * 4 : 0);
     order = take(sorted ? (size_t)tokens * 4 : 0);
@@ -1254,13 +1290,14 @@ void launch_project(const ProjArgs& p, hipStream_t s) {
   // under what a launch and its wait cost (5 us: 4096 -> 2048, BF16, rank 16, 11.9 -> 9.3 us).
   const bool alone = p.ids && p.slots && p.tokens * 16 * max_panels <= kAloneRanks &&
                      (double)p.rows / 16 * p.tokens * 32 * max_panels * p.cols <= kAloneBytes;
-  Pass a{tiles, alone, {}, {0, nullptr}, u, reinterpret_cast<float*>(work + w.parts)};
+  Pass a{tiles, alone, {}, {}, u, reinterpret_cast<float*>(work + w.parts)};
   if (tiles) a.shape = tile_shape(p.tokens, p.rows, p.cols, p.x_bf16 ? 1 : 3);
   // the first products (of ids without any slot: one workgroup or the order, which report them)
   Order order{};
   int firsts = 0, groups = 1, per = 1;
   bool by_token = false;
   if (p.ids && p.tokens > kFew) {
+    order.order = ints(w.order);
     if (p.tokens > kOwnBlocks) {
       order = Order{ints(w.order), ints(w.blocks), ints(w.n_blocks)};
       order_kernel<<<1, kOrderThreads, 0, s>>>(p, ints(w.order), ints(w.blocks), ints(w.n_blocks));
@@ -1299,8 +1336,10 @@ void launch_project(const ProjArgs& p, hipStream_t s) {
   if (planes) {
     q.x = planes;
     q.x_stride = p.cols;
-    a.rows = TileRows{(size_t)p.tokens * p.cols * 2, ints(w.needed)};
+    a.rows = TileRows{(size_t)p.tokens * p.cols * 2, ints(w.needed), nullptr};
   }
+  // (in order a tile's rows may lie anywhere: their offsets of 32 bits must reach all of them)
+  if (tiles && (uint64_t)p.tokens * q.x_stride < (1ull << 31)) a.rows.order = order.order;
   if (p.format == kFmtBF16) launch_types<kFmtBF16>(q, a, s);
   else if (p.format == kFmtMXFP4) launch_types<kFmtMXFP4>(q, a, s);
   else launch_types<kFmtMXFP8>(q, a, s);
