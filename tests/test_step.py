@@ -238,6 +238,15 @@ def test_rows_far_apart(dtype, stride):
     p.check(y, x, ids)
 
 
+def test_many_rows_farther_apart_than_32_bit_offsets():
+    T, cols, stride = 600, 128, (1 << 22) - 8
+    p = Proj("bf16", 48, cols, T, BF16, F32, ranks=(8, 9, 20))
+    x, ids = p.rows_of(T).cuda(), _mixed(T, 3, p.g)
+    far = torch.empty((T - 1) * stride + cols, dtype=BF16, device="cuda").as_strided((T, cols), (stride, 1))
+    far.copy_(x)
+    p.check(p.p.forward(far, ids), x, ids)
+
+
 def test_a_matrix_of_more_than_4_gib():
     rows, cols = 65536 + 64, 32768
     w = torch.randn(rows, cols, device="cuda", dtype=BF16,

@@ -11,9 +11,14 @@
 // zero for a whole operand (rows whose values are BF16 already) are skipped.  u is split the
 // same way, into two planes (16 bits) where the outputs are BF16, three where they are f32.
 //
-// A tile may hold rows of any adapters: each distinct adapter of the tile multiplies the tile's u with
-// the other adapters' rows set to zero.  A row has one adapter, so the order in which a tile takes its
-// adapters changes no sum, and a row's result does not depend on the rows beside it.
+// A tile may hold rows of any adapters: each distinct adapter of a block of 16 rows multiplies the block's
+// u with the other adapters' rows set to zero.  A row has one adapter, so the order in which a tile takes
+// its adapters changes no sum, and a row's result does not depend on the rows beside it.
+//
+// What bounds it.  Few rows: the weights' bytes (1 BF16 row, 16384 x 8192: 44.3 us without adapters, 6.1
+// TB/s); with adapters the launch of the first products before it and its latency.  Many: the matrix
+// instructions (4096 rows of 7168 -> 7168, BF16: 346 to 358 us without adapters, 1.2 PFLOP/s).  f32 rows whose
+// values need all 24 bits cost three products.
 #include "urb_panel.hpp"
 #include "urb_step.hpp"
 
@@ -21,7 +26,10 @@ namespace urb {
 
 namespace {
 
-constexpr int kTileTokens = 17;   // rows of a call that takes tiles
+// Rows of a call that takes tiles.  Below, one block of 16 rows per workgroup and the weights read once; a
+// second block reads them again (24 BF16 rows, 8192 -> 16384: 82.2 us, tiles 47.2; MXFP8, 6144 -> 9232: 31 and
+// 17.4; only of 16 M values in BF16 10.3 and 12.3).
+constexpr int kTileTokens = 17;
 constexpr int kMaxSlices = 16;    // most slices of K
 
 // __builtin_amdgcn_sched_barrier: VALU, SALU and LDS reads may cross; loads, LDS stores, MFMAs stay.
@@ -408,7 +416,8 @@ __global__ __launch_bounds__(64 * kPrepareWaves) void prepare_kernel(
   } else {
     const int tiles = (p.tokens + 15) / 16, who = unit / tiles, z = unit % tiles;
     const int id = lane < p.tokens ? p.ids[lane] : -1;
-    if (blockIdx.x == 0 && blockIdx.y == 0 && wave == 0 && id >= 0 && (id >= p.slots || p.table[id].rank == 0))
+    if (blockIdx.x == 0 && blockIdx.y == 0 && wave == 0 && id >= 0 &&
+        (id >= p.slots || p.table[id].rank == 0))
       flag(p.status, kStepArgument);
     slot = by_token ? __builtin_amdgcn_readlane(id, who) : who;
     if (slot < 0 || slot >= p.slots) return;
@@ -486,8 +495,8 @@ __global__ __launch_bounds__(64 * kPrepareWaves) void prepare_kernel(
 constexpr int kFinishThreads = 1024;
 // The slices' sums of a row's first product, in order, as planes; and the row's own planes (x_planes).
 template <int P>
-__global__ __launch_bounds__(kFinishThreads) void finish_kernel(ProjArgs p, FirstProduct u, const float* u_parts,
-                                                     int slices, uint16_t* x_planes, int* needed) {
+__global__ __launch_bounds__(kFinishThreads) void finish_kernel(
+    ProjArgs p, FirstProduct u, const float* u_parts, int slices, uint16_t* x_planes, int* needed) {
   const int t = blockIdx.x;
   const int id = p.ids[t], r = 8 * threadIdx.x;
   AdapterEntry e{0, 0.0f};
@@ -560,7 +569,8 @@ __device__ __forceinline__ bf16x8 load_up(const uint16_t* b, int r, int units) {
 // time, so the next operands are loaded before the present ones are used.
 template <int P, int MAX, int NP, int MB>
 __device__ __forceinline__ void add_adapters(const ProjArgs& p, const TileSlots<MAX>& s,
-                                             const FirstProduct& u, int panel0, int panels, int first, int part, int parts, f32x4 (&acc)[NP][MB]) {
+                                             const FirstProduct& u, int panel0, int panels, int first,
+                                             int part, int parts, f32x4 (&acc)[NP][MB]) {
   const int lane = threadIdx.x & 63, ln = lane & 15, lq = lane >> 4;
   int i = -1, r = 0, slot = 0, units = 0;
   // the next 32 ranks: of this slot or the next of this part; false past the last
@@ -679,8 +689,8 @@ __global__ __launch_bounds__(64 * kSplitWaves) void split_kernel(ProjArgs p, Fir
   for (int q = 0; q < NP; ++q)
 #pragma unroll
     for (int m = 0; m < MB; ++m) acc[q][m] = f32x4{0.f, 0.f, 0.f, 0.f};
-  // Weights DW steps ahead in a ring of R slots, rows one step ahead.  (Rows loaded where they are used
-  // left every step waiting for the L2: 24 rows, MXFP8, 6144 -> 9232 at 27 us.)
+  // Weights DW steps ahead in a ring of R slots, rows one step ahead (loaded where they are used, every
+  // step waits for the L2).
   constexpr int R = FMT == kFmtBF16 ? 2 : 4, DW = R - 1;
   BRaw<FMT> ring[R][NP];
   XRaw<XB> xr[2][4][MB];
@@ -839,9 +849,9 @@ __device__ __forceinline__ bf16x8 tile_operand(const uint4& q, float sc, int par
 
 // Rows in BF16 planes: plane i of row t is `plane` bytes after plane i - 1 of it; `planes`: how many of them
 // each row needs (NULL: one).  `order`: the rows by adapter (NULL: as they lie), so that a block of 16 holds
-// rows of one or two adapters instead of as many as the batch has: each adapter of a block multiplies all of it
-// (16 adapters of rank 64 mixed over 1000 rows, BF16, 4096 -> 4096: 96.7 -> 71.7 us; 32 over 3000 178 -> 132;
-// already in order 71.0 and 71.2).
+// rows of one or two adapters instead of as many as the batch has: each adapter of a block multiplies all
+// of it (16 adapters of rank 64 mixed over 1000 rows, BF16, 4096 -> 4096: 96.7 -> 71.7 us; 32 over 3000 178 ->
+// 132; already in order 71.0 and 71.2).
 struct TileRows {
   size_t plane;
   const int* planes;
@@ -903,7 +913,8 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(
   }
   int planes = 1;
   if (rows.planes) {
-    for (int i = lane; i < count; i += 64) planes = max(planes, rows.planes[rows.order ? rows.order[t0 + i] : t0 + i]);
+    for (int i = lane; i < count; i += 64)
+      planes = max(planes, rows.planes[rows.order ? rows.order[t0 + i] : t0 + i]);
     for (int o = 32; o > 0; o >>= 1) planes = max(planes, __shfl_xor(planes, o, 64));
     planes = __builtin_amdgcn_readfirstlane(planes);
   }
@@ -1126,9 +1137,9 @@ TileShape tile_shape(int tokens, int rows, int cols, int planes) {
   t.row_tiles = (tokens + 16 * t.blocks - 1) / (16 * t.blocks);
   // Panels per wave and slices of K by the time of the CU with the most workgroups.  Measured: a step of
   // 128 x 256 x 128 takes a workgroup 2.0 us alone on its CU (192 outputs 1.62) and two 1.72 each, smaller
-  // ones 0.9 at least (loads' latency); 2 us to fill and drain a workgroup; joining slices 4 us and their traffic.  (1000
-  // rows of 4096 -> 6144: 192 tiles of 256 outputs 66 us, 256 of 192 outputs 56; 4096 rows of 7168 -> 7168:
-  // 349 and 371.)
+  // ones 0.9 at least (loads' latency); 2 us to fill and drain a workgroup; joining slices 4 us and their
+  // traffic.  (1000 rows of 4096 -> 6144: 192 tiles of 256 outputs 66 us, 256 of 192 outputs 56; 4096 rows of
+  // 7168 -> 7168: 349 and 371.)
   const int steps = cols / kTileStep;
   double best = 0;
   for (int np = 4; np >= 3; --np) {

@@ -2,7 +2,8 @@
 //
 // A head's row h of D values: n = h / sqrt(mean(h^2) + eps) * w, then the first R values turned in
 // pairs by position * inv_freq.  Every value is read once and written once, so the kernel is bound by
-// HBM; the norm's sum stays in the lanes that hold the row.
+// HBM; the norm's sum stays in the lanes that hold the row.  32768 tokens of 18 heads of 256 in BF16 (604 MB):
+// 128 us, 4.7 TB/s, where a large copy reaches 5.0; 2000 tokens in f32 (61 MB): 14.5 us; a token 3.6.
 //
 // The angle is the f64 product of position and frequency (an f32 product has lost the fraction of a
 // turn at position 2^24), reduced to [-pi/4, pi/4] with a two-part pi/2 and evaluated by the Taylor
@@ -56,7 +57,9 @@ __device__ __forceinline__ void store_one(void* p, size_t i, float v) {
   else reinterpret_cast<float*>(p)[i] = v;
 }
 
-// Any head_dim, alignment and stride: one wave per head row, a value or a pair per lane and step.
+// Any head_dim, alignment and stride: one wave per head row, a value or a pair per lane and step (on heads
+// that the wide kernel takes 4.3 us against 4.1 for a token, 24 against 10.7 for 515, 548 against 138 for
+// 32768).
 template <bool BF16>
 __global__ __launch_bounds__(256) void rotate_any_kernel(RotateArgs a) {
   const uint64_t row = (uint64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
@@ -116,9 +119,10 @@ __device__ __forceinline__ void store8(uint8_t* p, const float (&v)[8]) {
 }
 
 // Sixteen-byte heads: `span` (a power of two) lanes hold a head row, 16 values each, loaded as two
-// eights that hold both values of every pair: eights u and R / 16 + u of the turned part, or neighbours.  A lane's place in its
-// row is the same for all its rows, so its weights stay in registers; a workgroup takes all heads of
-// `group` tokens (blockIdx.y: a part of them), whose cosines and sines it computes once into LDS.
+// eights that hold both values of every pair: eights u and R / 16 + u of the turned part, or neighbours.
+// A lane's place in its row is the same for all its rows, so its weights stay in registers; a workgroup
+// takes all heads of `group` tokens (blockIdx.y: a part of them), whose cosines and sines it computes once
+// into LDS.
 template <bool BF16, bool INTER>
 __global__ __launch_bounds__(256) void rotate_wide_kernel(RotateArgs a, int span, int group,
                                                           int parts) {

@@ -3,8 +3,8 @@
 // All three filters keep a beginning of one order (logit descending, index ascending), so a row's
 // kept tokens are those above a threshold logit plus the first few of those equal to it, and no row
 // is ever sorted.  Logits are compared as 32-bit keys in their order; masses e = exp((l - m) / tau) are
-// computed in f64 and summed as integers of 2^-shift (shift 42 to 51, by the vocabulary), so sums do not depend
-// on their order and a row's result is the same whatever workgroups share it.
+// computed in f64 and summed as integers of 2^-shift (shift 42 to 51, by the vocabulary), so sums do not
+// depend on their order and a row's result is the same whatever workgroups share it.
 #include "urb_device.hpp"
 #include "urb_step.hpp"
 
@@ -353,7 +353,11 @@ __device__ __noinline__ int draw_by_radix(const uint8_t* base, int V, const RowP
 // (With the bin found by the histogram's last workgroup, behind a device-scope fence in each, that launch
 // took 66 us for 256 rows, 53 of them without any sums: the fences write back and drop the L2s.)
 //
-// The row is read up to three times, after the first time from the Infinity Cache where a batch's logits fit it.
+// The row is read up to three times, after the first time from the Infinity Cache where a batch's logits
+// fit it.  256 rows of 129280 f32 logits, a mixture of all filters: 25, 37, 42 and 14 us for the four
+// launches; the first reads 132 MB at 5.3 TB/s, the next two are bound by the f64 exponentials of the tokens
+// within 36 temperatures of the largest and by LDS atomics.  One row: 4, 6, 5 and 7 us, all latency.  A row
+// by radix takes 340 us alone and 256 of them 800 (many passes of one workgroup).
 
 constexpr int kList = 1024;                 // tokens that the last launch orders, one per thread
 constexpr int kChunk = 8 * kRowThreads;     // values per chunk: eight per thread
@@ -379,7 +383,7 @@ constexpr int kGroup = 64, kAllBins = kBins + kBins / kGroup;
 
 struct Work {
   int chunks;            // of a row
-  int parts, bin_parts;  // workgroups that share a row's chunks; those of the histogram
+  int parts;             // workgroups that share them
   u64* best;          // [rows][parts] largest key << 32 | ~lowest index
   u64* sums;          // [rows][chunks * kRowWaves]: one per span
   u64* mass;          // [rows][kAllBins]: the bins, then groups of kGroup of them
@@ -444,8 +448,8 @@ __device__ __forceinline__ u64 block_max(u64 v, u64* slots) {
 // The chunks of a part: [first, last).
 struct Part {
   int first, last;
-  __device__ __forceinline__ Part(const Work& w, int part, int parts)
-      : first(w.chunks * part / parts), last(w.chunks * (part + 1) / parts) {}
+  __device__ __forceinline__ Part(const Work& w, int part)
+      : first(w.chunks * part / w.parts), last(w.chunks * (part + 1) / w.parts) {}
 };
 
 // Largest key of each part; clears what the next launches add to.
@@ -454,7 +458,7 @@ __global__ __launch_bounds__(kRowThreads, 8) void sample_best_kernel(SampleArgs 
   __shared__ u64 slots[kRowWaves];
   const int row = blockIdx.y, tid = threadIdx.x;
   const Row<BF16> r(a, row);
-  const Part part(w, blockIdx.x, w.parts);
+  const Part part(w, blockIdx.x);
   u64 best = 0;
   for (int c = part.first; c < part.last; ++c) {
     float l[8];
@@ -503,7 +507,7 @@ __global__ __launch_bounds__(kRowThreads, 8) void sample_bins_kernel(SampleArgs 
   if (trivial(p, best) || !(by_count || p.top_p < 1.0f)) return;
   const Row<BF16> r(a, row);
   const Mass m(key_in(best), p.tau, scale, powers);
-  const Part part(w, blockIdx.x, w.bin_parts);
+  const Part part(w, blockIdx.x);
   float next[8];
   r.values(part.first * kChunk + 8 * tid, next);
   fill_powers(powers);
@@ -608,7 +612,7 @@ __global__ __launch_bounds__(kRowThreads, 8) void sample_list_kernel(SampleArgs 
     return;
   }
   const Row<BF16> r(a, row);
-  const Part part(w, blockIdx.x, w.parts);
+  const Part part(w, blockIdx.x);
   float next[8];
   int at_next = r.values(part.first * kChunk + 8 * tid, next);
   RowRecord rec = find_cut(w, row, p, a.vocab);
@@ -753,8 +757,8 @@ __device__ __forceinline__ u64 first_before(u64 v, int waves, u64* slots, u64* t
 }
 
 // One workgroup per row: the last kept token of the list, then the draw.  SMALL: a vocabulary that fits
-// the list, in this launch alone.  Bound by latency, 10 us or so of one step after another, so waves without a
-// value skip what only the others need.
+// the list, in this launch alone.  Bound by latency, 7 to 14 us of one step after another, so waves without
+// a value skip what only the others need.
 template <bool BF16, bool SMALL>
 __global__ __launch_bounds__(kRowThreads) void sample_draw_kernel(SampleArgs a, Work w,
                                                                   double scale) {
@@ -901,8 +905,9 @@ __global__ __launch_bounds__(kRowThreads) void sample_draw_kernel(SampleArgs a, 
 }
 
 // Workgroups of a launch that shares rows, about: enough that rows which cost more than others are spread
-// over the chip; fewer for the histogram, where each adds up to 4096 bins to the row's.
-constexpr int kRowParts = 2048, kBinParts = 1024;
+// over the chip, few enough that the histograms they add up do not take over (256 rows of 129280: 122.6 us;
+// with 2048 for all but the histograms 125.4, with 4096 137; with 512 or 2048 for the histograms 130).
+constexpr int kParts = 1024;
 size_t row_bytes(int chunks) {
   return (size_t)chunks * 8 * (1 + kRowWaves) + kAllBins * 12 + kList * 8 + sizeof(RowRecord) + 4;
 }
@@ -917,7 +922,7 @@ void launch_rows(const SampleArgs& a, const Work& w, double scale, hipStream_t s
   }
   const dim3 grid(w.parts, a.rows);
   sample_best_kernel<BF16><<<grid, kRowThreads, 0, s>>>(a, w);
-  sample_bins_kernel<BF16><<<dim3(w.bin_parts, a.rows), kRowThreads, 0, s>>>(a, w, scale);
+  sample_bins_kernel<BF16><<<grid, kRowThreads, 0, s>>>(a, w, scale);
   sample_list_kernel<BF16><<<grid, kRowThreads, 0, s>>>(a, w, scale);
   sample_draw_kernel<BF16, false><<<a.rows, kRowThreads, 0, s>>>(a, w, scale);
 }
@@ -946,8 +951,7 @@ void launch_sample(const SampleArgs& a, bool bf16, hipStream_t s) {
     Work w{};
     if (a.vocab > kList) {
       w.chunks = row_chunks(a.vocab);
-      w.parts = std::min(w.chunks, std::max(1, kRowParts / p.rows));
-      w.bin_parts = std::min(w.chunks, std::max(1, kBinParts / p.rows));
+      w.parts = std::min(w.chunks, std::max(1, kParts / p.rows));
       const size_t rows = p.rows, most = w.chunks;
       char* at = static_cast<char*>(a.work);
       auto take = [&](auto** q, size_t n) {
