@@ -394,6 +394,50 @@ def test_results_do_not_depend_on_the_other_rows():
     assert torch.equal(p.p.forward(x[order].contiguous(), ids[order].contiguous()), first[order])
 
 
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("T", [60, 200, 1300])
+def test_tiles_give_a_row_the_same_among_any_others(T, dtype):
+    p = Proj("bf16", 272, 5120, T, dtype, F32, ranks=(8, 40, 0, 17), max_rank=64)
+    x, ids = p.rows_of(T).cuda(), _mixed(T, 4, p.g)
+    ids[ids == 2] = 3
+    x[::3] = x[::3].bfloat16().to(dtype)     # rows of one plane among rows of three
+    first = p.p.forward(x, ids)
+    p.check(first, x, ids)
+    for _ in range(3):
+        assert torch.equal(p.p.forward(x, ids), first)
+        order = torch.randperm(T, generator=p.g).cuda()
+        assert torch.equal(p.p.forward(x[order].contiguous(), ids[order].contiguous()), first[order])
+
+
+def test_a_captured_slot_change_follows_its_source():
+    p = Proj("mxfp8", 80, 256, 70, BF16, F32, ranks=(0, 4), max_rank=16)
+    x, ids = p.rows_of(70).cuda(), _mixed(70, 2, p.g)
+    ids[0] = 0
+    a, b = torch.zeros(9, 256, dtype=BF16, device="cuda"), torch.zeros(80, 9, dtype=BF16, device="cuda")
+    y = torch.empty(70, 80, device="cuda")
+    p.p.set_adapter(0, a, b, 0.5)
+    p.p.forward_into(x, y, ids)
+    stream, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=stream):
+        p.p.set_adapter(0, a, b, 0.5)
+        p.p.forward_into(x, y, ids)
+    for i in range(3):
+        a.copy_(torch.randn(9, 256, generator=p.g) / 16)
+        b.copy_(torch.randn(80, 9, generator=p.g))
+        p.adapters[0] = (a.cpu().double(), b.cpu().double(), 0.5)
+        graph.replay()
+        p.p.sync()
+        p.check(y, x, ids)
+    b[3, 3] = math.inf          # the slot becomes empty, its rows W x alone
+    graph.replay()
+    assert _status(p.p.sync) == N.ERR_NONFINITE
+    del p.adapters[0]
+    p.check(y, x, ids)
+    # (the rows that named the emptied slot had been latched with it)
+    assert _status(p.p.sync) == N.OK
+
+
 def test_slots_change_in_stream_order():
     p = Proj("bf16", 64, 256, 8, F32, ranks=(4, 6), max_rank=16)
     x = p.rows_of(8).cuda()
@@ -585,6 +629,13 @@ def test_angles_of_far_positions():
     pos = torch.tensor([0, -1, (1 << 24) + 1, (1 << 29) - 1, -(1 << 28) - 3]).cuda()
     got, _ = step().qk_norm_rope(h, None, w, None, pos, _freq(D), 1e-6)
     _check_turned(got, h, w, pos, _freq(D), zero_centered=False)
+
+
+def test_norms_alone():
+    h, w = torch.randn(9, 3, 96, generator=_gen(16)).cuda(), torch.rand(96, device="cuda")
+    got, none = step().qk_norm_rope(h, None, w, None, None, None, 1e-6)
+    assert none is None
+    _check_turned(got, h, w, torch.zeros(9), _freq(0), zero_centered=False)
 
 
 def test_rotation_of_rows_with_zeros_and_nan():
@@ -875,6 +926,16 @@ def test_samplers_on_two_streams():
         for t in range(20):
             id_, prob = _drawn(x[t], tau=float(tau[t]), p=float(p[t]), u=float(u[t]))
             assert int(ids[t]) == id_ and abs(float(probs[t]) - prob) <= (U + 2.0 ** -40) * prob
+
+
+def test_probabilities_may_be_left_out():
+    g = _gen(22)
+    for V in (700, 20000):
+        s, x, u = step().Sampler(V, 5), _logits(5, V, g), torch.rand(5, generator=g).cuda()
+        ids = torch.empty(5, dtype=torch.int32, device="cuda")
+        s.sample_into(x, u, ids)
+        s.sync()
+        assert torch.equal(ids, s.sample(x, u)[0])
 
 
 def test_rows_behind_the_last_are_left():
