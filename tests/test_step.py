@@ -475,6 +475,31 @@ def test_ids_without_an_adapter_are_reported_and_projected_alone():
     without.check(y, x)
 
 
+@pytest.mark.parametrize("T", [16, 17, 64, 65, 200, 1024, 1025, 1300])
+def test_ids_without_an_adapter_among_many_rows(T):
+    p = Proj("bf16", 80, 256, T, BF16, F32, ranks=(4, 0, 20), max_rank=24)
+    x = p.rows_of(T).cuda()
+    for bad in (1, 3, 2**31 - 1):
+        ids = _mixed(T, 3, p.g)
+        ids[ids == 1] = 0
+        assert _status(lambda: p.p.forward(x, ids)) == N.OK
+        ids[torch.randint(0, T, (1 + T // 50,), generator=p.g).cuda()] = bad
+        ids[T - 1] = -2**31
+        ids[T // 2] = bad
+        y = torch.empty(T, 80, device="cuda")
+        p.p.forward_into(x, y, ids)
+        assert _status(p.p.sync) == N.ERR_ARGUMENT and _status(p.p.sync) == N.OK
+        p.check(y, x, torch.where(ids == bad, -1, ids))
+    without = Proj("mxfp4", 80, 256, T, F32)
+    x, y = without.rows_of(T).cuda(), torch.empty(T, 80, device="cuda")
+    without.p.forward_into(x, y, torch.zeros(T, dtype=torch.int32, device="cuda"))
+    assert _status(without.p.sync) == N.ERR_ARGUMENT
+    without.check(y, x)
+    without.p.forward_into(x, y, torch.full((T,), -3, dtype=torch.int32, device="cuda"))
+    assert _status(without.p.sync) == N.OK
+    without.check(y, x)
+
+
 def test_projection_payloads_are_validated():
     w = torch.zeros(16, 128, dtype=BF16)
     w[3, 5] = math.inf
