@@ -953,6 +953,26 @@ def test_samplers_on_two_streams():
             assert int(ids[t]) == id_ and abs(float(probs[t]) - prob) <= (U + 2.0 ** -40) * prob
 
 
+@pytest.mark.parametrize("V", [65, 130, 700, 1024])
+@pytest.mark.parametrize("kept", [1, 5, 33, 64])
+def test_small_vocabularies_with_a_heavy_mask(V, kept):
+    # at most 64 tokens left, spread over all the waves that hold the row: the first wave orders them
+    # by itself while the others still take the row's largest logit
+    g = _gen(V + kept)
+    T = 512
+    x = torch.full((T, V), -math.inf)
+    for t in range(T):
+        at = torch.randperm(V, generator=g)[:kept]
+        x[t, at] = torch.randn(len(at), generator=g) * 2.0
+    pick = lambda values: [values[i % len(values)] for i in range(T)]
+    wide = torch.zeros(T, V + 9, device="cuda")
+    for start in (0, 3):
+        view = wide[:, start:start + V]
+        view.copy_(x)
+        _check_drawn(view, torch.rand(T, generator=g).tolist(), tau=pick([1.0, 0.6, 2.0]), k=pick([0, 3, 0, 40, 0]),
+                     p=pick([1.0, 0.9, 0.5, 0.99]), min_p=pick([0.0, 0.0, 0.05]))
+
+
 def test_probabilities_may_be_left_out():
     g = _gen(22)
     for V in (700, 20000):

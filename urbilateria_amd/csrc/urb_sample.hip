@@ -767,7 +767,7 @@ __global__ __launch_bounds__(kRowThreads) void sample_draw_kernel(SampleArgs a, 
     struct {
       u64 list[kList];
       u64 sums[kMaxSpans];
-      u64 slots[3][kRowWaves];
+      u64 slots[4][kRowWaves];  // one per exchange: none is written again while a wave may still read it
     } s;
   } lds;
   __shared__ int s_n, s_found;
@@ -794,7 +794,7 @@ __global__ __launch_bounds__(kRowThreads) void sample_draw_kernel(SampleArgs a, 
       rec.best = v;
       lds.s.list[atomicAdd(&s_n, 1)] = v;
     }
-    rec.best = block_max(rec.best, lds.s.slots[0]);
+    rec.best = block_max(rec.best, lds.s.slots[3]);
     rec.mode = kAllListed;
     n = s_n;
     mine = lds.s.list[tid];
