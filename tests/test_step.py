@@ -196,6 +196,34 @@ def test_single_tokens_of_low_rank(fmt, dtype, out, T, rank):
         p.check(y, x, torch.where(ids == bad, -1, ids))
 
 
+@pytest.mark.parametrize("dtype,out", [(BF16, BF16), (F32, BF16), (F32, F32)])
+@pytest.mark.parametrize("T,cols,rank", [(1, 256, 8), (1, 256, 24), (2, 256, 8), (3, 256, 20), (16, 512, 40),
+                                         (40, 256, 24), (131, 384, 70), (40, 5120, 24), (131, 5248, 40),
+                                         (1100, 256, 9)])
+def test_adapters_that_cancel_the_matrix(dtype, out, T, cols, rank):
+    # W = -scale B A but for one value per row: y is that column of x.  All values are whole numbers (and
+    # halves), all sums below 2^24 of them, so nothing is rounded while A x keeps its 20 bits and more
+    g = _gen(T + cols)
+    rows, most = 208, 127 if cols <= 512 else 31
+    whole = lambda *shape: torch.randint(1, most + 1, shape, generator=g).double()
+    proj = step().AdaptedProjection
+    a, x = whole(rank, cols), whole(T, cols)
+    r, c = torch.randint(0, rank, (rows,), generator=g), torch.randint(0, cols, (rows,), generator=g)
+    sign = torch.randint(0, 2, (rows,), generator=g).double() * 2 - 1
+    b = torch.zeros(rows, rank, dtype=torch.float64)
+    b[torch.arange(rows), r] = sign
+    assert cols * most * most < 2 ** 24
+    for scale in (1.0, -0.5):
+        w = -scale * (b @ a)
+        w[torch.arange(rows), c] += 1.0
+        wb = w.to(BF16)
+        assert torch.equal(wb.double(), w)
+        p = proj(wb.cuda(), None, C.FMT_BF16, rows, cols, T, dtype, out, slots=3, max_rank=rank)
+        p.set_adapter(1, a.to(BF16).cuda(), b.to(BF16).cuda(), scale)
+        got = p.forward(x.to(dtype).cuda(), torch.ones(T, dtype=torch.int32, device="cuda"))
+        assert torch.equal(got.cpu().double(), x[:, c])
+
+
 def test_calls_longer_than_one_pass():
     T = 8192 + 77
     p = Proj("bf16", 16, 128, T, BF16, F32, ranks=(3, 2))

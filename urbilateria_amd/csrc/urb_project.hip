@@ -8,8 +8,9 @@
 // Operands.  W streams in the panel layout (urb_kernels.hpp) straight into MFMA operands, MX codes
 // decoded to BF16 in registers (exact).  f32 rows are carried as three BF16 planes: truncating v to
 // 8 significant bits, then the rest, then the rest of that, loses none of its 24 bits; planes that are
-// zero for a whole operand (rows whose values are BF16 already) are skipped.  u is split the
-// same way, into two planes (16 bits) where the outputs are BF16, three where they are f32.
+// zero for a whole operand (rows whose values are BF16 already) are skipped.  u is carried the
+// same way, whatever the outputs' type: cut to two planes, 2^-17 of it were lost, ten times what the f32 sums
+// lose, and BF16 outputs would round to the other neighbour that much more often.
 //
 // A tile may hold rows of any adapters: each distinct adapter of a block of 16 rows multiplies the block's
 // u with the other adapters' rows set to zero.  A row has one adapter, so the order in which a tile takes
@@ -44,7 +45,8 @@ __device__ __forceinline__ uint32_t high_halves(float a, float b) {
   return __builtin_amdgcn_perm(f2u(b), f2u(a), 0x07060302u);
 }
 
-// Eight values in BF16 planes.
+// Eight values in P BF16 planes: one for BF16 values, kF32Planes for f32 ones.
+constexpr int kF32Planes = 3;
 template <int P>
 struct Planes {
   uint32_t w[P][4];
@@ -52,22 +54,16 @@ struct Planes {
     return __builtin_bit_cast(bf16x8, make_uint4(w[p][0], w[p][1], w[p][2], w[p][3]));
   }
 };
-template <int P>
-__device__ __forceinline__ Planes<P> split_planes(const float (&v)[8]) {
-  Planes<P> r;
+__device__ __forceinline__ Planes<kF32Planes> split_planes(const float (&v)[8]) {
+  Planes<kF32Planes> r;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     float a = v[2 * i], b = v[2 * i + 1];
 #pragma unroll
-    for (int p = 0; p < P; ++p) {
-      if (P == 2 && p == 1) {  // the last of two planes: rounded
-        r.w[p][i] = pk_bf16(a, b);
-      } else {
-        r.w[p][i] = high_halves(a, b);
-        const float ha = trunc_bf16(a), hb = trunc_bf16(b);
-        a = plane_rest(a, ha);
-        b = plane_rest(b, hb);
-      }
+    for (int p = 0; p < kF32Planes; ++p) {
+      r.w[p][i] = high_halves(a, b);
+      a = plane_rest(a, trunc_bf16(a));
+      b = plane_rest(b, trunc_bf16(b));
     }
   }
   return r;
@@ -79,7 +75,7 @@ __device__ __forceinline__ f32x4 mfma(bf16x8 a, bf16x8 b, f32x4 c) {
 
 // The eight values at `k` of a token row as MFMA planes: one for BF16 rows, three for f32 ones.
 template <bool XB>
-constexpr int x_planes() { return XB ? 1 : 3; }
+constexpr int x_planes() { return XB ? 1 : kF32Planes; }
 template <bool XB>
 __device__ __forceinline__ Planes<x_planes<XB>()> load_x(const uint8_t* row, int k) {
   if constexpr (XB) {
@@ -88,7 +84,7 @@ __device__ __forceinline__ Planes<x_planes<XB>()> load_x(const uint8_t* row, int
   } else {
     const float4 a = u2f4(ldg16(row + 4 * (size_t)k)), b = u2f4(ldg16(row + 4 * (size_t)k + 16));
     const float v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-    return split_planes<3>(v);
+    return split_planes(v);
   }
 }
 // The same as loaded, for loads ahead of their use.
@@ -105,7 +101,7 @@ struct XRaw {
     } else {
       const float4 a = u2f4(q[0]), b = u2f4(q[1]);
       const float v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-      return split_planes<3>(v);
+      return split_planes(v);
     }
   }
 };
@@ -113,7 +109,7 @@ struct XRaw {
 template <int P>
 __device__ __forceinline__ f32x4 mma_planes(bf16x8 w, const Planes<P>& x, f32x4 acc) {
   acc = mfma(w, x.operand(0), acc);
-  if constexpr (P == 3) {
+  if constexpr (P == kF32Planes) {
     if (__ballot((x.w[1][0] | x.w[1][1] | x.w[1][2] | x.w[1][3]) != 0)) {
       acc = mfma(w, x.operand(1), acc);
       acc = mfma(w, x.operand(2), acc);
@@ -262,8 +258,8 @@ __global__ __launch_bounds__(kOrderThreads) void order_kernel(ProjArgs p, int* o
   }
 }
 
-// The adapters' first products, as the planes that the second ones multiply: planes[(t * P + plane) * ld +
-// rank], scaled.
+// The adapters' first products, as the planes that the second ones multiply: planes[(t * kF32Planes + plane) *
+// ld + rank], scaled.
 struct FirstProduct {
   uint16_t* planes;
   int ld;
@@ -369,15 +365,15 @@ __device__ __forceinline__ void row_planes(const ProjArgs& p, int t, uint16_t* x
   const uint8_t* row = reinterpret_cast<const uint8_t*>(p.x) + (size_t)t * p.x_stride * 4;
   bool more = false;
   for (int c = 8 * threadIdx.x; c < p.cols; c += 8 * blockDim.x) {
-    const Planes<3> v = load_x<false>(row, c);
+    const Planes<kF32Planes> v = load_x<false>(row, c);
 #pragma unroll
-    for (int pl = 0; pl < 3; ++pl)
+    for (int pl = 0; pl < kF32Planes; ++pl)
       *reinterpret_cast<uint4*>(x_planes + ((size_t)pl * p.tokens + t) * p.cols + c) =
           make_uint4(v.w[pl][0], v.w[pl][1], v.w[pl][2], v.w[pl][3]);
     more |= (v.w[1][0] | v.w[1][1] | v.w[1][2] | v.w[1][3]) != 0;
   }
   more = __syncthreads_or(more);
-  if (threadIdx.x == 0) needed[t] = more ? 3 : 1;
+  if (threadIdx.x == 0) needed[t] = more ? kF32Planes : 1;
 }
 
 // What the products of a call need beforehand, in one launch.  Workgroups below `firsts`: the first product
@@ -387,7 +383,7 @@ __device__ __forceinline__ void row_planes(const ProjArgs& p, int t, uint16_t* x
 // slot of row `who` if no row before has it.
 // In a grid of several rows each takes a slice of K and writes its sum to u_parts [slice][tokens][ld]
 // for finish_kernel.  The other workgroups: a row of f32 values each (row_planes).
-template <bool XB, int P>
+template <bool XB>
 __global__ __launch_bounds__(64 * kPrepareWaves) void prepare_kernel(
     ProjArgs p, FirstProduct u, float* u_parts, Order order, int firsts, int groups, int per,
     bool by_token, uint16_t* x_planes, int* needed) {
@@ -483,10 +479,10 @@ __global__ __launch_bounds__(64 * kPrepareWaves) void prepare_kernel(
       return;
     }
     const float w[8] = {v[0] * e.scale, v[1] * e.scale, v[2] * e.scale, v[3] * e.scale};
-    const Planes<P> planes = split_planes<P>(w);
+    const Planes<kF32Planes> planes = split_planes(w);
 #pragma unroll
-    for (int pl = 0; pl < P; ++pl)
-      *reinterpret_cast<uint2*>(u.planes + ((size_t)t * P + pl) * u.ld + 16 * (q0 + wave) + 4 * lq) =
+    for (int pl = 0; pl < kF32Planes; ++pl)
+      *reinterpret_cast<uint2*>(u.planes + ((size_t)t * kF32Planes + pl) * u.ld + 16 * (q0 + wave) + 4 * lq) =
           make_uint2(planes.w[pl][0], planes.w[pl][1]);
   }
 }
@@ -494,7 +490,6 @@ __global__ __launch_bounds__(64 * kPrepareWaves) void prepare_kernel(
 // (a thread per eight values of a row of 8192: 131 rows of 7168 in 6.6 us; with 256 threads 7.7)
 constexpr int kFinishThreads = 1024;
 // The slices' sums of a row's first product, in order, as planes; and the row's own planes (x_planes).
-template <int P>
 __global__ __launch_bounds__(kFinishThreads) void finish_kernel(
     ProjArgs p, FirstProduct u, const float* u_parts, int slices, uint16_t* x_planes, int* needed) {
   const int t = blockIdx.x;
@@ -514,10 +509,10 @@ __global__ __launch_bounds__(kFinishThreads) void finish_kernel(
     }
 #pragma unroll
     for (int j = 0; j < 8; ++j) v[j] *= e.scale;
-    const Planes<P> out = split_planes<P>(v);
+    const Planes<kF32Planes> out = split_planes(v);
 #pragma unroll
-    for (int pl = 0; pl < P; ++pl)
-      *reinterpret_cast<uint4*>(u.planes + ((size_t)t * P + pl) * u.ld + r) =
+    for (int pl = 0; pl < kF32Planes; ++pl)
+      *reinterpret_cast<uint4*>(u.planes + ((size_t)t * kF32Planes + pl) * u.ld + r) =
           make_uint4(out.w[pl][0], out.w[pl][1], out.w[pl][2], out.w[pl][3]);
   }
   if (x_planes) row_planes(p, t, x_planes, needed);
@@ -567,7 +562,7 @@ __device__ __forceinline__ bf16x8 load_up(const uint16_t* b, int r, int units) {
 // the adapters' parts.  Of `parts` accumulators that are added up afterwards, each takes the slots with
 // slot % parts == part: a row's sum then has the same order in any batch.  B comes from HBM the first
 // time, so the next operands are loaded before the present ones are used.
-template <int P, int MAX, int NP, int MB>
+template <int MAX, int NP, int MB>
 __device__ __forceinline__ void add_adapters(const ProjArgs& p, const TileSlots<MAX>& s,
                                              const FirstProduct& u, int panel0, int panels, int first,
                                              int part, int parts, f32x4 (&acc)[NP][MB]) {
@@ -606,18 +601,18 @@ __device__ __forceinline__ void add_adapters(const ProjArgs& p, const TileSlots<
       const int local = first + 16 * m + ln;
       const bool mine = s.ids[local] == now;
       if (!__ballot(mine)) continue;
-      bf16x8 v[P];
+      bf16x8 v[kF32Planes];
 #pragma unroll
-      for (int pl = 0; pl < P; ++pl) {
+      for (int pl = 0; pl < kF32Planes; ++pl) {
         uint4 x = make_uint4(0, 0, 0, 0);
         if (mine && from + lq < to)
-          x = ldg16(u.planes + ((size_t)s.rows[local] * P + pl) * u.ld + 8 * (from + lq));
+          x = ldg16(u.planes + ((size_t)s.rows[local] * kF32Planes + pl) * u.ld + 8 * (from + lq));
         v[pl] = __builtin_bit_cast(bf16x8, x);
       }
 #pragma unroll
       for (int q = 0; q < NP; ++q)
 #pragma unroll
-        for (int pl = 0; pl < P; ++pl) acc[q][m] = mfma(w[q], v[pl], acc[q][m]);
+        for (int pl = 0; pl < kF32Planes; ++pl) acc[q][m] = mfma(w[q], v[pl], acc[q][m]);
     }
   }
 }
@@ -739,7 +734,7 @@ __global__ __launch_bounds__(64 * kSplitWaves) void split_kernel(ProjArgs p, Fir
         }
       }
     } else {
-      add_adapters<YB ? 2 : 3>(p, slots, u, panel0, panels, 0, wave, kSplitWaves, acc);
+      add_adapters(p, slots, u, panel0, panels, 0, wave, kSplitWaves, acc);
     }
   }
   for (int i0 = s0; i0 < s1; i0 += R) {
@@ -777,7 +772,6 @@ __global__ __launch_bounds__(64 * kSplitWaves) void split_kernel(ProjArgs p, Fir
     for (int z = 1; z < kSplitWaves; ++z) v += red[z][i][lane];  // K parts in order
     const int local = 16 * m + ln, t = t0 + local;
     if constexpr (ALONE) {
-      constexpr int P = YB ? 2 : 3;
       int at = 0;
       for (int j = 0; p.ids && j < slots.n; ++j) {
         // the lane's eight ranks: of panel lq / 2, held four each by two lanes of its row
@@ -799,9 +793,9 @@ __global__ __launch_bounds__(64 * kSplitWaves) void split_kernel(ProjArgs p, Fir
             uv[4 + r] = hi[r] * scale;
           }
         }
-        const Planes<P> planes = split_planes<P>(uv);
+        const Planes<kF32Planes> planes = split_planes(uv);
 #pragma unroll
-        for (int pl = 0; pl < P; ++pl) v = mfma(w, planes.operand(pl), v);
+        for (int pl = 0; pl < kF32Planes; ++pl) v = mfma(w, planes.operand(pl), v);
         at += (units + 1) / 2;
       }
     }
@@ -1040,7 +1034,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(
     if (s == steps) break;
   }
   if (p.ids)
-    add_adapters<YB ? 2 : 3>(p, slots, u, panel0, panels, wm * MB * 16, (int)blockIdx.y,
+    add_adapters(p, slots, u, panel0, panels, wm * MB * 16, (int)blockIdx.y,
                              (int)gridDim.y, acc);
 #pragma unroll
   for (int m = 0; m < MB; ++m) {
@@ -1253,14 +1247,14 @@ struct WorkLayout {
       return here;
     };
     const bool tiles = tokens >= kTileTokens, sorted = tokens > kFew;
-    u = take(p.slots ? (size_t)tokens * 16 * rank_panels(p.max_rank) * (p.y_bf16 ? 4 : 6) : 0);
+    u = take(p.slots ? (size_t)tokens * 16 * rank_panels(p.max_rank) * 2 * kF32Planes : 0);
     u_parts = take(p.slots ? (size_t)first_slices(tokens, p) * tokens * 16 * rank_panels(p.max_rank) * 4 : 0);
     order = take(sorted ? (size_t)tokens * 4 : 0);
     n_blocks = take(16);
     blocks = take(sorted ? (size_t)order_blocks(tokens, p.slots) * 12 : 0);
-    planes = take(!p.x_bf16 && tiles ? (size_t)tokens * p.cols * 6 : 0);
+    planes = take(!p.x_bf16 && tiles ? (size_t)tokens * p.cols * 2 * kF32Planes : 0);
     needed = take(!p.x_bf16 && tiles ? (size_t)tokens * 4 : 0);
-    const int slices = tiles ? tile_shape(tokens, p.rows, p.cols, p.x_bf16 ? 1 : 3).slices : 1;
+    const int slices = tiles ? tile_shape(tokens, p.rows, p.cols, p.x_bf16 ? 1 : kF32Planes).slices : 1;
     parts = take(slices > 1 ? (size_t)slices * tokens * p.rows * 4 : 0);
     total = at;
   }
@@ -1304,7 +1298,7 @@ void launch_project(const ProjArgs& p, hipStream_t s) {
   const bool alone = p.ids && p.slots && p.tokens * 16 * max_panels <= kAloneRanks &&
                      (double)p.rows / 16 * p.tokens * 32 * max_panels * p.cols <= kAloneBytes;
   Pass a{tiles, alone, {}, {}, u, reinterpret_cast<float*>(work + w.parts)};
-  if (tiles) a.shape = tile_shape(p.tokens, p.rows, p.cols, p.x_bf16 ? 1 : 3);
+  if (tiles) a.shape = tile_shape(p.tokens, p.rows, p.cols, p.x_bf16 ? 1 : kF32Planes);
   // the first products (of ids without any slot: one workgroup or the order, which report them)
   Order order{};
   int firsts = 0, groups = 1, per = 1;
@@ -1330,20 +1324,14 @@ void launch_project(const ProjArgs& p, hipStream_t s) {
   float* const u_parts = reinterpret_cast<float*>(work + w.u_parts);
   const dim3 grid(firsts + (planes && slices == 1 ? p.tokens : 0), slices);
   if (grid.x) {
-    auto go = [&](auto xb, auto count) {
-      constexpr int P = decltype(count)::value;
-      prepare_kernel<decltype(xb)::value, P><<<grid, 64 * kPrepareWaves, 0, s>>>(
+    auto go = [&](auto xb) {
+      prepare_kernel<decltype(xb)::value><<<grid, 64 * kPrepareWaves, 0, s>>>(
           p, u, u_parts, order, firsts, groups, per, by_token, planes, ints(w.needed));
       if (slices > 1)
-        finish_kernel<P><<<p.tokens, kFinishThreads, 0, s>>>(p, u, u_parts, slices, planes, ints(w.needed));
+        finish_kernel<<<p.tokens, kFinishThreads, 0, s>>>(p, u, u_parts, slices, planes, ints(w.needed));
     };
-    if (p.x_bf16) {
-      if (p.y_bf16) go(std::true_type{}, Int<2>{});
-      else go(std::true_type{}, Int<3>{});
-    } else {
-      if (p.y_bf16) go(std::false_type{}, Int<2>{});
-      else go(std::false_type{}, Int<3>{});
-    }
+    if (p.x_bf16) go(std::true_type{});
+    else go(std::false_type{});
   }
   ProjArgs q = p;
   if (planes) {
