@@ -412,6 +412,28 @@ def test_infinities_among_rows_with_and_without_an_adapter(dtype, T):
     assert bool(torch.isfinite(clean).all())
 
 
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("T,cols,rank", [(1, 256, 1), (1, 256, 9), (1, 256, 17), (2, 256, 7), (5, 256, 3), (40, 256, 20),
+                                         (40, 5120, 20), (200, 384, 33), (1100, 128, 5)])
+def test_infinite_values_stay_infinite_beside_padded_ranks(dtype, T, cols, rank):
+    # all weights above zero: a row with an infinity is infinite, of its sign, not NaN
+    g = _gen(T + rank)
+    w = (torch.rand(80, cols, generator=g) + 0.5).to(BF16)
+    a, b = ((torch.rand(s, generator=g) + 0.5).to(BF16) for s in ((rank, cols), (80, rank)))
+    p = step().AdaptedProjection(w.cuda(), None, C.FMT_BF16, 80, cols, T, dtype, slots=2, max_rank=rank)
+    p.set_adapter(1, a.cuda(), b.cuda(), 0.5)
+    x = torch.rand(T, cols, generator=g)
+    bad = {0: math.inf, T // 2: -math.inf, T - 1: math.inf}
+    for t, v in bad.items():
+        x[t, (37 * t + 5) % cols] = v
+    for ids in (torch.ones(T, dtype=torch.int32), torch.arange(T, dtype=torch.int32) % 2 * 2 - 1):
+        y = p.forward(x.to(dtype).cuda(), ids.cuda()).cpu()
+        for t in range(T):
+            if t in bad:
+                assert bool((y[t] == bad[t]).all()), (t, y[t])
+        assert bool(torch.isfinite(y[[t for t in range(T) if t not in bad]]).all())
+
+
 def test_results_do_not_depend_on_the_other_rows():
     p = Proj("mxfp8", 64, 512, 16, BF16, F32, ranks=(8, 8, 8))
     x, ids = p.rows_of(16).cuda(), _mixed(16, 3, p.g)

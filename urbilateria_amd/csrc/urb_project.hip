@@ -258,6 +258,12 @@ __global__ __launch_bounds__(kOrderThreads) void order_kernel(ProjArgs p, int* o
   }
 }
 
+// Rank r's value of an adapter's first product, scaled.  Ranks past the adapter's own pad it to a whole panel
+// with rows of A that are zero, whose products with an infinite or NaN x are NaN: they are zeros here.
+__device__ __forceinline__ float scaled(const AdapterEntry& e, int r, float v) {
+  return r < e.rank ? v * e.scale : 0.0f;
+}
+
 // The adapters' first products, as the planes that the second ones multiply: planes[(t * kF32Planes + plane) *
 // ld + rank], scaled.
 struct FirstProduct {
@@ -478,11 +484,13 @@ __global__ __launch_bounds__(64 * kPrepareWaves) void prepare_kernel(
                                 16 * (q0 + wave) + 4 * lq) = v;
       return;
     }
-    const float w[8] = {v[0] * e.scale, v[1] * e.scale, v[2] * e.scale, v[3] * e.scale};
+    const int r = 16 * (q0 + wave) + 4 * lq;
+    const float w[8] = {scaled(e, r, v[0]), scaled(e, r + 1, v[1]), scaled(e, r + 2, v[2]),
+                        scaled(e, r + 3, v[3])};
     const Planes<kF32Planes> planes = split_planes(w);
 #pragma unroll
     for (int pl = 0; pl < kF32Planes; ++pl)
-      *reinterpret_cast<uint2*>(u.planes + ((size_t)t * kF32Planes + pl) * u.ld + 16 * (q0 + wave) + 4 * lq) =
+      *reinterpret_cast<uint2*>(u.planes + ((size_t)t * kF32Planes + pl) * u.ld + r) =
           make_uint2(planes.w[pl][0], planes.w[pl][1]);
   }
 }
@@ -508,7 +516,7 @@ __global__ __launch_bounds__(kFinishThreads) void finish_kernel(
       from += (size_t)p.tokens * u.ld;
     }
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] *= e.scale;
+    for (int j = 0; j < 8; ++j) v[j] = scaled(e, r + j, v[j]);
     const Planes<kF32Planes> out = split_planes(v);
 #pragma unroll
     for (int pl = 0; pl < kF32Planes; ++pl)
@@ -786,11 +794,11 @@ __global__ __launch_bounds__(64 * kSplitWaves) void split_kernel(ProjArgs p, Fir
             lo += red_u[z][at + lq / 2][from];
             hi += red_u[z][at + lq / 2][from + 16];
           }
-          const float scale = p.table[slot].scale;
+          const AdapterEntry e = p.table[slot];
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            uv[r] = lo[r] * scale;
-            uv[4 + r] = hi[r] * scale;
+            uv[r] = scaled(e, 8 * lq + r, lo[r]);
+            uv[4 + r] = scaled(e, 8 * lq + 4 + r, hi[r]);
           }
         }
         const Planes<kF32Planes> planes = split_planes(uv);
