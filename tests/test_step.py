@@ -773,6 +773,30 @@ def test_heads_of_more_than_4_gib():
     assert bool((wide[-1, H * D:] == 0).all())
 
 
+@pytest.mark.parametrize("T,hq,hk,D,R,interleaved,start", [
+    ((1 << 20) + 5, 60, 4, 2, 2, True, 0),          # single values
+    (140000, 56, 8, 16, 16, False, 0), (140000, 62, 2, 16, 8, True, 0), (140000, 56, 8, 16, 16, False, 1),
+    ((1 << 27) + 77, 1, 0, 16, 16, False, 0),
+])
+def test_more_head_rows_than_a_launch_holds(T, hq, hk, D, R, interleaved, start):
+    # 2^23 head rows are a launch of either kernel; 2^26 of 64 threads, or 2^24 groups of 256, would be 2^32
+    # threads, more than there may be
+    g = torch.Generator("cuda").manual_seed(T)
+    wide = torch.randn(T, start + (hq + hk) * D, dtype=BF16, device="cuda", generator=g)
+    q = wide[:, start:start + hq * D].unflatten(1, (hq, D))
+    k = wide[:, start + hq * D:].unflatten(1, (hk, D))
+    wq, wk = (torch.rand(D, generator=_gen(i)).cuda() for i in (1, 2))
+    pos = torch.arange(T, device="cuda") * 3 - T
+    out = tuple(torch.full((T, h, D), math.nan, dtype=BF16, device="cuda") for h in (hq, hk))
+    step().qk_norm_rope(q, k if hk else None, wq, wk, pos, _freq(R), 1e-6, interleaved=interleaved, out=out)
+    assert all(bool(o.isfinite().all()) for o in out)
+    per = (1 << 23) // (hq + hk)
+    some = sorted({t for n in range(0, T, per) for t in (n - 1, n, n + 1) if 0 <= t < T} | {T // 2, T - 1})
+    for o, h, w in ((out[0], q, wq), (out[1], k, wk)):
+        if h.shape[1]:
+            _check_turned(o[some], h[some], w, pos[some], _freq(R), zero_centered=False, interleaved=interleaved)
+
+
 def test_outputs_that_overlap_themselves_are_refused():
     q, w = torch.zeros(4, 3, 64, device="cuda"), torch.ones(64, device="cuda")
     pos, buf = torch.arange(4).cuda(), torch.zeros(4 * 3 * 64, device="cuda")

@@ -239,9 +239,35 @@ void launch_wide(const RotateArgs& a, hipStream_t s) {
   else rotate_wide_kernel<BF16, false><<<grid, 256, lds, s>>>(a, span, group, parts);
 }
 
+// Head rows per launch (longer calls take several): a launch may have no more than 2^32 threads, and either
+// kernel has at most 256 of them per head row.
+constexpr uint32_t kMostRows = 1u << 23;
+
+// The same call from token t on.
+HeadRows rows_from(const HeadRows& m, uint32_t t, size_t b) {
+  HeadRows r = m;
+  if (!m.in) return r;
+  r.in = static_cast<const char*>(m.in) + t * m.in_token * b;
+  r.out = static_cast<char*>(m.out) + t * m.out_token * b;
+  return r;
+}
+
 }  // namespace
 
 void launch_rotate(const RotateArgs& a, bool bf16, hipStream_t s) {
+  const uint32_t most = std::max(1u, kMostRows / (uint32_t)a.heads);
+  if (a.tokens > most) {
+    const size_t b = bf16 ? 2 : 4;
+    for (uint32_t t = 0; t < a.tokens; t += most) {
+      RotateArgs c = a;
+      c.q = rows_from(a.q, t, b);
+      c.k = rows_from(a.k, t, b);
+      if (a.positions) c.positions = a.positions + t;
+      c.tokens = std::min(most, a.tokens - t);
+      launch_rotate(c, bf16, s);
+    }
+    return;
+  }
   const bool eights = a.dim % 16 == 0 && (a.interleaved || a.rotary % 16 == 0);
   if (eights && wide_rows(a.q, bf16 ? 2 : 4) && (!a.k.in || wide_rows(a.k, bf16 ? 2 : 4))) {
     if (bf16) launch_wide<true>(a, s);
