@@ -620,6 +620,25 @@ def test_borrowed_panels_and_host_matrices_give_the_same():
     assert borrowed.memory()[0] == 0 and make(data, scales).memory()[0] >= 64 * 256 // 2
 
 
+@pytest.mark.parametrize("source", [N.SOURCE_DEVICE_COPY, N.SOURCE_DEVICE_BORROW])
+def test_matrices_that_a_side_stream_still_writes(source):
+    # creating waits for the matrix, whatever stream it comes from
+    g = _gen(6)
+    data, _, _ = _weight("bf16", 64, 256, g)
+    x = torch.randn(9, 256, generator=g).cuda()
+    make = lambda d, src=None: step().AdaptedProjection(d, None, C.FMT_BF16, 64, 256, 9, F32, source=src)
+    want = make(data.cuda()).forward(x)
+    ready = data.cuda()
+    if source == N.SOURCE_DEVICE_BORROW:
+        ready, _ = moe_mod().pack_matrix(C.FMT_BF16, ready, None, 64, 256)
+    late, side = torch.full_like(ready.view(torch.uint8), 0xFF), torch.cuda.Stream()    # all NaN
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(100_000_000)
+        late.copy_(ready.view(torch.uint8))
+    assert torch.equal(make(late, source).forward(x), want)
+
+
 # ---- norms and rotation ------------------------------------------------------------------------
 
 def _turned(h, w, positions, freq, eps, zero_centered, interleaved):

@@ -140,11 +140,12 @@ urb_status create_proj(const urb_proj_desc* d, const urb_matrix* w, urb_weight_s
     c->b = c->a + slots * c->a_slot;
   }
   // ---- the matrix
+  if (source != URB_SOURCE_HOST)
+    URB_HIP(hipDeviceSynchronize());  // it may come from any stream, the borrowed one too: it is validated
   if (source == URB_SOURCE_DEVICE_BORROW) {
     c->data = static_cast<const uint8_t*>(w->data);
     c->scales = mx ? w->scales : nullptr;
   } else {
-    URB_HIP(hipDeviceSynchronize());  // a device source may come from any stream
     c->weight_bytes = align_up(data_bytes) + scale_bytes;
     URB_HIP(hipMalloc(&c->weights, c->weight_bytes));
     uint8_t* data = static_cast<uint8_t*>(c->weights);
