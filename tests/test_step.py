@@ -605,6 +605,22 @@ def test_projection_refuses_calls():
     torch.cuda.synchronize()
 
 
+def test_adapters_and_matrices_on_another_device_are_refused(monkeypatch):
+    # (a context of device 1: nothing is called that would read memory of device 0 there)
+    p = Proj("bf16", 64, 256, 4, F32, ranks=(4,)).p
+    a, b = torch.zeros(4, 256, dtype=BF16, device="cuda"), torch.zeros(64, 4, dtype=BF16, device="cuda")
+    p.set_adapter(0, a, b)
+    p.device = 1
+    with pytest.raises(ValueError, match="cuda:1"):
+        p.set_adapter(0, a, b)
+    p.device = 0
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 1)
+    for source in (None, N.SOURCE_DEVICE_BORROW):
+        with pytest.raises(ValueError, match="cuda:1"):
+            step().AdaptedProjection(torch.zeros(64, 256, dtype=BF16, device="cuda"), None, C.FMT_BF16, 64, 256, 4,
+                                     source=source)
+
+
 def test_borrowed_panels_and_host_matrices_give_the_same():
     g = _gen(5)
     data, scales, _ = _weight("mxfp4", 64, 256, g)

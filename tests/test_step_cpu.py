@@ -123,3 +123,66 @@ def test_rotation_refuses(change, status):
 ])
 def test_rotation_refuses_outputs_that_overlap_themselves(change):
     assert _rotate(**change) == N.ERR_SHAPE
+
+
+# ---- the wrapper's own refusals, before any call of the library ----
+
+def _wrapper():
+    import numpy as np
+    torch = pytest.importorskip("torch")
+    from urbilateria_amd import configs as C
+    from urbilateria_amd import step
+    return np, torch, C, step
+
+
+def test_matrices_of_another_type_are_refused():
+    np, torch, C, step = _wrapper()
+    make = lambda fmt, data, scales=None: step.AdaptedProjection(data, scales, fmt, 16, 128, 4)
+    scales = torch.full((16, 4), 127, dtype=torch.uint8)
+    for fmt, data, s in (
+            (C.FMT_BF16, torch.zeros(16, 128, dtype=torch.float16), None),
+            (C.FMT_BF16, np.zeros((16, 128), np.float16), None),
+            (C.FMT_BF16, torch.zeros(16, 64, dtype=torch.float32), None),
+            (C.FMT_BF16, torch.zeros(16, 32, dtype=torch.complex64), None),
+            (C.FMT_MXFP8, torch.zeros(16, 128, dtype=torch.uint8).view(torch.float8_e5m2), scales),
+            (C.FMT_MXFP8, torch.zeros(16, 128, dtype=torch.uint8).view(torch.float8_e4m3fnuz), scales),
+            (C.FMT_MXFP8, torch.zeros(16, 128, dtype=torch.uint8), scales.view(torch.float8_e4m3fn)),
+            (C.FMT_MXFP4, torch.zeros(16, 32, dtype=torch.float16), scales),
+            (C.FMT_MXFP4, torch.zeros(16, 64, dtype=torch.bool), scales)):
+        with pytest.raises(ValueError, match="holding its bits"):
+            make(fmt, data, s)
+
+
+def test_adapters_of_another_type_are_refused():
+    np, torch, C, step = _wrapper()
+    p = step.AdaptedProjection.__new__(step.AdaptedProjection)
+    p.rows, p.cols, p.device, p._ctx = 16, 128, 0, None
+    half = lambda *shape: torch.zeros(shape, dtype=torch.float16)
+    good = lambda *shape: torch.zeros(shape, dtype=torch.bfloat16)
+    for a, b in ((half(4, 128), half(16, 4)), (good(4, 128), half(16, 4)), (half(4, 128), good(16, 4)),
+                 (np.zeros((4, 128), np.float16), np.zeros((16, 4), np.float16))):
+        with pytest.raises(ValueError, match="holding its bits"):
+            p.set_adapter(0, a, b)
+
+
+def test_payloads_of_their_own_type_or_bits_are_taken():
+    np, torch, C, step = _wrapper()
+    for t, own in ((torch.zeros(2, dtype=torch.bfloat16), "bfloat16"), (torch.zeros(2, dtype=torch.int16), "bfloat16"),
+                   (torch.zeros(2, dtype=torch.uint16), "bfloat16"), (torch.zeros(4, dtype=torch.uint8), "bfloat16"),
+                   (np.zeros(2, np.uint16), "bfloat16"), (np.zeros(2, np.int16), "bfloat16"),
+                   (torch.zeros(2, dtype=torch.uint8).view(torch.float8_e4m3fn), step._VALUES[C.FMT_MXFP8]),
+                   (torch.zeros(2, dtype=torch.uint8), step._VALUES[C.FMT_MXFP4]),
+                   (torch.zeros(2, dtype=torch.uint8).view(torch.float8_e8m0fnu), step._SCALES)):
+        step._payload(t, "t", own, None)
+
+
+def test_payloads_elsewhere_are_refused():
+    np, torch, C, step = _wrapper()
+    away = torch.zeros(4, dtype=torch.bfloat16, device="meta")
+    with pytest.raises(ValueError, match="cuda:1"):
+        step._payload(away, "a", "bfloat16", 1)
+    p = step.AdaptedProjection.__new__(step.AdaptedProjection)
+    p.rows, p.cols, p.device, p._ctx = 16, 128, 0, None
+    make = lambda *shape: torch.zeros(shape, dtype=torch.bfloat16, device="meta")
+    with pytest.raises(ValueError, match="cuda:0"):
+        p.set_adapter(0, make(4, 128), make(16, 4))

@@ -45,6 +45,26 @@ def _on_host(t) -> bool:
     return isinstance(t, np.ndarray) or t.device.type == "cpu"
 
 
+# the types of a matrix's values, by format, and of its scales; integers are their bits
+_VALUES = {C.FMT_BF16: "bfloat16", C.FMT_MXFP4: "float4_e2m1fn_x2", C.FMT_MXFP8: "float8_e4m3fn"}
+_SCALES = "float8_e8m0fnu"
+
+
+def _payload(t, name: str, own: str, device: Optional[int]) -> None:
+    """Refuses values of another type than ``own`` that has the same number of bytes (float16 as
+    BF16, another 8-bit type) and, with ``device``, tensors that are not there."""
+    if isinstance(t, np.ndarray):
+        fits = t.dtype.kind in "iu" or t.dtype.name == own
+    else:
+        kind = t.dtype
+        fits = kind == getattr(torch, own, None) or not (
+            kind.is_floating_point or kind.is_complex or kind == torch.bool)
+    if not fits:
+        raise ValueError(f"{name} must be {own} or integers holding its bits, not {t.dtype}")
+    if device is not None and t.get_device() != device:
+        raise ValueError(f"{name} must be on cuda:{device}")
+
+
 class _Current:
     """torch.cuda.device(index), entered only where another device is current."""
     __slots__ = ("index", "guard")
@@ -114,8 +134,8 @@ class AdaptedProjection(_Context):
     """y = W x + scale_a B_a (A_a x) over token rows, a = the row's adapter (``urb_proj_ctx``).
 
     ``data``, ``scales``: the [rows, cols] matrix in the checkpoint layout (host or device; with
-    ``source`` SOURCE_DEVICE_BORROW in the panel layout of ``moe.pack_matrix``).  ``dtype``: the rows'
-    type, ``out_dtype`` the outputs' (the same by default).  ``slots`` adapters of up to
+    ``source`` SOURCE_DEVICE_BORROW in the panel layout of ``moe.pack_matrix``), as values of the
+    format's own type or integers holding their bits.  ``dtype``: the rows' type, ``out_dtype`` the outputs' (the same by default).  ``slots`` adapters of up to
     ``max_rank`` can be held at a time."""
 
     _destroy, _sync = "urb_proj_destroy", "urb_proj_sync"
@@ -137,6 +157,10 @@ class AdaptedProjection(_Context):
             want, want_scales = C.matrix_bytes(fmt, rows, cols)
             if _bytes(data) != want or (0 if scales is None else _bytes(scales)) != want_scales:
                 raise ValueError("the matrix does not have the bytes of its format and shape")
+            device = None if host else torch.cuda.current_device()
+            _payload(data, "data", _VALUES[fmt], device)
+            if scales is not None:
+                _payload(scales, "scales", _SCALES, device)
         self._borrowed = (data, scales) if source == N.SOURCE_DEVICE_BORROW else None
         desc = N.ProjDesc(rows, cols, fmt, _type(self.dtype), _type(self.out_dtype), max_tokens,
                           slots, max_rank)
@@ -153,6 +177,8 @@ class AdaptedProjection(_Context):
             raise ValueError("adapters are BF16")
         if _on_host(a) != _on_host(b):
             raise ValueError("a and b must be in the same memory")
+        for t, name in ((a, "a"), (b, "b")):
+            _payload(t, name, "bfloat16", None if _on_host(a) else self.device)
         ad = N.Adapter(_ptr(a), _ptr(b), rank, float(scale))
         source = N.SOURCE_HOST if _on_host(a) else N.SOURCE_DEVICE_COPY
         with _Current(self.device):
