@@ -1082,6 +1082,30 @@ def test_small_vocabularies_with_a_heavy_mask(V, kept):
                      p=pick([1.0, 0.9, 0.5, 0.99]), min_p=pick([0.0, 0.0, 0.05]))
 
 
+def test_draws_on_another_stream_are_waited_for():
+    # behind work of that stream, and after what the current one still does to the inputs
+    g = _gen(32)
+    s, side = step().Sampler(700, 4), torch.cuda.Stream()
+    x, u = _logits(4, 700, g), torch.rand(4, generator=g).cuda()
+    want = s.sample(x, u)
+    later, bad = torch.zeros_like(x), torch.full((4,), -1.0, device="cuda")
+    torch.cuda.synchronize()
+    for busy in (side, torch.cuda.current_stream()):
+        later.zero_()
+        with torch.cuda.stream(busy):
+            torch.cuda._sleep(100_000_000)
+        later.copy_(x)
+        ids, probs = s.sample(later, u, stream=side)
+        other = torch.cuda.Stream()
+        with torch.cuda.stream(other):     # done: another stream may read them at once
+            assert torch.equal(ids, want[0]) and torch.equal(probs, want[1])
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(100_000_000)
+    assert _status(lambda: s.sample(x, u, stream=side, temperature=bad)) == N.ERR_ARGUMENT
+    assert _status(s.sync) == N.OK
+    torch.cuda.synchronize()
+
+
 def test_probabilities_may_be_left_out():
     g = _gen(22)
     for V in (700, 20000):

@@ -302,10 +302,13 @@ class Sampler(_Context):
                 _vector(uniform, "uniform", T, f32, dev), _vector(ids, "ids", T, torch.int32, dev),
                 _vector(probs, "probs", T, f32, dev), _stream(stream, self.device)), "urb_sample")
 
-    def sample(self, logits, uniform, **params):
-        """-> (ids [T] int32, probs [T] f32); raises UrbError for parameters out of range."""
+    def sample(self, logits, uniform, stream=None, **params):
+        """-> (ids [T] int32, probs [T] f32); raises UrbError for parameters out of range.  On
+        ``stream`` after what the current one holds, and waited for there."""
         ids = torch.empty(logits.shape[0], dtype=torch.int32, device=logits.device)
         probs = torch.empty(logits.shape[0], dtype=torch.float32, device=logits.device)
-        self.sample_into(logits, uniform, ids, probs, **params)
-        self.sync()
+        if stream is not None:   # the inputs and the memory of ids and probs are the current one's
+            stream.wait_stream(torch.cuda.current_stream(self.device))
+        self.sample_into(logits, uniform, ids, probs, stream=stream, **params)
+        self.sync(stream)
         return ids, probs
