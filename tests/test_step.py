@@ -845,6 +845,25 @@ def test_outputs_that_overlap_themselves_are_refused():
     torch.cuda.synchronize()
 
 
+def test_new_outputs_belong_to_the_stream_of_the_call():
+    # memory that the current stream has freed but still writes is not handed to another stream
+    g = _gen(18)
+    T = 6000     # outputs of 12 MB, which the allocator keeps one by one
+    q = torch.randn(T, 4, 128, generator=g).cuda()
+    w, pos, side = torch.rand(128, generator=g).cuda(), torch.arange(T).cuda(), torch.cuda.Stream()
+    freq = _freq(64)
+    torch.cuda.synchronize()
+    freed = [torch.empty_like(q) for _ in range(4)]
+    torch.cuda._sleep(100_000_000)
+    for t in freed:
+        t.fill_(7.0)
+    del freed, t
+    got, got_k = step().qk_norm_rope(q, q, w, w, pos, freq, 1e-6, stream=side)
+    torch.cuda.synchronize()
+    for o in (got, got_k):
+        _check_turned(o, q, w, pos, freq, zero_centered=False)
+
+
 def test_rotation_wrapper_refuses():
     q, w = torch.zeros(2, 3, 64, device="cuda"), torch.ones(64, device="cuda")
     pos = torch.arange(2).cuda()

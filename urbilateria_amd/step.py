@@ -233,7 +233,8 @@ def qk_norm_rope(q, k, q_weight, k_weight, positions, inv_freq, eps: float,
     """``urb_qk_norm_rope``: q [T, heads, D] and k [T, k_heads, D] (or None) normed per head by
     ``q_weight`` / ``k_weight`` [D] f32 and turned by ``positions`` [T] int64 times ``inv_freq``
     [rotary_dim / 2] f32.  Tokens and heads may be strided, as in a fused q/k/v row.  ``out``: the
-    (q, k) tensors to write, which may be q and k themselves.  Stream-ordered."""
+    (q, k) tensors to write, which may be q and k themselves; without, new ones that belong to the
+    call's stream.  Stream-ordered."""
     dtype, device, shape = q.dtype, q.get_device(), q.shape
     if q.dim() != 3 or device < 0:
         raise ValueError("q must be a [T, heads, D] tensor on a GPU")
@@ -244,9 +245,10 @@ def qk_norm_rope(q, k, q_weight, k_weight, positions, inv_freq, eps: float,
             raise ValueError("k must be [T, k_heads, D]")
         hk = k.shape[1]
     k_shape = (T, hk, D)
-    if out is None:
-        out = (torch.empty(shape, dtype=dtype, device=q.device),
-               None if k is None else torch.empty(k_shape, dtype=dtype, device=q.device))
+    if out is None:   # (memory of the current stream may still be in use there)
+        with torch.cuda.stream(stream):
+            out = (torch.empty(shape, dtype=dtype, device=q.device),
+                   None if k is None else torch.empty(k_shape, dtype=dtype, device=q.device))
     qo, ko = out
     q_in, q_out = _heads(q, "q", shape, dtype, device), _heads(qo, "q_out", shape, dtype, device)
     k_in = k_out = (0, 0)
