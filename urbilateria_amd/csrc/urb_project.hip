@@ -566,13 +566,13 @@ __device__ __forceinline__ bf16x8 load_up(const uint16_t* b, int r, int units) {
   return __builtin_bit_cast(bf16x8, w);
 }
 
-// acc[q][m] (lane (ln, lq): rows 16 (panel0 + q) + 4 lq + [0, 4) of the tile's row first + 16 m + ln) +=
+// acc[q][m] (lane (ln, lq): rows 16 (panel0 + q) + 4 lq + [0, 4) of the tile's row 16 m + ln) +=
 // the adapters' parts.  Of `parts` accumulators that are added up afterwards, each takes the slots with
 // slot % parts == part: a row's sum then has the same order in any batch.  B comes from HBM the first
 // time, so the next operands are loaded before the present ones are used.
 template <int MAX, int NP, int MB>
 __device__ __forceinline__ void add_adapters(const ProjArgs& p, const TileSlots<MAX>& s,
-                                             const FirstProduct& u, int panel0, int panels, int first,
+                                             const FirstProduct& u, int panel0, int panels,
                                              int part, int parts, f32x4 (&acc)[NP][MB]) {
   const int lane = threadIdx.x & 63, ln = lane & 15, lq = lane >> 4;
   int i = -1, r = 0, slot = 0, units = 0;
@@ -606,7 +606,7 @@ __device__ __forceinline__ void add_adapters(const ProjArgs& p, const TileSlots<
     if (more) load(next);
 #pragma unroll
     for (int m = 0; m < MB; ++m) {
-      const int local = first + 16 * m + ln;
+      const int local = 16 * m + ln;
       const bool mine = s.ids[local] == now;
       if (!__ballot(mine)) continue;
       bf16x8 v[kF32Planes];
@@ -648,7 +648,7 @@ __device__ __forceinline__ void store_y(const ProjArgs& p, int t, int row, f32x4
   }
 }
 
-// ---- W x for a few tokens: eight waves split K of NP panels, 16 MB tokens per tile ----
+// ---- W x for up to 16 tokens: eight waves split K of one panel ----
 constexpr int kSplitWaves = 8;
 
 // ALONE: the tile computes its rows' first products itself, every workgroup all of them (kAloneRanks of at
@@ -656,67 +656,44 @@ constexpr int kSplitWaves = 8;
 constexpr int kAloneRanks = 32;
 constexpr double kAloneBytes = 50e6;
 
-template <int FMT, bool XB, bool YB, int MB, int NP, bool ALONE>
+template <int FMT, bool XB, bool YB, bool ALONE>
 __global__ __launch_bounds__(64 * kSplitWaves) void split_kernel(ProjArgs p, FirstProduct u) {
-  static_assert(!ALONE || (MB == 1 && NP == 1), "one block, one panel");
   constexpr int UP = kAloneRanks / 16;
   __shared__ f32x4 red_u[ALONE ? kSplitWaves : 1][UP][64];
-  constexpr int TILE = 16 * MB;
-  __shared__ f32x4 red[kSplitWaves][NP * MB][64];
-  __shared__ TileSlots<TILE> slots;
+  __shared__ f32x4 red[kSplitWaves][64];
+  __shared__ TileSlots<16> slots;
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int ln = lane & 15, lq = lane >> 4;
-  const int t0 = blockIdx.y * TILE, count = min(TILE, p.tokens - t0);
-  const int panels = p.rows / kPanelRows;
-  const int panel0 = blockIdx.x * NP;
+  const int count = p.tokens, panel = blockIdx.x;
   const int steps = p.cols / kGemmKStep;
   const int s0 = steps * wave / kSplitWaves, s1 = steps * (wave + 1) / kSplitWaves;
   const size_t pbytes = kPanelRows * panel_row_bytes<FMT>(p.cols);
   const size_t pscales = (size_t)kPanelRows * (p.cols / 32);
-  const uint8_t* pd[NP];
-  const uint8_t* ps[NP];
-#pragma unroll
-  for (int q = 0; q < NP; ++q) {  // a panel past the last reads the last again and stores nothing
-    const int panel = min(panel0 + q, panels - 1);
-    pd[q] = p.data + panel * pbytes;
-    ps[q] = FMT == kFmtBF16 ? nullptr : p.scales + panel * pscales;
-  }
-  const uint8_t* row[MB];
-#pragma unroll
-  for (int m = 0; m < MB; ++m)
-    row[m] = reinterpret_cast<const uint8_t*>(p.x) +
-             (size_t)(t0 + min(16 * m + ln, count - 1)) * p.x_stride * (XB ? 2 : 4);
-  f32x4 acc[NP][MB];
-#pragma unroll
-  for (int q = 0; q < NP; ++q)
-#pragma unroll
-    for (int m = 0; m < MB; ++m) acc[q][m] = f32x4{0.f, 0.f, 0.f, 0.f};
+  const uint8_t* const pd = p.data + panel * pbytes;
+  const uint8_t* const ps = FMT == kFmtBF16 ? nullptr : p.scales + panel * pscales;
+  const uint8_t* const row =
+      reinterpret_cast<const uint8_t*>(p.x) + (size_t)min(ln, count - 1) * p.x_stride * (XB ? 2 : 4);
+  f32x4 acc[1][1] = {{f32x4{0.f, 0.f, 0.f, 0.f}}};
   // Weights DW steps ahead in a ring of R slots, rows one step ahead (loaded where they are used, every
   // step waits for the L2).
   constexpr int R = FMT == kFmtBF16 ? 2 : 4, DW = R - 1;
-  BRaw<FMT> ring[R][NP];
-  XRaw<XB> xr[2][4][MB];
-  auto fetch = [&](int slot, int s) {
-#pragma unroll
-    for (int q = 0; q < NP; ++q) load_b<FMT>(ring[slot][q], pd[q], 16u * lane, ps[q], lane, s);
-  };
+  BRaw<FMT> ring[R];
+  XRaw<XB> xr[2][4];
+  auto fetch = [&](int slot, int s) { load_b<FMT>(ring[slot], pd, 16u * lane, ps, lane, s); };
   auto fetch_rows = [&](int half, int s) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-#pragma unroll
-      for (int m = 0; m < MB; ++m)
-        xr[half][j][m].load(row[m], kGemmKStep * s + frag_k<FMT>(j, lq));
+    for (int j = 0; j < 4; ++j) xr[half][j].load(row, kGemmKStep * s + frag_k<FMT>(j, lq));
   };
 #pragma unroll
   for (int d = 0; d < DW; ++d)
     if (s0 + d < s1) fetch(d, s0 + d);
   if (s0 < s1) fetch_rows(0, s0);
   if (p.ids) {
-    find_slots(p, nullptr, t0, count, slots);
+    find_slots(p, nullptr, 0, count, slots);
     if constexpr (ALONE) {
       if (blockIdx.x == 0 && (int)threadIdx.x < count) {
-        const int id = p.ids[t0 + threadIdx.x];
+        const int id = p.ids[threadIdx.x];
         if (id >= 0 && slots.ids[threadIdx.x] < 0) flag(p.status, kStepArgument);
       }
       int at = 0;
@@ -730,7 +707,7 @@ __global__ __launch_bounds__(64 * kSplitWaves) void split_kernel(ProjArgs p, Fir
             uint4 w[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-              xv[j].load(row[0], kGemmKStep * s + 32 * j + 8 * lq);
+              xv[j].load(row, kGemmKStep * s + 32 * j + 8 * lq);
               w[j] = ldg16(a + ((size_t)q * (4 * steps) + 4 * s + j) * 512);
             }
             __builtin_amdgcn_sched_barrier(kHoldLoads);
@@ -742,7 +719,7 @@ __global__ __launch_bounds__(64 * kSplitWaves) void split_kernel(ProjArgs p, Fir
         }
       }
     } else {
-      add_adapters(p, slots, u, panel0, panels, 0, wave, kSplitWaves, acc);
+      add_adapters(p, slots, u, panel, panel + 1, wave, kSplitWaves, acc);
     }
   }
   for (int i0 = s0; i0 < s1; i0 += R) {
@@ -755,71 +732,58 @@ __global__ __launch_bounds__(64 * kSplitWaves) void split_kernel(ProjArgs p, Fir
       __builtin_amdgcn_sched_barrier(kHoldLoads);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        bf16x8 w[NP];
-#pragma unroll
-        for (int q = 0; q < NP; ++q) w[q] = decode_b<FMT>(ring[d][q], j);
-#pragma unroll
-        for (int m = 0; m < MB; ++m) {
-          const auto xv = xr[d & 1][j][m].planes();
-#pragma unroll
-          for (int q = 0; q < NP; ++q) acc[q][m] = mma_planes(w[q], xv, acc[q][m]);
-        }
+        const bf16x8 w = decode_b<FMT>(ring[d], j);
+        acc[0][0] = mma_planes(w, xr[d & 1][j].planes(), acc[0][0]);
       }
     }
   }
-#pragma unroll
-  for (int q = 0; q < NP; ++q)
-#pragma unroll
-    for (int m = 0; m < MB; ++m) red[wave][q * MB + m][lane] = acc[q][m];
+  red[wave][lane] = acc[0][0];
   __syncthreads();
-  for (int i = wave; i < NP * MB; i += kSplitWaves) {
-    const int q = i / MB, m = i % MB, panel = panel0 + q;
-    if (panel >= panels) break;
-    f32x4 v = red[0][i][lane];
+  if (wave > 0) return;
+  f32x4 v = red[0][lane];
 #pragma unroll
-    for (int z = 1; z < kSplitWaves; ++z) v += red[z][i][lane];  // K parts in order
-    const int local = 16 * m + ln, t = t0 + local;
-    if constexpr (ALONE) {
-      int at = 0;
-      for (int j = 0; p.ids && j < slots.n; ++j) {
-        // the lane's eight ranks: of panel lq / 2, held four each by two lanes of its row
-        const int slot = slots.list[j].x, units = slots.list[j].y;
-        const bf16x8 w = load_up(p.b + (size_t)slot * p.b_slot + (size_t)panel * units * 128, 0, units);
-        float uv[8] = {};
-        if (slots.ids[local] == slot && lq < units) {
-          const int from = 32 * (lq & 1) + ln;
-          f32x4 lo = red_u[0][at + lq / 2][from], hi = red_u[0][at + lq / 2][from + 16];
+  for (int z = 1; z < kSplitWaves; ++z) v += red[z][lane];  // K parts in order
+  if constexpr (ALONE) {
+    int at = 0;
+    for (int j = 0; p.ids && j < slots.n; ++j) {
+      // the lane's eight ranks: of panel lq / 2, held four each by two lanes of its row
+      const int slot = slots.list[j].x, units = slots.list[j].y;
+      const bf16x8 w = load_up(p.b + (size_t)slot * p.b_slot + (size_t)panel * units * 128, 0, units);
+      float uv[8] = {};
+      if (slots.ids[ln] == slot && lq < units) {
+        const int from = 32 * (lq & 1) + ln;
+        f32x4 lo = red_u[0][at + lq / 2][from], hi = red_u[0][at + lq / 2][from + 16];
 #pragma unroll
-          for (int z = 1; z < kSplitWaves; ++z) {
-            lo += red_u[z][at + lq / 2][from];
-            hi += red_u[z][at + lq / 2][from + 16];
-          }
-          const AdapterEntry e = p.table[slot];
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            uv[r] = scaled(e, 8 * lq + r, lo[r]);
-            uv[4 + r] = scaled(e, 8 * lq + 4 + r, hi[r]);
-          }
+        for (int z = 1; z < kSplitWaves; ++z) {
+          lo += red_u[z][at + lq / 2][from];
+          hi += red_u[z][at + lq / 2][from + 16];
         }
-        const Planes<kF32Planes> planes = split_planes(uv);
+        const AdapterEntry e = p.table[slot];
 #pragma unroll
-        for (int pl = 0; pl < kF32Planes; ++pl) v = mfma(w, planes.operand(pl), v);
-        at += (units + 1) / 2;
+        for (int r = 0; r < 4; ++r) {
+          uv[r] = scaled(e, 8 * lq + r, lo[r]);
+          uv[4 + r] = scaled(e, 8 * lq + 4 + r, hi[r]);
+        }
       }
+      const Planes<kF32Planes> planes = split_planes(uv);
+#pragma unroll
+      for (int pl = 0; pl < kF32Planes; ++pl) v = mfma(w, planes.operand(pl), v);
+      at += (units + 1) / 2;
     }
-    if (local < count) store_y<YB>(p, t, panel * kPanelRows + 4 * lq, v);
   }
+  if (ln < count) store_y<YB>(p, ln, panel * kPanelRows + 4 * lq, v);
 }
 
-// ---- W x for many tokens: tiles of WM x MB 16-token blocks by WN x NP panels ----
+// ---- W x for many tokens: tiles of MB 16-token blocks by kTileWaves x NP panels ----
 //
-// Each of WM x WN waves multiplies NP panels by MB blocks.  Weights go from L2 straight into registers
+// Each wave multiplies NP panels by all MB blocks.  Weights go from L2 straight into registers
 // (a panel's slab is an MFMA operand as it lies), two slabs ahead; rows go through registers into LDS,
 // one step of 128 values ahead, in two halves between the step's MFMAs.  Row m's chunk c (16 bytes) of a
 // step lies at position c ^ x_swizzle(m) of the row's 256 bytes: a wave stores 1 KiB in a run, and the 16
 // lanes that an LDS read serves at a time hit 16 distinct bank groups.  Scheduling fences hold the loads
 // where they are written; left alone, the compiler sinks them to just before their use.
 constexpr int kTileStep = kGemmKStep;
+constexpr int kTileWaves = 4;
 
 template <int FMT>
 __device__ __forceinline__ int x_swizzle(int m) {
@@ -880,11 +844,11 @@ struct TileGrid {
   }
 };
 
-template <int FMT, bool YB, int WM, int WN, int MB, int NP>
-__global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(
+template <int FMT, bool YB, int MB, int NP>
+__global__ __launch_bounds__(64 * kTileWaves, 2) void tile_kernel(
     ProjArgs p, TileRows rows, FirstProduct u, TileGrid grid, float* parts) {
-  constexpr int WAVES = WM * WN, TM = 16 * WM * MB, TN = WN * NP;  // tokens, panels
-  constexpr int COPIES = TM * 16 / (64 * WAVES), HALF = COPIES / 2;  // per thread and step
+  constexpr int TM = 16 * MB, TN = kTileWaves * NP;  // tokens, panels
+  constexpr int COPIES = TM * 16 / (64 * kTileWaves), HALF = COPIES / 2;  // per thread and step
   constexpr int SL = tile_slabs<FMT>(), PARTS = 4 / SL;
   constexpr bool MX = FMT != kFmtBF16;
   __shared__ __attribute__((aligned(16))) u16 x0[TM * kTileStep];
@@ -893,12 +857,11 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int ln = lane & 15, lq = lane >> 4;
-  const int wm = wave % WM, wn = wave / WM;
   int row_tile, col_tile;
   if (!grid.place(blockIdx.x, &row_tile, &col_tile)) return;
   const int t0 = row_tile * TM, count = min(TM, p.tokens - t0);
   const int panels = p.rows / kPanelRows;
-  const int panel0 = col_tile * TN + wn * NP;
+  const int panel0 = col_tile * TN + wave * NP;
   // this slice's steps
   const int all_steps = p.cols / kTileStep;
   const int begin = all_steps * (int)blockIdx.y / (int)gridDim.y;
@@ -920,7 +883,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(
     for (int o = 32; o > 0; o >>= 1) planes = max(planes, __shfl_xor(planes, o, 64));
     planes = __builtin_amdgcn_readfirstlane(planes);
   }
-  // this lane's copies: rows 4 (wave + WAVES i) + lane / 16, the same chunk of each
+  // this lane's copies: rows 4 (wave + kTileWaves i) + lane / 16, the same chunk of each
   const int copy_row = 4 * wave + lane / 16;
   const int copy_chunk = (lane & 15) ^ x_swizzle<FMT>(copy_row);
   const uint8_t* const xt = reinterpret_cast<const uint8_t*>(p.x) +
@@ -929,7 +892,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(
   uint32_t copy_off[COPIES];
 #pragma unroll
   for (int i = 0; i < COPIES; ++i) {
-    const int at = min(copy_row + 4 * WAVES * i, count - 1);
+    const int at = min(copy_row + 4 * kTileWaves * i, count - 1);
     copy_off[i] = (uint32_t)(rows.order ? rows.order[t0 + at] : at) * (uint32_t)(p.x_stride * 2) +
                   16u * copy_chunk;
   }
@@ -942,13 +905,13 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(
   auto store_rows = [&](const uint4* st, int first, u16* to) {
 #pragma unroll
     for (int i = 0; i < HALF; ++i)
-      *reinterpret_cast<uint4*>(to + (wave + WAVES * (first + i)) * 512 + 8 * lane) = st[i];
+      *reinterpret_cast<uint4*>(to + (wave + kTileWaves * (first + i)) * 512 + 8 * lane) = st[i];
   };
-  // fragment reads: byte offsets of MFMA j's operand in block 0 of the wave's rows
+  // fragment reads: byte offsets of MFMA j's operand in block 0 of the rows
   uint32_t fo[4];
 #pragma unroll
   for (int j = 0; j < 4; ++j)
-    fo[j] = (uint32_t)(wm * MB * 16 + ln) * 256u +
+    fo[j] = (uint32_t)ln * 256u +
             16u * ((frag_k<FMT>(j, lq) >> 3) ^ x_swizzle<FMT>(ln));
 
   f32x4 acc[NP][MB];
@@ -1042,12 +1005,11 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(
     if (s == steps) break;
   }
   if (p.ids)
-    add_adapters(p, slots, u, panel0, panels, wm * MB * 16, (int)blockIdx.y,
-                             (int)gridDim.y, acc);
+    add_adapters(p, slots, u, panel0, panels, (int)blockIdx.y, (int)gridDim.y, acc);
 #pragma unroll
   for (int m = 0; m < MB; ++m) {
-    const int local = (wm * MB + m) * 16 + ln;
-    if ((wm * MB + m) * 16 >= count) break;
+    const int local = 16 * m + ln;
+    if (16 * m >= count) break;
     const int t = p.ids ? slots.rows[local] : t0 + local;
 #pragma unroll
     for (int q = 0; q < NP; ++q) {
@@ -1117,9 +1079,9 @@ __global__ void enter_adapter_kernel(int rank, float scale, AdapterEntry* entry,
 
 template <int FMT, bool XB, bool YB>
 void launch_rows(const ProjArgs& p, const FirstProduct& u, bool alone, hipStream_t s) {
-  const dim3 grid(p.rows / kPanelRows, (p.tokens + 15) / 16);
-  if (alone) split_kernel<FMT, XB, YB, 1, 1, true><<<grid, 64 * kSplitWaves, 0, s>>>(p, u);
-  else split_kernel<FMT, XB, YB, 1, 1, false><<<grid, 64 * kSplitWaves, 0, s>>>(p, u);
+  const int panels = p.rows / kPanelRows;
+  if (alone) split_kernel<FMT, XB, YB, true><<<panels, 64 * kSplitWaves, 0, s>>>(p, u);
+  else split_kernel<FMT, XB, YB, false><<<panels, 64 * kSplitWaves, 0, s>>>(p, u);
 }
 
 template <int FMT>
@@ -1145,7 +1107,7 @@ TileShape tile_shape(int tokens, int rows, int cols, int planes) {
   const int steps = cols / kTileStep;
   double best = 0;
   for (int np = 4; np >= 3; --np) {
-    const int col_tiles = (rows / kPanelRows + 4 * np - 1) / (4 * np);
+    const int col_tiles = (rows / kPanelRows + kTileWaves * np - 1) / (kTileWaves * np);
     const long tiles = (long)t.row_tiles * col_tiles;
     const double step = std::max(0.9, (np == 4 ? 2.0 : 1.62) * t.blocks / 8);
     for (int slices = 1; slices <= std::min(steps, kMaxSlices); ++slices) {
@@ -1156,7 +1118,7 @@ TileShape tile_shape(int tokens, int rows, int cols, int planes) {
       if (slices > 1) us += 4.0 + (double)slices * tokens * rows * 8 / 3.5e6;
       if (t.slices == 0 || us < best) {
         best = us;
-        t.panels = 4 * np;
+        t.panels = kTileWaves * np;
         t.col_tiles = col_tiles;
         t.slices = slices;
       }
@@ -1191,8 +1153,8 @@ void launch_tiles(const ProjArgs& p, const TileRows& rows, const FirstProduct& u
   const dim3 blocks(8 * grid.tall() * grid.wide(), t.slices);
   float* const out = t.slices > 1 ? parts : nullptr;
   auto go = [&](auto mb, auto np) {
-    tile_kernel<FMT, YB, 1, 4, decltype(mb)::value, decltype(np)::value>
-        <<<blocks, 256, 0, s>>>(p, rows, u, grid, out);
+    tile_kernel<FMT, YB, decltype(mb)::value, decltype(np)::value>
+        <<<blocks, 64 * kTileWaves, 0, s>>>(p, rows, u, grid, out);
   };
   auto tall = [&](auto np) {
     if (t.blocks == 2) go(Int<2>{}, np);
@@ -1200,7 +1162,7 @@ void launch_tiles(const ProjArgs& p, const TileRows& rows, const FirstProduct& u
     else if (t.blocks == 6) go(Int<6>{}, np);
     else go(Int<8>{}, np);
   };
-  if (t.panels == 12) tall(Int<3>{});
+  if (t.panels == 3 * kTileWaves) tall(Int<3>{});
   else tall(Int<4>{});
   if (out) {
     const size_t quads = (size_t)p.tokens * p.rows / 4;
