@@ -109,8 +109,8 @@ urb_status urb_proj_memory(const urb_proj_ctx *ctx, size_t *weight_bytes, size_t
  * q_heads + k_heads <= 65535, tokens * (q_heads + k_heads) < 2^31, else URB_ERR_SHAPE; eps not finite or <= 0 ->
  * URB_ERR_INVALID_GEOMETRY.  Strides are in values, from token to token and head to head; a head's
  * values are contiguous.  Heads may be parts of a wider buffer (a fused q/k/v row); an output may
- * be its own input (same address and strides) and must not overlap an input otherwise; strides by
- * which the heads of an output overlap each other -> URB_ERR_SHAPE. */
+ * be its own input (same address and strides) and must not overlap an input or the other output
+ * otherwise; strides by which the heads of an output overlap each other -> URB_ERR_SHAPE. */
 typedef struct {
   urb_dtype dtype; /* of q, k and the outputs: BF16, F32 */
   uint32_t q_heads, k_heads;

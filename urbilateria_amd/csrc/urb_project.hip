@@ -1197,9 +1197,10 @@ void launch_types(const ProjArgs& p, const Pass& a, hipStream_t s) {
 int order_blocks(int tokens, int slots) { return tokens / 16 + std::min(tokens, slots + 1); }
 
 // Slices of K of the first products (1: whole).  One workgroup pulls its rows and A at what a CU can, so
-// long rows of f32 are cut, where the launch that adds the slices also makes the rows' planes (a call of 64,
-// 131, 400 rows, 7168 -> 4096, MXFP4: 48.1 -> 43.2, 74.3 -> 68.8, 123.7 -> 119.4 us; of 131 rows of 2048
-// values 35.7 -> 39.5, so not there; BF16 rows lose as much by the launch as they gain).
+// long rows of f32 are cut, where the launch that adds the slices also makes the rows' planes.  Calls of 20,
+// 64, 131, 400 rows to 4096 outputs, MXFP4, whole and cut, in us: of 4096 values 24.5, 34.1, 48.7, 77.2 and
+// 25.4, 35.4, 49.1, 77.5; of 5120 values 27.1, 37.3, 56.9, 91.5 and 27.1, 36.4, 53.2, 88.1; of 8192 values 33.6,
+// 44.9, 73.0, 125.4 and 30.7, 44.3, 63.1, 116.8.  (BF16 rows lose as much by the launch as they gain.)
 int first_slices(int tokens, const ProjArgs& p) {
   if (p.x_bf16 || tokens < kTileTokens || tokens > 512) return 1;
   return p.cols >= 5120 ? std::min(8, p.cols / 1024) : 1;

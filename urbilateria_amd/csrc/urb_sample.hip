@@ -354,10 +354,11 @@ __device__ __noinline__ int draw_by_radix(const uint8_t* base, int V, const RowP
 // took 66 us for 256 rows, 53 of them without any sums: the fences write back and drop the L2s.)
 //
 // The row is read up to three times, after the first time from the Infinity Cache where a batch's logits
-// fit it.  256 rows of 129280 f32 logits, a mixture of all filters: 25, 37, 42 and 14 us for the four
+// fit it.  256 rows of 129280 f32 logits, a mixture of all filters: 24, 37, 40 and 14 us for the four
 // launches; the first reads 132 MB at 5.3 TB/s, the next two are bound by the f64 exponentials of the tokens
 // within 36 temperatures of the largest and by LDS atomics.  One row: 4, 6, 5 and 7 us, all latency.  A row
-// by radix takes 340 us alone and 256 of them 800 (many passes of one workgroup).
+// by radix (129280 logits within 0.1 temperatures, top-p 0.9) takes 450 us alone and 256 of them 780: many
+// passes of one workgroup.
 
 constexpr int kList = 1024;                 // tokens that the last launch orders, one per thread
 constexpr int kChunk = 8 * kRowThreads;     // values per chunk: eight per thread
