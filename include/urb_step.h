@@ -33,7 +33,8 @@ extern "C" {
  *
  * W [rows, cols] is one packed matrix for all tokens (urb_format; kept in the panel layout of
  * urb_pack_matrix), A_a [rank_a, cols] and B_a [rows, rank_a] are BF16 and live in numbered slots
- * of the context, in HBM from urb_proj_set_adapter on.  A x is carried in f32.
+ * of the context, in HBM from urb_proj_set_adapter on.  A x is carried in f32.  f32 values and A x
+ * are multiplied with all their 24 bits, as far as these lie at 2^-133 (BF16's least) or above.
  *
  * rows % 16 == 0 and cols % 128 == 0 (the panel layout), rows <= 2^20, cols <= 32768, max_tokens
  * 1 .. 2^30, adapter_slots <= 4096 and max_rank <= 256 (both 0, or neither), else URB_ERR_SHAPE. */
