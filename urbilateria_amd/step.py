@@ -135,8 +135,9 @@ class AdaptedProjection(_Context):
 
     ``data``, ``scales``: the [rows, cols] matrix in the checkpoint layout (host or device; with
     ``source`` SOURCE_DEVICE_BORROW in the panel layout of ``moe.pack_matrix``), as values of the
-    format's own type or integers holding their bits.  ``dtype``: the rows' type, ``out_dtype`` the outputs' (the same by default).  ``slots`` adapters of up to
-    ``max_rank`` can be held at a time."""
+    format's own type or integers holding their bits.  ``dtype``: the rows' type, ``out_dtype`` the
+    outputs' (the same by default).  ``slots`` adapters of up to ``max_rank`` can be held at a
+    time."""
 
     _destroy, _sync = "urb_proj_destroy", "urb_proj_sync"
 
