@@ -1,7 +1,8 @@
 /*
  * urb_step.h -- C ABI of the steps of a decoder on either side of the MoE block call
  * (urb_moe_forward_block, urb_moe.h): projections with low-rank adapters of many requests, the
- * norm of every query and key head with the position rotation, and sampling from logits.
+ * norm of every query and key head with the position rotation, sampling from logits, and beam search's
+ * selection.  The cache between them and its attention: urb_cache.h.
  *
  * The reference (inspirewind/Urbilateria) runs these steps on the CPU inside its model adapters;
  * none of the entry points mirrors one of its interfaces.  The conventions are urb_moe.h's: plain
@@ -185,6 +186,54 @@ urb_status urb_sample(urb_sampler *sampler, const void *logits, uint64_t row_str
 /* Waits for `stream` and returns the failure latched since the previous urb_sampler_sync (URB_OK
  * if none), then clears it. */
 urb_status urb_sampler_sync(urb_sampler *sampler, void *stream);
+
+/* ---- beam search's selection ----
+ *
+ * For each request, over its `width` beams b with scores c_b and rows of logits l: the candidates (b, v)
+ * of score
+ *   c_b + (l_v - m) - log(sum_i exp(l_i - m)),  m = the row's largest logit
+ * (l_v - m is 0 where both are +inf), and of a beam that has ended only (b, end_token), of score c_b.  The
+ * `picks` best are taken: by descending score, equal ones by ascending b * vocab + v.  Scores are compared
+ * in f64.  NaN logits count as -inf, and nothing of score -inf is taken: missing picks have score -inf,
+ * token -1 and parent -1.  A beam of score -inf is not there (of a search that begins, all but one are).
+ *
+ * vocab 1 .. 2^18, width 1 .. 32, picks 1 .. 64, max_requests 1 .. 65535, else URB_ERR_SHAPE. */
+typedef struct {
+  uint32_t vocab;
+  uint32_t width;        /* beams of a request */
+  uint32_t picks;
+  uint32_t max_requests;
+  urb_dtype dtype;       /* of the logits: BF16, F32 */
+} urb_beams_desc;
+
+typedef struct urb_beams urb_beams;
+
+urb_status urb_beams_create(const urb_beams_desc *desc, urb_beams **out);
+void urb_beams_destroy(urb_beams *beams);
+
+/* logits [requests * width, vocab], row_stride values from row to row, any alignment; scores and ended
+ * [requests, width] (ended NULL: none; else not 0 for a beam that has); scores_out, tokens, parents (0 ..
+ * width - 1) and ended_out (NULL, or 1 where the parent had ended, the token is end_token or the pick is
+ * missing) [requests, picks].  end_token 0 .. vocab - 1, or -1 for none where ended is NULL, else
+ * URB_ERR_ARGUMENT.  With picks = width, scores_out may be scores and ended_out ended; no other output may
+ * overlap anything.  A score that is NaN or +inf counts as -inf and is returned as URB_ERR_ARGUMENT by the
+ * next urb_beams_sync.  1 <= requests <= max_requests, row_stride >= vocab, else URB_ERR_SHAPE. */
+typedef struct {
+  const void *logits;
+  uint64_t row_stride;
+  uint32_t requests;
+  int32_t end_token;
+  const float *scores;
+  const int32_t *ended;
+  float *scores_out;
+  int32_t *tokens, *parents, *ended_out;
+} urb_beams_call;
+
+urb_status urb_beams_select(urb_beams *beams, const urb_beams_call *call, void *stream);
+
+/* Waits for `stream` and returns the failure latched since the previous urb_beams_sync (URB_OK if
+ * none), then clears it. */
+urb_status urb_beams_sync(urb_beams *beams, void *stream);
 
 #ifdef __cplusplus
 }

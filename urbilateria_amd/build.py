@@ -23,7 +23,9 @@ MOE_SOURCES = ["urb_route.hip", "urb_panel.hip", "urb_combine.hip", "urb_gemm.hi
                "urb_tall.hip", "urb_hy4.hip", "urb_decode.hip", "urb_scratch.hip",
                "urb_dense.hip", "urb_block.hip",
                "urb_rotate.hip", "urb_sample.hip", "urb_project.hip",
-               "urb_moe_host.cpp", "urb_step_host.cpp", "urb_residency.cpp"]
+               "urb_beam.hip", "urb_pages.hip", "urb_attend.hip",
+               "urb_moe_host.cpp", "urb_step_host.cpp", "urb_cache_host.cpp",
+               "urb_residency.cpp"]
 SYNTH_SOURCES = ["urb_synth.hip"]
 
 

@@ -1,0 +1,532 @@
+// urb_pages.hip -- the pages of a cache: what a step's new tokens need, rows into slots, and tables that
+// follow the beams of a search.
+#include "urb_cache.hpp"
+#include "urb_device.hpp"
+#include "urb_panel.hpp"
+
+#include <algorithm>
+
+namespace urb {
+
+namespace {
+
+// ---- rows into slots ----
+//
+// Every value is read once and written once: bound by HBM, or for a few tokens by the launch.  A row of a
+// head is held by dim / 16 lanes (of `span`, a power of two), sixteen values each, so an E4M3 row's largest
+// value is a few shuffles away and its codes leave in one 16-byte store per lane.
+template <bool BF16>
+__device__ __forceinline__ void load16(float (&v)[16], const uint8_t* p) {
+  if constexpr (BF16) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const uint4 q = ldg16(p + 16 * i);
+      const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        v[8 * i + 2 * j] = bf16_lo(w[j]);
+        v[8 * i + 2 * j + 1] = bf16_hi(w[j]);
+      }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float4 q = u2f4(ldg16(p + 16 * i));
+      v[4 * i] = q.x; v[4 * i + 1] = q.y; v[4 * i + 2] = q.z; v[4 * i + 3] = q.w;
+    }
+  }
+}
+
+template <bool BF16, bool F8>
+__global__ __launch_bounds__(256) void append_kernel(AppendArgs a, int span) {
+  const uint32_t row = blockIdx.x * (256 / span) + threadIdx.x / span;
+  const int u = threadIdx.x & (span - 1);
+  const uint32_t per_token = 2 * a.cache.heads;
+  const uint32_t t = row / per_token;
+  if (t >= a.tokens) return;
+  const uint32_t h2 = row - t * per_token;
+  const bool is_v = h2 >= a.cache.heads;
+  const uint32_t h = is_v ? h2 - a.cache.heads : h2;
+  const int64_t slot = a.slots[t];
+  if ((uint64_t)slot >= (uint64_t)a.cache.pages * a.cache.page) return;
+  const uint32_t page = (uint32_t)slot / a.cache.page, at = (uint32_t)slot - page * a.cache.page;
+  const bool there = u < (int)a.cache.dim / 16;
+  constexpr int B = BF16 ? 2 : 4;
+  const uint8_t* in = (is_v ? a.v + t * a.v_token + h * a.v_head : a.k + t * a.k_token + h * a.k_head) +
+                      16 * B * u;
+  uint8_t* out = (is_v ? a.cache.v : a.cache.k) + page * a.cache.page_stride +
+                 h * a.cache.head_stride + at * a.cache.token_stride;
+  if constexpr (!F8) {
+    if (!there) return;
+    out += 32 * u;
+    if constexpr (BF16) {
+      const uint4 lo = ldg16(in), hi = ldg16(in + 16);
+      reinterpret_cast<uint4*>(out)[0] = lo;
+      reinterpret_cast<uint4*>(out)[1] = hi;
+    } else {
+      float v[16];
+      load16<false>(v, in);
+      uint32_t w[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) w[j] = pk_bf16(v[2 * j], v[2 * j + 1]);
+      reinterpret_cast<uint4*>(out)[0] = make_uint4(w[0], w[1], w[2], w[3]);
+      reinterpret_cast<uint4*>(out)[1] = make_uint4(w[4], w[5], w[6], w[7]);
+    }
+  } else {
+    float v[16] = {};
+    if (there) load16<BF16>(v, in);
+    // the largest magnitude, as bits: those of infinities and NaNs are above all others'
+    uint32_t top = 0;
+#pragma unroll
+    for (int j = 0; j < 16; ++j) top = max(top, f2u(v[j]) & 0x7fffffffu);
+    for (int o = span / 2; o > 0; o >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, o, 64));
+    if (!there) return;
+    // 448 is 1.75 * 2^8: the power of two at or above a 448th is found from exponent and mantissa
+    const int e = (int)(top >> 23) - 8 + ((top & 0x7fffffu) > 0x600000u);
+    const bool bad = top >= 0x7f800000u;
+    const uint32_t scale = bad ? 127 : (uint32_t)max(e, 27);
+    const float inv = u2f((254 - scale) << 23);  // exact, as the products are
+    uint32_t w[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      int c = __builtin_amdgcn_cvt_pk_fp8_f32(v[4 * j] * inv, v[4 * j + 1] * inv, 0, false);
+      c = __builtin_amdgcn_cvt_pk_fp8_f32(v[4 * j + 2] * inv, v[4 * j + 3] * inv, c, true);
+      w[j] = bad ? 0x7f7f7f7fu : (uint32_t)c;
+    }
+    *reinterpret_cast<uint4*>(out + 16 * u) = make_uint4(w[0], w[1], w[2], w[3]);
+    if (u == 0)
+      (is_v ? a.cache.v_scales : a.cache.k_scales)[((uint64_t)page * a.cache.heads + h) *
+                                                       a.cache.page + at] = (uint8_t)scale;
+  }
+}
+
+// ---- block-wide helpers ----
+
+// Sum over the threads before this one; *total over all THREADS of them.  All threads take part.
+template <int THREADS>
+__device__ __forceinline__ int64_t before(int64_t v, int64_t* slots, int64_t* total) {
+  constexpr int WAVES = THREADS / 64;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  int64_t upto = v;
+  for (int o = 1; o < 64; o <<= 1) {
+    const int64_t w = __shfl_up((long long)upto, o, 64);
+    if (lane >= o) upto += w;
+  }
+  __syncthreads();
+  if (lane == 63) slots[wave] = upto;
+  __syncthreads();
+  int64_t base = 0, all = 0;
+#pragma unroll
+  for (int w = 0; w < WAVES; ++w) {
+    if (w < wave) base += slots[w];
+    all += slots[w];
+  }
+  *total = all;
+  return base + upto - v;
+}
+
+// Free pages that the stack's count stands for.
+__device__ __forceinline__ int stack_size(const int32_t* count, uint32_t pages, int* bits) {
+  const int n = *count;
+  if (n >= 0 && (uint32_t)n <= pages) return n;
+  *bits |= kCacheArgument;
+  return 0;
+}
+
+// ---- the pages and slots of a step ----
+//
+// Two sums over the rows say all: the tokens and the pages that the rows before a row bring.  They are one
+// workgroup's work (a row is 8 bytes); its tokens follow in the same launch while they are few, in a grid of
+// their own otherwise.
+constexpr int kPlanThreads = 1024;
+constexpr int kPlanWindow = 1024;  // rows whose first tokens are held in LDS
+
+// Tokens t0 .. t1 - 1, whose rows lie among first .. first + n - 1: starts (LDS or global) are their first
+// tokens.
+__device__ __forceinline__ void plan_tokens(const PlanArgs& a, uint32_t t0, uint32_t t1, uint32_t total,
+                                            const int32_t* starts, uint32_t first, uint32_t n) {
+  int bits = 0;
+  for (uint32_t t = t0 + threadIdx.x; t < t1; t += blockDim.x) {
+    int row = -1;
+    int64_t position = 0, slot = -1;
+    if (t < total) {
+      uint32_t lo = 0, hi = n;  // the last row that starts at t or before
+      while (hi - lo > 1) {
+        const uint32_t mid = (lo + hi) / 2;
+        if (starts[mid] <= (int)t) lo = mid;
+        else hi = mid;
+      }
+      row = (int)(first + lo);
+      const int have = a.row_have[row], top = a.row_top[row];
+      position = (int64_t)have + (int)t - starts[lo];
+      if (top >= 0) {
+        const uint32_t p = (uint32_t)position, block = p / a.page, held = (have + a.page - 1) / a.page;
+        int32_t* entry = a.tables + row * a.table_stride + block;
+        int page;
+        if (block < held) {
+          page = *entry;
+        } else {
+          page = a.free_pages[top - (int)(block - held)];
+          if (p % a.page == 0) *entry = page;
+        }
+        if ((uint32_t)page < a.pages) slot = (int64_t)page * a.page + p % a.page;
+        else bits |= kCacheArgument;
+      }
+    }
+    a.slots[t] = slot;
+    if (a.token_rows) a.token_rows[t] = row;
+    if (a.positions) a.positions[t] = position;
+  }
+  if (bits) flag(a.status, bits);
+}
+
+template <bool ALL>
+__global__ __launch_bounds__(kPlanThreads) void plan_rows_kernel(PlanArgs a) {
+  __shared__ int64_t slots[kPlanThreads / 64];
+  __shared__ int32_t starts[ALL ? kPlanWindow : 1];
+  int bits = 0;
+  const int count = stack_size(a.free_count, a.pages, &bits);
+  int64_t tokens_before = 0, pages_before = 0, used = 0;
+  for (uint32_t r0 = 0; r0 < a.rows; r0 += kPlanThreads) {
+    const uint32_t r = r0 + threadIdx.x;
+    const bool in = r < a.rows;
+    const int have = in ? a.lengths[r] : 0, add = in ? (a.added ? a.added[r] : 1) : 0;
+    const bool ok = have >= 0 && add >= 0 &&
+                    (int64_t)have + add <= (int64_t)a.max_blocks * a.page;
+    const int tokens = ok ? add : 0;
+    int64_t all;
+    const int64_t start = tokens_before + before<kPlanThreads>(tokens, slots, &all);
+    tokens_before += all;
+    const bool over = start + tokens > a.tokens;
+    const int need = ok && !over ? (int)((have + tokens + a.page - 1) / a.page -
+                                         (have + a.page - 1) / a.page)
+                                 : 0;
+    const int64_t first = pages_before + before<kPlanThreads>(need, slots, &all);
+    pages_before += all;
+    const bool enough = need == 0 || first + need <= count;
+    const bool served = ok && !over && enough;
+    (void)before<kPlanThreads>(served ? need : 0, slots, &all);
+    used += all;
+    if (!ok || over) bits |= kCacheArgument;
+    if (!enough) bits |= kCacheMemory;
+    const int at = (int)min(start, (int64_t)a.tokens);
+    if (in) {
+      a.row_have[r] = have;
+      a.row_start[r] = at;
+      a.row_top[r] = !served ? -1 : need ? count - 1 - (int)first : 0;
+      a.lengths_out[r] = served ? have + tokens : have;
+      if (a.starts) a.starts[r] = at;
+      if constexpr (ALL) starts[r] = at;
+    }
+  }
+  const int total = (int)min(tokens_before, (int64_t)a.tokens);
+  if (threadIdx.x == 0) {
+    if (a.starts) a.starts[a.rows] = total;
+    *a.free_count_out = count - (int)used;
+    a.row_start[a.rows] = total;
+  }
+  if (bits) flag(a.status, bits);
+  if constexpr (ALL) {
+    __syncthreads();
+    plan_tokens(a, 0, a.tokens, (uint32_t)total, starts, 0, a.rows);
+  }
+}
+
+// The last of rows 0 .. n - 1 whose first token is t or before, by a whole wave.
+__device__ __forceinline__ uint32_t row_of(const int32_t* starts, uint32_t n, uint32_t t) {
+  const int lane = threadIdx.x & 63;
+  uint32_t lo = 0;
+  while (n > 1) {
+    const uint32_t step = (n + 63) / 64;
+    const uint32_t at = lane * step;
+    const uint64_t below = __ballot(at < n && starts[lo + at] <= (int)t);
+    const uint32_t part = 63 - __clzll(below | 1);
+    lo += part * step;
+    n = min(step, n - part * step);
+  }
+  return lo;
+}
+
+constexpr int kPlanTokens = 1024;  // of a workgroup
+__global__ __launch_bounds__(256) void plan_tokens_kernel(PlanArgs a) {
+  __shared__ int32_t starts[kPlanWindow];
+  const uint32_t t0 = blockIdx.x * kPlanTokens, t1 = min(t0 + kPlanTokens, a.tokens);
+  const uint32_t total = (uint32_t)a.row_start[a.rows];
+  uint32_t first = 0, n = 1;
+  const int32_t* from = a.row_start;
+  if (t0 < total) {
+    first = row_of(a.row_start, a.rows, t0);
+    n = row_of(a.row_start, a.rows, min(t1, total) - 1) - first + 1;
+    from = a.row_start + first;
+    // (more rows than tokens where some bring none)
+    if (n <= kPlanWindow) {
+      for (uint32_t i = threadIdx.x; i < n; i += 256) starts[i] = from[i];
+      from = starts;
+    }
+  }
+  __syncthreads();
+  plan_tokens(a, t0, t1, total, from, first, n);
+}
+
+// ---- tables that follow their beams ----
+
+__device__ __forceinline__ uint32_t blocks_of(int length, uint32_t page) {
+  return (uint32_t)(length + page - 1) / page;
+}
+
+// Whether row i of a request takes a copy of its parent's last page: one that is filled in part and stays
+// with a lower child.
+__device__ __forceinline__ bool takes_copy(const int* parent, const int* length, int i, uint32_t page) {
+  const int p = parent[i];
+  if (p < 0 || length[p] % page == 0) return false;
+  for (int j = 0; j < i; ++j)
+    if (parent[j] == p) return true;
+  return false;
+}
+
+// One request per workgroup: its rows' tables, and the pages that none of them holds any more.  A page can
+// stand in several rows only in one column, so a column is one thread's work.
+__global__ __launch_bounds__(256) void fork_tables_kernel(ForkArgs a) {
+  __shared__ int parent[kForkWidth], length[kForkWidth];
+  __shared__ int64_t slots[4];
+  const uint32_t r = blockIdx.x, row0 = r * a.width;
+  const int tid = threadIdx.x, width = (int)a.width;
+  int bits = 0;
+  if (tid < width) {
+    int p = a.parents[row0 + tid];
+    if (p >= width) bits |= kCacheArgument;
+    parent[tid] = p < 0 || p >= width ? -1 : p;
+    int n = a.lengths[row0 + tid];
+    if (n < 0 || (int64_t)n > (int64_t)a.max_blocks * a.page) {
+      bits |= kCacheArgument;
+      n = 0;
+    }
+    length[tid] = n;
+    a.old_lengths[row0 + tid] = n;
+  }
+  __syncthreads();
+  if (tid < 64) {
+    const bool copy = tid < width && takes_copy(parent, length, tid, a.page);
+    const uint64_t copies = __ballot(copy);
+    if (tid == 0) a.copies[r] = __popcll(copies);
+  }
+  uint64_t used = 0;  // rows with a child
+  uint32_t columns = 0;
+  for (int i = 0; i < width; ++i) {
+    if (parent[i] >= 0) used |= 1ull << parent[i];
+    columns = max(columns, blocks_of(length[i], a.page));
+  }
+  const int32_t* in = a.tables + row0 * a.table_stride;
+  int32_t* out = a.tables_out + row0 * a.table_out_stride;
+  int32_t* list = a.dropped + (uint64_t)row0 * a.max_blocks;
+  int n_dropped = 0;
+  for (uint32_t c0 = 0; c0 < columns; c0 += 256) {
+    const uint32_t c = c0 + tid;
+    uint64_t drop = 0;
+    if (c < columns) {
+      for (int i = 0; i < width; ++i) {
+        const int p = parent[i];
+        if (p >= 0 && c < blocks_of(length[p], a.page))
+          out[i * a.table_out_stride + c] = in[p * a.table_stride + c];
+      }
+      for (int i = 0; i < width; ++i) {
+        if (used >> i & 1 || c >= blocks_of(length[i], a.page)) continue;
+        const int page = in[i * a.table_stride + c];
+        if ((uint32_t)page >= a.pages) {
+          bits |= kCacheArgument;
+          continue;
+        }
+        bool gone = true;  // held by no row with children, and by no lower row without
+        for (int j = 0; j < width && gone; ++j)
+          if ((used >> j & 1 || j < i) && c < blocks_of(length[j], a.page))
+            gone = in[j * a.table_stride + c] != page;
+        if (gone) drop |= 1ull << i;
+      }
+    }
+    int64_t all;
+    int at = n_dropped + (int)before<256>(__popcll(drop), slots, &all);
+    n_dropped += (int)all;
+    for (; drop; drop &= drop - 1)
+      list[at++] = in[(__ffsll((unsigned long long)drop) - 1) * a.table_stride + c];
+  }
+  if (tid == 0) {
+    a.drops[r] = n_dropped;
+    if (r == 0) *a.count = stack_size(a.free_count, a.pages, &bits);
+  }
+  if (bits) flag(a.status, bits);
+}
+
+struct ForkCaches {
+  KvCache c[kForkCaches];
+  int n;
+};
+
+__device__ __forceinline__ void copy_page(const KvCache& c, uint32_t from, uint32_t to, uint32_t tokens,
+                                          uint32_t part, uint32_t parts) {
+  const bool f8 = c.k_scales != nullptr;
+  const uint32_t row16 = c.dim * (f8 ? 1 : 2) / 16;  // 16-byte pieces of a row
+  const uint32_t rows = 2 * c.heads * tokens, items = rows * row16;
+  for (uint32_t i = part * 256 + threadIdx.x; i < items; i += parts * 256) {
+    const uint32_t row = i / row16, piece = i - row * row16;
+    const uint32_t h2 = row / tokens, t = row - h2 * tokens;
+    const bool is_v = h2 >= c.heads;
+    uint8_t* base = (is_v ? c.v : c.k) + (is_v ? h2 - c.heads : h2) * c.head_stride +
+                    t * c.token_stride + 16 * piece;
+    *reinterpret_cast<uint4*>(base + to * c.page_stride) = ldg16(base + from * c.page_stride);
+  }
+  if (!f8) return;
+  for (uint32_t row = part * 256 + threadIdx.x; row < rows; row += parts * 256) {
+    const uint32_t h2 = row / tokens, t = row - h2 * tokens;
+    const bool is_v = h2 >= c.heads;
+    const uint32_t h = is_v ? h2 - c.heads : h2;
+    uint8_t* s = is_v ? c.v_scales : c.k_scales;
+    s[((uint64_t)to * c.heads + h) * c.page + t] = s[((uint64_t)from * c.heads + h) * c.page + t];
+  }
+}
+
+// A row per blockIdx.x: its copied page, part blockIdx.y of it in every cache; in the first launch of a call
+// (`books`) its length, its table's entry for that page, and the stack.
+__global__ __launch_bounds__(256) void fork_copy_kernel(ForkArgs a, ForkCaches caches, bool books) {
+  __shared__ int parent[kForkWidth], length[kForkWidth];
+  __shared__ int64_t slots[4];
+  __shared__ int s_page;
+  const uint32_t row = blockIdx.x, r = row / a.width;
+  const int i = (int)(row - r * a.width), tid = threadIdx.x, width = (int)a.width;
+  books = books && blockIdx.y == 0;
+  if (tid < width) {
+    const int p = a.parents[r * a.width + tid];
+    parent[tid] = p < 0 || p >= width ? -1 : p;
+    length[tid] = a.old_lengths[r * a.width + tid];
+  }
+  if (tid == 0) s_page = -1;
+  __syncthreads();
+  const bool copy = takes_copy(parent, length, i, a.page);
+  const bool pushes = books && i == 0;
+  const int p = parent[i];
+  bool kept = p >= 0;  // whether the row goes on
+  int bits = 0;
+  if (copy || pushes) {
+    // pages dropped in all, and by the requests before; copies likewise
+    int64_t mine[4] = {0, 0, 0, 0}, sums[4];
+    for (uint32_t q = tid; q < a.requests; q += 256) {
+      const int d = a.drops[q], c = a.copies[q];
+      mine[0] += d;
+      mine[1] += c;
+      if (q < r) {
+        mine[2] += d;
+        mine[3] += c;
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) (void)before<256>(mine[k], slots, &sums[k]);
+    const int count = *a.count;
+    const int64_t room = (int64_t)a.pages - count;  // of the stack
+    const int64_t size = count + min(sums[0], room);
+    if (copy) {
+      int k = (int)sums[3];
+      for (int j = 0; j < i; ++j) k += takes_copy(parent, length, j, a.page);
+      const int64_t at = size - 1 - k;
+      int64_t passed = 0;
+      if (at < count) {
+        if (tid == 0 && at >= 0) s_page = a.free_pages[at];
+      } else {
+        // a page that a request has just dropped
+        const int64_t want = at - count;
+        for (uint32_t q0 = 0; q0 < a.requests && passed <= want; q0 += 256) {
+          const uint32_t q = q0 + tid;
+          const int d = q < a.requests ? a.drops[q] : 0;
+          int64_t all;
+          const int64_t first = passed + before<256>(d, slots, &all);
+          if (first <= want && want < first + d)
+            s_page = a.dropped[(uint64_t)q * a.width * a.max_blocks + (want - first)];
+          passed += all;
+        }
+      }
+      __syncthreads();
+      const uint32_t last = (uint32_t)length[p] / a.page;
+      const int to = s_page;
+      if (at < 0) {
+        kept = false;
+        bits |= kCacheMemory;
+      } else {
+        const int from = a.tables[(uint64_t)(r * a.width + p) * a.table_stride + last];
+        if (books && tid == 0) a.tables_out[row * a.table_out_stride + last] = to;
+        if ((uint32_t)to >= a.pages || (uint32_t)from >= a.pages) {
+          bits |= kCacheArgument;
+        } else {
+          const uint32_t tokens = (uint32_t)length[p] % a.page;
+          for (int c = 0; c < caches.n; ++c)
+            copy_page(caches.c[c], (uint32_t)from, (uint32_t)to, tokens, blockIdx.y, gridDim.y);
+        }
+      }
+    }
+    if (pushes) {
+      const int32_t* list = a.dropped + (uint64_t)r * a.width * a.max_blocks;
+      const int64_t first = count + sums[2];
+      const int n = a.drops[r];
+      for (int j = tid; j < n; j += 256)
+        if (first + j < a.pages) a.free_pages[first + j] = list[j];
+      if (r == 0 && tid == 0) {
+        *a.free_count_out = (int)max(size - sums[1], (int64_t)0);
+        if (sums[0] > room) bits |= kCacheArgument;
+      }
+    }
+  }
+  if (books && tid == 0) a.lengths_out[row] = kept ? length[p] : 0;
+  if (bits && tid == 0) flag(a.status, bits);
+}
+
+}  // namespace
+
+void launch_append(const AppendArgs& a, bool rows_bf16, hipStream_t s) {
+  int span = 1;
+  while (span < (int)a.cache.dim / 16) span *= 2;
+  // tokens of a launch: row numbers of 32 bits, fewer than 2^31 threads
+  const uint32_t most = std::max(1u, (1u << 26) / a.cache.heads);
+  for (uint32_t t = 0; t < a.tokens; t += most) {
+    AppendArgs c = a;
+    c.k += t * a.k_token;
+    c.v += t * a.v_token;
+    c.slots += t;
+    c.tokens = std::min(most, a.tokens - t);
+    const uint64_t threads = (uint64_t)c.tokens * 2 * a.cache.heads * span;
+    const dim3 grid((unsigned)((threads + 255) / 256));
+    const bool f8 = a.cache.k_scales != nullptr;
+    if (rows_bf16 && f8) append_kernel<true, true><<<grid, 256, 0, s>>>(c, span);
+    else if (rows_bf16) append_kernel<true, false><<<grid, 256, 0, s>>>(c, span);
+    else if (f8) append_kernel<false, true><<<grid, 256, 0, s>>>(c, span);
+    else append_kernel<false, false><<<grid, 256, 0, s>>>(c, span);
+  }
+}
+
+void launch_plan(const PlanArgs& a, hipStream_t s) {
+  // One launch while its workgroup has a few tokens per thread.
+  if (a.rows <= kPlanWindow && a.tokens <= 4 * kPlanThreads) {
+    plan_rows_kernel<true><<<1, kPlanThreads, 0, s>>>(a);
+    return;
+  }
+  plan_rows_kernel<false><<<1, kPlanThreads, 0, s>>>(a);
+  plan_tokens_kernel<<<(a.tokens + kPlanTokens - 1) / kPlanTokens, 256, 0, s>>>(a);
+}
+
+void launch_fork(const ForkArgs& a, const KvCache* caches, uint32_t n_caches, hipStream_t s) {
+  fork_tables_kernel<<<a.requests, 256, 0, s>>>(a);
+  uint32_t done = 0;
+  do {
+    ForkCaches some;
+    some.n = (int)std::min<uint32_t>(kForkCaches, n_caches - done);
+    uint64_t bytes = 0;
+    for (int i = 0; i < some.n; ++i) {
+      some.c[i] = caches[done + i];
+      bytes += 2ull * caches[done + i].heads * a.page * caches[done + i].dim;
+    }
+    // parts of a page: some 16 KB each, at most sixteen per CU over all rows
+    const uint32_t rows = a.requests * a.width;
+    const uint32_t parts = (uint32_t)std::max<uint64_t>(
+        1, std::min<uint64_t>(bytes / 16384, 4096 / rows));
+    fork_copy_kernel<<<dim3(rows, parts), 256, 0, s>>>(a, some, done == 0);
+    done += (uint32_t)some.n;
+  } while (done < n_caches);
+}
+
+}  // namespace urb

@@ -51,6 +51,29 @@ constexpr int kSamplePass = 512;
 size_t sample_work_bytes(int vocab, int rows);
 void launch_sample(const SampleArgs& a, bool bf16, hipStream_t s);
 
+// ---- beam search's selection (urb_beam.hip) ----
+constexpr int kBeamWidth = 32, kBeamPicks = 64, kBeamVocab = 1 << 18;
+constexpr int kBeamSlice = 8192;  // logits of a workgroup
+inline int beam_slices(int vocab) { return (vocab + kBeamSlice - 1) / kBeamSlice; }
+static_assert(kBeamWidth * (kBeamVocab / kBeamSlice) <= 1024, "a thread for every slice of a request");
+struct BeamSum;
+struct BeamArgs {
+  const void* logits;
+  uint64_t row_stride;  // values
+  int vocab, width, picks, requests, end_token;
+  const float* scores;
+  const int32_t* ended;
+  float* scores_out;
+  int32_t *tokens, *parents, *ended_out;
+  int* status;
+  // set by launch_beam: workspace
+  int slices;
+  unsigned long long* keys;
+  BeamSum* sums;
+};
+size_t beam_work_bytes(int vocab, int width, int picks, int requests);
+void launch_beam(BeamArgs a, bool bf16, int max_requests, void* work, hipStream_t s);
+
 // ---- projections with adapters (urb_project.hip) ----
 // Ranks are kept in units of 8 in B and in 16-rank panels in A.
 constexpr int kRankUnit = 8;

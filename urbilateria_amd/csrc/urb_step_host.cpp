@@ -2,60 +2,11 @@
 // the launches of each call.
 #include "../../include/urb_step.h"
 
-#include <hip/hip_runtime.h>
-
 #include <algorithm>
 #include <new>
-#include <utility>
 
-#include "urb_kernels.hpp"
 #include "urb_step.hpp"
-
-#define URB_HIP(call)                            \
-  do {                                           \
-    hipError_t e_ = (call);                      \
-    if (e_ == hipErrorOutOfMemory) return URB_ERR_OUT_OF_MEMORY; \
-    if (e_ != hipSuccess) return URB_ERR_DEVICE; \
-  } while (0)
-
-namespace {
-
-constexpr size_t kAlign = 256;
-size_t align_up(size_t v) { return (v + kAlign - 1) / kAlign * kAlign; }
-
-bool row_type(urb_dtype t) { return t == URB_DTYPE_BF16 || t == URB_DTYPE_F32; }
-size_t value_bytes(urb_dtype t) { return t == URB_DTYPE_BF16 ? 2 : 4; }
-bool finite_host(float v) { return v == v && v <= 3.4028235e38f && v >= -3.4028235e38f; }
-
-bool on_device(int device) {
-  int now = -1;
-  return hipGetDevice(&now) == hipSuccess && now == device;
-}
-
-// Whether the heads of an output lie apart: [tokens][heads] rows of dim values, either stride the larger.
-bool heads_apart(uint64_t tokens, uint64_t token_stride, uint64_t heads, uint64_t head_stride, uint64_t dim) {
-  if (token_stride < head_stride) {
-    std::swap(tokens, heads);
-    std::swap(token_stride, head_stride);
-  }
-  if (heads > 1 && head_stride < dim) return false;
-  if (tokens == 1) return true;
-  // (the larger stride against what the others span, without the product)
-  return token_stride >= dim && (heads == 1 || (token_stride - dim) / (heads - 1) >= head_stride);
-}
-
-// Waits for the stream, then reads and clears a status word (written by kernels of that stream).
-urb_status take_status(int* word, hipStream_t s, int* bits) {
-  *bits = 0;
-  URB_HIP(hipStreamSynchronize(s));
-  URB_HIP(hipMemcpy(bits, word, sizeof(int), hipMemcpyDeviceToHost));
-  urb::launch_fill_i32(word, 0, 1, s);
-  URB_HIP(hipGetLastError());
-  URB_HIP(hipStreamSynchronize(s));
-  return URB_OK;
-}
-
-}  // namespace
+#include "urb_step_host.hpp"
 
 struct urb_proj_ctx {
   urb_proj_desc desc{};
@@ -72,6 +23,13 @@ struct urb_proj_ctx {
   int* status = nullptr;  // [0] latched failures, [1] an adapter being entered, [2] validation
   urb::AdapterEntry* table = nullptr;
   void* pass = nullptr;
+};
+
+struct urb_beams {
+  urb_beams_desc desc{};
+  int device = 0;
+  void* work = nullptr;
+  int* status = nullptr;
 };
 
 struct urb_sampler {
@@ -426,6 +384,87 @@ urb_status urb_sample(urb_sampler* c, const void* logits, uint64_t row_stride, u
 }
 
 urb_status urb_sampler_sync(urb_sampler* c, void* stream) {
+  if (!c || !on_device(c->device)) return URB_ERR_ARGUMENT;
+  int bits = 0;
+  const urb_status st = take_status(c->status, static_cast<hipStream_t>(stream), &bits);
+  if (st) return st;
+  return bits ? URB_ERR_ARGUMENT : URB_OK;
+}
+
+urb_status urb_beams_create(const urb_beams_desc* d, urb_beams** out) {
+  if (!d || !out) return URB_ERR_ARGUMENT;
+  *out = nullptr;
+  if (!row_type(d->dtype)) return URB_ERR_ARGUMENT;
+  if (d->vocab == 0 || d->vocab > (uint32_t)urb::kBeamVocab || d->width == 0 ||
+      d->width > (uint32_t)urb::kBeamWidth || d->picks == 0 || d->picks > (uint32_t)urb::kBeamPicks ||
+      d->max_requests == 0 || d->max_requests > 65535)
+    return URB_ERR_SHAPE;
+  urb_beams* c = new (std::nothrow) urb_beams();
+  if (!c) return URB_ERR_OUT_OF_MEMORY;
+  c->desc = *d;
+  const urb_status st = [&]() -> urb_status {
+    URB_HIP(hipGetDevice(&c->device));
+    URB_HIP(hipMalloc(&c->work, kAlign + urb::beam_work_bytes((int)d->vocab, (int)d->width, (int)d->picks,
+                                                              (int)d->max_requests)));
+    c->status = static_cast<int*>(c->work);
+    urb::launch_fill_i32(c->status, 0, kAlign / 4, nullptr);
+    URB_HIP(hipGetLastError());
+    URB_HIP(hipDeviceSynchronize());
+    return URB_OK;
+  }();
+  if (st) {
+    (void)hipGetLastError();
+    if (c->work) (void)hipFree(c->work);
+    delete c;
+    return st;
+  }
+  *out = c;
+  return URB_OK;
+}
+
+void urb_beams_destroy(urb_beams* c) {
+  if (!c) return;
+  int now = 0;
+  const bool other = hipGetDevice(&now) == hipSuccess && now != c->device;
+  if (other) (void)hipSetDevice(c->device);
+  (void)hipDeviceSynchronize();
+  if (c->work) (void)hipFree(c->work);
+  delete c;
+  if (other) (void)hipSetDevice(now);
+}
+
+urb_status urb_beams_select(urb_beams* c, const urb_beams_call* p, void* stream) {
+  if (!c || !p || !p->logits || !p->scores || !p->scores_out || !p->tokens || !p->parents ||
+      !on_device(c->device))
+    return URB_ERR_ARGUMENT;
+  const urb_beams_desc& d = c->desc;
+  if (p->requests == 0 || p->requests > d.max_requests || p->row_stride < d.vocab) return URB_ERR_SHAPE;
+  if (reinterpret_cast<uintptr_t>(p->logits) % value_bytes(d.dtype)) return URB_ERR_ARGUMENT;
+  if (p->end_token < (p->ended ? 0 : -1) || p->end_token >= (int64_t)d.vocab) return URB_ERR_ARGUMENT;
+  if (d.picks != d.width && (p->scores_out == p->scores || (p->ended && p->ended_out == p->ended)))
+    return URB_ERR_ARGUMENT;
+  urb::BeamArgs a{};
+  a.logits = p->logits;
+  a.row_stride = p->row_stride;
+  a.vocab = (int)d.vocab;
+  a.width = (int)d.width;
+  a.picks = (int)d.picks;
+  a.requests = (int)p->requests;
+  a.end_token = p->end_token;
+  a.scores = p->scores;
+  a.ended = p->ended;
+  a.scores_out = p->scores_out;
+  a.tokens = p->tokens;
+  a.parents = p->parents;
+  a.ended_out = p->ended_out;
+  a.status = c->status;
+  urb::launch_beam(a, d.dtype == URB_DTYPE_BF16, (int)d.max_requests,
+                   static_cast<char*>(c->work) + kAlign, static_cast<hipStream_t>(stream));
+  URB_HIP(hipGetLastError());
+  return URB_OK;
+}
+
+urb_status urb_beams_sync(urb_beams* c, void* stream) {
   if (!c || !on_device(c->device)) return URB_ERR_ARGUMENT;
   int bits = 0;
   const urb_status st = take_status(c->status, static_cast<hipStream_t>(stream), &bits);

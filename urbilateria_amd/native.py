@@ -1,5 +1,5 @@
-"""ctypes binding of the C ABI in ``include/urb_moe.h`` and ``include/urb_step.h``
-(``liburb_moe.so``) and of the device workload generator (``liburb_synth.so``).
+"""ctypes binding of the C ABI in ``include/urb_moe.h``, ``include/urb_step.h`` and
+``include/urb_cache.h`` (``liburb_moe.so``) and of the device workload generator (``liburb_synth.so``).
 
 The shared libraries are built in-tree by ``__graft_entry__.build()``.  Loading fails loudly
 when they are missing: there is no CPU fallback for any entry point.
@@ -30,7 +30,12 @@ EXPORTS = ("urb_moe_create", "urb_moe_destroy", "urb_moe_forward", "urb_moe_rout
 # Every symbol include/urb_step.h declares.
 STEP_EXPORTS = ("urb_proj_create", "urb_proj_destroy", "urb_proj_set_adapter",
                 "urb_proj_forward", "urb_proj_sync", "urb_proj_memory", "urb_qk_norm_rope",
-                "urb_sampler_create", "urb_sampler_destroy", "urb_sample", "urb_sampler_sync")
+                "urb_sampler_create", "urb_sampler_destroy", "urb_sample", "urb_sampler_sync",
+                "urb_beams_create", "urb_beams_destroy", "urb_beams_select", "urb_beams_sync")
+# Every symbol include/urb_cache.h declares.
+CACHE_EXPORTS = ("urb_kv_append", "urb_pager_create", "urb_pager_destroy", "urb_pager_plan",
+                 "urb_pager_fork", "urb_pager_sync", "urb_attention_create",
+                 "urb_attention_destroy", "urb_attend", "urb_attention_sync")
 STAGES = ("router", "route", "permute", "gate_up", "down", "shared_gate_up", "shared_down",
           "combine")
 SYNTH_EXPORTS = ("urb_synth_bf16", "urb_synth_activations", "urb_synth_fp4", "urb_synth_fp8",
@@ -110,6 +115,72 @@ class SamplerDesc(ctypes.Structure):
 class SampleParams(ctypes.Structure):
     _fields_ = [("temperature", ctypes.c_void_p), ("top_k", ctypes.c_void_p),
                 ("top_p", ctypes.c_void_p), ("min_p", ctypes.c_void_p)]
+
+
+class BeamsDesc(ctypes.Structure):
+    _fields_ = [("vocab", ctypes.c_uint32), ("width", ctypes.c_uint32), ("picks", ctypes.c_uint32),
+                ("max_requests", ctypes.c_uint32), ("dtype", ctypes.c_int)]
+
+
+class BeamsCall(ctypes.Structure):
+    _fields_ = [("logits", ctypes.c_void_p), ("row_stride", ctypes.c_uint64),
+                ("requests", ctypes.c_uint32), ("end_token", ctypes.c_int32),
+                ("scores", ctypes.c_void_p), ("ended", ctypes.c_void_p),
+                ("scores_out", ctypes.c_void_p), ("tokens", ctypes.c_void_p),
+                ("parents", ctypes.c_void_p), ("ended_out", ctypes.c_void_p)]
+
+
+class KvCache(ctypes.Structure):
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("k_scales", ctypes.c_void_p),
+                ("v_scales", ctypes.c_void_p), ("dtype", ctypes.c_int), ("pages", ctypes.c_uint32),
+                ("heads", ctypes.c_uint32), ("page_size", ctypes.c_uint32),
+                ("head_dim", ctypes.c_uint32), ("page_stride", ctypes.c_uint64),
+                ("head_stride", ctypes.c_uint64), ("token_stride", ctypes.c_uint64)]
+
+
+class KvRows(ctypes.Structure):
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("dtype", ctypes.c_int),
+                ("k_token_stride", ctypes.c_uint64), ("k_head_stride", ctypes.c_uint64),
+                ("v_token_stride", ctypes.c_uint64), ("v_head_stride", ctypes.c_uint64)]
+
+
+class PagerDesc(ctypes.Structure):
+    _fields_ = [("pages", ctypes.c_uint32), ("page_size", ctypes.c_uint32),
+                ("max_rows", ctypes.c_uint32), ("max_blocks", ctypes.c_uint32),
+                ("max_tokens", ctypes.c_uint32)]
+
+
+class PagePlan(ctypes.Structure):
+    _fields_ = [("rows", ctypes.c_uint32), ("tokens", ctypes.c_uint32),
+                ("table_stride", ctypes.c_uint64)] + [
+        (name, ctypes.c_void_p) for name in (
+            "lengths", "added", "tables", "free_pages", "free_count", "lengths_out", "starts",
+            "token_rows", "positions", "slots", "free_count_out")]
+
+
+class PageFork(ctypes.Structure):
+    _fields_ = [("requests", ctypes.c_uint32), ("width", ctypes.c_uint32),
+                ("table_stride", ctypes.c_uint64), ("table_out_stride", ctypes.c_uint64)] + [
+        (name, ctypes.c_void_p) for name in (
+            "parents", "tables", "lengths", "tables_out", "lengths_out", "free_pages", "free_count",
+            "free_count_out", "caches")] + [("n_caches", ctypes.c_uint32)]
+
+
+class AttentionDesc(ctypes.Structure):
+    _fields_ = [("q_heads", ctypes.c_uint32), ("heads", ctypes.c_uint32),
+                ("head_dim", ctypes.c_uint32), ("page_size", ctypes.c_uint32),
+                ("dtype", ctypes.c_int), ("cache_dtype", ctypes.c_int),
+                ("queries", ctypes.c_uint32), ("window", ctypes.c_uint32), ("scale", ctypes.c_float),
+                ("max_rows", ctypes.c_uint32), ("max_length", ctypes.c_uint32)]
+
+
+class AttentionCall(ctypes.Structure):
+    _fields_ = [("rows", ctypes.c_uint32), ("q", ctypes.c_void_p), ("out", ctypes.c_void_p)] + [
+        (name, ctypes.c_uint64) for name in (
+            "q_row_stride", "q_token_stride", "q_head_stride", "out_row_stride",
+            "out_token_stride", "out_head_stride")] + [
+        ("tables", ctypes.c_void_p), ("table_stride", ctypes.c_uint64),
+        ("lengths", ctypes.c_void_p), ("sinks", ctypes.c_void_p), ("lse", ctypes.c_void_p)]
 
 
 _moe = None
@@ -196,9 +267,24 @@ def moe_lib() -> ctypes.CDLL:
         lib.urb_sampler_destroy.argtypes = [P]
         lib.urb_sample.argtypes = [P, P, u64, u32, ctypes.POINTER(SampleParams), P, P, P, P]
         lib.urb_sampler_sync.argtypes = [P, P]
-        for f in STEP_EXPORTS:
+        pp = ctypes.POINTER(ctypes.c_void_p)
+        lib.urb_beams_create.argtypes = [ctypes.POINTER(BeamsDesc), pp]
+        lib.urb_beams_destroy.argtypes = [P]
+        lib.urb_beams_select.argtypes = [P, ctypes.POINTER(BeamsCall), P]
+        lib.urb_beams_sync.argtypes = [P, P]
+        lib.urb_kv_append.argtypes = [ctypes.POINTER(KvCache), ctypes.POINTER(KvRows), P, u32, P]
+        lib.urb_pager_create.argtypes = [ctypes.POINTER(PagerDesc), pp]
+        lib.urb_pager_destroy.argtypes = [P]
+        lib.urb_pager_plan.argtypes = [P, ctypes.POINTER(PagePlan), P]
+        lib.urb_pager_fork.argtypes = [P, ctypes.POINTER(PageFork), P]
+        lib.urb_pager_sync.argtypes = [P, P]
+        lib.urb_attention_create.argtypes = [ctypes.POINTER(AttentionDesc), pp]
+        lib.urb_attention_destroy.argtypes = [P]
+        lib.urb_attend.argtypes = [P, ctypes.POINTER(KvCache), ctypes.POINTER(AttentionCall), P]
+        lib.urb_attention_sync.argtypes = [P, P]
+        for f in STEP_EXPORTS + CACHE_EXPORTS:
             getattr(lib, f).restype = None if f.endswith("_destroy") else status
-        for f in EXPORTS + STEP_EXPORTS:
+        for f in EXPORTS + STEP_EXPORTS + CACHE_EXPORTS:
             if getattr(lib, f).argtypes is None:
                 raise RuntimeError(f"{f}: no ctypes signature")
         _moe = lib

@@ -2,9 +2,10 @@
 
 ``AdaptedProjection``: token rows times one packed matrix (BF16, MXFP4, MXFP8) plus each row's
 low-rank adapter.  ``qk_norm_rope``: the norm of every query and key head with the position
-rotation.  ``Sampler``: a token per row of logits under temperature, top-k, top-p and min-p.  With
+rotation.  ``Sampler``: a token per row of logits under temperature, top-k, top-p and min-p.
+``BeamSelector``: the best candidates of beam search.  With
 ``moe.MoeLayer.forward_block`` between them, a decoder's residual stream stays on the GPU from
-block to block and to the next token (attention is the caller's).
+block to block and to the next token; attention over a paged cache: ``cache``.
 
 Rows are torch.bfloat16 or torch.float32 device tensors.  All compute runs in ``liburb_moe.so``; this
 module only checks tensors and passes their addresses.
@@ -315,3 +316,49 @@ class Sampler(_Context):
         self.sample_into(logits, uniform, ids, probs, stream=stream, **params)
         self.sync(stream)
         return ids, probs
+
+
+class BeamSelector(_Context):
+    """The best ``picks`` of ``width`` beams times ``vocab`` tokens per request (``urb_beams``)."""
+
+    _destroy, _sync = "urb_beams_destroy", "urb_beams_sync"
+
+    def __init__(self, vocab: int, width: int, picks: int, max_requests: int, dtype=None):
+        self.vocab, self.width, self.picks, self.max_requests = vocab, width, picks, max_requests
+        self.dtype = torch.float32 if dtype is None else dtype
+        desc = N.BeamsDesc(vocab, width, picks, max_requests, _type(self.dtype))
+        self._make(N.moe_lib().urb_beams_create, ctypes.byref(desc))
+
+    def select_into(self, logits, scores, scores_out, tokens, parents, ended=None, end_token: int = -1,
+                    ended_out=None, stream=None) -> None:
+        """logits [requests * width, vocab] (rows may be strided) and ``scores`` [requests, width] f32 ->
+        ``scores_out`` f32, ``tokens`` and ``parents`` int32, all [requests, picks], stream-ordered.
+        ``ended`` [requests, width] int32: not 0 for a beam that goes on with ``end_token`` alone;
+        ``ended_out`` [requests, picks] int32: 1 for those that have ended after the step.  With ``picks``
+        = ``width`` outputs may be the inputs of their name."""
+        dev = self.device
+        stride = _rows(logits, "logits", self.vocab, self.dtype, dev)
+        R, odd = divmod(logits.shape[0], self.width)
+        if odd:
+            raise ValueError(f"logits must have {self.width} rows per request")
+        n, m, f32, i32 = R * self.width, R * self.picks, torch.float32, torch.int32
+        call = N.BeamsCall(logits.data_ptr(), stride, R, end_token,
+                           _vector(scores, "scores", n, f32, dev), _vector(ended, "ended", n, i32, dev),
+                           _vector(scores_out, "scores_out", m, f32, dev),
+                           _vector(tokens, "tokens", m, i32, dev),
+                           _vector(parents, "parents", m, i32, dev),
+                           _vector(ended_out, "ended_out", m, i32, dev))
+        with _Current(dev):
+            st = N.moe_lib().urb_beams_select(self._ctx, ctypes.byref(call), _stream(stream, dev))
+        if st:
+            raise N.UrbError(st, "urb_beams_select")
+
+    def select(self, logits, scores, ended=None, end_token: int = -1):
+        """-> (scores f32, tokens int32, parents int32), [requests, picks]; raises UrbError for scores out of
+        range."""
+        R = logits.shape[0] // self.width
+        out = [torch.empty((R, self.picks), dtype=t, device=logits.device)
+               for t in (torch.float32, torch.int32, torch.int32)]
+        self.select_into(logits, scores, *out, ended=ended, end_token=end_token)
+        self.sync()
+        return tuple(out)
