@@ -22,16 +22,20 @@
 #include "urb_panel.hpp"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace urb {
 
 namespace {
 
 constexpr int kUnit = 128;       // tokens
+// A pair's start and end (its queries, the waves' join, an output) cost about what a unit does: counted as one,
+// 200 rows of log-spread lengths up to 12000 take 193 us and not 213, and of 2 no less.
+constexpr int kStart = 1;
 constexpr int kTile = 32;        // tokens of a wave's step
 constexpr int kWaves = 4;
 constexpr int kAttendRows = 1024;  // of a launch
-constexpr int kShares = 768;     // most workgroups of a launch
+constexpr int kCus = 256;
 constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
 constexpr float kMinusInf = -__builtin_inff();
 
@@ -42,12 +46,24 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 template <bool BF16> constexpr int kQueryPlanes = BF16 ? 1 : 3;
 template <bool BF16> constexpr int kWeightPlanes = BF16 ? 2 : 3;
 
-// floats of a part: o [16][dim], m [16], z [16]
+// floats of a part: o [16][dim], then m and z of each of the sixteen
 constexpr __host__ __device__ int part_floats(int dim) { return 16 * (dim + 2); }
 
+// What there is to join: parts of `n` shares from `first` on (n 0: nothing), kept by pairs of the launch or
+// by the share that the pair's second part begins, whichever are fewer.
+struct Join {
+  uint32_t row, pair, first, n;
+};
+
 struct Line {
-  uint32_t pairs;   // of a row
-  uint32_t shares;  // workgroups that can have units
+  uint32_t pairs, tiles;  // of a row; of a cache head's queries
+  uint32_t group;         // query heads of a cache head
+  float inv_group;
+  uint32_t shares;        // workgroups that can have units
+  bool by_pair;           // how joins are kept
+  Join* joins;            // [shares]
+  uint32_t page_magic, page_shift;  // t / page_size = t * page_magic >> page_shift for t < 2^25
+  uint32_t page16, token16;         // strides in units of 16 bytes
 };
 
 // The tokens in reach of any query of a row, [first, end), and first rounded down to a tile; a length that
@@ -62,11 +78,12 @@ __device__ __forceinline__ Reach reach_of(const AttendArgs& a, int length) {
   return Reach{first & ~(kTile - 1), first, length};
 }
 __device__ __forceinline__ uint32_t units_of(Reach r) {
-  return (uint32_t)max(1, (r.end - r.begin + kUnit - 1) / kUnit);
+  return kStart + (uint32_t)max(1, (r.end - r.begin + kUnit - 1) / kUnit);
 }
 
-// upto[i] = units per pair of rows 0 .. i; all threads, ends with a barrier.
-__device__ __forceinline__ void fill_line(const AttendArgs& a, uint32_t* upto, uint32_t* sums, bool flags) {
+// upto[i] = units per pair of rows 0 .. i, and the rows' lengths; all threads, ends with a barrier.
+__device__ __forceinline__ void fill_line(const AttendArgs& a, uint32_t* upto, int* lengths, uint32_t* sums,
+                                          bool flags) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   uint32_t base = 0;
   bool bad = false;
@@ -75,6 +92,7 @@ __device__ __forceinline__ void fill_line(const AttendArgs& a, uint32_t* upto, u
     uint32_t u = 0;
     if (r < a.rows) {
       const int length = a.lengths[r];
+      lengths[r] = length;
       bad |= length < 0 || (uint32_t)length > a.max_length;
       u = units_of(reach_of(a, length));
     }
@@ -96,48 +114,60 @@ __device__ __forceinline__ void fill_line(const AttendArgs& a, uint32_t* upto, u
   if (flags && bad) flag(a.status, kCacheArgument);
 }
 
-// The place of a unit: row, pair of it, first unit of that pair, units of a pair of the row.
+// A value of LDS that all lanes read alike, as a scalar.
+template <class T>
+__device__ __forceinline__ T same(T v) {
+  return (T)__builtin_amdgcn_readfirstlane((int)v);
+}
+
+// The place of a unit: row, pair of it, units of a pair of the row, the pair's first unit of tokens and the
+// end of its units.
 struct Place {
-  uint32_t row, pair, units;
-  uint64_t first;
+  uint32_t row, pair, units, first, end;
 };
-__device__ __forceinline__ Place place_of(const uint32_t* upto, uint32_t rows, uint32_t pairs, uint64_t unit) {
+__device__ __forceinline__ Place place_of(const uint32_t* upto, uint32_t rows, uint32_t pairs, uint32_t unit) {
   uint32_t lo = 0, hi = rows - 1;  // the first row whose units end beyond
   while (lo < hi) {
     const uint32_t mid = (lo + hi) / 2;
-    if ((uint64_t)upto[mid] * pairs > unit) hi = mid;
+    if (same(upto[mid]) * pairs > unit) hi = mid;
     else lo = mid + 1;
   }
-  const uint32_t under = lo ? upto[lo - 1] : 0;
+  const uint32_t under = lo ? same(upto[lo - 1]) : 0;
   Place p;
   p.row = lo;
-  p.units = upto[lo] - under;
-  const uint64_t start = (uint64_t)under * pairs;
-  p.pair = (uint32_t)((unit - start) / p.units);
-  p.first = start + (uint64_t)p.pair * p.units;
+  p.units = same(upto[lo]) - under;
+  const uint32_t start = under * pairs;
+  p.pair = same((unit - start) / p.units);
+  p.end = start + (p.pair + 1) * p.units;
+  p.first = p.end - p.units + kStart;
   return p;
 }
 
-// Units of share g of n: [total g / n, total (g + 1) / n).
-__device__ __forceinline__ uint64_t share_begin(uint64_t total, uint32_t g, uint32_t n) {
-  return total * g / n;
-}
-// The share that unit u lies in.
-__device__ __forceinline__ uint32_t share_of(uint64_t total, uint64_t u, uint32_t n) {
-  return (uint32_t)(((u + 1) * n - 1) / total);
-}
+// n shares of all the units: the first `more` of them have one unit more than the others' `each`.
+struct Shares {
+  uint32_t n, each, more;
+  __device__ __forceinline__ Shares(uint32_t total, uint32_t most)
+      : n(min(most, total)), each(same(total / n)), more(total - each * n) {}
+  __device__ __forceinline__ uint32_t begin(uint32_t g) const { return g * each + min(g, more); }
+  // the share that a unit lies in
+  __device__ __forceinline__ uint32_t of(uint32_t unit) const {
+    const uint32_t longer = more * (each + 1);
+    return same(unit < longer ? unit / (each + 1) : more + (unit - longer) / each);
+  }
+};
 
 // Query c of a pair's sixteen: new token and head.
 struct Query {
   uint32_t token, head;
   bool there;
 };
-__device__ __forceinline__ Query query_of(const AttendArgs& a, uint32_t pair, uint32_t tiles, int c) {
-  const uint32_t group = a.q_heads / a.cache.heads;
-  const uint32_t h = pair / tiles, i = (pair - h * tiles) * 16 + c;
+__device__ __forceinline__ Query query_of(const AttendArgs& a, const Line& line, uint32_t head, uint32_t pair,
+                                          int c) {
+  const uint32_t i = (pair - head * line.tiles) * 16 + c;
   Query q;
-  q.token = i / group;
-  q.head = h * group + (i - q.token * group);
+  // (i < 2^18: the quotient is off by less than the half that is added)
+  q.token = (uint32_t)(((float)i + 0.5f) * line.inv_group);
+  q.head = head * line.group + (i - q.token * line.group);
   q.there = q.token < a.queries;
   return q;
 }
@@ -200,9 +230,15 @@ __device__ __forceinline__ void finish4(const AttendArgs& a, uint32_t row, const
   store4<BF16>(a.out + row * a.out_row + q.token * a.out_token + q.head * a.out_head + d * (BF16 ? 2 : 4), r);
 }
 
+// Workgroups per CU, and with it shares: what the registers hold.  (More shares than can run at a time leave
+// the last ones to run by themselves: 64 rows of 4096 tokens of 8 heads of 128 in E4M3 take 100 us with 512 and
+// 143 with 768; f32 rows of 128 over BF16 have 5.55 TB/s with one per CU.)
+template <int DS, bool F8, bool BF16>
+constexpr int kPerCu = DS == 2 && F8 ? 3 : DS <= 3 || (DS == 4 && (F8 || BF16)) ? 2 : 1;
+
 // DS: head_dim in steps of 32, rounded up.
 template <int DS, bool F8, bool BF16>
-__global__ __launch_bounds__(64 * kWaves) void attend_kernel(AttendArgs a, Line line) {
+__global__ __launch_bounds__(64 * kWaves, (kPerCu<DS, F8, BF16>)) void attend_kernel(AttendArgs a, Line line) {
   constexpr int QP = kQueryPlanes<BF16>, PP = kWeightPlanes<BF16>;
   constexpr int KS = F8 ? 2 * ((DS + 1) / 2) : DS;  // MFMA steps over head_dim
   constexpr int KL = F8 ? KS / 2 : KS;              // 16-byte loads of 16 K rows per lane
@@ -216,167 +252,231 @@ __global__ __launch_bounds__(64 * kWaves) void attend_kernel(AttendArgs a, Line 
   __shared__ __attribute__((aligned(16))) uint4 q_lds[QP][KS][64];
   __shared__ float s_m[kWaves][16], s_z[kWaves][16];
   __shared__ uint32_t upto[kAttendRows], sums[kWaves];
+  __shared__ int lengths[kAttendRows];
 
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 15, grp = lane >> 4;
-  fill_line(a, upto, sums, blockIdx.x == 0);
-  const uint64_t total = (uint64_t)upto[a.rows - 1] * line.pairs;
-  const uint32_t shares = (uint32_t)min<uint64_t>(line.shares, total);
-  if (blockIdx.x >= shares) return;
-  uint64_t unit = share_begin(total, blockIdx.x, shares);
-  const uint64_t unit_end = share_begin(total, blockIdx.x + 1, shares);
-  const uint32_t tiles = line.pairs / a.cache.heads;
+  fill_line(a, upto, lengths, sums, blockIdx.x == 0);
+  const Shares shares(same(upto[a.rows - 1]) * line.pairs, line.shares);
+  if (blockIdx.x >= shares.n) {
+    if (!line.by_pair && tid == 0) line.joins[blockIdx.x].n = 0;
+    return;
+  }
+  const uint32_t unit_begin = shares.begin(blockIdx.x), unit_end = shares.begin(blockIdx.x + 1);
   const float scale2 = a.scale * kLog2e;
   const uint32_t dim = a.cache.dim;
+  const bool full = dim == (F8 ? 32 * KS : 32 * DS);
   uint8_t* const mine = stage[wave];
 
-  while (unit < unit_end) {
-    const Place at = place_of(upto, a.rows, line.pairs, unit);
-    const uint64_t stop = min(unit_end, at.first + at.units);
-    const Reach reach = reach_of(a, a.lengths[at.row]);
-    const int t0 = reach.begin + (int)(unit - at.first) * kUnit;
-    const int t1 = min(reach.end, reach.begin + (int)(stop - at.first) * kUnit);
-    const uint32_t head = at.pair / tiles;
-    const Query mine_q = query_of(a, at.pair, tiles, col);
+  // What of a pair lies in this share: tokens t0 .. t1 - 1 of row `row`, units up to `stop`; none past the
+  // share's last token.
+  struct Segment {
+    Place at;
+    Reach reach;
+    uint32_t stop;
+    int t0, t1;
+    uint32_t head;
+    bool begins, there;
+  };
+  auto segment_at = [&](uint32_t unit) -> Segment {
+    Segment g;
+    g.there = unit < unit_end;
+    if (!g.there) return g;
+    g.at = place_of(upto, a.rows, line.pairs, unit);
+    g.there = unit_end > g.at.first;
+    g.reach = reach_of(a, same(lengths[g.at.row]));
+    g.begins = unit <= g.at.first;
+    g.stop = min(unit_end, g.at.end);
+    g.t0 = g.reach.begin + (g.begins ? 0 : (int)(unit - g.at.first) * kUnit);
+    g.t1 = min(g.reach.end, g.reach.begin + (int)(g.stop - g.at.first) * kUnit);
+    g.head = same(g.at.pair / line.tiles);
+    return g;
+  };
 
-    // queries, in the order of the operand (an E4M3 step takes eight of sixteen neighbours)
-    __syncthreads();
-    for (int i = tid; i < KS * 64; i += 64 * kWaves) {
-      const int s = i >> 6, l = i & 63, g = l >> 4;
-      const int d = F8 ? 64 * (s >> 1) + 16 * g + 8 * (s & 1) : 32 * s + 8 * g;
-      const Query q = query_of(a, at.pair, tiles, l & 15);
-      float v[8] = {};
-      bf16x8 p[QP];
-      const bool in = q.there && d < (int)dim;
-      const uint8_t* from = a.q + at.row * a.q_row + q.token * a.q_token + q.head * a.q_head;
-      if constexpr (BF16) {
-        uint4 w = make_uint4(0, 0, 0, 0);
-        if (in) w = ldg16(from + 2 * d);
-        q_lds[0][s][l] = w;
-      } else {
-        if (in) {
-          const float4 x = u2f4(ldg16(from + 4 * d)), y = u2f4(ldg16(from + 4 * d + 16));
-          v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
-          v[4] = y.x; v[5] = y.y; v[6] = y.z; v[7] = y.w;
-        }
-        planes_of<QP>(v, p);
-#pragma unroll
-        for (int k = 0; k < QP; ++k) q_lds[k][s][l] = __builtin_bit_cast(uint4, p[k]);
-      }
+  auto block_of = [&](int t) -> uint32_t {
+    return (uint32_t)((uint64_t)(uint32_t)t * line.page_magic >> line.page_shift);
+  };
+  // The tile's token of this lane: lanes l and l + 32 have token l.
+  auto page_of = [&](const Segment& g, int tile) -> int {
+    const int t = tile + (lane & 31);
+    return t >= g.reach.first && t < g.t1 ? a.tables[g.at.row * a.table_stride + block_of(t)] : -1;
+  };
+  uint4 kr[2][KL], vr[VL];
+  uint32_t valid = 0, code = 0;  // tokens of the tile that there are; the scale code of the lane's token
+  // Starts the loads of a tile whose pages are known.
+  auto load = [&](const Segment& g, int tile, int page) __attribute__((always_inline)) {
+    const int t = tile + (lane & 31);
+    const bool fine = (uint32_t)page < a.cache.pages;
+    if (t >= g.reach.first && t < g.t1 && !fine) flag(a.status, kCacheArgument);
+    valid = (uint32_t)__ballot(fine);
+    const uint32_t slot = (uint32_t)t - block_of(t) * a.cache.page;
+    // 16-byte units from the head's base to the lane's token
+    const uint32_t off = fine ? (uint32_t)page * line.page16 + slot * line.token16 : 0;
+    if constexpr (F8) {
+      const uint8_t* const scales = lane < 32 ? a.cache.k_scales : a.cache.v_scales;
+      code = fine ? ldg_u8(scales + ((uint64_t)page * a.cache.heads + g.head) * a.cache.page + slot) : 127;
     }
-    __syncthreads();
-
-    const int my_end = mine_q.there ? reach.end - (int)(a.queries - 1 - mine_q.token) : 0;
-    const int my_begin = a.window ? (int)max<int64_t>(0, (int64_t)my_end - a.window) : 0;
-    // tiles inside these bounds need no mask for any query
-    const int all_begin = a.window ? (int)max<int64_t>(0, (int64_t)reach.end - a.window) : 0;
-    const int all_end = reach.end - (int)(a.queries - 1);
-
-    float m = kMinusInf, z = 0.0f;
-    f32x4 o[2 * DS];
-#pragma unroll
-    for (int j = 0; j < 2 * DS; ++j) o[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-
-    const int32_t* table = a.tables + at.row * a.table_stride;
-    const uint8_t* const kbase = a.cache.k + head * a.cache.head_stride;
-    const uint8_t* const vbase = a.cache.v + head * a.cache.head_stride;
-    const uint8_t* const scales = (lane < 32 ? a.cache.k_scales : a.cache.v_scales);
-
-    // The tile's token of this lane: lanes l and l + 32 have token l.
-    auto page_of = [&](int tile) -> int {
-      const int t = tile + (lane & 31);
-      return t >= reach.first && t < t1 ? table[(uint32_t)t / a.cache.page] : -1;
-    };
-    uint4 kr[2][KL], vr[VL];
-    uint32_t valid = 0, code = 0;  // tokens of the tile that there are; the scale code of the lane's token
-    uint32_t off = 0;              // 16-byte units from the head's base to the lane's token
-    auto place_tile = [&](int tile, int page) {
-      const int t = tile + (lane & 31);
-      const bool fine = (uint32_t)page < a.cache.pages;
-      if (t >= reach.first && t < t1 && !fine) flag(a.status, kCacheArgument);
-      valid = (uint32_t)__ballot(fine);
-      const uint32_t slot = (uint32_t)t % a.cache.page;
-      off = fine ? (uint32_t)((page * a.cache.page_stride + slot * a.cache.token_stride) >> 4) : 0;
-      if constexpr (F8)
-        code = fine ? ldg_u8(scales + ((uint64_t)page * a.cache.heads + head) * a.cache.page + slot) : 127;
-    };
-    auto load_k = [&]() {
+    const uint8_t* const kbase = a.cache.k + g.head * a.cache.head_stride;
+    const uint8_t* const vbase = a.cache.v + g.head * a.cache.head_stride;
+    // (values past the head's are not read; V's of tokens that are not there are zero, for a weight of zero
+    // does not undo a NaN)
+    auto both = [&](auto check) __attribute__((always_inline)) {
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const uint8_t* p = kbase + ((uint64_t)(uint32_t)__shfl((int)off, 16 * h + col, 64) << 4);
 #pragma unroll
         for (int s = 0; s < KL; ++s) {
           const uint32_t d = (F8 ? 64 : 32) * s + (F8 ? 16 : 8) * grp;
-          kr[h][s] = make_uint4(0, 0, 0, 0);
-          if (d < dim) kr[h][s] = ldg16(p + (F8 ? d : 2 * d));
+          const bool in = !decltype(check)::value || d < dim;
+          kr[h][s] = in ? ldg16(p + (F8 ? d : 2 * d)) : make_uint4(0, 0, 0, 0);
         }
       }
-    };
-    auto load_v = [&]() {
 #pragma unroll
       for (int i = 0; i < VL; ++i) {
-        const int n = i * 64 + lane, t = n / VP, piece = n - t * VP;
-        const uint8_t* p = vbase + ((uint64_t)(uint32_t)__shfl((int)off, t, 64) << 4);
-        vr[i] = make_uint4(0, 0, 0, 0);
-        // (values that are not there stay zero: a weight of zero does not undo a NaN)
-        if (valid >> t & 1 && piece * (F8 ? 16u : 8u) < dim) vr[i] = ldg16(p + 16 * piece);
+        const int n = i * 64 + lane, u = n / VP, piece = n - u * VP;
+        const uint8_t* p = vbase + ((uint64_t)(uint32_t)__shfl((int)off, u, 64) << 4) + 16 * piece;
+        const bool in = !decltype(check)::value || (valid >> u & 1 && piece * (F8 ? 16u : 8u) < dim);
+        vr[i] = in ? ldg16(p) : make_uint4(0, 0, 0, 0);
       }
     };
+    if (full && valid == 0xffffffffu) both(std::false_type{});
+    else both(std::true_type{});
+  };
 
-    int tile = t0 + kTile * wave;
-    int next_page = -1;
-    if (tile < t1) {
-      place_tile(tile, page_of(tile));
-      next_page = page_of(tile + kUnit);
-      load_k();
-      load_v();
+  // Queries, in the order of the operand (an E4M3 step takes eight of sixteen neighbours): read ahead, put
+  // into LDS when the products with the last ones are done.
+  constexpr int QL = (KS + kWaves - 1) / kWaves;
+  uint4 qr[QL][BF16 ? 1 : 2];
+  auto load_q = [&](const Segment& g) {
+#pragma unroll
+    for (int i = 0; i < QL; ++i) {
+      const int s = i * kWaves + wave;
+      const int d = F8 ? 64 * (s >> 1) + 16 * grp + 8 * (s & 1) : 32 * s + 8 * grp;
+      const Query q = query_of(a, line, g.head, g.at.pair, col);
+      const uint8_t* from = a.q + g.at.row * a.q_row + q.token * a.q_token + q.head * a.q_head;
+#pragma unroll
+      for (int k = 0; k < (BF16 ? 1 : 2); ++k) {
+        qr[i][k] = make_uint4(0, 0, 0, 0);
+        if (q.there && s < KS && d < (int)dim) qr[i][k] = ldg16(from + (BF16 ? 2 : 4) * d + 16 * k);
+      }
     }
-    for (; tile < t1; tile += kUnit) {
+  };
+  auto stage_q = [&]() {
+#pragma unroll
+    for (int i = 0; i < QL; ++i) {
+      const int s = i * kWaves + wave;
+      if (s >= KS) break;
+      if constexpr (BF16) {
+        q_lds[0][s][lane] = qr[i][0];
+      } else {
+        const float4 x = u2f4(qr[i][0]), y = u2f4(qr[i][1]);
+        float v[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+        bf16x8 p[QP];
+        planes_of<QP>(v, p);
+#pragma unroll
+        for (int k = 0; k < QP; ++k) q_lds[k][s][lane] = __builtin_bit_cast(uint4, p[k]);
+      }
+    }
+  };
+
+  Segment g = segment_at(unit_begin);
+  if (!line.by_pair && tid == 0) {
+    // the share's first boundary, for the second kernel
+    const uint32_t last = shares.of(g.at.end - 1);
+    const bool second = !g.begins && shares.of(g.at.first) == blockIdx.x - 1;
+    line.joins[blockIdx.x] = Join{g.at.row, g.at.pair, blockIdx.x - 1, second ? last - blockIdx.x + 2 : 0};
+  }
+  if (!g.there) return;
+  // Pages are known a segment, or two tiles, before their loads begin.
+  load_q(g);
+  int tile = g.t0 + kTile * wave;
+  int next_page = page_of(g, tile + kUnit);
+  const int first_page = page_of(g, tile);
+  Segment next = segment_at(g.stop);
+  int page0 = -1, page1 = -1, next_tile = 0;
+  auto pages_of_next = [&]() {
+    if (!next.there) return;
+    next_tile = next.t0 + kTile * wave;
+    page0 = page_of(next, next_tile);
+    page1 = page_of(next, next_tile + kUnit);
+  };
+  pages_of_next();
+  if (tile < g.t1) load(g, tile, first_page);
+  stage_q();
+  __syncthreads();
+
+  for (;;) {
+    const bool whole = g.begins && g.stop == g.at.end, goes_on = next.there;
+    if (line.by_pair && g.begins && tid == 0) {
+      const uint32_t last = shares.of(g.at.end - 1);
+      line.joins[g.at.row * line.pairs + g.at.pair] =
+          Join{g.at.row, g.at.pair, blockIdx.x, whole ? 0 : last - blockIdx.x + 1};
+    }
+    if (goes_on) load_q(next);
+
+    const Query mine_q = query_of(a, line, g.head, g.at.pair, col);
+    const int my_end = mine_q.there ? g.reach.end - (int)(a.queries - 1 - mine_q.token) : 0;
+    const int my_begin = a.window ? (int)max<int64_t>(0, (int64_t)my_end - a.window) : 0;
+    // tiles inside these bounds need no mask for any query
+    const int all_begin = a.window ? (int)max<int64_t>(0, (int64_t)g.reach.end - a.window) : 0;
+    const int all_end = g.reach.end - (int)(a.queries - 1);
+
+    float m = kMinusInf, z = 0.0f;
+    f32x4 o[2 * DS];
+#pragma unroll
+    for (int j = 0; j < 2 * DS; ++j) o[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+
+    do {
+      // (a wave without a tile in the segment comes here once, for the loads)
+      const bool have = tile < g.t1, stay = tile + kUnit < g.t1;
       const uint32_t now = valid, now_code = code;
-      const bool more = tile + kUnit < t1;
       // scores
       f32x4 s[2];
+      if (have) {
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        s[h] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-        float ks = 0.0f;
-        if constexpr (F8) ks = e8m0_to_f32((uint32_t)__shfl((int)now_code, 16 * h + col, 64));
+        for (int h = 0; h < 2; ++h) {
+          s[h] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+          float ks = 0.0f;
+          if constexpr (F8) ks = e8m0_to_f32((uint32_t)__shfl((int)now_code, 16 * h + col, 64));
 #pragma unroll
-        for (int j = 0; j < KS; ++j) {
-          uint4 w;
-          if constexpr (F8)
-            w = j & 1 ? decode8(kr[h][j / 2].z, kr[h][j / 2].w, ks) : decode8(kr[h][j / 2].x, kr[h][j / 2].y, ks);
-          else w = kr[h][j];
-          const bf16x8 k = __builtin_bit_cast(bf16x8, w);
+          for (int j = 0; j < KS; ++j) {
+            uint4 w;
+            if constexpr (F8)
+              w = j & 1 ? decode8(kr[h][j / 2].z, kr[h][j / 2].w, ks) : decode8(kr[h][j / 2].x, kr[h][j / 2].y, ks);
+            else w = kr[h][j];
+            const bf16x8 k = __builtin_bit_cast(bf16x8, w);
 #pragma unroll
-          for (int p = QP - 1; p >= 0; --p)
-            s[h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k, __builtin_bit_cast(bf16x8, q_lds[p][j][lane]),
-                                                           s[h], 0, 0, 0);
+            for (int p = QP - 1; p >= 0; --p)
+              s[h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k, __builtin_bit_cast(bf16x8, q_lds[p][j][lane]),
+                                                             s[h], 0, 0, 0);
+          }
+        }
+        // V into LDS, then the loads of the next tile
+        if constexpr (F8) {
+#pragma unroll
+          for (int i = 0; i < VL; ++i) {
+            const int n = i * 64 + lane, t = n / VP, piece = n - t * VP;
+            const float vs = e8m0_to_f32((uint32_t)__shfl((int)now_code, 32 + t, 64));
+            uint4* to = reinterpret_cast<uint4*>(mine + t * VSTRIDE + 32 * piece);
+            to[0] = decode8(vr[i].x, vr[i].y, vs);
+            to[1] = decode8(vr[i].z, vr[i].w, vs);
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < VL; ++i) {
+            const int n = i * 64 + lane, t = n / VP, piece = n - t * VP;
+            *reinterpret_cast<uint4*>(mine + t * VSTRIDE + 16 * piece) = vr[i];
+          }
         }
       }
-      // V into LDS, then the loads of the next tile
-      if constexpr (F8) {
-#pragma unroll
-        for (int i = 0; i < VL; ++i) {
-          const int n = i * 64 + lane, t = n / VP, piece = n - t * VP;
-          const float vs = e8m0_to_f32((uint32_t)__shfl((int)now_code, 32 + t, 64));
-          uint4* to = reinterpret_cast<uint4*>(mine + t * VSTRIDE + 32 * piece);
-          to[0] = decode8(vr[i].x, vr[i].y, vs);
-          to[1] = decode8(vr[i].z, vr[i].w, vs);
-        }
-      } else {
-#pragma unroll
-        for (int i = 0; i < VL; ++i) {
-          const int n = i * 64 + lane, t = n / VP, piece = n - t * VP;
-          *reinterpret_cast<uint4*>(mine + t * VSTRIDE + 16 * piece) = vr[i];
-        }
+      if (stay || goes_on) {
+        const Segment& to = stay ? g : next;
+        const int to_tile = stay ? tile + kUnit : next_tile;
+        const int page = stay ? next_page : page0;
+        next_page = stay ? page_of(g, tile + 2 * kUnit) : page1;
+        if (to_tile < to.t1) load(to, to_tile, page);
       }
-      if (more) {
-        place_tile(tile + kUnit, next_page);
-        next_page = page_of(tile + 2 * kUnit);
-        load_k();
-        load_v();
-      }
+      if (!have) break;
       // weights
       float e[8];
 #pragma unroll
@@ -426,7 +526,8 @@ __global__ __launch_bounds__(64 * kWaves) void attend_kernel(AttendArgs a, Line 
           o[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, w[k], o[j], 0, 0, 0);
       }
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    }
+      tile += kUnit;
+    } while (tile < g.t1);
 
     // the waves' sums, joined
     z += __shfl_xor(z, 16, 64);
@@ -440,6 +541,7 @@ __global__ __launch_bounds__(64 * kWaves) void attend_kernel(AttendArgs a, Line 
       s_z[wave][lane] = z;
     }
     __syncthreads();
+    if (goes_on) stage_q();
     const int c = tid >> 4;
     float mm = s_m[0][c];
 #pragma unroll
@@ -450,10 +552,9 @@ __global__ __launch_bounds__(64 * kWaves) void attend_kernel(AttendArgs a, Line 
       f[w] = mm == kMinusInf ? 0.0f : exp2f((s_m[w][c] - mm) * scale2);
       zz = fmaf(s_z[w][c], f[w], zz);
     }
-    const bool whole = unit == at.first && stop == at.first + at.units;
-    const Query q = query_of(a, at.pair, tiles, c);
+    const Query q = query_of(a, line, g.head, g.at.pair, c);
     // the first part of a pair that goes on in the next share is this one's second
-    float* const part = a.parts + (size_t)(2 * blockIdx.x + (unit == at.first)) * part_floats(32 * DS);
+    float* const part = a.parts + (size_t)(2 * blockIdx.x + g.begins) * part_floats(32 * DS);
     for (int d = 4 * (tid & 15); d < 32 * DS; d += 64) {
       float4 r = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
@@ -465,103 +566,166 @@ __global__ __launch_bounds__(64 * kWaves) void attend_kernel(AttendArgs a, Line 
         r.z = fmaf(v.z, f[w], r.z);
         r.w = fmaf(v.w, f[w], r.w);
       }
-      if (whole) finish4<BF16>(a, at.row, q, d, r, mm, zz);
+      if (whole) finish4<BF16>(a, g.at.row, q, d, r, mm, zz);
       else *reinterpret_cast<float4*>(part + 32 * DS * c + d) = r;
     }
-    if (!whole && (tid & 15) == 0) {
-      part[16 * 32 * DS + c] = mm;
-      part[16 * 32 * DS + 16 + c] = zz;
-    }
-    unit = stop;
+    if (!whole && (tid & 15) == 0)
+      *reinterpret_cast<float2*>(part + 16 * 32 * DS + 2 * c) = make_float2(mm, zz);
+    if (!goes_on) break;
+    __syncthreads();
+    g = next;
+    tile = next_tile;
+    next = segment_at(g.stop);
+    pages_of_next();
   }
 }
 
-// Workgroup (g, y) joins the pair that share g begins inside of, if share g - 1 holds its first unit:
-// dimensions 64 y .. 64 y + 63 of its sixteen queries.
+// Two parts of a query as one: (m, z, o) takes in (pm, pz, po).
+__device__ __forceinline__ void take_in(float& m, float& z, float4& o, float pm, float pz, const float4& po,
+                                        float scale2) {
+  const float top = fmaxf(m, pm);
+  if (top == kMinusInf) return;
+  const float f = exp2f((m - top) * scale2), g = exp2f((pm - top) * scale2);
+  m = top;
+  z = fmaf(pz, g, z * f);
+  o.x = fmaf(po.x, g, o.x * f);
+  o.y = fmaf(po.y, g, o.y * f);
+  o.z = fmaf(po.z, g, o.z * f);
+  o.w = fmaf(po.w, g, o.w * f);
+}
+
+// Workgroup (j, y) joins the parts of join j.  `lanes` threads hold a query's row, four values each; `groups`
+// of them take the parts in turn, so a row of many parts has many loads on their way.
 template <bool BF16>
-__global__ __launch_bounds__(256) void join_kernel(AttendArgs a, Line line, int width) {
-  __shared__ uint32_t upto[kAttendRows], sums[kWaves];
-  fill_line(a, upto, sums, false);
-  const uint64_t total = (uint64_t)upto[a.rows - 1] * line.pairs;
-  const uint32_t shares = (uint32_t)min<uint64_t>(line.shares, total);
-  const uint32_t g = blockIdx.x + 1;
-  if (g >= shares) return;
-  const uint64_t unit = share_begin(total, g, shares);
-  const Place at = place_of(upto, a.rows, line.pairs, unit);
-  if (at.first == unit || share_of(total, at.first, shares) != g - 1) return;
-  const uint32_t last = share_of(total, at.first + at.units - 1, shares);
-  const int c = threadIdx.x >> 4, d = 64 * blockIdx.y + 4 * (threadIdx.x & 15);
-  const size_t size = part_floats(width);
-  // the pair's first part is its share's second, the others are first
-  auto part = [&](uint32_t k) { return a.parts + (2 * (size_t)k + (k == g - 1)) * size; };
-  float m = kMinusInf;
-  for (uint32_t k = g - 1; k <= last; ++k) m = fmaxf(m, part(k)[16 * width + c]);
+__global__ __launch_bounds__(256) void join_kernel(AttendArgs a, Line line, int width, int lanes, int groups) {
+  __shared__ float4 s_o[256];
+  __shared__ float2 s_mz[256];
+  const Join join = line.joins[blockIdx.x + (line.by_pair ? 0 : 1)];
+  if (join.n == 0) return;
+  const int tid = threadIdx.x, set = tid / lanes, d = 4 * (tid - set * lanes);
+  const int queries = 256 / lanes / groups, group = set % groups;
+  const int c = blockIdx.y * queries + set / groups;
   const float scale2 = a.scale * kLog2e;
-  float z = 0.0f;
-  float4 r = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  const size_t size = part_floats(width);
+  float m = kMinusInf, z = 0.0f;
+  float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
   const bool in = d < width;
-  for (uint32_t k = g - 1; k <= last; ++k) {
-    const float* p = part(k);
-    const float f = m == kMinusInf ? 0.0f : exp2f((p[16 * width + c] - m) * scale2);
-    z = fmaf(p[16 * width + 16 + c], f, z);
-    if (in) {
-      const float4 v = *reinterpret_cast<const float4*>(p + width * c + d);
-      r.x = fmaf(v.x, f, r.x);
-      r.y = fmaf(v.y, f, r.y);
-      r.z = fmaf(v.z, f, r.z);
-      r.w = fmaf(v.w, f, r.w);
+  constexpr int AHEAD = 4;
+  for (uint32_t k0 = group; k0 < join.n; k0 += AHEAD * groups) {
+    float2 mz[AHEAD];
+    float4 v[AHEAD];
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) {
+      const uint32_t k = k0 + i * groups;
+      mz[i] = make_float2(kMinusInf, 0.0f);
+      v[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      if (k < join.n && in) {
+        // a pair's first part is its share's second, the others are first
+        const float* p = a.parts + (2 * (size_t)(join.first + k) + (k == 0)) * size;
+        mz[i] = *reinterpret_cast<const float2*>(p + 16 * width + 2 * c);
+        v[i] = *reinterpret_cast<const float4*>(p + width * c + d);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) take_in(m, z, o, mz[i].x, mz[i].y, v[i], scale2);
+  }
+  if (groups > 1) {
+    s_o[tid] = o;
+    s_mz[tid] = make_float2(m, z);
+    __syncthreads();
+    if (group) return;
+    for (int g = 1; g < groups; ++g) {
+      const float2 mz = s_mz[tid + g * lanes];
+      take_in(m, z, o, mz.x, mz.y, s_o[tid + g * lanes], scale2);
     }
   }
-  if (in) finish4<BF16>(a, at.row, query_of(a, at.pair, line.pairs / a.cache.heads, c), d, r, m, z);
+  if (in) finish4<BF16>(a, join.row, query_of(a, line, join.pair / line.tiles, join.pair, c), d, o, m, z);
 }
 
-// head_dim in steps of 32 as the kernels are built for
-int steps_of(uint32_t dim) {
-  const int s = ((int)dim + 31) / 32;
-  return s <= 2 ? 2 : s == 5 ? 6 : s == 7 ? 8 : s;
+// The most units of a pair.
+uint32_t most_units(const AttendArgs& a) { return kStart + (a.max_length + kUnit - 1) / kUnit + 1; }
+
+template <int DS, bool F8, bool BF16>
+void launch_pass(const AttendArgs& a, Line line, hipStream_t s) {
+  constexpr uint32_t most = kPerCu<DS, F8, BF16> * kCus;
+  // no more shares than there can be units
+  line.shares = (uint32_t)std::min<uint64_t>(most, (uint64_t)a.rows * line.pairs * most_units(a));
+  line.by_pair = (uint64_t)a.rows * line.pairs < line.shares;
+  line.joins = reinterpret_cast<Join*>(a.parts + (size_t)2 * most * part_floats(32 * DS));
+  attend_kernel<DS, F8, BF16><<<line.shares, 64 * kWaves, 0, s>>>(a, line);
+  const uint32_t joins = line.by_pair ? a.rows * line.pairs : line.shares - 1;
+  if (joins == 0) return;
+  // threads per query, and how many sets of them go through its parts: about four parts each
+  const int lanes = DS <= 2 ? 16 : DS <= 4 ? 32 : 64;
+  int groups = 1;
+  while (groups < 256 / lanes && 4 * groups * joins < line.shares) groups *= 2;
+  const int queries = 256 / lanes / groups;
+  join_kernel<BF16><<<dim3(joins, (16 + queries - 1) / queries), 256, 0, s>>>(a, line, 32 * DS, lanes, groups);
 }
 
-template <int DS, bool BF16>
-void launch_steps(const AttendArgs& a, const Line& line, hipStream_t s) {
-  if (a.cache.k_scales) attend_kernel<DS, true, BF16><<<line.shares, 64 * kWaves, 0, s>>>(a, line);
-  else attend_kernel<DS, false, BF16><<<line.shares, 64 * kWaves, 0, s>>>(a, line);
-  if (line.shares > 1) join_kernel<BF16><<<dim3(line.shares - 1, (DS + 1) / 2), 256, 0, s>>>(a, line, 32 * DS);
+template <int DS, bool F8, bool BF16>
+constexpr size_t work_of() {
+  return (size_t)kPerCu<DS, F8, BF16> * kCus * (2 * part_floats(32 * DS) * sizeof(float) + sizeof(Join));
 }
 
-template <bool BF16>
-void launch_rows(const AttendArgs& a, hipStream_t s) {
-  const uint32_t group = a.q_heads / a.cache.heads;
-  Line line;
-  line.pairs = a.cache.heads * ((a.queries * group + 15) / 16);
-  // as many shares as there can be units
-  const uint64_t most = (uint64_t)a.rows * line.pairs * ((a.max_length + kUnit - 1) / kUnit + 1);
-  line.shares = (uint32_t)std::min<uint64_t>(kShares, most);
-  switch (steps_of(a.cache.dim)) {
-    case 2: launch_steps<2, BF16>(a, line, s); break;
-    case 3: launch_steps<3, BF16>(a, line, s); break;
-    case 4: launch_steps<4, BF16>(a, line, s); break;
-    case 6: launch_steps<6, BF16>(a, line, s); break;
-    default: launch_steps<8, BF16>(a, line, s);
+// Calls f with the kernel's constants as types.
+template <class F>
+auto with_kernel(uint32_t dim, bool f8, bool bf16, F f) {
+  auto rows = [&](auto ds, auto f8_) {
+    return bf16 ? f(ds, f8_, std::true_type{}) : f(ds, f8_, std::false_type{});
+  };
+  auto types = [&](auto ds) { return f8 ? rows(ds, std::true_type{}) : rows(ds, std::false_type{}); };
+  switch (((int)dim + 31) / 32) {
+    case 1:
+    case 2: return types(std::integral_constant<int, 2>{});
+    case 3: return types(std::integral_constant<int, 3>{});
+    case 4: return types(std::integral_constant<int, 4>{});
+    case 5:
+    case 6: return types(std::integral_constant<int, 6>{});
+    default: return types(std::integral_constant<int, 8>{});
   }
+}
+
+Line line_of(const AttendArgs& a) {
+  Line line{};
+  line.group = a.q_heads / a.cache.heads;
+  line.inv_group = 1.0f / (float)line.group;
+  line.tiles = (a.queries * line.group + 15) / 16;
+  line.pairs = a.cache.heads * line.tiles;
+  // with 2^s < page_size <= 2^(s + 1), the magic number of shift 32 + s has 32 bits, and its excess times t
+  // stays below 2^(32 + s)
+  line.page_shift = 31;
+  while (a.cache.page > 1u << (line.page_shift - 31)) ++line.page_shift;
+  line.page_magic = (uint32_t)(((1ull << line.page_shift) + a.cache.page - 1) / a.cache.page);
+  line.page16 = (uint32_t)(a.cache.page_stride >> 4);
+  line.token16 = (uint32_t)(a.cache.token_stride >> 4);
+  return line;
 }
 
 }  // namespace
 
-size_t attend_work_bytes(uint32_t dim) {
-  return (size_t)2 * kShares * part_floats(32 * steps_of(dim)) * sizeof(float);
+size_t attend_work_bytes(uint32_t dim, bool f8, bool rows_bf16) {
+  return with_kernel(dim, f8, rows_bf16, [](auto ds, auto f8_, auto bf16) {
+    return work_of<decltype(ds)::value, decltype(f8_)::value, decltype(bf16)::value>();
+  });
 }
 
 void launch_attend(const AttendArgs& a, bool rows_bf16, hipStream_t s) {
-  for (uint32_t r = 0; r < a.rows; r += kAttendRows) {
+  const Line line = line_of(a);
+  // rows of a launch: their units have 32 bits (a row has fewer than 2^31)
+  const uint32_t most = (uint32_t)std::min<uint64_t>(kAttendRows, 0xffffffffu / (line.pairs * most_units(a)));
+  for (uint32_t r = 0; r < a.rows; r += most) {
     AttendArgs c = a;
-    c.rows = std::min<uint32_t>(kAttendRows, a.rows - r);
+    c.rows = std::min(most, a.rows - r);
     c.q += r * a.q_row;
     c.out += r * a.out_row;
     c.tables += r * a.table_stride;
     c.lengths += r;
     if (a.lse) c.lse += (uint64_t)r * a.queries * a.q_heads;
-    if (rows_bf16) launch_rows<true>(c, s);
-    else launch_rows<false>(c, s);
+    with_kernel(a.cache.dim, a.cache.k_scales != nullptr, rows_bf16, [&](auto ds, auto f8, auto bf16) {
+      launch_pass<decltype(ds)::value, decltype(f8)::value, decltype(bf16)::value>(c, line, s);
+      return 0;
+    });
   }
 }
 

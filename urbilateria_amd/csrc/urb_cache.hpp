@@ -78,7 +78,7 @@ struct AttendArgs {
   float* parts;  // attend_work_bytes
   int* status;
 };
-size_t attend_work_bytes(uint32_t dim);
+size_t attend_work_bytes(uint32_t dim, bool f8, bool rows_bf16);
 void launch_attend(const AttendArgs& a, bool rows_bf16, hipStream_t s);
 
 }  // namespace urb

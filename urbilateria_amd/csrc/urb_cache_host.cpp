@@ -276,14 +276,16 @@ urb_status urb_attention_create(const urb_attention_desc* d, urb_attention** out
   if (!row_type(d->dtype) || !cache_type(d->cache_dtype)) return URB_ERR_ARGUMENT;
   if (!geometry(d->heads, d->page_size, d->head_dim) || d->q_heads == 0 || d->q_heads > 8192 ||
       d->q_heads % d->heads || d->queries == 0 || d->queries > 16 || d->max_rows == 0 ||
-      d->max_rows > (1u << 20) || d->max_length == 0 || d->max_length > (1u << 27))
+      d->max_rows > (1u << 20) || d->max_length == 0 || d->max_length > (1u << 24))
     return URB_ERR_SHAPE;
   if (!finite_host(d->scale) || !(d->scale > 0.0f)) return URB_ERR_INVALID_GEOMETRY;
   urb_attention* c = new (std::nothrow) urb_attention();
   if (!c) return URB_ERR_OUT_OF_MEMORY;
   c->desc = *d;
   if (const urb_status st =
-          make_work(urb::attend_work_bytes(d->head_dim), &c->work, &c->device, &c->status)) {
+          make_work(urb::attend_work_bytes(d->head_dim, d->cache_dtype == URB_DTYPE_F8_E4M3,
+                                           d->dtype == URB_DTYPE_BF16),
+                    &c->work, &c->device, &c->status)) {
     (void)hipGetLastError();
     if (c->work) (void)hipFree(c->work);
     delete c;
