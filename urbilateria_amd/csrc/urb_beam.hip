@@ -12,25 +12,6 @@
 
 namespace urb {
 
-namespace {
-
-typedef unsigned long long u64;
-
-constexpr int kThreads = 256;
-constexpr int kJoinThreads = 1024;
-
-// Order-preserving key of a logit: NaN and -inf, which are never picked, 0; -0 as +0.
-__device__ __forceinline__ uint32_t key_of(float l) {
-  if (!(l > -__builtin_inff())) return 0;
-  const uint32_t b = f2u(l + 0.0f);
-  return b ^ ((b >> 31) ? 0xffffffffu : 0x80000000u);
-}
-__device__ __forceinline__ float key_value(uint32_t k) {
-  return u2f(k ^ ((k >> 31) ? 0x80000000u : 0xffffffffu));
-}
-
-}  // namespace
-
 struct BeamSum {
   double z;  // of exp(l - m)
   float m;
@@ -38,6 +19,25 @@ struct BeamSum {
 };
 
 namespace {
+
+typedef unsigned long long u64;
+
+constexpr int kThreads = 256;
+constexpr float kInf = __builtin_inff();
+
+// Order-preserving key of a logit: NaN and -inf, which are never picked, 0; -0 as +0.
+__device__ __forceinline__ uint32_t key_of(float l) {
+  if (!(l > -kInf)) return 0;
+  const uint32_t b = f2u(l + 0.0f);
+  return b ^ ((b >> 31) ? 0xffffffffu : 0x80000000u);
+}
+__device__ __forceinline__ float key_value(uint32_t k) {
+  return u2f(k ^ ((k >> 31) ? 0x80000000u : 0xffffffffu));
+}
+// A logit's key and its index: the larger logit, then the lower index.
+__device__ __forceinline__ u64 with_index(uint32_t key, int at) {
+  return (u64)key << 32 | (uint32_t)~at;
+}
 
 // Four neighbours of a row from i on; those past the end are -inf.
 template <bool BF16>
@@ -54,7 +54,7 @@ __device__ __forceinline__ void load4(float (&v)[4], const uint8_t* row, int i, 
   }
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    v[j] = -__builtin_inff();
+    v[j] = -kInf;
     if (i + j < vocab) {
       if constexpr (BF16) v[j] = u2f((uint32_t)reinterpret_cast<const uint16_t*>(row)[i + j] << 16);
       else v[j] = reinterpret_cast<const float*>(row)[i + j];
@@ -62,80 +62,132 @@ __device__ __forceinline__ void load4(float (&v)[4], const uint8_t* row, int i, 
   }
 }
 
-// exp(l - m) for l <= m, 1 where both are +inf.
-__device__ __forceinline__ double mass(float l, float m) {
-  if (l == m) return 1.0;
-  if (!(l > -__builtin_inff())) return 0.0;
-  return exp((double)l - (double)m);
+// exp(l - m) for l <= m finite: l - m = n ln 2 / 64 + r with |r| <= ln(2) / 128, 2^(n / 64) by a table in LDS
+// and the Taylor series to r^4, which leaves out 4e-14 of it.  Logits far below, of -inf and NaN count as
+// exp(-60): all the vocabulary's together are no 2^-50 of the largest's 1.
+constexpr int kPowers = 64;
+__device__ __forceinline__ void fill_powers(double* powers) {
+  if (threadIdx.x < kPowers) powers[threadIdx.x] = exp2((double)threadIdx.x / kPowers);
+}
+__device__ __forceinline__ double mass(float l, double m, const double* powers) {
+  const double x = fmax((double)l - m, -60.0);
+  const double magic = 0x1.8p52;  // adding it leaves an integer in the low bits
+  const double t = fma(x, 0x1.71547652b82fep+6, magic);  // 64 / ln 2
+  const int n = (int)__double_as_longlong(t);
+  const double r = fma(magic - t, 0x1.62e42fefa39efp-7, x);
+  double s = fma(1.0 / 24.0, r, 1.0 / 6.0);
+  s = fma(s, r, 0.5);
+  s = fma(s, r, 1.0);
+  // the table's value times 2^(n / 64): a sum in its exponent
+  const long long p = __double_as_longlong(powers[n & (kPowers - 1)]) + ((long long)(n >> 6) << 52);
+  const double q = __longlong_as_double(p);
+  return fma(s * r, q, q);
 }
 
-// A workgroup per slice and beam.
-template <bool BF16>
+// The upper half of the n-th largest key of a wave's lanes; 0 where fewer lanes have one.
+__device__ __forceinline__ uint32_t wave_nth(uint32_t key, int n) {
+  uint32_t t = 0;
+#pragma unroll
+  for (uint32_t bit = 1u << 31; bit > 0xffffu; bit >>= 1)
+    if (__popcll(__ballot(key >= (t | bit))) >= n) t |= bit;
+  return t;
+}
+
+// A workgroup per slice (of PER logits per thread) and beam.
+template <bool BF16, int PER>
 __global__ __launch_bounds__(kThreads) void beam_slice_kernel(BeamArgs a) {
-  constexpr int PER = kBeamSlice / kThreads;
-  __shared__ u64 best[kThreads];
-  __shared__ u64 list[kBeamPicks * PER];
-  __shared__ double s_z[kThreads / 64];
-  __shared__ u64 s_key[kThreads / 64];
-  __shared__ int n_list;
+  constexpr int WAVES = kThreads / 64;
+  __shared__ double powers[kPowers];
+  __shared__ u64 list[kBeamPicks * PER > kThreads ? kBeamPicks * PER : kThreads];
+  __shared__ double s_z[WAVES];
+  __shared__ float s_top[WAVES];
+  __shared__ uint32_t s_nth[WAVES];
+  __shared__ int n_heads, n_list;
   __shared__ u64 s_least;
-  const int slice = blockIdx.x, beam = blockIdx.y, tid = threadIdx.x;
+  const int slice = blockIdx.x, beam = blockIdx.y, tid = threadIdx.x, wave = tid >> 6;
   if (a.ended && a.ended[beam]) return;  // its logits count for nothing
   const uint8_t* row = reinterpret_cast<const uint8_t*>(a.logits) + beam * a.row_stride * (BF16 ? 2 : 4);
   const bool wide = reinterpret_cast<uintptr_t>(row) % (BF16 ? 8 : 16) == 0;
-  const int base = slice * kBeamSlice + 4 * tid;
+  const int base = slice * (PER * kThreads) + 4 * tid;
+  auto index = [&](int k, int j) { return base + k * 4 * kThreads + j; };
   float v[PER / 4][4];
 #pragma unroll
-  for (int k = 0; k < PER / 4; ++k) load4<BF16>(v[k], row, base + k * 4 * kThreads, a.vocab, wide);
-  // keys: the larger logit, then the lower index
-  u64 top = 0;
+  for (int k = 0; k < PER / 4; ++k) load4<BF16>(v[k], row, index(k, 0), a.vocab, wide);
+  fill_powers(powers);
+  if (tid == 0) {
+    n_heads = n_list = 0;
+    s_least = 0;
+  }
+  // the largest of the thread (fmaxf passes NaNs over) and of the slice
+  float top = -kInf;
 #pragma unroll
   for (int k = 0; k < PER / 4; ++k)
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const uint32_t key = key_of(v[k][j]);
-      const uint32_t at = (uint32_t)(base + k * 4 * kThreads + j);
-      const u64 both = (u64)key << 32 | (uint32_t)~at;
-      if (key && both > top) top = both;
-    }
-  best[tid] = top;
-  u64 most = top;
-  for (int o = 32; o > 0; o >>= 1) most = max(most, (u64)__shfl_xor((long long)most, o, 64));
-  if ((tid & 63) == 0) s_key[tid >> 6] = most;
-  if (tid == 0) {
-    n_list = 0;
-    s_least = 0;
+    for (int j = 0; j < 4; ++j) top = fmaxf(top, v[k][j]);
+  const uint32_t key = key_of(top);
+  float m = top;
+  for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+  const uint32_t nth = wave_nth(key, a.picks);
+  if ((tid & 63) == 0) {
+    s_top[wave] = m;
+    s_nth[wave] = nth;
   }
   __syncthreads();
+  // A wave that has so many bests gives a bound; among the few bests that reach the highest one, the
+  // picks-th itself is found by counting.
+  uint32_t bound = 0;
 #pragma unroll
-  for (int w = 0; w < kThreads / 64; ++w) most = max(most, s_key[w]);
-  const bool any = most != 0;
-  const float m = any ? key_value((uint32_t)(most >> 32)) : -__builtin_inff();
+  for (int w = 0; w < WAVES; ++w) {
+    m = fmaxf(m, s_top[w]);
+    bound = max(bound, s_nth[w]);
+  }
+  const bool head = key && key >= bound;
+  u64 best = 0;  // the thread's, if it is among them: the first of equal ones
+  if (head) {
+    int at = 0;
+#pragma unroll
+    for (int k = PER / 4; k-- > 0;)
+#pragma unroll
+      for (int j = 4; j-- > 0;)
+        if (v[k][j] == top) at = index(k, j);
+    best = with_index(key, at);
+    list[atomicAdd(&n_heads, 1)] = best;
+  }
   double z = 0.0;
-  if (any)
+  if (m == kInf) {  // as many as there are of it share all
 #pragma unroll
     for (int k = 0; k < PER / 4; ++k)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) z += mass(v[k][j], m);
+      for (int j = 0; j < 4; ++j) z += v[k][j] == kInf ? 1.0 : 0.0;
+  } else if (m > -kInf) {
+    const double md = (double)m;
+#pragma unroll
+    for (int k = 0; k < PER / 4; ++k)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) z += mass(v[k][j], md, powers);
+  }
   for (int o = 32; o > 0; o >>= 1) z += __shfl_xor(z, o, 64);
-  if ((tid & 63) == 0) s_z[tid >> 6] = z;
-  // the picks-th largest of the threads' best
-  if (top) {
+  if ((tid & 63) == 0) s_z[wave] = z;
+  __syncthreads();
+  if (head) {
+    const int n = n_heads;
     int above = 0;
-    for (int i = 0; i < kThreads; ++i) above += best[i] > top;
-    if (above == a.picks - 1) s_least = top;
+    for (int i = 0; i < n; ++i) above += list[i] > best;
+    if (above == a.picks - 1) s_least = best;
   }
   __syncthreads();
   const u64 least = s_least;  // 0: fewer threads than that have any
+  const float least_value = least ? key_value((uint32_t)(least >> 32)) : -kInf;
+  if (head && best >= least)  // (others have nothing that does)
 #pragma unroll
-  for (int k = 0; k < PER / 4; ++k)
+    for (int k = 0; k < PER / 4; ++k)
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const uint32_t key = key_of(v[k][j]);
-      const uint32_t at = (uint32_t)(base + k * 4 * kThreads + j);
-      const u64 both = (u64)key << 32 | (uint32_t)~at;
-      if (key && both >= least) list[atomicAdd(&n_list, 1)] = both;
-    }
+      for (int j = 0; j < 4; ++j)
+        if (v[k][j] >= least_value) {
+          const uint32_t one = key_of(v[k][j]);
+          const u64 both = with_index(one, index(k, j));
+          if (one && both >= least) list[atomicAdd(&n_list, 1)] = both;
+        }
   __syncthreads();
   const int n = n_list;
   u64* out = a.keys + ((size_t)beam * a.slices + slice) * a.picks;
@@ -148,7 +200,7 @@ __global__ __launch_bounds__(kThreads) void beam_slice_kernel(BeamArgs a) {
   for (int i = n + tid; i < a.picks; i += kThreads) out[i] = 0;
   if (tid == 0) {
     double sum = 0.0;
-    for (int w = 0; w < kThreads / 64; ++w) sum += s_z[w];
+    for (int w = 0; w < WAVES; ++w) sum += s_z[w];
     a.sums[(size_t)beam * a.slices + slice] = BeamSum{sum, m, 0};
   }
 }
@@ -157,88 +209,104 @@ struct Candidate {
   double score;
   uint32_t at;  // beam * vocab + token
 };
+constexpr uint32_t kNone = 0xffffffffu;
 __device__ __forceinline__ bool better(const Candidate& x, const Candidate& y) {
   return x.score > y.score || (x.score == y.score && x.at < y.at);
 }
 
-// A workgroup per request; a thread per slice of a beam, whose candidates are in order.
-__global__ __launch_bounds__(kJoinThreads) void beam_join_kernel(BeamArgs a) {
-  __shared__ Candidate head[kJoinThreads];
+// A workgroup per request; each slice of each of its beams is a list in order.  `span` lists (a power of two)
+// are counted for a beam, `team` threads go through a list.
+template <int THREADS>
+__global__ __launch_bounds__(THREADS) void beam_join_kernel(BeamArgs a, int span, int team) {
+  constexpr int WAVES = THREADS / 64, EARLY = 8;
+  __shared__ double powers[kPowers];
   __shared__ Candidate list[kBeamPicks * kBeamPicks];
-  __shared__ double s_base[kBeamWidth];  // score and logarithm of a beam: what a logit - m is added to
-  __shared__ float s_top[kBeamWidth];
-  __shared__ int s_live[kBeamWidth];     // 0: no candidates, 1: its slices', 2: ended
-  __shared__ int n_list, s_bad;
+  __shared__ int s_live[kBeamWidth];  // 0: no candidates, 1: its slices', 2: ended
+  __shared__ uint32_t s_nth[WAVES];
+  __shared__ int n_heads, n_list, s_bad;
   __shared__ Candidate s_least;
-  const int r = blockIdx.x, tid = threadIdx.x, width = a.width;
+  static_assert(kBeamPicks * kBeamPicks >= THREADS, "a place for every list's first");
+  const int r = blockIdx.x, tid = threadIdx.x;
+  const int b = tid / (span * team), slice = tid / team & (span - 1), place = tid & (team - 1);
+  const bool mine = b < a.width && slice < a.slices;
+  const int beam = r * a.width + (mine ? b : 0);
+  const size_t at = (size_t)beam * a.slices + (mine ? slice : 0);
+  const u64* keys = a.keys + at * a.picks;
+  // (all that is read is read at once: of a beam that has ended, keys and sum are what was there)
+  u64 early[EARLY];
+#pragma unroll
+  for (int i = 0; i < EARLY; ++i) early[i] = mine && place + i * team < a.picks ? keys[place + i * team] : 0;
+  const BeamSum sum = a.sums[at];
+  const float score = a.scores[beam];
+  const bool end = a.ended && a.ended[beam];
+  fill_powers(powers);
   if (tid == 0) {
-    n_list = 0;
-    s_bad = 0;
-    s_least = Candidate{-__builtin_inf(), 0xffffffffu};
+    n_heads = n_list = s_bad = 0;
+    s_least = Candidate{-__builtin_inf(), kNone};
   }
   __syncthreads();
-  // (a wave per beam in turn)
-  for (int b = tid >> 6; b < width; b += kJoinThreads / 64) {
-    const int lane = tid & 63, beam = r * width + b;
-    const float c = a.scores[beam];
-    const bool end = a.ended && a.ended[beam];
-    float m = -__builtin_inff();
-    double z = 0.0;
-    if (!end) {
-      const BeamSum* sums = a.sums + (size_t)beam * a.slices;
-      const BeamSum mine = lane < a.slices ? sums[lane] : BeamSum{0.0, -__builtin_inff(), 0};
-      m = mine.m;
-      for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
-      z = mine.z * mass(mine.m, m);
-      for (int o = 32; o > 0; o >>= 1) z += __shfl_xor(z, o, 64);
-    }
-    if (lane == 0) {
-      const bool bad = !(c <= 3.4028235e38f);  // NaN, +inf
-      if (bad) s_bad = 1;
-      const bool live = !bad && c > -__builtin_inff();
-      s_live[b] = !live ? 0 : end ? 2 : m > -__builtin_inff() ? 1 : 0;
-      s_top[b] = m;
-      s_base[b] = end ? (double)c : (double)c - log(z);
-    }
+  float m = mine && !end ? sum.m : -kInf;
+  const float own = m;
+  for (int o = span * team / 2; o >= team; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+  double z = 0.0;
+  if (m == kInf) z = own == kInf ? sum.z : 0.0;
+  else if (own > -kInf) z = sum.z * mass(own, (double)m, powers);
+  for (int o = span * team / 2; o >= team; o >>= 1) z += __shfl_xor(z, o, 64);
+  const bool bad = !(score <= 3.4028235e38f);  // NaN, +inf
+  const int live = bad || !(score > -kInf) ? 0 : end ? 2 : m > -kInf ? 1 : 0;
+  // what a logit - m is added to
+  const double base = end ? (double)score : (double)score - log(z);
+  if (mine && slice == 0 && place == 0) {
+    s_live[b] = live;
+    if (bad) s_bad = 1;
   }
-  __syncthreads();
-  // this thread's list
-  const int b = tid / a.slices, slice = tid - b * a.slices;
-  const bool mine = b < width && (s_live[b] == 1 || (s_live[b] == 2 && slice == 0));
-  const u64* keys = a.keys + ((size_t)(r * width + b) * a.slices + slice) * a.picks;
-  auto candidate = [&](int i) -> Candidate {
-    const Candidate none{-__builtin_inf(), 0xffffffffu};
-    if (s_live[b] == 2)
-      return i == 0 ? Candidate{s_base[b], (uint32_t)b * a.vocab + a.end_token} : none;
-    const u64 key = keys[i];
-    if (!key) return none;
-    const float l = key_value((uint32_t)(key >> 32));
-    const double gap = l == s_top[b] ? 0.0 : (double)l - (double)s_top[b];
-    const double score = s_base[b] + gap;
-    return score > -__builtin_inf() ? Candidate{score, (uint32_t)b * a.vocab + ~(uint32_t)key} : none;
+  // candidate i of this list
+  auto candidate = [&](int i, u64 key) -> Candidate {
+    const Candidate none{-__builtin_inf(), kNone};
+    if (live == 2) return slice == 0 && i == 0 ? Candidate{base, (uint32_t)b * a.vocab + a.end_token} : none;
+    if (live == 0 || !key) return none;
+    const float v = key_value((uint32_t)(key >> 32));
+    const double c = base + (v == m ? 0.0 : (double)v - (double)m);
+    return c > -__builtin_inf() ? Candidate{c, (uint32_t)b * a.vocab + ~(uint32_t)key} : none;
   };
-  Candidate first{-__builtin_inf(), 0xffffffffu};
-  if (mine) first = candidate(0);
-  head[tid] = first;
+  // the picks-th of the lists' first ones, as in the slices (a score's f32 keeps the order)
+  Candidate first{-__builtin_inf(), kNone};
+  if (mine && place == 0) first = candidate(0, early[0]);
+  const uint32_t key = first.at == kNone ? 0 : key_of(fmaxf((float)first.score, -3.4028235e38f));
+  const uint32_t nth = wave_nth(key, a.picks);
+  if ((tid & 63) == 0) s_nth[tid >> 6] = nth;
   __syncthreads();
-  const int lists = width * a.slices;
-  if (first.at != 0xffffffffu) {
+  uint32_t bound = 0;
+#pragma unroll
+  for (int w = 0; w < WAVES; ++w) bound = max(bound, s_nth[w]);
+  const bool head = key && key >= bound;
+  if (head) list[atomicAdd(&n_heads, 1)] = first;
+  __syncthreads();
+  if (head) {
+    const int n = n_heads;
     int above = 0;
-    for (int i = 0; i < lists; ++i) above += better(head[i], first);
+    for (int i = 0; i < n; ++i) above += better(list[i], first);
     if (above == a.picks - 1) s_least = first;
   }
   __syncthreads();
   const Candidate least = s_least;
-  if (first.at != 0xffffffffu)
-    for (int i = 0; i < a.picks; ++i) {
-      const Candidate c = i ? candidate(i) : first;
-      if (c.at == 0xffffffffu || better(least, c)) break;
-      list[atomicAdd(&n_list, 1)] = c;
-    }
+  // (lists are in order: behind one that falls short there is nothing)
+  auto take = [&](int i, u64 k) {
+    const Candidate c = candidate(i, k);
+    const bool in = c.at != kNone && !better(least, c);
+    if (in) list[atomicAdd(&n_list, 1)] = c;
+    return in;
+  };
+  if (mine) {
+    bool more = true;
+#pragma unroll
+    for (int i = 0; i < EARLY; ++i) more = more && place + i * team < a.picks && take(place + i * team, early[i]);
+    for (int i = place + EARLY * team; more && i < a.picks; i += team) more = take(i, keys[i]);
+  }
   __syncthreads();
   const int n = n_list;
   const size_t out = (size_t)r * a.picks;
-  for (int i = tid; i < n; i += kJoinThreads) {
+  for (int i = tid; i < n; i += THREADS) {
     const Candidate c = list[i];
     int above = 0;
     for (int j = 0; j < n; ++j) above += better(list[j], c);
@@ -251,8 +319,8 @@ __global__ __launch_bounds__(kJoinThreads) void beam_join_kernel(BeamArgs a) {
       if (a.ended_out) a.ended_out[out + above] = s_live[parent] == 2 || token == a.end_token;
     }
   }
-  for (int i = n + tid; i < a.picks; i += kJoinThreads) {
-    a.scores_out[out + i] = -__builtin_inff();
+  for (int i = n + tid; i < a.picks; i += THREADS) {
+    a.scores_out[out + i] = -kInf;
     a.tokens[out + i] = -1;
     a.parents[out + i] = -1;
     if (a.ended_out) a.ended_out[out + i] = 1;
@@ -260,22 +328,38 @@ __global__ __launch_bounds__(kJoinThreads) void beam_join_kernel(BeamArgs a) {
   if (tid == 0 && s_bad) flag(a.status, kStepArgument);
 }
 
-size_t keys_bytes(int vocab, int width, int picks, int requests) {
-  return (size_t)requests * width * beam_slices(vocab) * picks * sizeof(u64);
+int slices_of(int vocab, int slice) { return (vocab + slice - 1) / slice; }
+
+// Lists that the join counts for a beam: a power of two, for shuffles.
+int span_of(int slices) {
+  int span = 1;
+  while (span < slices) span *= 2;
+  return span;
 }
+
+// Short slices while they are no more workgroups than the chip has at a time (and a request's fit the join, a
+// beam's a wave of it): 4 beams over 50257 BF16 logits take @@ us with them and @@ without, 256 over 129280 f32
+// logits would take @@ and take @@.
+bool short_slices(int vocab, int width, int requests) {
+  const int64_t slices = slices_of(vocab, kBeamShortSlice);
+  return slices <= 64 && span_of((int)slices) * width <= 1024 && slices * width * requests <= 1024;
+}
+
+size_t lists_bytes(size_t lists, int picks) { return lists * (picks * sizeof(u64) + sizeof(BeamSum)); }
 
 }  // namespace
 
 size_t beam_work_bytes(int vocab, int width, int picks, int requests) {
-  return keys_bytes(vocab, width, picks, requests) +
-         (size_t)requests * width * beam_slices(vocab) * sizeof(BeamSum);
+  // (short slices of few requests may be more than long ones of all)
+  const size_t many = (size_t)requests * width * slices_of(vocab, kBeamSlice);
+  return lists_bytes(std::max<size_t>(many, 1024), picks);
 }
 
-void launch_beam(BeamArgs a, bool bf16, int max_requests, void* work, hipStream_t s) {
-  a.slices = beam_slices(a.vocab);
-  a.keys = static_cast<u64*>(work);
-  a.sums = reinterpret_cast<BeamSum*>(static_cast<char*>(work) +
-                                      keys_bytes(a.vocab, a.width, a.picks, max_requests));
+void launch_beam(BeamArgs a, bool bf16, void* work, hipStream_t s) {
+  const bool brief = short_slices(a.vocab, a.width, a.requests);
+  a.slices = slices_of(a.vocab, brief ? kBeamShortSlice : kBeamSlice);
+  a.sums = static_cast<BeamSum*>(work);
+  a.keys = reinterpret_cast<u64*>(a.sums + (size_t)a.requests * a.width * a.slices);
   // requests of a launch: blockIdx.y is below 2^16
   const int most = 65535 / a.width;
   for (int r = 0; r < a.requests; r += most) {
@@ -292,9 +376,17 @@ void launch_beam(BeamArgs a, bool bf16, int max_requests, void* work, hipStream_
     c.keys += beams * a.slices * a.picks;
     c.sums += beams * a.slices;
     const dim3 grid(a.slices, c.requests * a.width);
-    if (bf16) beam_slice_kernel<true><<<grid, kThreads, 0, s>>>(c);
-    else beam_slice_kernel<false><<<grid, kThreads, 0, s>>>(c);
-    beam_join_kernel<<<c.requests, kJoinThreads, 0, s>>>(c);
+    constexpr int LONG = kBeamSlice / kThreads, SHORT = kBeamShortSlice / kThreads;
+    if (bf16 && brief) beam_slice_kernel<true, SHORT><<<grid, kThreads, 0, s>>>(c);
+    else if (bf16) beam_slice_kernel<true, LONG><<<grid, kThreads, 0, s>>>(c);
+    else if (brief) beam_slice_kernel<false, SHORT><<<grid, kThreads, 0, s>>>(c);
+    else beam_slice_kernel<false, LONG><<<grid, kThreads, 0, s>>>(c);
+    // a thread for every list, or several where 256 suffice; a beam's are in one wave
+    const int span = span_of(a.slices), lists = span * a.width;
+    int team = 1;
+    while (2 * team * lists <= 256 && 2 * team * span <= 64) team *= 2;
+    if (lists <= 256) beam_join_kernel<256><<<c.requests, 256, 0, s>>>(c, span, team);
+    else beam_join_kernel<1024><<<c.requests, 1024, 0, s>>>(c, span, team);
   }
 }
 

@@ -53,8 +53,7 @@ void launch_sample(const SampleArgs& a, bool bf16, hipStream_t s);
 
 // ---- beam search's selection (urb_beam.hip) ----
 constexpr int kBeamWidth = 32, kBeamPicks = 64, kBeamVocab = 1 << 18;
-constexpr int kBeamSlice = 8192;  // logits of a workgroup
-inline int beam_slices(int vocab) { return (vocab + kBeamSlice - 1) / kBeamSlice; }
+constexpr int kBeamSlice = 8192, kBeamShortSlice = 2048;  // logits of a workgroup
 static_assert(kBeamWidth * (kBeamVocab / kBeamSlice) <= 1024, "a thread for every slice of a request");
 struct BeamSum;
 struct BeamArgs {
@@ -72,7 +71,7 @@ struct BeamArgs {
   BeamSum* sums;
 };
 size_t beam_work_bytes(int vocab, int width, int picks, int requests);
-void launch_beam(BeamArgs a, bool bf16, int max_requests, void* work, hipStream_t s);
+void launch_beam(BeamArgs a, bool bf16, void* work, hipStream_t s);
 
 // ---- projections with adapters (urb_project.hip) ----
 // Ranks are kept in units of 8 in B and in 16-rank panels in A.

@@ -458,8 +458,8 @@ urb_status urb_beams_select(urb_beams* c, const urb_beams_call* p, void* stream)
   a.parents = p->parents;
   a.ended_out = p->ended_out;
   a.status = c->status;
-  urb::launch_beam(a, d.dtype == URB_DTYPE_BF16, (int)d.max_requests,
-                   static_cast<char*>(c->work) + kAlign, static_cast<hipStream_t>(stream));
+  urb::launch_beam(a, d.dtype == URB_DTYPE_BF16, static_cast<char*>(c->work) + kAlign,
+                   static_cast<hipStream_t>(stream));
   URB_HIP(hipGetLastError());
   return URB_OK;
 }
