@@ -46,7 +46,10 @@ struct PlanArgs {
 void launch_plan(const PlanArgs& a, hipStream_t s);
 
 constexpr int kForkCaches = 16;  // of a launch
-constexpr int kForkWidth = 64;
+constexpr int kForkWidth = 64, kForkRequests = 4096;
+struct ForkCopy {
+  uint32_t from, to, tokens;  // pages; 0 tokens: nothing
+};
 struct ForkArgs {
   uint32_t requests, width, page, pages, max_blocks;
   uint64_t table_stride, table_out_stride;
@@ -58,6 +61,7 @@ struct ForkArgs {
   // workspace: lengths before [max_rows]; pages dropped and copies needed by each request; the dropped
   // pages of request r from r * width * max_blocks on; the free pages before
   int32_t *old_lengths, *drops, *copies, *dropped, *count;
+  ForkCopy* page_copies;  // of each row
   int* status;
 };
 void launch_fork(const ForkArgs& a, const KvCache* caches, uint32_t n_caches, hipStream_t s);

@@ -13,9 +13,10 @@ struct urb_pager {
   int device = 0;
   void* work = nullptr;
   int* status = nullptr;
-  // plans: [max_rows + 1] each; forks: [max_rows], [kMostRequests] twice, [1], [max_rows * max_blocks]
+  // plans: [max_rows + 1] each; forks: [max_rows], [kForkRequests] twice, [1], [max_rows * max_blocks]
   int32_t *row_have = nullptr, *row_start = nullptr, *row_top = nullptr;
   int32_t *old_lengths = nullptr, *drops = nullptr, *copies = nullptr, *count = nullptr, *dropped = nullptr;
+  urb::ForkCopy* page_copies = nullptr;  // [max_rows]
 };
 
 struct urb_attention {
@@ -27,8 +28,6 @@ struct urb_attention {
 };
 
 namespace {
-
-constexpr uint32_t kMostRequests = 4096;  // of a fork
 
 bool cache_type(urb_dtype t) { return t == URB_DTYPE_BF16 || t == URB_DTYPE_F8_E4M3; }
 
@@ -146,7 +145,7 @@ urb_status urb_pager_create(const urb_pager_desc* d, urb_pager** out) {
   if (!c) return URB_ERR_OUT_OF_MEMORY;
   c->desc = *d;
   const size_t rows = d->max_rows, table = rows * d->max_blocks;
-  const size_t requests = std::min<size_t>(kMostRequests, rows);
+  const size_t requests = std::min<size_t>(urb::kForkRequests, rows);
   char* p = nullptr;  // (offsets first, addresses when the memory is there)
   auto lay = [&]() {
     c->row_have = carve<int32_t>(p, rows + 1);
@@ -157,6 +156,7 @@ urb_status urb_pager_create(const urb_pager_desc* d, urb_pager** out) {
     c->copies = carve<int32_t>(p, requests);
     c->count = carve<int32_t>(p, 1);
     c->dropped = carve<int32_t>(p, table);
+    c->page_copies = carve<urb::ForkCopy>(p, rows);
   };
   lay();
   if (const urb_status st = make_work(reinterpret_cast<size_t>(p), &c->work, &c->device, &c->status)) {
@@ -216,7 +216,7 @@ urb_status urb_pager_fork(urb_pager* c, const urb_page_fork* f, void* stream) {
       f->tables == f->tables_out || (f->n_caches && !f->caches))
     return URB_ERR_ARGUMENT;
   const urb_pager_desc& d = c->desc;
-  if (f->requests == 0 || f->requests > kMostRequests || f->width == 0 || f->width > urb::kForkWidth ||
+  if (f->requests == 0 || f->requests > urb::kForkRequests || f->width == 0 || f->width > urb::kForkWidth ||
       (uint64_t)f->requests * f->width > d.max_rows || f->table_stride < d.max_blocks ||
       f->table_out_stride < d.max_blocks || f->n_caches > 4096)
     return URB_ERR_SHAPE;
@@ -251,6 +251,7 @@ urb_status urb_pager_fork(urb_pager* c, const urb_page_fork* f, void* stream) {
     a.drops = c->drops;
     a.copies = c->copies;
     a.dropped = c->dropped;
+    a.page_copies = c->page_copies;
     a.count = c->count;
     a.status = c->status;
     urb::launch_fork(a, caches, f->n_caches, static_cast<hipStream_t>(stream));

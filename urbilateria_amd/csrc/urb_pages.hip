@@ -274,19 +274,92 @@ __device__ __forceinline__ uint32_t blocks_of(int length, uint32_t page) {
   return (uint32_t)(length + page - 1) / page;
 }
 
-// Whether row i of a request takes a copy of its parent's last page: one that is filled in part and stays
-// with a lower child.
-__device__ __forceinline__ bool takes_copy(const int* parent, const int* length, int i, uint32_t page) {
-  const int p = parent[i];
-  if (p < 0 || length[p] % page == 0) return false;
-  for (int j = 0; j < i; ++j)
-    if (parent[j] == p) return true;
-  return false;
+// The rows of a request that take a copy of their parent's last page, one filled in part that stays with a
+// lower child; a whole wave, one row per lane.
+__device__ __forceinline__ uint64_t copying_rows(const int* parent, const int* length, int width,
+                                                 uint32_t page) {
+  const int i = threadIdx.x & 63;
+  const int p = i < width ? parent[i] : -1;
+  bool lower = false;
+  for (int j = 0; j < width; ++j) lower |= j < i && parent[j] == p;
+  return __ballot(p >= 0 && lower && length[p < 0 ? 0 : p] % page != 0);
+}
+
+// The pages, lengths and stack of a request's rows, when all requests' dropped pages and copies are known:
+// dropped ones go on the stack, copies take theirs off it.  What a page on top is, when it is one that a
+// request has just dropped, is looked up in that request's list and not on the stack, which another workgroup
+// may not have written yet.
+__device__ __forceinline__ void fork_books(const ForkArgs& a, const int* parent, const int* length,
+                                           int64_t* slots, int* s_upto) {
+  const uint32_t r = blockIdx.x, row0 = r * a.width;
+  const int tid = threadIdx.x, width = (int)a.width;
+  // pages dropped by requests 0 .. q, and copies before this request and in all (fewer than 2^20)
+  int dropped = 0;
+  int64_t copies = 0, all;
+  for (uint32_t q0 = 0; q0 < a.requests; q0 += 256) {
+    const uint32_t q = q0 + tid;
+    const int d = q < a.requests ? a.drops[q] : 0;
+    const int64_t c = q < a.requests ? a.copies[q] : 0;
+    copies += c << 32 | (q < r ? c : 0);
+    const int upto = dropped + (int)before<256>(d, slots, &all) + d;
+    if (q < a.requests) s_upto[q] = upto;
+    dropped += (int)all;
+  }
+  (void)before<256>(copies, slots, &all);
+  const int copies_before = (int)(all & 0xffffffff), copies_all = (int)(all >> 32);
+  const int count = *a.count;
+  const int64_t room = (int64_t)a.pages - count;  // of the stack
+  const int64_t size = count + min((int64_t)dropped, room);
+  const int32_t* list = a.dropped + (uint64_t)row0 * a.max_blocks;
+  const int before_r = r ? s_upto[r - 1] : 0, n = s_upto[r] - before_r;
+  const int64_t first = (int64_t)count + before_r;
+  for (int j = tid; j < n; j += 256)
+    if (first + j < a.pages) a.free_pages[first + j] = list[j];
+  if (r == 0 && tid == 0) {
+    *a.free_count_out = (int)max(size - copies_all, (int64_t)0);
+    if (dropped > room) flag(a.status, kCacheArgument);
+  }
+  if (tid >= 64) return;
+  const uint64_t copying = copying_rows(parent, length, width, a.page);
+  if (tid >= width) return;
+  const int p = parent[tid];
+  int kept = p >= 0 ? length[p] : 0;
+  ForkCopy copy{0, 0, 0};
+  if (copying >> tid & 1) {
+    const int64_t at = size - 1 - copies_before - __popcll(copying & ((1ull << tid) - 1));
+    if (at < 0) {
+      kept = 0;
+      flag(a.status, kCacheMemory);
+    } else {
+      int to;
+      if (at < count) {
+        to = a.free_pages[at];
+      } else {
+        const int want = (int)(at - count);
+        uint32_t q = 0, end = a.requests - 1;  // the first request whose dropped pages end beyond
+        while (q < end) {
+          const uint32_t mid = (q + end) / 2;
+          if (s_upto[mid] > want) end = mid;
+          else q = mid + 1;
+        }
+        to = a.dropped[(uint64_t)q * a.width * a.max_blocks + (want - (q ? s_upto[q - 1] : 0))];
+      }
+      const uint32_t last = (uint32_t)length[p] / a.page;
+      const int from = a.tables[(uint64_t)(row0 + p) * a.table_stride + last];
+      a.tables_out[(uint64_t)(row0 + tid) * a.table_out_stride + last] = to;
+      if ((uint32_t)to >= a.pages || (uint32_t)from >= a.pages) flag(a.status, kCacheArgument);
+      else copy = ForkCopy{(uint32_t)from, (uint32_t)to, (uint32_t)length[p] % a.page};
+    }
+  }
+  a.page_copies[row0 + tid] = copy;
+  a.lengths_out[row0 + tid] = kept;
 }
 
 // One request per workgroup: its rows' tables, and the pages that none of them holds any more.  A page can
 // stand in several rows only in one column, so a column is one thread's work.
+template <bool ALONE>
 __global__ __launch_bounds__(256) void fork_tables_kernel(ForkArgs a) {
+  extern __shared__ int column[];  // [width][256]
   __shared__ int parent[kForkWidth], length[kForkWidth];
   __shared__ int64_t slots[4];
   const uint32_t r = blockIdx.x, row0 = r * a.width;
@@ -306,8 +379,7 @@ __global__ __launch_bounds__(256) void fork_tables_kernel(ForkArgs a) {
   }
   __syncthreads();
   if (tid < 64) {
-    const bool copy = tid < width && takes_copy(parent, length, tid, a.page);
-    const uint64_t copies = __ballot(copy);
+    const uint64_t copies = copying_rows(parent, length, width, a.page);
     if (tid == 0) a.copies[r] = __popcll(copies);
   }
   uint64_t used = 0;  // rows with a child
@@ -322,24 +394,33 @@ __global__ __launch_bounds__(256) void fork_tables_kernel(ForkArgs a) {
   int n_dropped = 0;
   for (uint32_t c0 = 0; c0 < columns; c0 += 256) {
     const uint32_t c = c0 + tid;
-    uint64_t drop = 0;
-    if (c < columns) {
-      for (int i = 0; i < width; ++i) {
-        const int p = parent[i];
-        if (p >= 0 && c < blocks_of(length[p], a.page))
-          out[i * a.table_out_stride + c] = in[p * a.table_stride + c];
+    uint64_t held = 0, drop = 0;
+    for (int i = 0; i < width; ++i)
+      if (c < blocks_of(length[i], a.page)) held |= 1ull << i;
+    if (held) {
+      // the column in LDS (each thread its own): eight loads on their way at a time
+      for (int i0 = 0; i0 < width; i0 += 8) {
+        int e[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) e[i] = held >> (i0 + i) & 1 ? in[(i0 + i) * a.table_stride + c] : -1;
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (i0 + i < width) column[(i0 + i) * 256 + tid] = e[i];
       }
       for (int i = 0; i < width; ++i) {
-        if (used >> i & 1 || c >= blocks_of(length[i], a.page)) continue;
-        const int page = in[i * a.table_stride + c];
+        const int p = parent[i];
+        if (p >= 0 && held >> p & 1) out[i * a.table_out_stride + c] = column[p * 256 + tid];
+      }
+      for (uint64_t rest = held & ~used; rest; rest &= rest - 1) {
+        const int i = __ffsll((unsigned long long)rest) - 1, page = column[i * 256 + tid];
         if ((uint32_t)page >= a.pages) {
           bits |= kCacheArgument;
           continue;
         }
-        bool gone = true;  // held by no row with children, and by no lower row without
-        for (int j = 0; j < width && gone; ++j)
-          if ((used >> j & 1 || j < i) && c < blocks_of(length[j], a.page))
-            gone = in[j * a.table_stride + c] != page;
+        // held by no row with children, and by no lower row without
+        bool gone = true;
+        for (uint64_t others = held & (used | ((1ull << i) - 1)); others && gone; others &= others - 1)
+          gone = column[(__ffsll((unsigned long long)others) - 1) * 256 + tid] != page;
         if (gone) drop |= 1ull << i;
       }
     }
@@ -347,133 +428,75 @@ __global__ __launch_bounds__(256) void fork_tables_kernel(ForkArgs a) {
     int at = n_dropped + (int)before<256>(__popcll(drop), slots, &all);
     n_dropped += (int)all;
     for (; drop; drop &= drop - 1)
-      list[at++] = in[(__ffsll((unsigned long long)drop) - 1) * a.table_stride + c];
+      list[at++] = column[(__ffsll((unsigned long long)drop) - 1) * 256 + tid];
   }
   if (tid == 0) {
     a.drops[r] = n_dropped;
     if (r == 0) *a.count = stack_size(a.free_count, a.pages, &bits);
   }
   if (bits) flag(a.status, bits);
+  if constexpr (ALONE) {
+    // a single request has its books done here
+    __shared__ int s_upto[1];
+    __syncthreads();
+    fork_books(a, parent, length, slots, s_upto);
+  }
+}
+
+__global__ __launch_bounds__(256) void fork_books_kernel(ForkArgs a) {
+  __shared__ int parent[kForkWidth], length[kForkWidth];
+  __shared__ int64_t slots[4];
+  __shared__ int s_upto[kForkRequests];
+  const int tid = threadIdx.x, width = (int)a.width;
+  if (tid < width) {
+    const int p = a.parents[blockIdx.x * a.width + tid];
+    parent[tid] = p < 0 || p >= width ? -1 : p;
+    length[tid] = a.old_lengths[blockIdx.x * a.width + tid];
+  }
+  fork_books(a, parent, length, slots, s_upto);
 }
 
 struct ForkCaches {
   KvCache c[kForkCaches];
-  int n;
 };
 
-__device__ __forceinline__ void copy_page(const KvCache& c, uint32_t from, uint32_t to, uint32_t tokens,
-                                          uint32_t part, uint32_t parts) {
+// Copies the first tokens of one page per blockIdx.x in the cache blockIdx.z; blockIdx.y takes the pieces of
+// 16 bytes in turn, four at a time so that a lane has four loads on their way.
+__global__ __launch_bounds__(256) void fork_copy_kernel(const ForkCopy* copies, ForkCaches caches) {
+  const ForkCopy copy = copies[blockIdx.x];
+  const uint32_t tokens = copy.tokens;
+  if (tokens == 0) return;
+  const KvCache& c = caches.c[blockIdx.z];
   const bool f8 = c.k_scales != nullptr;
-  const uint32_t row16 = c.dim * (f8 ? 1 : 2) / 16;  // 16-byte pieces of a row
+  const uint32_t row16 = c.dim * (f8 ? 1 : 2) / 16;  // pieces of a row
   const uint32_t rows = 2 * c.heads * tokens, items = rows * row16;
-  for (uint32_t i = part * 256 + threadIdx.x; i < items; i += parts * 256) {
-    const uint32_t row = i / row16, piece = i - row * row16;
-    const uint32_t h2 = row / tokens, t = row - h2 * tokens;
-    const bool is_v = h2 >= c.heads;
-    uint8_t* base = (is_v ? c.v : c.k) + (is_v ? h2 - c.heads : h2) * c.head_stride +
-                    t * c.token_stride + 16 * piece;
-    *reinterpret_cast<uint4*>(base + to * c.page_stride) = ldg16(base + from * c.page_stride);
+  const uint64_t from = copy.from * c.page_stride, to = copy.to * c.page_stride;
+  const uint32_t step = gridDim.y * 256;
+  constexpr int AHEAD = 4;
+  for (uint32_t j0 = blockIdx.y * 256 + threadIdx.x; j0 < items; j0 += AHEAD * step) {
+    uint8_t* base[AHEAD];
+    uint4 v[AHEAD];
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u) {
+      const uint32_t j = min(j0 + u * step, items - 1);
+      const uint32_t row = j / row16, piece = j - row * row16;
+      const uint32_t h2 = row / tokens, t = row - h2 * tokens;
+      const bool is_v = h2 >= c.heads;
+      base[u] = (is_v ? c.v : c.k) + (is_v ? h2 - c.heads : h2) * c.head_stride + t * c.token_stride + 16 * piece;
+      v[u] = ldg16(base[u] + from);
+    }
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u)
+      if (j0 + u * step < items) *reinterpret_cast<uint4*>(base[u] + to) = v[u];
   }
   if (!f8) return;
-  for (uint32_t row = part * 256 + threadIdx.x; row < rows; row += parts * 256) {
+  for (uint32_t row = blockIdx.y * 256 + threadIdx.x; row < rows; row += step) {
     const uint32_t h2 = row / tokens, t = row - h2 * tokens;
     const bool is_v = h2 >= c.heads;
     const uint32_t h = is_v ? h2 - c.heads : h2;
     uint8_t* s = is_v ? c.v_scales : c.k_scales;
-    s[((uint64_t)to * c.heads + h) * c.page + t] = s[((uint64_t)from * c.heads + h) * c.page + t];
+    s[((uint64_t)copy.to * c.heads + h) * c.page + t] = s[((uint64_t)copy.from * c.heads + h) * c.page + t];
   }
-}
-
-// A row per blockIdx.x: its copied page, part blockIdx.y of it in every cache; in the first launch of a call
-// (`books`) its length, its table's entry for that page, and the stack.
-__global__ __launch_bounds__(256) void fork_copy_kernel(ForkArgs a, ForkCaches caches, bool books) {
-  __shared__ int parent[kForkWidth], length[kForkWidth];
-  __shared__ int64_t slots[4];
-  __shared__ int s_page;
-  const uint32_t row = blockIdx.x, r = row / a.width;
-  const int i = (int)(row - r * a.width), tid = threadIdx.x, width = (int)a.width;
-  books = books && blockIdx.y == 0;
-  if (tid < width) {
-    const int p = a.parents[r * a.width + tid];
-    parent[tid] = p < 0 || p >= width ? -1 : p;
-    length[tid] = a.old_lengths[r * a.width + tid];
-  }
-  if (tid == 0) s_page = -1;
-  __syncthreads();
-  const bool copy = takes_copy(parent, length, i, a.page);
-  const bool pushes = books && i == 0;
-  const int p = parent[i];
-  bool kept = p >= 0;  // whether the row goes on
-  int bits = 0;
-  if (copy || pushes) {
-    // pages dropped in all, and by the requests before; copies likewise
-    int64_t mine[4] = {0, 0, 0, 0}, sums[4];
-    for (uint32_t q = tid; q < a.requests; q += 256) {
-      const int d = a.drops[q], c = a.copies[q];
-      mine[0] += d;
-      mine[1] += c;
-      if (q < r) {
-        mine[2] += d;
-        mine[3] += c;
-      }
-    }
-#pragma unroll
-    for (int k = 0; k < 4; ++k) (void)before<256>(mine[k], slots, &sums[k]);
-    const int count = *a.count;
-    const int64_t room = (int64_t)a.pages - count;  // of the stack
-    const int64_t size = count + min(sums[0], room);
-    if (copy) {
-      int k = (int)sums[3];
-      for (int j = 0; j < i; ++j) k += takes_copy(parent, length, j, a.page);
-      const int64_t at = size - 1 - k;
-      int64_t passed = 0;
-      if (at < count) {
-        if (tid == 0 && at >= 0) s_page = a.free_pages[at];
-      } else {
-        // a page that a request has just dropped
-        const int64_t want = at - count;
-        for (uint32_t q0 = 0; q0 < a.requests && passed <= want; q0 += 256) {
-          const uint32_t q = q0 + tid;
-          const int d = q < a.requests ? a.drops[q] : 0;
-          int64_t all;
-          const int64_t first = passed + before<256>(d, slots, &all);
-          if (first <= want && want < first + d)
-            s_page = a.dropped[(uint64_t)q * a.width * a.max_blocks + (want - first)];
-          passed += all;
-        }
-      }
-      __syncthreads();
-      const uint32_t last = (uint32_t)length[p] / a.page;
-      const int to = s_page;
-      if (at < 0) {
-        kept = false;
-        bits |= kCacheMemory;
-      } else {
-        const int from = a.tables[(uint64_t)(r * a.width + p) * a.table_stride + last];
-        if (books && tid == 0) a.tables_out[row * a.table_out_stride + last] = to;
-        if ((uint32_t)to >= a.pages || (uint32_t)from >= a.pages) {
-          bits |= kCacheArgument;
-        } else {
-          const uint32_t tokens = (uint32_t)length[p] % a.page;
-          for (int c = 0; c < caches.n; ++c)
-            copy_page(caches.c[c], (uint32_t)from, (uint32_t)to, tokens, blockIdx.y, gridDim.y);
-        }
-      }
-    }
-    if (pushes) {
-      const int32_t* list = a.dropped + (uint64_t)r * a.width * a.max_blocks;
-      const int64_t first = count + sums[2];
-      const int n = a.drops[r];
-      for (int j = tid; j < n; j += 256)
-        if (first + j < a.pages) a.free_pages[first + j] = list[j];
-      if (r == 0 && tid == 0) {
-        *a.free_count_out = (int)max(size - sums[1], (int64_t)0);
-        if (sums[0] > room) bits |= kCacheArgument;
-      }
-    }
-  }
-  if (books && tid == 0) a.lengths_out[row] = kept ? length[p] : 0;
-  if (bits && tid == 0) flag(a.status, bits);
 }
 
 }  // namespace
@@ -510,23 +533,29 @@ void launch_plan(const PlanArgs& a, hipStream_t s) {
 }
 
 void launch_fork(const ForkArgs& a, const KvCache* caches, uint32_t n_caches, hipStream_t s) {
-  fork_tables_kernel<<<a.requests, 256, 0, s>>>(a);
-  uint32_t done = 0;
-  do {
+  const size_t lds = a.width * 256 * sizeof(int);
+  if (a.requests == 1) {
+    fork_tables_kernel<true><<<1, 256, lds, s>>>(a);
+  } else {
+    fork_tables_kernel<false><<<a.requests, 256, lds, s>>>(a);
+    fork_books_kernel<<<a.requests, 256, 0, s>>>(a);
+  }
+  for (uint32_t done = 0; done < n_caches;) {
     ForkCaches some;
-    some.n = (int)std::min<uint32_t>(kForkCaches, n_caches - done);
+    const uint32_t n = std::min<uint32_t>(kForkCaches, n_caches - done);
     uint64_t bytes = 0;
-    for (int i = 0; i < some.n; ++i) {
+    for (uint32_t i = 0; i < n; ++i) {
       some.c[i] = caches[done + i];
-      bytes += 2ull * caches[done + i].heads * a.page * caches[done + i].dim;
+      bytes = std::max<uint64_t>(bytes, 2ull * caches[done + i].heads * a.page * caches[done + i].dim);
     }
-    // parts of a page: some 16 KB each, at most sixteen per CU over all rows
+    // parts of a page: four pieces for every lane where the cache is the largest, while that is no more than
+    // 64 workgroups per CU
     const uint32_t rows = a.requests * a.width;
     const uint32_t parts = (uint32_t)std::max<uint64_t>(
-        1, std::min<uint64_t>(bytes / 16384, 4096 / rows));
-    fork_copy_kernel<<<dim3(rows, parts), 256, 0, s>>>(a, some, done == 0);
-    done += (uint32_t)some.n;
-  } while (done < n_caches);
+        1, std::min<uint64_t>(bytes / 16384, 16384 / (rows * n)));
+    fork_copy_kernel<<<dim3(rows, parts, n), 256, 0, s>>>(a.page_copies, some);
+    done += n;
+  }
 }
 
 }  // namespace urb
