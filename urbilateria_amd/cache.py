@@ -16,7 +16,7 @@ from typing import Optional, Sequence
 
 from . import native as N
 from .moe import torch
-from .step import _Context, _Current, _stream, _type, _vector
+from .step import _Context, _stream, _type, _vector
 
 _CACHE_TYPES = {} if torch is None else {torch.bfloat16: N.DTYPES["BF16"],
                                          torch.float8_e4m3fn: N.DTYPES["F8_E4M3"]}
@@ -24,6 +24,20 @@ _CACHE_TYPES = {} if torch is None else {torch.bfloat16: N.DTYPES["BF16"],
 
 def _cache_type(dtype) -> int:
     return _CACHE_TYPES.get(dtype, 7)
+
+
+def _call(name: str, device: int, stream, *args) -> None:
+    """The library's function, on the device and the stream.  (torch.cuda.current_device() and a context
+    manager take a microsecond of a call of six.)"""
+    function = getattr(N.moe_lib(), name)
+    handle = _stream(stream, device)
+    if torch._C._cuda_getDevice() == device:
+        st = function(*args, handle)
+    else:
+        with torch.cuda.device(device):
+            st = function(*args, handle)
+    if st:
+        raise N.UrbError(st, name)
 
 
 def _address(t, name: str, shape, dtype, device: int) -> int:
@@ -97,23 +111,34 @@ class PagedCache:
                         *_strides(k, "k", shape, k.dtype, self.device),
                         *_strides(v, "v", shape, k.dtype, self.device))
         at = _vector(slots, "slots", shape[0], torch.int64, self.device)
-        with _Current(self.device):
-            st = N.moe_lib().urb_kv_append(self._ref, ctypes.byref(rows), at, shape[0],
-                                           _stream(stream, self.device))
-        if st:
-            raise N.UrbError(st, "urb_kv_append")
+        _call("urb_kv_append", self.device, stream, self._ref, ctypes.byref(rows), at, shape[0])
 
 
 class Plan:
     """What ``Pager.plan_into`` writes: ``lengths`` [rows] int32 after the step, ``starts`` [rows + 1]
     int32, ``rows`` [tokens] int32, ``positions`` and ``slots`` [tokens] int64, ``count`` [1] int32, the
-    free pages that are left."""
-
-    __slots__ = ("lengths", "starts", "rows", "positions", "slots", "count")
+    free pages that are left.  Its tensors may be replaced, but not resized."""
 
     def __init__(self, lengths, starts, rows, positions, slots, count):
         self.lengths, self.starts, self.rows = lengths, starts, rows
         self.positions, self.slots, self.count = positions, slots, count
+
+    def __setattr__(self, name, value):
+        # the checked call is built again when a tensor is replaced
+        object.__setattr__(self, name, value)
+        object.__setattr__(self, "_checked", None)
+
+    def _call_of(self, rows: int, device: int) -> tuple:
+        if self._checked is None or self._checked[:2] != (rows, device):
+            i32, i64, tokens = torch.int32, torch.int64, self.slots.numel()
+            call = N.PagePlan(rows=rows, tokens=tokens)
+            for name, field, n, dtype in (
+                    ("lengths", "lengths_out", rows, i32), ("starts", "starts", rows + 1, i32),
+                    ("rows", "token_rows", tokens, i32), ("positions", "positions", tokens, i64),
+                    ("slots", "slots", tokens, i64), ("count", "free_count_out", 1, i32)):
+                setattr(call, field, _vector(getattr(self, name), "plan." + name, n, dtype, device))
+            object.__setattr__(self, "_checked", (rows, device, call, ctypes.byref(call)))
+        return self._checked
 
 
 class Pager(_Context):
@@ -147,25 +172,16 @@ class Pager(_Context):
         """The pages and slots for ``added`` [rows] int32 new tokens (None: one each) behind ``lengths``
         [rows] int32: enters pages in ``tables`` and fills ``plan``.  ``plan.lengths`` may be ``lengths``
         and ``plan.count`` ``count``; ``plan.starts``, ``rows`` and ``positions`` may be None."""
-        dev, rows, tokens = self.device, lengths.numel(), plan.slots.numel()
-        i32, i64 = torch.int32, torch.int64
-        at, stride, columns = _table(tables, "tables", rows, dev)
+        dev, rows, i32 = self.device, lengths.numel(), torch.int32
+        call, ref = plan._call_of(rows, dev)[2:]
+        call.tables, call.table_stride, columns = _table(tables, "tables", rows, dev)
         if columns < self.max_blocks:
             raise ValueError(f"tables must have {self.max_blocks} columns")
-        call = N.PagePlan(rows, tokens, stride, _vector(lengths, "lengths", rows, i32, dev),
-                          _vector(added, "added", rows, i32, dev), at,
-                          _vector(free, "free", self.pages, i32, dev),
-                          _vector(count, "count", 1, i32, dev),
-                          _vector(plan.lengths, "plan.lengths", rows, i32, dev),
-                          _vector(plan.starts, "plan.starts", rows + 1, i32, dev),
-                          _vector(plan.rows, "plan.rows", tokens, i32, dev),
-                          _vector(plan.positions, "plan.positions", tokens, i64, dev),
-                          _vector(plan.slots, "plan.slots", tokens, i64, dev),
-                          _vector(plan.count, "plan.count", 1, i32, dev))
-        with _Current(dev):
-            st = N.moe_lib().urb_pager_plan(self._ctx, ctypes.byref(call), _stream(stream, dev))
-        if st:
-            raise N.UrbError(st, "urb_pager_plan")
+        call.lengths = _vector(lengths, "lengths", rows, i32, dev)
+        call.added = _vector(added, "added", rows, i32, dev)
+        call.free_pages = _vector(free, "free", self.pages, i32, dev)
+        call.free_count = _vector(count, "count", 1, i32, dev)
+        _call("urb_pager_plan", dev, stream, self._ctx, ref)
 
     def plan(self, lengths, added, tables, free, count, tokens: int) -> Plan:
         """``plan_into`` with new tensors for ``tokens`` tokens; raises UrbError for rows that are not
@@ -203,10 +219,7 @@ class Pager(_Context):
                           _vector(count, "count", 1, i32, dev),
                           _vector(count_out, "count_out", 1, i32, dev),
                           ctypes.addressof(layers) if caches else None, len(caches))
-        with _Current(dev):
-            st = N.moe_lib().urb_pager_fork(self._ctx, ctypes.byref(call), _stream(stream, dev))
-        if st:
-            raise N.UrbError(st, "urb_pager_fork")
+        _call("urb_pager_fork", dev, stream, self._ctx, ctypes.byref(call))
 
 
 class PagedAttention(_Context):
@@ -249,10 +262,7 @@ class PagedAttention(_Context):
                                _vector(sinks, "sinks", self.q_heads, torch.float32, dev),
                                None if lse is None else _address(lse, "lse", shape[:3], torch.float32,
                                                                  dev))
-        with _Current(dev):
-            st = N.moe_lib().urb_attend(self._ctx, cache._ref, ctypes.byref(call), _stream(stream, dev))
-        if st:
-            raise N.UrbError(st, "urb_attend")
+        _call("urb_attend", dev, stream, self._ctx, cache._ref, ctypes.byref(call))
 
     def attend(self, q, cache: PagedCache, tables, lengths, sinks=None):
         """-> out; raises UrbError for lengths or table entries out of range."""

@@ -62,8 +62,8 @@ struct Line {
   uint32_t shares;        // workgroups that can have units
   bool by_pair;           // how joins are kept
   Join* joins;            // [shares]
-  uint32_t page_magic, page_shift;  // t / page_size = t * page_magic >> page_shift for t < 2^25
-  uint32_t page16, token16;         // strides in units of 16 bytes
+  PageDivision page;
+  uint32_t page16, token16;  // strides in units of 16 bytes
 };
 
 // The tokens in reach of any query of a row, [first, end), and first rounded down to a tile; a length that
@@ -293,13 +293,10 @@ __global__ __launch_bounds__(64 * kWaves, (kPerCu<DS, F8, BF16>)) void attend_ke
     return g;
   };
 
-  auto block_of = [&](int t) -> uint32_t {
-    return (uint32_t)((uint64_t)(uint32_t)t * line.page_magic >> line.page_shift);
-  };
   // The tile's token of this lane: lanes l and l + 32 have token l.
   auto page_of = [&](const Segment& g, int tile) -> int {
     const int t = tile + (lane & 31);
-    return t >= g.reach.first && t < g.t1 ? a.tables[g.at.row * a.table_stride + block_of(t)] : -1;
+    return t >= g.reach.first && t < g.t1 ? a.tables[g.at.row * a.table_stride + line.page.of((uint32_t)t)] : -1;
   };
   uint4 kr[2][KL], vr[VL];
   uint32_t valid = 0, code = 0;  // tokens of the tile that there are; the scale code of the lane's token
@@ -309,7 +306,7 @@ __global__ __launch_bounds__(64 * kWaves, (kPerCu<DS, F8, BF16>)) void attend_ke
     const bool fine = (uint32_t)page < a.cache.pages;
     if (t >= g.reach.first && t < g.t1 && !fine) flag(a.status, kCacheArgument);
     valid = (uint32_t)__ballot(fine);
-    const uint32_t slot = (uint32_t)t - block_of(t) * a.cache.page;
+    const uint32_t slot = (uint32_t)t - line.page.of((uint32_t)t) * line.page.size;
     // 16-byte units from the head's base to the lane's token
     const uint32_t off = fine ? (uint32_t)page * line.page16 + slot * line.token16 : 0;
     if constexpr (F8) {
@@ -692,11 +689,7 @@ Line line_of(const AttendArgs& a) {
   line.inv_group = 1.0f / (float)line.group;
   line.tiles = (a.queries * line.group + 15) / 16;
   line.pairs = a.cache.heads * line.tiles;
-  // with 2^s < page_size <= 2^(s + 1), the magic number of shift 32 + s has 32 bits, and its excess times t
-  // stays below 2^(32 + s)
-  line.page_shift = 31;
-  while (a.cache.page > 1u << (line.page_shift - 31)) ++line.page_shift;
-  line.page_magic = (uint32_t)(((1ull << line.page_shift) + a.cache.page - 1) / a.cache.page);
+  line.page = PageDivision::by(a.cache.page);
   line.page16 = (uint32_t)(a.cache.page_stride >> 4);
   line.token16 = (uint32_t)(a.cache.token_stride >> 4);
   return line;

@@ -11,6 +11,20 @@ namespace urb {
 constexpr int kCacheArgument = 1;
 constexpr int kCacheMemory = 2;
 
+// Division by a page size d <= 1024: n / d = n * magic >> shift for n < 2^31.  With 2^s < d <= 2^(s + 1) and shift
+// 32 + s the magic number ceil(2^shift / d) has 32 bits, and its excess (below d / 2^shift) times n is below 1 / d.
+struct PageDivision {
+  uint32_t size, magic, shift;
+  static PageDivision by(uint32_t size) {
+    PageDivision d{size, 0, 31};
+    while (size > 1u << (d.shift - 31)) ++d.shift;
+    d.magic = (uint32_t)(((1ull << d.shift) + size - 1) / size);
+    return d;
+  }
+  __host__ __device__ uint32_t of(uint32_t n) const { return (uint32_t)((uint64_t)n * magic >> shift); }
+  __host__ __device__ uint32_t up(uint32_t n) const { return of(n + size - 1); }
+};
+
 // One layer's cache; strides in bytes.
 struct KvCache {
   uint8_t *k, *v;
@@ -29,8 +43,14 @@ struct AppendArgs {
 };
 void launch_append(const AppendArgs& a, bool rows_bf16, hipStream_t s);
 
+// A row's first token, its length before, and the place on the stack of its first new page (-1: the row is
+// not served).
+struct __attribute__((aligned(16))) PlanRow {
+  int32_t start, have, top, pad;
+};
 struct PlanArgs {
-  uint32_t rows, tokens, page, pages, max_blocks;
+  uint32_t rows, tokens, pages, max_blocks;
+  PageDivision page;
   uint64_t table_stride;
   const int32_t *lengths, *added;
   int32_t* tables;
@@ -38,9 +58,7 @@ struct PlanArgs {
   int32_t *lengths_out, *starts, *token_rows;
   int64_t *positions, *slots;
   int32_t* free_count_out;
-  // workspace, [max_rows] each: a row's length before, its first token, the place on the stack of its
-  // first new page (-1: the row is not served)
-  int32_t *row_have, *row_start, *row_top;
+  PlanRow* row_plans;  // workspace, [max_rows + 1]
   int* status;
 };
 void launch_plan(const PlanArgs& a, hipStream_t s);

@@ -13,8 +13,8 @@ struct urb_pager {
   int device = 0;
   void* work = nullptr;
   int* status = nullptr;
-  // plans: [max_rows + 1] each; forks: [max_rows], [kForkRequests] twice, [1], [max_rows * max_blocks]
-  int32_t *row_have = nullptr, *row_start = nullptr, *row_top = nullptr;
+  urb::PlanRow* row_plans = nullptr;  // [max_rows + 1]
+  // forks: [max_rows], [kForkRequests] twice, [1], [max_rows * max_blocks]
   int32_t *old_lengths = nullptr, *drops = nullptr, *copies = nullptr, *count = nullptr, *dropped = nullptr;
   urb::ForkCopy* page_copies = nullptr;  // [max_rows]
 };
@@ -148,9 +148,7 @@ urb_status urb_pager_create(const urb_pager_desc* d, urb_pager** out) {
   const size_t requests = std::min<size_t>(urb::kForkRequests, rows);
   char* p = nullptr;  // (offsets first, addresses when the memory is there)
   auto lay = [&]() {
-    c->row_have = carve<int32_t>(p, rows + 1);
-    c->row_start = carve<int32_t>(p, rows + 1);
-    c->row_top = carve<int32_t>(p, rows + 1);
+    c->row_plans = carve<urb::PlanRow>(p, rows + 1);
     c->old_lengths = carve<int32_t>(p, rows);
     c->drops = carve<int32_t>(p, requests);
     c->copies = carve<int32_t>(p, requests);
@@ -186,7 +184,7 @@ urb_status urb_pager_plan(urb_pager* c, const urb_page_plan* p, void* stream) {
   urb::PlanArgs a{};
   a.rows = p->rows;
   a.tokens = p->tokens;
-  a.page = d.page_size;
+  a.page = urb::PageDivision::by(d.page_size);
   a.pages = d.pages;
   a.max_blocks = d.max_blocks;
   a.table_stride = p->table_stride;
@@ -201,9 +199,7 @@ urb_status urb_pager_plan(urb_pager* c, const urb_page_plan* p, void* stream) {
   a.positions = p->positions;
   a.slots = p->slots;
   a.free_count_out = p->free_count_out;
-  a.row_have = c->row_have;
-  a.row_start = c->row_start;
-  a.row_top = c->row_top;
+  a.row_plans = c->row_plans;
   a.status = c->status;
   urb::launch_plan(a, static_cast<hipStream_t>(stream));
   URB_HIP(hipGetLastError());

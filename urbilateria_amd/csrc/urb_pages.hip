@@ -136,15 +136,43 @@ __device__ __forceinline__ int stack_size(const int32_t* count, uint32_t pages, 
 // ---- the pages and slots of a step ----
 //
 // Two sums over the rows say all: the tokens and the pages that the rows before a row bring.  They are one
-// workgroup's work (a row is 8 bytes); its tokens follow in the same launch while they are few, in a grid of
-// their own otherwise.
-constexpr int kPlanThreads = 1024;
-constexpr int kPlanWindow = 1024;  // rows whose first tokens are held in LDS
+// workgroup's work (a row is 8 bytes, four of them a thread's); the tokens follow in the same launch while they
+// are few, in a grid of their own otherwise.  Latency bounds both: loads, two sums, the stack or the table,
+// stores.
+constexpr int kPlanThreads = 1024, kPlanPer = 4;
+constexpr int kPlanWindow = 1024;  // rows of a search in LDS
+constexpr int kPlanTokens = 1024;  // tokens of a workgroup of their own
 
-// Tokens t0 .. t1 - 1, whose rows lie among first .. first + n - 1: starts (LDS or global) are their first
-// tokens.
+// The sums over the lanes up to this one, no more than `most` (such sums do not depend on their order).
+__device__ __forceinline__ uint32_t wave_upto(uint32_t v, uint32_t most) {
+  auto add = [&](int moved) { v = min(v + (uint32_t)moved, most); };
+  add(__builtin_amdgcn_update_dpp(0, (int)v, 0x111, 0xf, 0xf, false));  // row_shr 1, 2, 4, 8: rows of 16
+  add(__builtin_amdgcn_update_dpp(0, (int)v, 0x112, 0xf, 0xf, false));
+  add(__builtin_amdgcn_update_dpp(0, (int)v, 0x114, 0xf, 0xf, false));
+  add(__builtin_amdgcn_update_dpp(0, (int)v, 0x118, 0xf, 0xf, false));
+  add(__builtin_amdgcn_update_dpp(0, (int)v, 0x142, 0xa, 0xf, false));  // row 0's last into 1, 2's into 3
+  add(__builtin_amdgcn_update_dpp(0, (int)v, 0x143, 0xc, 0xf, false));  // row 1's last into 2 and 3
+  return v;
+}
+// The sums over the threads before this one and over all, no more than `most` (below 2^31).
+__device__ __forceinline__ uint32_t plan_before(uint32_t v, uint32_t most, uint32_t* slots, uint32_t* all) {
+  constexpr int WAVES = kPlanThreads / 64;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const uint32_t upto = wave_upto(v, most);
+  __syncthreads();
+  if (lane == 63) slots[wave] = upto;
+  __syncthreads();
+  const uint32_t sums = wave_upto(lane < WAVES ? slots[lane] : 0, most);
+  *all = (uint32_t)__builtin_amdgcn_readlane((int)sums, WAVES - 1);
+  const uint32_t before = wave ? (uint32_t)__builtin_amdgcn_readlane((int)sums, wave - 1) : 0;
+  const uint32_t lower = (uint32_t)__shfl_up((int)upto, 1, 64);
+  return min(before + (lane ? lower : 0), most);
+}
+
+// The tokens t0 .. t1 - 1 (total of them real), whose rows are among the n from `first` on: rows[i] is row
+// first + i, in LDS or not.
 __device__ __forceinline__ void plan_tokens(const PlanArgs& a, uint32_t t0, uint32_t t1, uint32_t total,
-                                            const int32_t* starts, uint32_t first, uint32_t n) {
+                                            const PlanRow* rows, uint32_t first, uint32_t n) {
   int bits = 0;
   for (uint32_t t = t0 + threadIdx.x; t < t1; t += blockDim.x) {
     int row = -1;
@@ -153,23 +181,24 @@ __device__ __forceinline__ void plan_tokens(const PlanArgs& a, uint32_t t0, uint
       uint32_t lo = 0, hi = n;  // the last row that starts at t or before
       while (hi - lo > 1) {
         const uint32_t mid = (lo + hi) / 2;
-        if (starts[mid] <= (int)t) lo = mid;
+        if (rows[mid].start <= (int)t) lo = mid;
         else hi = mid;
       }
+      const PlanRow r = rows[lo];
       row = (int)(first + lo);
-      const int have = a.row_have[row], top = a.row_top[row];
-      position = (int64_t)have + (int)t - starts[lo];
-      if (top >= 0) {
-        const uint32_t p = (uint32_t)position, block = p / a.page, held = (have + a.page - 1) / a.page;
+      position = (int64_t)r.have + (int)t - r.start;
+      if (r.top >= 0) {
+        const uint32_t p = (uint32_t)position, block = a.page.of(p), at = p - block * a.page.size;
+        const uint32_t held = a.page.up((uint32_t)r.have);
         int32_t* entry = a.tables + row * a.table_stride + block;
         int page;
         if (block < held) {
           page = *entry;
         } else {
-          page = a.free_pages[top - (int)(block - held)];
-          if (p % a.page == 0) *entry = page;
+          page = a.free_pages[r.top - (int)(block - held)];
+          if (at == 0) *entry = page;
         }
-        if ((uint32_t)page < a.pages) slot = (int64_t)page * a.page + p % a.page;
+        if ((uint32_t)page < a.pages) slot = (int64_t)page * a.page.size + at;
         else bits |= kCacheArgument;
       }
     }
@@ -182,87 +211,107 @@ __device__ __forceinline__ void plan_tokens(const PlanArgs& a, uint32_t t0, uint
 
 template <bool ALL>
 __global__ __launch_bounds__(kPlanThreads) void plan_rows_kernel(PlanArgs a) {
-  __shared__ int64_t slots[kPlanThreads / 64];
-  __shared__ int32_t starts[ALL ? kPlanWindow : 1];
+  __shared__ uint32_t slots[kPlanThreads / 64];
+  __shared__ int s_used;
+  __shared__ PlanRow rows[ALL ? kPlanWindow : 1];
+  constexpr int PER = ALL ? 1 : kPlanPer;  // rows of a thread
+  const uint32_t most_tokens = a.tokens + 1, most_pages = a.pages + 1;
+  const int tid = threadIdx.x;
   int bits = 0;
+  if (tid == 0) s_used = 0;
   const int count = stack_size(a.free_count, a.pages, &bits);
-  int64_t tokens_before = 0, pages_before = 0, used = 0;
-  for (uint32_t r0 = 0; r0 < a.rows; r0 += kPlanThreads) {
-    const uint32_t r = r0 + threadIdx.x;
-    const bool in = r < a.rows;
-    const int have = in ? a.lengths[r] : 0, add = in ? (a.added ? a.added[r] : 1) : 0;
-    const bool ok = have >= 0 && add >= 0 &&
-                    (int64_t)have + add <= (int64_t)a.max_blocks * a.page;
-    const int tokens = ok ? add : 0;
-    int64_t all;
-    const int64_t start = tokens_before + before<kPlanThreads>(tokens, slots, &all);
-    tokens_before += all;
-    const bool over = start + tokens > a.tokens;
-    const int need = ok && !over ? (int)((have + tokens + a.page - 1) / a.page -
-                                         (have + a.page - 1) / a.page)
-                                 : 0;
-    const int64_t first = pages_before + before<kPlanThreads>(need, slots, &all);
-    pages_before += all;
-    const bool enough = need == 0 || first + need <= count;
-    const bool served = ok && !over && enough;
-    (void)before<kPlanThreads>(served ? need : 0, slots, &all);
-    used += all;
-    if (!ok || over) bits |= kCacheArgument;
-    if (!enough) bits |= kCacheMemory;
-    const int at = (int)min(start, (int64_t)a.tokens);
-    if (in) {
-      a.row_have[r] = have;
-      a.row_start[r] = at;
-      a.row_top[r] = !served ? -1 : need ? count - 1 - (int)first : 0;
-      a.lengths_out[r] = served ? have + tokens : have;
-      if (a.starts) a.starts[r] = at;
-      if constexpr (ALL) starts[r] = at;
+  uint32_t tokens_before = 0, pages_before = 0;
+  for (uint32_t r0 = 0; r0 < a.rows; r0 += PER * kPlanThreads) {
+    const uint32_t first_row = r0 + PER * tid;
+    int have[PER], tokens[PER];
+    bool ok[PER];
+    uint32_t sum = 0, all;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const uint32_t r = first_row + i;
+      have[i] = r < a.rows ? a.lengths[r] : 0;
+      tokens[i] = r < a.rows ? a.added ? a.added[r] : 1 : 0;
     }
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      ok[i] = have[i] >= 0 && tokens[i] >= 0 &&
+              (int64_t)have[i] + tokens[i] <= (int64_t)a.max_blocks * a.page.size;
+      if (!ok[i]) tokens[i] = 0;
+      sum = min(sum + (uint32_t)tokens[i], most_tokens);
+    }
+    uint32_t start[PER];
+    start[0] = min(tokens_before + plan_before(sum, most_tokens, slots, &all), most_tokens);
+    tokens_before = min(tokens_before + all, most_tokens);
+#pragma unroll
+    for (int i = 1; i < PER; ++i) start[i] = min(start[i - 1] + (uint32_t)tokens[i - 1], most_tokens);
+    // pages, of the rows whose tokens have their places
+    int need[PER];
+    bool over[PER];
+    sum = 0;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      over[i] = start[i] + (uint32_t)tokens[i] > a.tokens;
+      need[i] = ok[i] && !over[i]
+                    ? (int)(a.page.up((uint32_t)(have[i] + tokens[i])) - a.page.up((uint32_t)have[i]))
+                    : 0;
+      sum = min(sum + (uint32_t)need[i], most_pages);
+    }
+    uint32_t page = min(pages_before + plan_before(sum, most_pages, slots, &all), most_pages);
+    pages_before = min(pages_before + all, most_pages);
+    int used = 0;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const uint32_t r = first_row + i;
+      const bool enough = need[i] == 0 || page + (uint32_t)need[i] <= (uint32_t)count;
+      const bool served = ok[i] && !over[i] && enough;
+      if (served && need[i]) used = (int)page + need[i];
+      if (r < a.rows) {
+        if (!ok[i] || over[i]) bits |= kCacheArgument;
+        if (!enough) bits |= kCacheMemory;
+        const int at = (int)min(start[i], a.tokens);
+        const PlanRow row{at, have[i], !served ? -1 : need[i] ? count - 1 - (int)page : 0, 0};
+        if constexpr (ALL) rows[r] = row;
+        else a.row_plans[r] = row;
+        a.lengths_out[r] = served ? have[i] + tokens[i] : have[i];
+        if (a.starts) a.starts[r] = at;
+      }
+      page = min(page + (uint32_t)need[i], most_pages);
+    }
+    // (of the rows that need pages, those that are served come first)
+    if (used) atomicMax(&s_used, used);
   }
-  const int total = (int)min(tokens_before, (int64_t)a.tokens);
-  if (threadIdx.x == 0) {
-    if (a.starts) a.starts[a.rows] = total;
-    *a.free_count_out = count - (int)used;
-    a.row_start[a.rows] = total;
+  __syncthreads();
+  const uint32_t total = min(tokens_before, a.tokens);
+  if (tid == 0) {
+    if (a.starts) a.starts[a.rows] = (int)total;
+    *a.free_count_out = count - s_used;
+    if constexpr (!ALL) a.row_plans[a.rows] = PlanRow{(int)total, 0, -1, 0};
   }
   if (bits) flag(a.status, bits);
-  if constexpr (ALL) {
-    __syncthreads();
-    plan_tokens(a, 0, a.tokens, (uint32_t)total, starts, 0, a.rows);
-  }
+  if constexpr (ALL) plan_tokens(a, 0, a.tokens, total, rows, 0, a.rows);
 }
 
-// The last of rows 0 .. n - 1 whose first token is t or before, by a whole wave.
-__device__ __forceinline__ uint32_t row_of(const int32_t* starts, uint32_t n, uint32_t t) {
-  const int lane = threadIdx.x & 63;
-  uint32_t lo = 0;
-  while (n > 1) {
-    const uint32_t step = (n + 63) / 64;
-    const uint32_t at = lane * step;
-    const uint64_t below = __ballot(at < n && starts[lo + at] <= (int)t);
-    const uint32_t part = 63 - __clzll(below | 1);
-    lo += part * step;
-    n = min(step, n - part * step);
-  }
-  return lo;
-}
-
-constexpr int kPlanTokens = 1024;  // of a workgroup
 __global__ __launch_bounds__(256) void plan_tokens_kernel(PlanArgs a) {
-  __shared__ int32_t starts[kPlanWindow];
+  __shared__ PlanRow rows[kPlanWindow];
   const uint32_t t0 = blockIdx.x * kPlanTokens, t1 = min(t0 + kPlanTokens, a.tokens);
-  const uint32_t total = (uint32_t)a.row_start[a.rows];
-  uint32_t first = 0, n = 1;
-  const int32_t* from = a.row_start;
-  if (t0 < total) {
-    first = row_of(a.row_start, a.rows, t0);
-    n = row_of(a.row_start, a.rows, min(t1, total) - 1) - first + 1;
-    from = a.row_start + first;
-    // (more rows than tokens where some bring none)
-    if (n <= kPlanWindow) {
-      for (uint32_t i = threadIdx.x; i < n; i += 256) starts[i] = from[i];
-      from = starts;
-    }
+  const uint32_t total = (uint32_t)a.row_plans[a.rows].start;
+  // The rows from that of the first token to that of the last: all of them, cut down by probes of every
+  // step-th while they are too many for LDS (and the probes tell: many rows may bring no token).
+  uint32_t first = 0, n = a.rows;
+  while (n > kPlanWindow) {
+    const uint32_t step = (n + 255) / 256, at = threadIdx.x * step;
+    const int start = at < n ? a.row_plans[first + at].start : 0x7fffffff;
+    const uint32_t lower = (uint32_t)max(1, __syncthreads_count(start <= (int)t0));
+    const uint32_t upper = (uint32_t)max(1, __syncthreads_count(start < (int)t1));
+    const uint32_t skip = (lower - 1) * step, left = min(n, upper * step) - skip;
+    first += skip;
+    if (left == n) break;
+    n = left;
+  }
+  const PlanRow* from = a.row_plans + first;
+  if (n <= kPlanWindow) {
+    for (uint32_t i = threadIdx.x; i < n; i += 256) rows[i] = from[i];
+    from = rows;
   }
   __syncthreads();
   plan_tokens(a, t0, t1, total, from, first, n);
