@@ -34,6 +34,7 @@ constexpr int kUnit = 128;       // tokens
 constexpr int kStart = 1;
 constexpr int kTile = 32;        // tokens of a wave's step
 constexpr int kWaves = 4;
+constexpr int kStep = kTile * kWaves;  // tokens of a workgroup's step
 constexpr int kAttendRows = 1024;  // of a launch
 constexpr int kCus = 256;
 constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
@@ -64,6 +65,7 @@ struct Line {
   Join* joins;            // [shares]
   PageDivision page;
   uint32_t page16, token16;  // strides in units of 16 bytes
+  bool near;                 // 16 tokens from a multiple of 16 on lie at one distance, in less than 2^32 bytes
 };
 
 // The tokens in reach of any query of a row, [first, end), and first rounded down to a tile; a length that
@@ -82,12 +84,11 @@ __device__ __forceinline__ uint32_t units_of(Reach r) {
 }
 
 // upto[i] = units per pair of rows 0 .. i, and the rows' lengths; all threads, ends with a barrier.
-__device__ __forceinline__ void fill_line(const AttendArgs& a, uint32_t* upto, int* lengths, uint32_t* sums,
-                                          bool flags) {
+__device__ __forceinline__ void fill_line(const AttendArgs& a, uint32_t* upto, int* lengths, uint32_t* sums) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   uint32_t base = 0;
   bool bad = false;
-  for (uint32_t r0 = 0; r0 < a.rows; r0 += 256) {
+  for (uint32_t r0 = 0; r0 < a.rows; r0 += 64 * kWaves) {
     const uint32_t r = r0 + tid;
     uint32_t u = 0;
     if (r < a.rows) {
@@ -111,13 +112,22 @@ __device__ __forceinline__ void fill_line(const AttendArgs& a, uint32_t* upto, i
     if (r < a.rows) upto[r] = below + u;
     __syncthreads();
   }
-  if (flags && bad) flag(a.status, kCacheArgument);
+  if (blockIdx.x == 0 && bad) flag(a.status, kCacheArgument);
 }
 
 // A value of LDS that all lanes read alike, as a scalar.
 template <class T>
 __device__ __forceinline__ T same(T v) {
   return (T)__builtin_amdgcn_readfirstlane((int)v);
+}
+
+// n / d for quotients below 2^20, as a scalar.
+__device__ __forceinline__ uint32_t quotient(uint32_t n, uint32_t d) {
+  int q = (int)((float)n * __builtin_amdgcn_rcpf((float)d));
+  // (the product is off by less than one)
+  const int left = (int)(n - (uint32_t)q * d);
+  q += left < 0 ? -1 : (uint32_t)left >= d ? 1 : 0;
+  return same((uint32_t)q);
 }
 
 // The place of a unit: row, pair of it, units of a pair of the row, the pair's first unit of tokens and the
@@ -137,7 +147,7 @@ __device__ __forceinline__ Place place_of(const uint32_t* upto, uint32_t rows, u
   p.row = lo;
   p.units = same(upto[lo]) - under;
   const uint32_t start = under * pairs;
-  p.pair = same((unit - start) / p.units);
+  p.pair = quotient(unit - start, p.units);
   p.end = start + (p.pair + 1) * p.units;
   p.first = p.end - p.units + kStart;
   return p;
@@ -256,7 +266,7 @@ __global__ __launch_bounds__(64 * kWaves, (kPerCu<DS, F8, BF16>)) void attend_ke
 
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 15, grp = lane >> 4;
-  fill_line(a, upto, lengths, sums, blockIdx.x == 0);
+  fill_line(a, upto, lengths, sums);
   const Shares shares(same(upto[a.rows - 1]) * line.pairs, line.shares);
   if (blockIdx.x >= shares.n) {
     if (!line.by_pair && tid == 0) line.joins[blockIdx.x].n = 0;
@@ -289,7 +299,7 @@ __global__ __launch_bounds__(64 * kWaves, (kPerCu<DS, F8, BF16>)) void attend_ke
     g.stop = min(unit_end, g.at.end);
     g.t0 = g.reach.begin + (g.begins ? 0 : (int)(unit - g.at.first) * kUnit);
     g.t1 = min(g.reach.end, g.reach.begin + (int)(g.stop - g.at.first) * kUnit);
-    g.head = same(g.at.pair / line.tiles);
+    g.head = quotient(g.at.pair, line.tiles);
     return g;
   };
 
@@ -298,6 +308,16 @@ __global__ __launch_bounds__(64 * kWaves, (kPerCu<DS, F8, BF16>)) void attend_ke
     const int t = tile + (lane & 31);
     return t >= g.reach.first && t < g.t1 ? a.tables[g.at.row * a.table_stride + line.page.of((uint32_t)t)] : -1;
   };
+  // Where the pages are multiples of 16 tokens, a tile's half has one base, and these lie beyond it.
+  constexpr bool HALVES = VL % 2 == 0;  // (else a load of V takes tokens of both)
+  const bool near = HALVES && line.near && full;
+  const uint32_t k_off = col * (line.token16 << 4) + 16 * grp;
+  uint32_t v_off[HALVES ? VL / 2 : 1];
+#pragma unroll
+  for (int i = 0; i < (HALVES ? VL / 2 : 0); ++i) {
+    const int n = i * 64 + lane, u = n / VP, piece = n - u * VP;
+    v_off[i] = u * (line.token16 << 4) + 16 * piece;
+  }
   uint4 kr[2][KL], vr[VL];
   uint32_t valid = 0, code = 0;  // tokens of the tile that there are; the scale code of the lane's token
   // Starts the loads of a tile whose pages are known.
@@ -315,29 +335,34 @@ __global__ __launch_bounds__(64 * kWaves, (kPerCu<DS, F8, BF16>)) void attend_ke
     }
     const uint8_t* const kbase = a.cache.k + g.head * a.cache.head_stride;
     const uint8_t* const vbase = a.cache.v + g.head * a.cache.head_stride;
-    // (values past the head's are not read; V's of tokens that are not there are zero, for a weight of zero
-    // does not undo a NaN)
-    auto both = [&](auto check) __attribute__((always_inline)) {
+    if (near && valid == 0xffffffffu) {
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const uint8_t* p = kbase + ((uint64_t)(uint32_t)__shfl((int)off, 16 * h + col, 64) << 4);
+        const uint64_t at = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)off, 16 * h) << 4;
 #pragma unroll
-        for (int s = 0; s < KL; ++s) {
-          const uint32_t d = (F8 ? 64 : 32) * s + (F8 ? 16 : 8) * grp;
-          const bool in = !decltype(check)::value || d < dim;
-          kr[h][s] = in ? ldg16(p + (F8 ? d : 2 * d)) : make_uint4(0, 0, 0, 0);
-        }
-      }
+        for (int s = 0; s < KL; ++s) kr[h][s] = ldg16(kbase + at + (k_off + 64 * s));
 #pragma unroll
-      for (int i = 0; i < VL; ++i) {
-        const int n = i * 64 + lane, u = n / VP, piece = n - u * VP;
-        const uint8_t* p = vbase + ((uint64_t)(uint32_t)__shfl((int)off, u, 64) << 4) + 16 * piece;
-        const bool in = !decltype(check)::value || (valid >> u & 1 && piece * (F8 ? 16u : 8u) < dim);
-        vr[i] = in ? ldg16(p) : make_uint4(0, 0, 0, 0);
+        for (int i = 0; i < VL / 2; ++i) vr[h * (VL / 2) + i] = ldg16(vbase + at + v_off[HALVES ? i : 0]);
       }
-    };
-    if (full && valid == 0xffffffffu) both(std::false_type{});
-    else both(std::true_type{});
+      return;
+    }
+    // (values past the head's are not read; V's of tokens that are not there are zero, for a weight of zero
+    // does not undo a NaN)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const uint8_t* p = kbase + ((uint64_t)(uint32_t)__shfl((int)off, 16 * h + col, 64) << 4);
+#pragma unroll
+      for (int s = 0; s < KL; ++s) {
+        const uint32_t d = (F8 ? 64 : 32) * s + (F8 ? 16 : 8) * grp;
+        kr[h][s] = d < dim ? ldg16(p + (F8 ? d : 2 * d)) : make_uint4(0, 0, 0, 0);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < VL; ++i) {
+      const int n = i * 64 + lane, u = n / VP, piece = n - u * VP;
+      const uint8_t* p = vbase + ((uint64_t)(uint32_t)__shfl((int)off, u, 64) << 4) + 16 * piece;
+      vr[i] = valid >> u & 1 && piece * (F8 ? 16u : 8u) < dim ? ldg16(p) : make_uint4(0, 0, 0, 0);
+    }
   };
 
   // Queries, in the order of the operand (an E4M3 step takes eight of sixteen neighbours): read ahead, put
@@ -377,6 +402,9 @@ __global__ __launch_bounds__(64 * kWaves, (kPerCu<DS, F8, BF16>)) void attend_ke
   };
 
   Segment g = segment_at(unit_begin);
+  // Pages are known a segment, or two tiles, before their loads begin.
+  int tile = g.t0 + kTile * wave;
+  const int first_page = g.there ? page_of(g, tile) : -1;
   if (!line.by_pair && tid == 0) {
     // the share's first boundary, for the second kernel
     const uint32_t last = shares.of(g.at.end - 1);
@@ -384,18 +412,15 @@ __global__ __launch_bounds__(64 * kWaves, (kPerCu<DS, F8, BF16>)) void attend_ke
     line.joins[blockIdx.x] = Join{g.at.row, g.at.pair, blockIdx.x - 1, second ? last - blockIdx.x + 2 : 0};
   }
   if (!g.there) return;
-  // Pages are known a segment, or two tiles, before their loads begin.
+  int next_page = page_of(g, tile + kStep);
   load_q(g);
-  int tile = g.t0 + kTile * wave;
-  int next_page = page_of(g, tile + kUnit);
-  const int first_page = page_of(g, tile);
   Segment next = segment_at(g.stop);
   int page0 = -1, page1 = -1, next_tile = 0;
   auto pages_of_next = [&]() {
     if (!next.there) return;
     next_tile = next.t0 + kTile * wave;
     page0 = page_of(next, next_tile);
-    page1 = page_of(next, next_tile + kUnit);
+    page1 = page_of(next, next_tile + kStep);
   };
   pages_of_next();
   if (tile < g.t1) load(g, tile, first_page);
@@ -425,7 +450,7 @@ __global__ __launch_bounds__(64 * kWaves, (kPerCu<DS, F8, BF16>)) void attend_ke
 
     do {
       // (a wave without a tile in the segment comes here once, for the loads)
-      const bool have = tile < g.t1, stay = tile + kUnit < g.t1;
+      const bool have = tile < g.t1, stay = tile + kStep < g.t1;
       const uint32_t now = valid, now_code = code;
       // scores
       f32x4 s[2];
@@ -468,9 +493,9 @@ __global__ __launch_bounds__(64 * kWaves, (kPerCu<DS, F8, BF16>)) void attend_ke
       }
       if (stay || goes_on) {
         const Segment& to = stay ? g : next;
-        const int to_tile = stay ? tile + kUnit : next_tile;
+        const int to_tile = stay ? tile + kStep : next_tile;
         const int page = stay ? next_page : page0;
-        next_page = stay ? page_of(g, tile + 2 * kUnit) : page1;
+        next_page = stay ? page_of(g, tile + 2 * kStep) : page1;
         if (to_tile < to.t1) load(to, to_tile, page);
       }
       if (!have) break;
@@ -523,7 +548,7 @@ __global__ __launch_bounds__(64 * kWaves, (kPerCu<DS, F8, BF16>)) void attend_ke
           o[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, w[k], o[j], 0, 0, 0);
       }
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-      tile += kUnit;
+      tile += kStep;
     } while (tile < g.t1);
 
     // the waves' sums, joined
@@ -692,6 +717,7 @@ Line line_of(const AttendArgs& a) {
   line.page = PageDivision::by(a.cache.page);
   line.page16 = (uint32_t)(a.cache.page_stride >> 4);
   line.token16 = (uint32_t)(a.cache.token_stride >> 4);
+  line.near = a.cache.page % 16 == 0 && a.cache.token_stride < 1u << 27;
   return line;
 }
 

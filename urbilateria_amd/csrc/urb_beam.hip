@@ -62,14 +62,14 @@ __device__ __forceinline__ void load4(float (&v)[4], const uint8_t* row, int i, 
   }
 }
 
-// exp(l - m) for l <= m finite: l - m = n ln 2 / 64 + r with |r| <= ln(2) / 128, 2^(n / 64) by a table in LDS
+// z + exp(l - m) for l <= m finite: l - m = n ln 2 / 64 + r with |r| <= ln(2) / 128, 2^(n / 64) by a table in LDS
 // and the Taylor series to r^4, which leaves out 4e-14 of it.  Logits far below, of -inf and NaN count as
 // exp(-60): all the vocabulary's together are no 2^-50 of the largest's 1.
 constexpr int kPowers = 64;
 __device__ __forceinline__ void fill_powers(double* powers) {
   if (threadIdx.x < kPowers) powers[threadIdx.x] = exp2((double)threadIdx.x / kPowers);
 }
-__device__ __forceinline__ double mass(float l, double m, const double* powers) {
+__device__ __forceinline__ double add_mass(double z, float l, double m, const double* powers) {
   const double x = fmax((double)l - m, -60.0);
   const double magic = 0x1.8p52;  // adding it leaves an integer in the low bits
   const double t = fma(x, 0x1.71547652b82fep+6, magic);  // 64 / ln 2
@@ -81,7 +81,7 @@ __device__ __forceinline__ double mass(float l, double m, const double* powers) 
   // the table's value times 2^(n / 64): a sum in its exponent
   const long long p = __double_as_longlong(powers[n & (kPowers - 1)]) + ((long long)(n >> 6) << 52);
   const double q = __longlong_as_double(p);
-  return fma(s * r, q, q);
+  return fma(q, fma(s, r, 1.0), z);
 }
 
 // The upper half of the n-th largest key of a wave's lanes; 0 where fewer lanes have one.
@@ -91,6 +91,21 @@ __device__ __forceinline__ uint32_t wave_nth(uint32_t key, int n) {
   for (uint32_t bit = 1u << 31; bit > 0xffffu; bit >>= 1)
     if (__popcll(__ballot(key >= (t | bit))) >= n) t |= bit;
   return t;
+}
+
+// Calls with(item, how many of list[0 .. n - 1] are before it) for every item, in a lane 0: a wave per item in
+// turn, a lane for each of the others.
+template <int WAVES, class T, class Before, class With>
+__device__ __forceinline__ void rank_all(const T* list, int n, Before before, With with) {
+  const int lane = threadIdx.x & 63;
+  T others = lane < n ? list[lane] : T{};
+#pragma unroll 2
+  for (int i = threadIdx.x >> 6; i < n; i += WAVES) {
+    const T mine = list[i];
+    int above = __popcll(__ballot(lane < n && before(others, mine)));
+    for (int j = 64 + lane; j - lane < n; j += 64) above += __popcll(__ballot(j < n && before(list[j], mine)));
+    if (lane == 0) with(mine, above);
+  }
 }
 
 // A workgroup per slice (of PER logits per thread) and beam.
@@ -108,7 +123,7 @@ __global__ __launch_bounds__(kThreads) void beam_slice_kernel(BeamArgs a) {
   if (a.ended && a.ended[beam]) return;  // its logits count for nothing
   const uint8_t* row = reinterpret_cast<const uint8_t*>(a.logits) + beam * a.row_stride * (BF16 ? 2 : 4);
   const bool wide = reinterpret_cast<uintptr_t>(row) % (BF16 ? 8 : 16) == 0;
-  const int base = slice * (PER * kThreads) + 4 * tid;
+  const int base = slice * (PER * kThreads) + 4 * tid, item = beam * a.slices + slice;
   auto index = [&](int k, int j) { return base + k * 4 * kThreads + j; };
   float v[PER / 4][4];
 #pragma unroll
@@ -164,17 +179,15 @@ __global__ __launch_bounds__(kThreads) void beam_slice_kernel(BeamArgs a) {
 #pragma unroll
     for (int k = 0; k < PER / 4; ++k)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) z += mass(v[k][j], md, powers);
+      for (int j = 0; j < 4; ++j) z = add_mass(z, v[k][j], md, powers);
   }
   for (int o = 32; o > 0; o >>= 1) z += __shfl_xor(z, o, 64);
   if ((tid & 63) == 0) s_z[wave] = z;
   __syncthreads();
-  if (head) {
-    const int n = n_heads;
-    int above = 0;
-    for (int i = 0; i < n; ++i) above += list[i] > best;
-    if (above == a.picks - 1) s_least = best;
-  }
+  auto above = [](u64 x, u64 y) { return x > y; };
+  rank_all<WAVES>(list, n_heads, above, [&](u64 x, int n) {
+    if (n == a.picks - 1) s_least = x;
+  });
   __syncthreads();
   const u64 least = s_least;  // 0: fewer threads than that have any
   const float least_value = least ? key_value((uint32_t)(least >> 32)) : -kInf;
@@ -190,18 +203,15 @@ __global__ __launch_bounds__(kThreads) void beam_slice_kernel(BeamArgs a) {
         }
   __syncthreads();
   const int n = n_list;
-  u64* out = a.keys + ((size_t)beam * a.slices + slice) * a.picks;
-  for (int i = tid; i < n; i += kThreads) {
-    const u64 mine = list[i];
-    int above = 0;
-    for (int j = 0; j < n; ++j) above += list[j] > mine;
-    if (above < a.picks) out[above] = mine;
-  }
+  u64* out = a.keys + (size_t)item * a.picks;
+  rank_all<WAVES>(list, n, above, [&](u64 x, int place) {
+    if (place < a.picks) out[place] = x;
+  });
   for (int i = n + tid; i < a.picks; i += kThreads) out[i] = 0;
   if (tid == 0) {
     double sum = 0.0;
     for (int w = 0; w < WAVES; ++w) sum += s_z[w];
-    a.sums[(size_t)beam * a.slices + slice] = BeamSum{sum, m, 0};
+    a.sums[item] = BeamSum{sum, m, 0};
   }
 }
 
@@ -250,7 +260,7 @@ __global__ __launch_bounds__(THREADS) void beam_join_kernel(BeamArgs a, int span
   for (int o = span * team / 2; o >= team; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
   double z = 0.0;
   if (m == kInf) z = own == kInf ? sum.z : 0.0;
-  else if (own > -kInf) z = sum.z * mass(own, (double)m, powers);
+  else if (own > -kInf) z = sum.z * add_mass(0.0, own, (double)m, powers);
   for (int o = span * team / 2; o >= team; o >>= 1) z += __shfl_xor(z, o, 64);
   const bool bad = !(score <= 3.4028235e38f);  // NaN, +inf
   const int live = bad || !(score > -kInf) ? 0 : end ? 2 : m > -kInf ? 1 : 0;
@@ -282,12 +292,9 @@ __global__ __launch_bounds__(THREADS) void beam_join_kernel(BeamArgs a, int span
   const bool head = key && key >= bound;
   if (head) list[atomicAdd(&n_heads, 1)] = first;
   __syncthreads();
-  if (head) {
-    const int n = n_heads;
-    int above = 0;
-    for (int i = 0; i < n; ++i) above += better(list[i], first);
-    if (above == a.picks - 1) s_least = first;
-  }
+  rank_all<WAVES>(list, n_heads, better, [&](const Candidate& c, int above) {
+    if (above == a.picks - 1) s_least = c;
+  });
   __syncthreads();
   const Candidate least = s_least;
   // (lists are in order: behind one that falls short there is nothing)
@@ -306,19 +313,15 @@ __global__ __launch_bounds__(THREADS) void beam_join_kernel(BeamArgs a, int span
   __syncthreads();
   const int n = n_list;
   const size_t out = (size_t)r * a.picks;
-  for (int i = tid; i < n; i += THREADS) {
-    const Candidate c = list[i];
-    int above = 0;
-    for (int j = 0; j < n; ++j) above += better(list[j], c);
-    if (above < a.picks) {
-      const int parent = (int)(c.at / (uint32_t)a.vocab);
-      const int token = (int)(c.at - (uint32_t)parent * a.vocab);
-      a.scores_out[out + above] = (float)c.score;
-      a.tokens[out + above] = token;
-      a.parents[out + above] = parent;
-      if (a.ended_out) a.ended_out[out + above] = s_live[parent] == 2 || token == a.end_token;
-    }
-  }
+  rank_all<WAVES>(list, n, better, [&](const Candidate& c, int place) {
+    if (place >= a.picks) return;
+    const int parent = (int)(c.at / (uint32_t)a.vocab);
+    const int token = (int)(c.at - (uint32_t)parent * a.vocab);
+    a.scores_out[out + place] = (float)c.score;
+    a.tokens[out + place] = token;
+    a.parents[out + place] = parent;
+    if (a.ended_out) a.ended_out[out + place] = s_live[parent] == 2 || token == a.end_token;
+  });
   for (int i = n + tid; i < a.picks; i += THREADS) {
     a.scores_out[out + i] = -kInf;
     a.tokens[out + i] = -1;
@@ -337,9 +340,8 @@ int span_of(int slices) {
   return span;
 }
 
-// Short slices while they are no more workgroups than the chip has at a time (and a request's fit the join, a
-// beam's a wave of it): 4 beams over 50257 BF16 logits take @@ us with them and @@ without, 256 over 129280 f32
-// logits would take @@ and take @@.
+// Short slices while they are no more workgroups than four per CU (and a request's fit the join, a beam's a
+// wave of it): 4 beams over 50257 BF16 logits take 11.9 us with them and 16.4 without, 40 of them 13.8 and 18.1.
 bool short_slices(int vocab, int width, int requests) {
   const int64_t slices = slices_of(vocab, kBeamShortSlice);
   return slices <= 64 && span_of((int)slices) * width <= 1024 && slices * width * requests <= 1024;

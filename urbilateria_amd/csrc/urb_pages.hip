@@ -467,9 +467,15 @@ __global__ __launch_bounds__(256) void fork_tables_kernel(ForkArgs a) {
           continue;
         }
         // held by no row with children, and by no lower row without
+        const uint64_t others = held & (used | ((1ull << i) - 1));
         bool gone = true;
-        for (uint64_t others = held & (used | ((1ull << i) - 1)); others && gone; others &= others - 1)
-          gone = column[(__ffsll((unsigned long long)others) - 1) * 256 + tid] != page;
+        for (int j0 = 0; j0 < width; j0 += 8) {
+          int e[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) e[j] = column[min(j0 + j, width - 1) * 256 + tid];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) gone = gone && !(others >> (j0 + j) & 1 && e[j] == page);
+        }
         if (gone) drop |= 1ull << i;
       }
     }
