@@ -69,7 +69,8 @@ struct ForkCopy {
   uint32_t from, to, tokens;  // pages; 0 tokens: nothing
 };
 struct ForkArgs {
-  uint32_t requests, width, page, pages, max_blocks;
+  uint32_t requests, width, pages, max_blocks;
+  PageDivision page;
   uint64_t table_stride, table_out_stride;
   const int32_t *parents, *tables, *lengths;
   int32_t *tables_out, *lengths_out;

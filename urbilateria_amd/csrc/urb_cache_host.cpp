@@ -230,7 +230,7 @@ urb_status urb_pager_fork(urb_pager* c, const urb_page_fork* f, void* stream) {
     urb::ForkArgs a{};
     a.requests = f->requests;
     a.width = f->width;
-    a.page = d.page_size;
+    a.page = urb::PageDivision::by(d.page_size);
     a.pages = d.pages;
     a.max_blocks = d.max_blocks;
     a.table_stride = f->table_stride;

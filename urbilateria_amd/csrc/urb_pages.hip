@@ -319,19 +319,16 @@ __global__ __launch_bounds__(256) void plan_tokens_kernel(PlanArgs a) {
 
 // ---- tables that follow their beams ----
 
-__device__ __forceinline__ uint32_t blocks_of(int length, uint32_t page) {
-  return (uint32_t)(length + page - 1) / page;
-}
-
 // The rows of a request that take a copy of their parent's last page, one filled in part that stays with a
 // lower child; a whole wave, one row per lane.
 __device__ __forceinline__ uint64_t copying_rows(const int* parent, const int* length, int width,
-                                                 uint32_t page) {
+                                                 const PageDivision& page) {
   const int i = threadIdx.x & 63;
   const int p = i < width ? parent[i] : -1;
   bool lower = false;
   for (int j = 0; j < width; ++j) lower |= j < i && parent[j] == p;
-  return __ballot(p >= 0 && lower && length[p < 0 ? 0 : p] % page != 0);
+  const uint32_t n = (uint32_t)length[p < 0 ? 0 : p];
+  return __ballot(p >= 0 && lower && page.of(n) * page.size != n);
 }
 
 // The pages, lengths and stack of a request's rows, when all requests' dropped pages and copies are known:
@@ -393,11 +390,11 @@ __device__ __forceinline__ void fork_books(const ForkArgs& a, const int* parent,
         }
         to = a.dropped[(uint64_t)q * a.width * a.max_blocks + (want - (q ? s_upto[q - 1] : 0))];
       }
-      const uint32_t last = (uint32_t)length[p] / a.page;
+      const uint32_t last = a.page.of((uint32_t)length[p]);
       const int from = a.tables[(uint64_t)(row0 + p) * a.table_stride + last];
       a.tables_out[(uint64_t)(row0 + tid) * a.table_out_stride + last] = to;
       if ((uint32_t)to >= a.pages || (uint32_t)from >= a.pages) flag(a.status, kCacheArgument);
-      else copy = ForkCopy{(uint32_t)from, (uint32_t)to, (uint32_t)length[p] % a.page};
+      else copy = ForkCopy{(uint32_t)from, (uint32_t)to, (uint32_t)length[p] - last * a.page.size};
     }
   }
   a.page_copies[row0 + tid] = copy;
@@ -410,33 +407,40 @@ template <bool ALONE>
 __global__ __launch_bounds__(256) void fork_tables_kernel(ForkArgs a) {
   extern __shared__ int column[];  // [width][256]
   __shared__ int parent[kForkWidth], length[kForkWidth];
+  __shared__ uint32_t blocks[kForkWidth];
+  __shared__ unsigned long long s_used;  // rows with a child
+  __shared__ uint32_t s_columns;
   __shared__ int64_t slots[4];
   const uint32_t r = blockIdx.x, row0 = r * a.width;
   const int tid = threadIdx.x, width = (int)a.width;
   int bits = 0;
+  if (tid == 0) {
+    s_used = 0;
+    s_columns = 0;
+  }
+  __syncthreads();
   if (tid < width) {
     int p = a.parents[row0 + tid];
     if (p >= width) bits |= kCacheArgument;
     parent[tid] = p < 0 || p >= width ? -1 : p;
     int n = a.lengths[row0 + tid];
-    if (n < 0 || (int64_t)n > (int64_t)a.max_blocks * a.page) {
+    if (n < 0 || (int64_t)n > (int64_t)a.max_blocks * a.page.size) {
       bits |= kCacheArgument;
       n = 0;
     }
     length[tid] = n;
     a.old_lengths[row0 + tid] = n;
+    blocks[tid] = a.page.up((uint32_t)n);
+    if (parent[tid] >= 0) atomicOr(&s_used, 1ull << parent[tid]);
+    atomicMax(&s_columns, blocks[tid]);
   }
   __syncthreads();
   if (tid < 64) {
     const uint64_t copies = copying_rows(parent, length, width, a.page);
     if (tid == 0) a.copies[r] = __popcll(copies);
   }
-  uint64_t used = 0;  // rows with a child
-  uint32_t columns = 0;
-  for (int i = 0; i < width; ++i) {
-    if (parent[i] >= 0) used |= 1ull << parent[i];
-    columns = max(columns, blocks_of(length[i], a.page));
-  }
+  const uint64_t used = s_used;
+  const uint32_t columns = s_columns;
   const int32_t* in = a.tables + row0 * a.table_stride;
   int32_t* out = a.tables_out + row0 * a.table_out_stride;
   int32_t* list = a.dropped + (uint64_t)row0 * a.max_blocks;
@@ -444,8 +448,8 @@ __global__ __launch_bounds__(256) void fork_tables_kernel(ForkArgs a) {
   for (uint32_t c0 = 0; c0 < columns; c0 += 256) {
     const uint32_t c = c0 + tid;
     uint64_t held = 0, drop = 0;
-    for (int i = 0; i < width; ++i)
-      if (c < blocks_of(length[i], a.page)) held |= 1ull << i;
+#pragma unroll 8
+    for (int i = 0; i < width; ++i) held |= (uint64_t)(c < blocks[i]) << i;
     if (held) {
       // the column in LDS (each thread its own): eight loads on their way at a time
       for (int i0 = 0; i0 < width; i0 += 8) {
@@ -601,7 +605,7 @@ void launch_fork(const ForkArgs& a, const KvCache* caches, uint32_t n_caches, hi
     uint64_t bytes = 0;
     for (uint32_t i = 0; i < n; ++i) {
       some.c[i] = caches[done + i];
-      bytes = std::max<uint64_t>(bytes, 2ull * caches[done + i].heads * a.page * caches[done + i].dim);
+      bytes = std::max<uint64_t>(bytes, 2ull * caches[done + i].heads * a.page.size * caches[done + i].dim);
     }
     // parts of a page: four pieces for every lane where the cache is the largest, while that is no more than
     // 64 workgroups per CU
