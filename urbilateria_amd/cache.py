@@ -106,12 +106,18 @@ class PagedCache:
         """Writes rows ``k`` and ``v`` [T, heads, head_dim] (torch.bfloat16 or torch.float32; tokens and
         heads may be strided, as in a fused q/k/v row) into the slots ``slots`` [T] int64; slots outside
         the cache, such as -1, skip their token."""
-        shape = (k.shape[0], self.heads, self.head_dim)
-        rows = N.KvRows(k.data_ptr(), v.data_ptr(), _type(k.dtype),
-                        *_strides(k, "k", shape, k.dtype, self.device),
-                        *_strides(v, "v", shape, k.dtype, self.device))
-        at = _vector(slots, "slots", shape[0], torch.int64, self.device)
-        _call("urb_kv_append", self.device, stream, self._ref, ctypes.byref(rows), at, shape[0])
+        tokens, dtype, dev = k.shape[0], k.dtype, self.device
+        shape = (tokens, self.heads, self.head_dim)
+        if k.shape != shape or v.shape != shape or v.dtype is not dtype or k.get_device() != dev or (
+                v.get_device() != dev):
+            raise ValueError(f"k and v must be {list(shape)} tensors of one type on cuda:{dev}")
+        k_token, k_head, k_value = k.stride()
+        v_token, v_head, v_value = v.stride()
+        if k_value != 1 or v_value != 1:
+            raise ValueError("k, v: the values of a head must be contiguous")
+        rows = N.KvRows(k.data_ptr(), v.data_ptr(), _type(dtype), k_token, k_head, v_token, v_head)
+        _call("urb_kv_append", dev, stream, self._ref, ctypes.byref(rows),
+              _vector(slots, "slots", tokens, torch.int64, dev), tokens)
 
 
 class Plan:

@@ -65,7 +65,6 @@ struct Line {
   Join* joins;            // [shares]
   PageDivision page;
   uint32_t page16, token16;  // strides in units of 16 bytes
-  bool near;                 // 16 tokens from a multiple of 16 on lie at one distance, in less than 2^32 bytes
 };
 
 // The tokens in reach of any query of a row, [first, end), and first rounded down to a tile; a length that
@@ -135,21 +134,39 @@ __device__ __forceinline__ uint32_t quotient(uint32_t n, uint32_t d) {
 struct Place {
   uint32_t row, pair, units, first, end;
 };
+// (A whole wave searches: the last of every sixteen rows, then the rows of one sixteen.)
 __device__ __forceinline__ Place place_of(const uint32_t* upto, uint32_t rows, uint32_t pairs, uint32_t unit) {
-  uint32_t lo = 0, hi = rows - 1;  // the first row whose units end beyond
-  while (lo < hi) {
-    const uint32_t mid = (lo + hi) / 2;
-    if (same(upto[mid]) * pairs > unit) hi = mid;
-    else lo = mid + 1;
-  }
-  const uint32_t under = lo ? same(upto[lo - 1]) : 0;
+  const uint32_t lane = threadIdx.x & 63;
+  static_assert(kAttendRows == 64 * 16, "two steps");
+  // rows whose units all lie before
+  const uint32_t whole = __popcll(__ballot(16 * lane + 15 < rows && upto[16 * lane + 15] * pairs <= unit)) * 16;
+  const uint32_t row = whole + lane;
+  const uint32_t mine = lane < 16 && row < rows ? upto[row] : 0xffffffffu;
+  const uint32_t more = __popcll(__ballot(mine != 0xffffffffu && mine * pairs <= unit));
   Place p;
-  p.row = lo;
-  p.units = same(upto[lo]) - under;
+  p.row = whole + more;
+  const uint32_t to = (uint32_t)__builtin_amdgcn_readlane((int)mine, (int)more);
+  const uint32_t under = more ? (uint32_t)__builtin_amdgcn_readlane((int)mine, (int)more - 1)
+                              : whole ? same(upto[whole - 1]) : 0;
+  p.units = to - under;
   const uint32_t start = under * pairs;
   p.pair = quotient(unit - start, p.units);
   p.end = start + (p.pair + 1) * p.units;
   p.first = p.end - p.units + kStart;
+  return p;
+}
+// The place behind a pair, if there is one.
+__device__ __forceinline__ Place place_after(const uint32_t* upto, uint32_t pairs, const Place& at) {
+  Place p = at;
+  if (at.pair + 1 < pairs) {
+    ++p.pair;
+  } else {
+    p.pair = 0;
+    p.row = at.row + 1;
+    p.units = same(upto[p.row]) - same(upto[at.row]);
+  }
+  p.end = at.end + p.units;
+  p.first = at.end + kStart;
   return p;
 }
 
@@ -244,7 +261,7 @@ __device__ __forceinline__ void finish4(const AttendArgs& a, uint32_t row, const
 // the last ones to run by themselves: 64 rows of 4096 tokens of 8 heads of 128 in E4M3 take 100 us with 512 and
 // 143 with 768; f32 rows of 128 over BF16 have 5.55 TB/s with one per CU.)
 template <int DS, bool F8, bool BF16>
-constexpr int kPerCu = DS == 2 && F8 ? 3 : DS <= 3 || (DS == 4 && (F8 || BF16)) ? 2 : 1;
+constexpr int kPerCu = DS == 2 && F8 ? 3 : DS <= 3 || (DS == 4 && (F8 || BF16)) || (DS == 6 && F8) ? 2 : 1;
 
 // DS: head_dim in steps of 32, rounded up.
 template <int DS, bool F8, bool BF16>
@@ -288,11 +305,9 @@ __global__ __launch_bounds__(64 * kWaves, (kPerCu<DS, F8, BF16>)) void attend_ke
     uint32_t head;
     bool begins, there;
   };
-  auto segment_at = [&](uint32_t unit) -> Segment {
+  auto segment_of = [&](const Place& at, uint32_t unit) -> Segment {
     Segment g;
-    g.there = unit < unit_end;
-    if (!g.there) return g;
-    g.at = place_of(upto, a.rows, line.pairs, unit);
+    g.at = at;
     g.there = unit_end > g.at.first;
     g.reach = reach_of(a, same(lengths[g.at.row]));
     g.begins = unit <= g.at.first;
@@ -308,16 +323,6 @@ __global__ __launch_bounds__(64 * kWaves, (kPerCu<DS, F8, BF16>)) void attend_ke
     const int t = tile + (lane & 31);
     return t >= g.reach.first && t < g.t1 ? a.tables[g.at.row * a.table_stride + line.page.of((uint32_t)t)] : -1;
   };
-  // Where the pages are multiples of 16 tokens, a tile's half has one base, and these lie beyond it.
-  constexpr bool HALVES = VL % 2 == 0;  // (else a load of V takes tokens of both)
-  const bool near = HALVES && line.near && full;
-  const uint32_t k_off = col * (line.token16 << 4) + 16 * grp;
-  uint32_t v_off[HALVES ? VL / 2 : 1];
-#pragma unroll
-  for (int i = 0; i < (HALVES ? VL / 2 : 0); ++i) {
-    const int n = i * 64 + lane, u = n / VP, piece = n - u * VP;
-    v_off[i] = u * (line.token16 << 4) + 16 * piece;
-  }
   uint4 kr[2][KL], vr[VL];
   uint32_t valid = 0, code = 0;  // tokens of the tile that there are; the scale code of the lane's token
   // Starts the loads of a tile whose pages are known.
@@ -335,34 +340,29 @@ __global__ __launch_bounds__(64 * kWaves, (kPerCu<DS, F8, BF16>)) void attend_ke
     }
     const uint8_t* const kbase = a.cache.k + g.head * a.cache.head_stride;
     const uint8_t* const vbase = a.cache.v + g.head * a.cache.head_stride;
-    if (near && valid == 0xffffffffu) {
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const uint64_t at = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)off, 16 * h) << 4;
-#pragma unroll
-        for (int s = 0; s < KL; ++s) kr[h][s] = ldg16(kbase + at + (k_off + 64 * s));
-#pragma unroll
-        for (int i = 0; i < VL / 2; ++i) vr[h * (VL / 2) + i] = ldg16(vbase + at + v_off[HALVES ? i : 0]);
-      }
-      return;
-    }
     // (values past the head's are not read; V's of tokens that are not there are zero, for a weight of zero
     // does not undo a NaN)
+    auto both = [&](auto check) __attribute__((always_inline)) {
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const uint8_t* p = kbase + ((uint64_t)(uint32_t)__shfl((int)off, 16 * h + col, 64) << 4);
+      for (int h = 0; h < 2; ++h) {
+        const uint8_t* p = kbase + ((uint64_t)(uint32_t)__shfl((int)off, 16 * h + col, 64) << 4);
 #pragma unroll
-      for (int s = 0; s < KL; ++s) {
-        const uint32_t d = (F8 ? 64 : 32) * s + (F8 ? 16 : 8) * grp;
-        kr[h][s] = d < dim ? ldg16(p + (F8 ? d : 2 * d)) : make_uint4(0, 0, 0, 0);
+        for (int s = 0; s < KL; ++s) {
+          const uint32_t d = (F8 ? 64 : 32) * s + (F8 ? 16 : 8) * grp;
+          const bool in = !decltype(check)::value || d < dim;
+          kr[h][s] = in ? ldg16(p + (F8 ? d : 2 * d)) : make_uint4(0, 0, 0, 0);
+        }
       }
-    }
 #pragma unroll
-    for (int i = 0; i < VL; ++i) {
-      const int n = i * 64 + lane, u = n / VP, piece = n - u * VP;
-      const uint8_t* p = vbase + ((uint64_t)(uint32_t)__shfl((int)off, u, 64) << 4) + 16 * piece;
-      vr[i] = valid >> u & 1 && piece * (F8 ? 16u : 8u) < dim ? ldg16(p) : make_uint4(0, 0, 0, 0);
-    }
+      for (int i = 0; i < VL; ++i) {
+        const int n = i * 64 + lane, u = n / VP, piece = n - u * VP;
+        const uint8_t* p = vbase + ((uint64_t)(uint32_t)__shfl((int)off, u, 64) << 4) + 16 * piece;
+        const bool in = !decltype(check)::value || (valid >> u & 1 && piece * (F8 ? 16u : 8u) < dim);
+        vr[i] = in ? ldg16(p) : make_uint4(0, 0, 0, 0);
+      }
+    };
+    if (full && valid == 0xffffffffu) both(std::false_type{});
+    else both(std::true_type{});
   };
 
   // Queries, in the order of the operand (an E4M3 step takes eight of sixteen neighbours): read ahead, put
@@ -401,7 +401,7 @@ __global__ __launch_bounds__(64 * kWaves, (kPerCu<DS, F8, BF16>)) void attend_ke
     }
   };
 
-  Segment g = segment_at(unit_begin);
+  Segment g = segment_of(place_of(upto, a.rows, line.pairs, unit_begin), unit_begin);
   // Pages are known a segment, or two tiles, before their loads begin.
   int tile = g.t0 + kTile * wave;
   const int first_page = g.there ? page_of(g, tile) : -1;
@@ -414,7 +414,13 @@ __global__ __launch_bounds__(64 * kWaves, (kPerCu<DS, F8, BF16>)) void attend_ke
   if (!g.there) return;
   int next_page = page_of(g, tile + kStep);
   load_q(g);
-  Segment next = segment_at(g.stop);
+  auto segment_after = [&](const Segment& g) -> Segment {
+    if (g.stop < unit_end) return segment_of(place_after(upto, line.pairs, g.at), g.stop);
+    Segment none = g;
+    none.there = false;
+    return none;
+  };
+  Segment next = segment_after(g);
   int page0 = -1, page1 = -1, next_tile = 0;
   auto pages_of_next = [&]() {
     if (!next.there) return;
@@ -455,22 +461,28 @@ __global__ __launch_bounds__(64 * kWaves, (kPerCu<DS, F8, BF16>)) void attend_ke
       // scores
       f32x4 s[2];
       if (have) {
+        float ks[2] = {0.0f, 0.0f};
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           s[h] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-          float ks = 0.0f;
-          if constexpr (F8) ks = e8m0_to_f32((uint32_t)__shfl((int)now_code, 16 * h + col, 64));
+          if constexpr (F8) ks[h] = e8m0_to_f32((uint32_t)__shfl((int)now_code, 16 * h + col, 64));
+        }
 #pragma unroll
-          for (int j = 0; j < KS; ++j) {
+        for (int j = 0; j < KS; ++j) {
+          bf16x8 q[QP];
+#pragma unroll
+          for (int p = 0; p < QP; ++p) q[p] = __builtin_bit_cast(bf16x8, q_lds[p][j][lane]);
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
             uint4 w;
             if constexpr (F8)
-              w = j & 1 ? decode8(kr[h][j / 2].z, kr[h][j / 2].w, ks) : decode8(kr[h][j / 2].x, kr[h][j / 2].y, ks);
+              w = j & 1 ? decode8(kr[h][j / 2].z, kr[h][j / 2].w, ks[h])
+                        : decode8(kr[h][j / 2].x, kr[h][j / 2].y, ks[h]);
             else w = kr[h][j];
             const bf16x8 k = __builtin_bit_cast(bf16x8, w);
 #pragma unroll
             for (int p = QP - 1; p >= 0; --p)
-              s[h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k, __builtin_bit_cast(bf16x8, q_lds[p][j][lane]),
-                                                             s[h], 0, 0, 0);
+              s[h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k, q[p], s[h], 0, 0, 0);
           }
         }
         // V into LDS, then the loads of the next tile
@@ -597,7 +609,7 @@ __global__ __launch_bounds__(64 * kWaves, (kPerCu<DS, F8, BF16>)) void attend_ke
     __syncthreads();
     g = next;
     tile = next_tile;
-    next = segment_at(g.stop);
+    next = segment_after(g);
     pages_of_next();
   }
 }
@@ -717,7 +729,6 @@ Line line_of(const AttendArgs& a) {
   line.page = PageDivision::by(a.cache.page);
   line.page16 = (uint32_t)(a.cache.page_stride >> 4);
   line.token16 = (uint32_t)(a.cache.token_stride >> 4);
-  line.near = a.cache.page % 16 == 0 && a.cache.token_stride < 1u << 27;
   return line;
 }
 
