@@ -525,6 +525,20 @@ def test_lengths_shared_out_over_the_chip(dtype, rows, lengths, q_heads, heads, 
     assert torch.equal(_bits(out), _bits(again[0])) and torch.equal(_bits(lse), _bits(again[1]))
 
 
+@pytest.mark.parametrize("dtype,rows,dim,page,queries", [
+    (BF16, BF16, 128, 24, 1), (BF16, F32, 96, 16, 3), (BF16, BF16, 80, 64, 1), (F8, BF16, 128, 7, 2),
+    (F8, F32, 192, 100, 1)])
+def test_more_than_the_caches_of_the_chip_hold(dtype, rows, dim, page, queries):
+    size = 1 if dtype == F8 else 2
+    n = (160 << 20) // (2 * 8 * dim * size)
+    lengths = [n // 2, 0, 1, n // 4 + 5, 33, n // 8, n // 8 + 130, 127]
+    c = Cached(lengths, 16, 8, dim, page, dtype, rows, queries)
+    out, lse = c.run()
+    c.check(out, lse, some=[1, 2, 4, 5, 6, 7])
+    again = c.run()
+    assert torch.equal(_bits(out), _bits(again[0])) and torch.equal(_bits(lse), _bits(again[1]))
+
+
 def test_more_rows_than_a_launch_takes():
     lengths = [(7 * r) % 50 for r in range(2100)]
     c = Cached(lengths, 2, 1, 32, 16)
@@ -668,6 +682,22 @@ def test_attention_on_another_stream():
     c.attention.sync(s)
     torch.cuda.synchronize()
     assert torch.equal(_bits(out), _bits(want))
+
+
+def test_two_contexts_at_once():
+    cases = [Cached([9000, 40, 0, 700], 8, 2, 128, 16, seed=5), Cached([6000, 1, 3000], 4, 4, 64, 24, F8, F32, seed=6)]
+    want = [c.run() for c in cases]
+    tensors = [(c.q.cuda(), c.tables.cuda(), _i32(c.lengths), torch.empty_like(w[0]), torch.empty_like(w[1]))
+               for c, w in zip(cases, want)]
+    streams = [torch.cuda.Stream() for _ in cases]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for c, (q, tables, n, out, lse), s in zip(cases, tensors, streams):
+            c.attention.attend_into(q, c.cache, tables, n, out, lse, stream=s)
+    torch.cuda.synchronize()
+    for c, (_, _, _, out, lse), w, s in zip(cases, tensors, want, streams):
+        c.attention.sync(s)
+        assert torch.equal(_bits(out), _bits(w[0])) and torch.equal(_bits(lse), _bits(w[1]))
 
 
 def test_attention_refuses():

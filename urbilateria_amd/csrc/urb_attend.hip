@@ -37,6 +37,10 @@ constexpr int kWaves = 4;
 constexpr int kStep = kTile * kWaves;  // tokens of a workgroup's step
 constexpr int kAttendRows = 1024;  // of a launch
 constexpr int kCus = 256;
+// Loads that leave the caches alone are faster (200 ragged rows, 985 MB: 178 us and 194; a row of 131071 tokens
+// of E4M3, 268 MB: 56.7 and 61.1) but for a cache that a later call finds in the 256 MB of the last level (24
+// rows, 35 MB, one call after another: 21.9 and 20.1).
+constexpr float kCachedBytes = 128.0f * 1048576.0f;
 constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
 constexpr float kMinusInf = -__builtin_inff();
 
@@ -284,7 +288,8 @@ __global__ __launch_bounds__(64 * kWaves, (kPerCu<DS, F8, BF16>)) void attend_ke
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 15, grp = lane >> 4;
   fill_line(a, upto, lengths, sums);
-  const Shares shares(same(upto[a.rows - 1]) * line.pairs, line.shares);
+  const uint32_t total = same(upto[a.rows - 1]) * line.pairs;
+  const Shares shares(total, line.shares);
   if (blockIdx.x >= shares.n) {
     if (!line.by_pair && tid == 0) line.joins[blockIdx.x].n = 0;
     return;
@@ -292,6 +297,9 @@ __global__ __launch_bounds__(64 * kWaves, (kPerCu<DS, F8, BF16>)) void attend_ke
   const uint32_t unit_begin = shares.begin(blockIdx.x), unit_end = shares.begin(blockIdx.x + 1);
   const float scale2 = a.scale * kLog2e;
   const uint32_t dim = a.cache.dim;
+  // Whether K and V pass the caches by: what one call reads once, a line in one load (rows of 160 bytes have 5.6
+  // TB/s and so 5.3), and is too much to be there at the next.
+  const bool once = line.tiles == 1 && dim * (F8 ? 1 : 2) % 64 == 0 && (float)total * (float)(kUnit * 2 * (F8 ? 1 : 2)) * (float)dim > kCachedBytes;
   const bool full = dim == (F8 ? 32 * KS : 32 * DS);
   uint8_t* const mine = stage[wave];
 
@@ -342,7 +350,8 @@ __global__ __launch_bounds__(64 * kWaves, (kPerCu<DS, F8, BF16>)) void attend_ke
     const uint8_t* const vbase = a.cache.v + g.head * a.cache.head_stride;
     // (values past the head's are not read; V's of tokens that are not there are zero, for a weight of zero
     // does not undo a NaN)
-    auto both = [&](auto check) __attribute__((always_inline)) {
+    auto both = [&](auto check, auto once) __attribute__((always_inline)) {
+      auto get = [](const uint8_t* p) { return decltype(once)::value ? ldg16_stream(p) : ldg16(p); };
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const uint8_t* p = kbase + ((uint64_t)(uint32_t)__shfl((int)off, 16 * h + col, 64) << 4);
@@ -350,7 +359,7 @@ __global__ __launch_bounds__(64 * kWaves, (kPerCu<DS, F8, BF16>)) void attend_ke
         for (int s = 0; s < KL; ++s) {
           const uint32_t d = (F8 ? 64 : 32) * s + (F8 ? 16 : 8) * grp;
           const bool in = !decltype(check)::value || d < dim;
-          kr[h][s] = in ? ldg16(p + (F8 ? d : 2 * d)) : make_uint4(0, 0, 0, 0);
+          kr[h][s] = in ? get(p + (F8 ? d : 2 * d)) : make_uint4(0, 0, 0, 0);
         }
       }
 #pragma unroll
@@ -358,11 +367,17 @@ __global__ __launch_bounds__(64 * kWaves, (kPerCu<DS, F8, BF16>)) void attend_ke
         const int n = i * 64 + lane, u = n / VP, piece = n - u * VP;
         const uint8_t* p = vbase + ((uint64_t)(uint32_t)__shfl((int)off, u, 64) << 4) + 16 * piece;
         const bool in = !decltype(check)::value || (valid >> u & 1 && piece * (F8 ? 16u : 8u) < dim);
-        vr[i] = in ? ldg16(p) : make_uint4(0, 0, 0, 0);
+        vr[i] = in ? get(p) : make_uint4(0, 0, 0, 0);
       }
     };
-    if (full && valid == 0xffffffffu) both(std::false_type{});
-    else both(std::true_type{});
+    const bool check = !full || valid != 0xffffffffu;
+    if (once) {
+      if (check) both(std::true_type{}, std::true_type{});
+      else both(std::false_type{}, std::true_type{});
+    } else {
+      if (check) both(std::true_type{}, std::false_type{});
+      else both(std::false_type{}, std::false_type{});
+    }
   };
 
   // Queries, in the order of the operand (an E4M3 step takes eight of sixteen neighbours): read ahead, put
