@@ -117,8 +117,9 @@ urb_status urb_pager_plan(urb_pager *pager, const urb_page_plan *plan, void *str
  * requests, columns and rows, before the new ones are taken off it, in the order of rows.  With all
  * parents negative a request ends and its pages are free.
  *
- * A page may stand in several rows of one request, in the same column, and in no two requests.  A row
- * for which no page is left ends with length 0, and the next urb_pager_sync returns
+ * A page may stand in several rows of one request, in the same column, and in no two requests; one that
+ * is filled in part in several rows at once (a prompt's last page in all the rows of a search that begins)
+ * if no more than one of them has children.  A row for which no page is left ends with length 0, and the next urb_pager_sync returns
  * URB_ERR_OUT_OF_MEMORY.  A length that is negative or above max_blocks * page_size counts as 0, a
  * parent of `width` or more as negative, an entry that is no page is neither put on the stack nor
  * copied, pages beyond a full stack are left out, a *free_count out of range counts as 0:
@@ -151,7 +152,7 @@ urb_status urb_pager_sync(urb_pager *pager, void *stream);
  * For row r of lengths[r] cached tokens, its last `queries` ones among them, and query token i of them:
  *   e_j = exp(scale q . k_j),  o = sum_j e_j v_j / (exp(sink) + sum_j e_j)
  * over j < n = lengths[r] - (queries - 1 - i), and j >= n - window if window > 0; without sinks that
- * term is 0.  Query head h reads cache head h / (q_heads / heads).  lse is the logarithm of the
+ * term is 0 (as with one of -inf; one of +inf leaves 0 of the values).  Query head h reads cache head h / (q_heads / heads).  lse is the logarithm of the
  * denominator; where that is 0, as with no j in reach, o is 0 and lse -inf.  Tokens that no query of the
  * row reaches are not used, whatever the cache holds there; an infinity or a NaN that one of its queries
  * reaches may come out of all of them.

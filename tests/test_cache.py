@@ -513,6 +513,20 @@ def test_sinks(dtype, rows, lengths):
     assert bool((out == 0).all()) and bool((lse == 1e4).all())
 
 
+@pytest.mark.parametrize("lengths", [[0], [40], [5, 0, 9000]])
+def test_infinite_sinks(lengths):
+    c = Cached(lengths, 4, 2, 64, 16, seed=8)
+    want, want_lse = c.run()
+    c.sinks = torch.tensor([math.inf, -math.inf, -math.inf, math.inf])
+    out, lse = c.run()
+    for h, s in enumerate(c.sinks.tolist()):
+        if s > 0:
+            assert bool((out[:, :, h] == 0).all()) and bool((lse[:, :, h] == math.inf).all())
+        else:
+            assert torch.equal(_bits(out[:, :, h].contiguous()), _bits(want[:, :, h].contiguous()))
+            assert torch.equal(lse[:, :, h], want_lse[:, :, h])
+
+
 @pytest.mark.parametrize("dtype,rows", KINDS)
 @pytest.mark.parametrize("lengths,q_heads,heads,dim", [
     ([20000], 16, 2, 256), ([131071], 4, 1, 64), ([5000, 3, 40, 9000, 0, 777], 32, 8, 128),
@@ -698,6 +712,35 @@ def test_two_contexts_at_once():
     for c, (_, _, _, out, lse), w, s in zip(cases, tensors, want, streams):
         c.attention.sync(s)
         assert torch.equal(_bits(out), _bits(w[0])) and torch.equal(_bits(lse), _bits(w[1]))
+
+
+def test_a_step_on_another_stream():
+    C, g = cache_mod(), _gen(9)
+    rows, page, blocks = 6, 4, 8
+    k, v = (torch.randn(rows, 2, 64, generator=g).to(BF16).cuda() for _ in range(2))
+    q = torch.randn(rows, 1, 8, 64, generator=g).to(BF16).cuda()
+    results = []
+    for stream in (None, torch.cuda.Stream()):
+        cache = C.PagedCache.zeros(40, 2, page, 64)
+        pager = C.Pager(40, page, rows, blocks, rows)
+        attention = C.PagedAttention(8, cache, rows, page * blocks)
+        (free, count), plan = pager.new_stack(), pager.new_plan(rows, rows)
+        plan.count, plan.lengths = count, torch.zeros(rows, dtype=torch.int32, device="cuda")
+        tables, other = (torch.zeros(rows, blocks, dtype=torch.int32, device="cuda") for _ in range(2))
+        out, parents = torch.empty_like(q), _i32([[1, 1, -1], [0, 2, 0]])
+        torch.cuda.synchronize()
+        for _ in range(6):
+            pager.plan_into(plan.lengths, None, tables, free, count, plan, stream)
+            cache.append(k, v, plan.slots, stream)
+            attention.attend_into(q, cache, tables, plan.lengths, out, stream=stream)
+            pager.fork_into(parents, tables, plan.lengths, free, count, other, plan.lengths, count, [cache], stream)
+            tables, other = other, tables
+        for c in (pager, attention):
+            c.sync(stream)
+        results.append([t.cpu() for t in (plan.lengths, plan.slots, count, _bits(out), _bits(cache.k), _bits(cache.v))])
+    for one, two in zip(*results):
+        assert torch.equal(one, two)
+    assert results[0][0].tolist() == [6, 6, 0, 6, 6, 6]
 
 
 def test_attention_refuses():

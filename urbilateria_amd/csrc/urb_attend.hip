@@ -3,8 +3,10 @@
 // One pass with a running maximum m and sum z: for a tile of tokens with scores s,
 //   m' = max(m, max s),  z' = z e(m - m') + sum e(s - m'),  o' = o e(m - m') + sum e(s - m') v
 // with e(x) = exp(scale x), and two parts of a row join by the same rule.  (The maximum is of the products
-// before the scale, so that rounding errs by their distance to it and not by their size.)  Every cached row is read once, 4
-// operations per value and query head that shares it, so HBM bounds all but the shortest calls.
+// before the scale, so that rounding errs by their distance to it and not by their size.)  Every cached row is
+// read once, 4 operations per value and query head that shares it, so HBM bounds all but the shortest calls: 64
+// rows of 4096 tokens of 8 heads of 128 are read at 6.4 TB/s (166 us), in E4M3 at 5.75 (93 us), 200 rows of
+// lengths from 8 to 12000 at 5.5 (178 us); one row of 500 tokens takes 15 us, latencies of its two kernels.
 //
 // Work: a pair is a row and up to sixteen of its query heads (of all its new tokens) that share a cache head;
 // a unit is kUnit tokens of a pair.  All units lie in one line, of which every workgroup takes an equal
@@ -30,7 +32,7 @@ namespace {
 
 constexpr int kUnit = 128;       // tokens
 // A pair's start and end (its queries, the waves' join, an output) cost about what a unit does: counted as one,
-// 200 rows of log-spread lengths up to 12000 take 193 us and not 213, and of 2 no less.
+// 200 rows of log-spread lengths up to 12000 take 178 us and not 183, and of 2 185.
 constexpr int kStart = 1;
 constexpr int kTile = 32;        // tokens of a wave's step
 constexpr int kWaves = 4;
@@ -247,7 +249,7 @@ __device__ __forceinline__ void finish4(const AttendArgs& a, uint32_t row, const
     const float s = a.sinks[q.head];
     const float top = fmaxf(m, s), t = top == kMinusInf ? 0.0f : top;
     const float f = exp2f((m - t) * kLog2e);
-    z = z * f + exp2f((s - t) * kLog2e);
+    z = z * f + (s == t ? 1.0f : exp2f((s - t) * kLog2e));  // (of a sink of +inf all)
     o.x *= f; o.y *= f; o.z *= f; o.w *= f;
     m = top;
   }
@@ -261,9 +263,8 @@ __device__ __forceinline__ void finish4(const AttendArgs& a, uint32_t row, const
   store4<BF16>(a.out + row * a.out_row + q.token * a.out_token + q.head * a.out_head + d * (BF16 ? 2 : 4), r);
 }
 
-// Workgroups per CU, and with it shares: what the registers hold.  (More shares than can run at a time leave
-// the last ones to run by themselves: 64 rows of 4096 tokens of 8 heads of 128 in E4M3 take 100 us with 512 and
-// 143 with 768; f32 rows of 128 over BF16 have 5.55 TB/s with one per CU.)
+// Workgroups per CU, and with it shares: what the registers hold without spilling.  (64 rows of 4096 tokens of 8
+// heads of 128 in E4M3 take 93 us with two per CU and 102 with three; f32 rows over BF16 have 6.1 TB/s with one.)
 template <int DS, bool F8, bool BF16>
 constexpr int kPerCu = DS == 2 && F8 ? 3 : DS <= 3 || (DS == 4 && (F8 || BF16)) || (DS == 6 && F8) ? 2 : 1;
 
@@ -299,7 +300,9 @@ __global__ __launch_bounds__(64 * kWaves, (kPerCu<DS, F8, BF16>)) void attend_ke
   const uint32_t dim = a.cache.dim;
   // Whether K and V pass the caches by: what one call reads once, a line in one load (rows of 160 bytes have 5.6
   // TB/s and so 5.3), and is too much to be there at the next.
-  const bool once = line.tiles == 1 && dim * (F8 ? 1 : 2) % 64 == 0 && (float)total * (float)(kUnit * 2 * (F8 ? 1 : 2)) * (float)dim > kCachedBytes;
+  constexpr int B = F8 ? 1 : 2;
+  const bool once = line.tiles == 1 && dim * B % 64 == 0 &&
+                    (float)total * (float)(kUnit * 2 * B) * (float)dim > kCachedBytes;
   const bool full = dim == (F8 ? 32 * KS : 32 * DS);
   uint8_t* const mine = stage[wave];
 
