@@ -1139,6 +1139,21 @@ def test_beams_in_place_and_captured():
             assert torch.equal(got, w)
 
 
+@pytest.mark.parametrize("R,W,picks,V", [(20, 4, 8, 50257), (21, 4, 16, 50257), (32, 4, 64, 32000), (3, 8, 16, 129280)])
+def test_beams_on_either_side_of_the_short_slices(R, W, picks, V):
+    logits, scores, ended = _beam_case(R, W, V, BF16, R + W)
+    _check_beams(logits, scores, picks, ended, end_token=7)
+
+
+@pytest.mark.parametrize("first,n", [(0, 40), (250, 300), (2000, 100), (8190, 4), (15000, 1900)])
+def test_few_logits_that_are_not_masked(first, n):
+    logits, scores, _ = _beam_case(3, 4, 17000, F32, 11)
+    logits[:, :first] = -math.inf
+    logits[:, first + n:] = -math.inf
+    for picks in (1, 5, 64):
+        _check_beams(logits, scores, picks)
+
+
 def test_beams_of_many_requests():
     logits, scores, ended = _beam_case(2500, 32, 60, F32, 4)
     _check_beams(logits, scores, 32, ended, end_token=1)

@@ -144,19 +144,20 @@ __global__ __launch_bounds__(kThreads) void beam_slice_kernel(BeamArgs a) {
   const uint32_t key = key_of(top);
   float m = top;
   for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
-  const uint32_t nth = wave_nth(key, a.picks);
+  const uint32_t nth = wave_nth(key, (a.picks + WAVES - 1) / WAVES);
   if ((tid & 63) == 0) {
     s_top[wave] = m;
     s_nth[wave] = nth;
   }
   __syncthreads();
-  // A wave that has so many bests gives a bound; among the few bests that reach the highest one, the
-  // picks-th itself is found by counting.
-  uint32_t bound = 0;
+  // What every wave has its part of `picks` above is a bound (32 x 8 beams of 129280 logits take 49 us with it and
+  // 50.6 with the picks-th of one wave, 16 x 32 with 64 picks 299 and 412); among the few bests that reach it,
+  // the picks-th itself is found by counting.
+  uint32_t bound = s_nth[0];
 #pragma unroll
   for (int w = 0; w < WAVES; ++w) {
     m = fmaxf(m, s_top[w]);
-    bound = max(bound, s_nth[w]);
+    bound = min(bound, s_nth[w]);
   }
   const bool head = key && key >= bound;
   u64 best = 0;  // the thread's, if it is among them: the first of equal ones
@@ -342,11 +343,15 @@ int span_of(int slices) {
   return span;
 }
 
-// Short slices while they are no more workgroups than four per CU (and a request's fit the join, a beam's a
-// wave of it): 4 beams over 50257 BF16 logits take 11.9 us with them and 16.4 without, 40 of them 13.8 and 18.1.
+// Short slices while they are no more workgroups than eight per CU, or four where the join takes its large
+// workgroups for them (and a request's fit the join, a beam's a wave of it): 4 beams over 50257 BF16 logits take
+// 11.9 us with them and 16.4 without, 64 of them 15.8 and 18.5, 128 (with more workgroups) 21.4 and 23.8, but 64 over
+// 129280 f32 logits 22.6 and 21.0; 24 beams of 3 requests over 129280 take 19.5 and 19.1.
+constexpr int kBeamShortWork = 2048;
 bool short_slices(int vocab, int width, int requests) {
   const int64_t slices = slices_of(vocab, kBeamShortSlice);
-  return slices <= 64 && span_of((int)slices) * width <= 1024 && slices * width * requests <= 1024;
+  const int64_t lists = span_of((int)slices) * width;
+  return slices <= 64 && lists <= 1024 && slices * width * requests <= (lists <= 256 ? kBeamShortWork : 1024);
 }
 
 size_t lists_bytes(size_t lists, int picks) { return lists * (picks * sizeof(u64) + sizeof(BeamSum)); }
@@ -356,7 +361,7 @@ size_t lists_bytes(size_t lists, int picks) { return lists * (picks * sizeof(u64
 size_t beam_work_bytes(int vocab, int width, int picks, int requests) {
   // (short slices of few requests may be more than long ones of all)
   const size_t many = (size_t)requests * width * slices_of(vocab, kBeamSlice);
-  return lists_bytes(std::max<size_t>(many, 1024), picks);
+  return lists_bytes(std::max<size_t>(many, kBeamShortWork), picks);
 }
 
 void launch_beam(BeamArgs a, bool bf16, void* work, hipStream_t s) {
