@@ -163,7 +163,7 @@ urb_status urb_pager_sync(urb_pager *pager, void *stream);
  *
  * q_heads a multiple of heads, q_heads <= 8192, queries 1 .. 16, max_rows 1 .. 2^20, max_length
  * 1 .. 2^24, heads, page_size and head_dim as in urb_kv_cache, else URB_ERR_SHAPE; a scale that is not
- * finite or <= 0 -> URB_ERR_INVALID_GEOMETRY. */
+ * finite, <= 0 or above 2^127 -> URB_ERR_INVALID_GEOMETRY. */
 typedef struct {
   uint32_t q_heads, heads, head_dim, page_size;
   urb_dtype dtype;       /* of queries and outputs: BF16, F32 */

@@ -114,6 +114,7 @@ def test_pagers_are_refused(change):
     (dict(max_length=0), N.ERR_SHAPE), (dict(max_length=(1 << 27) + 1), N.ERR_SHAPE),
     (dict(scale=0.0), N.ERR_INVALID_GEOMETRY), (dict(scale=-1.0), N.ERR_INVALID_GEOMETRY),
     (dict(scale=float("nan")), N.ERR_INVALID_GEOMETRY), (dict(scale=float("inf")), N.ERR_INVALID_GEOMETRY),
+    (dict(scale=2.0 ** 127.5), N.ERR_INVALID_GEOMETRY),
 ])
 def test_attentions_are_refused(change, status):
     desc = _struct(N.AttentionDesc, dict(q_heads=8, heads=2, head_dim=64, page_size=16, dtype=0, cache_dtype=0,

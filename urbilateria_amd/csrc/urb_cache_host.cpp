@@ -275,7 +275,8 @@ urb_status urb_attention_create(const urb_attention_desc* d, urb_attention** out
       d->q_heads % d->heads || d->queries == 0 || d->queries > 16 || d->max_rows == 0 ||
       d->max_rows > (1u << 20) || d->max_length == 0 || d->max_length > (1u << 24))
     return URB_ERR_SHAPE;
-  if (!finite_host(d->scale) || !(d->scale > 0.0f)) return URB_ERR_INVALID_GEOMETRY;
+  // (times log2(e) it is finite)
+  if (!(d->scale > 0.0f) || d->scale > 0x1p127f) return URB_ERR_INVALID_GEOMETRY;
   urb_attention* c = new (std::nothrow) urb_attention();
   if (!c) return URB_ERR_OUT_OF_MEMORY;
   c->desc = *d;
