@@ -948,6 +948,36 @@ def test_forks_without_enough_pages(spare):
     b.check(in_place=True)
 
 
+@pytest.mark.parametrize("spare", [0, 1, 2])
+def test_a_single_request_without_enough_pages(spare):
+    b = Beams(1, 4, 16, 3, 5)
+    b.lengths = np.array([21, 0, 0, 0])
+    b.parents[:] = 0
+    b.tables[0, :2] = [0, 1]
+    b.pages = 2 + spare
+    b.free, b.count = np.arange(2 + spare) + 2, spare
+    b.layers = [b._filled(b.pages, 2, 16, 32, BF16, 1)]
+    assert b.check()[5] == N.ERR_OUT_OF_MEMORY
+    b.check(in_place=True)
+
+
+def test_a_single_request_that_cannot_be():
+    b = Beams(1, 4, 16, 3, 6)
+    b.parents[0, 1], b.lengths[2] = 4, -1
+    assert b.check()[5] == N.ERR_ARGUMENT
+    for seed in (6, 7):
+        for count in (-1, 10 ** 6):
+            b = Beams(1, 4, 16, 3, seed)
+            b.count = count
+            assert b.check(in_place=True)[5] == N.ERR_ARGUMENT
+    # two pages dropped on a stack with room for one, and one that is none
+    b = Beams(1, 3, 16, 3, 7)
+    b.lengths[:], b.parents[:] = 32, [0, 0, 0]
+    b.tables[:, :2] = [[0, 1], [2, 3], [4, 10 ** 6]]
+    b.count = b.pages - 1
+    assert b.check()[5] == N.ERR_ARGUMENT
+
+
 def test_forks_of_rows_that_cannot_be():
     b = Beams(6, 4, 16, 3, 6)
     b.parents[0, 1], b.parents[2, 0] = 4, 2 ** 31 - 1

@@ -335,39 +335,44 @@ __device__ __forceinline__ uint64_t copying_rows(const int* parent, const int* l
 // The pages, lengths and stack of a request's rows, when all requests' dropped pages and copies are known:
 // dropped ones go on the stack, copies take theirs off it.  What a page on top is, when it is one that a
 // request has just dropped, is looked up in that request's list and not on the stack, which another workgroup
-// may not have written yet.
+// may not have written yet.  A single request's (ALONE) count, dropped pages, put on the stack already, and, in the
+// first wave, rows that copy are known.
+template <bool ALONE>
 __device__ __forceinline__ void fork_books(const ForkArgs& a, const int* parent, const int* length,
-                                           int64_t* slots, int* s_upto) {
+                                           int64_t* slots, int* s_upto, int count, int dropped, uint64_t copying) {
   const uint32_t r = blockIdx.x, row0 = r * a.width;
   const int tid = threadIdx.x, width = (int)a.width;
-  // pages dropped by requests 0 .. q, and copies before this request and in all (fewer than 2^20)
-  int dropped = 0;
-  int64_t copies = 0, all;
-  for (uint32_t q0 = 0; q0 < a.requests; q0 += 256) {
-    const uint32_t q = q0 + tid;
-    const int d = q < a.requests ? a.drops[q] : 0;
-    const int64_t c = q < a.requests ? a.copies[q] : 0;
-    copies += c << 32 | (q < r ? c : 0);
-    const int upto = dropped + (int)before<256>(d, slots, &all) + d;
-    if (q < a.requests) s_upto[q] = upto;
-    dropped += (int)all;
+  int copies_before = 0, copies_all = 0;
+  if constexpr (!ALONE) {
+    // pages dropped by requests 0 .. q, and copies before this request and in all (fewer than 2^20)
+    int64_t copies = 0, all;
+    for (uint32_t q0 = 0; q0 < a.requests; q0 += 256) {
+      const uint32_t q = q0 + tid;
+      const int d = q < a.requests ? a.drops[q] : 0;
+      const int64_t c = q < a.requests ? a.copies[q] : 0;
+      copies += c << 32 | (q < r ? c : 0);
+      const int upto = dropped + (int)before<256>(d, slots, &all) + d;
+      if (q < a.requests) s_upto[q] = upto;
+      dropped += (int)all;
+    }
+    (void)before<256>(copies, slots, &all);
+    copies_before = (int)(all & 0xffffffff);
+    copies_all = (int)(all >> 32);
+    const int32_t* list = a.dropped + (uint64_t)row0 * a.max_blocks;
+    const int before_r = r ? s_upto[r - 1] : 0, n = s_upto[r] - before_r;
+    const int64_t first = (int64_t)count + before_r;
+    for (int j = tid; j < n; j += 256)
+      if (first + j < a.pages) a.free_pages[first + j] = list[j];
   }
-  (void)before<256>(copies, slots, &all);
-  const int copies_before = (int)(all & 0xffffffff), copies_all = (int)(all >> 32);
-  const int count = *a.count;
+  if (tid >= 64) return;
+  if constexpr (ALONE) copies_all = __popcll(copying);
+  else copying = copying_rows(parent, length, width, a.page);
   const int64_t room = (int64_t)a.pages - count;  // of the stack
   const int64_t size = count + min((int64_t)dropped, room);
-  const int32_t* list = a.dropped + (uint64_t)row0 * a.max_blocks;
-  const int before_r = r ? s_upto[r - 1] : 0, n = s_upto[r] - before_r;
-  const int64_t first = (int64_t)count + before_r;
-  for (int j = tid; j < n; j += 256)
-    if (first + j < a.pages) a.free_pages[first + j] = list[j];
   if (r == 0 && tid == 0) {
     *a.free_count_out = (int)max(size - copies_all, (int64_t)0);
     if (dropped > room) flag(a.status, kCacheArgument);
   }
-  if (tid >= 64) return;
-  const uint64_t copying = copying_rows(parent, length, width, a.page);
   if (tid >= width) return;
   const int p = parent[tid];
   int kept = p >= 0 ? length[p] : 0;
@@ -383,7 +388,7 @@ __device__ __forceinline__ void fork_books(const ForkArgs& a, const int* parent,
         to = a.free_pages[at];
       } else {
         const int want = (int)(at - count);
-        uint32_t q = 0, end = a.requests - 1;  // the first request whose dropped pages end beyond
+        uint32_t q = 0, end = ALONE ? 0 : a.requests - 1;  // the first request whose dropped pages end beyond
         while (q < end) {
           const uint32_t mid = (q + end) / 2;
           if (s_upto[mid] > want) end = mid;
@@ -404,7 +409,7 @@ __device__ __forceinline__ void fork_books(const ForkArgs& a, const int* parent,
 
 // One request per workgroup: its rows' tables, and the pages that none of them holds any more.  A page can
 // stand in several rows only in one column, so a column is one thread's work.  Latency bounds it (parents and
-// lengths, the column, the pages' places): 8 us for 4 rows of 59 pages, 10 for 32 requests of 8 rows of 43.
+// lengths, the column, the pages' places): 6 us for 4 rows of 59 pages, 10 for 32 requests of 8 rows of 43.
 template <bool ALONE>
 __global__ __launch_bounds__(256) void fork_tables_kernel(ForkArgs a) {
   extern __shared__ int column[];  // [width][256]
@@ -421,6 +426,8 @@ __global__ __launch_bounds__(256) void fork_tables_kernel(ForkArgs a) {
     s_columns = 0;
   }
   __syncthreads();
+  // (read with the parents, and written at the end)
+  const int count = ALONE || (r == 0 && tid == 0) ? stack_size(a.free_count, a.pages, &bits) : 0;
   if (tid < width) {
     int p = a.parents[row0 + tid];
     if (p >= width) bits |= kCacheArgument;
@@ -437,9 +444,10 @@ __global__ __launch_bounds__(256) void fork_tables_kernel(ForkArgs a) {
     atomicMax(&s_columns, blocks[tid]);
   }
   __syncthreads();
+  uint64_t copying = 0;
   if (tid < 64) {
-    const uint64_t copies = copying_rows(parent, length, width, a.page);
-    if (tid == 0) a.copies[r] = __popcll(copies);
+    copying = copying_rows(parent, length, width, a.page);
+    if (!ALONE && tid == 0) a.copies[r] = __popcll(copying);
   }
   const uint64_t used = s_used;
   const uint32_t columns = s_columns;
@@ -488,19 +496,21 @@ __global__ __launch_bounds__(256) void fork_tables_kernel(ForkArgs a) {
     int64_t all;
     int at = n_dropped + (int)before<256>(__popcll(drop), slots, &all);
     n_dropped += (int)all;
-    for (; drop; drop &= drop - 1)
-      list[at++] = column[(__ffsll((unsigned long long)drop) - 1) * 256 + tid];
+    for (; drop; drop &= drop - 1, ++at) {
+      const int page = column[(__ffsll((unsigned long long)drop) - 1) * 256 + tid];
+      list[at] = page;
+      if (ALONE && (int64_t)count + at < a.pages) a.free_pages[count + at] = page;
+    }
   }
-  if (tid == 0) {
+  if (!ALONE && tid == 0) {
     a.drops[r] = n_dropped;
-    if (r == 0) *a.count = stack_size(a.free_count, a.pages, &bits);
+    if (r == 0) *a.count = count;
   }
   if (bits) flag(a.status, bits);
   if constexpr (ALONE) {
     // a single request has its books done here
-    __shared__ int s_upto[1];
     __syncthreads();
-    fork_books(a, parent, length, slots, s_upto);
+    fork_books<true>(a, parent, length, slots, nullptr, count, n_dropped, copying);
   }
 }
 
@@ -508,13 +518,13 @@ __global__ __launch_bounds__(256) void fork_books_kernel(ForkArgs a) {
   __shared__ int parent[kForkWidth], length[kForkWidth];
   __shared__ int64_t slots[4];
   __shared__ int s_upto[kForkRequests];
-  const int tid = threadIdx.x, width = (int)a.width;
+  const int tid = threadIdx.x, width = (int)a.width, count = *a.count;
   if (tid < width) {
     const int p = a.parents[blockIdx.x * a.width + tid];
     parent[tid] = p < 0 || p >= width ? -1 : p;
     length[tid] = a.old_lengths[blockIdx.x * a.width + tid];
   }
-  fork_books(a, parent, length, slots, s_upto);
+  fork_books<false>(a, parent, length, slots, s_upto, count, 0, 0);
 }
 
 struct ForkCaches {
