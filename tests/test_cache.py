@@ -634,6 +634,21 @@ def test_infinities_and_nans_stay_in_their_rows():
     assert bool(torch.isnan(out[1, 0, 2:, 7]).all())
 
 
+@pytest.mark.parametrize("lengths", [[40], [9000], [5, 0, 9000]])
+@pytest.mark.parametrize("rows", [BF16, F32])
+def test_queries_of_nan_stay_nan(lengths, rows):
+    # in a row of one workgroup and in one that several share
+    c = Cached(lengths, 8, 2, 64, 16, rows=rows, queries=2)
+    want, want_lse = c.run()
+    c.q[-1, 1, 3], c.q[-1, 0, 6, 5] = NAN, NAN
+    out, lse = c.run()
+    hit = torch.zeros(out.shape[:3], dtype=torch.bool)
+    hit[-1, 1, 3] = hit[-1, 0, 6] = True
+    assert bool(torch.isnan(out.cpu()[hit].float()).all()) and bool(torch.isnan(lse.cpu()[hit]).all())
+    assert torch.equal(_bits(out)[~hit], _bits(want)[~hit])
+    assert torch.equal(_bits(lse)[~hit], _bits(want_lse)[~hit])
+
+
 def test_lengths_and_pages_out_of_range():
     c = Cached([100, 40, 64, 90], 4, 2, 64, 16, max_length=100)
     want, lse = c.run()

@@ -632,12 +632,12 @@ __global__ __launch_bounds__(64 * kWaves, (kPerCu<DS, F8, BF16>)) void attend_ke
   }
 }
 
-// Two parts of a query as one: (m, z, o) takes in (pm, pz, po).
+// Two parts of a query as one: (m, z, o) takes in (pm, pz, po).  (Scores of NaN alone leave a maximum of -inf, and
+// sums of NaN that stay so.)
 __device__ __forceinline__ void take_in(float& m, float& z, float4& o, float pm, float pz, const float4& po,
                                         float scale2) {
-  const float top = fmaxf(m, pm);
-  if (top == kMinusInf) return;
-  const float f = exp2f((m - top) * scale2), g = exp2f((pm - top) * scale2);
+  const float top = fmaxf(m, pm), base = top == kMinusInf ? 0.0f : top;
+  const float f = exp2f((m - base) * scale2), g = exp2f((pm - base) * scale2);
   m = top;
   z = fmaf(pz, g, z * f);
   o.x = fmaf(po.x, g, o.x * f);
