@@ -1127,6 +1127,54 @@ def test_candidates_that_tie(dtype, V):
                  torch.tensor([[True, False, True]] * 2), end_token=3)
 
 
+# beam scores and logits [n] that differ but whose scores, in f64, do not: the lowest tokens, not the largest logits
+ONE_SCORE = {
+    "nearly 0": (-1.0, lambda n, g: 1e-20 * torch.arange(n)),
+    "falling": (-2.0, lambda n, g: 1e-25 * torch.arange(n, 0, -1)),
+    "subnormal": (0.0, lambda n, g: torch.randint(0, 200, (n,), generator=g) * 1e-44),
+    "either sign": (-3.0, lambda n, g: 1e-30 * torch.randn(n, generator=g)),
+    "a few larger": (-1.0, lambda n, g: torch.where(torch.rand(n, generator=g) < 4 / n, 1.0, 1e-20) * torch.rand(
+        n, generator=g)),
+    "neighbours": (-1e9, lambda n, g: 0.5 + 2.0 ** -24 * torch.randint(0, 40, (n,), generator=g)),
+    "far below": (-1e12, lambda n, g: 1e-3 * torch.randn(n, generator=g)),
+    "lowest": (-3.4e38, lambda n, g: 5 * torch.randn(n, generator=g)),
+}
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("V", [5, 3000, 8195, 70000])
+@pytest.mark.parametrize("kind", sorted(ONE_SCORE))
+def test_logits_that_differ_under_one_score(dtype, V, kind):
+    g = _gen(V)
+    score, make = ONE_SCORE[kind]
+    logits = torch.stack([make(V, g).float() for _ in range(8)])
+    logits[torch.rand(8, V, generator=g) < 0.2] = -math.inf
+    logits = logits.to(dtype)
+    for picks in (1, 4, 64):
+        _check_beams(logits, torch.full((2, 4), score), picks)
+        # (other beams' few candidates before and behind them, and some that have ended)
+        some = logits.clone()
+        some[[0, 6], 2:] = -math.inf
+        scores = torch.full((2, 4), score)
+        scores[0, 0] = scores[1, 2] = score / 2 + 1
+        _check_beams(some, scores, picks, torch.tensor([[0, 1, 0, 0], [0, 0, 0, 1]]), end_token=V - 2, strided=True)
+
+
+def test_one_score_in_place():
+    V, R, W = 5000, 3, 4
+    s = step().BeamSelector(V, W, W, R)
+    logits = 1e-20 * torch.randn(R * W, V, generator=_gen(3))
+    scores, ended = -torch.ones(R, W), torch.tensor([[0, 0, 0, 0], [1, 0, 0, 0], [0, 0, 1, 1]], dtype=torch.int32)
+    want, tokens, parents = _select_by_hand(logits, scores, W, ended, 7)
+    c, e, t, p = scores.cuda(), ended.cuda(), ended.clone().cuda(), ended.clone().cuda()
+    s.select_into(logits.cuda(), c, c, t, p, ended=e, end_token=7, ended_out=e)
+    s.sync()
+    _same(t, tokens)
+    _same(p, parents)
+    _same(c, want.float())
+    _same(e, (ended.gather(1, parents.long()) != 0) | (tokens == 7))
+
+
 def test_few_candidates():
     V = 30000
     logits = torch.full((4, V), -math.inf)

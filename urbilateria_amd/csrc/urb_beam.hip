@@ -220,24 +220,105 @@ __global__ __launch_bounds__(kThreads) void beam_slice_kernel(BeamArgs a) {
 
 struct Candidate {
   double score;
-  uint32_t at;  // beam * vocab + token
+  uint32_t at;   // beam << kTokenBits | token
+  uint32_t key;  // of its logit
 };
+constexpr int kTokenBits = 18;
+static_assert(kBeamVocab <= 1 << kTokenBits && kBeamWidth < 1 << (31 - kTokenBits), "beam and token in 32 bits");
 constexpr uint32_t kNone = 0xffffffffu;
+// The order of the picks.
 __device__ __forceinline__ bool better(const Candidate& x, const Candidate& y) {
   return x.score > y.score || (x.score == y.score && x.at < y.at);
+}
+// The order that the lists are in: a beam's candidates of one score by their logits first, which may differ in less
+// than a score shows.
+__device__ __forceinline__ bool ahead(const Candidate& x, const Candidate& y) {
+  if (x.score != y.score) return x.score > y.score;
+  return (x.at ^ y.at) >> kTokenBits || x.key == y.key ? x.at < y.at : x.key > y.key;
+}
+
+// What a beam's logits are scored with: c + ((l - m) - log z).
+struct Scored {
+  double c, log_z;
+  float m;
+  __device__ __forceinline__ double of(float v) const {
+    return c + ((v == m ? 0.0 : (double)v - (double)m) - log_z);
+  }
+  // Logits above this in size have scores of their own: they lie 2^-24 of their size apart, and the three roundings of
+  // two scores are off by less than 2^-52 (3 |v| + 3 |m| + |c| + 26), log z being below 13.
+  __device__ __forceinline__ float own_scores() const {
+    return (float)((fabs(c) + fabs((double)m) + 32.0) * 0x1p-25);
+  }
+  // whether a logit next to this one has its score too
+  __device__ __forceinline__ bool shared(uint32_t key) const {
+    const float v = key_value(key);
+    const double score = of(v);
+    return of(key_value(key - 1)) == score || (v < m && of(key_value(key + 1)) == score);
+  }
+};
+
+// The picks from place `from` on: the lowest tokens of beam b with this score, of its row of logits.  All threads.
+template <int THREADS>
+__device__ __forceinline__ void pick_lowest(const BeamArgs& a, int r, int b, const Scored& beam, double score, int from,
+                                            uint32_t* counts) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const size_t size = a.bf16 ? 2 : 4, out = (size_t)r * a.picks;
+  const uint8_t* row = reinterpret_cast<const uint8_t*>(a.logits) + (r * a.width + b) * a.row_stride * size;
+  const bool wide = reinterpret_cast<uintptr_t>(row) % (4 * size) == 0;
+  for (int i0 = 0; i0 < a.vocab && from < a.picks; i0 += 4 * THREADS) {
+    const int i = i0 + 4 * tid;
+    float v[4];
+    if (a.bf16) load4<true>(v, row, i, a.vocab, wide);
+    else load4<false>(v, row, i, a.vocab, wide);
+    bool hit[4];
+    int before = 0, mine = 0, all = 0;  // of lower lanes, of this, of the wave
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      hit[j] = beam.of(v[j]) == score;
+      const uint64_t hits = __ballot(hit[j]);
+      before += __popcll(hits & ((1ull << lane) - 1));
+      all += __popcll(hits);
+      mine += hit[j];
+    }
+    __syncthreads();
+    if (lane == 0) counts[wave] = (uint32_t)all;
+    __syncthreads();
+    int place = from + before;
+    for (int w = 0; w < THREADS / 64; ++w) {
+      if (w < wave) place += (int)counts[w];
+      from += (int)counts[w];
+    }
+    if (mine == 0) continue;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (hit[j] && place < a.picks) {
+        a.scores_out[out + place] = (float)score;
+        a.tokens[out + place] = i + j;
+        a.parents[out + place] = b;
+        if (a.ended_out) a.ended_out[out + place] = i + j == a.end_token;
+        ++place;
+      }
+  }
 }
 
 // A workgroup per request; each slice of each of its beams is a list in order.  `span` lists (a power of two)
 // are counted for a beam, `team` threads go through a list.
+//
+// Logits that differ may share a score: close ones of a beam whose score is large, or of nearly 0.  Where a candidate
+// that counts may be one of them, the lists are gone through again in the order that they are in.  A list has the largest
+// logits of its slice, so it has all candidates above the last pick's score; of those with that very score lower
+// tokens may be missing in the last pick's beam (lists of beams before it that end at that score would fill the picks
+// by themselves).  They are looked up in the row, which only such calls read again.
 template <int THREADS>
 __global__ __launch_bounds__(THREADS) void beam_join_kernel(BeamArgs a, int span, int team) {
   constexpr int WAVES = THREADS / 64, EARLY = 8;
   __shared__ double powers[kPowers];
   __shared__ Candidate list[kBeamPicks * kBeamPicks];
   __shared__ int s_live[kBeamWidth];  // 0: no candidates, 1: its slices', 2: ended
+  __shared__ Scored s_beams[kBeamWidth];
   __shared__ uint32_t s_nth[WAVES];
-  __shared__ int n_heads, n_list, s_bad;
-  __shared__ Candidate s_least;
+  __shared__ int n_heads, n_list, s_bad, s_close;
+  __shared__ Candidate s_least, s_last;
   static_assert(kBeamPicks * kBeamPicks >= THREADS, "a place for every list's first");
   const int r = blockIdx.x, tid = threadIdx.x;
   const int b = tid / (span * team), slice = tid / team & (span - 1), place = tid & (team - 1);
@@ -253,9 +334,10 @@ __global__ __launch_bounds__(THREADS) void beam_join_kernel(BeamArgs a, int span
   const float score = a.scores[beam];
   const bool end = a.ended && a.ended[beam];
   fill_powers(powers);
+  const Candidate none{-__builtin_inf(), kNone, 0};
   if (tid == 0) {
-    n_heads = n_list = s_bad = 0;
-    s_least = Candidate{-__builtin_inf(), kNone};
+    n_heads = n_list = s_bad = s_close = 0;
+    s_least = s_last = none;
   }
   __syncthreads();
   float m = mine && !end ? sum.m : -kInf;
@@ -267,63 +349,77 @@ __global__ __launch_bounds__(THREADS) void beam_join_kernel(BeamArgs a, int span
   for (int o = span * team / 2; o >= team; o >>= 1) z += __shfl_xor(z, o, 64);
   const bool bad = !(score <= 3.4028235e38f);  // NaN, +inf
   const int live = bad || !(score > -kInf) ? 0 : end ? 2 : m > -kInf ? 1 : 0;
-  // what a logit - m is added to
-  const double base = end ? (double)score : (double)score - log(z);
+  const Scored scored{(double)score, end ? 0.0 : log(z), m};
   if (mine && slice == 0 && place == 0) {
     s_live[b] = live;
+    s_beams[b] = scored;
     if (bad) s_bad = 1;
   }
   // candidate i of this list
-  auto candidate = [&](int i, u64 key) -> Candidate {
-    const Candidate none{-__builtin_inf(), kNone};
-    if (live == 2) return slice == 0 && i == 0 ? Candidate{base, (uint32_t)b * a.vocab + a.end_token} : none;
-    if (live == 0 || !key) return none;
-    const float v = key_value((uint32_t)(key >> 32));
-    const double c = base + (v == m ? 0.0 : (double)v - (double)m);
-    return c > -__builtin_inf() ? Candidate{c, (uint32_t)b * a.vocab + ~(uint32_t)key} : none;
+  auto candidate = [&](int i, u64 both) -> Candidate {
+    const uint32_t first = (uint32_t)b << kTokenBits, key = (uint32_t)(both >> 32);
+    if (live == 2) return slice == 0 && i == 0 ? Candidate{scored.c, first | (uint32_t)a.end_token, 0} : none;
+    if (live == 0 || !both) return none;
+    const double c = scored.of(key_value(key));
+    return c > -__builtin_inf() ? Candidate{c, first | ~(uint32_t)both, key} : none;
   };
-  // the picks-th of the lists' first ones, as in the slices (a score's f32 keeps the order)
-  Candidate first{-__builtin_inf(), kNone};
-  if (mine && place == 0) first = candidate(0, early[0]);
-  const uint32_t key = first.at == kNone ? 0 : key_of(fmaxf((float)first.score, -3.4028235e38f));
-  const uint32_t nth = wave_nth(key, a.picks);
-  if ((tid & 63) == 0) s_nth[tid >> 6] = nth;
-  __syncthreads();
-  uint32_t bound = 0;
+  const float own_scores = scored.own_scores();
+  auto collect = [&](auto before) __attribute__((always_inline)) {
+    // the picks-th of the lists' first ones, as in the slices (a score's f32 keeps the order)
+    Candidate first = none;
+    if (mine && place == 0) first = candidate(0, early[0]);
+    const uint32_t key = first.at == kNone ? 0 : key_of(fmaxf((float)first.score, -3.4028235e38f));
+    const uint32_t nth = wave_nth(key, a.picks);
+    if ((tid & 63) == 0) s_nth[tid >> 6] = nth;
+    __syncthreads();
+    uint32_t bound = 0;
 #pragma unroll
-  for (int w = 0; w < WAVES; ++w) bound = max(bound, s_nth[w]);
-  const bool head = key && key >= bound;
-  if (head) list[atomicAdd(&n_heads, 1)] = first;
-  __syncthreads();
-  rank_all<WAVES>(list, n_heads, better, [&](const Candidate& c, int above) {
-    if (above == a.picks - 1) s_least = c;
-  });
-  __syncthreads();
-  const Candidate least = s_least;
-  // (lists are in order: behind one that falls short there is nothing)
-  auto take = [&](int i, u64 k) {
-    const Candidate c = candidate(i, k);
-    const bool in = c.at != kNone && !better(least, c);
-    if (in) list[atomicAdd(&n_list, 1)] = c;
-    return in;
+    for (int w = 0; w < WAVES; ++w) bound = max(bound, s_nth[w]);
+    const bool head = key && key >= bound;
+    if (head) list[atomicAdd(&n_heads, 1)] = first;
+    __syncthreads();
+    rank_all<WAVES>(list, n_heads, before, [&](const Candidate& c, int above) {
+      if (above == a.picks - 1) s_least = c;
+    });
+    __syncthreads();
+    const Candidate least = s_least;
+    // (lists are in order: behind one that falls short there is nothing)
+    auto take = [&](int i, u64 k) {
+      const Candidate c = candidate(i, k);
+      const bool in = c.at != kNone && !before(least, c);
+      if (in) list[atomicAdd(&n_list, 1)] = c;
+      if (fabsf(key_value(c.key)) <= own_scores) s_close = 1;  // (NaN where there is no logit)
+      return in;
+    };
+    if (mine) {
+      bool more = true;
+#pragma unroll
+      for (int i = 0; i < EARLY; ++i) more = more && place + i * team < a.picks && take(place + i * team, early[i]);
+      for (int i = place + EARLY * team; more && i < a.picks; i += team) more = take(i, keys[i]);
+    }
+    __syncthreads();
   };
-  if (mine) {
-    bool more = true;
-#pragma unroll
-    for (int i = 0; i < EARLY; ++i) more = more && place + i * team < a.picks && take(place + i * team, early[i]);
-    for (int i = place + EARLY * team; more && i < a.picks; i += team) more = take(i, keys[i]);
+  collect([](const Candidate& x, const Candidate& y) { return better(x, y); });
+  const bool close = s_close;
+  if (close) {
+    __syncthreads();
+    if (tid == 0) {
+      n_heads = n_list = 0;
+      s_least = none;
+    }
+    __syncthreads();
+    collect([](const Candidate& x, const Candidate& y) { return ahead(x, y); });
   }
-  __syncthreads();
   const int n = n_list;
   const size_t out = (size_t)r * a.picks;
   rank_all<WAVES>(list, n, better, [&](const Candidate& c, int place) {
     if (place >= a.picks) return;
-    const int parent = (int)(c.at / (uint32_t)a.vocab);
-    const int token = (int)(c.at - (uint32_t)parent * a.vocab);
+    const int parent = (int)(c.at >> kTokenBits), token = (int)(c.at & ((1u << kTokenBits) - 1));
     a.scores_out[out + place] = (float)c.score;
     a.tokens[out + place] = token;
     a.parents[out + place] = parent;
     if (a.ended_out) a.ended_out[out + place] = s_live[parent] == 2 || token == a.end_token;
+    if (close && place == a.picks - 1 && s_live[parent] == 1 && s_beams[parent].shared(c.key)) s_last = c;
   });
   for (int i = n + tid; i < a.picks; i += THREADS) {
     a.scores_out[out + i] = -kInf;
@@ -332,6 +428,18 @@ __global__ __launch_bounds__(THREADS) void beam_join_kernel(BeamArgs a, int span
     if (a.ended_out) a.ended_out[out + i] = 1;
   }
   if (tid == 0 && s_bad) flag(a.status, kStepArgument);
+  if (!close) return;
+  __syncthreads();
+  const Candidate last = s_last;
+  if (last.at == kNone) return;
+  const uint32_t parent = last.at >> kTokenBits;
+  int from = 0;  // picks before those of the last one's beam and score
+  for (int i0 = 0; i0 < n; i0 += THREADS) {
+    const int i = i0 + tid;
+    from += __syncthreads_count(i < n && (list[i].score > last.score || (list[i].score == last.score &&
+                                                                         list[i].at >> kTokenBits < parent)));
+  }
+  pick_lowest<THREADS>(a, r, (int)parent, s_beams[parent], last.score, from, s_nth);
 }
 
 int slices_of(int vocab, int slice) { return (vocab + slice - 1) / slice; }
@@ -382,6 +490,7 @@ void launch_beam(BeamArgs a, bool bf16, void* work, hipStream_t s) {
     c.tokens += picks;
     c.parents += picks;
     if (a.ended_out) c.ended_out += picks;
+    c.bf16 = bf16;
     c.keys += beams * a.slices * a.picks;
     c.sums += beams * a.slices;
     const dim3 grid(a.slices, c.requests * a.width);

@@ -65,7 +65,8 @@ struct BeamArgs {
   float* scores_out;
   int32_t *tokens, *parents, *ended_out;
   int* status;
-  // set by launch_beam: workspace
+  // set by launch_beam: the logits' type, workspace
+  bool bf16;
   int slices;
   unsigned long long* keys;
   BeamSum* sums;
