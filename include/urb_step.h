@@ -195,8 +195,9 @@ urb_status urb_sampler_sync(urb_sampler *sampler, void *stream);
  * (l_v - m is 0 where both are +inf), and of a beam that has ended only (b, end_token), of score c_b.  The
  * `picks` best are taken: by descending score, equal ones by ascending b * vocab + v.  Scores are compared
  * in f64, where those of different logits of a beam may be equal too (under a score of -1e12, or of logits of
- * nearly 0).  NaN logits count as -inf, and nothing of score -inf is taken: missing picks have score -inf,
- * token -1 and parent -1.  A beam of score -inf is not there (of a search that begins, all but one are).
+ * nearly 0).  NaN logits count as -inf, and nothing of score -inf, or below f32's range, is taken: missing
+ * picks have score -inf, token -1 and parent -1.  A beam of score -inf is not there (of a search that begins,
+ * all but one are).
  *
  * vocab 1 .. 2^18, width 1 .. 32, picks 1 .. 64, max_requests 1 .. 65535, else URB_ERR_SHAPE. */
 typedef struct {

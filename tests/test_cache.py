@@ -1175,6 +1175,25 @@ def test_one_score_in_place():
     _same(e, (ended.gather(1, parents.long()) != 0) | (tokens == 7))
 
 
+@pytest.mark.parametrize("V", [4, 9000, 70000])
+def test_scores_below_the_range_of_f32(V):
+    # masks of f32's lowest value: a beam that took one has nothing but its first token
+    low = torch.finfo(F32).min
+    logits = torch.full((6, V), -math.inf)
+    logits[:, [0, 2, V - 1]] = torch.tensor([1.0, low, low])
+    scores = torch.tensor([[low, 0.9 * low, -math.inf], [low, -1.0, low / 2]])
+    for picks in (1, 3, 8, 64):
+        total, tokens, parents = _select_by_hand(logits, scores, min(picks, 3 * V), None, -1)
+        none = total.float() == -math.inf
+        assert picks < 5 or bool((none & (total > -math.inf)).any())
+        got = step().BeamSelector(V, 3, picks, 2).select(logits.cuda(), scores.cuda())
+        n = total.shape[1]
+        _same(got[0][:, :n], total.float())
+        _same(got[1][:, :n], torch.where(none, -1, tokens))
+        _same(got[2][:, :n], torch.where(none, -1, parents))
+        assert bool((got[1][:, n:] == -1).all()) and bool((got[0][:, n:] == -math.inf).all())
+
+
 def test_few_candidates():
     V = 30000
     logits = torch.full((4, V), -math.inf)

@@ -361,14 +361,14 @@ __global__ __launch_bounds__(THREADS) void beam_join_kernel(BeamArgs a, int span
     if (live == 2) return slice == 0 && i == 0 ? Candidate{scored.c, first | (uint32_t)a.end_token, 0} : none;
     if (live == 0 || !both) return none;
     const double c = scored.of(key_value(key));
-    return c > -__builtin_inf() ? Candidate{c, first | ~(uint32_t)both, key} : none;
+    return (float)c > -kInf ? Candidate{c, first | ~(uint32_t)both, key} : none;
   };
   const float own_scores = scored.own_scores();
   auto collect = [&](auto before) __attribute__((always_inline)) {
     // the picks-th of the lists' first ones, as in the slices (a score's f32 keeps the order)
     Candidate first = none;
     if (mine && place == 0) first = candidate(0, early[0]);
-    const uint32_t key = first.at == kNone ? 0 : key_of(fmaxf((float)first.score, -3.4028235e38f));
+    const uint32_t key = first.at == kNone ? 0 : key_of((float)first.score);
     const uint32_t nth = wave_nth(key, a.picks);
     if ((tid & 63) == 0) s_nth[tid >> 6] = nth;
     __syncthreads();
