@@ -358,6 +358,18 @@ def test_appends_of_many_heads_in_several_launches():
         assert torch.equal(t[0].float().cpu(), want.expand(heads, 8, 16))
 
 
+@pytest.mark.parametrize("dtype", [BF16, F8])
+def test_a_caches_tensors_stay(dtype):
+    c = _make_cache(2, 1, 4, 16, dtype)
+    for name in ("k", "v", "k_scales", "v_scales", "heads", "dtype"):
+        was = getattr(c, name)
+        with pytest.raises(AttributeError):
+            setattr(c, name, None if was is None else was.clone() if torch.is_tensor(was) else was)
+        assert getattr(c, name) is was
+    for c.layer in (1, 2):     # what is not the cache's own
+        pass
+
+
 # ---- attention ----------------------------------------------------------------------------------
 
 class Cached:

@@ -71,7 +71,8 @@ class PagedCache:
     """One layer's keys and values (``urb_kv_cache``): ``k`` and ``v`` [pages, heads, page_size, head_dim],
     torch.bfloat16 or torch.float8_e4m3fn, of the same strides (either may be a view of another layout or
     a part of a wider buffer; a head's values are contiguous); for E4M3 ``k_scales`` and ``v_scales``
-    [pages, heads, page_size] uint8, contiguous (E8M0)."""
+    [pages, heads, page_size] uint8, contiguous (E8M0).  Its tensors are not to be replaced (AttributeError) or
+    resized: another cache takes others."""
 
     def __init__(self, k, v, k_scales=None, v_scales=None):
         if k.dim() != 4 or k.get_device() < 0:
@@ -89,6 +90,13 @@ class PagedCache:
         self._desc = N.KvCache(k.data_ptr(), v.data_ptr(), *at, _cache_type(k.dtype), self.pages,
                                self.heads, self.page_size, self.head_dim, *strides)
         self._ref = ctypes.byref(self._desc)
+        self._fixed = frozenset(self.__dict__)
+
+    def __setattr__(self, name, value):
+        # calls go by the addresses and sizes that were checked
+        if name in self.__dict__.get("_fixed", ()):
+            raise AttributeError(f"{name} of a PagedCache cannot be replaced")
+        object.__setattr__(self, name, value)
 
     @classmethod
     def zeros(cls, pages: int, heads: int, page_size: int, head_dim: int, dtype=None, device="cuda"):
