@@ -1030,6 +1030,41 @@ def test_forks_of_rows_that_cannot_be():
     assert b.check()[5] == N.ERR_ARGUMENT
 
 
+@pytest.mark.parametrize("width", [2, 4, 16, 17, 64])
+@pytest.mark.parametrize("requests", [1, 3])
+def test_rows_with_children_that_share_a_page_filled_in_part(requests, width):
+    rows, page, last = requests * width, 4, width - 1
+    common = [[0, 1, 2 + i] for i in range(width)]      # the first two pages are all rows'
+    stay = list(range(width))
+    for status, lengths, parents, tables in (
+            (N.OK, [8] * width, stay, common),                                   # whole pages
+            (N.OK, [11] * width, stay, common),                                  # and one in part for each
+            (N.ERR_ARGUMENT, [7] * width, stay, common),                         # a prompt that all go on with
+            (N.OK, [7] * width, [last] + [-1] * last, common),                   # ... one does
+            (N.OK, [7] * width, [last] * width, common),                         # ... with all the children
+            (N.ERR_ARGUMENT, [7] * width, [0, last] + [-1] * (width - 2), common),
+            (N.ERR_ARGUMENT, [8] * last + [6], stay, common),                    # whole in the others
+            (N.ERR_ARGUMENT, [6] + [12] * last, stay, common),
+            (N.OK, [4] * last + [6], stay, common),                              # the others end before it
+            (N.OK, [7] * width, stay, [[0, -1, 2]] * width)):                    # no page
+        own = width + 2
+        tables = np.array([[p + r * own if p >= 0 else p for p in row] for r in range(requests) for row in tables])
+        lengths, parents = np.array(lengths * requests), np.array([parents] * requests)
+        free = list(range(requests * own, requests * own + rows)) + [-4] * 7
+        pages = len(free) + requests * own
+        free += [-4] * (pages - len(free))
+        P = cache_mod().Pager(pages, page, rows, 3)
+        out, n, stack, count = torch.full((rows, 3), -8, dtype=torch.int32, device="cuda"), _i32(lengths), _i32(
+            free), _i32([rows])
+        want = _fork_by_hand(parents, tables.tolist(), out.tolist(), lengths, free, rows, page, pages, 3)
+        assert want[5] == N.OK
+        P.fork_into(_i32(parents), _i32(tables), n, stack, count, out, n, count)
+        assert _status(P.sync) == status, (lengths, parents)
+        for got, w in zip((out, n, stack, count), want):
+            _same(got, w)
+        assert _status(P.sync) == N.OK
+
+
 def test_forks_refuse():
     P = cache_mod().Pager(20, 16, 8, 3)
     t, n, one = torch.zeros(8, 3, dtype=torch.int32, device="cuda"), _i32([0] * 8), _i32([0])

@@ -452,6 +452,20 @@ __global__ __launch_bounds__(256) void fork_tables_kernel(ForkArgs a) {
   const uint64_t used = s_used;
   const uint32_t columns = s_columns;
   const int32_t* in = a.tables + row0 * a.table_stride;
+  // Two rows with children that hold the last page of one of them, filled in part, would write over each other's
+  // tokens: pair q of rows is compared by its entries in that column.
+  struct Pair {
+    int mine, other;
+  };
+  auto entries = [&](int q) -> Pair {
+    const int i = q / width, j = q - i * width;
+    if (i >= width || i == j || !(used >> i & 1) || !(used >> j & 1)) return Pair{-1, -1};
+    const uint32_t last = a.page.of((uint32_t)length[i]);
+    if (last == blocks[i] || last >= blocks[j]) return Pair{-1, -1};
+    return Pair{in[i * a.table_stride + last], in[j * a.table_stride + last]};
+  };
+  auto shared = [&](Pair p) { return p.mine == p.other && (uint32_t)p.mine < a.pages; };
+  const Pair first_pair = entries(tid);  // (read with the first columns)
   int32_t* out = a.tables_out + row0 * a.table_out_stride;
   int32_t* list = a.dropped + (uint64_t)row0 * a.max_blocks;
   int n_dropped = 0;
@@ -502,6 +516,9 @@ __global__ __launch_bounds__(256) void fork_tables_kernel(ForkArgs a) {
       if (ALONE && (int64_t)count + at < a.pages) a.free_pages[count + at] = page;
     }
   }
+  bool twice = shared(first_pair);
+  for (int q = 256 + tid; q < width * width; q += 256) twice |= shared(entries(q));
+  if (twice) bits |= kCacheArgument;
   if (!ALONE && tid == 0) {
     a.drops[r] = n_dropped;
     if (r == 0) *a.count = count;
