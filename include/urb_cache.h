@@ -119,15 +119,17 @@ urb_status urb_pager_plan(urb_pager *pager, const urb_page_plan *plan, void *str
  *
  * A page may stand in several rows of one request, in the same column, and in no two requests; one that
  * is filled in part in a row that has children (a prompt's last page in all the rows of a search that begins)
- * in no other row that has: such rows go on sharing it, and URB_ERR_ARGUMENT is returned by the next sync.  A row
- * for which no page is left ends with length 0, and the next urb_pager_sync returns URB_ERR_OUT_OF_MEMORY.  A length that is negative or above max_blocks * page_size counts as 0, a
- * parent of `width` or more as negative, an entry that is no page is neither put on the stack nor
- * copied, pages beyond a full stack are left out, a *free_count out of range counts as 0:
- * URB_ERR_ARGUMENT by the next sync.
+ * in no other row that has: such rows go on sharing it, and URB_ERR_ARGUMENT is returned by the next
+ * sync.  A row for which no page is left ends with length 0, and the next urb_pager_sync returns
+ * URB_ERR_OUT_OF_MEMORY.  A length that is negative or above max_blocks * page_size counts as 0, a parent
+ * of `width` or more as negative, an entry that is no page is neither put on the stack nor copied, pages
+ * beyond a full stack are left out, a *free_count out of range counts as 0: URB_ERR_ARGUMENT by the next
+ * sync.
  *
- * tables_out must not overlap tables; lengths_out may be lengths, free_count_out free_count.  caches
- * (host array) have the pager's pages and page_size.  requests, width >= 1, width <= 64, requests *
- * width <= max_rows, requests <= 4096, n_caches <= 4096, both table strides >= max_blocks, else URB_ERR_SHAPE. */
+ * The first max_blocks columns of tables_out must not overlap those of tables (URB_ERR_ARGUMENT);
+ * lengths_out may be lengths, free_count_out free_count.  caches (host array) have the pager's pages and
+ * page_size.  requests, width >= 1, width <= 64, requests * width <= max_rows, requests <= 4096, n_caches
+ * <= 4096, both table strides >= max_blocks, else URB_ERR_SHAPE. */
 typedef struct {
   uint32_t requests, width;
   uint64_t table_stride, table_out_stride;

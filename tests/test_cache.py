@@ -1086,6 +1086,24 @@ def test_forks_refuse():
                                          one)) == N.ERR_SHAPE
 
 
+def test_forks_of_tables_that_overlap_refuse():
+    P = cache_mod().Pager(20, 16, 4, 3)
+    n, one, parents = _i32([0] * 4), _i32([0]), _i32([[0, 1], [0, 1]])
+    free = torch.zeros(20, dtype=torch.int32, device="cuda")
+    raw = torch.zeros(200, dtype=torch.int32, device="cuda")
+    table = lambda at, stride, columns=3: torch.as_strided(raw, (4, columns), (stride, 1), at)
+    call = lambda a, b: _status(lambda: P.fork_into(parents, a, n, free, one, b, n, one))
+    for a, b in ((table(0, 3), table(12, 3)), (table(20, 3), table(8, 3)),            # one behind the other
+                 (table(0, 6), table(3, 6)), (table(3, 6), table(0, 6)),              # rows by turns
+                 (table(0, 7), table(24, 10)), (table(0, 8, 5), table(3, 8, 5)),      # more columns than blocks
+                 (table(0, 40), table(3, 5)), (table(3, 5), table(43, 40))):
+        assert call(a, b) == N.OK
+    for a, b in ((table(0, 3), table(11, 3)), (table(0, 3), table(3, 3)), (table(1, 3), table(0, 3)),
+                 (table(0, 6), table(2, 6)), (table(0, 6), table(4, 6)), (table(0, 7), table(23, 10)),
+                 (table(0, 40), table(38, 5)), (table(37, 5), table(0, 40)), (table(0, 20), table(60, 3))):
+        assert call(a, b) == N.ERR_ARGUMENT and call(b, a) == N.ERR_ARGUMENT
+
+
 # ---- beam search's selection ----------------------------------------------------------------------
 
 def _select_by_hand(logits, scores, picks, ended, end_token):

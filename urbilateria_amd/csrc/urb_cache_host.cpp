@@ -53,6 +53,26 @@ uint64_t span_of(Axis a, Axis b, Axis c, uint64_t dim) {
   return (uint64_t)span;
 }
 
+// Whether two tables' rows of n entries, each one's rows apart, have an entry in common.
+bool tables_meet(const int32_t* a, uint64_t a_stride, const int32_t* b, uint64_t b_stride, uint64_t rows,
+                 uint64_t n) {
+  typedef unsigned __int128 Wide;  // (strides may be anything)
+  const Wide size = (Wide)n * sizeof(int32_t);
+  auto at = [](const int32_t* p, uint64_t stride, uint64_t row) {
+    return (Wide) reinterpret_cast<uintptr_t>(p) + (Wide)row * stride * sizeof(int32_t);
+  };
+  // the rows of both in their order (one table behind the other: no step)
+  if (at(a, a_stride, rows - 1) + size <= at(b, b_stride, 0) || at(b, b_stride, rows - 1) + size <= at(a, a_stride, 0))
+    return false;
+  for (uint64_t i = 0, j = 0; i < rows && j < rows;) {
+    const Wide x = at(a, a_stride, i), y = at(b, b_stride, j);
+    if (x + size <= y) ++i;
+    else if (y + size <= x) ++j;
+    else return true;
+  }
+  return false;
+}
+
 bool geometry(uint32_t heads, uint32_t page_size, uint32_t head_dim) {
   return heads >= 1 && heads <= 1024 && page_size >= 1 && page_size <= 1024 && head_dim >= 16 &&
          head_dim <= 256 && head_dim % 16 == 0;
@@ -216,6 +236,9 @@ urb_status urb_pager_fork(urb_pager* c, const urb_page_fork* f, void* stream) {
       (uint64_t)f->requests * f->width > d.max_rows || f->table_stride < d.max_blocks ||
       f->table_out_stride < d.max_blocks || f->n_caches > 4096)
     return URB_ERR_SHAPE;
+  if (tables_meet(f->tables, f->table_stride, f->tables_out, f->table_out_stride, (uint64_t)f->requests * f->width,
+                  d.max_blocks))
+    return URB_ERR_ARGUMENT;
   urb::KvCache* caches = nullptr;
   if (f->n_caches) {
     caches = new (std::nothrow) urb::KvCache[f->n_caches];
