@@ -1086,6 +1086,32 @@ def test_forks_refuse():
                                          one)) == N.ERR_SHAPE
 
 
+def test_forks_of_the_most_requests_and_caches():
+    rows = 4097
+    P = cache_mod().Pager(rows, 4, rows, 1)
+    t, n, one = torch.arange(rows, dtype=torch.int32, device="cuda").view(-1, 1), _i32([3] * rows), _i32([0])
+    free, out = torch.zeros(rows, dtype=torch.int32, device="cuda"), torch.full_like(t, -1)
+    def call(R, W=1, caches=()):
+        k = R * W
+        P.fork_into(torch.zeros(R, W, dtype=torch.int32, device="cuda"), t[:k], n[:k].clone(), free, one, out[:k],
+                    torch.empty_like(n[:k]), torch.empty_like(one), caches)
+    call(4096)
+    assert _status(P.sync) == N.OK and torch.equal(out[:4096], t[:4096]) and int(out[4096]) == -1
+    assert _status(lambda: call(4097)) == N.ERR_SHAPE
+    layers = [_make_cache(rows, 1, 4, 16, BF16) for _ in range(3)]
+    for c in layers:
+        c.k.view(-1)[:] = torch.arange(c.k.numel(), device="cuda").to(BF16)
+    was = layers[0].k.clone()
+    few = [layers[i % 3] for i in range(4096)]
+    n[0], n[1], one[0] = 3, 0, 1
+    free[0] = rows - 1
+    P.fork_into(_i32([[0, 0]]), t[:2], n[:2], free, one, out[:2], torch.empty_like(n[:2]), torch.empty_like(one), few)
+    assert _status(P.sync) == N.OK
+    was[rows - 1, :, :3] = was[0, :, :3]
+    assert all(torch.equal(c.k, was) for c in layers)
+    assert _status(lambda: call(1, caches=few + few[:1])) == N.ERR_SHAPE
+
+
 def test_forks_of_tables_that_overlap_refuse():
     P = cache_mod().Pager(20, 16, 4, 3)
     n, one, parents = _i32([0] * 4), _i32([0]), _i32([[0, 1], [0, 1]])

@@ -2,6 +2,8 @@
 bindings and the refusals that come before any GPU work."""
 
 import ctypes
+import shutil
+import subprocess
 
 import pytest
 
@@ -135,6 +137,15 @@ def test_beams_are_refused(change, status):
     out = ctypes.c_void_p()
     assert N.moe_lib().urb_beams_create(ctypes.byref(desc), ctypes.byref(out)) == status
     assert out.value is None
+
+
+def test_no_call_allocates_an_array():
+    # contexts and plans are single objects; only a call would need an array that may be missing
+    if shutil.which("nm") is None:
+        pytest.skip("nm not available")
+    r = subprocess.run(["nm", "-D", "--undefined-only", N.MOE_LIB], capture_output=True, text=True, check=True)
+    assert "_ZnwmRKSt9nothrow_t" in r.stdout
+    assert "_ZnamRKSt9nothrow_t" not in r.stdout
 
 
 def test_null_arguments_are_refused():

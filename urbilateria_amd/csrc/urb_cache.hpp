@@ -83,7 +83,12 @@ struct ForkArgs {
   ForkCopy* page_copies;  // of each row
   int* status;
 };
-void launch_fork(const ForkArgs& a, const KvCache* caches, uint32_t n_caches, hipStream_t s);
+void launch_fork(const ForkArgs& a, hipStream_t s);
+struct ForkCaches {
+  KvCache c[kForkCaches];
+};
+// The copies of pages that the fork before it found, in n caches.
+void launch_fork_copies(const ForkArgs& a, const ForkCaches& caches, uint32_t n, hipStream_t s);
 
 // ---- attention (urb_attend.hip) ----
 struct AttendArgs {

@@ -239,44 +239,43 @@ urb_status urb_pager_fork(urb_pager* c, const urb_page_fork* f, void* stream) {
   if (tables_meet(f->tables, f->table_stride, f->tables_out, f->table_out_stride, (uint64_t)f->requests * f->width,
                   d.max_blocks))
     return URB_ERR_ARGUMENT;
-  urb::KvCache* caches = nullptr;
-  if (f->n_caches) {
-    caches = new (std::nothrow) urb::KvCache[f->n_caches];
-    if (!caches) return URB_ERR_OUT_OF_MEMORY;
+  // (all caches are checked before the first launch)
+  for (uint32_t i = 0; i < f->n_caches; ++i) {
+    urb::KvCache c;
+    if (const urb_status st = take_cache(f->caches + i, &c)) return st;
+    if (c.pages != d.pages || c.page != d.page_size) return URB_ERR_SHAPE;
   }
-  urb_status st = URB_OK;
-  for (uint32_t i = 0; i < f->n_caches && !st; ++i) {
-    st = take_cache(f->caches + i, caches + i);
-    if (!st && (caches[i].pages != d.pages || caches[i].page != d.page_size)) st = URB_ERR_SHAPE;
+  urb::ForkArgs a{};
+  a.requests = f->requests;
+  a.width = f->width;
+  a.page = urb::PageDivision::by(d.page_size);
+  a.pages = d.pages;
+  a.max_blocks = d.max_blocks;
+  a.table_stride = f->table_stride;
+  a.table_out_stride = f->table_out_stride;
+  a.parents = f->parents;
+  a.tables = f->tables;
+  a.lengths = f->lengths;
+  a.tables_out = f->tables_out;
+  a.lengths_out = f->lengths_out;
+  a.free_pages = f->free_pages;
+  a.free_count = f->free_count;
+  a.free_count_out = f->free_count_out;
+  a.old_lengths = c->old_lengths;
+  a.drops = c->drops;
+  a.copies = c->copies;
+  a.dropped = c->dropped;
+  a.page_copies = c->page_copies;
+  a.count = c->count;
+  a.status = c->status;
+  urb::launch_fork(a, static_cast<hipStream_t>(stream));
+  for (uint32_t done = 0; done < f->n_caches;) {
+    urb::ForkCaches some;
+    const uint32_t n = std::min<uint32_t>(urb::kForkCaches, f->n_caches - done);
+    for (uint32_t i = 0; i < n; ++i) (void)take_cache(f->caches + done + i, &some.c[i]);
+    urb::launch_fork_copies(a, some, n, static_cast<hipStream_t>(stream));
+    done += n;
   }
-  if (!st) {
-    urb::ForkArgs a{};
-    a.requests = f->requests;
-    a.width = f->width;
-    a.page = urb::PageDivision::by(d.page_size);
-    a.pages = d.pages;
-    a.max_blocks = d.max_blocks;
-    a.table_stride = f->table_stride;
-    a.table_out_stride = f->table_out_stride;
-    a.parents = f->parents;
-    a.tables = f->tables;
-    a.lengths = f->lengths;
-    a.tables_out = f->tables_out;
-    a.lengths_out = f->lengths_out;
-    a.free_pages = f->free_pages;
-    a.free_count = f->free_count;
-    a.free_count_out = f->free_count_out;
-    a.old_lengths = c->old_lengths;
-    a.drops = c->drops;
-    a.copies = c->copies;
-    a.dropped = c->dropped;
-    a.page_copies = c->page_copies;
-    a.count = c->count;
-    a.status = c->status;
-    urb::launch_fork(a, caches, f->n_caches, static_cast<hipStream_t>(stream));
-  }
-  delete[] caches;
-  if (st) return st;
   URB_HIP(hipGetLastError());
   return URB_OK;
 }

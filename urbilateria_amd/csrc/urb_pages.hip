@@ -544,10 +544,6 @@ __global__ __launch_bounds__(256) void fork_books_kernel(ForkArgs a) {
   fork_books<false>(a, parent, length, slots, s_upto, count, 0, 0);
 }
 
-struct ForkCaches {
-  KvCache c[kForkCaches];
-};
-
 // Copies the first tokens of one page per blockIdx.x in the cache blockIdx.z; blockIdx.y takes the pieces of
 // 16 bytes in turn, four at a time so that a lane has four loads on their way.  Bound by the way to HBM and back, with
 // the rows that copy nothing in the grid too: 67 MB of 32 x 8 beams in six caches in 20 to 23 us, 2.9 TB/s.
@@ -621,7 +617,7 @@ void launch_plan(const PlanArgs& a, hipStream_t s) {
   plan_tokens_kernel<<<(a.tokens + kPlanTokens - 1) / kPlanTokens, 256, 0, s>>>(a);
 }
 
-void launch_fork(const ForkArgs& a, const KvCache* caches, uint32_t n_caches, hipStream_t s) {
+void launch_fork(const ForkArgs& a, hipStream_t s) {
   const size_t lds = a.width * 256 * sizeof(int);
   if (a.requests == 1) {
     fork_tables_kernel<true><<<1, 256, lds, s>>>(a);
@@ -629,22 +625,17 @@ void launch_fork(const ForkArgs& a, const KvCache* caches, uint32_t n_caches, hi
     fork_tables_kernel<false><<<a.requests, 256, lds, s>>>(a);
     fork_books_kernel<<<a.requests, 256, 0, s>>>(a);
   }
-  for (uint32_t done = 0; done < n_caches;) {
-    ForkCaches some;
-    const uint32_t n = std::min<uint32_t>(kForkCaches, n_caches - done);
-    uint64_t bytes = 0;
-    for (uint32_t i = 0; i < n; ++i) {
-      some.c[i] = caches[done + i];
-      bytes = std::max<uint64_t>(bytes, 2ull * caches[done + i].heads * a.page.size * caches[done + i].dim);
-    }
-    // parts of a page: four pieces for every lane where the cache is the largest, while that is no more than
-    // 64 workgroups per CU
-    const uint32_t rows = a.requests * a.width;
-    const uint32_t parts = (uint32_t)std::max<uint64_t>(
-        1, std::min<uint64_t>(bytes / 16384, 16384 / (rows * n)));
-    fork_copy_kernel<<<dim3(rows, parts, n), 256, 0, s>>>(a.page_copies, some);
-    done += n;
-  }
+}
+
+void launch_fork_copies(const ForkArgs& a, const ForkCaches& caches, uint32_t n, hipStream_t s) {
+  uint64_t bytes = 0;
+  for (uint32_t i = 0; i < n; ++i)
+    bytes = std::max<uint64_t>(bytes, 2ull * caches.c[i].heads * a.page.size * caches.c[i].dim);
+  // parts of a page: four pieces for every lane where the cache is the largest, while that is no more than
+  // 64 workgroups per CU
+  const uint32_t rows = a.requests * a.width;
+  const uint32_t parts = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(bytes / 16384, 16384 / (rows * n)));
+  fork_copy_kernel<<<dim3(rows, parts, n), 256, 0, s>>>(a.page_copies, caches);
 }
 
 }  // namespace urb
