@@ -179,6 +179,27 @@ def test_plans_of_one_token_each():
     assert s.check(added=False)[7] in (N.OK, N.ERR_ARGUMENT)
 
 
+@pytest.mark.parametrize("rows,page", [(1, 1), (300, 16), (300, 1), (1024, 7), (2000, 4)])
+def test_plans_of_one_token_each_take_pages(rows, page):
+    s = Steps(rows, page, 9, 1, 5, idle=0.0)
+    s.lengths = np.arange(rows) % (9 * page)        # every place in a page, and whole pages, among them
+    s.added[:] = 1
+    held, need = -(-s.lengths // page), -(-(s.lengths + 1) // page)
+    s.pages, s.count = int(need.sum()) + 3, int((need - held).sum()) + 3
+    assert s.count > 3
+    ids, at = np.random.default_rng(6).permutation(s.pages), 0
+    s.tables[:] = -7
+    for r in range(rows):
+        s.tables[r, :held[r]] = ids[at:at + held[r]]
+        at += held[r]
+    s.free = np.full(s.pages, -9)
+    s.free[:s.count] = ids[at:]
+    s.tokens = rows + 2
+    want = s.check(added=False)
+    assert want[7] == N.OK and want[6] == 3 and want[5].count(-1) == 2
+    s.check(in_place=True, added=False)
+
+
 def test_plans_with_many_rows_that_bring_nothing():
     s = Steps(9000, 16, 4, 3, 5, idle=0.95, tokens=6000)
     assert s.check()[7] == N.OK
@@ -934,6 +955,27 @@ def test_forks(dtype, requests, width, page, blocks):
     for seed in (1, 2):
         want = Beams(requests, width, page, blocks, seed, dtype=dtype).check(in_place=seed == 2)
         assert want[5] == N.OK
+
+
+@pytest.mark.parametrize("dtype", [BF16, F8])
+@pytest.mark.parametrize("width,page,blocks", [
+    (4, 2, 700), (64, 7, 6), (9, 3, 300), (8, 16, 43), (63, 1, 513), (64, 2, 257), (2, 100, 3)])
+def test_forks_of_a_single_request(dtype, width, page, blocks):
+    # more than 256 columns, more than eight rows, all of the LDS
+    for seed in (1, 2):
+        assert Beams(1, width, page, blocks, seed, dtype=dtype).check(in_place=seed == 2)[5] == N.OK
+    b = Beams(1, width, page, blocks, 3, dtype=dtype, ragged=True)
+    b.lengths[0] = blocks * page            # (its pages in all the passes over columns, and dropped)
+    b.tables[0] = np.arange(blocks) + b.pages
+    b.pages += blocks
+    b.free = np.concatenate((b.free, np.full(blocks, -4)))
+    b.layers = [b._filled(b.pages, 2, page, 32, dtype, 1)]
+    b.parents[:] = np.where(np.arange(width) % 3, width - 1, -1)
+    want = b.check()
+    assert want[5] == N.OK and want[3] >= b.count + blocks - (width - 1)
+    b.parents[:] = -1
+    want = b.check(in_place=True)
+    assert want[5] == N.OK and not want[4]
 
 
 def test_forks_of_every_layer():

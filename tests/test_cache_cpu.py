@@ -126,6 +126,17 @@ def test_attentions_are_refused(change, status):
     assert out.value is None
 
 
+@pytest.mark.parametrize("change", [
+    dict(max_length=(1 << 24) + 1), dict(max_rows=(1 << 20) + 1), dict(page_size=1025), dict(q_heads=8196, heads=4),
+    dict(head_dim=0), dict(head_dim=272)])
+def test_attentions_just_past_their_limits_are_refused(change):
+    desc = _struct(N.AttentionDesc, dict(q_heads=8, heads=2, head_dim=64, page_size=16, dtype=0, cache_dtype=0,
+                                         queries=1, window=0, scale=0.1, max_rows=4, max_length=100), change)
+    out = ctypes.c_void_p()
+    assert N.moe_lib().urb_attention_create(ctypes.byref(desc), ctypes.byref(out)) == N.ERR_SHAPE
+    assert out.value is None
+
+
 @pytest.mark.parametrize("change,status", [
     (dict(vocab=0), N.ERR_SHAPE), (dict(vocab=(1 << 18) + 1), N.ERR_SHAPE), (dict(width=0), N.ERR_SHAPE),
     (dict(width=33), N.ERR_SHAPE), (dict(picks=0), N.ERR_SHAPE), (dict(picks=65), N.ERR_SHAPE),
