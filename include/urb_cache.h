@@ -31,9 +31,9 @@ extern "C" {
  * contiguous: a value is its code times 2^(scale - 127).  Scales of 0 and 255 must not be used.
  *
  * pages 1 .. 2^24, heads 1 .. 1024, page_size 1 .. 1024, head_dim a multiple of 16 in 16 .. 256, less
- * than 2^36 bytes from the first value of K (of V) to the last, strides by which no two rows overlap,
- * else URB_ERR_SHAPE; rows that start at multiples of 16 bytes, BF16 or E4M3, scales with E4M3 and
- * only there, else URB_ERR_ARGUMENT. */
+ * than 2^36 bytes from the first value of K (of V) to the last, each stride (of an axis of more than one) at
+ * least what the axes of smaller strides span, else URB_ERR_SHAPE; rows that start at multiples of 16 bytes,
+ * BF16 or E4M3, scales with E4M3 and only there, else URB_ERR_ARGUMENT. */
 typedef struct {
   void *k, *v;
   uint8_t *k_scales, *v_scales; /* E4M3 alone */
@@ -154,14 +154,17 @@ urb_status urb_pager_sync(urb_pager *pager, void *stream);
  * For row r of lengths[r] cached tokens, its last `queries` ones among them, and query token i of them:
  *   e_j = exp(scale q . k_j),  o = sum_j e_j v_j / (exp(sink) + sum_j e_j)
  * over j < n = lengths[r] - (queries - 1 - i), and j >= n - window if window > 0; without sinks that
- * term is 0 (as with one of -inf; one of +inf leaves 0 of the values).  Query head h reads cache head h / (q_heads / heads).  lse is the logarithm of the
- * denominator; where that is 0, as with no j in reach, o is 0 and lse -inf.  Tokens that no query of the
- * row reaches are not used, whatever the cache holds there; an infinity or a NaN that one of its queries
- * reaches may come out of all of them.
+ * term is 0 (as with one of -inf; one of +inf leaves 0 of the values).  Query head h reads cache head
+ * h / (q_heads / heads).  lse is the logarithm of the denominator; where that is 0, as with no j in reach, o
+ * is 0 and lse -inf.  Tokens that no query of the row reaches are not used, whatever the cache holds there;
+ * an infinity or a NaN that one of its queries reaches may come out of all of them, and either may come out
+ * where queries, cached values, products q . k_j (before the scale) or sums e_j v_j reach 2^127.
  *
  * The products, sums and statistics are f32; the weights e are multiplied with 16 bits for BF16 rows and
  * with 24 for f32 rows, whose queries keep their 24 bits too.  A row's result may differ in its last bits
  * with the other rows of a call (they decide how its length is shared out), not between equal calls.
+ *
+ * A row's pages are read once for every sixteen queries of a cache head (queries * q_heads / heads of them).
  *
  * q_heads a multiple of heads, q_heads <= 8192, queries 1 .. 16, max_rows 1 .. 2^20, max_length
  * 1 .. 2^24, heads, page_size and head_dim as in urb_kv_cache, else URB_ERR_SHAPE; a scale that is not
@@ -183,8 +186,8 @@ void urb_attention_destroy(urb_attention *attention);
 
 /* Queries and outputs, [rows, queries, q_heads, head_dim] each: strides in values; a head's values are
  * contiguous and start at a multiple of 16 bytes (URB_ERR_ARGUMENT).  out may be q itself (same address
- * and strides) and must not overlap it otherwise; strides by which the heads of the output overlap each
- * other -> URB_ERR_SHAPE. */
+ * and strides) and must not overlap it otherwise; strides of the output that are less than what the axes of
+ * smaller strides span -> URB_ERR_SHAPE. */
 typedef struct {
   uint32_t rows;
   const void *q;

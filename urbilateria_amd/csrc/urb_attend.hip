@@ -3,10 +3,12 @@
 // One pass with a running maximum m and sum z: for a tile of tokens with scores s,
 //   m' = max(m, max s),  z' = z e(m - m') + sum e(s - m'),  o' = o e(m - m') + sum e(s - m') v
 // with e(x) = exp(scale x), and two parts of a row join by the same rule.  (The maximum is of the products
-// before the scale, so that rounding errs by their distance to it and not by their size.)  Every cached row is
-// read once, 4 operations per value and query head that shares it, so HBM bounds all but the shortest calls: 64
-// rows of 4096 tokens of 8 heads of 128 are read at 6.4 TB/s (166 us), in E4M3 at 5.75 (93 us), 200 rows of
-// lengths from 8 to 12000 at 5.5 (178 us); one row of 500 tokens takes 15 us, latencies of its two kernels.
+// before the scale, so that rounding errs by their distance to it and not by their size.)  A cached row is read
+// once for up to sixteen queries of its head, 4 operations per value and query, so HBM bounds all but the shortest
+// calls of so many: 64 rows of 4096 tokens of 8 heads of 128 are read at 6.4 TB/s (166 us), in E4M3 at 5.7 (95 us;
+// f32 rows 6.1 and 5.3), 200 rows of lengths from 8 to 12000 at 5.5 (178 us); one row of 500 tokens takes 15 us,
+// latencies of its two kernels.  More queries (drafted tokens of wide groups) read it again for every sixteen: 24 of
+// a head take 368 us and 193 where 16 take 167 and 96.
 //
 // Work: a pair is a row and up to sixteen of its query heads (of all its new tokens) that share a cache head;
 // a unit is kUnit tokens of a pair.  All units lie in one line, of which every workgroup takes an equal

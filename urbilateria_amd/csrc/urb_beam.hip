@@ -5,8 +5,9 @@
 // best `picks` logits, for more cannot be taken from one beam.  They are found with a threshold: the
 // picks-th largest of the threads' own largest is no more than the picks-th largest of all, and few others
 // lie above it.  The second kernel joins a request's slices the same way over their candidates' scores.
-// 256 rows of 129280 f32 logits (132 MB) take 39 us, bound by the vector units: an exponential in
-// f64 for each; the second kernel 8 to 12 for 32 requests, latency of its steps; 4 rows of 50257 take 6 and 5.
+// 256 rows of 129280 f32 logits (132 MB) take 39 us, bound by the vector units, which are busy for 78 % of it (an
+// exponential in f64 for each; LDS, with its table, for 23 %); the second kernel 8 to 13 for 32 requests, latency of
+// its steps; 4 rows of 50257 take 6 and 5.
 #include "urb_device.hpp"
 #include "urb_step.hpp"
 
@@ -305,10 +306,10 @@ __device__ __forceinline__ void pick_lowest(const BeamArgs& a, int r, int b, con
 // are counted for a beam, `team` threads go through a list.
 //
 // Logits that differ may share a score: close ones of a beam whose score is large, or of nearly 0.  Where a candidate
-// that counts may be one of them, the lists are gone through again in the order that they are in.  A list has the largest
-// logits of its slice, so it has all candidates above the last pick's score; of those with that very score lower
-// tokens may be missing in the last pick's beam (lists of beams before it that end at that score would fill the picks
-// by themselves).  They are looked up in the row, which only such calls read again.
+// that counts may be one of them, the lists are gone through again in the order that they are in.  A list has the
+// largest logits of its slice, so it has all candidates above the last pick's score; of those with that very score
+// lower tokens may be missing in the last pick's beam (lists of beams before it that end at that score would fill the
+// picks by themselves).  They are looked up in the row, which only such calls read again.
 template <int THREADS>
 __global__ __launch_bounds__(THREADS) void beam_join_kernel(BeamArgs a, int span, int team) {
   constexpr int WAVES = THREADS / 64, EARLY = 8;

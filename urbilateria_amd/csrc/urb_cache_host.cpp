@@ -38,8 +38,8 @@ struct Axis {
   // in bytes; the stride of an axis of one is not used
   uint64_t bytes(uint64_t b) const { return n > 1 ? stride * b : 0; }
 };
-// The values from the first to behind the last of rows of dim values along three axes; 0 if rows overlap or
-// it is 2^40 or more.
+// The values from the first to behind the last of rows of dim values along three axes; 0 if a stride is less than
+// what the axes of smaller ones span, as it is where rows overlap, or if it is 2^40 or more.
 uint64_t span_of(Axis a, Axis b, Axis c, uint64_t dim) {
   Axis axes[3] = {a, b, c};
   std::sort(axes, axes + 3, [](const Axis& x, const Axis& y) { return x.stride < y.stride; });

@@ -13,8 +13,8 @@ namespace {
 // ---- rows into slots ----
 //
 // Every value is read once and written once: bound by HBM (8190 tokens of 8 heads of 128, BF16 to E4M3: 50 MB in
-// 10.4 us, 4.85 TB/s), or for a few tokens by the launch (33 of 2 heads of 256: 3 us).  A row of a
-// head is held by dim / 16 lanes (of `span`, a power of two), sixteen values each, so an E4M3 row's largest
+// 10.4 us, 4.85 TB/s, the vector units busy for 88 %), or for a few tokens by the launch (33 of 2 heads of 256:
+// 3 us).  A row of a head is held by dim / 16 lanes (of `span`, a power of two), sixteen values each, so an E4M3 row's largest
 // value is a few shuffles away and its codes leave in one 16-byte store per lane.
 template <bool BF16>
 __device__ __forceinline__ void load16(float (&v)[16], const uint8_t* p) {
@@ -409,7 +409,7 @@ __device__ __forceinline__ void fork_books(const ForkArgs& a, const int* parent,
 
 // One request per workgroup: its rows' tables, and the pages that none of them holds any more.  A page can
 // stand in several rows only in one column, so a column is one thread's work.  Latency bounds it (parents and
-// lengths, the column, the pages' places): 6 us for 4 rows of 59 pages, 10 for 32 requests of 8 rows of 43.
+// lengths, the column, the pages' places): 7 us for 4 rows of 59 pages, 11 for 32 requests of 8 rows of 43.
 template <bool ALONE>
 __global__ __launch_bounds__(256) void fork_tables_kernel(ForkArgs a) {
   extern __shared__ int column[];  // [width][256]
@@ -546,7 +546,8 @@ __global__ __launch_bounds__(256) void fork_books_kernel(ForkArgs a) {
 
 // Copies the first tokens of one page per blockIdx.x in the cache blockIdx.z; blockIdx.y takes the pieces of
 // 16 bytes in turn, four at a time so that a lane has four loads on their way.  Bound by the way to HBM and back, with
-// the rows that copy nothing in the grid too: 67 MB of 32 x 8 beams in six caches in 20 to 23 us, 2.9 TB/s.
+// the rows that copy nothing in the grid too, and by the arithmetic of addresses (vector units are busy for 43 % of
+// it): 67 MB of 32 x 8 beams in six caches in 20 to 23 us, 2.9 TB/s.
 __global__ __launch_bounds__(256) void fork_copy_kernel(const ForkCopy* copies, ForkCaches caches) {
   const ForkCopy copy = copies[blockIdx.x];
   const uint32_t tokens = copy.tokens;
@@ -631,8 +632,8 @@ void launch_fork_copies(const ForkArgs& a, const ForkCaches& caches, uint32_t n,
   uint64_t bytes = 0;
   for (uint32_t i = 0; i < n; ++i)
     bytes = std::max<uint64_t>(bytes, 2ull * caches.c[i].heads * a.page.size * caches.c[i].dim);
-  // parts of a page: four pieces for every lane where the cache is the largest, while that is no more than
-  // 64 workgroups per CU
+  // parts of a page: four pieces for every lane in the largest of E4M3 caches, eight of BF16, while that is no more
+  // than 64 workgroups per CU
   const uint32_t rows = a.requests * a.width;
   const uint32_t parts = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(bytes / 16384, 16384 / (rows * n)));
   fork_copy_kernel<<<dim3(rows, parts, n), 256, 0, s>>>(a.page_copies, caches);
