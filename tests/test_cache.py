@@ -560,6 +560,28 @@ def test_infinite_sinks(lengths):
             assert torch.equal(lse[:, :, h], want_lse[:, :, h])
 
 
+@pytest.mark.parametrize("lengths", [[1, 1, 1], [3, 40, 2], [1, 9000]])
+def test_sinks_beside_scores_past_the_range(lengths):
+    # scores of 2^127 products: the largest is past f32's range (its lse +-inf), and the weights are 1 or 0
+    c = Cached(lengths, 8, 2, 64, 16, sharp=100.0, scale=2.0 ** 127, seed=12)
+    plain, plain_lse = c.run()
+    c.sinks = torch.tensor([0.5, -3.0, -math.inf, math.inf] * 2)
+    out, lse = c.run()
+    signs = set()
+    for r, n in enumerate(lengths):
+        top = (c.q[r, 0].double().unsqueeze(1) * c.k[r].repeat_interleave(4, 0)).sum(2).amax(1)
+        assert bool((top.abs() > 2).all())
+        for h, s in enumerate(c.sinks.tolist()):
+            over = top[h] > 0
+            signs.add(bool(over))
+            assert plain_lse[r, 0, h] == (math.inf if over else -math.inf)
+            takes_all = s == math.inf or (s > -math.inf and not over)
+            want = torch.zeros_like(plain[r, 0, h]) if takes_all else plain[r, 0, h]
+            assert torch.equal(out[r, 0, h], want), (r, h)      # (a zero's sign is not part of the definition)
+            assert lse[r, 0, h] == (s if takes_all else plain_lse[r, 0, h]), (r, h)
+    assert max(lengths) > 1 or len(signs) == 2
+
+
 @pytest.mark.parametrize("dtype,rows", KINDS)
 @pytest.mark.parametrize("lengths,q_heads,heads,dim", [
     ([20000], 16, 2, 256), ([131071], 4, 1, 64), ([5000, 3, 40, 9000, 0, 777], 32, 8, 128),

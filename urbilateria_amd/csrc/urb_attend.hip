@@ -246,12 +246,13 @@ __device__ __forceinline__ void finish4(const AttendArgs& a, uint32_t row, const
                                         float m, float z) {
   if (!q.there) return;
   m *= a.scale;
-  if (a.sinks) {
-    // the sink as one more score, with no value
-    const float s = a.sinks[q.head];
-    const float top = fmaxf(m, s), t = top == kMinusInf ? 0.0f : top;
-    const float f = exp2f((m - t) * kLog2e);
-    z = z * f + (s == t ? 1.0f : exp2f((s - t) * kLog2e));  // (of a sink of +inf all)
+  const float s = a.sinks ? a.sinks[q.head] : kMinusInf;
+  if (s != kMinusInf) {
+    // the sink as one more score, with no value: all of it where it is +inf, and nothing of it where the largest
+    // score has left f32's range
+    const float top = fmaxf(m, s);
+    const float f = s == -kMinusInf ? 0.0f : m == top ? 1.0f : exp2f((m - top) * kLog2e);
+    z = z * f + (s == top ? 1.0f : exp2f((s - top) * kLog2e));
     o.x *= f; o.y *= f; o.z *= f; o.w *= f;
     m = top;
   }
